@@ -46,6 +46,14 @@ class LayerDesc(C.Structure):
                                                           ("kv_pool_elems", C.c_int64)]
 
 
+class KvSlab(C.Structure):
+    _fields_ = [("base", C.c_int64), ("cap", C.c_int32), ("pad", C.c_int32)]
+
+
+class KvMove(C.Structure):
+    _fields_ = [("base", C.c_int64), ("cap", C.c_int32), ("start", C.c_int32), ("n", C.c_int32), ("pad", C.c_int32)]
+
+
 P, I32, I64, F32, SZ = C.c_void_p, C.c_int32, C.c_int64, C.c_float, C.c_size_t
 
 # name -> (restype, argtypes)
@@ -83,6 +91,11 @@ _PROTOS = {
     "flyai_attn_plan_prefill": (C.c_int, [P, P, I32, I32, I32, I32, I32, P, I32, P, I32, P, I32, P, P, P, P]),
     "flyai_attn_prefill": (C.c_int, [P, P, P, P, P, P, I32, I32, I32, I32, P, I32, P, P]),
     "flyai_attn_ragged": (C.c_int, [P, P, P, P, P, P, I32, I32, I32, I32, P, I32, I32, P, I32, P, P, P]),
+    "flyai_linear_lora_workspace_bytes": (SZ, [I32, I32, I32, I32, I32]),
+    "flyai_linear_lora_bf16": (C.c_int, [P, P, P, I32, I32, I32, P, P, P, P, I32, I32, P, I32, P, P, I32, P, P, P, P]),
+    "flyai_rope": (C.c_int, [P, I64, I64, P, P, F32, I32, I32, I32, I32, I32, I32, I32, P, I64, I64, P]),
+    "flyai_kv_fork": (C.c_int, [P, P, I64, I64, P, P, I64, I64, I32, I32, I32, P, P, I32, I32, I32, P]),
+    "flyai_kv_compact": (C.c_int, [P, P, I64, I64, I32, I32, I32, P, I32, P, P]),
     "flyai_bf16_tile_packed_bytes": (SZ, [I32, I32]),
     "flyai_bf16_tile_repack": (C.c_int, [P, I32, I32, P, P]),
     "flyai_embed_gather": (C.c_int, [P, P, I32, I32, I32, P, P]),

@@ -732,6 +732,9 @@ __global__ __launch_bounds__(64 * kTiledWaves) void gemm_tiled_lds_kernel(const 
 
 int gemm_slices(int K) { return ((K + 127) / 128 + kKQW - 1) / kKQW; }
 
+// fp32 planes launch_gemm writes
+int gemm_planes(int M, int K) { return M >= kTiledMinRows ? 1 : gemm_slices(K); }
+
 size_t linear_partials_bytes(int M, int N, int K) { return (size_t)gemm_slices(K) * M * N * sizeof(float); }
 
 int launch_gemm_splitk(const uint16_t* x, const uint16_t* W, int M, int N, int K, float* part,
@@ -1107,8 +1110,7 @@ static int linear_scratch(float** out) {
 
 // bytes of partial planes launch_gemm writes and the finalizer reads for this shape
 static size_t linear_partials_used(int M, int N, int K) {
-  const int planes = M >= kTiledMinRows ? 1 : gemm_slices(K);
-  return (size_t)planes * M * N * sizeof(float);
+  return (size_t)gemm_planes(M, K) * M * N * sizeof(float);
 }
 
 extern "C" size_t flyai_linear_noalloc_max_bytes(void) { return kLinearScratchBytes; }

@@ -4,6 +4,7 @@ PyTorch provides device memory and the stream; every computation happens in libf
 Each wrapper checks dtype / device / contiguity / shape on the host before the launch."""
 import ctypes as C
 
+import numpy as np
 import torch
 
 from . import _lib
@@ -312,6 +313,138 @@ def attn_ragged(q, k_pool, v_pool, kv_base, kv_cap, sinks, window, items, groups
                                   n_small, _ptr(groups_d), groups.shape[0], _ptr(parts), _ptr(out),
                                   _stream()))
     return out
+
+
+# ---- many requests at once: adapters, rotary positions, the cache's slabs ------------------------
+
+def _same_device(x, *others):
+    for name, t in others:
+        if t is not None and t.device != x.device:
+            raise ValueError(f"{name} is on {t.device}, not on {x.device}")
+
+
+def linear_lora(x, w, b, lora_a, lora_b, scale, ranks, adapter, segments=None, row_seq=None, residual=None):
+    """``linear`` with a low-rank adapter of its own for each row: y = bf16(x W^T + b + s_a (x A_a^T) B_a^T), with residual
+    residual <- bf16(residual + y) (returned).  lora_a bf16 [n, S * R, K], lora_b bf16 [n, N, R], scale fp32 [n], ranks
+    int32 [n] (adapter a uses the first ranks[a] of R rows of each segment's A and columns of B; nothing past them is
+    used); R a multiple of 16 up to 128.  segments: the S (at most 4) widths of the output's runs that have an A of
+    their own (None: one of N).  adapter int32: of each row [M], or with row_seq int32 [M] of each sequence; ids outside
+    [0, n) mean no adapter, and such a row has ``linear``'s bits.  A row's result depends on that row alone."""
+    M, K = x.shape
+    N = w.shape[0]
+    _need(x, torch.bfloat16, (M, K), "x")
+    _need(w, torch.bfloat16, (N, K), "weight")
+    if b is not None:
+        _need(b, torch.bfloat16, (N,), "bias")
+    segments = (N,) if segments is None else tuple(int(v) for v in segments)
+    S = len(segments)
+    if lora_b.dim() != 3:
+        raise ValueError("lora_b must be [adapters, N, R]")
+    n, _, R = lora_b.shape
+    _need(lora_b, torch.bfloat16, (n, N, R), "lora_b")
+    _need(lora_a, torch.bfloat16, (n, S * R, K), "lora_a")
+    _need(scale, torch.float32, (n,), "scale")
+    _need(ranks, torch.int32, (n,), "ranks")
+    if row_seq is None:
+        _need(adapter, torch.int32, (M,), "adapter")
+    else:
+        _need(row_seq, torch.int32, (M,), "row_seq")
+        _need(adapter, torch.int32, (adapter.numel(),), "adapter")
+    y = None
+    if residual is not None:
+        _need(residual, torch.bfloat16, (M, N), "residual")
+    else:
+        y = torch.empty(M, N, dtype=torch.bfloat16, device=x.device)
+    _same_device(x, ("weight", w), ("bias", b), ("lora_a", lora_a), ("lora_b", lora_b), ("scale", scale), ("ranks", ranks),
+                 ("adapter", adapter), ("row_seq", row_seq), ("residual", residual))
+    ws = torch.empty(max(16, int(lib().flyai_linear_lora_workspace_bytes(M, N, K, R, S))), dtype=torch.uint8, device=x.device)
+    with torch.cuda.device(x.device):
+        check(lib().flyai_linear_lora_bf16(_ptr(x), _ptr(w), _ptr(b), M, N, K, _ptr(lora_a), _ptr(lora_b), _ptr(scale),
+                                           _ptr(ranks), n, R, (C.c_int32 * S)(*segments), S, _ptr(adapter), _ptr(row_seq),
+                                           adapter.numel(), _ptr(y), _ptr(residual), _ptr(ws), _stream()))
+    return residual if residual is not None else y
+
+
+_ROPE_TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
+_ROPE_LAYOUTS = {"half": 0, "interleaved": 1}
+
+
+def rope(x, positions, inv_freq, layout="half", scaling=1.0, inverse=False, out=None):
+    """Rotary positions on x [T, H, D] (bf16, fp16 or fp32; a view whose last dim is contiguous, such as the q and k heads
+    of fused projection rows): dims [0, 2 * len(inv_freq)) of each head are turned by positions[t] * inv_freq[i] (int32 [T],
+    fp64; ``rope.rope_frequencies`` gives scaled ones) and multiplied by scaling, the others copied.  Pairs are (i, i +
+    rot/2) ("half") or (2i, 2i + 1) ("interleaved").  inverse turns back: the gradient of the rotation.  out: a tensor
+    of x's shape and type (x itself: in place; otherwise it must not overlap x), None: a new contiguous one."""
+    if not isinstance(x, torch.Tensor) or x.dim() != 3:
+        raise ValueError("x must be a [T, H, D] tensor")
+    if x.device.type != "cuda":
+        raise ValueError("x must be on the GPU")
+    if x.dtype not in _ROPE_TYPES:
+        raise TypeError(f"x must be bf16, fp16 or fp32, got {x.dtype}")
+    if layout not in _ROPE_LAYOUTS:
+        raise ValueError(f"layout must be one of {sorted(_ROPE_LAYOUTS)}, got {layout!r}")
+    T, H, D = x.shape
+    _need(positions, torch.int32, (T,), "positions")
+    _need(inv_freq, torch.float64, (inv_freq.numel(),), "inv_freq")
+    if out is None:
+        out = torch.empty(T, H, D, dtype=x.dtype, device=x.device)
+    elif out.dtype != x.dtype or out.shape != x.shape:
+        raise ValueError(f"out must be {x.dtype} of shape {tuple(x.shape)}")
+    _same_device(x, ("positions", positions), ("inv_freq", inv_freq), ("out", out))
+    if D > 1 and (x.stride(2) != 1 or out.stride(2) != 1):
+        raise ValueError("the last dim of x and out must be contiguous")
+    if T == 0 or H == 0:
+        return out
+    with torch.cuda.device(x.device):
+        check(lib().flyai_rope(_ptr(x), x.stride(0), x.stride(1), _ptr(positions), _ptr(inv_freq), float(scaling), T, H, D,
+                               2 * inv_freq.numel(), _ROPE_TYPES[x.dtype], _ROPE_LAYOUTS[layout], int(bool(inverse)),
+                               _ptr(out), out.stride(0), out.stride(1), _stream()))
+    return out
+
+
+def _kv_pools(k, v):
+    """(layers, elements a layer, layer stride) of K and V pools [L, n] (or one layer's [n])."""
+    if not isinstance(k, torch.Tensor) or not isinstance(v, torch.Tensor) or k.dim() not in (1, 2) or k.shape != v.shape:
+        raise ValueError("k and v must be pools of one shape, [layers, elements] or [elements]")
+    _need(k, torch.bfloat16, None, "k")
+    _need(v, torch.bfloat16, None, "v")
+    _same_device(k, ("v", v))
+    n = k.shape[-1]
+    return (k.shape[0] if k.dim() == 2 else 1), n, n
+
+
+def kv_fork(k, v, n_kv_heads, src, dsts, lo, hi, src_k=None, src_v=None):
+    """Copy positions [lo, hi) of slab src to the same positions of the slabs dsts, every layer, in one launch.  k, v: pools
+    bf16 [L, elements] in the tiled slab layout; a slab is (base, cap).  src_k, src_v: the pools that hold src, when
+    they are others.  Nothing outside [lo, hi) changes.  Positions past a slab raise ContextOverflow."""
+    src_k, src_v = (k, v) if src_k is None else (src_k, src_v)
+    L, n, stride = _kv_pools(k, v)
+    sL, sn, sstride = _kv_pools(src_k, src_v)
+    if sL != L:
+        raise ValueError(f"pools of {sL} and of {L} layers")
+    _same_device(k, ("src_k", src_k))
+    one = _lib.KvSlab(int(src[0]), int(src[1]), 0)
+    many = (_lib.KvSlab * max(1, len(dsts)))(*[_lib.KvSlab(int(b), int(c), 0) for b, c in dsts])
+    with torch.cuda.device(k.device):
+        check(lib().flyai_kv_fork(_ptr(src_k), _ptr(src_v), sstride, sn, _ptr(k), _ptr(v), stride, n, L, int(n_kv_heads), 64,
+                                  C.byref(one), many, len(dsts), int(lo), int(hi), _stream()))
+
+
+def kv_compact(k, v, n_kv_heads, moves):
+    """For each move (base, cap, start, keep): position start + i of the slab takes what position start + keep[i] held
+    before the call, every layer, in one launch (more beyond 704 moved rows).  keep: host integers (list, numpy or CPU
+    tensor), in any order up to 704, strictly ascending beyond.  The moves' slabs must not overlap."""
+    L, n, stride = _kv_pools(k, v)
+    keeps = [np.asarray(m[3]).reshape(-1) for m in moves]
+    for a in keeps:
+        if a.size and (a.dtype.kind not in "iu" or a.min() < 0 or a.max() > 0x7fffffff):
+            raise ValueError("keep must hold positions (non-negative integers)")
+    flat = np.concatenate([a.astype(np.int32) for a in keeps]) if keeps else np.zeros(0, np.int32)
+    rows = (_lib.KvMove * max(1, len(moves)))(*[_lib.KvMove(int(m[0]), int(m[1]), int(m[2]), a.size, 0)
+                                               for m, a in zip(moves, keeps)])
+    with torch.cuda.device(k.device):
+        check(lib().flyai_kv_compact(_ptr(k), _ptr(v), stride, n, L, int(n_kv_heads), 64, rows, len(moves),
+                                     flat.ctypes.data_as(C.c_void_p), _stream()))
 
 
 # ---- DeepSeek-V3-shaped FP8 MoE ------------------------------------------------------------------

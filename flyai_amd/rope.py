@@ -51,3 +51,40 @@ class YarnRotary:
         self.attention_scaling = att
         self.head_dim = head_dim
         self._tables(n_positions, device)
+
+
+def rope_frequencies(rot_dim, base=10000.0, scaling=None, factor=1.0, original_max=4096, beta_fast=32.0,
+                     beta_slow=1.0, device="cuda"):
+    """(inv_freq fp64 [rot_dim / 2], attention scaling) for ``ops.rope``, scaled for contexts longer than the
+    ``original_max`` positions a model was trained on:
+
+    * None: base^(-2i / rot_dim), scaling 1;
+    * "linear": positions divided by ``factor``;
+    * "ntk": the base raised to base * factor^(rot_dim / (rot_dim - 2)), so that the slowest pair turns ``factor`` times
+      slower and the fastest as before;
+    * "yarn": pairs that turn more than ``beta_fast`` times over the original context keep their frequency, those below
+      ``beta_slow`` are divided by ``factor``, a linear ramp between; scaling 0.1 ln(factor) + 1."""
+    if rot_dim < 2 or rot_dim % 2:
+        raise ValueError(f"rot_dim must be even and positive, got {rot_dim}")
+    if scaling not in (None, "linear", "ntk", "yarn"):
+        raise ValueError(f"scaling must be None, 'linear', 'ntk' or 'yarn', got {scaling!r}")
+    if base <= 1 or factor < 1 or original_max < 1:
+        raise ValueError("needs base > 1, factor >= 1 and original_max >= 1")
+    if scaling == "ntk":
+        if rot_dim < 4:
+            raise ValueError("ntk scaling needs rot_dim >= 4")
+        base = base * factor ** (rot_dim / (rot_dim - 2))
+    i = torch.arange(0, rot_dim, 2, dtype=torch.float64)
+    inv = float(base) ** (-i / rot_dim)
+    att = 1.0
+    if scaling == "linear":
+        inv = inv / factor
+    elif scaling == "yarn":
+        def pair_of(turns):  # the pair that turns this often over the original context
+            return rot_dim * math.log(original_max / (turns * 2 * math.pi)) / (2 * math.log(base))
+
+        low, high = max(pair_of(beta_fast), 0.0), min(pair_of(beta_slow), rot_dim - 1.0)
+        ramp = ((i / 2 - low) / max(high - low, 0.001)).clamp(0, 1)
+        inv = inv * (1 - ramp) + inv / factor * ramp
+        att = 0.1 * math.log(factor) + 1.0
+    return inv.to(device), att

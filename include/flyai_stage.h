@@ -307,6 +307,74 @@ int flyai_attn_prefill(const uint16_t* q, const uint16_t* k_pool, const uint16_t
                        int32_t Hq, int32_t Hkv, int32_t D, const flyai_attn_item* pitems_dev, int32_t n_pitems,
                        uint16_t* out, flyai_stream_t stream);
 
+/* ---- many requests at once: adapters, rotary positions, the cache's slabs -------------------------
+ * Low-rank adapters beside a shared projection: y[t] = bf16(x[t] W^T + b + d[t]), and for a row t whose
+ * adapter is a, d[t, f] = scale[a] * sum_{j < ranks[a]} (x[t] . A[a][seg(f) R + j]) B[a][f][j]; a row
+ * without one has the bits of flyai_linear_bf16.  The output is n_segments (1..4) runs of
+ * segments_host[i] features (multiples of 16, summing to N), each with an A of its own: the fused q, k, v
+ * projection has three.  x bf16 [M, K]; W bf16 [N, K]; b bf16 [N] or NULL; A bf16 [n_adapters,
+ * n_segments * R, K]; B bf16 [n_adapters, N, R]; scale fp32 and ranks int32 [n_adapters] (a rank outside
+ * [0, R] is clamped; entries past it are not used, whatever they hold); R in 16, 32, ..., 128.  adapter int32: of
+ * row t, or with row_seq int32 [M] of row t's sequence (adapter[row_seq[t]], n_seqs entries); an adapter
+ * outside [0, n_adapters) or a sequence outside [0, n_seqs) means none.  With residual the result is bf16(residual +
+ * y), written to residual.  A row's result depends on that row alone: not on its batch, nor on what other
+ * rows' adapters hold.  Pointers to bf16 are 16-byte aligned.  workspace: flyai_linear_lora_workspace_bytes,
+ * 16-byte aligned; two calls that may overlap need one each.  N % 16 == 0, K % 32 == 0, K <= 8192. */
+size_t flyai_linear_lora_workspace_bytes(int32_t M, int32_t N, int32_t K, int32_t R, int32_t n_segments);
+int flyai_linear_lora_bf16(const uint16_t* x, const uint16_t* w, const uint16_t* b, int32_t M, int32_t N,
+                           int32_t K, const uint16_t* lora_a, const uint16_t* lora_b, const float* scale,
+                           const int32_t* ranks, int32_t n_adapters, int32_t R, const int32_t* segments_host,
+                           int32_t n_segments, const int32_t* adapter, const int32_t* row_seq,
+                           int32_t n_seqs, uint16_t* y, uint16_t* residual, void* workspace,
+                           flyai_stream_t stream);
+
+/* Rotary positions on x [T, H, D] (dtype FLYAI_BF16, FLYAI_F16 or FLYAI_F32; the last dim contiguous,
+ * token and head strides in elements): dims [0, rot) of every head are turned by the angles
+ * positions[t] * inv_freq[i] (int32 [T], fp64 [rot / 2]) and scaled, the others copied.  Pair i is dims
+ * (i, i + rot/2), or with interleaved (2i, 2i + 1).  inverse turns the other way: the gradient.  out may be x
+ * with x's strides, or must not overlap it.  Any int32 position: the angle is computed in 64 bits.  T and H * D
+ * at most 2^22, rot at most 2048. */
+#define FLYAI_BF16 0
+#define FLYAI_F16 1
+#define FLYAI_F32 2
+int flyai_rope(const void* x, int64_t x_token, int64_t x_head, const int32_t* positions,
+               const double* inv_freq, float scaling, int32_t T, int32_t H, int32_t D, int32_t rot,
+               int32_t dtype, int32_t interleaved, int32_t inverse, void* out, int64_t o_token,
+               int64_t o_head, flyai_stream_t stream);
+
+/* Slabs of the KV cache (the layout of flyai_rope_kv_append) forked and compacted, every layer, K and V and
+ * kv head in one launch (replaces the per-layer index copies of FastVerify.tree_gather,
+ * phase0/fastverify.py:301-309, and BatchedFastVerify.load_prefix, phase0/batchverify.py:125-130).  A pool is n_layers layers of
+ * `elems` elements, `layer` elements apart.  All descriptions are host memory, read before the call returns
+ * and passed to the kernel by value.
+ * fork: positions [lo, hi) of the source slab to the same positions of n_dst other slabs; nothing else of
+ * them changes.  Slabs of one pool must not overlap.
+ * compact: for each move, slab position start + i takes what position start + keep[i] held before the call
+ * (keep_host holds the moves' entries one after the other).  keep may be in any order and name a position twice up to
+ * 704 entries a move, and is strictly ascending beyond.  The moves' slabs must not overlap.
+ * Positions past a slab -> FLYAI_ERANGE, before any launch. */
+typedef struct {
+  int64_t base;  /* element offset of the slab in a layer's pool (base % 8 == 0) */
+  int32_t cap;   /* positions (cap % 64 == 0) */
+  int32_t pad;
+} flyai_kv_slab;
+
+typedef struct {
+  int64_t base;
+  int32_t cap;
+  int32_t start;
+  int32_t n;     /* rows start .. start + n - 1 are written */
+  int32_t pad;
+} flyai_kv_move;
+
+int flyai_kv_fork(const uint16_t* src_k, const uint16_t* src_v, int64_t src_layer, int64_t src_elems,
+                  uint16_t* dst_k, uint16_t* dst_v, int64_t dst_layer, int64_t dst_elems, int32_t n_layers,
+                  int32_t Hkv, int32_t D, const flyai_kv_slab* src_host, const flyai_kv_slab* dsts_host,
+                  int32_t n_dst, int32_t lo, int32_t hi, flyai_stream_t stream);
+int flyai_kv_compact(uint16_t* k_pool, uint16_t* v_pool, int64_t layer, int64_t pool_elems, int32_t n_layers,
+                     int32_t Hkv, int32_t D, const flyai_kv_move* moves_host, int32_t n_moves,
+                     const int32_t* keep_host, flyai_stream_t stream);
+
 /* ---- head and tail of a served model (the continuous-batch backend's token step) --------------
  * Embedding: replaces parts["embed"](token_ids) (phase0/specpipe.py:595-596, :779): out[t] =
  * table[ids[t]] (bf16 [V, H] table; an id outside [0, V) gives a zero row).  H % 8 == 0.

@@ -1,0 +1,135 @@
+"""Refusals of the adapters', rotary and slab operators through the C ABI: every one comes back as an error code before
+anything is launched, so they run without a GPU (the pointers are never read)."""
+import ctypes as C
+
+import numpy as np
+import pytest
+import torch
+
+from flyai_amd import _lib
+from flyai_amd.rope import rope_frequencies
+
+PTR = C.c_void_p(0x100000)
+ODD = C.c_void_p(0x100002)
+
+
+@pytest.fixture(scope="module")
+def lib():
+    return _lib.lib()
+
+
+def _lora(lib, M=4, N=48, K=64, n=2, R=16, segments=(32, 16), x=PTR, a=PTR, adapter=PTR, row_seq=None, n_seqs=0, y=PTR, ws=PTR):
+    return lib.flyai_linear_lora_bf16(x, PTR, None, M, N, K, a, PTR, PTR, PTR, n, R, (C.c_int32 * len(segments))(*segments),
+                                      len(segments), adapter, row_seq, n_seqs, y, None, ws, None)
+
+
+@pytest.mark.parametrize("change", [
+    {"M": -1}, {"M": (1 << 20) + 1}, {"N": 40}, {"K": 48}, {"K": 8224}, {"n": 0}, {"R": 8}, {"R": 24}, {"R": 144},
+    {"segments": (48, 8)}, {"segments": (24, 24)}, {"segments": (32,)}, {"segments": (16, 16, 16, 16)}, {"segments": (64, -16)},
+    {"segments": (2 ** 31 - 16, 2 ** 31 - 16)}, {"segments": (16,) * 5}, {"x": None}, {"x": ODD}, {"a": ODD}, {"a": None}, {"adapter": None},
+    {"row_seq": PTR, "n_seqs": 0}, {"y": None}, {"ws": None}, {"ws": ODD}])
+def test_lora_refusals(lib, change):
+    assert _lora(lib, **change) == _lib.FLYAI_EINVAL
+    assert lib.flyai_last_error()
+
+
+def test_lora_of_no_rows(lib):
+    assert _lora(lib, M=0) == 0
+    assert lib.flyai_linear_lora_workspace_bytes(0, 48, 64, 16, 2) == 0
+    small, large = (int(lib.flyai_linear_lora_workspace_bytes(m, 5120, 2880, 64, 3)) for m in (255, 256))
+    # below 256 rows the projection leaves one plane of partial sums per 512 of K, from 256 rows one
+    assert small >= 255 * (6 * 5120 * 4 + 3 * 64 * 4) and large >= 256 * (5120 * 4 + 3 * 64 * 4)
+
+
+def _rope(lib, x=PTR, xt=256, xh=64, pos=PTR, T=2, H=4, D=64, rot=64, dtype=0, out=C.c_void_p(0x200000), ot=256, oh=64):
+    return lib.flyai_rope(x, xt, xh, pos, PTR, 1.0, T, H, D, rot, dtype, 0, 0, out, ot, oh, None)
+
+
+@pytest.mark.parametrize("change", [
+    {"T": -1}, {"H": 0}, {"rot": 0}, {"rot": 33}, {"rot": 66}, {"dtype": 3}, {"dtype": -1}, {"xt": -256}, {"x": None}, {"pos": None},
+    {"out": None}, {"ot": 128}, {"oh": 32}, {"oh": 0}, {"ot": 0}, {"out": C.c_void_p(0x100080)}, {"out": PTR, "ot": 512},
+    {"T": (1 << 22) + 1}, {"H": 1 << 17}, {"D": 4096, "rot": 2050, "xh": 4096, "oh": 4096, "xt": 1 << 20, "ot": 1 << 20}])
+def test_rope_refusals(lib, change):
+    assert _rope(lib, **change) == _lib.FLYAI_EINVAL
+    assert lib.flyai_last_error()
+
+
+def test_rope_of_no_tokens(lib):
+    assert _rope(lib, T=0) == 0
+
+
+def _slab(base, cap):
+    return _lib.KvSlab(base, cap, 0)
+
+
+def _fork(lib, src=(0, 128), dsts=((2 * 128 * 64, 128),), lo=0, hi=10, layer=8 * 128 * 64, elems=8 * 128 * 64, L=2, heads=2, D=64,
+          k=PTR, dk=PTR):
+    many = (_lib.KvSlab * max(1, len(dsts)))(*[_slab(*d) for d in dsts])
+    one = _slab(*src)
+    return lib.flyai_kv_fork(k, PTR, layer, elems, dk, PTR, layer, elems, L, heads, D, C.byref(one), many, len(dsts), lo, hi, None)
+
+
+@pytest.mark.parametrize("change,code", [
+    ({"hi": 129}, _lib.FLYAI_ERANGE), ({"dsts": ((2 * 128 * 64, 64),), "hi": 65}, _lib.FLYAI_ERANGE),
+    ({"dsts": ((7 * 128 * 64, 128),)}, _lib.FLYAI_ERANGE), ({"src": (7 * 128 * 64, 128)}, _lib.FLYAI_ERANGE),
+    ({"dsts": ((64, 128),)}, _lib.FLYAI_EINVAL), ({"dsts": ((4 * 128 * 64, 128), (5 * 128 * 64, 128))}, _lib.FLYAI_EINVAL),
+    ({"lo": 11}, _lib.FLYAI_EINVAL), ({"lo": -1}, _lib.FLYAI_EINVAL), ({"src": (0, 100)}, _lib.FLYAI_EINVAL),
+    ({"src": (-8, 128)}, _lib.FLYAI_EINVAL), ({"src": (4, 128)}, _lib.FLYAI_EINVAL), ({"D": 128}, _lib.FLYAI_EINVAL),
+    ({"L": 0}, _lib.FLYAI_EINVAL), ({"heads": 0}, _lib.FLYAI_EINVAL), ({"k": None}, _lib.FLYAI_EINVAL),
+    ({"dk": C.c_void_p(0x100008)}, _lib.FLYAI_EINVAL), ({"layer": 4 * 128 * 64}, _lib.FLYAI_EINVAL)])
+def test_fork_refusals(lib, change, code):
+    assert _fork(lib, **change) == code
+    assert lib.flyai_last_error()
+
+
+def test_fork_of_nothing(lib):
+    assert _fork(lib, lo=10) == 0
+    assert _fork(lib, dsts=()) == 0
+
+
+def _compact(lib, moves, keep, elems=8 * 128 * 64, v=PTR):
+    rows = (_lib.KvMove * max(1, len(moves)))(*[_lib.KvMove(b, c, s, n, 0) for b, c, s, n in moves])
+    flat = np.asarray(keep, dtype=np.int32)
+    return lib.flyai_kv_compact(PTR, v, elems, elems, 2, 2, 64, rows, len(moves), flat.ctypes.data_as(C.c_void_p), None)
+
+
+@pytest.mark.parametrize("moves,keep,code", [
+    ([(0, 128, 100, 2)], [0, 28], _lib.FLYAI_ERANGE), ([(0, 128, 127, 2)], [0, 0], _lib.FLYAI_ERANGE),
+    ([(7 * 128 * 64, 128, 0, 1)], [1], _lib.FLYAI_ERANGE), ([(0, 128, 0, 1)], [-1], _lib.FLYAI_EINVAL),
+    ([(0, 128, 0, 1)], [2 ** 31 - 1], _lib.FLYAI_ERANGE), ([(0, 128, -1, 1)], [1], _lib.FLYAI_EINVAL),
+    ([(0, 128, 0, -1)], [1], _lib.FLYAI_EINVAL), ([(0, 96, 0, 1)], [1], _lib.FLYAI_EINVAL),
+    ([(0, 128, 0, 1), (64, 128, 0, 1)], [1, 1], _lib.FLYAI_EINVAL), ([(0, 128, 0, 1), (0, 128, 50, 1)], [1, 1], _lib.FLYAI_EINVAL)])
+def test_compact_refusals(lib, moves, keep, code):
+    assert _compact(lib, moves, keep) == code
+    assert lib.flyai_last_error()
+
+
+def test_long_moves_must_ascend(lib):
+    big = 2 * 1024 * 64
+    keep = list(range(1, 706))
+    keep[300] = keep[299]
+    assert _compact(lib, [(0, 1024, 0, 705)], keep, elems=big) == _lib.FLYAI_EINVAL
+    assert b"ascending" in lib.flyai_last_error()
+
+
+def test_compact_of_nothing(lib):
+    assert _compact(lib, [], []) == 0
+    assert _compact(lib, [(0, 128, 5, 0)], []) == 0
+    assert _compact(lib, [(0, 128, 5, 3)], [0, 1, 2]) == 0           # every row stays
+    assert _compact(lib, [], [], v=None) == _lib.FLYAI_EINVAL
+
+
+def test_rope_frequencies():
+    inv, att = rope_frequencies(64, 10000.0, device="cpu")
+    assert att == 1.0 and inv.dtype == torch.float64 and inv.shape == (32,)
+    assert inv[0] == 1.0 and abs(float(inv[31]) - 10000.0 ** (-62 / 64)) < 1e-18
+    lin, _ = rope_frequencies(64, 10000.0, "linear", factor=8.0, device="cpu")
+    assert torch.equal(lin, inv / 8)
+    ntk, _ = rope_frequencies(64, 10000.0, "ntk", factor=8.0, device="cpu")
+    assert ntk[0] == 1.0 and abs(float(ntk[31] * 8 / inv[31]) - 1) < 1e-12
+    yarn, att = rope_frequencies(64, 10000.0, "yarn", factor=8.0, device="cpu")
+    assert yarn[0] == inv[0] and abs(float(yarn[31] * 8 / inv[31]) - 1) < 1e-12 and att > 1.2
+    for bad in ({"rot_dim": 63}, {"rot_dim": 0}, {"base": 1.0}, {"factor": 0.5}, {"scaling": "other"}, {"original_max": 0},
+                {"rot_dim": 2, "scaling": "ntk"}):
+        with pytest.raises(ValueError):
+            rope_frequencies(**{"rot_dim": 64, "device": "cpu", **bad})

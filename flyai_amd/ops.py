@@ -430,6 +430,9 @@ def kv_fork(k, v, n_kv_heads, src, dsts, lo, hi, src_k=None, src_v=None):
                                   C.byref(one), many, len(dsts), int(lo), int(hi), _stream()))
 
 
+KV_COMPACT_ANY_ORDER = 704  # rows of one slab that kv_compact moves in any order (one launch holds them)
+
+
 def kv_compact(k, v, n_kv_heads, moves):
     """For each move (base, cap, start, keep): position start + i of the slab takes what position start + keep[i] held
     before the call, every layer, in one launch (more beyond 704 moved rows).  keep: host integers (list, numpy or CPU

@@ -50,8 +50,10 @@ class KVWorkspace:
         self.bases = np.concatenate([[0], np.cumsum(self.slabs)]).astype(np.int64)
         self.slab = self.slabs[0]
         n = int(self.bases[-1])
-        self.k = [torch.zeros(n, dtype=torch.bfloat16, device=device) for _ in range(n_layers)]
-        self.v = [torch.zeros(n, dtype=torch.bfloat16, device=device) for _ in range(n_layers)]
+        # every layer's pool in one tensor, so that fork and compact reach them all in one launch; k[i] and v[i] are views
+        self.k_pools = torch.zeros(n_layers, n, dtype=torch.bfloat16, device=device)
+        self.v_pools = torch.zeros(n_layers, n, dtype=torch.bfloat16, device=device)
+        self.k, self.v = self.k_pools.unbind(0), self.v_pools.unbind(0)
 
     def base(self, slot):
         return int(self.bases[slot])
@@ -84,9 +86,38 @@ class KVWorkspace:
         k, v = self.k_dense(layer, slot, src), self.v_dense(layer, slot, src)
         self.set_dense(layer, slot, k, v, dst)
 
+    def _slab_of(self, slot):
+        if not 0 <= int(slot) < self.n_slots:
+            raise ValueError(f"slot {slot} out of range")
+        return self.base(int(slot)), self.caps[int(slot)]
+
+    def fork(self, src, dsts, hi, lo=0, src_ws=None):
+        """Copy positions [lo, hi) of slot src (of src_ws, if it is in another workspace) to the same positions of the
+        slots dsts, every layer, in one launch (``ops.kv_fork``): a prompt's K/V shared by several samples, or a stream
+        that branches.  Nothing else of dsts changes.  Raises ContextOverflow before any write."""
+        w = self if src_ws is None else src_ws
+        if w.n_kv_heads != self.n_kv_heads or w.n_layers < self.n_layers:
+            raise ValueError("fork needs workspaces of the same heads and layers")
+        ops.kv_fork(self.k_pools, self.v_pools, self.n_kv_heads, w._slab_of(src), [self._slab_of(d) for d in dsts], lo, hi,
+                    src_k=w.k_pools[:self.n_layers], src_v=w.v_pools[:self.n_layers])
+
+    def compact(self, slots, starts, keeps):
+        """For each of the slots, move positions start + keep[i] to start + i, every layer, in one launch
+        (``ops.kv_compact``): the accepted path of a drafted tree, or the part of a context that stays in the cache.
+        Raises ContextOverflow before any write."""
+        if not (len(slots) == len(starts) == len(keeps)):
+            raise ValueError("slots, starts and keeps must have one entry per slot")
+        ops.kv_compact(self.k_pools, self.v_pools, self.n_kv_heads,
+                       [(*self._slab_of(s), a, keep) for s, a, keep in zip(slots, starts, keeps)])
+
     def copy_slot(self, dst, src_ws, src_slot=0):
         if src_ws.caps[src_slot] != self.caps[dst] or src_ws.n_kv_heads != self.n_kv_heads:
             raise ValueError("load_prefix needs workspaces of the same capacity and heads")
+        if src_ws is self and src_slot == dst:
+            return
+        if self.k_pools.is_cuda and src_ws.k_pools.device == self.k_pools.device and src_ws.n_layers >= self.n_layers:
+            self.fork(src_slot, [dst], self.caps[dst], src_ws=src_ws)
+            return
         for l in range(self.n_layers):
             self._slab(self.k, l, dst).copy_(src_ws._slab(src_ws.k, l, src_slot))
             self._slab(self.v, l, dst).copy_(src_ws._slab(src_ws.v, l, src_slot))
@@ -321,6 +352,10 @@ class FastVerifyStage:
     def tree_gather(self, start, keep):
         """Compact the accepted path's KV (scratch slots start+keep[i]) to start+i, every layer
         (fastverify.py:301-309)."""
+        keep = [int(k) for k in keep]
+        if len(keep) <= ops.KV_COMPACT_ANY_ORDER or all(a < b for a, b in zip(keep, keep[1:])):
+            self.cache.compact([0], [start], [keep])
+            return
         src = torch.tensor([start + k for k in keep], device=self.dev)
         dst = torch.arange(start, start + len(keep), device=self.dev)
         for l in range(self.n_layers):

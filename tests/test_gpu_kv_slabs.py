@@ -174,3 +174,67 @@ def test_refusals_leave_the_pools_alone():
         ops.kv_fork(k.float(), v.float(), heads, (0, cap), [(slab, cap)], 0, 10)
     torch.cuda.synchronize()
     assert torch.equal(_bits(k), _bits(before[0])) and torch.equal(_bits(v), _bits(before[1]))
+
+
+# ---- through the workspace ---------------------------------------------------------------------------
+
+def _workspace(layers=2, slots=3, caps=(100, 200, 100), heads=2, seed=20):
+    from flyai_amd.runtime import KVWorkspace
+    kv = KVWorkspace(layers, slots, 0, heads, 64, DEV, caps=list(caps))
+    k, v = _pools(layers, kv.k_pools.shape[1], seed)
+    kv.k_pools.copy_(k)
+    kv.v_pools.copy_(v)
+    return kv
+
+
+def _dense(kv):
+    return [[(_bits(kv.k_dense(l, s)), _bits(kv.v_dense(l, s))) for s in range(kv.n_slots)] for l in range(kv.n_layers)]
+
+
+def test_workspace_fork_and_compact():
+    kv = _workspace()
+    before = _dense(kv)
+    kv.fork(1, [0, 2], 77)
+    kv.compact([1, 2], [10, 0], [[3, 8, 20], list(range(4)) + list(range(50, 120))])
+    after = _dense(kv)
+    for l in range(kv.n_layers):
+        for t in range(2):
+            b, a = [x[t] for x in before[l]], [x[t] for x in after[l]]
+            assert torch.equal(a[0][:, :77], b[1][:, :77]) and torch.equal(a[0][:, 77:], b[0][:, 77:])
+            want = b[1].clone()
+            want[:, 10:13] = b[1][:, [13, 18, 30]]
+            assert torch.equal(a[1], want)
+            forked = b[2].clone()
+            forked[:, :77] = b[1][:, :77]
+            want = forked.clone()
+            want[:, 4:74] = forked[:, 50:120]
+            assert torch.equal(a[2], want)
+    with pytest.raises(ContextOverflow):
+        kv.fork(1, [0], 129)
+    with pytest.raises(ValueError):
+        kv.fork(3, [0], 10)
+    with pytest.raises(ValueError):
+        kv.compact([0], [1, 2], [[1]])
+
+
+def test_copy_slot_between_workspaces():
+    kv, other = _workspace(), _workspace(layers=3, slots=1, caps=(200,), seed=21)
+    kv.copy_slot(1, other, 0)
+    for l in range(2):
+        assert torch.equal(_bits(kv.k_dense(l, 1)), _bits(other.k_dense(l, 0)))
+        assert torch.equal(_bits(kv.v_dense(l, 1)), _bits(other.v_dense(l, 0)))
+    before = _dense(kv)
+    kv.copy_slot(0, kv, 2)
+    kv.copy_slot(1, kv, 1)
+    after = _dense(kv)
+    for l in range(2):
+        assert torch.equal(after[l][0][0], before[l][2][0]) and torch.equal(after[l][1][1], before[l][1][1])
+    with pytest.raises(ValueError):
+        kv.copy_slot(0, other, 0)
+
+
+def test_workspace_pools_are_the_layers():
+    kv = _workspace()
+    assert kv.k[1].data_ptr() == kv.k_pools[1].data_ptr() and kv.v[0].data_ptr() == kv.v_pools.data_ptr()
+    kv.zero()
+    assert not bool(kv.k_pools.any()) and not bool(kv.v_pools.any())

@@ -3,6 +3,7 @@
 #include <type_traits>
 
 #include "common.h"
+#include "gemm.h"
 
 namespace flyai {
 
@@ -21,124 +22,7 @@ int launch_rmsnorm(const uint16_t* x, const float* w, int T, int H, float eps, u
   return check_launch("rmsnorm");
 }
 
-// ---- bf16 projections: split-K partial GEMM + fused finalize kernels -------------------------------
-// gemm_splitk: workgroup = 4 or 8 waves on as many consecutive 16-feature tiles and one K slice of kKQW groups
-// of 128.  MFMA step j of group q takes, in lane (r, g), K = 128q + 32j + 8g .. +7 for both operands
-// (any K order shared by the two operands is valid), so each weight load instruction reads one
-// whole 64-byte run of each of its 16 rows.  The activation slice (64 rows x 512 K, bf16) is staged once in LDS; each wave issues all
-// of its weight loads for the slice before its first MFMA (a single HBM round trip per wave) and
-// writes fp32 partial sums part[slice][row][feature].  A finalize kernel adds the slices in slice
-// order (so the result is independent of timing), the bias, and the fused epilogue.
-typedef float f32x4_dw __attribute__((ext_vector_type(4), aligned(4)));  // partials are 4-byte aligned,
-typedef uint16_t u16x4_h __attribute__((ext_vector_type(4), aligned(2)));  // bf16 tensors 2-byte
-constexpr int kKQW = 4;       // K groups of 128 per slice
-constexpr int kGemmRows = 64; // activation rows per pass
-
-// More rows than a pass: the weights stay in registers over the passes of 64 rows, and the next pass's activations
-// are loaded into registers under the current pass's MFMAs (one barrier pair a pass, on LDS only: the loads stay in
-// flight).  A pass used to be staged behind a barrier that drained every load, by workgroups of 64 features: the
-// two projections of 5,120 x 2,880 and 2,880 x 4,096 took 19.2 and 18.5 us at 137 rows, now 16.3 and 15.6; 24.9 and
-// 24.3 at 255, now 22.5 and 22.2.  Eight waves and 128 features read the activations half as often from L2, where
-// that grid still gives most CUs a workgroup (launch_gemm_splitk); wider waves (two feature tiles each) made no
-// difference.  What is left past the weights' 5 us is the partial planes' way out, about 4 us per 64 rows.
-// No load sits under a lane's branch: rows past M and features past N read a clamped one (their sums are not
-// stored), K past the row's end is replaced by zero in both operands.  With the loads predicated the weights' waited
-// for the activations' to return: 7.7 us for 1 row of either projection, 8.1 for 16; now 7.2 and 7.5.  The weights'
-// are under no branch at all (a slice of fewer groups reads its last steps again): with one per group of 128 the
-// compiler could not count them, and the LDS stores waited for all but three of them: kernel and finalize at 64 rows
-// 14.4 us for 5,120 x 2,880, now 14.0, 14.0 for 2,880 x 4,096, now 13.6.
-template <int WAVES>
-__global__ __launch_bounds__(64 * WAVES) void gemm_splitk_bf16_kernel(
-    const uint16_t* __restrict__ x, const uint16_t* __restrict__ W, int M, int N, int K,
-    float* __restrict__ part) {
-  typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
-  __shared__ u32x4 as[kGemmRows][kKQW * 16 + 1];  // 64 rows x 512 bf16, +16 B per row vs bank conflicts
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int r = lane & 15, g = lane >> 4;
-  const int nt = blockIdx.x * WAVES + wave;
-  const int slice = blockIdx.y;
-  const int KQ = (K + 127) / 128;
-  const int kq0 = slice * kKQW;
-  const int nkq = min(kKQW, KQ - kq0);
-  const int feat = nt * 16 + r;
-  // a wave loads whole rows of the slice (64 lanes x 16 bytes): row WAVES j + wave of the pass in load j
-  constexpr int kPer = kGemmRows / WAVES, kPerTile = 16 / WAVES;
-  static_assert(kKQW * 16 == 64, "one row of a slice is one wave load");
-  const int k = 128 * kq0 + 8 * lane;
-  const bool kval = k < K;
-  const uint16_t* xk = x + min(k, K - 8);
-  u32x4 av[kPer];
-  auto load_rows = [&](int m0) __attribute__((always_inline)) {
-#pragma unroll
-    for (int t = 0; t < kGemmRows / 16; ++t)
-      if (m0 + 16 * t < M) {
-#pragma unroll
-        for (int j = t * kPerTile; j < (t + 1) * kPerTile; ++j)
-          av[j] = *reinterpret_cast<const u32x4*>(xk + (size_t)min(m0 + WAVES * j + wave, M - 1) * K);
-      }
-  };
-  auto store_rows = [&](int m0) __attribute__((always_inline)) {
-#pragma unroll
-    for (int t = 0; t < kGemmRows / 16; ++t)
-      if (m0 + 16 * t < M) {
-#pragma unroll
-        for (int j = t * kPerTile; j < (t + 1) * kPerTile; ++j)
-          as[WAVES * j + wave][lane] = kval ? av[j] : u32x4{0u, 0u, 0u, 0u};
-      }
-  };
-  // The activation slice's loads go out first, then the weights, so the LDS stores wait only for the activations
-  // (loads complete in issue order) and the L2 round trip for them overlaps the HBM fetch of the weights.
-  load_rows(0);
-  const uint16_t* wrow = W + (size_t)min(feat, N - 1) * K + 8 * g;
-  u32x4 wv[kKQW][4];
-#pragma unroll
-  for (int q = 0; q < kKQW; ++q)
-#pragma unroll
-    for (int j = 0; j < 4; ++j)  // step j reads K kb + 32j .. +31 (K % 32 == 0)
-      wv[q][j] = *reinterpret_cast<const u32x4*>(wrow + min(128 * (kq0 + q) + 32 * j, K - 32));
-  float* pp = part + (size_t)slice * M * N;
-  for (int m0 = 0; m0 < M; m0 += kGemmRows) {
-    if (m0) lds_barrier();  // every wave has read the previous pass's rows
-    store_rows(m0);
-    if (m0 + kGemmRows < M) load_rows(m0 + kGemmRows);
-    lds_barrier();
-    // the row tiles of the pass as a constant: without branches between them their MFMA chains interleave
-    const auto pass = [&](auto tiles) __attribute__((always_inline)) {
-      constexpr int MT = decltype(tiles)::value;
-      f32x4_t acc[MT];
-#pragma unroll
-      for (int m = 0; m < MT; ++m) acc[m] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int q = 0; q < kKQW; ++q) {
-        if (q >= nkq) break;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const u32x4 w = 128 * (kq0 + q) + 32 * j < K ? wv[q][j] : u32x4{0u, 0u, 0u, 0u};
-#pragma unroll
-          for (int m = 0; m < MT; ++m)
-            acc[m] = mfma16x16x32(__builtin_bit_cast(bf16x8_t, w),
-                                  __builtin_bit_cast(bf16x8_t, as[16 * m + r][q * 16 + 4 * j + g]), acc[m]);
-        }
-      }
-      // weights as the first operand: lane (r, g) holds features 4g .. +3 of row 16m + r, one 16-byte store
-      if (nt * 16 >= N) return;
-#pragma unroll
-      for (int m = 0; m < MT; ++m) {
-        const int row = m0 + 16 * m + r;
-        if (row >= M) continue;
-        auto* o = reinterpret_cast<f32x4_dw*>(pp + (size_t)row * N + nt * 16 + 4 * g);
-        if (WAVES == 8) __builtin_nontemporal_store(acc[m], o);  // planes beyond L2: 137 rows 18.3 -> 16.6 us
-        else *o = acc[m];
-      }
-    };
-    const int mt_count = (min(kGemmRows, M - m0) + 15) / 16;
-    if (mt_count == 4) pass(std::integral_constant<int, 4>{});
-    else if (mt_count == 3) pass(std::integral_constant<int, 3>{});
-    else if (mt_count == 2) pass(std::integral_constant<int, 2>{});
-    else pass(std::integral_constant<int, 1>{});
-  }
-}
-
+// ---- bf16 projections: split-K partial GEMM (gemm.h) + fused finalize kernels ----------------------
 constexpr int kMaxSlices = 16;  // K <= 8192
 
 // Sum of the split-K partials in slice order; all loads are issued before the first add.
@@ -348,7 +232,6 @@ __global__ __launch_bounds__(kRowThreads) void residual_rmsnorm_logits_kernel(
 // which kernel the batch size chose.
 constexpr int kTileM = 128, kTileN = 128;
 constexpr int kTiledWaves = 8;      // 4 (rows) x 2 (features), each wave 32 rows x 64 features
-constexpr int kTiledMinRows = 256;  // batches of at least this many rows take the tiled kernel
 
 __global__ __launch_bounds__(64 * kTiledWaves) void gemm_tiled_bf16_kernel(const uint16_t* __restrict__ x,
                                                                            const uint16_t* __restrict__ W,
@@ -478,12 +361,24 @@ struct QkvEpilogue {
   int rope_positions, Hq, Hkv;
 };
 
-template <bool QKV>
+// The projection with adapters ends in the kernel: y = bf16(sum + up + bias), or bf16(residual + that) to residual.
+struct LinearEpilogue {
+  const uint16_t* bias;
+  uint16_t* y;
+  uint16_t* residual;
+};
+
+enum { kEpiPlane, kEpiQkv, kEpiLinear };
+
+// LORA: the adapters' up products (lora.h) are added to the sums before the epilogue.  A segment is a multiple of the
+// wave's 64 features.
+template <int EPI, bool LORA>
 __global__ __launch_bounds__(64 * kTiledWaves) void gemm_tiled_lds_kernel(const uint16_t* __restrict__ x,
                                                                           const uint16_t* __restrict__ W,
                                                                           int M, int N, int K,
                                                                           float* __restrict__ out,
-                                                                          QkvEpilogue ep) {
+                                                                          QkvEpilogue ep, LinearEpilogue le, LoraArgs lo) {
+  constexpr bool QKV = EPI == kEpiQkv;
   typedef __attribute__((address_space(3))) void* lds_ptr;
   // per stage: the A fragment blocks and the B fragment blocks as separate arrays
   __shared__ __align__(1024) char sa0[kTlStageBytes / 2], sb0[kTlStageBytes / 2];
@@ -594,6 +489,15 @@ __global__ __launch_bounds__(64 * kTiledWaves) void gemm_tiled_lds_kernel(const 
 #pragma unroll
     for (int b = 0; b < 4; ++b) bv[b] = ep.bias ? bf2f(ep.bias[fb + 16 * b + r]) : 0.f;
   }
+  int2 who[2];  // adapter and rank of row 16 (2 wm + a) + r, fetched under the GEMM
+  if constexpr (LORA) {
+#pragma unroll
+    for (int a = 0; a < 2; ++a) who[a] = lo.meta[min(m0 + 16 * (2 * wm + a) + r, M - 1)];
+  }
+  if constexpr (EPI == kEpiLinear) {
+#pragma unroll
+    for (int b = 0; b < 4; ++b) bv[b] = le.bias ? bf2f(le.bias[min(n0 + 64 * wn + 16 * b + r, N - 1)]) : 0.f;
+  }
   // the stage waits count loads per group in issue order: no load may move across a group
   asm volatile("" ::: "memory");
   issue(sa0, sb0, 0);
@@ -646,8 +550,49 @@ __global__ __launch_bounds__(64 * kTiledWaves) void gemm_tiled_lds_kernel(const 
     fold();
   }
   __builtin_amdgcn_s_waitcnt(waitcnt_vm(0));  // the loads issued past the end have landed
+  if constexpr (LORA) {
+    if (n0 + 64 * wn < N) {
+#pragma unroll
+      for (int a = 0; a < 2; ++a) lora_up_rows(lo, M, N, m0 + 16 * (2 * wm + a), n0 + 64 * wn, who[a], tot[a]);
+    }
+  }
   // lane (r, g) holds rows 16(2wm + a) + 4g + v of feature 16(4wn + b) + r
-  if constexpr (!QKV) {
+  if constexpr (EPI == kEpiLinear) {
+    // Each wave turns its 32 x 64 block round in its own 4 KiB of the first stage, so that a row's 128 bytes go out
+    // together: 16-byte chunk c of row q sits at position c ^ (q / 4) % 8.
+    lds_barrier();  // every wave is done with the stages
+    char* blk = wave < 4 ? sa0 + 4096 * wave : sb0 + 4096 * (wave - 4);
+#pragma unroll
+    for (int a = 0; a < 2; ++a)
+#pragma unroll
+      for (int b = 0; b < 4; ++b)
+#pragma unroll
+        for (int v = 0; v < 4; ++v) {
+          const int q = 16 * a + 4 * g + v, c = (16 * b + r) >> 3;
+          *reinterpret_cast<uint16_t*>(blk + q * 128 + ((c ^ ((q >> 2) & 7)) << 4) + (r & 7) * 2) = f2bf(tot[a][b][v] + bv[b]);
+        }
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt(kWaitLgkm0);
+    asm volatile("" ::: "memory");
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int q = 8 * j + (lane >> 3), c = lane & 7;
+      const int row = m0 + 32 * wm + q, feat = n0 + 64 * wn + 8 * c;
+      u32x4_t w = *reinterpret_cast<const u32x4_t*>(blk + q * 128 + ((c ^ ((q >> 2) & 7)) << 4));
+      if (row >= M || feat >= N) continue;
+      if (le.residual) {
+        auto* to = reinterpret_cast<u32x4_t*>(le.residual + (size_t)row * N + feat);
+        const u32x4_t old = *to;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          w[i] = f2bf(__uint_as_float(old[i] << 16) + __uint_as_float(w[i] << 16)) |
+                 (uint32_t)f2bf(__uint_as_float(old[i] & 0xffff0000u) + __uint_as_float(w[i] & 0xffff0000u)) << 16;
+        *to = w;
+      } else {
+        *reinterpret_cast<u32x4_t*>(le.y + (size_t)row * N + feat) = w;
+      }
+    }
+  } else if constexpr (!QKV) {
 #pragma unroll
     for (int a = 0; a < 2; ++a)
 #pragma unroll
@@ -733,13 +678,12 @@ __global__ __launch_bounds__(64 * kTiledWaves) void gemm_tiled_lds_kernel(const 
 int gemm_slices(int K) { return ((K + 127) / 128 + kKQW - 1) / kKQW; }
 
 // fp32 planes launch_gemm writes
-int gemm_planes(int M, int K) { return M >= kTiledMinRows ? 1 : gemm_slices(K); }
+bool gemm_is_tiled(int M) { return M >= kTiledMinRows; }
+int gemm_planes(int M, int K) { return gemm_is_tiled(M) ? 1 : gemm_slices(K); }
 
 size_t linear_partials_bytes(int M, int N, int K) { return (size_t)gemm_slices(K) * M * N * sizeof(float); }
 
-int launch_gemm_splitk(const uint16_t* x, const uint16_t* W, int M, int N, int K, float* part,
-                       hipStream_t s) {
-  const int slices = gemm_slices(K);
+bool splitk_eight_waves(int M, int N, int slices) {
   // Past 64 rows eight waves and 128 features a workgroup, where those workgroups have a CU each and those of four waves
   // would not.  With fewer, half of the chip is idle; with more, the second round is as long as the first.  Kernel and
   // finalize at 137 rows, four waves / eight: 512 x 512 (4 workgroups of eight waves) 11.0 / 15.0 us, 1,024 x 2,880
@@ -747,10 +691,16 @@ int launch_gemm_splitk(const uint16_t* x, const uint16_t* W, int M, int N, int K
   // 2,880 x 4,096 (184) 20.7 / 19.3, 5,120 x 2,880 (240) 22.6 / 20.8; 5,120 x 4,608 (360) 32.0 / 34.3, 2,880 x 8,192
   // (368) 32.4 / 35.5.
   const int cus = device_cus();
-  if (M > kGemmRows && (int64_t)ceil_div(N, 64) * slices > cus && (int64_t)ceil_div(N, 128) * slices <= cus)
-    hipLaunchKernelGGL(gemm_splitk_bf16_kernel<8>, dim3(ceil_div(N, 128), slices), dim3(512), 0, s, x, W, M, N, K, part);
+  return M > kGemmRows && (int64_t)ceil_div(N, 64) * slices > cus && (int64_t)ceil_div(N, 128) * slices <= cus;
+}
+
+int launch_gemm_splitk(const uint16_t* x, const uint16_t* W, int M, int N, int K, float* part,
+                       hipStream_t s) {
+  const int slices = gemm_slices(K);
+  if (splitk_eight_waves(M, N, slices))
+    hipLaunchKernelGGL((gemm_splitk_bf16_kernel<8, false>), dim3(ceil_div(N, 128), slices), dim3(512), 0, s, x, W, M, N, K, part, LoraArgs{}, 0, 0);
   else
-    hipLaunchKernelGGL(gemm_splitk_bf16_kernel<4>, dim3(ceil_div(N, 64), slices), dim3(256), 0, s, x, W, M, N, K, part);
+    hipLaunchKernelGGL((gemm_splitk_bf16_kernel<4, false>), dim3(ceil_div(N, 64), slices), dim3(256), 0, s, x, W, M, N, K, part, LoraArgs{}, 0, 0);
   return check_launch("gemm_splitk_bf16");
 }
 
@@ -762,8 +712,8 @@ int launch_gemm(const uint16_t* x, const uint16_t* W, int M, int N, int K, float
     *slices = 1;
     if (K % 64 == 0) {
       const int tiles = ceil_div(N, kTileN) * ceil_div(M, kTileM);
-      hipLaunchKernelGGL(gemm_tiled_lds_kernel<false>, dim3(8 * ceil_div(tiles, 8)), dim3(64 * kTiledWaves), 0, s, x,
-                         W, M, N, K, part, QkvEpilogue{});
+      hipLaunchKernelGGL((gemm_tiled_lds_kernel<kEpiPlane, false>), dim3(8 * ceil_div(tiles, 8)), dim3(64 * kTiledWaves), 0, s, x,
+                         W, M, N, K, part, QkvEpilogue{}, LinearEpilogue{}, LoraArgs{});
       return check_launch("gemm_tiled_lds");
     }
     hipLaunchKernelGGL(gemm_tiled_bf16_kernel, dim3(ceil_div(N, kTileN), ceil_div(M, kTileM)),
@@ -773,6 +723,22 @@ int launch_gemm(const uint16_t* x, const uint16_t* W, int M, int N, int K, float
   }
   *slices = gemm_slices(K);
   return launch_gemm_splitk(x, W, M, N, K, part, s);
+}
+
+// The tiled kernel ends a projection with adapters by itself where it runs (K % 64 == 0) and no wave's 64 features
+// straddle two segments.
+bool gemm_tiled_lora_fits(int M, int K, const LoraArgs& a) {
+  bool whole = true;
+  for (int i = 0; i + 1 < a.n_seg; ++i) whole &= a.seg_end[i] % 64 == 0;
+  return gemm_is_tiled(M) && K % 64 == 0 && whole;
+}
+
+int launch_gemm_tiled_lora(const uint16_t* x, const uint16_t* W, const uint16_t* b, int M, int N, int K, uint16_t* y,
+                           uint16_t* residual, const LoraArgs& a, hipStream_t s) {
+  const int tiles = ceil_div(N, kTileN) * ceil_div(M, kTileM);
+  hipLaunchKernelGGL((gemm_tiled_lds_kernel<kEpiLinear, true>), dim3(8 * ceil_div(tiles, 8)), dim3(64 * kTiledWaves), 0, s, x, W, M,
+                     N, K, nullptr, QkvEpilogue{}, LinearEpilogue{b, y, residual}, a);
+  return check_launch("gemm_tiled_lora");
 }
 
 int launch_linear(const uint16_t* x, const uint16_t* W, const uint16_t* b, int M, int N, int K,
@@ -1024,8 +990,8 @@ int launch_qkv_rope_kv(const uint16_t* x, const uint16_t* Wqkv, const uint16_t* 
     const int tiles = ceil_div(width, kTileN) * ceil_div(T, kTileM);
     const QkvEpilogue ep{bqkv, positions, seq_id, cos_tab, sin_tab, kv_base, kv_cap, q_out, k_pool, v_pool,
                          rope_positions, Hq, Hkv};
-    hipLaunchKernelGGL(gemm_tiled_lds_kernel<true>, dim3(8 * ceil_div(tiles, 8)), dim3(64 * kTiledWaves), 0, s, x,
-                       Wqkv, T, width, H, part, ep);
+    hipLaunchKernelGGL((gemm_tiled_lds_kernel<kEpiQkv, false>), dim3(8 * ceil_div(tiles, 8)), dim3(64 * kTiledWaves), 0, s, x,
+                       Wqkv, T, width, H, part, ep, LinearEpilogue{}, LoraArgs{});
     return check_launch("gemm_tiled_lds_qkv");
   }
   int slices = 0;

@@ -1,5 +1,8 @@
-// The low-rank adapters' arguments and their up product, for the kernels that add it to a projection.
+// Low-rank adapters of many requests at once, for the kernels that add them to a projection: the arguments, the down
+// product h = scale (x A^T) of each row's adapter, and the up product d = h B^T.
 #pragma once
+#include <type_traits>
+
 #include "common.h"
 
 namespace flyai {
@@ -13,20 +16,15 @@ struct LoraArgs {
   const int32_t* row_seq;  // null: adapter is per row
   int n, R, n_seg, n_seqs;
   int seg_end[3];  // first feature past segments 0, 1, 2
+  // the workspace: h as two bf16 terms [M][n_seg][R32 high | R32 low], R32 = R rounded up to 32, and each row's adapter
+  // and rank (0: none)
+  uint16_t* h;
+  int2* meta;
 };
 
-// The adapter of row t, -1 for none (an id or a sequence out of range is none).
-__device__ __forceinline__ int lora_of_row(const LoraArgs& a, int t) {
-  int i = t;
-  if (a.row_seq) {
-    i = a.row_seq[t];
-    if ((unsigned)i >= (unsigned)a.n_seqs) return -1;
-  }
-  const int ad = a.adapter[i];
-  return (unsigned)ad < (unsigned)a.n ? ad : -1;
-}
+constexpr int kLoraCols = 32;  // rank columns of one product: an MFMA's K
 
-__device__ __forceinline__ int lora_rank(const LoraArgs& a, int ad) { return min(max(a.ranks[ad], 0), a.R); }
+__host__ __device__ inline int lora_cols(int R) { return (R + kLoraCols - 1) / kLoraCols * kLoraCols; }
 
 // The segment of feature f (wave-uniform when f is).
 __device__ __forceinline__ int lora_segment(const LoraArgs& a, int f) {
@@ -36,33 +34,261 @@ __device__ __forceinline__ int lora_segment(const LoraArgs& a, int f) {
   return seg;
 }
 
-// d += h B^T on a tile of 16 rows from m0 and 16 features from f0 (one segment, a multiple of 16): lane (r, g) gets
-// features f0 + 4g .. +3 of row m0 + r, whose adapter is `mine` (-1: none).  One product per adapter among the rows, from
-// zero over its rank's chunks in order, kept by its own rows alone: what another row's adapter holds, an infinity or a
-// NaN among it, never reaches this one, and the sum does not depend on the tile.
-__device__ __forceinline__ void lora_up_tile(const LoraArgs& a, const uint16_t* __restrict__ h, int M, int N, int m0, int f0,
-                                             int mine, f32x4_t& d) {
+// ---- down ----------------------------------------------------------------------------------------------------------
+// The batch's work is the pairs of a 64-row tile and an adapter among its rows, times the groups of 32 rank columns in
+// every segment.  Each workgroup lists the pairs for itself (adapters of up to 64 * TILES rows in LDS, and how many distinct
+// ones each tile has) and takes every wgs-th item: none is launched in vain, whatever the mix.
+// An item multiplies the tile's rows that have the adapter, gathered, 16 to an MFMA tile, with 32 rows of A.  K is cut into
+// four parts, a wave each, whose sums are added in order through LDS; lane (r, g) of an MFMA holds row r in its second
+// operand, so a row's products never meet another row's: a row's h depends neither on its tile nor on the launch.
+// What bounds it is how fast rows of x and A come from L2.  A wave loads whole 128-byte runs (8 rows an instruction) and
+// turns them round in LDS of its own (the tiled GEMM's swizzle); loaded as MFMA operands, 16 rows of 64 bytes an
+// instruction, every quarter of an instruction touched 16 lines, and 2,096 rows of 192 rank columns took 51 us.
+// h is kept as two bf16 terms, the value and what its rounding left out: 16 significant bits (2^-17 of d at most) for the
+// bytes of one fp32 value, and the up product takes them as they are.
+constexpr int kDownParts = 4;   // parts of K
+constexpr int kDownRows = 64;   // rows of a tile
+constexpr int kDownCols = kLoraCols;
+
+template <int WAVES, int TILES>
+struct LoraDownLds {
+  union {
+    char stage[kDownParts][(kDownRows + kDownCols) * 128];       // a wave's 64-K group: rows of x, rows of A
+    float red[kDownParts][kDownRows][kDownCols + 4];
+  };
+  int adapter[kDownRows * TILES];       // -1 where the row has none, or one of rank 0
+  int first[TILES + 1];                 // pairs before the tile
+  int of_seq[64 * WAVES], rank_of[64 * WAVES];
+  int row[kDownRows];                   // the item's rows within its tile
+};
+
+inline int lora_down_groups(const LoraArgs& a) { return a.n_seg * (lora_cols(a.R) / kDownCols); }
+
+// One wave's part of an item's product: NP * 16 gathered rows (l.row, n of them) against 32 rows of A from ar, over the
+// 64-K groups [k0, k1).  D groups are in flight in registers.
+template <int NP, int D, typename Lds>
+__device__ __forceinline__ void lora_down_part(const uint16_t* __restrict__ x, const uint16_t* __restrict__ ar, int a_rows, int K,
+                                               int m0, int n, int k0, int k1, char* st, const Lds& l, f32x4_t (&acc)[4][2]) {
+  constexpr int NX = 2 * NP, NI = NX + kDownCols / 8;  // load instructions a group: 8 rows each
   const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
-  const int chunks = a.R / 16, seg = lora_segment(a, f0);
-  const uint16_t* hr = h + ((size_t)min(m0 + r, M - 1) * a.n_seg + seg) * chunks * 32 + 8 * g;
-  uint64_t todo = __ballot(mine >= 0) & 0xffff;
-  for (; todo;) {
-    const int ad = __builtin_amdgcn_readlane(mine, __builtin_ctzll(todo));
-    todo &= ~__ballot(mine == ad);
-    const int rank = lora_rank(a, ad);
-    const uint16_t* br = a.B + ((size_t)ad * N + f0 + r) * a.R + 8 * (g & 1);
-    f32x4_t acc = {0.f, 0.f, 0.f, 0.f};
-    for (int c = 0; 16 * c < rank; ++c) {
-      uint4 bw = *reinterpret_cast<const uint4*>(br + 16 * c);
-      const int left = rank - 16 * c - 8 * (g & 1);  // columns of this lane's eight within the rank
-      if (left < 8) {
-        uint32_t* w = reinterpret_cast<uint32_t*>(&bw);
+  const uint16_t* src[NI];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) w[i] = 2 * i + 1 < left ? w[i] : 2 * i < left ? w[i] & 0xffffu : 0u;
-      }
-      acc = mfma16x16x32(as_bf16x8(bw), as_bf16x8(*reinterpret_cast<const uint4*>(hr + 32 * c)), acc);
+  for (int i = 0; i < NI; ++i) {
+    const int q = 8 * (i < NX ? i : i - NX) + (lane >> 3);
+    src[i] = i < NX ? x + (size_t)(m0 + l.row[min(q, n - 1)]) * K : ar + (size_t)min(q, a_rows - 1) * K;
+  }
+  u32x4_t buf[D][NI];
+  auto load = [&](u32x4_t (&b)[NI], int kg) __attribute__((always_inline)) {
+    const int k = 64 * min(kg, k1 - 1);
+    const int within = k + 64 <= K ? 7 : 3;  // the last group may have 32 K: the others are read again and not used
+#pragma unroll
+    for (int i = 0; i < NI; ++i) {
+      const int c = (lane & 7) ^ (4 * (i & 1) + (lane >> 4));  // position lane % 8 holds chunk c: the row's swizzle
+      b[i] = *reinterpret_cast<const u32x4_t*>(src[i] + k + 8 * (c & within));
     }
-    if (mine == ad) d = acc;
+  };
+#pragma unroll
+  for (int d = 0; d < D; ++d) load(buf[d], k0 + d);
+  const int frag = r * 128 + ((g ^ ((r >> 1) & 7)) << 4);
+  for (int kb = k0; kb < k1; kb += D) {
+#pragma unroll
+    for (int d = 0; d < D; ++d) {
+      if (kb + d >= k1) break;
+#pragma unroll
+      for (int i = 0; i < NI; ++i) *reinterpret_cast<u32x4_t*>(st + 1024 * i + 16 * lane) = buf[d][i];
+      asm volatile("" ::: "memory");  // this wave's LDS operations complete in order
+      load(buf[d], kb + d + D);
+      const bool half = 64 * (kb + d) + 64 > K;
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        if (j == 1 && half) break;
+        bf16x8_t av[2], xv[NP];
+#pragma unroll
+        for (int c = 0; c < 2; ++c) av[c] = as_bf16x8(*reinterpret_cast<const uint4*>(st + 1024 * NX + 2048 * c + (frag ^ (j << 6))));
+#pragma unroll
+        for (int p = 0; p < NP; ++p) xv[p] = as_bf16x8(*reinterpret_cast<const uint4*>(st + 2048 * p + (frag ^ (j << 6))));
+#pragma unroll
+        for (int p = 0; p < NP; ++p)
+#pragma unroll
+          for (int c = 0; c < 2; ++c) acc[p][c] = mfma16x16x32(av[c], xv[p], acc[p][c]);
+      }
+      asm volatile("" ::: "memory");
+    }
+  }
+}
+
+template <int WAVES, int TILES>
+__device__ __forceinline__ void lora_down(const uint16_t* __restrict__ x, int M, int K, const LoraArgs& a, int wg, int wgs,
+                                          LoraDownLds<WAVES, TILES>& l) {
+  constexpr int kThreads = 64 * WAVES;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), r = lane & 15, g = lane >> 4;
+  const int cols = lora_cols(a.R), per_seg = cols / kDownCols, groups = a.n_seg * per_seg;
+  const int KG = (K + 63) / 64;
+  const int32_t* row_of = a.row_seq ? a.row_seq : a.adapter;
+  // Rows, sequences and ranks are fetched side by side where the tables fit a workgroup: one round trip, not three.
+  const bool small = a.n <= kThreads && (!a.row_seq || a.n_seqs <= kThreads);
+  for (int t0 = 0; t0 < M; t0 += kDownRows * TILES) {
+    const int rows = min(M - t0, kDownRows * TILES), tiles = (rows + kDownRows - 1) / kDownRows;
+    if (t0) __syncthreads();
+    const int mine0 = row_of[t0 + min(tid, rows - 1)];  // the wave's first tile
+    if (t0 == 0 && small) {
+      if (tid < a.n) l.rank_of[tid] = min(max(a.ranks[tid], 0), a.R);
+      if (a.row_seq && tid < a.n_seqs) l.of_seq[tid] = a.adapter[tid];
+    }
+    if (tid == 0) l.first[0] = 0;
+    __syncthreads();
+    for (int t = wave; t < tiles; t += WAVES) {
+      const int i = kDownRows * t + lane;
+      int ad = t == wave ? mine0 : row_of[t0 + min(i, rows - 1)], rank = 0;
+      if (a.row_seq) {
+        const bool in = (unsigned)ad < (unsigned)a.n_seqs;
+        const int sq = in ? ad : 0;
+        ad = small ? l.of_seq[sq] : a.adapter[sq];
+        if (!in) ad = -1;
+      }
+      if ((unsigned)ad < (unsigned)a.n) rank = small ? l.rank_of[ad] : min(max(a.ranks[ad], 0), a.R);
+      if (i >= rows || rank == 0) ad = -1;
+      l.adapter[i] = ad;
+      if (wg == 0 && i < rows) a.meta[t0 + i] = make_int2(ad, ad < 0 ? 0 : rank);
+      int n = 0;
+      for (uint64_t todo = __ballot(ad >= 0); todo; ++n)
+        todo &= ~__ballot(ad == __builtin_amdgcn_readlane(ad, __builtin_ctzll(todo)));
+      if (lane == 0) l.first[t + 1] = n;
+    }
+    __syncthreads();
+    if (wave == 0) {  // running sums
+      static_assert(TILES <= 64, "a lane a tile");
+      int sum = lane < tiles ? l.first[lane + 1] : 0;
+#pragma unroll
+      for (int off = 1; off < TILES; off <<= 1) {
+        const int o = __shfl_up(sum, off, 64);
+        if (lane >= off) sum += o;
+      }
+      if (lane < tiles) l.first[lane + 1] = sum;
+    }
+    __syncthreads();
+    const int items = __builtin_amdgcn_readfirstlane(l.first[tiles]) * groups;
+    const int before = l.first[min(lane, tiles)];
+    for (int it = wg; it < items; it += wgs) {
+      const int pair = it / groups, seg = it % groups / per_seg, c0 = it % groups % per_seg * kDownCols;
+      const int tile = __builtin_popcountll(__ballot(lane < tiles && before <= pair)) - 1;  // the last that starts at or before it
+      const int nth = pair - __builtin_amdgcn_readlane(before, tile);
+      const int m0 = t0 + kDownRows * tile;
+      const int mine = l.adapter[kDownRows * tile + lane];
+      uint64_t todo = __ballot(mine >= 0);
+      for (int i = 0; i < nth; ++i) todo &= ~__ballot(mine == __builtin_amdgcn_readlane(mine, __builtin_ctzll(todo)));
+      const int ad = __builtin_amdgcn_readlane(mine, __builtin_ctzll(todo));
+      const uint64_t rows_of = __ballot(mine == ad);
+      const int n = __builtin_popcountll(rows_of);
+      const int rank = __builtin_amdgcn_readfirstlane(small ? l.rank_of[ad] : min(max(a.ranks[ad], 0), a.R));
+      if (c0 >= rank) continue;  // the same in every wave: columns past the rank's last 32 are never read
+      const float scale = a.scale[ad];
+      if (wave == 0 && mine == ad) l.row[__builtin_popcountll(rows_of & ((1ull << lane) - 1))] = lane;
+      __syncthreads();
+      f32x4_t acc[4][2];
+#pragma unroll
+      for (int p = 0; p < 4; ++p) acc[p][0] = acc[p][1] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+      if (wave < kDownParts) {
+        const uint16_t* ar = a.A + (((size_t)ad * a.n_seg + seg) * a.R + c0) * K;
+        const int k0 = KG * wave / kDownParts, k1 = KG * (wave + 1) / kDownParts, a_rows = min(rank - c0, kDownCols);
+        if (k0 == k1) {}  // fewer groups than waves
+        else if (n <= 16) lora_down_part<1, 4>(x, ar, a_rows, K, m0, n, k0, k1, l.stage[wave], l, acc);
+        else if (n <= 32) lora_down_part<2, 2>(x, ar, a_rows, K, m0, n, k0, k1, l.stage[wave], l, acc);
+        else lora_down_part<4, 2>(x, ar, a_rows, K, m0, n, k0, k1, l.stage[wave], l, acc);
+      }
+      __syncthreads();  // red lies over the stages
+      if (wave < kDownParts) {  // lane (r, g): rank columns 4g .. +3 of row r
+#pragma unroll
+        for (int p = 0; p < 4; ++p)
+          if (16 * p < n) {
+#pragma unroll
+            for (int c = 0; c < 2; ++c) *reinterpret_cast<f32x4_t*>(&l.red[wave][16 * p + r][16 * c + 4 * g]) = acc[p][c];
+          }
+      }
+      __syncthreads();
+      for (int i = tid; i < n * kDownCols; i += kThreads) {
+        const int q = i / kDownCols, j = i % kDownCols;
+        float v = 0.f;  // columns past the rank are zero, whatever A holds
+        if (c0 + j < rank) {
+          v = l.red[0][q][j];
+#pragma unroll
+          for (int e = 1; e < kDownParts; ++e) v += l.red[e][q][j];
+          v *= scale;
+        }
+        const uint16_t hi = f2bf(v);
+        const float rest = v - bf2f(hi);
+        uint16_t* o = a.h + ((size_t)(m0 + l.row[q]) * a.n_seg + seg) * 2 * cols + c0 + j;
+        o[0] = hi;
+        o[cols] = rest == rest ? f2bf(rest) : 0;  // a value past bf16's range keeps its infinity: inf - inf would be NaN
+      }
+      __syncthreads();
+    }
+  }
+}
+
+// ---- up ------------------------------------------------------------------------------------------------------------
+// d = h B^T in products of 32 rank columns, the high terms of h and then the low ones against the same columns of B: lane
+// (r, g) of an operand takes columns 32c + 8g .. +7.  A sum starts from zero for each adapter and is kept by its own rows
+// alone, so nothing of another row's adapter, an infinity or a NaN among it, reaches a row, and it does not depend on the
+// tile.
+
+// Columns past the rank as zero, whatever they hold; `left` of this lane's eight are within it.
+__device__ __forceinline__ bf16x8_t lora_within(uint4 w, int left) {
+  uint32_t v[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) v[i] = 2 * i + 1 < left ? v[i] : 2 * i < left ? v[i] & 0xffffu : 0u;
+  return as_bf16x8(make_uint4(v[0], v[1], v[2], v[3]));
+}
+
+// Where lane (r, g) reads its eight columns from 32c on in a row of B of R columns (clamped: those past R are masked).
+__device__ __forceinline__ int lora_col(int R, int c, int g) { return min(kLoraCols * c + 8 * g, R - 8); }
+
+// The up product of 16 rows from m0 and 64 features from f0 (one segment), added to the tiled GEMM's sums: lane (r, g)
+// holds rows 4g .. +3 of feature f0 + 16 b + r in sum[b].  `who` is row m0 + r's adapter and rank.
+__device__ __forceinline__ void lora_up_rows(const LoraArgs& a, int M, int N, int m0, int f0, int2 who, f32x4_t (&sum)[4]) {
+  const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
+  const int cols = lora_cols(a.R), seg = lora_segment(a, f0);
+  const int mine = m0 + r < M && who.y > 0 ? who.x : -1;
+  int of_row[4];
+#pragma unroll
+  for (int v = 0; v < 4; ++v) of_row[v] = __builtin_amdgcn_ds_bpermute(4 * (4 * g + v), mine);
+  const uint16_t* hr = a.h + ((size_t)min(m0 + r, M - 1) * a.n_seg + seg) * 2 * cols + 8 * g;
+  const uint16_t* br[4];
+#pragma unroll
+  for (int b = 0; b < 4; ++b) br[b] = a.B + (size_t)min(f0 + 16 * b + r, N - 1) * a.R;
+  uint64_t todo = __ballot(mine >= 0) & 0xffff;
+  while (todo) {
+    const int first = __builtin_ctzll(todo);
+    const int ad = __builtin_amdgcn_readlane(mine, first), rank = __builtin_amdgcn_readlane(who.y, first);
+    todo &= ~__ballot(mine == ad);
+    f32x4_t up[4];
+#pragma unroll
+    for (int b = 0; b < 4; ++b) up[b] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+    for (int c0 = 0; kLoraCols * c0 < rank; c0 += 2) {
+      uint4 hi[2], lo[2], bv[4][2];
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        const int cc = min(c0 + c, (rank - 1) / kLoraCols);
+        hi[c] = *reinterpret_cast<const uint4*>(hr + kLoraCols * cc);
+        lo[c] = *reinterpret_cast<const uint4*>(hr + kLoraCols * cc + cols);
+#pragma unroll
+        for (int b = 0; b < 4; ++b) bv[b][c] = *reinterpret_cast<const uint4*>(br[b] + (size_t)ad * N * a.R + lora_col(a.R, cc, g));
+      }
+#pragma unroll
+      for (int c = 0; c < 2; ++c)
+        if (kLoraCols * (c0 + c) < rank) {
+#pragma unroll
+          for (int b = 0; b < 4; ++b) {
+            const bf16x8_t w = lora_within(bv[b][c], rank - kLoraCols * (c0 + c) - 8 * g);
+            up[b] = mfma16x16x32(as_bf16x8(hi[c]), w, up[b]);
+            up[b] = mfma16x16x32(as_bf16x8(lo[c]), w, up[b]);
+          }
+        }
+    }
+#pragma unroll
+    for (int b = 0; b < 4; ++b)
+#pragma unroll
+      for (int v = 0; v < 4; ++v) sum[b][v] += of_row[v] == ad ? up[b][v] : -0.f;
   }
 }
 

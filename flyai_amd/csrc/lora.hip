@@ -1,120 +1,185 @@
 // Low-rank adapters of many requests at once beside a shared projection.
 #include <algorithm>
+#include <type_traits>
 
 #include "common.h"
-#include "lora.h"
+#include "gemm.h"
 
 namespace flyai {
 
 int launch_gemm(const uint16_t* x, const uint16_t* W, int M, int N, int K, float* part, int* slices, hipStream_t s);
+int launch_gemm_tiled_lora(const uint16_t* x, const uint16_t* W, const uint16_t* b, int M, int N, int K, uint16_t* y, uint16_t* residual,
+                           const LoraArgs& a, hipStream_t s);
+bool gemm_tiled_lora_fits(int M, int K, const LoraArgs& a);
+bool gemm_is_tiled(int M);
 int gemm_planes(int M, int K);
 
-// ---- down: h = scale (x A^T) of each row's adapter ---------------------------------------------------------------
-// A workgroup takes 16 rows and one chunk of 16 rank columns of one segment; its waves split K and their sums are added
-// in wave order through LDS, so a row's h does not depend on its tile.  Lane (r, g) of an MFMA holds row r in both
-// operands, so a row's products never meet another row's: for each adapter among the 16 rows the whole tile is
-// multiplied and only its own rows keep the result.
-// h is kept as two bf16 terms, the value and what its rounding left out, side by side as the 32 values of one MFMA's K:
-// [row][segment][chunk][16 high | 16 low].  Against the up matrix's 16 columns, taken twice, one MFMA gives the
-// product with an h of 16 significant bits (2^-17 of d at most), for the bytes of one fp32 value.
-constexpr int kDownWaves = 8;
+// The down product by itself, for batches whose projection takes the tiled kernel (smaller ones have it in the
+// projection's launch, gemm_splitk_bf16_kernel).
+constexpr int kDownTiles = 64;
 
-__global__ __launch_bounds__(64 * kDownWaves) void lora_down_kernel(const uint16_t* __restrict__ x, int M, int K,
-                                                                    LoraArgs a, uint16_t* __restrict__ h) {
-  __shared__ float red[kDownWaves][16][20];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, g = lane >> 4;
-  const int m0 = blockIdx.x * 16, chunks = a.R / 16;
-  const int sc = blockIdx.y, seg = sc / chunks, c = sc % chunks;
-  const int mine = m0 + r < M ? lora_of_row(a, m0 + r) : -1;
-  const int steps = K / 32, s0 = steps * wave / kDownWaves, s1 = steps * (wave + 1) / kDownWaves;
-  const uint16_t* xr = x + (size_t)min(m0 + r, M - 1) * K + 8 * g;
-  uint64_t todo = __ballot(mine >= 0) & 0xffff;
-  for (; todo;) {
-    const int ad = __builtin_amdgcn_readlane(mine, __builtin_ctzll(todo));
-    const uint64_t rows = __ballot(mine == ad) & 0xffff;
-    todo &= ~rows;
-    const int rank = lora_rank(a, ad);
-    const bool live = 16 * c < rank;  // a chunk past the adapter's rank is never read
-    if (live) {
-      const uint16_t* ar = a.A + ((size_t)ad * a.n_seg * a.R + (size_t)seg * a.R + 16 * c + r) * K + 8 * g;
-      f32x4_t acc = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 8
-      for (int s = s0; s < s1; ++s)
-        acc = mfma16x16x32(as_bf16x8(*reinterpret_cast<const uint4*>(ar + 32 * s)),
-                           as_bf16x8(*reinterpret_cast<const uint4*>(xr + 32 * s)), acc);
-      // lane (r, g): rank columns 4g .. +3 of row r
-      if (mine == ad) *reinterpret_cast<f32x4_t*>(&red[wave][r][4 * g]) = acc;
-    }
-  }
-  __syncthreads();
-  const int row = threadIdx.x >> 4, j = threadIdx.x & 15;
-  if (row < 16 && m0 + row < M) {
-    const int ad = lora_of_row(a, m0 + row);
-    const int rank = ad >= 0 ? lora_rank(a, ad) : 0;
-    if (16 * c < rank) {
-      float v = red[0][row][j];
-#pragma unroll
-      for (int w = 1; w < kDownWaves; ++w) v += red[w][row][j];
-      v = 16 * c + j < rank ? v * a.scale[ad] : 0.f;
-      const uint16_t hi = f2bf(v);
-      // a value past bf16's range keeps its infinity: inf - inf would make it NaN
-      const float rest = v - bf2f(hi);
-      uint16_t* o = h + (((size_t)(m0 + row) * a.n_seg + seg) * chunks + c) * 32 + j;
-      o[0] = hi;
-      o[16] = rest == rest ? f2bf(rest) : 0;
-    }
-  }
+__global__ __launch_bounds__(64 * kDownParts) void lora_down_kernel(const uint16_t* __restrict__ x, int M, int K, LoraArgs a) {
+  __shared__ LoraDownLds<kDownParts, kDownTiles> lds;
+  lora_down<kDownParts, kDownTiles>(x, M, K, a, blockIdx.x, gridDim.x, lds);
 }
 
-// ---- up: y = bf16(sum of the projection's planes + h B^T + bias) -------------------------------------------------
-// A wave takes 16 rows x 16 features: lane (r, g) holds features 4g .. +3 of row r.
-__global__ __launch_bounds__(256) void lora_finalize_kernel(const float* __restrict__ part, int slices, int M, int N,
-                                                            LoraArgs a, const uint16_t* __restrict__ h,
-                                                            const uint16_t* __restrict__ b, uint16_t* __restrict__ y,
-                                                            uint16_t* __restrict__ residual) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, g = lane >> 4;
-  const int f0 = (blockIdx.x * 4 + wave) * 16, m0 = blockIdx.y * 16;
-  if (f0 >= N) return;
-  const int row = m0 + r;
-  const size_t idx = (size_t)min(row, M - 1) * N + f0 + 4 * g;
-  const int mine = row < M ? lora_of_row(a, row) : -1;
-  f32x4_t d = {0.f, 0.f, 0.f, 0.f};
-  lora_up_tile(a, h, M, N, m0, f0, mine, d);
-  const size_t plane = (size_t)M * N;
-  f32x4_t o = *reinterpret_cast<const f32x4_t*>(part + idx);
-  for (int i = 1; i < slices; ++i) o += *reinterpret_cast<const f32x4_t*>(part + i * plane + idx);
-  if (row >= M) return;
-  ushort4 bv = make_ushort4(0, 0, 0, 0), rv = bv, out;
-  if (b) bv = *reinterpret_cast<const ushort4*>(b + f0 + 4 * g);
-  if (residual) rv = *reinterpret_cast<const ushort4*>(residual + idx);
-  const uint16_t bb[4] = {bv.x, bv.y, bv.z, bv.w}, rr[4] = {rv.x, rv.y, rv.z, rv.w};
-  uint16_t oo[4];
+// ---- up, and the projection's finalize ---------------------------------------------------------------------------
+// y = bf16(sum of the projection's planes + h B^T + bias); or, without planes, h B^T as a plane of its own for another
+// finalize to add (-0 where a row has no adapter: x + -0 is x).
+// A workgroup takes 16 rows x 16 features.  Its four waves share the adapters among the rows: each multiplies the whole
+// tile with its own, and the adapter's rows keep the result.  Up to NS adapters of a wave and 64 columns of each are
+// loaded together: what bounds this kernel is latency, not bytes.
+// `firsts` has a bit for each distinct adapter, at its first row.
+template <int NS>
+__device__ __forceinline__ void lora_up_wave(const LoraArgs& a, int M, int N, int m0, int f0, int2 who, uint64_t firsts, int wave,
+                                             float (*d)[17]) {
+  const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
+  const int cols = lora_cols(a.R), seg = lora_segment(a, f0);
+  const uint16_t* hr = a.h + ((size_t)min(m0 + r, M - 1) * a.n_seg + seg) * 2 * cols + 8 * g;
+  const uint16_t* br = a.B + (size_t)(f0 + r) * a.R;
+  int ads[NS], ranks[NS], most = 0;
+  for (int i = 0; i < wave; ++i) firsts &= firsts - 1;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const float v = mine >= 0 ? o[i] + d[i] : o[i];
-    const float q = bf16_round(v + (b ? bf2f(bb[i]) : 0.f));
-    oo[i] = residual ? f2bf(bf2f(rr[i]) + q) : f2bf(q);
+  for (int s = 0; s < NS; ++s) {  // slots past the wave's adapters repeat the one before
+    if (s == 0 || firsts) {
+      const int at = __builtin_ctzll(firsts);
+      ads[s] = __builtin_amdgcn_readlane(who.x, at);
+      ranks[s] = __builtin_amdgcn_readlane(who.y, at);
+      for (int i = 0; i < 4; ++i) firsts &= firsts - 1;
+    } else {
+      ads[s] = ads[s ? s - 1 : 0], ranks[s] = ranks[s ? s - 1 : 0];
+    }
+    most = max(most, ranks[s]);
   }
-  out = make_ushort4(oo[0], oo[1], oo[2], oo[3]);
-  *reinterpret_cast<ushort4*>((residual ? residual : y) + idx) = out;
+  f32x4_t acc[NS];
+#pragma unroll
+  for (int s = 0; s < NS; ++s) acc[s] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+  for (int c0 = 0; kLoraCols * c0 < most; c0 += 2) {
+    uint4 bv[NS][2], hi[2], lo[2];
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      const int cc = min(kLoraCols * (c0 + c), cols - kLoraCols);
+      hi[c] = *reinterpret_cast<const uint4*>(hr + cc);
+      lo[c] = *reinterpret_cast<const uint4*>(hr + cc + cols);
+    }
+#pragma unroll
+    for (int s = 0; s < NS; ++s)
+#pragma unroll
+      for (int c = 0; c < 2; ++c)
+        bv[s][c] = *reinterpret_cast<const uint4*>(br + (size_t)ads[s] * N * a.R + lora_col(a.R, min(c0 + c, (ranks[s] - 1) / kLoraCols), g));
+#pragma unroll
+    for (int c = 0; c < 2; ++c)
+#pragma unroll
+      for (int s = 0; s < NS; ++s)
+        if (kLoraCols * (c0 + c) < ranks[s]) {
+          const bf16x8_t w = lora_within(bv[s][c], ranks[s] - kLoraCols * (c0 + c) - 8 * g);
+          acc[s] = mfma16x16x32(w, as_bf16x8(hi[c]), acc[s]);
+          acc[s] = mfma16x16x32(w, as_bf16x8(lo[c]), acc[s]);
+        }
+  }
+  // lane (r, g): features 4g .. +3 of row r
+#pragma unroll
+  for (int s = 0; s < NS; ++s)
+    if (who.y > 0 && who.x == ads[s]) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) d[r][4 * g + i] = acc[s][i];
+    }
+}
+
+template <bool PLANE>
+__global__ __launch_bounds__(256) void lora_finalize_kernel(const float* __restrict__ part, int slices, int M, int N,
+                                                            LoraArgs a, const uint16_t* __restrict__ b,
+                                                            uint16_t* __restrict__ y, uint16_t* __restrict__ residual,
+                                                            float* __restrict__ plane_out) {
+  __shared__ float d[16][17];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = lane & 15;
+  const int f0 = blockIdx.x * 16, m0 = blockIdx.y * 16;
+  int2 who = a.meta[min(m0 + r, M - 1)];
+  // this thread's output: row 4 * wave + lane / 16, feature lane % 16
+  const int mine = 4 * wave + (lane >> 4), row = m0 + mine;
+  const size_t idx = (size_t)min(row, M - 1) * N + f0 + r, plane = (size_t)M * N;
+  float p[8];
+  uint16_t bias = 0, res = 0;
+  if constexpr (!PLANE) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) p[i] = part[min(i, slices - 1) * plane + idx];
+    // no load under a branch: its wait would be for everything before it
+    bias = *(b ? b + f0 + r : a.B);
+    res = *(residual ? residual + idx : a.B);
+  }
+  if (m0 + r >= M) who.y = 0;
+  const bool has = __builtin_amdgcn_ds_bpermute(4 * mine, who.y) > 0;
+  const int key = who.y > 0 ? who.x : -1;
+  bool fresh = key >= 0;  // the first of its adapter's rows
+#pragma unroll
+  for (int i = 0; i < 15; ++i) fresh &= i >= r || __builtin_amdgcn_readlane(key, i) != key;
+  const uint64_t firsts = __ballot(fresh) & 0xffff;
+  const int n = __builtin_popcountll(firsts), share = (n - wave + 3) / 4;
+  if (share > 2) lora_up_wave<4>(a, M, N, m0, f0, who, firsts, wave, d);
+  else if (share == 2) lora_up_wave<2>(a, M, N, m0, f0, who, firsts, wave, d);
+  else if (share == 1) lora_up_wave<1>(a, M, N, m0, f0, who, firsts, wave, d);
+  if (n > 0) __syncthreads();
+  if (row >= M) return;
+  const float up = has ? d[mine][r] : -0.f;
+  if constexpr (PLANE) {
+    plane_out[idx] = up;
+  } else {
+    float o = p[0];
+#pragma unroll
+    for (int i = 1; i < 8; ++i)
+      if (i < slices) o += p[i];
+    for (int i = 8; i < slices; ++i) o += part[i * plane + idx];
+    const float q = bf16_round(o + up + (b ? bf2f(bias) : 0.f));
+    if (residual) residual[idx] = f2bf(bf2f(res) + q);
+    else y[idx] = f2bf(q);
+  }
 }
 
 static size_t align256(size_t v) { return (v + 255) & ~(size_t)255; }
 
 static size_t partial_bytes(int M, int N, int K) { return (size_t)gemm_planes(M, K) * M * N * sizeof(float); }
 
-int launch_linear_lora(const uint16_t* x, const uint16_t* W, const uint16_t* b, int M, int N, int K, const LoraArgs& a,
-                       uint16_t* y, uint16_t* residual, char* ws, hipStream_t s) {
+static int launch_lora_down(const uint16_t* x, int M, int K, const LoraArgs& a, hipStream_t s) {
+  const int wgs = std::min(2 * device_cus(), M * lora_down_groups(a));
+  hipLaunchKernelGGL(lora_down_kernel, dim3(wgs), dim3(64 * kDownParts), 0, s, x, M, K, a);
+  return check_launch("lora_down");
+}
+
+// The projection's planes and h: one launch where the split-K kernel has four waves, the down product's own before it
+// otherwise (with eight waves its registers would cost the projection its second workgroup a CU).
+static int launch_gemm_lora(const uint16_t* x, const uint16_t* W, int M, int N, int K, float* part, int* slices, const LoraArgs& a,
+                            hipStream_t s) {
+  if (gemm_is_tiled(M) || splitk_eight_waves(M, N, gemm_slices(K))) {
+    const int rc = launch_lora_down(x, M, K, a, s);
+    return rc ? rc : launch_gemm(x, W, M, N, K, part, slices, s);
+  }
+  *slices = gemm_slices(K);
+  const int wgs = std::min(device_cus() / 2, ceil_div(M, kDownRows) * std::min({kDownRows, M, a.n}) * lora_down_groups(a));
+  const int bxs = ceil_div(N, 64);
+  hipLaunchKernelGGL((gemm_splitk_bf16_kernel<4, true>), dim3(wgs + bxs * *slices), dim3(256), 0, s, x, W, M, N, K, part, a, wgs, bxs);
+  return check_launch("gemm_splitk_lora");
+}
+
+size_t lora_h_bytes(int M, int R, int n_seg) { return align256((size_t)M * n_seg * lora_cols(R) * 4) + align256((size_t)M * sizeof(int2)); }
+
+void lora_bind(LoraArgs* a, char* ws, int M) {
+  a->h = reinterpret_cast<uint16_t*>(ws);
+  a->meta = reinterpret_cast<int2*>(ws + align256((size_t)M * a->n_seg * lora_cols(a->R) * 4));
+}
+
+int launch_linear_lora(const uint16_t* x, const uint16_t* W, const uint16_t* b, int M, int N, int K, LoraArgs a, uint16_t* y,
+                       uint16_t* residual, char* ws, hipStream_t s) {
   float* part = reinterpret_cast<float*>(ws);
-  uint16_t* h = reinterpret_cast<uint16_t*>(ws + align256(partial_bytes(M, N, K)));
-  hipLaunchKernelGGL(lora_down_kernel, dim3(ceil_div(M, 16), a.n_seg * a.R / 16), dim3(64 * kDownWaves), 0, s, x, M, K, a, h);
-  int rc = check_launch("lora_down");
+  lora_bind(&a, ws + align256(partial_bytes(M, N, K)), M);
+  int slices = 0, rc;
+  if (gemm_tiled_lora_fits(M, K, a)) {
+    rc = launch_lora_down(x, M, K, a, s);
+    return rc ? rc : launch_gemm_tiled_lora(x, W, b, M, N, K, y, residual, a, s);
+  }
+  rc = launch_gemm_lora(x, W, M, N, K, part, &slices, a, s);
   if (rc) return rc;
-  int slices = 0;
-  rc = launch_gemm(x, W, M, N, K, part, &slices, s);
-  if (rc) return rc;
-  hipLaunchKernelGGL(lora_finalize_kernel, dim3(ceil_div(N, 64), ceil_div(M, 16)), dim3(256), 0, s, part, slices, M, N, a, h,
-                     b, y, residual);
+  hipLaunchKernelGGL(lora_finalize_kernel<false>, dim3(N / 16, ceil_div(M, 16)), dim3(256), 0, s, part, slices, M, N, a, b, y, residual,
+                     nullptr);
   return check_launch("lora_finalize");
 }
 
@@ -126,7 +191,7 @@ int make_lora_args(LoraArgs* out, const uint16_t* A, const uint16_t* B, const fl
   FLYAI_REQUIRE(((uintptr_t)A | (uintptr_t)B) % 16 == 0, "lora: A and B must be 16-byte aligned");
   FLYAI_REQUIRE(!row_seq || n_seqs >= 1, "lora: row_seq needs n_seqs >= 1");
   int64_t sum = 0;
-  LoraArgs a{A, B, scale, ranks, adapter, row_seq, n, R, n_seg, n_seqs, {0, 0, 0}};
+  LoraArgs a{A, B, scale, ranks, adapter, row_seq, n, R, n_seg, n_seqs, {0, 0, 0}, nullptr, nullptr};
   for (int i = 0; i < n_seg; ++i) {
     FLYAI_REQUIRE(segments[i] > 0 && segments[i] % 16 == 0, "lora: segment %d of %d features: a multiple of 16", i, segments[i]);
     sum += segments[i];
@@ -143,7 +208,7 @@ using namespace flyai;
 
 extern "C" size_t flyai_linear_lora_workspace_bytes(int32_t M, int32_t N, int32_t K, int32_t R, int32_t n_segments) {
   if (M <= 0 || N <= 0 || K <= 0 || R <= 0 || n_segments <= 0) return 0;
-  return align256(partial_bytes(M, N, K)) + (size_t)M * n_segments * R * 4;
+  return align256(partial_bytes(M, N, K)) + lora_h_bytes(M, R, n_segments);
 }
 
 extern "C" int flyai_linear_lora_bf16(const uint16_t* x, const uint16_t* w, const uint16_t* b, int32_t M, int32_t N,

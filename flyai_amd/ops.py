@@ -2,7 +2,10 @@
 
 PyTorch provides device memory and the stream; every computation happens in libflyai_stage.so.
 Each wrapper checks dtype / device / contiguity / shape on the host before the launch."""
+import array
 import ctypes as C
+import functools
+import struct
 
 import numpy as np
 import torch
@@ -317,10 +320,36 @@ def attn_ragged(q, k_pool, v_pool, kv_base, kv_cap, sinks, window, items, groups
 
 # ---- many requests at once: adapters, rotary positions, the cache's slabs ------------------------
 
-def _same_device(x, *others):
-    for name, t in others:
-        if t is not None and t.device != x.device:
-            raise ValueError(f"{name} is on {t.device}, not on {x.device}")
+def _need_all(device, *tensors):
+    """``_need`` of each (name, tensor, dtype, shape), and all on one device; the checks that pass cost little."""
+    for name, t, dtype, shape in tensors:
+        if not (isinstance(t, torch.Tensor) and t.dtype is dtype and t.shape == shape and t.is_contiguous()
+                and t.get_device() == device and device >= 0):
+            _need(t, dtype, shape, name)
+            raise ValueError(f"{name} is on {t.device}, the first tensor on another device")
+
+
+def _on(device, fn, *args):
+    """fn(*args, the current stream of the device) with the device current: a launch goes to the current device."""
+    if device == torch._C._cuda_getDevice():
+        check(fn(*args, torch._C._cuda_getCurrentRawStream(device)))
+    else:
+        with torch.cuda.device(device):
+            check(fn(*args, torch._C._cuda_getCurrentRawStream(device)))
+
+
+def _address(t):
+    return t.data_ptr() if t is not None else None
+
+
+@functools.lru_cache(maxsize=64)
+def _int32s(values):
+    return (C.c_int32 * len(values))(*values)
+
+
+@functools.lru_cache(maxsize=256)
+def _lora_workspace_bytes(M, N, K, R, S):
+    return max(16, int(lib().flyai_linear_lora_workspace_bytes(M, N, K, R, S)))
 
 
 def linear_lora(x, w, b, lora_a, lora_b, scale, ranks, adapter, segments=None, row_seq=None, residual=None):
@@ -332,36 +361,29 @@ def linear_lora(x, w, b, lora_a, lora_b, scale, ranks, adapter, segments=None, r
     [0, n) mean no adapter, and such a row has ``linear``'s bits.  A row's result depends on that row alone."""
     M, K = x.shape
     N = w.shape[0]
-    _need(x, torch.bfloat16, (M, K), "x")
-    _need(w, torch.bfloat16, (N, K), "weight")
-    if b is not None:
-        _need(b, torch.bfloat16, (N,), "bias")
     segments = (N,) if segments is None else tuple(int(v) for v in segments)
     S = len(segments)
     if lora_b.dim() != 3:
         raise ValueError("lora_b must be [adapters, N, R]")
     n, _, R = lora_b.shape
-    _need(lora_b, torch.bfloat16, (n, N, R), "lora_b")
-    _need(lora_a, torch.bfloat16, (n, S * R, K), "lora_a")
-    _need(scale, torch.float32, (n,), "scale")
-    _need(ranks, torch.int32, (n,), "ranks")
-    if row_seq is None:
-        _need(adapter, torch.int32, (M,), "adapter")
-    else:
-        _need(row_seq, torch.int32, (M,), "row_seq")
-        _need(adapter, torch.int32, (adapter.numel(),), "adapter")
+    dev, bf16, i32 = x.get_device(), torch.bfloat16, torch.int32
+    n_ids = adapter.numel()
+    _need_all(dev, ("x", x, bf16, (M, K)), ("weight", w, bf16, (N, K)), ("lora_b", lora_b, bf16, (n, N, R)),
+              ("lora_a", lora_a, bf16, (n, S * R, K)), ("scale", scale, torch.float32, (n,)), ("ranks", ranks, i32, (n,)),
+              ("adapter", adapter, i32, (M,) if row_seq is None else (n_ids,)))
+    if b is not None:
+        _need_all(dev, ("bias", b, bf16, (N,)))
+    if row_seq is not None:
+        _need_all(dev, ("row_seq", row_seq, i32, (M,)))
     y = None
     if residual is not None:
-        _need(residual, torch.bfloat16, (M, N), "residual")
+        _need_all(dev, ("residual", residual, bf16, (M, N)))
     else:
-        y = torch.empty(M, N, dtype=torch.bfloat16, device=x.device)
-    _same_device(x, ("weight", w), ("bias", b), ("lora_a", lora_a), ("lora_b", lora_b), ("scale", scale), ("ranks", ranks),
-                 ("adapter", adapter), ("row_seq", row_seq), ("residual", residual))
-    ws = torch.empty(max(16, int(lib().flyai_linear_lora_workspace_bytes(M, N, K, R, S))), dtype=torch.uint8, device=x.device)
-    with torch.cuda.device(x.device):
-        check(lib().flyai_linear_lora_bf16(_ptr(x), _ptr(w), _ptr(b), M, N, K, _ptr(lora_a), _ptr(lora_b), _ptr(scale),
-                                           _ptr(ranks), n, R, (C.c_int32 * S)(*segments), S, _ptr(adapter), _ptr(row_seq),
-                                           adapter.numel(), _ptr(y), _ptr(residual), _ptr(ws), _stream()))
+        y = torch.empty(M, N, dtype=bf16, device=x.device)
+    ws = torch.empty(_lora_workspace_bytes(M, N, K, R, S), dtype=torch.uint8, device=x.device)
+    _on(dev, lib().flyai_linear_lora_bf16, x.data_ptr(), w.data_ptr(), _address(b), M, N, K, lora_a.data_ptr(),
+        lora_b.data_ptr(), scale.data_ptr(), ranks.data_ptr(), n, R, _int32s(segments), S, adapter.data_ptr(),
+        _address(row_seq), n_ids, _address(y), _address(residual), ws.data_ptr())
     return residual if residual is not None else y
 
 
@@ -377,77 +399,92 @@ def rope(x, positions, inv_freq, layout="half", scaling=1.0, inverse=False, out=
     of x's shape and type (x itself: in place; otherwise it must not overlap x), None: a new contiguous one."""
     if not isinstance(x, torch.Tensor) or x.dim() != 3:
         raise ValueError("x must be a [T, H, D] tensor")
-    if x.device.type != "cuda":
+    dev = x.get_device()
+    if dev < 0:
         raise ValueError("x must be on the GPU")
-    if x.dtype not in _ROPE_TYPES:
+    dtype = _ROPE_TYPES.get(x.dtype)
+    if dtype is None:
         raise TypeError(f"x must be bf16, fp16 or fp32, got {x.dtype}")
     if layout not in _ROPE_LAYOUTS:
         raise ValueError(f"layout must be one of {sorted(_ROPE_LAYOUTS)}, got {layout!r}")
     T, H, D = x.shape
-    _need(positions, torch.int32, (T,), "positions")
-    _need(inv_freq, torch.float64, (inv_freq.numel(),), "inv_freq")
+    pairs = inv_freq.numel()
+    _need_all(dev, ("positions", positions, torch.int32, (T,)), ("inv_freq", inv_freq, torch.float64, (pairs,)))
     if out is None:
         out = torch.empty(T, H, D, dtype=x.dtype, device=x.device)
-    elif out.dtype != x.dtype or out.shape != x.shape:
-        raise ValueError(f"out must be {x.dtype} of shape {tuple(x.shape)}")
-    _same_device(x, ("positions", positions), ("inv_freq", inv_freq), ("out", out))
-    if D > 1 and (x.stride(2) != 1 or out.stride(2) != 1):
+    elif out.dtype != x.dtype or out.shape != x.shape or out.get_device() != dev:
+        raise ValueError(f"out must be {x.dtype} of shape {tuple(x.shape)} on {x.device}")
+    xt, xh, xd = x.stride()
+    ot, oh, od = out.stride()
+    if D > 1 and (xd != 1 or od != 1):
         raise ValueError("the last dim of x and out must be contiguous")
     if T == 0 or H == 0:
         return out
-    with torch.cuda.device(x.device):
-        check(lib().flyai_rope(_ptr(x), x.stride(0), x.stride(1), _ptr(positions), _ptr(inv_freq), float(scaling), T, H, D,
-                               2 * inv_freq.numel(), _ROPE_TYPES[x.dtype], _ROPE_LAYOUTS[layout], int(bool(inverse)),
-                               _ptr(out), out.stride(0), out.stride(1), _stream()))
+    _on(dev, lib().flyai_rope, x.data_ptr(), xt, xh, positions.data_ptr(), inv_freq.data_ptr(), scaling, T, H, D, 2 * pairs,
+        dtype, _ROPE_LAYOUTS[layout], 1 if inverse else 0, out.data_ptr(), ot, oh)
     return out
 
 
 def _kv_pools(k, v):
-    """(layers, elements a layer, layer stride) of K and V pools [L, n] (or one layer's [n])."""
-    if not isinstance(k, torch.Tensor) or not isinstance(v, torch.Tensor) or k.dim() not in (1, 2) or k.shape != v.shape:
+    """(layers, elements a layer, device) of K and V pools [L, n] (or one layer's [n])."""
+    if not isinstance(k, torch.Tensor) or k.dim() not in (1, 2):
         raise ValueError("k and v must be pools of one shape, [layers, elements] or [elements]")
-    _need(k, torch.bfloat16, None, "k")
-    _need(v, torch.bfloat16, None, "v")
-    _same_device(k, ("v", v))
-    n = k.shape[-1]
-    return (k.shape[0] if k.dim() == 2 else 1), n, n
+    dev = k.get_device()
+    _need_all(dev, ("k", k, torch.bfloat16, k.shape), ("v", v, torch.bfloat16, k.shape))
+    return (k.shape[0] if k.dim() == 2 else 1), k.shape[-1], dev
+
+
+_KV_SLAB, _KV_MOVE = struct.Struct("qii"), struct.Struct("qiiii")  # flyai_kv_slab, flyai_kv_move
+KV_COMPACT_ANY_ORDER = 704  # rows of one slab that kv_compact moves in any order (one launch holds them)
 
 
 def kv_fork(k, v, n_kv_heads, src, dsts, lo, hi, src_k=None, src_v=None):
     """Copy positions [lo, hi) of slab src to the same positions of the slabs dsts, every layer, in one launch.  k, v: pools
     bf16 [L, elements] in the tiled slab layout; a slab is (base, cap).  src_k, src_v: the pools that hold src, when
     they are others.  Nothing outside [lo, hi) changes.  Positions past a slab raise ContextOverflow."""
-    src_k, src_v = (k, v) if src_k is None else (src_k, src_v)
-    L, n, stride = _kv_pools(k, v)
-    sL, sn, sstride = _kv_pools(src_k, src_v)
-    if sL != L:
-        raise ValueError(f"pools of {sL} and of {L} layers")
-    _same_device(k, ("src_k", src_k))
-    one = _lib.KvSlab(int(src[0]), int(src[1]), 0)
-    many = (_lib.KvSlab * max(1, len(dsts)))(*[_lib.KvSlab(int(b), int(c), 0) for b, c in dsts])
-    with torch.cuda.device(k.device):
-        check(lib().flyai_kv_fork(_ptr(src_k), _ptr(src_v), sstride, sn, _ptr(k), _ptr(v), stride, n, L, int(n_kv_heads), 64,
-                                  C.byref(one), many, len(dsts), int(lo), int(hi), _stream()))
+    L, n, dev = _kv_pools(k, v)
+    sn = n
+    if src_k is None:
+        src_k, src_v = k, v
+    else:
+        sL, sn, sdev = _kv_pools(src_k, src_v)
+        if sL != L or sdev != dev:
+            raise ValueError(f"the source's pools have {sL} layers on device {sdev}, the others {L} on {dev}")
+    slabs = _packed(_KV_SLAB, [(b, c, 0) for b, c in (src, *dsts)])
+    _on(dev, lib().flyai_kv_fork, src_k.data_ptr(), src_v.data_ptr(), sn, sn, k.data_ptr(), v.data_ptr(), n, n, L, n_kv_heads,
+        64, slabs[:_KV_SLAB.size], slabs[_KV_SLAB.size:], len(dsts), lo, hi)
 
 
-KV_COMPACT_ANY_ORDER = 704  # rows of one slab that kv_compact moves in any order (one launch holds them)
+def _host_positions(keep):
+    """The int32s of a list, an array or a CPU tensor of positions, as bytes."""
+    try:
+        if isinstance(keep, (list, tuple, range)):
+            if len(keep) == 0 or min(keep) >= 0:
+                return array.array("i", keep).tobytes()
+        else:
+            a = np.asarray(keep).reshape(-1)
+            if a.size == 0 or (a.dtype.kind in "iu" and a.min() >= 0 and a.max() <= 0x7fffffff):
+                return a.astype(np.int32).tobytes()
+    except (TypeError, OverflowError):
+        pass
+    raise ValueError("keep must hold positions (non-negative integers)")
+
+
+def _packed(layout, rows):
+    try:
+        return b"".join([layout.pack(*r) for r in rows])
+    except struct.error:
+        raise ValueError("slabs and starts must be integers in range") from None
 
 
 def kv_compact(k, v, n_kv_heads, moves):
     """For each move (base, cap, start, keep): position start + i of the slab takes what position start + keep[i] held
     before the call, every layer, in one launch (more beyond 704 moved rows).  keep: host integers (list, numpy or CPU
     tensor), in any order up to 704, strictly ascending beyond.  The moves' slabs must not overlap."""
-    L, n, stride = _kv_pools(k, v)
-    keeps = [np.asarray(m[3]).reshape(-1) for m in moves]
-    for a in keeps:
-        if a.size and (a.dtype.kind not in "iu" or a.min() < 0 or a.max() > 0x7fffffff):
-            raise ValueError("keep must hold positions (non-negative integers)")
-    flat = np.concatenate([a.astype(np.int32) for a in keeps]) if keeps else np.zeros(0, np.int32)
-    rows = (_lib.KvMove * max(1, len(moves)))(*[_lib.KvMove(int(m[0]), int(m[1]), int(m[2]), a.size, 0)
-                                               for m, a in zip(moves, keeps)])
-    with torch.cuda.device(k.device):
-        check(lib().flyai_kv_compact(_ptr(k), _ptr(v), stride, n, L, int(n_kv_heads), 64, rows, len(moves),
-                                     flat.ctypes.data_as(C.c_void_p), _stream()))
+    L, n, dev = _kv_pools(k, v)
+    keeps = [_host_positions(m[3]) for m in moves]
+    rows = _packed(_KV_MOVE, [(base, cap, start, len(a) // 4, 0) for (base, cap, start, _), a in zip(moves, keeps)])
+    _on(dev, lib().flyai_kv_compact, k.data_ptr(), v.data_ptr(), n, n, L, n_kv_heads, 64, rows, len(moves), b"".join(keeps))
 
 
 # ---- DeepSeek-V3-shaped FP8 MoE ------------------------------------------------------------------

@@ -68,83 +68,113 @@ __global__ __launch_bounds__(kForkThreads) void kv_fork_kernel(ForkArgs a) {
   }
 }
 
-// ---- compact: within a slab, position start + i takes position start + keep[i] --------------------------------
-// A slab's dims are independent of each other: a workgroup owns 16 dims of one head of one layer's K or V, reads all
-// of its rows into registers and only then writes, so it needs nothing from any other workgroup.  A launch takes up to
-// kMoveRows rows; with keep ascending, a later launch's sources lie past every earlier one's destinations.
-constexpr int kMoveRows = 704;
-constexpr int kMoveSlabs = 24;
-constexpr int kMoveThreads = 256;
+// ---- compact: within a slab, the kept positions move up, in order ------------------------------------------------
+// A kept position never moves down, so a part of the positions, read whole before it is written, overwrites nothing that
+// a later part reads.  A slab's dims do not depend on each other: a workgroup owns 16 dims of one head of one layer's K or
+// V and goes through the positions in parts of 512, through LDS, needing nothing from other workgroups.  What stays is a
+// bitmap, a word per 64-position block.
+// Four slabs of 2,041 moved rows in 8 layers, 267 MB: 198 us with the positions themselves in the arguments (704 a launch,
+// 12 launches), 106 with parts of 1,024 in registers (whose unrolled code, 20 KB, cost a launch of 6 rows 18 us), now 58, a
+// large copy's rate; parts of 256 take 62, of 1,024 62, four waves instead of eight 72.
+constexpr int kMoveThreads = 512;
+constexpr int kMoveBlocks = 8;    // 64-position blocks of a part
+constexpr int kMoveRow = 64 * kMoveBlocks + 8;  // a dim's positions in LDS, + 16 B vs bank conflicts
+constexpr int kMoveWords = 416;   // words of a launch: 26,624 positions
+constexpr int kMoveSlabs = 16;
 
 struct MoveSlab {
   int64_t base;
-  int cap, start, first, n;  // rows start .. start + n - 1 take start0 + keep[first ..]
-  int from;                  // what keep counts from
+  int cap, dst;             // the first kept position goes to dst
+  int block, first, words;  // words[first ..] are blocks block .. block + words - 1
+  int pad;
 };
 
 struct MoveArgs {
   uint16_t* pool[2];
   int64_t layer;
-  int heads, n_slabs;
   MoveSlab slab[kMoveSlabs];
-  int keep[kMoveRows];
+  uint64_t words[kMoveWords];
 };
 static_assert(sizeof(MoveArgs) <= 4096 && sizeof(ForkArgs) <= 4096, "kernel arguments are at most 4 KiB");
 
 __global__ __launch_bounds__(kMoveThreads) void kv_compact_kernel(MoveArgs a) {
-  const int kind = blockIdx.x & 1, dq = (blockIdx.x >> 1) & 3, head = blockIdx.x >> 3, layer = blockIdx.z;
+  __shared__ uint16_t kept[64 * kMoveBlocks];  // of the part: offsets from its first position
+  __shared__ __align__(16) uint16_t data[16 * kMoveRow];
+  const int kind = blockIdx.x & 1, dq = (blockIdx.x >> 1) & 3, head = blockIdx.x >> 3;
   const MoveSlab& m = a.slab[blockIdx.y];
-  uint16_t* region = a.pool[kind] + layer * a.layer + m.base + (int64_t)head * m.cap * 64;
-  const int* keep = a.keep + m.first;
-  const int n = m.n;
-  if (kind == 0) {
-    // K: 16 dims of a row are two 16-byte chunks
-    constexpr int kPer = (2 * kMoveRows + kMoveThreads - 1) / kMoveThreads;
-    u32x4_t v[kPer];
+  uint16_t* region = a.pool[kind] + blockIdx.z * a.layer + m.base + (int64_t)head * m.cap * 64;
+  const int tid = threadIdx.x;
+  int dst = m.dst;
+  for (int b0 = 0; b0 < m.words; b0 += kMoveBlocks) {
+    const int p0 = 64 * (m.block + b0);
+    uint64_t words[kMoveBlocks];
+    int n = 0;
 #pragma unroll
-    for (int j = 0; j < kPer; ++j) {
-      const int u = threadIdx.x + kMoveThreads * j;
-      if (u < 2 * n) v[j] = *reinterpret_cast<const u32x4_t*>(region + kv_k_off(m.from + keep[u >> 1], 16 * dq + 8 * (u & 1)));
+    for (int i = 0; i < kMoveBlocks; ++i) {
+      words[i] = b0 + i < m.words ? a.words[min(m.first + b0 + i, kMoveWords - 1)] : 0;
+      n += __builtin_popcountll(words[i]);
     }
-    __syncthreads();
+    if (n == 0) continue;
+    {
+      constexpr int kPer = 64 * kMoveBlocks / kMoveThreads;  // positions a thread
+      const int blk = kPer * tid / 64, bit = kPer * tid % 64;
+      uint64_t word = 0;
+      int at = 0;
 #pragma unroll
-    for (int j = 0; j < kPer; ++j) {
-      const int u = threadIdx.x + kMoveThreads * j;
-      if (u < 2 * n) *reinterpret_cast<u32x4_t*>(region + kv_k_off(m.start + (u >> 1), 16 * dq + 8 * (u & 1))) = v[j];
-    }
-  } else {
-    // V: a destination chunk is one dim of eight positions; its elements come from eight places
-    constexpr int kPer = (16 * (kMoveRows / 8 + 1) + kMoveThreads - 1) / kMoveThreads;
-    const int g0 = m.start >> 3, units = 16 * (((m.start + n - 1) >> 3) - g0 + 1);
-    uint16_t v[kPer][8];
-#pragma unroll
-    for (int j = 0; j < kPer; ++j) {
-      const int u = threadIdx.x + kMoveThreads * j;
-      if (u < units) {
-        const int d = 16 * dq + (u & 15), i0 = 8 * (g0 + (u >> 4)) - m.start;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[j][i] = region[kv_v_off(m.from + keep[min(max(i0 + i, 0), n - 1)], d)];
+      for (int i = 0; i < kMoveBlocks; ++i) {
+        if (i < blk) at += __builtin_popcountll(words[i]);
+        if (i == blk) word = words[i];
       }
-    }
-    __syncthreads();
+      at += __builtin_popcountll(word & ((1ull << bit) - 1));
 #pragma unroll
-    for (int j = 0; j < kPer; ++j) {
-      const int u = threadIdx.x + kMoveThreads * j;
-      if (u < units) {
-        const int d = 16 * dq + (u & 15), p0 = 8 * (g0 + (u >> 4)), i0 = p0 - m.start;
-        uint16_t* to = region + kv_v_off(p0, d);
-        if (i0 >= 0 && i0 + 8 <= n) {
+      for (int i = 0; i < kPer; ++i)
+        if (word >> (bit + i) & 1) kept[at++] = (uint16_t)(64 * blk + bit + i);
+    }
+    if (kind == 0) {
+      // K: 16 dims of a row are two 16-byte chunks
+      __syncthreads();
+#pragma unroll 4
+      for (int u = tid; u < 2 * n; u += kMoveThreads)
+        reinterpret_cast<u32x4_t*>(data)[u] =
+            *reinterpret_cast<const u32x4_t*>(region + kv_k_off(p0 + kept[u >> 1], 16 * dq + 8 * (u & 1)));
+      __syncthreads();
+      for (int u = tid; u < 2 * n; u += kMoveThreads)
+        *reinterpret_cast<u32x4_t*>(region + kv_k_off(dst + (u >> 1), 16 * dq + 8 * (u & 1))) = reinterpret_cast<u32x4_t*>(data)[u];
+    } else {
+      // V: a chunk is one dim of eight positions; those with none kept are not read.  A destination chunk's elements come
+      // from wherever each lies.
+#pragma unroll
+      for (int j = 0; j < 16 * 8 * kMoveBlocks / kMoveThreads; ++j) {
+        const int u = tid + kMoveThreads * j, d = u & 15, g = u >> 4;  // chunk: dim, eighth positions
+        uint64_t word = 0;
+#pragma unroll
+        for (int i = 0; i < 2; ++i)  // 16 chunk groups, two blocks, an iteration
+          if (g >> 3 == 2 * j + i) word = words[2 * j + i];
+        if (word >> (8 * (g & 7)) & 255)
+          *reinterpret_cast<u32x4_t*>(data + d * kMoveRow + 8 * g) = *reinterpret_cast<const u32x4_t*>(region + kv_v_off(p0 + 8 * g, 16 * dq + d));
+      }
+      __syncthreads();
+      const int g0 = dst >> 3, units = 16 * (((dst + n - 1) >> 3) - g0 + 1);
+      for (int u = tid; u < units; u += kMoveThreads) {
+        const int d = u & 15, at = 8 * (g0 + (u >> 4)), i0 = at - dst;
+        uint16_t e[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) e[i] = data[d * kMoveRow + kept[min(max(i0 + i, 0), n - 1)]];
+        uint16_t* to = region + kv_v_off(at, 16 * dq + d);
+        if (i0 >= 0 && i0 + 7 < n) {
           u32x4_t w;
 #pragma unroll
-          for (int i = 0; i < 4; ++i) w[i] = v[j][2 * i] | (uint32_t)v[j][2 * i + 1] << 16;
+          for (int i = 0; i < 4; ++i) w[i] = e[2 * i] | (uint32_t)e[2 * i + 1] << 16;
           *reinterpret_cast<u32x4_t*>(to) = w;
         } else {
 #pragma unroll
           for (int i = 0; i < 8; ++i)
-            if (i0 + i >= 0 && i0 + i < n) to[i] = v[j][i];
+            if (i0 + i >= 0 && i0 + i < n) to[i] = e[i];
         }
       }
     }
+    __syncthreads();  // the part's LDS is free again
+    dst += n;
   }
 }
 
@@ -228,11 +258,10 @@ extern "C" int flyai_kv_compact(uint16_t* k_pool, uint16_t* v_pool, int64_t laye
       return set_error(FLYAI_ERANGE, "kv_compact: move %d ends past its slab's %d positions", i, m.cap);
     const int32_t* keep = keep_host + first;
     for (int r = 0; r < m.n; ++r) {
-      FLYAI_REQUIRE(keep[r] >= 0, "kv_compact: move %d keeps position %d", i, keep[r]);
+      FLYAI_REQUIRE(keep[r] >= 0 && (r == 0 || keep[r] > keep[r - 1]),
+                    "kv_compact: move %d must keep positions in strictly ascending order (entry %d)", i, r);
       if ((int64_t)m.start + keep[r] >= m.cap)
         return set_error(FLYAI_ERANGE, "kv_compact: move %d keeps position %d + %d of a slab of %d", i, m.start, keep[r], m.cap);
-      FLYAI_REQUIRE(m.n <= kMoveRows || r == 0 || keep[r] > keep[r - 1],
-                    "kv_compact: move %d of more than %d rows must keep them in ascending order", i, kMoveRows);
     }
     for (int j = 0; j < i; ++j) {
       const flyai_kv_move& o = moves_host[j];
@@ -243,12 +272,12 @@ extern "C" int flyai_kv_compact(uint16_t* k_pool, uint16_t* v_pool, int64_t laye
   }
   hipStream_t s = as_stream(stream);
   MoveArgs a;
-  a.pool[0] = k_pool, a.pool[1] = v_pool, a.layer = layer, a.heads = Hkv, a.n_slabs = 0;
-  int rows = 0;
+  a.pool[0] = k_pool, a.pool[1] = v_pool, a.layer = layer;
+  int slabs = 0, words = 0;
   auto flush = [&]() {
-    if (a.n_slabs == 0) return FLYAI_OK;
-    hipLaunchKernelGGL(kv_compact_kernel, dim3(8 * Hkv, a.n_slabs, n_layers), dim3(kMoveThreads), 0, s, a);
-    a.n_slabs = rows = 0;
+    if (slabs == 0) return FLYAI_OK;
+    hipLaunchKernelGGL(kv_compact_kernel, dim3(8 * Hkv, slabs, n_layers), dim3(kMoveThreads), 0, s, a);
+    slabs = words = 0;
     return check_launch("kv_compact");
   };
   first = 0;
@@ -257,17 +286,19 @@ extern "C" int flyai_kv_compact(uint16_t* k_pool, uint16_t* v_pool, int64_t laye
     const int32_t* keep = keep_host + first;
     first += m.n;
     int r = 0;
-    while (r < m.n && keep[r] == r) ++r;  // rows that stay where they are
-    const bool whole = m.n - r <= kMoveRows;
+    while (r < m.n && keep[r] == r) ++r;  // positions that stay where they are
     while (r < m.n) {
-      // a move of up to kMoveRows rows in any order goes into one launch whole; a longer one in pieces
-      if (a.n_slabs == kMoveSlabs || rows == kMoveRows || (whole && rows + (m.n - r) > kMoveRows)) RUN(flush());
-      const int n = std::min(m.n - r, kMoveRows - rows);
-      a.slab[a.n_slabs++] = MoveSlab{m.base, m.cap, m.start + r, rows, n, m.start};
-      std::copy(keep + r, keep + r + n, a.keep + rows);
-      rows += n;
-      r += n;
-      if (r < m.n) RUN(flush());  // the next piece reads what this one must not have passed yet
+      // a slab's kept positions go into one launch as far as its words last; the next launch takes up from there
+      if (slabs == kMoveSlabs || words == kMoveWords) RUN(flush());
+      MoveSlab& out = a.slab[slabs++];
+      out = MoveSlab{m.base, m.cap, m.start + r, (m.start + keep[r]) >> 6, words, 0, 0};
+      for (; r < m.n; ++r) {
+        const int pos = m.start + keep[r], w = (pos >> 6) - out.block;
+        if (out.first + w >= kMoveWords) break;
+        for (; out.words <= w; ++out.words) a.words[words++] = 0;
+        a.words[out.first + w] |= 1ull << (pos & 63);
+      }
+      if (r < m.n) RUN(flush());  // the rest moves into positions that this piece reads
     }
   }
   return flush();

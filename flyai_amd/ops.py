@@ -2,7 +2,6 @@
 
 PyTorch provides device memory and the stream; every computation happens in libflyai_stage.so.
 Each wrapper checks dtype / device / contiguity / shape on the host before the launch."""
-import array
 import ctypes as C
 import functools
 import struct
@@ -435,7 +434,6 @@ def _kv_pools(k, v):
 
 
 _KV_SLAB, _KV_MOVE = struct.Struct("qii"), struct.Struct("qiiii")  # flyai_kv_slab, flyai_kv_move
-KV_COMPACT_ANY_ORDER = 704  # rows of one slab that kv_compact moves in any order (one launch holds them)
 
 
 def kv_fork(k, v, n_kv_heads, src, dsts, lo, hi, src_k=None, src_v=None):
@@ -459,13 +457,13 @@ def _host_positions(keep):
     """The int32s of a list, an array or a CPU tensor of positions, as bytes."""
     try:
         if isinstance(keep, (list, tuple, range)):
-            if len(keep) == 0 or min(keep) >= 0:
-                return array.array("i", keep).tobytes()
+            if not keep or keep[0] >= 0:  # ascending from there: the C call checks
+                return struct.pack(f"{len(keep)}i", *keep)
         else:
             a = np.asarray(keep).reshape(-1)
             if a.size == 0 or (a.dtype.kind in "iu" and a.min() >= 0 and a.max() <= 0x7fffffff):
                 return a.astype(np.int32).tobytes()
-    except (TypeError, OverflowError):
+    except (TypeError, struct.error):
         pass
     raise ValueError("keep must hold positions (non-negative integers)")
 
@@ -479,8 +477,8 @@ def _packed(layout, rows):
 
 def kv_compact(k, v, n_kv_heads, moves):
     """For each move (base, cap, start, keep): position start + i of the slab takes what position start + keep[i] held
-    before the call, every layer, in one launch (more beyond 704 moved rows).  keep: host integers (list, numpy or CPU
-    tensor), in any order up to 704, strictly ascending beyond.  The moves' slabs must not overlap."""
+    before the call, every layer, in one launch (or one per 26,624 positions).  keep: host integers (list, numpy or CPU
+    tensor), strictly ascending.  The moves' slabs must not overlap."""
     L, n, dev = _kv_pools(k, v)
     keeps = [_host_positions(m[3]) for m in moves]
     rows = _packed(_KV_MOVE, [(base, cap, start, len(a) // 4, 0) for (base, cap, start, _), a in zip(moves, keeps)])

@@ -353,9 +353,10 @@ class FastVerifyStage:
         """Compact the accepted path's KV (scratch slots start+keep[i]) to start+i, every layer
         (fastverify.py:301-309)."""
         keep = [int(k) for k in keep]
-        if len(keep) <= ops.KV_COMPACT_ANY_ORDER or all(a < b for a, b in zip(keep, keep[1:])):
+        if all(a < b for a, b in zip(keep, keep[1:])):
             self.cache.compact([0], [start], [keep])
             return
+        # a tree whose parents come after their children
         src = torch.tensor([start + k for k in keep], device=self.dev)
         dst = torch.arange(start, start + len(keep), device=self.dev)
         for l in range(self.n_layers):

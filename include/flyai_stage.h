@@ -350,8 +350,8 @@ int flyai_rope(const void* x, int64_t x_token, int64_t x_head, const int32_t* po
  * fork: positions [lo, hi) of the source slab to the same positions of n_dst other slabs; nothing else of
  * them changes.  Slabs of one pool must not overlap.
  * compact: for each move, slab position start + i takes what position start + keep[i] held before the call
- * (keep_host holds the moves' entries one after the other).  keep may be in any order and name a position twice up to
- * 704 entries a move, and is strictly ascending beyond.  The moves' slabs must not overlap.
+ * (keep_host holds the moves' entries one after the other, each move's strictly ascending).  The moves' slabs must
+ * not overlap.
  * Positions past a slab -> FLYAI_ERANGE, before any launch. */
 typedef struct {
   int64_t base;  /* element offset of the slab in a layer's pool (base % 8 == 0) */

@@ -76,8 +76,8 @@ def _keep_cases():
         "by_one": (0, list(range(1, 300))), "by_64": (0, list(range(64, 300))), "by_8": (40, list(range(8, 200))),
         "ends": (0, list(range(4)) + list(range(250, 1000))), "sparse": (3, sorted(rng.choice(1000, 333, replace=False).tolist())),
         "long": (0, sorted(rng.choice(1020, 900, replace=False).tolist())), "full_704": (5, list(range(300, 1004))),
-        "705": (5, list(range(300, 1005))), "any_order": (17, rng.permutation(600).tolist()),
-        "twice": (17, [5, 5, 5, 0, 9, 9, 1]), "back": (10, [0, 0, 1, 2, 3, 4, 5, 6, 7]),
+        "by_5_all": (5, list(range(5, 1019))), "alternate": (1, list(range(0, 1020, 2))), "last": (1023, [0]),
+        "runs": (9, [i for i in range(1000) if i % 20 < 11]),
     }
 
 
@@ -91,6 +91,22 @@ def test_compact(name):
     wk = _moved(k, "k", heads, src, dst, (base, cap), (base, cap))
     wv = _moved(v, "v", heads, src, dst, (base, cap), (base, cap))
     ops.kv_compact(k, v, heads, [(base, cap, start, keep)])
+    assert torch.equal(_bits(k), _bits(wk)) and torch.equal(_bits(v), _bits(wv))
+
+
+def test_compact_past_one_launch():
+    """More positions than one launch's words: pieces of a long slab, beside a short one."""
+    heads, cap = 1, 60032
+    rng = np.random.RandomState(5)
+    k, v = _pools(1, heads * (cap + 128) * 64, 5)
+    keep = np.sort(rng.choice(60000, 41000, replace=False))
+    slabs = [(0, 128), (128 * heads * 64, cap)]
+    moves = [(*slabs[0], 1, [2, 70, 100]), (*slabs[1], 30, keep)]
+    wk, wv = k, v
+    for (b, c, start, kp) in moves:
+        src, dst = start + np.asarray(kp), start + np.arange(len(kp))
+        wk, wv = (_moved(wk, "k", heads, src, dst, (b, c), (b, c)), _moved(wv, "v", heads, src, dst, (b, c), (b, c)))
+    ops.kv_compact(k, v, heads, moves)
     assert torch.equal(_bits(k), _bits(wk)) and torch.equal(_bits(v), _bits(wv))
 
 
@@ -168,6 +184,9 @@ def test_refusals_leave_the_pools_alone():
         ops.kv_compact(k, v, heads, [(0, cap, 0, [-1])])
     with pytest.raises(ValueError):
         ops.kv_compact(k, v, heads, [(0, cap, 0, [0.5])])
+    for keep in ([3, 2], [2, 2]):
+        with pytest.raises(FlyaiError, match="ascending"):
+            ops.kv_compact(k, v, heads, [(0, cap, 0, keep)])
     with pytest.raises(ValueError):
         ops.kv_fork(k, v[:1], heads, (0, cap), [(slab, cap)], 0, 10)
     with pytest.raises(TypeError):

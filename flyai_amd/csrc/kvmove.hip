@@ -71,13 +71,14 @@ __global__ __launch_bounds__(kForkThreads) void kv_fork_kernel(ForkArgs a) {
 // ---- compact: within a slab, the kept positions move up, in order ------------------------------------------------
 // A kept position never moves down, so a part of the positions, read whole before it is written, overwrites nothing that
 // a later part reads.  A slab's dims do not depend on each other: a workgroup owns 16 dims of one head of one layer's K or
-// V and goes through the positions in parts of 512, through LDS, needing nothing from other workgroups.  What stays is a
+// V and goes through the positions in parts of 256, through LDS, needing nothing from other workgroups.  What stays is a
 // bitmap, a word per 64-position block.
 // Four slabs of 2,041 moved rows in 8 layers, 267 MB: 198 us with the positions themselves in the arguments (704 a launch,
-// 12 launches), 106 with parts of 1,024 in registers (whose unrolled code, 20 KB, cost a launch of 6 rows 18 us), now 58, a
-// large copy's rate; parts of 256 take 62, of 1,024 62, four waves instead of eight 72.
-constexpr int kMoveThreads = 512;
-constexpr int kMoveBlocks = 8;    // 64-position blocks of a part
+// 12 launches), 106 with parts of 1,024 in registers (whose unrolled code, 20 KB, cost a launch of 6 rows 18 us), now 62,
+// 4.3 TB/s; parts of 128, 512 and 1,024 take 67, 68 and 71.  1,501 scattered rows of 6,000 (two slabs, 12 layers): 98 us, 82
+// and 67, most of it for lines that few kept positions share.
+constexpr int kMoveThreads = 256;
+constexpr int kMoveBlocks = 4;    // 64-position blocks of a part
 constexpr int kMoveRow = 64 * kMoveBlocks + 8;  // a dim's positions in LDS, + 16 B vs bank conflicts
 constexpr int kMoveWords = 416;   // words of a launch: 26,624 positions
 constexpr int kMoveSlabs = 16;
@@ -143,13 +144,15 @@ __global__ __launch_bounds__(kMoveThreads) void kv_compact_kernel(MoveArgs a) {
     } else {
       // V: a chunk is one dim of eight positions; those with none kept are not read.  A destination chunk's elements come
       // from wherever each lies.
+      constexpr int kBlocks = kMoveThreads / 16 / 8;  // that an iteration reads
+      static_assert(kMoveBlocks % kBlocks == 0 && kMoveThreads % 128 == 0, "whole iterations of whole blocks");
 #pragma unroll
       for (int j = 0; j < 16 * 8 * kMoveBlocks / kMoveThreads; ++j) {
         const int u = tid + kMoveThreads * j, d = u & 15, g = u >> 4;  // chunk: dim, eighth positions
         uint64_t word = 0;
 #pragma unroll
-        for (int i = 0; i < 2; ++i)  // 16 chunk groups, two blocks, an iteration
-          if (g >> 3 == 2 * j + i) word = words[2 * j + i];
+        for (int i = 0; i < kBlocks; ++i)
+          if (g >> 3 == kBlocks * j + i) word = words[kBlocks * j + i];
         if (word >> (8 * (g & 7)) & 255)
           *reinterpret_cast<u32x4_t*>(data + d * kMoveRow + 8 * g) = *reinterpret_cast<const u32x4_t*>(region + kv_v_off(p0 + 8 * g, 16 * dq + d));
       }

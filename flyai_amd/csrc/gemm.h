@@ -36,7 +36,7 @@ constexpr int kTiledMinRows = 256;  // batches of at least this many rows take t
 // LORA: the adapters' down product is in the launch, in its first `wgs` workgroups, beside the stream of the weights; the
 // grid has one axis then.
 template <int WAVES, bool LORA>
-__global__ __launch_bounds__(64 * WAVES) void gemm_splitk_bf16_kernel(
+__global__ __launch_bounds__(64 * WAVES, LORA ? 2 : 1) void gemm_splitk_bf16_kernel(
     const uint16_t* __restrict__ x, const uint16_t* __restrict__ W, int M, int N, int K,
     float* __restrict__ part, LoraArgs lo, int wgs, int bxs) {
   typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));

@@ -489,10 +489,14 @@ __global__ __launch_bounds__(64 * kTiledWaves) void gemm_tiled_lds_kernel(const 
 #pragma unroll
     for (int b = 0; b < 4; ++b) bv[b] = ep.bias ? bf2f(ep.bias[fb + 16 * b + r]) : 0.f;
   }
-  int2 who[2];  // adapter and rank of row 16 (2 wm + a) + r, fetched under the GEMM
+  // LORA: what the up products need is fetched under the GEMM too: each row's adapter before the prologue, h and the B
+  // columns of one adapter, the middle row's (a prompt's rows share theirs), behind it.
+  __shared__ __align__(1024) char held_b[LORA && !QKV ? kTileN * 128 : 16];
+  int2 who = make_int2(-1, 0), held = make_int2(-1, 0);  // of row 32 wm + lane, of the middle row
+  u32x4_t hv[8];
   if constexpr (LORA) {
-#pragma unroll
-    for (int a = 0; a < 2; ++a) who[a] = lo.meta[min(m0 + 16 * (2 * wm + a) + r, M - 1)];
+    held = lo.meta[min(m0 + kTileM / 2, M - 1)];
+    who = lo.meta[min(m0 + 32 * wm + (lane & 31), M - 1)];
   }
   if constexpr (EPI == kEpiLinear) {
 #pragma unroll
@@ -520,6 +524,18 @@ __global__ __launch_bounds__(64 * kTiledWaves) void gemm_tiled_lds_kernel(const 
     __builtin_amdgcn_global_load_lds((const void*)(ep.sin_tab + roff), (lds_ptr)(rot_s + 16 * wave * 32), 16, 0, 0);
     e_cap = ep.kv_cap[e_sq];
     e_base = ep.kv_base[e_sq];
+    asm volatile("" ::: "memory");
+  }
+  if constexpr (LORA) {
+    held.x = !QKV && __builtin_amdgcn_readfirstlane(held.y) > 0 ? __builtin_amdgcn_readfirstlane(held.x) : -1;
+    if (held.x >= 0) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+        __builtin_amdgcn_global_load_lds((const void*)(lo.B + ((size_t)held.x * N + min(n0 + 16 * wave + 8 * i + (lane >> 3), N - 1)) * lo.R +
+                                                       lora_chunk(8 * i, 0, lo.R)),
+                                         (lds_ptr)(held_b + 2048 * wave + 1024 * i), 16, 0, 0);
+    }
+    lora_fetch_h(lo, M, m0 + 32 * wm, min(n0 + 64 * wn, N - 1), hv);
     asm volatile("" ::: "memory");
   }
   read_ab(a0, b0, sa0, sb0, 0);
@@ -550,18 +566,24 @@ __global__ __launch_bounds__(64 * kTiledWaves) void gemm_tiled_lds_kernel(const 
     fold();
   }
   __builtin_amdgcn_s_waitcnt(waitcnt_vm(0));  // the loads issued past the end have landed
+  // after the GEMM each wave has 16 KiB of the stages to itself: its h, then another adapter's columns or its results
+  char* own = nullptr;
+  if constexpr (LORA || EPI == kEpiLinear) {
+    lds_barrier();  // every wave is done with the stages; every wave's part of the held columns has landed
+    own = wave < 4 ? (wave < 2 ? wave ? sb0 : sa0 : wave & 1 ? sb1 : sa1) : (wave < 6 ? wave & 1 ? sb2 : sa2 : wave & 1 ? sb3 : sa3);
+  }
   if constexpr (LORA) {
-    if (n0 + 64 * wn < N) {
 #pragma unroll
-      for (int a = 0; a < 2; ++a) lora_up_rows(lo, M, N, m0 + 16 * (2 * wm + a), n0 + 64 * wn, who[a], tot[a]);
-    }
+    for (int k = 0; k < 8; ++k) *reinterpret_cast<u32x4_t*>(own + 1024 * k + 16 * lane) = hv[k];
+    if (n0 + 64 * wn < N)
+      lora_up_block(lo, M, N, m0 + 32 * wm, n0 + 64 * wn, who, own, held.x, held_b + (QKV ? 0 : 8192 * wn), own + 8192, tot);
   }
   // lane (r, g) holds rows 16(2wm + a) + 4g + v of feature 16(4wn + b) + r
   if constexpr (EPI == kEpiLinear) {
-    // Each wave turns its 32 x 64 block round in its own 4 KiB of the first stage, so that a row's 128 bytes go out
-    // together: 16-byte chunk c of row q sits at position c ^ (q / 4) % 8.
-    lds_barrier();  // every wave is done with the stages
-    char* blk = wave < 4 ? sa0 + 4096 * wave : sb0 + 4096 * (wave - 4);
+    // Each wave turns its 32 x 64 block round in LDS, so that a row's 128 bytes go out together: 16-byte chunk c of row q
+    // sits at position c ^ (q / 4) % 8.
+    char* blk = own + 8192;
+    asm volatile("" ::: "memory");
 #pragma unroll
     for (int a = 0; a < 2; ++a)
 #pragma unroll

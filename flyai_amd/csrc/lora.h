@@ -39,22 +39,23 @@ __device__ __forceinline__ int lora_segment(const LoraArgs& a, int f) {
 // every segment.  Each workgroup lists the pairs for itself (adapters of up to 64 * TILES rows in LDS, and how many distinct
 // ones each tile has) and takes every wgs-th item: none is launched in vain, whatever the mix.
 // An item multiplies the tile's rows that have the adapter, gathered, 16 to an MFMA tile, with 32 rows of A.  K is cut into
-// four parts, a wave each, whose sums are added in order through LDS; lane (r, g) of an MFMA holds row r in its second
-// operand, so a row's products never meet another row's: a row's h depends neither on its tile nor on the launch.
+// eight parts, summed in pairs and then in order through LDS, a wave one part or (with four waves) a pair of them; lane
+// (r, g) of an MFMA holds row r in its second operand, so a row's products never meet another row's: a row's h depends
+// neither on its tile nor on the launch.
 // What bounds it is how fast rows of x and A come from L2.  A wave loads whole 128-byte runs (8 rows an instruction) and
 // turns them round in LDS of its own (the tiled GEMM's swizzle); loaded as MFMA operands, 16 rows of 64 bytes an
 // instruction, every quarter of an instruction touched 16 lines, and 2,096 rows of 192 rank columns took 51 us.
 // h is kept as two bf16 terms, the value and what its rounding left out: 16 significant bits (2^-17 of d at most) for the
 // bytes of one fp32 value, and the up product takes them as they are.
-constexpr int kDownParts = 4;   // parts of K
+constexpr int kDownParts = 8;   // parts of K
 constexpr int kDownRows = 64;   // rows of a tile
 constexpr int kDownCols = kLoraCols;
 
 template <int WAVES, int TILES>
 struct LoraDownLds {
   union {
-    char stage[kDownParts][(kDownRows + kDownCols) * 128];       // a wave's 64-K group: rows of x, rows of A
-    float red[kDownParts][kDownRows][kDownCols + 4];
+    char stage[WAVES][(kDownRows + kDownCols) * 128];       // a wave's 64-K group: rows of x, rows of A
+    float red[WAVES][kDownRows][kDownCols + 4];
   };
   int adapter[kDownRows * TILES];       // -1 where the row has none, or one of rank 0
   int first[TILES + 1];                 // pairs before the tile
@@ -65,10 +66,11 @@ struct LoraDownLds {
 inline int lora_down_groups(const LoraArgs& a) { return a.n_seg * (lora_cols(a.R) / kDownCols); }
 
 // One wave's part of an item's product: NP * 16 gathered rows (l.row, n of them) against 32 rows of A from ar, over the
-// 64-K groups [k0, k1).  D groups are in flight in registers.
-template <int NP, int D, typename Lds>
+// 64-K groups [k0, k1): the sum of the parts before `mid` and from it on, each from zero.  D groups are in flight in
+// registers.
+template <int NP, int D, bool PAIR, typename Lds>
 __device__ __forceinline__ void lora_down_part(const uint16_t* __restrict__ x, const uint16_t* __restrict__ ar, int a_rows, int K,
-                                               int m0, int n, int k0, int k1, char* st, const Lds& l, f32x4_t (&acc)[4][2]) {
+                                               int m0, int n, int k0, int mid, int k1, char* st, const Lds& l, f32x4_t (&acc)[4][2]) {
   constexpr int NX = 2 * NP, NI = NX + kDownCols / 8;  // load instructions a group: 8 rows each
   const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
   const uint16_t* src[NI];
@@ -90,10 +92,23 @@ __device__ __forceinline__ void lora_down_part(const uint16_t* __restrict__ x, c
 #pragma unroll
   for (int d = 0; d < D; ++d) load(buf[d], k0 + d);
   const int frag = r * 128 + ((g ^ ((r >> 1) & 7)) << 4);
+  f32x4_t head[PAIR ? NP : 1][2];
+  if constexpr (PAIR) {
+#pragma unroll
+    for (int p = 0; p < NP; ++p) head[p][0] = head[p][1] = f32x4_t{-0.f, -0.f, -0.f, -0.f};  // -0 + x is x
+  }
   for (int kb = k0; kb < k1; kb += D) {
 #pragma unroll
     for (int d = 0; d < D; ++d) {
       if (kb + d >= k1) break;
+      if constexpr (PAIR) {
+        if (kb + d == mid) {
+#pragma unroll
+          for (int p = 0; p < NP; ++p)
+#pragma unroll
+            for (int c = 0; c < 2; ++c) head[p][c] = acc[p][c], acc[p][c] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+        }
+      }
 #pragma unroll
       for (int i = 0; i < NI; ++i) *reinterpret_cast<u32x4_t*>(st + 1024 * i + 16 * lane) = buf[d][i];
       asm volatile("" ::: "memory");  // this wave's LDS operations complete in order
@@ -115,12 +130,20 @@ __device__ __forceinline__ void lora_down_part(const uint16_t* __restrict__ x, c
       asm volatile("" ::: "memory");
     }
   }
+  if constexpr (PAIR) {
+#pragma unroll
+    for (int p = 0; p < NP; ++p)
+#pragma unroll
+      for (int c = 0; c < 2; ++c) acc[p][c] = head[p][c] + acc[p][c];
+  }
 }
 
 template <int WAVES, int TILES>
 __device__ __forceinline__ void lora_down(const uint16_t* __restrict__ x, int M, int K, const LoraArgs& a, int wg, int wgs,
                                           LoraDownLds<WAVES, TILES>& l) {
-  constexpr int kThreads = 64 * WAVES;
+  constexpr int kThreads = 64 * WAVES, kPairs = kDownParts / WAVES;  // parts a wave
+  static_assert(kPairs == 1 || kPairs == 2, "a wave takes a part or a pair");
+  constexpr int kMine = (TILES + WAVES - 1) / WAVES;  // tiles a wave lists
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), r = lane & 15, g = lane >> 4;
   const int cols = lora_cols(a.R), per_seg = cols / kDownCols, groups = a.n_seg * per_seg;
   const int KG = (K + 63) / 64;
@@ -130,16 +153,20 @@ __device__ __forceinline__ void lora_down(const uint16_t* __restrict__ x, int M,
   for (int t0 = 0; t0 < M; t0 += kDownRows * TILES) {
     const int rows = min(M - t0, kDownRows * TILES), tiles = (rows + kDownRows - 1) / kDownRows;
     if (t0) __syncthreads();
-    const int mine0 = row_of[t0 + min(tid, rows - 1)];  // the wave's first tile
+    int fetched[kMine];
+#pragma unroll
+    for (int j = 0; j < kMine; ++j) fetched[j] = row_of[t0 + min(kDownRows * (wave + WAVES * j) + lane, rows - 1)];
     if (t0 == 0 && small) {
       if (tid < a.n) l.rank_of[tid] = min(max(a.ranks[tid], 0), a.R);
       if (a.row_seq && tid < a.n_seqs) l.of_seq[tid] = a.adapter[tid];
     }
     if (tid == 0) l.first[0] = 0;
     __syncthreads();
-    for (int t = wave; t < tiles; t += WAVES) {
-      const int i = kDownRows * t + lane;
-      int ad = t == wave ? mine0 : row_of[t0 + min(i, rows - 1)], rank = 0;
+#pragma unroll
+    for (int j = 0; j < kMine; ++j) {
+      const int t = wave + WAVES * j, i = kDownRows * t + lane;
+      if (t >= tiles) break;
+      int ad = fetched[j], rank = 0;
       if (a.row_seq) {
         const bool in = (unsigned)ad < (unsigned)a.n_seqs;
         const int sq = in ? ad : 0;
@@ -188,31 +215,32 @@ __device__ __forceinline__ void lora_down(const uint16_t* __restrict__ x, int M,
       f32x4_t acc[4][2];
 #pragma unroll
       for (int p = 0; p < 4; ++p) acc[p][0] = acc[p][1] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-      if (wave < kDownParts) {
-        const uint16_t* ar = a.A + (((size_t)ad * a.n_seg + seg) * a.R + c0) * K;
-        const int k0 = KG * wave / kDownParts, k1 = KG * (wave + 1) / kDownParts, a_rows = min(rank - c0, kDownCols);
-        if (k0 == k1) {}  // fewer groups than waves
-        else if (n <= 16) lora_down_part<1, 4>(x, ar, a_rows, K, m0, n, k0, k1, l.stage[wave], l, acc);
-        else if (n <= 32) lora_down_part<2, 2>(x, ar, a_rows, K, m0, n, k0, k1, l.stage[wave], l, acc);
-        else lora_down_part<4, 2>(x, ar, a_rows, K, m0, n, k0, k1, l.stage[wave], l, acc);
-      }
+      const uint16_t* ar = a.A + (((size_t)ad * a.n_seg + seg) * a.R + c0) * K;
+      const int e = kPairs * wave, a_rows = min(rank - c0, kDownCols);
+      const int k0 = KG * e / kDownParts, mid = kPairs == 2 ? KG * (e + 1) / kDownParts : -1, k1 = KG * (e + kPairs) / kDownParts;
+      if (k0 == k1) {}  // fewer groups than waves
+      else if (n <= 16) lora_down_part<1, 4, kPairs == 2>(x, ar, a_rows, K, m0, n, k0, mid, k1, l.stage[wave], l, acc);
+      else if (n <= 32) lora_down_part<2, 2, kPairs == 2>(x, ar, a_rows, K, m0, n, k0, mid, k1, l.stage[wave], l, acc);
+      else lora_down_part<4, 1, kPairs == 2>(x, ar, a_rows, K, m0, n, k0, mid, k1, l.stage[wave], l, acc);
       __syncthreads();  // red lies over the stages
-      if (wave < kDownParts) {  // lane (r, g): rank columns 4g .. +3 of row r
+      // lane (r, g): rank columns 4g .. +3 of row r
 #pragma unroll
-        for (int p = 0; p < 4; ++p)
-          if (16 * p < n) {
+      for (int p = 0; p < 4; ++p)
+        if (16 * p < n) {
 #pragma unroll
-            for (int c = 0; c < 2; ++c) *reinterpret_cast<f32x4_t*>(&l.red[wave][16 * p + r][16 * c + 4 * g]) = acc[p][c];
-          }
-      }
+          for (int c = 0; c < 2; ++c) *reinterpret_cast<f32x4_t*>(&l.red[wave][16 * p + r][16 * c + 4 * g]) = acc[p][c];
+        }
       __syncthreads();
       for (int i = tid; i < n * kDownCols; i += kThreads) {
         const int q = i / kDownCols, j = i % kDownCols;
         float v = 0.f;  // columns past the rank are zero, whatever A holds
         if (c0 + j < rank) {
-          v = l.red[0][q][j];
 #pragma unroll
-          for (int e = 1; e < kDownParts; ++e) v += l.red[e][q][j];
+          for (int e = 0; e < WAVES; e += WAVES / 4) {
+            float pair = l.red[e][q][j];
+            if (kPairs == 1) pair += l.red[e + 1][q][j];
+            v = e ? v + pair : pair;
+          }
           v *= scale;
         }
         const uint16_t hi = f2bf(v);
@@ -243,52 +271,110 @@ __device__ __forceinline__ bf16x8_t lora_within(uint4 w, int left) {
 // Where lane (r, g) reads its eight columns from 32c on in a row of B of R columns (clamped: those past R are masked).
 __device__ __forceinline__ int lora_col(int R, int c, int g) { return min(kLoraCols * c + 8 * g, R - 8); }
 
-// The up product of 16 rows from m0 and 64 features from f0 (one segment), added to the tiled GEMM's sums: lane (r, g)
-// holds rows 4g .. +3 of feature f0 + 16 b + r in sum[b].  `who` is row m0 + r's adapter and rank.
-__device__ __forceinline__ void lora_up_rows(const LoraArgs& a, int M, int N, int m0, int f0, int2 who, f32x4_t (&sum)[4]) {
-  const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
+// 64 columns from c0 of 8 rows of `pitch` elements each as one instruction reads them: lane L takes row L / 8 and the chunk
+// that belongs at position L % 8 of row `at` + L / 8 of a tile in the GEMM's swizzle.  Columns past `end` are clamped.
+__device__ __forceinline__ int lora_chunk(int at, int c0, int end) {
+  const int lane = threadIdx.x & 63, q = at + (lane >> 3);
+  return min(c0 + 8 * ((lane & 7) ^ ((q >> 1) & 7)), end - 8);
+}
+
+// h of the tiled GEMM's wave, 32 rows from m0 in the segment of feature f0, columns 0 .. 63: h[4 a + 2 t + i] is rows 16 a +
+// 8 i .. +7, high (t = 0) or low terms, for 1 KiB of LDS each.
+__device__ __forceinline__ void lora_fetch_h(const LoraArgs& a, int M, int m0, int f0, u32x4_t (&h)[8]) {
   const int cols = lora_cols(a.R), seg = lora_segment(a, f0);
-  const int mine = m0 + r < M && who.y > 0 ? who.x : -1;
-  int of_row[4];
 #pragma unroll
-  for (int v = 0; v < 4; ++v) of_row[v] = __builtin_amdgcn_ds_bpermute(4 * (4 * g + v), mine);
-  const uint16_t* hr = a.h + ((size_t)min(m0 + r, M - 1) * a.n_seg + seg) * 2 * cols + 8 * g;
-  const uint16_t* br[4];
+  for (int k = 0; k < 8; ++k) {
+    const int row = m0 + 16 * (k >> 2) + 8 * (k & 1) + ((threadIdx.x & 63) >> 3);
+    h[k] = *reinterpret_cast<const u32x4_t*>(a.h + ((size_t)min(row, M - 1) * a.n_seg + seg) * 2 * cols + (k & 2 ? cols : 0) +
+                                             lora_chunk(8 * (k & 1), 0, cols));
+  }
+}
+
+// The up products of 32 rows from m0 and 64 features from f0 (one segment), added to the tiled GEMM's sums: lane (r, g)
+// holds rows 16 a + 4g .. +3 of feature f0 + 16 b + r in sum[a][b].  `who`: row m0 + lane's adapter and rank (lanes 0 ..
+// 31).  hl: lora_fetch_h's tiles; held_b: columns 0 .. 63 of adapter `held` (-1: of none), this wave's features, 16 to a
+// tile; bl: room for another adapter's, which come in whole runs like the GEMM's operands (as MFMA operands from memory a
+// tile of 128 rows of 45 adapters took 50,000 clocks, more than its projection).
+__device__ __forceinline__ void lora_up_block(const LoraArgs& a, int M, int N, int m0, int f0, int2 who, const char* hl, int held,
+                                              const char* held_b, char* bl, f32x4_t (&sum)[2][4]) {
+  const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
+  const int cols = lora_cols(a.R);
+  const int key = lane < 32 && m0 + lane < M && who.y > 0 ? who.x : -1;
+  int of_row[2][4];
 #pragma unroll
-  for (int b = 0; b < 4; ++b) br[b] = a.B + (size_t)min(f0 + 16 * b + r, N - 1) * a.R;
-  uint64_t todo = __ballot(mine >= 0) & 0xffff;
-  while (todo) {
+  for (int t = 0; t < 2; ++t)
+#pragma unroll
+    for (int v = 0; v < 4; ++v) of_row[t][v] = __builtin_amdgcn_ds_bpermute(4 * (16 * t + 4 * g + v), key);
+  uint64_t todo = __ballot(key >= 0);
+  int ad = -1, rank = 0;
+  uint64_t rows = 0;
+  u32x4_t nb[8];
+  auto next = [&]() __attribute__((always_inline)) {
+    ad = -1;
+    if (!todo) return;
     const int first = __builtin_ctzll(todo);
-    const int ad = __builtin_amdgcn_readlane(mine, first), rank = __builtin_amdgcn_readlane(who.y, first);
-    todo &= ~__ballot(mine == ad);
-    f32x4_t up[4];
+    ad = __builtin_amdgcn_readlane(key, first);
+    rank = __builtin_amdgcn_readlane(who.y, first);
+    rows = __ballot(key == ad);
+    todo &= ~rows;
+    if (ad == held) return;
 #pragma unroll
-    for (int b = 0; b < 4; ++b) up[b] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-    for (int c0 = 0; kLoraCols * c0 < rank; c0 += 2) {
-      uint4 hi[2], lo[2], bv[4][2];
+    for (int k = 0; k < 8; ++k)
+      nb[k] = *reinterpret_cast<const u32x4_t*>(a.B + ((size_t)ad * N + min(f0 + 8 * k + (lane >> 3), N - 1)) * a.R +
+                                                lora_chunk(8 * (k & 1), 0, a.R));
+  };
+  const int frag = r * 128 + ((g ^ ((r >> 1) & 7)) << 4);
+  next();
+  while (ad >= 0) {
+    const int now = ad, cur_rank = rank;
+    const uint64_t cur_rows = rows;
+    const char* src = now == held ? held_b : bl;
+    if (now != held) {
+      asm volatile("" ::: "memory");  // a wave's LDS operations complete in order
+#pragma unroll
+      for (int k = 0; k < 8; ++k) *reinterpret_cast<u32x4_t*>(bl + 1024 * k + 16 * lane) = nb[k];
+      asm volatile("" ::: "memory");
+    }
+    next();  // the next adapter's columns are on their way under this one's products
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      if (!(cur_rows >> (16 * t) & 0xffff)) continue;
+      f32x4_t up[4];
+#pragma unroll
+      for (int b = 0; b < 4; ++b) up[b] = f32x4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
-        const int cc = min(c0 + c, (rank - 1) / kLoraCols);
-        hi[c] = *reinterpret_cast<const uint4*>(hr + kLoraCols * cc);
-        lo[c] = *reinterpret_cast<const uint4*>(hr + kLoraCols * cc + cols);
+        const int left = cur_rank - kLoraCols * c;
+        if (left <= 0) break;
+        const bf16x8_t hi = as_bf16x8(*reinterpret_cast<const uint4*>(hl + 4096 * t + (frag ^ (c << 6))));
+        const bf16x8_t lo = as_bf16x8(*reinterpret_cast<const uint4*>(hl + 4096 * t + 2048 + (frag ^ (c << 6))));
 #pragma unroll
-        for (int b = 0; b < 4; ++b) bv[b][c] = *reinterpret_cast<const uint4*>(br[b] + (size_t)ad * N * a.R + lora_col(a.R, cc, g));
+        for (int b = 0; b < 4; ++b) {
+          const uint4 raw = *reinterpret_cast<const uint4*>(src + 2048 * b + (frag ^ (c << 6)));
+          const bf16x8_t w = left < kLoraCols ? lora_within(raw, left - 8 * g) : as_bf16x8(raw);
+          up[b] = mfma16x16x32(hi, w, up[b]);
+          up[b] = mfma16x16x32(lo, w, up[b]);
+        }
+      }
+      for (int c = 2; kLoraCols * c < cur_rank; ++c) {  // ranks past 64: straight from memory
+        const int row = min(m0 + 16 * t + r, M - 1), left = cur_rank - kLoraCols * c;
+        const uint16_t* hr = a.h + ((size_t)row * a.n_seg + lora_segment(a, f0)) * 2 * cols + kLoraCols * c + 8 * g;
+        const bf16x8_t hi = as_bf16x8(*reinterpret_cast<const uint4*>(hr));
+        const bf16x8_t lo = as_bf16x8(*reinterpret_cast<const uint4*>(hr + cols));
+#pragma unroll
+        for (int b = 0; b < 4; ++b) {
+          const bf16x8_t w = lora_within(*reinterpret_cast<const uint4*>(a.B + ((size_t)now * N + min(f0 + 16 * b + r, N - 1)) * a.R +
+                                                                         lora_col(a.R, c, g)),
+                                         left - 8 * g);
+          up[b] = mfma16x16x32(hi, w, up[b]);
+          up[b] = mfma16x16x32(lo, w, up[b]);
+        }
       }
 #pragma unroll
-      for (int c = 0; c < 2; ++c)
-        if (kLoraCols * (c0 + c) < rank) {
+      for (int b = 0; b < 4; ++b)
 #pragma unroll
-          for (int b = 0; b < 4; ++b) {
-            const bf16x8_t w = lora_within(bv[b][c], rank - kLoraCols * (c0 + c) - 8 * g);
-            up[b] = mfma16x16x32(as_bf16x8(hi[c]), w, up[b]);
-            up[b] = mfma16x16x32(as_bf16x8(lo[c]), w, up[b]);
-          }
-        }
+        for (int v = 0; v < 4; ++v) sum[t][b][v] += of_row[t][v] == now ? up[b][v] : -0.f;
     }
-#pragma unroll
-    for (int b = 0; b < 4; ++b)
-#pragma unroll
-      for (int v = 0; v < 4; ++v) sum[b][v] += of_row[v] == ad ? up[b][v] : -0.f;
   }
 }
 

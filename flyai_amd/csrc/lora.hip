@@ -27,74 +27,32 @@ __global__ __launch_bounds__(64 * kDownParts) void lora_down_kernel(const uint16
 // y = bf16(sum of the projection's planes + h B^T + bias); or, without planes, h B^T as a plane of its own for another
 // finalize to add (-0 where a row has no adapter: x + -0 is x).
 // A workgroup takes 16 rows x 16 features.  Its four waves share the adapters among the rows: each multiplies the whole
-// tile with its own, and the adapter's rows keep the result.  Up to NS adapters of a wave and 64 columns of each are
-// loaded together: what bounds this kernel is latency, not bytes.
-// `firsts` has a bit for each distinct adapter, at its first row.
-template <int NS>
-__device__ __forceinline__ void lora_up_wave(const LoraArgs& a, int M, int N, int m0, int f0, int2 who, uint64_t firsts, int wave,
-                                             float (*d)[17]) {
-  const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
-  const int cols = lora_cols(a.R), seg = lora_segment(a, f0);
-  const uint16_t* hr = a.h + ((size_t)min(m0 + r, M - 1) * a.n_seg + seg) * 2 * cols + 8 * g;
-  const uint16_t* br = a.B + (size_t)(f0 + r) * a.R;
-  int ads[NS], ranks[NS], most = 0;
-  for (int i = 0; i < wave; ++i) firsts &= firsts - 1;
-#pragma unroll
-  for (int s = 0; s < NS; ++s) {  // slots past the wave's adapters repeat the one before
-    if (s == 0 || firsts) {
-      const int at = __builtin_ctzll(firsts);
-      ads[s] = __builtin_amdgcn_readlane(who.x, at);
-      ranks[s] = __builtin_amdgcn_readlane(who.y, at);
-      for (int i = 0; i < 4; ++i) firsts &= firsts - 1;
-    } else {
-      ads[s] = ads[s ? s - 1 : 0], ranks[s] = ranks[s ? s - 1 : 0];
-    }
-    most = max(most, ranks[s]);
-  }
-  f32x4_t acc[NS];
-#pragma unroll
-  for (int s = 0; s < NS; ++s) acc[s] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-  for (int c0 = 0; kLoraCols * c0 < most; c0 += 2) {
-    uint4 bv[NS][2], hi[2], lo[2];
-#pragma unroll
-    for (int c = 0; c < 2; ++c) {
-      const int cc = min(kLoraCols * (c0 + c), cols - kLoraCols);
-      hi[c] = *reinterpret_cast<const uint4*>(hr + cc);
-      lo[c] = *reinterpret_cast<const uint4*>(hr + cc + cols);
-    }
-#pragma unroll
-    for (int s = 0; s < NS; ++s)
-#pragma unroll
-      for (int c = 0; c < 2; ++c)
-        bv[s][c] = *reinterpret_cast<const uint4*>(br + (size_t)ads[s] * N * a.R + lora_col(a.R, min(c0 + c, (ranks[s] - 1) / kLoraCols), g));
-#pragma unroll
-    for (int c = 0; c < 2; ++c)
-#pragma unroll
-      for (int s = 0; s < NS; ++s)
-        if (kLoraCols * (c0 + c) < ranks[s]) {
-          const bf16x8_t w = lora_within(bv[s][c], ranks[s] - kLoraCols * (c0 + c) - 8 * g);
-          acc[s] = mfma16x16x32(w, as_bf16x8(hi[c]), acc[s]);
-          acc[s] = mfma16x16x32(w, as_bf16x8(lo[c]), acc[s]);
-        }
-  }
-  // lane (r, g): features 4g .. +3 of row r
-#pragma unroll
-  for (int s = 0; s < NS; ++s)
-    if (who.y > 0 && who.x == ads[s]) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) d[r][4 * g + i] = acc[s][i];
-    }
-}
+// tile with its own, and the adapter's rows keep the result.  h and B come in whole 128-byte runs and are turned round in
+// LDS (the tiled GEMM's swizzle): as MFMA operands from memory, 16 rows of 64 bytes an instruction, they took 5 of the
+// 10 us at 48 rows of 12 adapters.
+constexpr int kUpCols = 64;  // rank columns a pass
+constexpr int kUpMine = 4;   // adapters a wave: 16 rows have at most 16
+
+struct LoraUpLds {
+  char h[2][16 * 128];               // high and low terms: 16 rows of 64 columns
+  char b[4][kUpMine][16 * 128];      // a wave's adapters: 16 features of 64 columns
+  float d[16][17];
+};
 
 template <bool PLANE>
-__global__ __launch_bounds__(256) void lora_finalize_kernel(const float* __restrict__ part, int slices, int M, int N,
+__global__ __launch_bounds__(256, 4) void lora_finalize_kernel(const float* __restrict__ part, int slices, int M, int N,
                                                             LoraArgs a, const uint16_t* __restrict__ b,
                                                             uint16_t* __restrict__ y, uint16_t* __restrict__ residual,
                                                             float* __restrict__ plane_out) {
-  __shared__ float d[16][17];
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = lane & 15;
+  __shared__ __align__(1024) LoraUpLds l;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = lane & 15, g = lane >> 4;
   const int f0 = blockIdx.x * 16, m0 = blockIdx.y * 16;
+  const int cols = lora_cols(a.R), seg = lora_segment(a, f0);
   int2 who = a.meta[min(m0 + r, M - 1)];
+  // h: the wave's four rows, 16 lanes each, 8 chunks of the high terms and 8 of the low ones
+  const int hq = 4 * wave + (lane >> 4), hc = (lane & 7) ^ ((hq >> 1) & 7);
+  const uint16_t* hp = a.h + ((size_t)min(m0 + hq, M - 1) * a.n_seg + seg) * 2 * cols + (lane & 8 ? cols : 0);
+  u32x4_t hv = *reinterpret_cast<const u32x4_t*>(hp + min(8 * hc, cols - 8));
   // this thread's output: row 4 * wave + lane / 16, feature lane % 16
   const int mine = 4 * wave + (lane >> 4), row = m0 + mine;
   const size_t idx = (size_t)min(row, M - 1) * N + f0 + r, plane = (size_t)M * N;
@@ -113,14 +71,75 @@ __global__ __launch_bounds__(256) void lora_finalize_kernel(const float* __restr
   bool fresh = key >= 0;  // the first of its adapter's rows
 #pragma unroll
   for (int i = 0; i < 15; ++i) fresh &= i >= r || __builtin_amdgcn_readlane(key, i) != key;
-  const uint64_t firsts = __ballot(fresh) & 0xffff;
-  const int n = __builtin_popcountll(firsts), share = (n - wave + 3) / 4;
-  if (share > 2) lora_up_wave<4>(a, M, N, m0, f0, who, firsts, wave, d);
-  else if (share == 2) lora_up_wave<2>(a, M, N, m0, f0, who, firsts, wave, d);
-  else if (share == 1) lora_up_wave<1>(a, M, N, m0, f0, who, firsts, wave, d);
-  if (n > 0) __syncthreads();
+  uint64_t firsts = __ballot(fresh) & 0xffff;
+  const int n = __builtin_popcountll(firsts);
+  if (n > 0) {
+    // the wave's adapters: every fourth
+    for (int i = 0; i < wave; ++i) firsts &= firsts - 1;
+    int ads[kUpMine], ranks[kUpMine];
+#pragma unroll
+    for (int s = 0; s < kUpMine; ++s) {
+      const int at = __builtin_ctzll(firsts | 1ull << 63);
+      ads[s] = firsts ? __builtin_amdgcn_readlane(who.x, at & 15) : -1;
+      ranks[s] = firsts ? __builtin_amdgcn_readlane(who.y, at & 15) : 0;
+      for (int i = 0; i < 4; ++i) firsts &= firsts - 1;
+    }
+    f32x4_t acc[kUpMine];
+#pragma unroll
+    for (int s = 0; s < kUpMine; ++s) acc[s] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+    int top = who.y;  // the largest rank of the tile: the same in every wave
+#pragma unroll
+    for (int off = 1; off < 16; off <<= 1) top = max(top, __shfl_xor(top, off, 64));
+    top = __builtin_amdgcn_readfirstlane(top);
+    const int frag = r * 128 + ((g ^ ((r >> 1) & 7)) << 4);
+    for (int c0 = 0; c0 < top; c0 += kUpCols) {
+      if (c0) {
+        __syncthreads();
+        hv = *reinterpret_cast<const u32x4_t*>(hp + min(c0 + 8 * hc, cols - 8));
+      }
+      u32x4_t bv[kUpMine][2];
+#pragma unroll
+      for (int s = 0; s < kUpMine; ++s)
+        if (c0 < ranks[s]) {
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {  // 8 features an instruction
+            const int q = 8 * i + (lane >> 3), c = (lane & 7) ^ ((q >> 1) & 7);
+            bv[s][i] = *reinterpret_cast<const u32x4_t*>(a.B + ((size_t)ads[s] * N + f0 + q) * a.R + min(c0 + 8 * c, a.R - 8));
+          }
+        }
+      *reinterpret_cast<u32x4_t*>(l.h[lane >> 3 & 1] + hq * 128 + 16 * (lane & 7)) = hv;
+#pragma unroll
+      for (int s = 0; s < kUpMine; ++s)
+        if (c0 < ranks[s]) {
+#pragma unroll
+          for (int i = 0; i < 2; ++i) *reinterpret_cast<u32x4_t*>(l.b[wave][s] + 1024 * i + 16 * lane) = bv[s][i];
+        }
+      __syncthreads();
+#pragma unroll
+      for (int c = 0; c < kUpCols / kLoraCols; ++c) {
+        const bf16x8_t hi = as_bf16x8(*reinterpret_cast<const uint4*>(l.h[0] + (frag ^ (c << 6))));
+        const bf16x8_t lo = as_bf16x8(*reinterpret_cast<const uint4*>(l.h[1] + (frag ^ (c << 6))));
+#pragma unroll
+        for (int s = 0; s < kUpMine; ++s)
+          if (c0 + kLoraCols * c < ranks[s]) {
+            const bf16x8_t w = lora_within(*reinterpret_cast<const uint4*>(l.b[wave][s] + (frag ^ (c << 6))),
+                                           ranks[s] - c0 - kLoraCols * c - 8 * g);
+            acc[s] = mfma16x16x32(w, hi, acc[s]);
+            acc[s] = mfma16x16x32(w, lo, acc[s]);
+          }
+      }
+    }
+    // lane (r, g): features 4g .. +3 of row r
+#pragma unroll
+    for (int s = 0; s < kUpMine; ++s)
+      if (key >= 0 && key == ads[s]) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) l.d[r][4 * g + i] = acc[s][i];
+      }
+    __syncthreads();
+  }
   if (row >= M) return;
-  const float up = has ? d[mine][r] : -0.f;
+  const float up = has ? l.d[mine][r] : -0.f;
   if constexpr (PLANE) {
     plane_out[idx] = up;
   } else {
@@ -140,16 +159,16 @@ static size_t align256(size_t v) { return (v + 255) & ~(size_t)255; }
 static size_t partial_bytes(int M, int N, int K) { return (size_t)gemm_planes(M, K) * M * N * sizeof(float); }
 
 static int launch_lora_down(const uint16_t* x, int M, int K, const LoraArgs& a, hipStream_t s) {
-  const int wgs = std::min(2 * device_cus(), M * lora_down_groups(a));
+  const int wgs = std::min(device_cus(), M * lora_down_groups(a));
   hipLaunchKernelGGL(lora_down_kernel, dim3(wgs), dim3(64 * kDownParts), 0, s, x, M, K, a);
   return check_launch("lora_down");
 }
 
-// The projection's planes and h: one launch where the split-K kernel has four waves, the down product's own before it
-// otherwise (with eight waves its registers would cost the projection its second workgroup a CU).
+// The projection's planes and h: one launch below the tiled kernel's rows, of the split-K kernel with four waves (with eight
+// the down product's registers would not fit), the down product's own before the tiled kernel.
 static int launch_gemm_lora(const uint16_t* x, const uint16_t* W, int M, int N, int K, float* part, int* slices, const LoraArgs& a,
                             hipStream_t s) {
-  if (gemm_is_tiled(M) || splitk_eight_waves(M, N, gemm_slices(K))) {
+  if (gemm_is_tiled(M)) {
     const int rc = launch_lora_down(x, M, K, a, s);
     return rc ? rc : launch_gemm(x, W, M, N, K, part, slices, s);
   }

@@ -54,6 +54,15 @@ class KvMove(C.Structure):
     _fields_ = [("base", C.c_int64), ("cap", C.c_int32), ("start", C.c_int32), ("n", C.c_int32), ("pad", C.c_int32)]
 
 
+class LoraLayer(C.Structure):
+    _fields_ = [(n, C.c_void_p) for n in ("qkv_a", "qkv_b", "o_a", "o_b")]
+
+
+class StageLora(C.Structure):
+    _fields_ = [("n_adapters", C.c_int32), ("max_rank", C.c_int32), ("scale", C.c_void_p), ("ranks", C.c_void_p),
+                ("layers_host", C.POINTER(LoraLayer)), ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t)]
+
+
 P, I32, I64, F32, SZ = C.c_void_p, C.c_int32, C.c_int64, C.c_float, C.c_size_t
 
 # name -> (restype, argtypes)
@@ -115,6 +124,10 @@ _PROTOS = {
     "flyai_stage_set_workspace": (C.c_int, [P, P, SZ, P, SZ]),
     "flyai_stage_forward": (C.c_int, [P, P, P, P, P, I32, P, P]),
     "flyai_stage_forward_tree": (C.c_int, [P, I32, I32, P, P, I64, I32, P, P]),
+    "flyai_stage_lora_workspace_bytes": (SZ, [P, I32]),
+    "flyai_stage_set_lora": (C.c_int, [P, P]),
+    "flyai_stage_forward_lora": (C.c_int, [P, P, P, P, P, P, I32, P, P]),
+    "flyai_stage_forward_tree_lora": (C.c_int, [P, I32, I32, P, P, I64, I32, I32, P, P]),
     "flyai_stage_debug_buffer": (P, [P, I32]),
     "flyai_stage_set_graphs": (C.c_int, [P, I32]),
     "flyai_stage_graphs_captured": (I32, [P]),

@@ -9,6 +9,7 @@
 #include <vector>
 
 #include "common.h"
+#include "gemm.h"
 
 namespace flyai {
 
@@ -48,17 +49,20 @@ int launch_moe_down_fp8act(const uint16_t*, const uint8_t*, const uint8_t*, cons
 bool moe_batch_is_dense(int rows_total, int E, int K);
 int launch_rmsnorm(const uint16_t*, const float*, int, int, float, uint16_t*, hipStream_t);
 int launch_linear_residual_rmsnorm(const uint16_t*, const uint16_t*, const uint16_t*, int, int, int,
-                                   uint16_t*, const float*, float, uint16_t*, float*, hipStream_t);
+                                   uint16_t*, const float*, float, uint16_t*, float*, const LoraArgs*, hipStream_t);
 int launch_linear_residual_rmsnorm_logits(const uint16_t*, const uint16_t*, const uint16_t*, int, int,
                                           int, const uint16_t*, uint16_t*, const float*, float, uint16_t*,
-                                          float*, const uint16_t*, const uint16_t*, int, float*, hipStream_t);
+                                          float*, const uint16_t*, const uint16_t*, int, float*, const LoraArgs*,
+                                          hipStream_t);
 int launch_topk_permute(const float*, int, int, int, int32_t*, float*, int32_t*, int32_t*, int32_t*,
                         int32_t*, hipStream_t);
 int launch_qkv_rope_kv(const uint16_t*, const uint16_t*, const uint16_t*, float*, const int32_t*,
                        const int32_t*, const uint16_t*, const uint16_t*, int, int, int, int, int, int,
                        const int64_t*, const int32_t*, uint16_t*, uint16_t*, uint16_t*, const int32_t*,
-                       hipStream_t);
+                       const LoraArgs*, hipStream_t);
 size_t linear_partials_bytes(int M, int N, int K);
+bool gemm_is_tiled(int M);
+int gemm_planes(int M, int K);
 int launch_attn(const uint16_t*, const uint16_t*, const uint16_t*, const int64_t*, const int32_t*,
                 const float*, int, int, const flyai_attn_item*, int, int, const flyai_attn_group*, int,
                 const int32_t*, float*, uint16_t*, const flyai_attn_tree*, bool, hipStream_t);
@@ -127,7 +131,7 @@ struct flyai_stage {
   bool graphs = false;
   hipStream_t capture_stream = nullptr;
   struct Graph {
-    int64_t key[12];
+    int64_t key[13];
     hipGraphExec_t exec;
     uint64_t last_use;
   };
@@ -136,6 +140,10 @@ struct flyai_stage {
   int graphs_captured = 0;
   std::vector<int> slab_order;  // host scratch of the slab-overlap check (max_seqs entries)
   int tree_cap = 0;             // largest tree: min(max_tokens, FLYAI_TREE_MAX_NODES) nodes
+  // adapters (flyai_stage_set_lora): the bank, its layers' matrices, and the workspace of steps that have any
+  bool has_lora = false;
+  flyai_stage_lora lora = {};
+  std::vector<flyai_lora_layer> lora_layers;
   std::vector<char> tree_img;   // host image of a tree step's flyai_attn_tree (header, depths, masks)
   std::vector<int> tree_order;  // host scratch: the nodes in order of depth
 };
@@ -163,7 +171,7 @@ static size_t blob_bytes(int S, int n_items0, int n_items1, int n_groups0, int n
   return align256(4 * sizeof(int32_t)) + align256((size_t)S * 4) * 3 + align256((size_t)S * 8) +
          align256((size_t)n_items0 * sizeof(flyai_attn_item)) + align256((size_t)n_items1 * sizeof(flyai_attn_item)) +
          align256((size_t)n_groups0 * sizeof(flyai_attn_group)) + align256((size_t)n_groups1 * sizeof(flyai_attn_group)) +
-         2 * align256((size_t)n_pitems * sizeof(flyai_attn_item)) + align256(tree_bytes(tree_nodes));
+         2 * align256((size_t)n_pitems * sizeof(flyai_attn_item)) + align256(tree_bytes(tree_nodes)) + align256((size_t)S * 4);
 }
 
 static void layout(flyai_stage* st) {
@@ -297,6 +305,71 @@ extern "C" int flyai_stage_set_rope(flyai_stage* st, const uint16_t* cos_tab, co
   return FLYAI_OK;
 }
 
+// Partial planes of the larger projection below the tiled kernel's rows, the up products' plane included (from there on the
+// stage's own region holds the one plane), then h.
+static size_t lora_planes_bytes(const flyai_stage* st) {
+  const flyai_stage_config& c = st->cfg;
+  const int rows = std::min(c.max_tokens, kTiledMinRows - 1);
+  const int K = c.n_q_heads * c.head_dim;
+  return align256(std::max((size_t)(gemm_planes(1, c.hidden) + 1) * st->qkv_width, (size_t)(gemm_planes(1, K) + 1) * c.hidden) * rows *
+                  sizeof(float));
+}
+
+extern "C" size_t flyai_stage_lora_workspace_bytes(const flyai_stage* st, int32_t R) {
+  return st && R > 0 ? lora_planes_bytes(st) + lora_h_bytes(st->cfg.max_tokens, R, 3) : 0;
+}
+
+// The arguments of layer l's projection (0: q, k, v; 1: output) in a step.
+static int stage_lora_args(flyai_stage* st, int l, int which, const int32_t* adapter, const int32_t* seq_id, int S, LoraArgs* out) {
+  const flyai_stage_config& c = st->cfg;
+  const flyai_lora_layer& L = st->lora_layers[l];
+  const int q = c.n_q_heads * c.head_dim, kv = c.n_kv_heads * c.head_dim;
+  const int32_t qkv[3] = {q, kv, kv}, o[1] = {c.hidden};
+  const int rc = which ? make_lora_args(out, L.o_a, L.o_b, st->lora.scale, st->lora.ranks, st->lora.n_adapters, st->lora.max_rank, o, 1,
+                                        c.hidden, adapter, seq_id, S)
+                       : make_lora_args(out, L.qkv_a, L.qkv_b, st->lora.scale, st->lora.ranks, st->lora.n_adapters, st->lora.max_rank,
+                                        qkv, 3, st->qkv_width, adapter, seq_id, S);
+  if (rc) return rc;
+  lora_bind(out, static_cast<char*>(st->lora.workspace) + lora_planes_bytes(st), c.max_tokens);
+  return FLYAI_OK;
+}
+
+extern "C" int flyai_stage_set_lora(flyai_stage* st, const flyai_stage_lora* lora) {
+  FLYAI_REQUIRE(st, "set_lora: null stage");
+  if (!lora) {
+    drop_graphs(st);
+    st->has_lora = false;
+    return FLYAI_OK;
+  }
+  FLYAI_REQUIRE(lora->layers_host && lora->workspace && ((uintptr_t)lora->workspace & 255) == 0,
+                "set_lora: needs the layers, and a 256-byte aligned workspace");
+  FLYAI_REQUIRE(lora->max_rank > 0 && lora->workspace_bytes >= flyai_stage_lora_workspace_bytes(st, lora->max_rank),
+                "set_lora: needs a workspace of %zu bytes", flyai_stage_lora_workspace_bytes(st, lora->max_rank));
+  const flyai_stage_lora old = st->lora;
+  std::vector<flyai_lora_layer> layers;
+  try {
+    layers.assign(lora->layers_host, lora->layers_host + st->cfg.n_layers);
+  } catch (...) {
+    return set_error(FLYAI_EINVAL, "set_lora: out of host memory");
+  }
+  st->lora = *lora;
+  st->lora.layers_host = nullptr;
+  st->lora_layers.swap(layers);
+  LoraArgs a;
+  for (int l = 0; l < st->cfg.n_layers; ++l)
+    for (int which = 0; which < 2; ++which) {
+      const int rc = stage_lora_args(st, l, which, lora->ranks, nullptr, 0, &a);  // every check; the arguments are made anew each step
+      if (rc) {
+        st->lora = old;
+        st->lora_layers.swap(layers);
+        return rc;
+      }
+    }
+  drop_graphs(st);
+  st->has_lora = true;
+  return FLYAI_OK;
+}
+
 extern "C" size_t flyai_stage_workspace_bytes(const flyai_stage* st) { return st ? st->dev_bytes : 0; }
 extern "C" size_t flyai_stage_host_staging_bytes(const flyai_stage* st) {
   return st ? 2 * st->host_half : 0;
@@ -362,6 +435,8 @@ struct StepPlan {
   int lean[2];      // every split item has <= 2 tokens: the three-wave step kernel (part of the graph key)
   size_t off_counts, off_q, off_st, off_cap, off_base, off_items[2], off_groups[2], off_pitems[2];
   bool tree = false;  // a tree-verify step: the blob carries the flyai_attn_tree at off_tree
+  bool lora = false;  // some sequence has an adapter: the blob carries theirs at off_adapter
+  size_t off_adapter = 0;
   size_t off_tree = 0, off_tree_depth = 0;
 };
 }  // namespace
@@ -382,6 +457,8 @@ static int record_step(flyai_stage* st, const StepPlan& sp, const int32_t* count
   const int32_t* kv_pos = sp.tree ? I32(st->o_kvpos) : nullptr;
 
   const int Tn = sp.Tn;
+  // the projections' partial planes: a step with adapters has one more of them below the tiled kernel's rows
+  float* planes = sp.lora && !gemm_is_tiled(Tn) ? static_cast<float*>(st->lora.workspace) : F32(st->o_gemm);
   const int H = c.hidden, E = c.n_experts, k = c.top_k, I = c.intermediate;
   const bool fused_route = Tn <= 256 && Tn * k <= 4096;
   // the batch packing and the first layer's input RMSNorm in one launch (independent of each other)
@@ -394,11 +471,19 @@ static int record_step(flyai_stage* st, const StepPlan& sp, const int32_t* count
   for (int l = 0; l < c.n_layers; ++l) {
     const flyai_layer_desc& L = st->layers[l];
     const int p = L.sliding ? 1 : 0;
+    LoraArgs lo_qkv, lo_o;
+    const LoraArgs *qkv_lora = nullptr, *o_lora = nullptr;
+    if (sp.lora) {
+      const int32_t* adapter = reinterpret_cast<const int32_t*>(blob + sp.off_adapter);
+      RUN(stage_lora_args(st, l, 0, adapter, I32(st->o_sid), sp.S, &lo_qkv));
+      RUN(stage_lora_args(st, l, 1, adapter, I32(st->o_sid), sp.S, &lo_o));
+      qkv_lora = &lo_qkv, o_lora = &lo_o;
+    }
     // xn holds this layer's input RMSNorm (written by the previous layer's combine)
-    RUN(launch_qkv_rope_kv(B16(st->o_xn), L.wqkv, L.bqkv, F32(st->o_gemm), I32(st->o_pos),
+    RUN(launch_qkv_rope_kv(B16(st->o_xn), L.wqkv, L.bqkv, planes, I32(st->o_pos),
                            I32(st->o_sid), st->cos_tab, st->sin_tab, c.rope_positions, Tn, H,
                            c.n_q_heads, c.n_kv_heads, c.head_dim, base_d, cap_d, B16(st->o_qrot),
-                           L.k_pool, L.v_pool, kv_pos, s));
+                           L.k_pool, L.v_pool, kv_pos, qkv_lora, s));
     if (sp.n_pitems[p] > 0 && !tree_d) {
       // prefill and split items share one launch (attn_step_kernel)
       RUN(launch_attn_step(B16(st->o_qrot), L.k_pool, L.v_pool, base_d, cap_d, L.sinks, L.sliding ? c.window : 0,
@@ -424,13 +509,13 @@ static int record_step(flyai_stage* st, const StepPlan& sp, const int32_t* count
       // decode-sized: o-proj finalize + residual + RMSNorm + router logits, then top-k + permute
       RUN(launch_linear_residual_rmsnorm_logits(B16(st->o_attn), L.wo, L.bo, Tn, H, c.n_q_heads * c.head_dim,
                                                 hidden, B16(st->o_h2), L.ln2, c.rms_eps, B16(st->o_xn),
-                                                F32(st->o_gemm), L.router_w, L.router_b, E,
-                                                F32(st->o_logits), s));
+                                                planes, L.router_w, L.router_b, E,
+                                                F32(st->o_logits), o_lora, s));
       RUN(launch_topk_permute(F32(st->o_logits), Tn, E, k, I32(st->o_ids), F32(st->o_w), I32(st->o_hist),
                               I32(st->o_off), I32(st->o_perm), I32(st->o_inv), s));
     } else {
       RUN(launch_linear_residual_rmsnorm(B16(st->o_attn), L.wo, L.bo, Tn, H, c.n_q_heads * c.head_dim,
-                                         hidden, L.ln2, c.rms_eps, B16(st->o_xn), F32(st->o_gemm), s));
+                                         hidden, L.ln2, c.rms_eps, B16(st->o_xn), planes, o_lora, s));
       RUN(launch_route_permute(B16(st->o_xn), L.router_w, L.router_b, Tn, H, E, k, I32(st->o_ids),
                                F32(st->o_w), F32(st->o_logits), I32(st->o_hist), I32(st->o_off),
                                I32(st->o_perm), I32(st->o_inv), s));
@@ -468,8 +553,8 @@ static int hip_fail(const char* what, hipError_t e) {
 
 // The executable graph for this step's key, captured on first use (least recently used evicted).
 static int step_graph(flyai_stage* st, const StepPlan& sp, hipGraphExec_t* out) {
-  const int64_t key[12] = {sp.Tn, sp.S, sp.grid_items[0], sp.grid_items[1], sp.grid_groups[0], sp.grid_groups[1],
-                           sp.n_pitems[0], sp.n_pitems[1], sp.merge[0], sp.merge[1], sp.lean[0], sp.lean[1]};
+  const int64_t key[13] = {sp.Tn, sp.S, sp.grid_items[0], sp.grid_items[1], sp.grid_groups[0], sp.grid_groups[1],
+                           sp.n_pitems[0], sp.n_pitems[1], sp.merge[0], sp.merge[1], sp.lean[0], sp.lean[1], sp.lora};
   ++st->use_clock;
   for (auto& g : st->graph_cache)
     if (memcmp(g.key, key, sizeof(key)) == 0) {
@@ -534,7 +619,7 @@ static int plan_needs_merge(const flyai_attn_group* groups, int n) {
 // launch (blob_fetch_kernel; an H2D copy if the staging is not mapped).
 static int stage_blob(flyai_stage* st, StepPlan& sp, const int32_t* q_lens, const int32_t* starts,
                       const int64_t* kv_base, const int32_t* kv_cap, const int* n_items,
-                      const int* n_groups, const std::vector<char>* tree, hipStream_t s) {
+                      const int* n_groups, const std::vector<char>* tree, const int32_t* adapter, hipStream_t s) {
   const int S = sp.S;
   Carve b;
   sp.off_counts = b.take(4 * sizeof(int32_t));
@@ -550,6 +635,8 @@ static int stage_blob(flyai_stage* st, StepPlan& sp, const int32_t* q_lens, cons
     sp.off_tree = b.take(tree->size());
     sp.off_tree_depth = sp.off_tree + reinterpret_cast<const flyai_attn_tree*>(tree->data())->depth_off;
   }
+  sp.lora = adapter != nullptr;
+  if (adapter) sp.off_adapter = b.take((size_t)S * 4);
   if (b.off > st->blob_max) return set_error(FLYAI_ERANGE, "batch blob exceeds its reservation");
   // wait until the GPU consumed this staging half's previous contents, then fill it
   const int h = st->half;
@@ -569,6 +656,7 @@ static int stage_blob(flyai_stage* st, StepPlan& sp, const int32_t* q_lens, cons
     memcpy(hb + sp.off_pitems[p], st->plan_pitems[p].data(), sp.n_pitems[p] * sizeof(flyai_attn_item));
   }
   if (tree) memcpy(hb + sp.off_tree, tree->data(), tree->size());
+  if (adapter) memcpy(hb + sp.off_adapter, adapter, (size_t)S * 4);
   if (st->host_dev)
     RUN(launch_blob_fetch(st->host_dev + h * st->host_half, st->dev + st->o_blob, b.off, s));
   else
@@ -606,9 +694,29 @@ static int check_slabs(flyai_stage* st, const int64_t* kv_base, const int32_t* k
   return FLYAI_OK;
 }
 
+// The adapters of a step's sequences: *used is null if there are none.
+static int check_adapters(const flyai_stage* st, const int32_t* adapter, int S, const int32_t** used) {
+  *used = nullptr;
+  if (!adapter) return FLYAI_OK;
+  for (int b = 0; b < S; ++b) {
+    if (adapter[b] == -1) continue;
+    FLYAI_REQUIRE(st->has_lora, "sequence %d has adapter %d and the stage has none (flyai_stage_set_lora)", b, adapter[b]);
+    FLYAI_REQUIRE(adapter[b] >= 0 && adapter[b] < st->lora.n_adapters, "sequence %d: adapter %d outside [-1, %d)", b, adapter[b],
+                  st->lora.n_adapters);
+    *used = adapter;
+  }
+  return FLYAI_OK;
+}
+
 extern "C" int flyai_stage_forward(flyai_stage* st, const int32_t* q_lens, const int32_t* starts,
                                    const int64_t* kv_base, const int32_t* kv_cap, int32_t S,
                                    uint16_t* hidden, flyai_stream_t stream) {
+  return flyai_stage_forward_lora(st, q_lens, starts, kv_base, kv_cap, nullptr, S, hidden, stream);
+}
+
+extern "C" int flyai_stage_forward_lora(flyai_stage* st, const int32_t* q_lens, const int32_t* starts,
+                                        const int64_t* kv_base, const int32_t* kv_cap, const int32_t* adapter, int32_t S,
+                                        uint16_t* hidden, flyai_stream_t stream) {
   FLYAI_REQUIRE(st && q_lens && starts && kv_base && kv_cap && hidden, "forward: null pointer");
   const flyai_stage_config& c = st->cfg;
   FLYAI_REQUIRE(S >= 1 && S <= c.max_seqs, "forward: n_seqs %d out of [1, %d]", S, c.max_seqs);
@@ -632,6 +740,7 @@ extern "C" int flyai_stage_forward(flyai_stage* st, const int32_t* q_lens, const
   for (int l = 0; l < c.n_layers; ++l)
     FLYAI_REQUIRE(st->layers[l].wqkv, "forward: layer %d not bound", l);
   RUN(check_slabs(st, kv_base, kv_cap, S));
+  RUN(check_adapters(st, adapter, S, &adapter));
   FLYAI_REQUIRE(st->dev && st->host, "forward: workspace not set");
   FLYAI_REQUIRE(st->cos_tab && st->sin_tab, "forward: rope tables not set");
   hipStream_t s = as_stream(stream);
@@ -653,7 +762,7 @@ extern "C" int flyai_stage_forward(flyai_stage* st, const int32_t* q_lens, const
     sp.merge[p] = plan_needs_merge(st->plan_groups[p].data(), n_groups[p]);
     sp.lean[p] = sp.n_small[p] == n_items[p];
   }
-  RUN(stage_blob(st, sp, q_lens, starts, kv_base, kv_cap, n_items, n_groups, nullptr, s));
+  RUN(stage_blob(st, sp, q_lens, starts, kv_base, kv_cap, n_items, n_groups, nullptr, adapter, s));
   if (!st->graphs) return record_step(st, sp, nullptr, hidden, s);
 
   hipGraphExec_t exec = nullptr;
@@ -674,6 +783,12 @@ extern "C" int flyai_stage_forward(flyai_stage* st, const int32_t* q_lens, const
 extern "C" int flyai_stage_forward_tree(flyai_stage* st, int32_t start, int32_t n, const int32_t* parent,
                                         const int32_t* depth, int64_t kv_base, int32_t kv_cap,
                                         uint16_t* hidden, flyai_stream_t stream) {
+  return flyai_stage_forward_tree_lora(st, start, n, parent, depth, kv_base, kv_cap, -1, hidden, stream);
+}
+
+extern "C" int flyai_stage_forward_tree_lora(flyai_stage* st, int32_t start, int32_t n, const int32_t* parent,
+                                             const int32_t* depth, int64_t kv_base, int32_t kv_cap, int32_t adapter_id,
+                                             uint16_t* hidden, flyai_stream_t stream) {
   FLYAI_REQUIRE(st && parent && depth && hidden, "forward_tree: null pointer");
   const flyai_stage_config& c = st->cfg;
   FLYAI_REQUIRE(n >= 1 && n <= st->tree_cap, "forward_tree: tree size %d outside [1, %d] (min(max_tokens, %d))", n,
@@ -701,6 +816,8 @@ extern "C" int flyai_stage_forward_tree(flyai_stage* st, int32_t start, int32_t 
   for (int l = 0; l < c.n_layers; ++l)
     FLYAI_REQUIRE(st->layers[l].wqkv, "forward_tree: layer %d not bound", l);
   RUN(check_slabs(st, &kv_base, &kv_cap, 1));
+  const int32_t* adapter = nullptr;
+  RUN(check_adapters(st, &adapter_id, 1, &adapter));
   FLYAI_REQUIRE(st->dev && st->host, "forward_tree: workspace not set");
   FLYAI_REQUIRE(st->cos_tab && st->sin_tab, "forward_tree: rope tables not set");
   // The two visibility masks (FastVerify._tset, phase0/fastverify.py:250-272): row i of mask 0 holds
@@ -759,6 +876,6 @@ extern "C" int flyai_stage_forward_tree(flyai_stage* st, int32_t start, int32_t 
     sp.lean[p] = 0;
   }
   const int32_t q_len = n, st0 = start;
-  RUN(stage_blob(st, sp, &q_len, &st0, &kv_base, &kv_cap, n_items, n_groups, &st->tree_img, s));
+  RUN(stage_blob(st, sp, &q_len, &st0, &kv_base, &kv_cap, n_items, n_groups, &st->tree_img, adapter, s));
   return record_step(st, sp, nullptr, hidden, s);
 }

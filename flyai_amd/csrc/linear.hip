@@ -755,12 +755,20 @@ bool gemm_tiled_lora_fits(int M, int K, const LoraArgs& a) {
   return gemm_is_tiled(M) && K % 64 == 0 && whole;
 }
 
-int launch_gemm_tiled_lora(const uint16_t* x, const uint16_t* W, const uint16_t* b, int M, int N, int K, uint16_t* y,
+// `out` NULL: bf16 rows to y or residual; otherwise the sums, up products included, as a plane.
+int launch_gemm_tiled_lora(const uint16_t* x, const uint16_t* W, const uint16_t* b, int M, int N, int K, float* out, uint16_t* y,
                            uint16_t* residual, const LoraArgs& a, hipStream_t s) {
   const int tiles = ceil_div(N, kTileN) * ceil_div(M, kTileM);
-  hipLaunchKernelGGL((gemm_tiled_lds_kernel<kEpiLinear, true>), dim3(8 * ceil_div(tiles, 8)), dim3(64 * kTiledWaves), 0, s, x, W, M,
-                     N, K, nullptr, QkvEpilogue{}, LinearEpilogue{b, y, residual}, a);
+  const auto kernel = out ? gemm_tiled_lds_kernel<kEpiPlane, true> : gemm_tiled_lds_kernel<kEpiLinear, true>;
+  hipLaunchKernelGGL(kernel, dim3(8 * ceil_div(tiles, 8)), dim3(64 * kTiledWaves), 0, s, x, W, M, N, K, out, QkvEpilogue{},
+                     LinearEpilogue{b, y, residual}, a);
   return check_launch("gemm_tiled_lora");
+}
+
+// launch_gemm, with the adapters' up products in the planes where the step has adapters.
+static int gemm_with(const LoraArgs* lo, const uint16_t* x, const uint16_t* W, int M, int N, int K, float* part, int* slices,
+                     hipStream_t s) {
+  return lo ? launch_gemm_lora_planes(x, W, M, N, K, part, slices, *lo, s) : launch_gemm(x, W, M, N, K, part, slices, s);
 }
 
 int launch_linear(const uint16_t* x, const uint16_t* W, const uint16_t* b, int M, int N, int K,
@@ -782,10 +790,10 @@ int launch_linear(const uint16_t* x, const uint16_t* W, const uint16_t* b, int M
 
 int launch_linear_residual_rmsnorm(const uint16_t* x, const uint16_t* W, const uint16_t* b, int M,
                                    int N, int K, uint16_t* h, const float* lnw, float eps,
-                                   uint16_t* xn, float* part, hipStream_t s) {
+                                   uint16_t* xn, float* part, const LoraArgs* lo, hipStream_t s) {
   if (M == 0) return FLYAI_OK;
   int slices = 0;
-  int rc = launch_gemm(x, W, M, N, K, part, &slices, s);
+  int rc = gemm_with(lo, x, W, M, N, K, part, &slices, s);
   if (rc) return rc;
   if (N > 7 * kRowThreads) return set_error(FLYAI_EINVAL, "residual_rmsnorm: H <= %d", 7 * kRowThreads);
   auto go = [&](auto iters, auto smax) {
@@ -813,12 +821,12 @@ int launch_linear_residual_rmsnorm_logits(const uint16_t* x, const uint16_t* W, 
                                           int N, int K, const uint16_t* h_in, uint16_t* h_out,
                                           const float* lnw, float eps, uint16_t* xn, float* part,
                                           const uint16_t* rw, const uint16_t* rb, int E, float* logits,
-                                          hipStream_t s) {
+                                          const LoraArgs* lo, hipStream_t s) {
   if (M == 0) return FLYAI_OK;
   if (M > kFusedRouteTokens || N > 7168 || N % 8 || E > 256)
     return set_error(FLYAI_EINVAL, "fused router logits: needs T <= 256, H %% 8 == 0, H <= 7168, E <= 256");
   int slices = 0;
-  int rc = launch_gemm(x, W, M, N, K, part, &slices, s);
+  int rc = gemm_with(lo, x, W, M, N, K, part, &slices, s);
   if (rc) return rc;
   auto go = [&](auto jmax, auto smax) {
     hipLaunchKernelGGL((residual_rmsnorm_logits_kernel<decltype(jmax)::value, decltype(smax)::value>),
@@ -1004,7 +1012,7 @@ int launch_qkv_rope_kv(const uint16_t* x, const uint16_t* Wqkv, const uint16_t* 
                        const int32_t* positions, const int32_t* seq_id, const uint16_t* cos_tab,
                        const uint16_t* sin_tab, int rope_positions, int T, int H, int Hq, int Hkv,
                        int D, const int64_t* kv_base, const int32_t* kv_cap, uint16_t* q_out,
-                       uint16_t* k_pool, uint16_t* v_pool, const int32_t* kv_pos, hipStream_t s) {
+                       uint16_t* k_pool, uint16_t* v_pool, const int32_t* kv_pos, const LoraArgs* lo, hipStream_t s) {
   if (T == 0) return FLYAI_OK;
   const int width = (Hq + 2 * Hkv) * D;
   if (T >= kTiledMinRows && H % 64 == 0 && D == 64 && !kv_pos) {
@@ -1012,12 +1020,21 @@ int launch_qkv_rope_kv(const uint16_t* x, const uint16_t* Wqkv, const uint16_t* 
     const int tiles = ceil_div(width, kTileN) * ceil_div(T, kTileM);
     const QkvEpilogue ep{bqkv, positions, seq_id, cos_tab, sin_tab, kv_base, kv_cap, q_out, k_pool, v_pool,
                          rope_positions, Hq, Hkv};
-    hipLaunchKernelGGL((gemm_tiled_lds_kernel<kEpiQkv, false>), dim3(8 * ceil_div(tiles, 8)), dim3(64 * kTiledWaves), 0, s, x,
-                       Wqkv, T, width, H, part, ep, LinearEpilogue{}, LoraArgs{});
-    return check_launch("gemm_tiled_lds_qkv");
+    if (lo && gemm_tiled_lora_fits(T, H, *lo)) {
+      const int rc = launch_lora_down(x, T, H, *lo, s);
+      if (rc) return rc;
+      hipLaunchKernelGGL((gemm_tiled_lds_kernel<kEpiQkv, true>), dim3(8 * ceil_div(tiles, 8)), dim3(64 * kTiledWaves), 0, s, x,
+                         Wqkv, T, width, H, part, ep, LinearEpilogue{}, *lo);
+      return check_launch("gemm_tiled_lds_qkv_lora");
+    }
+    if (!lo) {
+      hipLaunchKernelGGL((gemm_tiled_lds_kernel<kEpiQkv, false>), dim3(8 * ceil_div(tiles, 8)), dim3(64 * kTiledWaves), 0, s, x,
+                         Wqkv, T, width, H, part, ep, LinearEpilogue{}, LoraArgs{});
+      return check_launch("gemm_tiled_lds_qkv");
+    }
   }
   int slices = 0;
-  int rc = launch_gemm(x, Wqkv, T, width, H, part, &slices, s);
+  int rc = gemm_with(lo, x, Wqkv, T, width, H, part, &slices, s);
   if (rc) return rc;
   if (D % 8 == 0 && slices <= 16) {
     const int units = (Hq + Hkv) * (D / 8) + Hkv * (D / 4);

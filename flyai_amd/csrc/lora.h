@@ -22,6 +22,15 @@ struct LoraArgs {
   int2* meta;
 };
 
+// lora.hip: h alone; the projection's planes with the up products in them (in the tiled kernel's plane, or as one more)
+int launch_lora_down(const uint16_t* x, int M, int K, const LoraArgs& a, hipStream_t s);
+int launch_gemm_lora_planes(const uint16_t* x, const uint16_t* W, int M, int N, int K, float* part, int* slices, const LoraArgs& a,
+                            hipStream_t s);
+size_t lora_h_bytes(int M, int R, int n_seg);
+void lora_bind(LoraArgs* a, char* ws, int M);
+int make_lora_args(LoraArgs* out, const uint16_t* A, const uint16_t* B, const float* scale, const int32_t* ranks, int n, int R,
+                   const int32_t* segments, int n_seg, int N, const int32_t* adapter, const int32_t* row_seq, int n_seqs);
+
 constexpr int kLoraCols = 32;  // rank columns of one product: an MFMA's K
 
 __host__ __device__ inline int lora_cols(int R) { return (R + kLoraCols - 1) / kLoraCols * kLoraCols; }

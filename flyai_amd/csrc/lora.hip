@@ -8,8 +8,8 @@
 namespace flyai {
 
 int launch_gemm(const uint16_t* x, const uint16_t* W, int M, int N, int K, float* part, int* slices, hipStream_t s);
-int launch_gemm_tiled_lora(const uint16_t* x, const uint16_t* W, const uint16_t* b, int M, int N, int K, uint16_t* y, uint16_t* residual,
-                           const LoraArgs& a, hipStream_t s);
+int launch_gemm_tiled_lora(const uint16_t* x, const uint16_t* W, const uint16_t* b, int M, int N, int K, float* out, uint16_t* y,
+                           uint16_t* residual, const LoraArgs& a, hipStream_t s);
 bool gemm_tiled_lora_fits(int M, int K, const LoraArgs& a);
 bool gemm_is_tiled(int M);
 int gemm_planes(int M, int K);
@@ -158,7 +158,7 @@ static size_t align256(size_t v) { return (v + 255) & ~(size_t)255; }
 
 static size_t partial_bytes(int M, int N, int K) { return (size_t)gemm_planes(M, K) * M * N * sizeof(float); }
 
-static int launch_lora_down(const uint16_t* x, int M, int K, const LoraArgs& a, hipStream_t s) {
+int launch_lora_down(const uint16_t* x, int M, int K, const LoraArgs& a, hipStream_t s) {
   const int wgs = std::min(device_cus(), M * lora_down_groups(a));
   hipLaunchKernelGGL(lora_down_kernel, dim3(wgs), dim3(64 * kDownParts), 0, s, x, M, K, a);
   return check_launch("lora_down");
@@ -179,6 +179,21 @@ static int launch_gemm_lora(const uint16_t* x, const uint16_t* W, int M, int N, 
   return check_launch("gemm_splitk_lora");
 }
 
+int launch_gemm_lora_planes(const uint16_t* x, const uint16_t* W, int M, int N, int K, float* part, int* slices, const LoraArgs& a,
+                            hipStream_t s) {
+  if (gemm_tiled_lora_fits(M, K, a)) {
+    *slices = 1;
+    const int rc = launch_lora_down(x, M, K, a, s);
+    return rc ? rc : launch_gemm_tiled_lora(x, W, nullptr, M, N, K, part, nullptr, nullptr, a, s);
+  }
+  const int rc = launch_gemm_lora(x, W, M, N, K, part, slices, a, s);
+  if (rc) return rc;
+  hipLaunchKernelGGL(lora_finalize_kernel<true>, dim3(N / 16, ceil_div(M, 16)), dim3(256), 0, s, part, 0, M, N, a, nullptr, nullptr,
+                     nullptr, part + (size_t)*slices * M * N);
+  ++*slices;
+  return check_launch("lora_plane");
+}
+
 size_t lora_h_bytes(int M, int R, int n_seg) { return align256((size_t)M * n_seg * lora_cols(R) * 4) + align256((size_t)M * sizeof(int2)); }
 
 void lora_bind(LoraArgs* a, char* ws, int M) {
@@ -193,7 +208,7 @@ int launch_linear_lora(const uint16_t* x, const uint16_t* W, const uint16_t* b, 
   int slices = 0, rc;
   if (gemm_tiled_lora_fits(M, K, a)) {
     rc = launch_lora_down(x, M, K, a, s);
-    return rc ? rc : launch_gemm_tiled_lora(x, W, b, M, N, K, y, residual, a, s);
+    return rc ? rc : launch_gemm_tiled_lora(x, W, b, M, N, K, nullptr, y, residual, a, s);
   }
   rc = launch_gemm_lora(x, W, M, N, K, part, &slices, a, s);
   if (rc) return rc;

@@ -1,7 +1,7 @@
 """Stage runtimes over libflyai_stage: a ragged continuous-batch step, plus classes that keep the
 call surface of the reference's stage runtimes so they drop in for that path.
 
-* ``RaggedStage.forward(hidden, q_lens, starts, slots)`` -- one step over a flat token batch that
+* ``RaggedStage.forward(hidden, q_lens, starts, slots, adapters)`` -- one step over a flat token batch that
   mixes decode rows (q=1), spec-verify rows (q=K+1) and chunked-prefill rows (q=chunk).
 * ``FastVerifyStage`` -- ``FastVerify`` (phase0/fastverify.py:80-309): ``reset``, ``prefill(h, start)``,
   ``decode(h, start)``, ``tree_decode`` (ancestor-masked tree verify), ``tree_gather``; raises
@@ -128,8 +128,9 @@ class RaggedStage:
 
     def __init__(self, shape: GptOssShape, layers, rotary, kv: KVWorkspace, max_tokens, max_seqs,
                  max_attn_items=None, split_keys=1024, device="cuda", use_graphs=False, prefill_min=32,
-                 dense_fp8=False):
-        """dense_fp8: expert groups large enough for the dense kernels run on the scaled f8f6f4 MFMA with
+                 dense_fp8=False, lora=None):
+        """lora: an ``flyai_amd.lora.AdapterBank`` whose adapters ``forward`` and ``forward_tree`` take (``set_lora`` binds
+        one later).  dense_fp8: expert groups large enough for the dense kernels run on the scaled f8f6f4 MFMA with
         two-term fp8 activation operands (within fp32 accumulation order of the bf16 path, slower on
         groups of a 2048-token prefill chunk); the default keeps them on bf16 activations, bit-identical to the decode path."""
         self.shape, self.layers, self.rotary, self.kv = shape, layers, rotary, kv
@@ -162,6 +163,22 @@ class RaggedStage:
         self.set_workspace()
         self.use_graphs = False
         self.set_graphs(use_graphs)
+        self.lora = self._lora_ws = None
+        if lora is not None:
+            self.set_lora(lora)
+
+    def set_lora(self, bank):
+        """Bind an ``AdapterBank`` (None: unbind).  Drops every captured step graph."""
+        if bank is None:
+            check(lib().flyai_stage_set_lora(self._h, None))
+            self.lora = self._lora_ws = None
+            return
+        if bank.n_layers != len(self.layers) or bank.shape != self.shape:
+            raise ValueError("the adapter bank is of another shape or number of layers")
+        if bank.scale.device != self.workspace.device:
+            raise ValueError(f"the adapter bank is on {bank.scale.device}, the stage on {self.workspace.device}")
+        ws = bank.bind(self._h)
+        self.lora, self._lora_ws = bank, ws
 
     def set_layer(self, i, lw):
         """Bind layer i to the weights of ``lw`` and the workspace's layer-i KV pools.  Drops every
@@ -209,9 +226,11 @@ class RaggedStage:
                 pass
             self._destroy(h)
 
-    def forward(self, hidden, q_lens, starts, slots):
+    def forward(self, hidden, q_lens, starts, slots, adapters=None):
         """hidden bf16 [T, H] (packed token order, updated in place and returned); q_lens/starts/slots
-        per sequence (host ints).  Raises ContextOverflow before any write."""
+        per sequence (host ints); adapters: the bank's slot of each sequence, -1 or None for none (None: of all).  K/V that a
+        sequence shares (``KVWorkspace.fork``) belongs to the adapter it was computed with.  Raises ContextOverflow
+        before any write."""
         S = len(q_lens)
         if not (len(starts) == S == len(slots)):
             raise ValueError("q_lens, starts and slots must have one entry per sequence")
@@ -232,17 +251,24 @@ class RaggedStage:
         if np.any(need > lim):
             b = int(np.argmax(need > lim))
             raise ContextOverflow(_lib.FLYAI_ERANGE, f"sequence {b} needs {int(need[b])} positions > max_ctx {int(lim[b])}")
-        check(lib().flyai_stage_forward(
+        ad = None
+        if adapters is not None:
+            if len(adapters) != S:
+                raise ValueError("adapters must have one entry per sequence")
+            ad = np.ascontiguousarray([-1 if a is None else int(a) for a in adapters], dtype=np.int32)
+        check(lib().flyai_stage_forward_lora(
             self._h, ql.ctypes.data_as(C.c_void_p), st.ctypes.data_as(C.c_void_p),
-            base.ctypes.data_as(C.c_void_p), cap.ctypes.data_as(C.c_void_p), S,
+            base.ctypes.data_as(C.c_void_p), cap.ctypes.data_as(C.c_void_p),
+            None if ad is None else ad.ctypes.data_as(C.c_void_p), S,
             C.c_void_p(hidden.data_ptr()), C.c_void_p(torch.cuda.current_stream(self.device).cuda_stream)))
         return hidden
 
-    def forward_tree(self, hidden, start, par, dep, slot=0):
+    def forward_tree(self, hidden, start, par, dep, slot=0, adapter=None):
         """Tree verify of one sequence (``FastVerify.tree_decode``, phase0/fastverify.py:281-299):
         hidden bf16 [M, H] holds the M tree nodes (updated in place and returned); node i is rotated
         at position start + dep[i], its K/V goes to slot start + i and it attends the committed
-        prefix and its ancestors.  The caller validates the tree (``validate_tree``)."""
+        prefix and its ancestors, with the bank's slot ``adapter`` (None: none).  The caller validates the tree
+        (``validate_tree``)."""
         M = len(par)
         if hidden.dtype != torch.bfloat16 or not hidden.is_contiguous() or tuple(hidden.shape) != (M, self.shape.hidden):
             raise ValueError(f"hidden must be contiguous bf16 [{M}, {self.shape.hidden}]")
@@ -250,9 +276,9 @@ class RaggedStage:
             raise ValueError(f"slot {slot} out of range")
         pa = np.ascontiguousarray(par, dtype=np.int32)
         de = np.ascontiguousarray(dep, dtype=np.int32)
-        check(lib().flyai_stage_forward_tree(
+        check(lib().flyai_stage_forward_tree_lora(
             self._h, int(start), M, pa.ctypes.data_as(C.c_void_p), de.ctypes.data_as(C.c_void_p),
-            self.kv.base(int(slot)), self.kv.slot_cap(int(slot)), C.c_void_p(hidden.data_ptr()),
+            self.kv.base(int(slot)), self.kv.slot_cap(int(slot)), -1 if adapter is None else int(adapter), C.c_void_p(hidden.data_ptr()),
             C.c_void_p(torch.cuda.current_stream(self.device).cuda_stream)))
         return hidden
 

@@ -62,7 +62,8 @@ class GptOssModel:
     ``max_context`` positions."""
 
     def __init__(self, shape, layers, embed, norm_w, lm_head, rotary, max_jobs, max_context,
-                 max_step_rows, device="cuda"):
+                 max_step_rows, device="cuda", lora=None):
+        """lora: an ``AdapterBank`` whose adapters ``step`` takes."""
         self.shape, self.device = shape, torch.device(device)
         self.embed, self.norm_w = embed, norm_w
         self.vocab = int(embed.shape[0])
@@ -71,24 +72,24 @@ class GptOssModel:
         self.lm_packed = ops.bf16_tile_repack(lm_head)
         self.max_jobs, self.max_context, self.max_step_rows = max_jobs, max_context, max_step_rows
         self.kv = KVWorkspace(len(layers), max_jobs, max_context, shape.n_kv_heads, shape.head_dim, device)
-        self.stage = RaggedStage(shape, layers, rotary, self.kv, max_step_rows, max_jobs, device=device)
+        self.stage = RaggedStage(shape, layers, rotary, self.kv, max_step_rows, max_jobs, device=device, lora=lora)
         self.n_layers = len(layers)
 
     @property
     def per_job_state_bytes(self):
         return self.n_layers * 2 * self.kv.slab * 2
 
-    def step(self, chunks, starts, slots, pick):
+    def step(self, chunks, starts, slots, pick, adapters=None):
         """One ragged step.  chunks[i]: token ids fed for sequence i at positions starts[i]...; slots[i]
-        its KV slot; pick[i]: whether to return the greedy token after its last row.  Returns a list
-        with a token id (or None) per sequence."""
+        its KV slot; pick[i]: whether to return the greedy token after its last row; adapters[i]: its adapter's slot in the
+        bank, or None.  Returns a list with a token id (or None) per sequence."""
         q_lens = [len(c) for c in chunks]
         T = sum(q_lens)
         if T > self.max_step_rows:
             raise ValueError(f"step of {T} rows exceeds {self.max_step_rows}")
         flat = torch.tensor([t for c in chunks for t in c], dtype=torch.int32).to(self.device, non_blocking=True)
         h = ops.embed_gather(self.embed, flat)
-        self.stage.forward(h, q_lens, starts, slots)
+        self.stage.forward(h, q_lens, starts, slots, adapters)
         xn = ops.rmsnorm(h, self.norm_w, self.shape.rms_eps)
         ends = np.cumsum(q_lens) - 1
         rows = [int(ends[i]) for i in range(len(chunks)) if pick[i]]

@@ -521,6 +521,39 @@ typedef struct {
 int flyai_stage_forward_tree(flyai_stage* st, int32_t start, int32_t n_nodes,
                              const int32_t* parent_host, const int32_t* depth_host, int64_t kv_base,
                              int32_t kv_cap, uint16_t* hidden, flyai_stream_t stream);
+/* Adapters in a step: flyai_linear_lora_bf16 in place of each layer's q, k, v and output projections, for the
+ * sequences that have one.  flyai_stage_set_lora binds a bank of n_adapters (NULL unbinds it): scale fp32 and ranks
+ * int32 [n_adapters], max_rank R (16, 32, ..., 128), per layer A and B in flyai_linear_lora_bf16's layout (q, k and v are three
+ * segments), all device memory that the caller owns and may refill between steps, and a device workspace of
+ * flyai_stage_lora_workspace_bytes(st, R), 256-byte aligned.  It drops every captured step graph.
+ * flyai_stage_forward_lora is flyai_stage_forward with an adapter for each sequence (-1: none); a sequence's rows
+ * do not depend on the others' adapters, and with none they have flyai_stage_forward's bits.
+ * flyai_stage_forward_tree_lora is flyai_stage_forward_tree with one. */
+typedef struct {
+  const uint16_t* qkv_a;  /* bf16 [n_adapters, 3 R, H] */
+  const uint16_t* qkv_b;  /* bf16 [n_adapters, (Hq+2Hkv)*D, R] */
+  const uint16_t* o_a;    /* bf16 [n_adapters, R, Hq*D] */
+  const uint16_t* o_b;    /* bf16 [n_adapters, H, R] */
+} flyai_lora_layer;
+
+typedef struct {
+  int32_t n_adapters, max_rank;
+  const float* scale;
+  const int32_t* ranks;
+  const flyai_lora_layer* layers_host;  /* [n_layers], read before the call returns */
+  void* workspace;
+  size_t workspace_bytes;
+} flyai_stage_lora;
+
+size_t flyai_stage_lora_workspace_bytes(const flyai_stage* st, int32_t max_rank);
+int flyai_stage_set_lora(flyai_stage* st, const flyai_stage_lora* lora);
+int flyai_stage_forward_lora(flyai_stage* st, const int32_t* q_lens_host, const int32_t* starts_host,
+                             const int64_t* kv_base_host, const int32_t* kv_cap_host,
+                             const int32_t* adapter_host, int32_t n_seqs, uint16_t* hidden,
+                             flyai_stream_t stream);
+int flyai_stage_forward_tree_lora(flyai_stage* st, int32_t start, int32_t n_nodes,
+                                  const int32_t* parent_host, const int32_t* depth_host, int64_t kv_base,
+                                  int32_t kv_cap, int32_t adapter, uint16_t* hidden, flyai_stream_t stream);
 /* HIP-graph replay of flyai_stage_forward (the CUDA-graph capture of FastVerify.decode /
  * BatchedFastVerify.decode, phase0/fastverify.py:221-231, phase0/batchverify.py:180-190).  When
  * enabled, each step's kernels are one graph per (tokens, sequences, attention-plan capacity) key:

@@ -69,24 +69,25 @@ struct LoraDownLds {
   int adapter[kDownRows * TILES];       // -1 where the row has none, or one of rank 0
   int first[TILES + 1];                 // pairs before the tile
   int of_seq[64 * WAVES], rank_of[64 * WAVES];
-  int row[kDownRows];                   // the item's rows within its tile
+  int row[WAVES][kDownRows];            // the item's rows within its tile, for each wave
 };
 
 inline int lora_down_groups(const LoraArgs& a) { return a.n_seg * (lora_cols(a.R) / kDownCols); }
 
-// One wave's part of an item's product: NP * 16 gathered rows (l.row, n of them) against 32 rows of A from ar, over the
+// One wave's part of an item's product: up to 8 NX gathered rows (`row`, n of them) against 32 rows of A from ar, over the
 // 64-K groups [k0, k1): the sum of the parts before `mid` and from it on, each from zero.  D groups are in flight in
 // registers.
-template <int NP, int D, bool PAIR, typename Lds>
+template <int NX, int D, bool PAIR>
 __device__ __forceinline__ void lora_down_part(const uint16_t* __restrict__ x, const uint16_t* __restrict__ ar, int a_rows, int K,
-                                               int m0, int n, int k0, int mid, int k1, char* st, const Lds& l, f32x4_t (&acc)[4][2]) {
-  constexpr int NX = 2 * NP, NI = NX + kDownCols / 8;  // load instructions a group: 8 rows each
+                                               int m0, int n, int k0, int mid, int k1, char* st, const int* row, f32x4_t (&acc)[4][2]) {
+  constexpr int NP = (NX + 1) / 2;           // 16-row tiles (NX == 1: the upper half of one holds what LDS held, for nobody)
+  constexpr int NI = NX + kDownCols / 8;     // load instructions a group: 8 rows each
   const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
   const uint16_t* src[NI];
 #pragma unroll
   for (int i = 0; i < NI; ++i) {
     const int q = 8 * (i < NX ? i : i - NX) + (lane >> 3);
-    src[i] = i < NX ? x + (size_t)(m0 + l.row[min(q, n - 1)]) * K : ar + (size_t)min(q, a_rows - 1) * K;
+    src[i] = i < NX ? x + (size_t)(m0 + row[min(q, n - 1)]) * K : ar + (size_t)min(q, a_rows - 1) * K;
   }
   u32x4_t buf[D][NI];
   auto load = [&](u32x4_t (&b)[NI], int kg) __attribute__((always_inline)) {
@@ -94,7 +95,7 @@ __device__ __forceinline__ void lora_down_part(const uint16_t* __restrict__ x, c
     const int within = k + 64 <= K ? 7 : 3;  // the last group may have 32 K: the others are read again and not used
 #pragma unroll
     for (int i = 0; i < NI; ++i) {
-      const int c = (lane & 7) ^ (4 * (i & 1) + (lane >> 4));  // position lane % 8 holds chunk c: the row's swizzle
+      const int c = (lane & 7) ^ (4 * ((i < NX ? i : i - NX) & 1) + (lane >> 4));  // position lane % 8 holds chunk c: the row's swizzle
       b[i] = *reinterpret_cast<const u32x4_t*>(src[i] + k + 8 * (c & within));
     }
   };
@@ -119,7 +120,7 @@ __device__ __forceinline__ void lora_down_part(const uint16_t* __restrict__ x, c
         }
       }
 #pragma unroll
-      for (int i = 0; i < NI; ++i) *reinterpret_cast<u32x4_t*>(st + 1024 * i + 16 * lane) = buf[d][i];
+      for (int i = 0; i < NI; ++i) *reinterpret_cast<u32x4_t*>(st + 1024 * (i < NX ? i : i - NX + 2 * NP) + 16 * lane) = buf[d][i];
       asm volatile("" ::: "memory");  // this wave's LDS operations complete in order
       load(buf[d], kb + d + D);
       const bool half = 64 * (kb + d) + 64 > K;
@@ -128,7 +129,7 @@ __device__ __forceinline__ void lora_down_part(const uint16_t* __restrict__ x, c
         if (j == 1 && half) break;
         bf16x8_t av[2], xv[NP];
 #pragma unroll
-        for (int c = 0; c < 2; ++c) av[c] = as_bf16x8(*reinterpret_cast<const uint4*>(st + 1024 * NX + 2048 * c + (frag ^ (j << 6))));
+        for (int c = 0; c < 2; ++c) av[c] = as_bf16x8(*reinterpret_cast<const uint4*>(st + 2048 * NP + 2048 * c + (frag ^ (j << 6))));
 #pragma unroll
         for (int p = 0; p < NP; ++p) xv[p] = as_bf16x8(*reinterpret_cast<const uint4*>(st + 2048 * p + (frag ^ (j << 6))));
 #pragma unroll
@@ -159,68 +160,90 @@ __device__ __forceinline__ void lora_down(const uint16_t* __restrict__ x, int M,
   const int32_t* row_of = a.row_seq ? a.row_seq : a.adapter;
   // Rows, sequences and ranks are fetched side by side where the tables fit a workgroup: one round trip, not three.
   const bool small = a.n <= kThreads && (!a.row_seq || a.n_seqs <= kThreads);
+  // A decode batch, one tile: every wave has the tables in its lanes, and no barrier is needed.
+  const bool one = M <= kDownRows && a.n <= 64 && (!a.row_seq || a.n_seqs <= 64);
+  int key1 = -1, rank1 = 0, pairs1 = 0;
+  if (one) {
+    const int sq = row_of[min(lane, M - 1)];
+    const int of_seq = a.row_seq ? a.adapter[min(lane, a.n_seqs - 1)] : 0;
+    const int rank_of = min(max(a.ranks[min(lane, a.n - 1)], 0), a.R);
+    int ad = sq;
+    if (a.row_seq) {
+      ad = __builtin_amdgcn_ds_bpermute(4 * sq, of_seq);
+      if ((unsigned)sq >= (unsigned)a.n_seqs) ad = -1;
+    }
+    rank1 = __builtin_amdgcn_ds_bpermute(4 * ad, rank_of);
+    if ((unsigned)ad >= (unsigned)a.n || lane >= M) rank1 = 0;
+    key1 = rank1 > 0 ? ad : -1;
+    if (wg == 0 && tid < M) a.meta[tid] = make_int2(key1, rank1);
+    for (uint64_t todo = __ballot(key1 >= 0); todo; ++pairs1)
+      todo &= ~__ballot(key1 == __builtin_amdgcn_readlane(key1, __builtin_ctzll(todo)));
+  }
   for (int t0 = 0; t0 < M; t0 += kDownRows * TILES) {
     const int rows = min(M - t0, kDownRows * TILES), tiles = (rows + kDownRows - 1) / kDownRows;
-    if (t0) __syncthreads();
-    int fetched[kMine];
+    if (!one) {
+      if (t0) __syncthreads();
+      int fetched[kMine];
 #pragma unroll
-    for (int j = 0; j < kMine; ++j) fetched[j] = row_of[t0 + min(kDownRows * (wave + WAVES * j) + lane, rows - 1)];
-    if (t0 == 0 && small) {
-      if (tid < a.n) l.rank_of[tid] = min(max(a.ranks[tid], 0), a.R);
-      if (a.row_seq && tid < a.n_seqs) l.of_seq[tid] = a.adapter[tid];
-    }
-    if (tid == 0) l.first[0] = 0;
-    __syncthreads();
-#pragma unroll
-    for (int j = 0; j < kMine; ++j) {
-      const int t = wave + WAVES * j, i = kDownRows * t + lane;
-      if (t >= tiles) break;
-      int ad = fetched[j], rank = 0;
-      if (a.row_seq) {
-        const bool in = (unsigned)ad < (unsigned)a.n_seqs;
-        const int sq = in ? ad : 0;
-        ad = small ? l.of_seq[sq] : a.adapter[sq];
-        if (!in) ad = -1;
+      for (int j = 0; j < kMine; ++j) fetched[j] = row_of[t0 + min(kDownRows * (wave + WAVES * j) + lane, rows - 1)];
+      if (t0 == 0 && small) {
+        if (tid < a.n) l.rank_of[tid] = min(max(a.ranks[tid], 0), a.R);
+        if (a.row_seq && tid < a.n_seqs) l.of_seq[tid] = a.adapter[tid];
       }
-      if ((unsigned)ad < (unsigned)a.n) rank = small ? l.rank_of[ad] : min(max(a.ranks[ad], 0), a.R);
-      if (i >= rows || rank == 0) ad = -1;
-      l.adapter[i] = ad;
-      if (wg == 0 && i < rows) a.meta[t0 + i] = make_int2(ad, ad < 0 ? 0 : rank);
-      int n = 0;
-      for (uint64_t todo = __ballot(ad >= 0); todo; ++n)
-        todo &= ~__ballot(ad == __builtin_amdgcn_readlane(ad, __builtin_ctzll(todo)));
-      if (lane == 0) l.first[t + 1] = n;
-    }
-    __syncthreads();
-    if (wave == 0) {  // running sums
-      static_assert(TILES <= 64, "a lane a tile");
-      int sum = lane < tiles ? l.first[lane + 1] : 0;
+      if (tid == 0) l.first[0] = 0;
+      __syncthreads();
 #pragma unroll
-      for (int off = 1; off < TILES; off <<= 1) {
-        const int o = __shfl_up(sum, off, 64);
-        if (lane >= off) sum += o;
+      for (int j = 0; j < kMine; ++j) {
+        const int t = wave + WAVES * j, i = kDownRows * t + lane;
+        if (t >= tiles) break;
+        int ad = fetched[j], rank = 0;
+        if (a.row_seq) {
+          const bool in = (unsigned)ad < (unsigned)a.n_seqs;
+          const int sq = in ? ad : 0;
+          ad = small ? l.of_seq[sq] : a.adapter[sq];
+          if (!in) ad = -1;
+        }
+        if ((unsigned)ad < (unsigned)a.n) rank = small ? l.rank_of[ad] : min(max(a.ranks[ad], 0), a.R);
+        if (i >= rows || rank == 0) ad = -1;
+        l.adapter[i] = ad;
+        if (wg == 0 && i < rows) a.meta[t0 + i] = make_int2(ad, ad < 0 ? 0 : rank);
+        int n = 0;
+        for (uint64_t todo = __ballot(ad >= 0); todo; ++n)
+          todo &= ~__ballot(ad == __builtin_amdgcn_readlane(ad, __builtin_ctzll(todo)));
+        if (lane == 0) l.first[t + 1] = n;
       }
-      if (lane < tiles) l.first[lane + 1] = sum;
+      __syncthreads();
+      if (wave == 0) {  // running sums
+        static_assert(TILES <= 64, "a lane a tile");
+        int sum = lane < tiles ? l.first[lane + 1] : 0;
+#pragma unroll
+        for (int off = 1; off < TILES; off <<= 1) {
+          const int o = __shfl_up(sum, off, 64);
+          if (lane >= off) sum += o;
+        }
+        if (lane < tiles) l.first[lane + 1] = sum;
+      }
+      __syncthreads();
     }
-    __syncthreads();
-    const int items = __builtin_amdgcn_readfirstlane(l.first[tiles]) * groups;
-    const int before = l.first[min(lane, tiles)];
+    const int items = (one ? pairs1 : __builtin_amdgcn_readfirstlane(l.first[tiles])) * groups;
+    const int before = one ? 0 : l.first[min(lane, tiles)];
     for (int it = wg; it < items; it += wgs) {
       const int pair = it / groups, seg = it % groups / per_seg, c0 = it % groups % per_seg * kDownCols;
       const int tile = __builtin_popcountll(__ballot(lane < tiles && before <= pair)) - 1;  // the last that starts at or before it
       const int nth = pair - __builtin_amdgcn_readlane(before, tile);
       const int m0 = t0 + kDownRows * tile;
-      const int mine = l.adapter[kDownRows * tile + lane];
+      const int mine = one ? key1 : l.adapter[kDownRows * tile + lane];
       uint64_t todo = __ballot(mine >= 0);
       for (int i = 0; i < nth; ++i) todo &= ~__ballot(mine == __builtin_amdgcn_readlane(mine, __builtin_ctzll(todo)));
-      const int ad = __builtin_amdgcn_readlane(mine, __builtin_ctzll(todo));
+      const int lead = __builtin_ctzll(todo), ad = __builtin_amdgcn_readlane(mine, lead);
       const uint64_t rows_of = __ballot(mine == ad);
       const int n = __builtin_popcountll(rows_of);
-      const int rank = __builtin_amdgcn_readfirstlane(small ? l.rank_of[ad] : min(max(a.ranks[ad], 0), a.R));
+      const int rank = one ? __builtin_amdgcn_readlane(rank1, lead)
+                           : __builtin_amdgcn_readfirstlane(small ? l.rank_of[ad] : min(max(a.ranks[ad], 0), a.R));
       if (c0 >= rank) continue;  // the same in every wave: columns past the rank's last 32 are never read
       const float scale = a.scale[ad];
-      if (wave == 0 && mine == ad) l.row[__builtin_popcountll(rows_of & ((1ull << lane) - 1))] = lane;
-      __syncthreads();
+      if (mine == ad) l.row[wave][__builtin_popcountll(rows_of & ((1ull << lane) - 1))] = lane;
+      asm volatile("" ::: "memory");  // a wave's LDS operations complete in order
       f32x4_t acc[4][2];
 #pragma unroll
       for (int p = 0; p < 4; ++p) acc[p][0] = acc[p][1] = f32x4_t{0.f, 0.f, 0.f, 0.f};
@@ -228,9 +251,11 @@ __device__ __forceinline__ void lora_down(const uint16_t* __restrict__ x, int M,
       const int e = kPairs * wave, a_rows = min(rank - c0, kDownCols);
       const int k0 = KG * e / kDownParts, mid = kPairs == 2 ? KG * (e + 1) / kDownParts : -1, k1 = KG * (e + kPairs) / kDownParts;
       if (k0 == k1) {}  // fewer groups than waves
-      else if (n <= 16) lora_down_part<1, 4, kPairs == 2>(x, ar, a_rows, K, m0, n, k0, mid, k1, l.stage[wave], l, acc);
-      else if (n <= 32) lora_down_part<2, 2, kPairs == 2>(x, ar, a_rows, K, m0, n, k0, mid, k1, l.stage[wave], l, acc);
-      else lora_down_part<4, 1, kPairs == 2>(x, ar, a_rows, K, m0, n, k0, mid, k1, l.stage[wave], l, acc);
+      // the fewer rows, the more groups in flight: with few rows there are few items, and latency is all there is
+      else if (n <= 8) lora_down_part<1, kPairs == 2 ? 7 : 4, kPairs == 2>(x, ar, a_rows, K, m0, n, k0, mid, k1, l.stage[wave], l.row[wave], acc);
+      else if (n <= 16) lora_down_part<2, 4, kPairs == 2>(x, ar, a_rows, K, m0, n, k0, mid, k1, l.stage[wave], l.row[wave], acc);
+      else if (n <= 32) lora_down_part<4, 2, kPairs == 2>(x, ar, a_rows, K, m0, n, k0, mid, k1, l.stage[wave], l.row[wave], acc);
+      else lora_down_part<8, 1, kPairs == 2>(x, ar, a_rows, K, m0, n, k0, mid, k1, l.stage[wave], l.row[wave], acc);
       __syncthreads();  // red lies over the stages
       // lane (r, g): rank columns 4g .. +3 of row r
 #pragma unroll
@@ -254,7 +279,7 @@ __device__ __forceinline__ void lora_down(const uint16_t* __restrict__ x, int M,
         }
         const uint16_t hi = f2bf(v);
         const float rest = v - bf2f(hi);
-        uint16_t* o = a.h + ((size_t)(m0 + l.row[q]) * a.n_seg + seg) * 2 * cols + c0 + j;
+        uint16_t* o = a.h + ((size_t)(m0 + l.row[wave][q]) * a.n_seg + seg) * 2 * cols + c0 + j;
         o[0] = hi;
         o[cols] = rest == rest ? f2bf(rest) : 0;  // a value past bf16's range keeps its infinity: inf - inf would be NaN
       }

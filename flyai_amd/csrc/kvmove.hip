@@ -1,6 +1,5 @@
 // The cache's slabs forked and compacted: every layer, K and V, every kv head in one launch.
 #include <algorithm>
-#include <vector>
 
 #include "common.h"
 

@@ -250,12 +250,12 @@ extern "C" int flyai_linear_lora_bf16(const uint16_t* x, const uint16_t* w, cons
                                       const int32_t* ranks, int32_t n_adapters, int32_t R, const int32_t* segments_host,
                                       int32_t n_segments, const int32_t* adapter, const int32_t* row_seq, int32_t n_seqs,
                                       uint16_t* y, uint16_t* residual, void* workspace, flyai_stream_t stream) {
-  FLYAI_REQUIRE(M >= 0 && M <= (1 << 20) && N > 0 && K > 0 && N % 16 == 0 && K % 32 == 0 && K <= 8192,
-                "linear_lora: need M <= %d, N %% 16 == 0, K %% 32 == 0, K <= 8192", 1 << 20);
+  FLYAI_REQUIRE(M >= 0 && M <= (1 << 19) && N > 0 && K > 0 && N % 16 == 0 && K % 32 == 0 && K <= 8192,
+                "linear_lora: need M <= %d, N %% 16 == 0, K %% 32 == 0, K <= 8192", 1 << 19);
   if (M == 0) return FLYAI_OK;  // an empty tensor has no address
   FLYAI_REQUIRE(x && w && (y || residual) && workspace, "linear_lora: null pointer");
-  FLYAI_REQUIRE(((uintptr_t)x | (uintptr_t)w | (uintptr_t)b | (uintptr_t)y | (uintptr_t)residual | (uintptr_t)workspace) % 16 == 0,
-                "linear_lora: pointers must be 16-byte aligned");
+  FLYAI_REQUIRE(((uintptr_t)x | (uintptr_t)w | (uintptr_t)y | (uintptr_t)residual | (uintptr_t)workspace) % 16 == 0,
+                "linear_lora: x, w, y, residual and workspace must be 16-byte aligned");
   LoraArgs a;
   const int rc = make_lora_args(&a, lora_a, lora_b, scale, ranks, n_adapters, R, segments_host, n_segments, N, adapter, row_seq,
                                 n_seqs);

@@ -395,7 +395,7 @@ def rope(x, positions, inv_freq, layout="half", scaling=1.0, inverse=False, out=
     of fused projection rows): dims [0, 2 * len(inv_freq)) of each head are turned by positions[t] * inv_freq[i] (int32 [T],
     fp64; ``rope.rope_frequencies`` gives scaled ones) and multiplied by scaling, the others copied.  Pairs are (i, i +
     rot/2) ("half") or (2i, 2i + 1) ("interleaved").  inverse turns back: the gradient of the rotation.  out: a tensor
-    of x's shape and type (x itself: in place; otherwise it must not overlap x), None: a new contiguous one."""
+    of x's shape and type (x itself: in place; otherwise wholly before or behind x in memory), None: a new contiguous one."""
     if not isinstance(x, torch.Tensor) or x.dim() != 3:
         raise ValueError("x must be a [T, H, D] tensor")
     dev = x.get_device()
@@ -419,7 +419,7 @@ def rope(x, positions, inv_freq, layout="half", scaling=1.0, inverse=False, out=
         raise ValueError("the last dim of x and out must be contiguous")
     if T == 0 or H == 0:
         return out
-    _on(dev, lib().flyai_rope, x.data_ptr(), xt, xh, positions.data_ptr(), inv_freq.data_ptr(), scaling, T, H, D, 2 * pairs,
+    _on(dev, lib().flyai_rope, x.data_ptr(), xt, xh, positions.data_ptr(), inv_freq.data_ptr(), float(scaling), T, H, D, 2 * pairs,
         dtype, _ROPE_LAYOUTS[layout], 1 if inverse else 0, out.data_ptr(), ot, oh)
     return out
 
@@ -449,8 +449,8 @@ def kv_fork(k, v, n_kv_heads, src, dsts, lo, hi, src_k=None, src_v=None):
         if sL != L or sdev != dev:
             raise ValueError(f"the source's pools have {sL} layers on device {sdev}, the others {L} on {dev}")
     slabs = _packed(_KV_SLAB, [(b, c, 0) for b, c in (src, *dsts)])
-    _on(dev, lib().flyai_kv_fork, src_k.data_ptr(), src_v.data_ptr(), sn, sn, k.data_ptr(), v.data_ptr(), n, n, L, n_kv_heads,
-        64, slabs[:_KV_SLAB.size], slabs[_KV_SLAB.size:], len(dsts), lo, hi)
+    _on(dev, lib().flyai_kv_fork, src_k.data_ptr(), src_v.data_ptr(), sn, sn, k.data_ptr(), v.data_ptr(), n, n, L, int(n_kv_heads),
+        64, slabs[:_KV_SLAB.size], slabs[_KV_SLAB.size:], len(dsts), int(lo), int(hi))
 
 
 def _host_positions(keep):
@@ -482,7 +482,7 @@ def kv_compact(k, v, n_kv_heads, moves):
     L, n, dev = _kv_pools(k, v)
     keeps = [_host_positions(m[3]) for m in moves]
     rows = _packed(_KV_MOVE, [(base, cap, start, len(a) // 4, 0) for (base, cap, start, _), a in zip(moves, keeps)])
-    _on(dev, lib().flyai_kv_compact, k.data_ptr(), v.data_ptr(), n, n, L, n_kv_heads, 64, rows, len(moves), b"".join(keeps))
+    _on(dev, lib().flyai_kv_compact, k.data_ptr(), v.data_ptr(), n, n, L, int(n_kv_heads), 64, rows, len(moves), b"".join(keeps))
 
 
 # ---- DeepSeek-V3-shaped FP8 MoE ------------------------------------------------------------------

@@ -318,8 +318,9 @@ int flyai_attn_prefill(const uint16_t* q, const uint16_t* k_pool, const uint16_t
  * row t, or with row_seq int32 [M] of row t's sequence (adapter[row_seq[t]], n_seqs entries); an adapter
  * outside [0, n_adapters) or a sequence outside [0, n_seqs) means none.  With residual the result is bf16(residual +
  * y), written to residual.  A row's result depends on that row alone: not on its batch, nor on what other
- * rows' adapters hold.  Pointers to bf16 are 16-byte aligned.  workspace: flyai_linear_lora_workspace_bytes,
- * 16-byte aligned; two calls that may overlap need one each.  N % 16 == 0, K % 32 == 0, K <= 8192. */
+ * rows' adapters hold.  All bf16 matrices and the workspace are 16-byte aligned (b need not be).  workspace:
+ * flyai_linear_lora_workspace_bytes; two calls that may overlap need one each.  M <= 524288, N % 16 == 0,
+ * K % 32 == 0, K <= 8192. */
 size_t flyai_linear_lora_workspace_bytes(int32_t M, int32_t N, int32_t K, int32_t R, int32_t n_segments);
 int flyai_linear_lora_bf16(const uint16_t* x, const uint16_t* w, const uint16_t* b, int32_t M, int32_t N,
                            int32_t K, const uint16_t* lora_a, const uint16_t* lora_b, const float* scale,
@@ -332,7 +333,7 @@ int flyai_linear_lora_bf16(const uint16_t* x, const uint16_t* w, const uint16_t*
  * token and head strides in elements): dims [0, rot) of every head are turned by the angles
  * positions[t] * inv_freq[i] (int32 [T], fp64 [rot / 2]) and scaled, the others copied.  Pair i is dims
  * (i, i + rot/2), or with interleaved (2i, 2i + 1).  inverse turns the other way: the gradient.  out may be x
- * with x's strides, or must not overlap it.  Any int32 position: the angle is computed in 64 bits.  T and H * D
+ * with x's strides, or lies wholly before or behind it in memory.  Any int32 position: the angle is computed in 64 bits.  T and H * D
  * at most 2^22, rot at most 2048. */
 #define FLYAI_BF16 0
 #define FLYAI_F16 1

@@ -90,6 +90,10 @@ SHAPES = [  # M, K, segments, adapters, R
     (257, 96, (144, 16), 3, 32),
     (300, 2880, (512, 64, 64), 40, 64),
     (700, 1056, (272,), 2, 112),
+    (40, 64, (32,), 70, 16),        # more adapters than a wave's lanes
+    (290, 96, (48,), 300, 16),      # more than a workgroup's threads
+    (700, 64, (64,), 600, 16),
+    (4500, 64, (32, 32), 5, 32),    # more rows than a workgroup lists at once
 ]
 
 
@@ -119,6 +123,19 @@ def test_rows_by_sequence(M):
     seq = torch.arange(M, device=DEV, dtype=torch.int32) * 8 // M - 1          # -1 .. 6
     rows = torch.where((seq >= 0) & (seq < 6), of_seq[seq.clamp(0, 5).long()], -1).to(torch.int32)
     assert torch.equal(_run(c, of_seq, row_seq=seq), _run(c, rows))
+
+
+@pytest.mark.parametrize("M,n_seqs", [(50, 65), (200, 300), (900, 700)])
+def test_many_sequences(M, n_seqs):
+    """More sequences than a wave's lanes, a workgroup's threads, and the tiled kernel's: the bits of adapters of rows."""
+    c = _inputs(M, 128, (64, 16), 7, 16, 14)
+    of_seq = _adapters(n_seqs, 7, 15)
+    g = torch.Generator().manual_seed(16)
+    seq = torch.randint(0, n_seqs, (M,), generator=g, dtype=torch.int32).to(DEV)
+    rows = of_seq[seq.long()].contiguous()
+    got = _run(c, of_seq, row_seq=seq)
+    assert torch.equal(got, _run(c, rows))
+    _check(got, c, rows)
 
 
 @pytest.mark.parametrize("M", [1, 40, 90, 137, 255, 256, 600])
@@ -218,6 +235,18 @@ def test_captured(M):
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(y, _run(c, adapter))
+
+
+def test_unaligned_bias_and_views():
+    """A bias that starts anywhere; matrices and rows must start at 16 bytes."""
+    c = _inputs(70, 64, (32,), 2, 16, 17)
+    adapter = _adapters(70, 2, 17)
+    want = _run(c, adapter)
+    c["b"] = torch.cat([c["b"][:1], c["b"]])[1:]
+    assert c["b"].data_ptr() % 16 and torch.equal(_run(c, adapter), want)
+    c["x"] = torch.cat([c["x"].view(-1)[:1], c["x"].view(-1)])[1:].view(70, 64)
+    with pytest.raises(RuntimeError, match="aligned"):
+        _run(c, adapter)
 
 
 def test_refusals():

@@ -24,7 +24,7 @@ def _lora(lib, M=4, N=48, K=64, n=2, R=16, segments=(32, 16), x=PTR, a=PTR, adap
 
 
 @pytest.mark.parametrize("change", [
-    {"M": -1}, {"M": (1 << 20) + 1}, {"N": 40}, {"K": 48}, {"K": 8224}, {"n": 0}, {"R": 8}, {"R": 24}, {"R": 144},
+    {"M": -1}, {"M": (1 << 19) + 1}, {"N": 40}, {"K": 48}, {"K": 8224}, {"n": 0}, {"R": 8}, {"R": 24}, {"R": 144},
     {"segments": (48, 8)}, {"segments": (24, 24)}, {"segments": (32,)}, {"segments": (16, 16, 16, 16)}, {"segments": (64, -16)},
     {"segments": (2 ** 31 - 16, 2 ** 31 - 16)}, {"segments": (16,) * 5}, {"x": None}, {"x": ODD}, {"a": ODD}, {"a": None}, {"adapter": None},
     {"row_seq": PTR, "n_seqs": 0}, {"y": None}, {"ws": None}, {"ws": ODD}])

@@ -47,7 +47,8 @@ __device__ __forceinline__ int lora_segment(const LoraArgs& a, int f) {
 // The batch's work is the pairs of a 64-row tile and an adapter among its rows, times the groups of 32 rank columns in
 // every segment.  Each workgroup lists the pairs for itself (adapters of up to 64 * TILES rows in LDS, and how many distinct
 // ones each tile has) and takes every wgs-th item: none is launched in vain, whatever the mix.
-// An item multiplies the tile's rows that have the adapter, gathered, 16 to an MFMA tile, with 32 rows of A.  K is cut into
+// An item multiplies the tile's rows that have the adapter, gathered, 16 to an MFMA tile, or (split) a half or a quarter of
+// them where the batch has few tiles, with 32 rows of A.  K is cut into
 // eight parts, summed in pairs and then in order through LDS, a wave one part or (with four waves) a pair of them; lane
 // (r, g) of an MFMA holds row r in its second operand, so a row's products never meet another row's: a row's h depends
 // neither on its tile nor on the launch.
@@ -225,10 +226,15 @@ __device__ __forceinline__ void lora_down(const uint16_t* __restrict__ x, int M,
       }
       __syncthreads();
     }
-    const int items = (one ? pairs1 : __builtin_amdgcn_readfirstlane(l.first[tiles])) * groups;
+    const int pairs = one ? pairs1 : __builtin_amdgcn_readfirstlane(l.first[tiles]);
+    // few items of many rows are split as far as the workgroups last: 512 rows of one adapter of 192 rank columns are 48 items
+    // of 64 rows, 14.1 us, or 192 of 16, 10.4
+    const int split = rows < 32 * pairs ? 1 : 4 * pairs * groups <= wgs ? 4 : 2 * pairs * groups <= wgs ? 2 : 1;
+    const int items = pairs * groups * split;
     const int before = one ? 0 : l.first[min(lane, tiles)];
     for (int it = wg; it < items; it += wgs) {
-      const int pair = it / groups, seg = it % groups / per_seg, c0 = it % groups % per_seg * kDownCols;
+      const int q0 = it % split * (kDownRows / split), ig = it / split;  // the first of the item's rows
+      const int pair = ig / groups, seg = ig % groups / per_seg, c0 = ig % groups % per_seg * kDownCols;
       const int tile = __builtin_popcountll(__ballot(lane < tiles && before <= pair)) - 1;  // the last that starts at or before it
       const int nth = pair - __builtin_amdgcn_readlane(before, tile);
       const int m0 = t0 + kDownRows * tile;
@@ -237,12 +243,13 @@ __device__ __forceinline__ void lora_down(const uint16_t* __restrict__ x, int M,
       for (int i = 0; i < nth; ++i) todo &= ~__ballot(mine == __builtin_amdgcn_readlane(mine, __builtin_ctzll(todo)));
       const int lead = __builtin_ctzll(todo), ad = __builtin_amdgcn_readlane(mine, lead);
       const uint64_t rows_of = __ballot(mine == ad);
-      const int n = __builtin_popcountll(rows_of);
+      const int n = min(__builtin_popcountll(rows_of) - q0, kDownRows / split);
       const int rank = one ? __builtin_amdgcn_readlane(rank1, lead)
                            : __builtin_amdgcn_readfirstlane(small ? l.rank_of[ad] : min(max(a.ranks[ad], 0), a.R));
-      if (c0 >= rank) continue;  // the same in every wave: columns past the rank's last 32 are never read
+      if (n <= 0 || c0 >= rank) continue;  // the same in every wave: columns past the rank's last 32 are never read
       const float scale = a.scale[ad];
-      if (mine == ad) l.row[wave][__builtin_popcountll(rows_of & ((1ull << lane) - 1))] = lane;
+      const int at = __builtin_popcountll(rows_of & ((1ull << lane) - 1)) - q0;
+      if (mine == ad && at >= 0) l.row[wave][at] = lane;
       asm volatile("" ::: "memory");  // a wave's LDS operations complete in order
       f32x4_t acc[4][2];
 #pragma unroll

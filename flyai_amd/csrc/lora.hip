@@ -26,132 +26,112 @@ __global__ __launch_bounds__(64 * kDownParts) void lora_down_kernel(const uint16
 // ---- up, and the projection's finalize ---------------------------------------------------------------------------
 // y = bf16(sum of the projection's planes + h B^T + bias); or, without planes, h B^T as a plane of its own for another
 // finalize to add (-0 where a row has no adapter: x + -0 is x).
-// A workgroup takes 16 rows x 16 features.  Its four waves share the adapters among the rows: each multiplies the whole
-// tile with its own, and the adapter's rows keep the result.  h and B come in whole 128-byte runs and are turned round in
-// LDS (the tiled GEMM's swizzle): as MFMA operands from memory, 16 rows of 64 bytes an instruction, they took 5 of the
-// 10 us at 48 rows of 12 adapters.
-constexpr int kUpCols = 64;  // rank columns a pass
-constexpr int kUpMine = 4;   // adapters a wave: 16 rows have at most 16
-
-struct LoraUpLds {
-  char h[2][16 * 128];               // high and low terms: 16 rows of 64 columns
-  char b[4][kUpMine][16 * 128];      // a wave's adapters: 16 features of 64 columns
-  float d[16][17];
-};
-
+// A wave takes 16 rows x 16 features and all of the rows' adapters, one after the other, the next one's columns on their way
+// under the products: it multiplies the whole tile with an adapter, and the adapter's rows keep the result.  h and B come in
+// whole 128-byte runs and are turned round in the wave's own LDS (the tiled GEMM's swizzle; as MFMA operands from memory, 16
+// rows of 64 bytes an instruction, they were half of the time).  Nothing is shared, so there is no barrier.  Lane (r, g) holds
+// features 4g .. +3 of row r from the planes to the result.
+// 5,120 features, R = 64: 4.0 us for 1 row, 7.5 for 48 rows of 12 adapters, 8.6 for 200 rows (8 KB a row); what bounds it is a
+// chain of three round trips at few rows, the planes' bytes at many.  The four waves of a workgroup sharing 16 features'
+// adapters took 4.2, 8.0 and 16.4.
 template <bool PLANE>
-__global__ __launch_bounds__(256, 4) void lora_finalize_kernel(const float* __restrict__ part, int slices, int M, int N,
-                                                            LoraArgs a, const uint16_t* __restrict__ b,
-                                                            uint16_t* __restrict__ y, uint16_t* __restrict__ residual,
-                                                            float* __restrict__ plane_out) {
-  __shared__ __align__(1024) LoraUpLds l;
+__global__ __launch_bounds__(256) void lora_finalize_kernel(const float* __restrict__ part, int slices, int M, int N,
+                                                                 LoraArgs a, const uint16_t* __restrict__ b,
+                                                                 uint16_t* __restrict__ y, uint16_t* __restrict__ residual,
+                                                                 float* __restrict__ plane_out) {
+  __shared__ __align__(1024) char stage[4][3 * 2048];  // a wave's h (high terms, low terms), an adapter's columns
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = lane & 15, g = lane >> 4;
-  const int f0 = blockIdx.x * 16, m0 = blockIdx.y * 16;
-  const int cols = lora_cols(a.R), seg = lora_segment(a, f0);
-  int2 who = a.meta[min(m0 + r, M - 1)];
-  // h: the wave's four rows, 16 lanes each, 8 chunks of the high terms and 8 of the low ones
-  const int hq = 4 * wave + (lane >> 4), hc = (lane & 7) ^ ((hq >> 1) & 7);
-  const uint16_t* hp = a.h + ((size_t)min(m0 + hq, M - 1) * a.n_seg + seg) * 2 * cols + (lane & 8 ? cols : 0);
-  u32x4_t hv = *reinterpret_cast<const u32x4_t*>(hp + min(8 * hc, cols - 8));
-  // this thread's output: row 4 * wave + lane / 16, feature lane % 16
-  const int mine = 4 * wave + (lane >> 4), row = m0 + mine;
-  const size_t idx = (size_t)min(row, M - 1) * N + f0 + r, plane = (size_t)M * N;
-  float p[8];
-  uint16_t bias = 0, res = 0;
+  const int f0 = (blockIdx.x * 4 + wave) * 16, m0 = blockIdx.y * 16;
+  if (f0 >= N) return;
+  char* l = stage[wave];
+  const int cols = lora_cols(a.R), seg = lora_segment(a, f0), row = m0 + r;
+  const int2 who = a.meta[min(row, M - 1)];
+  u32x4_t hv[4];  // 8 rows an instruction
+#pragma unroll
+  for (int k = 0; k < 4; ++k)
+    hv[k] = *reinterpret_cast<const u32x4_t*>(a.h + ((size_t)min(m0 + 8 * (k & 1) + (lane >> 3), M - 1) * a.n_seg + seg) * 2 * cols +
+                                              (k & 2 ? cols : 0) + lora_chunk(8 * (k & 1), 0, cols));
+  const size_t idx = (size_t)min(row, M - 1) * N + f0 + 4 * g, plane = (size_t)M * N;
+  f32x4_dw p[8];
+  u16x4_h bias, res;
   if constexpr (!PLANE) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) p[i] = part[min(i, slices - 1) * plane + idx];
+    for (int i = 0; i < 8; ++i) p[i] = *reinterpret_cast<const f32x4_dw*>(part + min(i, slices - 1) * plane + idx);
     // no load under a branch: its wait would be for everything before it
-    bias = *(b ? b + f0 + r : a.B);
-    res = *(residual ? residual + idx : a.B);
+    bias = *reinterpret_cast<const u16x4_h*>(b ? b + f0 + 4 * g : a.B);
+    res = *reinterpret_cast<const u16x4_h*>(residual ? residual + idx : a.B);
   }
-  if (m0 + r >= M) who.y = 0;
-  const bool has = __builtin_amdgcn_ds_bpermute(4 * mine, who.y) > 0;
-  const int key = who.y > 0 ? who.x : -1;
-  bool fresh = key >= 0;  // the first of its adapter's rows
+  const int key = row < M && who.y > 0 ? who.x : -1;
+  uint64_t todo = __ballot(key >= 0) & 0xffff;
+  f32x4_t d = {-0.f, -0.f, -0.f, -0.f};
+  if (todo) {
+    int ad = -1, rank = 0;
+    u32x4_t nb[2];
+    auto next = [&]() __attribute__((always_inline)) {
+      ad = -1;
+      if (!todo) return;
+      const int first = __builtin_ctzll(todo);
+      ad = __builtin_amdgcn_readlane(key, first), rank = __builtin_amdgcn_readlane(who.y, first);
+      todo &= ~__ballot(key == ad);
 #pragma unroll
-  for (int i = 0; i < 15; ++i) fresh &= i >= r || __builtin_amdgcn_readlane(key, i) != key;
-  uint64_t firsts = __ballot(fresh) & 0xffff;
-  const int n = __builtin_popcountll(firsts);
-  if (n > 0) {
-    // the wave's adapters: every fourth
-    for (int i = 0; i < wave; ++i) firsts &= firsts - 1;
-    int ads[kUpMine], ranks[kUpMine];
+      for (int i = 0; i < 2; ++i)
+        nb[i] = *reinterpret_cast<const u32x4_t*>(a.B + ((size_t)ad * N + f0 + 8 * i + (lane >> 3)) * a.R + lora_chunk(8 * i, 0, a.R));
+    };
+    next();
 #pragma unroll
-    for (int s = 0; s < kUpMine; ++s) {
-      const int at = __builtin_ctzll(firsts | 1ull << 63);
-      ads[s] = firsts ? __builtin_amdgcn_readlane(who.x, at & 15) : -1;
-      ranks[s] = firsts ? __builtin_amdgcn_readlane(who.y, at & 15) : 0;
-      for (int i = 0; i < 4; ++i) firsts &= firsts - 1;
-    }
-    f32x4_t acc[kUpMine];
-#pragma unroll
-    for (int s = 0; s < kUpMine; ++s) acc[s] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-    int top = who.y;  // the largest rank of the tile: the same in every wave
-#pragma unroll
-    for (int off = 1; off < 16; off <<= 1) top = max(top, __shfl_xor(top, off, 64));
-    top = __builtin_amdgcn_readfirstlane(top);
+    for (int k = 0; k < 4; ++k) *reinterpret_cast<u32x4_t*>(l + 1024 * k + 16 * lane) = hv[k];
     const int frag = r * 128 + ((g ^ ((r >> 1) & 7)) << 4);
-    for (int c0 = 0; c0 < top; c0 += kUpCols) {
-      if (c0) {
-        __syncthreads();
-        hv = *reinterpret_cast<const u32x4_t*>(hp + min(c0 + 8 * hc, cols - 8));
-      }
-      u32x4_t bv[kUpMine][2];
+    while (ad >= 0) {
+      const int now = ad, cur = rank;
+      asm volatile("" ::: "memory");  // a wave's LDS operations complete in order
 #pragma unroll
-      for (int s = 0; s < kUpMine; ++s)
-        if (c0 < ranks[s]) {
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {  // 8 features an instruction
-            const int q = 8 * i + (lane >> 3), c = (lane & 7) ^ ((q >> 1) & 7);
-            bv[s][i] = *reinterpret_cast<const u32x4_t*>(a.B + ((size_t)ads[s] * N + f0 + q) * a.R + min(c0 + 8 * c, a.R - 8));
-          }
+      for (int i = 0; i < 2; ++i) *reinterpret_cast<u32x4_t*>(l + 4096 + 1024 * i + 16 * lane) = nb[i];
+      asm volatile("" ::: "memory");
+      next();
+      f32x4_t acc = {0.f, 0.f, 0.f, 0.f};
+      for (int c = 0; kLoraCols * c < cur; ++c) {
+        const int left = cur - kLoraCols * c;
+        uint4 raw, hi, lo;
+        if (c < 2) {
+          raw = *reinterpret_cast<const uint4*>(l + 4096 + (frag ^ (c << 6)));
+          hi = *reinterpret_cast<const uint4*>(l + (frag ^ (c << 6)));
+          lo = *reinterpret_cast<const uint4*>(l + 2048 + (frag ^ (c << 6)));
+        } else {  // ranks past 64: straight from memory
+          const uint16_t* hr = a.h + ((size_t)min(row, M - 1) * a.n_seg + seg) * 2 * cols + kLoraCols * c + 8 * g;
+          raw = *reinterpret_cast<const uint4*>(a.B + ((size_t)now * N + f0 + r) * a.R + lora_col(a.R, c, g));
+          hi = *reinterpret_cast<const uint4*>(hr), lo = *reinterpret_cast<const uint4*>(hr + cols);
         }
-      *reinterpret_cast<u32x4_t*>(l.h[lane >> 3 & 1] + hq * 128 + 16 * (lane & 7)) = hv;
-#pragma unroll
-      for (int s = 0; s < kUpMine; ++s)
-        if (c0 < ranks[s]) {
-#pragma unroll
-          for (int i = 0; i < 2; ++i) *reinterpret_cast<u32x4_t*>(l.b[wave][s] + 1024 * i + 16 * lane) = bv[s][i];
-        }
-      __syncthreads();
-#pragma unroll
-      for (int c = 0; c < kUpCols / kLoraCols; ++c) {
-        const bf16x8_t hi = as_bf16x8(*reinterpret_cast<const uint4*>(l.h[0] + (frag ^ (c << 6))));
-        const bf16x8_t lo = as_bf16x8(*reinterpret_cast<const uint4*>(l.h[1] + (frag ^ (c << 6))));
-#pragma unroll
-        for (int s = 0; s < kUpMine; ++s)
-          if (c0 + kLoraCols * c < ranks[s]) {
-            const bf16x8_t w = lora_within(*reinterpret_cast<const uint4*>(l.b[wave][s] + (frag ^ (c << 6))),
-                                           ranks[s] - c0 - kLoraCols * c - 8 * g);
-            acc[s] = mfma16x16x32(w, hi, acc[s]);
-            acc[s] = mfma16x16x32(w, lo, acc[s]);
-          }
+        const bf16x8_t w = left < kLoraCols ? lora_within(raw, left - 8 * g) : as_bf16x8(raw);
+        acc = mfma16x16x32(w, as_bf16x8(hi), acc);
+        acc = mfma16x16x32(w, as_bf16x8(lo), acc);
       }
+      if (key == now) d = acc;
     }
-    // lane (r, g): features 4g .. +3 of row r
-#pragma unroll
-    for (int s = 0; s < kUpMine; ++s)
-      if (key >= 0 && key == ads[s]) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) l.d[r][4 * g + i] = acc[s][i];
-      }
-    __syncthreads();
   }
   if (row >= M) return;
-  const float up = has ? l.d[mine][r] : -0.f;
   if constexpr (PLANE) {
-    plane_out[idx] = up;
+    *reinterpret_cast<f32x4_t*>(plane_out + idx) = d;
   } else {
-    float o = p[0];
+    f32x4_dw o = p[0];
 #pragma unroll
     for (int i = 1; i < 8; ++i)
       if (i < slices) o += p[i];
-    for (int i = 8; i < slices; ++i) o += part[i * plane + idx];
-    const float q = bf16_round(o + up + (b ? bf2f(bias) : 0.f));
-    if (residual) residual[idx] = f2bf(bf2f(res) + q);
-    else y[idx] = f2bf(q);
+    for (int i = 8; i < slices; ++i) o += *reinterpret_cast<const f32x4_dw*>(part + i * plane + idx);
+    u16x4_h out;
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      const float q = bf16_round(o[c] + d[c] + (b ? bf2f(bias[c]) : 0.f));
+      out[c] = residual ? f2bf(bf2f(res[c]) + q) : f2bf(q);
+    }
+    *reinterpret_cast<u16x4_h*>((residual ? residual : y) + idx) = out;
   }
+}
+
+static int launch_lora_finalize(const float* part, int slices, int M, int N, const LoraArgs& a, const uint16_t* b, uint16_t* y,
+                                uint16_t* residual, float* plane_out, hipStream_t s) {
+  const auto kernel = plane_out ? lora_finalize_kernel<true> : lora_finalize_kernel<false>;
+  hipLaunchKernelGGL(kernel, dim3(ceil_div(N, 64), ceil_div(M, 16)), dim3(256), 0, s, part, slices, M, N, a, b, y, residual, plane_out);
+  return check_launch("lora_finalize");
 }
 
 static size_t align256(size_t v) { return (v + 255) & ~(size_t)255; }
@@ -194,10 +174,7 @@ int launch_gemm_lora_planes(const uint16_t* x, const uint16_t* W, int M, int N, 
   }
   const int rc = launch_gemm_lora(x, W, M, N, K, part, slices, a, s);
   if (rc) return rc;
-  hipLaunchKernelGGL(lora_finalize_kernel<true>, dim3(N / 16, ceil_div(M, 16)), dim3(256), 0, s, part, 0, M, N, a, nullptr, nullptr,
-                     nullptr, part + (size_t)*slices * M * N);
-  ++*slices;
-  return check_launch("lora_plane");
+  return launch_lora_finalize(part, 0, M, N, a, nullptr, nullptr, nullptr, part + (size_t)(*slices)++ * M * N, s);
 }
 
 size_t lora_h_bytes(int M, int R, int n_seg) { return align256((size_t)M * n_seg * lora_cols(R) * 4) + align256((size_t)M * sizeof(int2)); }
@@ -218,9 +195,7 @@ int launch_linear_lora(const uint16_t* x, const uint16_t* W, const uint16_t* b, 
   }
   rc = launch_gemm_lora(x, W, M, N, K, part, &slices, a, s);
   if (rc) return rc;
-  hipLaunchKernelGGL(lora_finalize_kernel<false>, dim3(N / 16, ceil_div(M, 16)), dim3(256), 0, s, part, slices, M, N, a, b, y, residual,
-                     nullptr);
-  return check_launch("lora_finalize");
+  return launch_lora_finalize(part, slices, M, N, a, b, y, residual, nullptr, s);
 }
 
 int make_lora_args(LoraArgs* out, const uint16_t* A, const uint16_t* B, const float* scale, const int32_t* ranks, int n, int R,

@@ -183,7 +183,7 @@ __global__ __launch_bounds__(kMoveThreads) void kv_compact_kernel(MoveArgs a) {
 static int check_slab(const char* what, int64_t base, int cap, int heads, int64_t pool_elems) {
   FLYAI_REQUIRE(cap > 0 && cap % 64 == 0 && base >= 0 && base % 8 == 0,
                 "%s: a slab needs cap %% 64 == 0 and base %% 8 == 0", what);
-  if (base + (int64_t)heads * cap * 64 > pool_elems)
+  if (base > pool_elems - (int64_t)heads * cap * 64)  // no sum that could wrap
     return set_error(FLYAI_ERANGE, "%s: slab at %lld of %d positions ends past the pool (%lld elements)", what,
                      (long long)base, cap, (long long)pool_elems);
   return FLYAI_OK;

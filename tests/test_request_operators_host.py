@@ -82,6 +82,15 @@ def test_fork_refusals(lib, change, code):
     assert lib.flyai_last_error()
 
 
+@pytest.mark.parametrize("base", [2 ** 63 - 8, 2 ** 63 - 128 * 128, 2 ** 62])
+def test_slabs_at_the_end_of_64_bits(lib, base):
+    """A base whose slab would end past 2^63 is past the pool, not before it."""
+    assert _fork(lib, src=(base, 128)) == _lib.FLYAI_ERANGE
+    assert _fork(lib, dsts=((base, 128),)) == _lib.FLYAI_ERANGE
+    assert _compact(lib, [(base, 128, 0, 1)], [1]) == _lib.FLYAI_ERANGE
+    assert _compact(lib, [(base, 128, 0, 1)], [0]) == _lib.FLYAI_ERANGE
+
+
 def test_fork_of_nothing(lib):
     assert _fork(lib, lo=10) == 0
     assert _fork(lib, dsts=()) == 0

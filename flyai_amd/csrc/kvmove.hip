@@ -200,6 +200,18 @@ static int check_pools(const char* what, const void* k, const void* v, int64_t l
   return FLYAI_OK;
 }
 
+// Whether two pools of n_layers layers share no element: spans that lie apart, or layers at one distance that lie between
+// each other's.
+static bool pools_apart(const uint16_t* a, int64_t a_layer, int64_t a_elems, const uint16_t* b, int64_t b_layer, int64_t b_elems,
+                        int n_layers) {
+  const uintptr_t A = (uintptr_t)a, B = (uintptr_t)b;
+  const uint64_t far_a = 2 * ((uint64_t)(n_layers - 1) * a_layer + a_elems), far_b = 2 * ((uint64_t)(n_layers - 1) * b_layer + b_elems);
+  if (A <= B ? B - A >= far_a : A - B >= far_b) return true;
+  if (n_layers == 1 || a_layer != b_layer) return false;
+  const uint64_t step = 2 * (uint64_t)a_layer, off = A <= B ? (B - A) % step : (step - (A - B) % step) % step;  // b's layers behind a's
+  return off >= 2 * (uint64_t)a_elems && step - off >= 2 * (uint64_t)b_elems;
+}
+
 }  // namespace flyai
 
 using namespace flyai;
@@ -216,6 +228,7 @@ extern "C" int flyai_kv_fork(const uint16_t* src_k, const uint16_t* src_v, int64
                              int32_t lo, int32_t hi, flyai_stream_t stream) {
   RUN(check_pools("kv_fork", src_k, src_v, src_layer, src_elems, n_layers, Hkv, D));
   RUN(check_pools("kv_fork", dst_k, dst_v, dst_layer, dst_elems, n_layers, Hkv, D));
+  const bool same = src_k == dst_k && src_v == dst_v && (n_layers == 1 || src_layer == dst_layer);
   FLYAI_REQUIRE(src_host && n_dst >= 0 && (n_dst == 0 || dsts_host), "kv_fork: null slab");
   const flyai_kv_slab src = *src_host;
   FLYAI_REQUIRE(0 <= lo && lo <= hi, "kv_fork: positions [%d, %d) are no range", lo, hi);
@@ -229,10 +242,16 @@ extern "C" int flyai_kv_fork(const uint16_t* src_k, const uint16_t* src_v, int64
     auto apart = [&](const flyai_kv_slab& o) {
       return o.base + (int64_t)Hkv * o.cap * 64 <= d.base || d.base + (int64_t)Hkv * d.cap * 64 <= o.base;
     };
-    FLYAI_REQUIRE(src_k != dst_k || apart(src), "kv_fork: destination %d overlaps the source", i);
+    FLYAI_REQUIRE(!same || apart(src), "kv_fork: destination %d overlaps the source", i);
     for (int j = 0; j < i; ++j) FLYAI_REQUIRE(apart(dsts_host[j]), "kv_fork: destinations %d and %d overlap", j, i);
   }
-  if (lo == hi) return FLYAI_OK;
+  if (lo == hi || n_dst == 0) return FLYAI_OK;
+  // K and V are written side by side, and the source is read meanwhile: its pools are the destinations' or share nothing
+  FLYAI_REQUIRE(pools_apart(dst_k, dst_layer, dst_elems, dst_v, dst_layer, dst_elems, n_layers), "kv_fork: the K and V pools overlap");
+  const uint16_t *srcs[2] = {src_k, src_v}, *dsts[2] = {dst_k, dst_v};
+  for (int i = 0; i < 4 && !same; ++i)
+    FLYAI_REQUIRE(pools_apart(srcs[i & 1], src_layer, src_elems, dsts[i >> 1], dst_layer, dst_elems, n_layers),
+                  "kv_fork: the source's pools overlap the destinations' and are not the same");
   hipStream_t s = as_stream(stream);
   for (int i = 0; i < n_dst; i += kForkDsts) {
     ForkArgs a;
@@ -276,8 +295,9 @@ extern "C" int flyai_kv_compact(uint16_t* k_pool, uint16_t* v_pool, int64_t laye
   MoveArgs a;
   a.pool[0] = k_pool, a.pool[1] = v_pool, a.layer = layer;
   int slabs = 0, words = 0;
-  auto flush = [&]() {
+  auto flush = [&]() -> int {
     if (slabs == 0) return FLYAI_OK;
+    FLYAI_REQUIRE(pools_apart(k_pool, layer, pool_elems, v_pool, layer, pool_elems, n_layers), "kv_compact: the K and V pools overlap");
     hipLaunchKernelGGL(kv_compact_kernel, dim3(8 * Hkv, slabs, n_layers), dim3(kMoveThreads), 0, s, a);
     slabs = words = 0;
     return check_launch("kv_compact");

@@ -91,6 +91,25 @@ def test_slabs_at_the_end_of_64_bits(lib, base):
     assert _compact(lib, [(base, 128, 0, 1)], [0]) == _lib.FLYAI_ERANGE
 
 
+def test_overlapping_pools(lib):
+    """K and V in one place, or a source that lies across the destination's layers: two workgroups would race."""
+    slab, L = 2 * 128 * 64, 2
+    elems = 8 * 128 * 64
+
+    def fork(src_k, src_v, k, v, src_layer=elems):
+        src, dst = _slab(0, 128), _slab(slab, 128)
+        return lib.flyai_kv_fork(src_k, src_v, src_layer, elems, k, v, elems, elems, L, 2, 64, C.byref(src), C.byref(dst), 1, 0, 10, None)
+
+    at = lambda layers: 0x100000 + layers * elems * 2                # whole pools of one layer behind each other
+    for case in [(at(0), at(2), at(0), at(0)), (at(0), at(2), at(0), at(1)), (at(4), at(6), at(0), at(1)),   # K across V
+                 (at(1), at(4), at(0), at(4)), (at(0), at(3), at(0), at(4)), (at(6), at(8), at(0) + 16, at(8)),  # the source across
+                 (at(4), at(0), at(0), at(4)), (at(8), at(9), at(0), at(8)), (at(0), at(4), at(0), at(4), 2 * elems)]:
+        assert fork(*case) == _lib.FLYAI_EINVAL, case
+        assert b"overlap" in lib.flyai_last_error()
+    assert _compact(lib, [(0, 128, 0, 1)], [1]) == _lib.FLYAI_EINVAL
+    assert b"overlap" in lib.flyai_last_error()
+
+
 def test_fork_of_nothing(lib):
     assert _fork(lib, lo=10) == 0
     assert _fork(lib, dsts=()) == 0

@@ -4,6 +4,7 @@ PyTorch provides device memory and the stream; every computation happens in libf
 Each wrapper checks dtype / device / contiguity / shape on the host before the launch."""
 import ctypes as C
 import functools
+import operator
 import struct
 
 import numpy as np
@@ -360,7 +361,7 @@ def linear_lora(x, w, b, lora_a, lora_b, scale, ranks, adapter, segments=None, r
     [0, n) mean no adapter, and such a row has ``linear``'s bits.  A row's result depends on that row alone."""
     M, K = x.shape
     N = w.shape[0]
-    segments = (N,) if segments is None else tuple(int(v) for v in segments)
+    segments = (N,) if segments is None else tuple(_position(v) for v in segments)
     S = len(segments)
     if lora_b.dim() != 3:
         raise ValueError("lora_b must be [adapters, N, R]")
@@ -449,8 +450,14 @@ def kv_fork(k, v, n_kv_heads, src, dsts, lo, hi, src_k=None, src_v=None):
         if sL != L or sdev != dev:
             raise ValueError(f"the source's pools have {sL} layers on device {sdev}, the others {L} on {dev}")
     slabs = _packed(_KV_SLAB, [(b, c, 0) for b, c in (src, *dsts)])
-    _on(dev, lib().flyai_kv_fork, src_k.data_ptr(), src_v.data_ptr(), sn, sn, k.data_ptr(), v.data_ptr(), n, n, L, int(n_kv_heads),
-        64, slabs[:_KV_SLAB.size], slabs[_KV_SLAB.size:], len(dsts), int(lo), int(hi))
+    lo, hi = (_position(p) for p in (lo, hi))
+    _on(dev, lib().flyai_kv_fork, src_k.data_ptr(), src_v.data_ptr(), sn, sn, k.data_ptr(), v.data_ptr(), n, n, L, _position(n_kv_heads),
+        64, slabs[:_KV_SLAB.size], slabs[_KV_SLAB.size:], len(dsts), lo, hi)
+
+
+def _position(p):
+    """An int32 that is out of range where p is: what a C int would make of a larger one may be a position."""
+    return min(max(operator.index(p), -1), 0x7fffffff)
 
 
 def _host_positions(keep):
@@ -482,7 +489,7 @@ def kv_compact(k, v, n_kv_heads, moves):
     L, n, dev = _kv_pools(k, v)
     keeps = [_host_positions(m[3]) for m in moves]
     rows = _packed(_KV_MOVE, [(base, cap, start, len(a) // 4, 0) for (base, cap, start, _), a in zip(moves, keeps)])
-    _on(dev, lib().flyai_kv_compact, k.data_ptr(), v.data_ptr(), n, n, L, int(n_kv_heads), 64, rows, len(moves), b"".join(keeps))
+    _on(dev, lib().flyai_kv_compact, k.data_ptr(), v.data_ptr(), n, n, L, _position(n_kv_heads), 64, rows, len(moves), b"".join(keeps))
 
 
 # ---- DeepSeek-V3-shaped FP8 MoE ------------------------------------------------------------------

@@ -195,6 +195,32 @@ def test_refusals_leave_the_pools_alone():
     assert torch.equal(_bits(k), _bits(before[0])) and torch.equal(_bits(v), _bits(before[1]))
 
 
+def test_positions_past_32_bits_are_refused():
+    heads, cap = 2, 128
+    slab = heads * cap * 64
+    k, v = _pools(2, 2 * slab, 12)
+    before = k.clone()
+    with pytest.raises(ContextOverflow):
+        ops.kv_fork(k, v, heads, (0, cap), [(slab, cap)], 0, 2 ** 32 + 5)
+    with pytest.raises(FlyaiError):
+        ops.kv_fork(k, v, heads, (0, cap), [(slab, cap)], 2 ** 32, 5)
+    with pytest.raises(FlyaiError):
+        ops.kv_fork(k, v, heads, (0, cap), [(slab, cap)], -2 ** 32, 5)
+    with pytest.raises(TypeError):
+        ops.kv_fork(k, v, heads, (0, cap), [(slab, cap)], 0, 5.5)
+    for n_heads in (2 ** 32 + 2, -2 ** 32 + 2):
+        with pytest.raises(FlyaiError):
+            ops.kv_fork(k, v, n_heads, (0, cap), [(slab, cap)], 0, 5)
+        with pytest.raises(FlyaiError):
+            ops.kv_compact(k, v, n_heads, [(0, cap, 0, [1])])
+    with pytest.raises(ValueError):
+        ops.kv_compact(k, v, heads, [(0, cap, 2 ** 32, [1])])
+    with pytest.raises(ValueError):
+        ops.kv_compact(k, v, heads, [(0, cap, 0, [2 ** 32 + 1])])
+    torch.cuda.synchronize()
+    assert torch.equal(_bits(k), _bits(before))
+
+
 # ---- through the workspace ---------------------------------------------------------------------------
 
 def _workspace(layers=2, slots=3, caps=(100, 200, 100), heads=2, seed=20):

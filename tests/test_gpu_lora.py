@@ -262,6 +262,8 @@ def test_refusals():
         _run(dict(c, segments=(40, 8)), ad)
     with pytest.raises(RuntimeError, match="features"):
         _run(dict(c, segments=(16, 16)), ad)
+    with pytest.raises(RuntimeError, match="segment"):
+        _run(dict(c, segments=(2 ** 32 + 32, 16)), ad)    # not 32
     with pytest.raises(TypeError):
         _run(dict(c, scale=c["scale"].double()), ad)
     with pytest.raises(ValueError):

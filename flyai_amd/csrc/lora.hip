@@ -241,5 +241,8 @@ extern "C" int flyai_linear_lora_bf16(const uint16_t* x, const uint16_t* w, cons
   const int rc = make_lora_args(&a, lora_a, lora_b, scale, ranks, n_adapters, R, segments_host, n_segments, N, adapter, row_seq,
                                 n_seqs);
   if (rc) return rc;
+  // other workgroups read x while one writes its result
+  const char *xb = reinterpret_cast<const char*>(x), *yb = reinterpret_cast<const char*>(residual ? residual : y);
+  FLYAI_REQUIRE(xb + (size_t)M * K * 2 <= yb || yb + (size_t)M * N * 2 <= xb, "linear_lora: the result overlaps x");
   return launch_linear_lora(x, w, b, M, N, K, a, y, residual, static_cast<char*>(workspace), as_stream(stream));
 }

@@ -354,7 +354,7 @@ def _lora_workspace_bytes(M, N, K, R, S):
 
 def linear_lora(x, w, b, lora_a, lora_b, scale, ranks, adapter, segments=None, row_seq=None, residual=None):
     """``linear`` with a low-rank adapter of its own for each row: y = bf16(x W^T + b + s_a (x A_a^T) B_a^T), with residual
-    residual <- bf16(residual + y) (returned).  lora_a bf16 [n, S * R, K], lora_b bf16 [n, N, R], scale fp32 [n], ranks
+    residual <- bf16(residual + y) (returned; it must not overlap x).  lora_a bf16 [n, S * R, K], lora_b bf16 [n, N, R], scale fp32 [n], ranks
     int32 [n] (adapter a uses the first ranks[a] of R rows of each segment's A and columns of B; nothing past them is
     used); R a multiple of 16 up to 128.  segments: the S (at most 4) widths of the output's runs that have an A of
     their own (None: one of N).  adapter int32: of each row [M], or with row_seq int32 [M] of each sequence; ids outside

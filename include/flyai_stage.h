@@ -317,7 +317,7 @@ int flyai_attn_prefill(const uint16_t* q, const uint16_t* k_pool, const uint16_t
  * [0, R] is clamped; entries past it are not used, whatever they hold); R in 16, 32, ..., 128.  adapter int32: of
  * row t, or with row_seq int32 [M] of row t's sequence (adapter[row_seq[t]], n_seqs entries); an adapter
  * outside [0, n_adapters) or a sequence outside [0, n_seqs) means none.  With residual the result is bf16(residual +
- * y), written to residual.  A row's result depends on that row alone: not on its batch, nor on what other
+ * y), written to residual; the result must not overlap x.  A row's result depends on that row alone: not on its batch, nor on what other
  * rows' adapters hold.  All bf16 matrices and the workspace are 16-byte aligned (b need not be).  workspace:
  * flyai_linear_lora_workspace_bytes; two calls that may overlap need one each.  M <= 524288, N % 16 == 0,
  * K % 32 == 0, K <= 8192. */

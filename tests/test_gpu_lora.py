@@ -249,6 +249,15 @@ def test_unaligned_bias_and_views():
         _run(c, adapter)
 
 
+def test_residual_over_x_is_refused():
+    c = _inputs(300, 64, (64,), 2, 16, 18)
+    before = c["x"].clone()
+    with pytest.raises(RuntimeError, match="overlaps"):
+        _run(c, _adapters(300, 2, 18), residual=c["x"])
+    torch.cuda.synchronize()
+    assert torch.equal(c["x"], before)
+
+
 def test_refusals():
     c = _inputs(4, 64, (32, 16), 2, 16, 13)
     ad = torch.zeros(4, dtype=torch.int32, device=DEV)

@@ -33,6 +33,13 @@ def test_lora_refusals(lib, change):
     assert lib.flyai_last_error()
 
 
+def test_lora_result_over_x(lib):
+    """x is read while the result is written: as residual it would be read half updated."""
+    for at in (0x100000, 0x100000 + 4 * 64 * 2 - 16, 0x100000 - 4 * 48 * 2 + 16):
+        assert _lora(lib, y=C.c_void_p(at)) == _lib.FLYAI_EINVAL
+        assert b"overlaps" in lib.flyai_last_error()
+
+
 def test_lora_of_no_rows(lib):
     assert _lora(lib, M=0) == 0
     assert lib.flyai_linear_lora_workspace_bytes(0, 48, 64, 16, 2) == 0

@@ -284,11 +284,12 @@ __device__ __forceinline__ void lora_down(const uint16_t* __restrict__ x, int M,
           }
           v *= scale;
         }
-        const uint16_t hi = f2bf(v);
+        uint16_t hi = f2bf(v);
+        if ((hi & 0x7fff) == 0x7f80 && fabsf(v) <= 3.402823466e+38f) --hi;  // finite: bf16's largest, and the rest in the low term
         const float rest = v - bf2f(hi);
         uint16_t* o = a.h + ((size_t)(m0 + l.row[wave][q]) * a.n_seg + seg) * 2 * cols + c0 + j;
         o[0] = hi;
-        o[cols] = rest == rest ? f2bf(rest) : 0;  // a value past bf16's range keeps its infinity: inf - inf would be NaN
+        o[cols] = rest == rest ? f2bf(rest) : 0;  // an infinity stays one: inf - inf would be NaN
       }
       __syncthreads();
     }

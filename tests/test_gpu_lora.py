@@ -195,6 +195,20 @@ def test_large_h_keeps_its_infinity():
     assert bool((got.float() == float("inf")).all())
 
 
+@pytest.mark.parametrize("M", [3, 300])
+@pytest.mark.parametrize("sign", [1.0, -1.0])
+def test_h_between_the_largest_bf16_and_fp32(M, sign):
+    """h of 3.4e38 rounds to an infinite bf16; with B = 1/2 the result is finite."""
+    c = _inputs(M, 64, (64,), 1, 16, 19, ranks=[1])
+    c["x"][:] = 0
+    c["x"][:, 0] = 1
+    c["lora_a"][:] = sign
+    c["scale"][:] = 3.4e38
+    c["lora_b"][:] = 0.5
+    adapter = torch.zeros(M, dtype=torch.int32, device=DEV)
+    _check(_run(c, adapter), c, adapter)
+
+
 def test_ranks_out_of_range_are_clamped():
     c = _inputs(20, 160, (64,), 2, 32, 10, ranks=[32, 0])
     adapter = _adapters(20, 2, 10)

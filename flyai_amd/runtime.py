@@ -379,7 +379,7 @@ class FastVerifyStage:
         """Compact the accepted path's KV (scratch slots start+keep[i]) to start+i, every layer
         (fastverify.py:301-309)."""
         keep = [int(k) for k in keep]
-        if all(a < b for a, b in zip(keep, keep[1:])):
+        if all(a < b for a, b in zip([-1] + keep, keep)):
             self.cache.compact([0], [start], [keep])
             return
         # a tree whose parents come after their children

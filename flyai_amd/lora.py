@@ -40,8 +40,8 @@ class AdapterBank:
 
     def load(self, index, layers, scale):
         """Fill slot ``index``.  layers: per layer a dict of "q", "k", "v", "o" -> (A [r, in], B [out, r]); a projection
-        that is missing stays as it is without the adapter.  r may differ from place to place, up to max_rank; scale is
-        alpha / r.  Nothing changes if anything does not fit.  Call between steps, on the stream that they run on."""
+        that is missing stays as it is without the adapter.  r may differ from place to place, up to max_rank; values are
+        rounded to bf16; scale is alpha / r.  Nothing changes if anything does not fit.  Call between steps, on the stream that they run on."""
         i = self._slot(index)
         if len(layers) != self.n_layers:
             raise ValueError(f"the adapter has {len(layers)} layers, the bank {self.n_layers}")
@@ -51,11 +51,14 @@ class AdapterBank:
                 if name not in self._places:
                     raise ValueError(f"layer {l}: no projection {name!r} (only {', '.join(PROJECTIONS)})")
                 n_in, n_out, _, _ = self._places[name]
+                if not all(isinstance(t, torch.Tensor) and t.is_floating_point() and t.dim() == 2 for t in (a, b)):
+                    raise ValueError(f"layer {l} {name}: A and B must be floating-point matrices")
                 r = a.shape[0]
                 if tuple(a.shape) != (r, n_in) or tuple(b.shape) != (n_out, r) or not 1 <= r <= self.max_rank:
                     raise ValueError(f"layer {l} {name}: A {tuple(a.shape)} and B {tuple(b.shape)} are not [r, {n_in}] and "
                                      f"[{n_out}, r] with r in [1, {self.max_rank}]")
                 top = max(top, r)
+        scale = float(scale)
         self.unload(i)
         for t in (self.qkv_a, self.qkv_b, self.o_a, self.o_b):
             t[:, i].zero_()
@@ -63,9 +66,10 @@ class AdapterBank:
             for name, (a, b) in projections.items():
                 _, n_out, row, col = self._places[name]
                 ta, tb = (self.o_a, self.o_b) if name == "o" else (self.qkv_a, self.qkv_b)
-                ta[l, i, row:row + a.shape[0]] = a
-                tb[l, i, col:col + n_out, :a.shape[0]] = b
-        self.scale[i] = float(scale)
+                # detached: a parameter under training would draw the bank into its graph
+                ta[l, i, row:row + a.shape[0]] = a.detach()
+                tb[l, i, col:col + n_out, :a.shape[0]] = b.detach()
+        self.scale[i] = scale
         self.ranks[i] = top
 
     def unload(self, index):

@@ -152,6 +152,27 @@ def test_compact_of_nothing(lib):
     assert _compact(lib, [], [], v=None) == _lib.FLYAI_EINVAL
 
 
+def test_adapter_bank_on_the_host():
+    """What does not fit changes nothing; parameters under training are read, not tied to the bank."""
+    from flyai_amd.lora import AdapterBank
+    from flyai_amd.runtime import GptOssShape
+
+    shape = GptOssShape(hidden=64, n_q_heads=8, n_kv_heads=1, head_dim=64)
+    bank = AdapterBank(shape, 2, 2, 16, "cpu")
+    a, b = torch.nn.Parameter(torch.randn(3, 64)), torch.nn.Parameter(torch.randn(512, 3))
+    for _ in range(2):
+        bank.load(1, [{"q": (a, b)}, {}], 0.5)
+    assert not any(t.requires_grad for t in (bank.qkv_a, bank.qkv_b, bank.scale, bank.ranks))
+    assert torch.equal(bank.qkv_a[0, 1, :3], a.detach().bfloat16()) and torch.equal(bank.qkv_b[0, 1, :512, :3], b.detach().bfloat16())
+    assert not bool(bank.qkv_a[1].any()) and bank.ranks.tolist() == [0, 3] and bank.scale.tolist() == [0.0, 0.5]
+    before = bank.qkv_a.clone()
+    for layers, scale in [([{"q": (a.detach().numpy(), b)}, {}], 1.0), ([{"q": (a.detach().long(), b)}, {}], 1.0),
+                          ([{"q": (a[0], b)}, {}], 1.0), ([{"q": (a, b)}, {}], "1/16"), ([{"q": (a, b)}], 1.0)]:
+        with pytest.raises(ValueError):
+            bank.load(1, layers, scale)
+        assert torch.equal(bank.qkv_a, before) and bank.ranks.tolist() == [0, 3]
+
+
 def test_rope_frequencies():
     inv, att = rope_frequencies(64, 10000.0, device="cpu")
     assert att == 1.0 and inv.dtype == torch.float64 and inv.shape == (32,)

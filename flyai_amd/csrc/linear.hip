@@ -748,7 +748,7 @@ int launch_gemm(const uint16_t* x, const uint16_t* W, int M, int N, int K, float
 }
 
 // The tiled kernel ends a projection with adapters by itself where it runs (K % 64 == 0) and no wave's 64 features
-// straddle two segments: 2,096 rows of 13 adapters, 5,120 x 2,880, 92 us; the plain kernel, 76.5, with a finalize behind it,
+// straddle two segments: 2,096 rows of 12 adapters, 5,120 x 2,880, 92 us; the plain kernel, 76.5, with a finalize behind it,
 // 56.5, is for the others.  (300 rows of 2,880 x 4,096: 30.7 us, or 28.4 + 7.6.)
 bool gemm_tiled_lora_fits(int M, int K, const LoraArgs& a) {
   bool whole = true;

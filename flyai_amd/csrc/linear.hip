@@ -535,7 +535,7 @@ __global__ __launch_bounds__(64 * kTiledWaves) void gemm_tiled_lds_kernel(const 
                                                        lora_chunk(8 * i, 0, lo.R)),
                                          (lds_ptr)(held_b + 2048 * wave + 1024 * i), 16, 0, 0);
     }
-    lora_fetch_h(lo, M, m0 + 32 * wm, min(n0 + 64 * wn, N - 1), hv);
+    lora_fetch_h<2>(lo, M, m0 + 32 * wm, min(n0 + 64 * wn, N - 1), hv);
     asm volatile("" ::: "memory");
   }
   read_ab(a0, b0, sa0, sb0, 0);
@@ -575,8 +575,12 @@ __global__ __launch_bounds__(64 * kTiledWaves) void gemm_tiled_lds_kernel(const 
   if constexpr (LORA) {
 #pragma unroll
     for (int k = 0; k < 8; ++k) *reinterpret_cast<u32x4_t*>(own + 1024 * k + 16 * lane) = hv[k];
-    if (n0 + 64 * wn < N)
-      lora_up_block(lo, M, N, m0 + 32 * wm, n0 + 64 * wn, who, own, held.x, held_b + (QKV ? 0 : 8192 * wn), own + 8192, tot);
+    const auto h = [&](int t, int c, int k) __attribute__((always_inline)) {
+      return as_bf16x8(*reinterpret_cast<const uint4*>(own + 4096 * t + 2048 * k + (frag0 ^ (c << 6))));
+    };
+    const int f0 = __builtin_amdgcn_readfirstlane(n0 + 64 * wn);
+    if (f0 < N)
+      lora_up_block<2, false>(lo, M, N, m0 + 32 * wm, f0, who, h, held.x, held_b + (QKV ? 0 : 8192 * wn), own + 8192, tot);
   }
   // lane (r, g) holds rows 16(2wm + a) + 4g + v of feature 16(4wn + b) + r
   if constexpr (EPI == kEpiLinear) {

@@ -320,102 +320,118 @@ __device__ __forceinline__ int lora_chunk(int at, int c0, int end) {
   return min(c0 + 8 * ((lane & 7) ^ ((q >> 1) & 7)), end - 8);
 }
 
-// h of the tiled GEMM's wave, 32 rows from m0 in the segment of feature f0, columns 0 .. 63: h[4 a + 2 t + i] is rows 16 a +
+// h of a tiled GEMM's wave, 16 MT rows from m0 in the segment of feature f0, columns 0 .. 63: h[4 a + 2 t + i] is rows 16 a +
 // 8 i .. +7, high (t = 0) or low terms, for 1 KiB of LDS each.
-__device__ __forceinline__ void lora_fetch_h(const LoraArgs& a, int M, int m0, int f0, u32x4_t (&h)[8]) {
+template <int MT>
+__device__ __forceinline__ void lora_fetch_h(const LoraArgs& a, int M, int m0, int f0, u32x4_t (&h)[4 * MT]) {
   const int cols = lora_cols(a.R), seg = lora_segment(a, f0);
 #pragma unroll
-  for (int k = 0; k < 8; ++k) {
+  for (int k = 0; k < 4 * MT; ++k) {
     const int row = m0 + 16 * (k >> 2) + 8 * (k & 1) + ((threadIdx.x & 63) >> 3);
     h[k] = *reinterpret_cast<const u32x4_t*>(a.h + ((size_t)min(row, M - 1) * a.n_seg + seg) * 2 * cols + (k & 2 ? cols : 0) +
                                              lora_chunk(8 * (k & 1), 0, cols));
   }
 }
 
-// The up products of 32 rows from m0 and 64 features from f0 (one segment), added to the tiled GEMM's sums: lane (r, g)
-// holds rows 16 a + 4g .. +3 of feature f0 + 16 b + r in sum[a][b].  `who`: row m0 + lane's adapter and rank (lanes 0 ..
-// 31).  hl: lora_fetch_h's tiles; held_b: columns 0 .. 63 of adapter `held` (-1: of none), this wave's features, 16 to a
-// tile; bl: room for another adapter's, which come in whole runs like the GEMM's operands (as MFMA operands from memory a
-// tile of 128 rows of 45 adapters took 50,000 clocks, more than its projection).
-__device__ __forceinline__ void lora_up_block(const LoraArgs& a, int M, int N, int m0, int f0, int2 who, const char* hl, int held,
-                                              const char* held_b, char* bl, f32x4_t (&sum)[2][4]) {
+// The up products of 16 MT rows from m0 and 64 features from f0 (one segment; a wave's, uniform), added to a tiled GEMM's
+// sums: lane (r, g) holds rows 16 t + 4g .. +3 of feature f0 + 16 b + r in sum[t][b], or (FEATURES) features f0 + 16 b + 4g ..
+// +3 of row 16 t + r.  `who`: row m0 + lane's adapter and rank.  h(t, c, k): this lane's operand of row tile t, columns 32c ..
+// +31, high (k = 0) or low terms; held_b: columns 0 .. 63 of adapter `held` (-1: of none), this wave's features, 16 to a
+// tile; bl: room for an adapter's, which come in whole runs like the GEMM's operands (as MFMA operands from memory a tile of
+// 128 rows of 45 adapters took 50,000 clocks, more than its projection).  Columns past the rank become zero on their way to
+// LDS.  A CU runs this once a tile, so its time is the code's way from memory as much as anything: masking at the products,
+// three times the instructions, made 2,096 rows 8 us slower, two adapters in flight (twice the code) 10.
+template <int MT, bool FEATURES, typename H>
+__device__ __forceinline__ void lora_up_block(const LoraArgs& a, int M, int N, int m0, int f0, int2 who, const H& h, int held,
+                                              const char* held_b, char* bl, f32x4_t (&sum)[MT][4]) {
   const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
-  const int cols = lora_cols(a.R);
-  const int key = lane < 32 && m0 + lane < M && who.y > 0 ? who.x : -1;
-  int of_row[2][4];
-#pragma unroll
-  for (int t = 0; t < 2; ++t)
-#pragma unroll
-    for (int v = 0; v < 4; ++v) of_row[t][v] = __builtin_amdgcn_ds_bpermute(4 * (16 * t + 4 * g + v), key);
+  const int key = lane < 16 * MT && m0 + lane < M && who.y > 0 ? who.x : -1;
   uint64_t todo = __ballot(key >= 0);
-  int ad = -1, rank = 0;
-  uint64_t rows = 0;
-  u32x4_t nb[8];
-  auto next = [&]() __attribute__((always_inline)) {
-    ad = -1;
-    if (!todo) return;
-    const int first = __builtin_ctzll(todo);
-    ad = __builtin_amdgcn_readlane(key, first);
-    rank = __builtin_amdgcn_readlane(who.y, first);
-    rows = __ballot(key == ad);
-    todo &= ~rows;
-    if (ad == held) return;
+  if (!todo) return;
+  int of_row[MT][FEATURES ? 1 : 4];
 #pragma unroll
-    for (int k = 0; k < 8; ++k)
-      nb[k] = *reinterpret_cast<const u32x4_t*>(a.B + ((size_t)ad * N + min(f0 + 8 * k + (lane >> 3), N - 1)) * a.R +
-                                                lora_chunk(8 * (k & 1), 0, a.R));
+  for (int t = 0; t < MT; ++t)
+#pragma unroll
+    for (int v = 0; v < (FEATURES ? 1 : 4); ++v) of_row[t][v] = __builtin_amdgcn_ds_bpermute(4 * (16 * t + (FEATURES ? r : 4 * g + v)), key);
+  uint32_t off[8];  // of the lane's chunks in an adapter's rows from f0 on
+#pragma unroll
+  for (int k = 0; k < 8; ++k) off[k] = min(8 * k + (lane >> 3), N - 1 - f0) * a.R + lora_chunk(8 * (k & 1), 0, a.R);
+  u32x4_t nb[8];
+  auto columns = [&](int ad) __attribute__((always_inline)) { return a.B + ((size_t)ad * N + f0) * a.R; };
+  auto fetch = [&](int ad) __attribute__((always_inline)) {
+    if (ad == held) return;
+    const uint16_t* B = columns(ad);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) nb[k] = *reinterpret_cast<const u32x4_t*>(B + off[k]);
   };
   const int frag = r * 128 + ((g ^ ((r >> 1) & 7)) << 4);
-  next();
+  int ad = __builtin_amdgcn_readlane(key, __builtin_ctzll(todo));
+  fetch(ad);
   while (ad >= 0) {
-    const int now = ad, cur_rank = rank;
-    const uint64_t cur_rows = rows;
-    const char* src = now == held ? held_b : bl;
-    if (now != held) {
-      asm volatile("" ::: "memory");  // a wave's LDS operations complete in order
+    const int now = ad, rank = __builtin_amdgcn_readlane(who.y, __builtin_ctzll(todo));
+    const uint64_t rows = __ballot(key == now);
+    if (now == held) {
 #pragma unroll
-      for (int k = 0; k < 8; ++k) *reinterpret_cast<u32x4_t*>(bl + 1024 * k + 16 * lane) = nb[k];
-      asm volatile("" ::: "memory");
+      for (int k = 0; k < 8; ++k) nb[k] = *reinterpret_cast<const u32x4_t*>(held_b + 1024 * k + 16 * lane);
     }
-    next();  // the next adapter's columns are on their way under this one's products
+    if (rank < 2 * kLoraCols) {
+      uint32_t keep[2][4];
 #pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      if (!(cur_rows >> (16 * t) & 0xffff)) continue;
+      for (int i = 0; i < 2; ++i) {
+        const int left = rank - 8 * ((lane & 7) ^ (4 * i + (lane >> 4)));  // of the chunk's eight columns
+#pragma unroll
+        for (int j = 0; j < 4; ++j) keep[i][j] = 2 * j + 1 < left ? 0xffffffffu : 2 * j < left ? 0xffffu : 0u;
+      }
+#pragma unroll
+      for (int k = 0; k < 8; ++k)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) nb[k][j] &= keep[k & 1][j];
+    }
+    asm volatile("" ::: "memory");  // a wave's LDS operations complete in order
+#pragma unroll
+    for (int k = 0; k < 8; ++k) *reinterpret_cast<u32x4_t*>(bl + 1024 * k + 16 * lane) = nb[k];
+    asm volatile("" ::: "memory");
+    todo &= ~rows;
+    ad = todo ? __builtin_amdgcn_readlane(key, __builtin_ctzll(todo)) : -1;
+    if (ad >= 0) fetch(ad);  // on its way under this one's products
+    auto product = [&](bf16x8_t w, bf16x8_t v, f32x4_t c) __attribute__((always_inline)) {
+      return FEATURES ? mfma16x16x32(w, v, c) : mfma16x16x32(v, w, c);
+    };
+#pragma unroll
+    for (int t = 0; t < MT; ++t) {
+      if (!(rows >> (16 * t) & 0xffff)) continue;
       f32x4_t up[4];
 #pragma unroll
       for (int b = 0; b < 4; ++b) up[b] = f32x4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
-        const int left = cur_rank - kLoraCols * c;
-        if (left <= 0) break;
-        const bf16x8_t hi = as_bf16x8(*reinterpret_cast<const uint4*>(hl + 4096 * t + (frag ^ (c << 6))));
-        const bf16x8_t lo = as_bf16x8(*reinterpret_cast<const uint4*>(hl + 4096 * t + 2048 + (frag ^ (c << 6))));
+        if (kLoraCols * c >= rank) break;
+        const bf16x8_t hi = h(t, c, 0), lo = h(t, c, 1);
 #pragma unroll
         for (int b = 0; b < 4; ++b) {
-          const uint4 raw = *reinterpret_cast<const uint4*>(src + 2048 * b + (frag ^ (c << 6)));
-          const bf16x8_t w = left < kLoraCols ? lora_within(raw, left - 8 * g) : as_bf16x8(raw);
-          up[b] = mfma16x16x32(hi, w, up[b]);
-          up[b] = mfma16x16x32(lo, w, up[b]);
+          const bf16x8_t w = as_bf16x8(*reinterpret_cast<const uint4*>(bl + 2048 * b + (frag ^ (c << 6))));
+          up[b] = product(w, hi, up[b]);
+          up[b] = product(w, lo, up[b]);
         }
       }
-      for (int c = 2; kLoraCols * c < cur_rank; ++c) {  // ranks past 64: straight from memory
-        const int row = min(m0 + 16 * t + r, M - 1), left = cur_rank - kLoraCols * c;
+      for (int c = 2; kLoraCols * c < rank; ++c) {  // ranks past 64: straight from memory
+        const int row = min(m0 + 16 * t + r, M - 1), left = rank - kLoraCols * c, cols = lora_cols(a.R);
         const uint16_t* hr = a.h + ((size_t)row * a.n_seg + lora_segment(a, f0)) * 2 * cols + kLoraCols * c + 8 * g;
         const bf16x8_t hi = as_bf16x8(*reinterpret_cast<const uint4*>(hr));
         const bf16x8_t lo = as_bf16x8(*reinterpret_cast<const uint4*>(hr + cols));
+        const uint16_t* B = columns(now);
 #pragma unroll
         for (int b = 0; b < 4; ++b) {
-          const bf16x8_t w = lora_within(*reinterpret_cast<const uint4*>(a.B + ((size_t)now * N + min(f0 + 16 * b + r, N - 1)) * a.R +
-                                                                         lora_col(a.R, c, g)),
+          const bf16x8_t w = lora_within(*reinterpret_cast<const uint4*>(B + (uint32_t)(min(16 * b + r, N - 1 - f0) * a.R + lora_col(a.R, c, g))),
                                          left - 8 * g);
-          up[b] = mfma16x16x32(hi, w, up[b]);
-          up[b] = mfma16x16x32(lo, w, up[b]);
+          up[b] = product(w, hi, up[b]);
+          up[b] = product(w, lo, up[b]);
         }
       }
 #pragma unroll
       for (int b = 0; b < 4; ++b)
 #pragma unroll
-        for (int v = 0; v < 4; ++v) sum[t][b][v] += of_row[t][v] == now ? up[b][v] : -0.f;
+        for (int v = 0; v < 4; ++v) sum[t][b][v] += of_row[t][FEATURES ? 0 : v] == now ? up[b][v] : -0.f;
     }
   }
 }

@@ -10,6 +10,9 @@ namespace flyai {
 int launch_gemm(const uint16_t* x, const uint16_t* W, int M, int N, int K, float* part, int* slices, hipStream_t s);
 int launch_gemm_tiled_lora(const uint16_t* x, const uint16_t* W, const uint16_t* b, int M, int N, int K, float* out, uint16_t* y,
                            uint16_t* residual, const LoraArgs& a, hipStream_t s);
+int launch_gemm_tall_lora(const uint16_t* x, const uint16_t* W, const uint16_t* b, int M, int N, int K, float* out, uint16_t* y,
+                          uint16_t* residual, const LoraArgs& a, hipStream_t s);
+bool gemm_tall_pays(int M, int N);
 bool gemm_tiled_lora_fits(int M, int K, const LoraArgs& a);
 bool gemm_is_tiled(int M);
 int gemm_planes(int M, int K);
@@ -172,7 +175,8 @@ int launch_gemm_lora_planes(const uint16_t* x, const uint16_t* W, int M, int N, 
   if (gemm_tiled_lora_fits(M, K, a)) {
     *slices = 1;
     const int rc = launch_lora_down(x, M, K, a, s);
-    return rc ? rc : launch_gemm_tiled_lora(x, W, nullptr, M, N, K, part, nullptr, nullptr, a, s);
+    if (rc) return rc;
+    return (gemm_tall_pays(M, N) ? launch_gemm_tall_lora : launch_gemm_tiled_lora)(x, W, nullptr, M, N, K, part, nullptr, nullptr, a, s);
   }
   const int rc = launch_gemm_lora(x, W, M, N, K, part, slices, a, s);
   if (rc) return rc;
@@ -193,7 +197,8 @@ int launch_linear_lora(const uint16_t* x, const uint16_t* W, const uint16_t* b, 
   int slices = 0, rc;
   if (gemm_tiled_lora_fits(M, K, a)) {
     rc = launch_lora_down(x, M, K, a, s);
-    return rc ? rc : launch_gemm_tiled_lora(x, W, b, M, N, K, nullptr, y, residual, a, s);
+    if (rc) return rc;
+    return (gemm_tall_pays(M, N) ? launch_gemm_tall_lora : launch_gemm_tiled_lora)(x, W, b, M, N, K, nullptr, y, residual, a, s);
   }
   rc = launch_gemm_lora(x, W, M, N, K, part, &slices, a, s);
   if (rc) return rc;

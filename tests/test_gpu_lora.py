@@ -104,6 +104,29 @@ def test_matches_64_bits(M, K, segments, n, R):
     _check(_run(c, adapter), c, adapter)
 
 
+@pytest.mark.parametrize("M,K,segments,n,R", [
+    (1000, 512, (4096, 512, 512), 9, 48),
+    (769, 192, (4096, 1008), 40, 128),     # rows and features that end inside a tile
+    (960, 64, (5120,), 3, 16),
+    (1000, 128, (4096, 960), 2, 64),
+    (803, 1088, (5072,), 300, 32),         # an adapter or two a row
+])
+@pytest.mark.parametrize("residual", [False, True])
+def test_large_batches(M, K, segments, n, R, residual):
+    """Batches of several rounds of tiles, and their rows' bits in a small one."""
+    c = _inputs(M, K, segments, n, R, M + n)
+    adapter = _adapters(M, n, M)
+    res = torch.randn(M, sum(segments), device=DEV).to(BF16) if residual else None
+    got = _run(c, adapter, **({"residual": res.clone()} if residual else {}))
+    _check(got, c, adapter, res)
+    some = torch.arange(3, M, M // 20, device=DEV)
+    few = _run(dict(c, x=c["x"][some]), adapter[some], **({"residual": res[some]} if residual else {}))
+    assert torch.equal(few, got[some])
+    if not residual:
+        none = adapter < 0
+        assert torch.equal(got[none], ops.linear(c["x"], c["w"], c["b"])[none])
+
+
 @pytest.mark.parametrize("M", [1, 31, 130, 400])
 def test_residual_and_no_bias(M):
     c = _inputs(M, 512, (256, 64), 3, 32, 3)

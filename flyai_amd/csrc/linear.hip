@@ -392,8 +392,8 @@ __global__ __launch_bounds__(64 * kTiledWaves) void gemm_tiled_lds_kernel(const 
   // (23 feature tiles) read about 11x its operand bytes from HBM
   const int gm_ = (M + kTileM - 1) / kTileM, gn_ = (N + kTileN - 1) / kTileN;
   const int per = (gm_ * gn_ + 7) / 8;
-  const int tile = (int)(blockIdx.x % 8) * per + (int)(blockIdx.x / 8);
-  if (tile >= gm_ * gn_) return;
+  const int tile = LORA ? lora_tile(blockIdx.x, gm_, gn_) : (int)(blockIdx.x % 8) * per + (int)(blockIdx.x / 8);
+  if (LORA ? tile < 0 : tile >= gm_ * gn_) return;
   const int m0 = (tile % gm_) * kTileM, n0 = (tile / gm_) * kTileN;
   const int wm = wave >> 1, wn = wave & 1;  // the wave's 32 x 64 block: row tiles 2wm, 2wm+1
   const int KG = K / 64;
@@ -752,8 +752,8 @@ int launch_gemm(const uint16_t* x, const uint16_t* W, int M, int N, int K, float
 }
 
 // The tiled kernel ends a projection with adapters by itself where it runs (K % 64 == 0) and no wave's 64 features
-// straddle two segments: 2,096 rows of 12 adapters, 5,120 x 2,880, 92 us; the plain kernel, 76.5, with a finalize behind it,
-// 56.5, is for the others.  (300 rows of 2,880 x 4,096: 30.7 us, or 28.4 + 7.6.)
+// straddle two segments: 2,096 rows of 12 adapters, 5,120 x 2,880, 92 us (72.5 in lora_gemm.hip's tiles); the plain kernel,
+// 76.5, with a finalize behind it, 56.5, is for the others.  (300 rows of 2,880 x 4,096: 30.7 us, or 28.4 + 7.6.)
 bool gemm_tiled_lora_fits(int M, int K, const LoraArgs& a) {
   bool whole = true;
   for (int i = 0; i + 1 < a.n_seg; ++i) whole &= a.seg_end[i] % 64 == 0;

@@ -320,6 +320,22 @@ __device__ __forceinline__ int lora_chunk(int at, int c0, int end) {
   return min(c0 + 8 * ((lane & 7) ^ ((q >> 1) & 7)), end - 8);
 }
 
+// The tile of workgroup b of a tiled GEMM, row-fastest (-1: none).  As in gemm_tiled_lds_kernel an XCD takes a band of whole
+// feature columns, but within it the first and the last rows' tiles come first: a batch's short sequences, and with them
+// tiles of many adapters, which take longer, are often at one of its ends, and a long tile must not start last.  2,096 rows of
+// which 120 have 12 adapters, 5,120 x 2,880: 79.7 us in the other's order, 72.5 in this.
+__device__ __forceinline__ int lora_tile(int b, int gm, int gn) {
+  const int per = (gm * gn + 7) / 8, start = b % 8 * per, end = min(start + per, gm * gn), i = b / 8;
+  if (start + i >= end) return -1;
+  if (gm <= 2) return start + i;
+  const int first = (start + gm - 1) / gm, n_first = (end + gm - 1) / gm - first;  // columns whose first tile is in the band
+  const int last = start / gm, n_last = end / gm - last;                           // ... whose last one is
+  if (i < n_first) return (first + i) * gm;
+  if (i < n_first + n_last) return (last + i - n_first) * gm + gm - 1;
+  const int inner = last * (gm - 2) + max(start - last * gm - 1, 0) + i - n_first - n_last;  // inner tiles before it
+  return inner / (gm - 2) * gm + 1 + inner % (gm - 2);
+}
+
 // h of a tiled GEMM's wave, 16 MT rows from m0 in the segment of feature f0, columns 0 .. 63: h[4 a + 2 t + i] is rows 16 a +
 // 8 i .. +7, high (t = 0) or low terms, for 1 KiB of LDS each.
 template <int MT>
@@ -340,7 +356,7 @@ __device__ __forceinline__ void lora_fetch_h(const LoraArgs& a, int M, int m0, i
 // tile; bl: room for an adapter's, which come in whole runs like the GEMM's operands (as MFMA operands from memory a tile of
 // 128 rows of 45 adapters took 50,000 clocks, more than its projection).  Columns past the rank become zero on their way to
 // LDS.  A CU runs this once a tile, so its time is the code's way from memory as much as anything: masking at the products,
-// three times the instructions, made 2,096 rows 8 us slower, two adapters in flight (twice the code) 10.
+// with twice the instructions, was 2 us slower at 2,096 rows, two adapters in flight (twice the code again) 10.
 template <int MT, bool FEATURES, typename H>
 __device__ __forceinline__ void lora_up_block(const LoraArgs& a, int M, int N, int m0, int f0, int2 who, const H& h, int held,
                                               const char* held_b, char* bl, f32x4_t (&sum)[MT][4]) {

@@ -9,7 +9,9 @@ typedef uint16_t u16x4_t __attribute__((ext_vector_type(4)));
 // gemm_tiled_lds_kernel's arithmetic (linear.hip) with 48 rows x 64 features a wave: 7 KiB of operands from LDS for 12 MFMAs where
 // waves of 32 x 64 read 6 for 8, which is what bounds those (835 clocks a 64-K group of 128 x 128, 512 of them MFMA).  The
 // same MFMAs in the same K order, each 512-K slice from zero and the slices added in order, so a row's bits do not depend
-// on which of the two kernels a batch takes.  Operands go global -> LDS in whole 128-byte runs through three stages of one
+// on which of the two kernels a batch takes.  W is the first operand: a lane then holds four features of a row, which go out
+// (and a row's adapter is chosen) together.  The products of a group's first half are kept before its barrier; scheduled
+// behind it, the reads' time was all waiting (2,096 rows 89 -> 82.6 us).  Operands go global -> LDS in whole 128-byte runs through three stages of one
 // 64-K group each, a group's loads issued two groups ahead; a row's eight 16-byte chunks are swizzled by row.  Rows and
 // features past M / N load clamped ones and are never stored.
 constexpr int kTallM = 192, kTallN = 128, kTallTiles = 3;  // 4 x 2 waves of 3 row tiles
@@ -26,10 +28,8 @@ __global__ __launch_bounds__(512) void gemm_tall_lora_kernel(const uint16_t* __r
   __shared__ __align__(1024) char sb0[kTallB], sb1[kTallB], sb2[kTallB];
   __shared__ __align__(1024) char held_b[kTallN * 128];  // one adapter's columns
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = lane & 15, g = lane >> 4;
-  // XCD-aware order: an XCD takes a band of whole feature columns (as gemm_tiled_lds_kernel)
-  const int gm = (M + kTallM - 1) / kTallM, gn = (N + kTallN - 1) / kTallN, per = (gm * gn + 7) / 8;
-  const int tile = (int)(blockIdx.x % 8) * per + (int)(blockIdx.x / 8);
-  if (tile >= gm * gn) return;
+  const int gm = (M + kTallM - 1) / kTallM, tile = lora_tile(blockIdx.x, gm, (N + kTallN - 1) / kTallN);
+  if (tile < 0) return;
   const int m0 = (tile % gm) * kTallM, n0 = (tile / gm) * kTallN;
   const int wm = wave >> 1, wn = wave & 1, mw = m0 + 48 * wm, nw = n0 + 64 * wn;  // the wave's 48 x 64 block
   const int KG = K / 64;
@@ -202,10 +202,13 @@ int launch_gemm_tall_lora(const uint16_t* x, const uint16_t* W, const uint16_t* 
   return check_launch("gemm_tall_lora");
 }
 
-// Rounds over the CUs, one workgroup each.
+// Rounds over the CUs, one workgroup each: a round takes 35 to 37 us (K = 2,880), one of 128 x 128 tiles 30 to 34.  5,120 x 2,880,
+// these tiles / those: 800 rows of 20 adapters (1 round / 2) 47.5 / 48.7 us, 1,000 of 5 (1 / 2) 40.4 / 53.1, 2,096 of 12 (2 / 3) 72.5
+// / 92; 2,880 x 4,096: 1,500 rows of 8 (1 / 2) 51 / 64, 2,000 of 24 (1 / 2) 63 / 75; 3,000 rows
+// of 9, 5,120 x 2,880 (3 / 4) 105 / 121, 4,096 of 2 (4 / 5) 154 / 168.
 bool gemm_tall_pays(int M, int N) {
   const int cus = device_cus(), n = ceil_div(N, kTallN);
-  return 4 * ceil_div(ceil_div(M, kTallM) * n, cus) < 3 * ceil_div(ceil_div(M, 128) * n, cus);
+  return ceil_div(ceil_div(M, kTallM) * n, cus) < ceil_div(ceil_div(M, 128) * n, cus);
 }
 
 }  // namespace flyai

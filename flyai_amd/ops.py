@@ -429,9 +429,11 @@ def _kv_pools(k, v):
     """(layers, elements a layer, device) of K and V pools [L, n] (or one layer's [n])."""
     if not isinstance(k, torch.Tensor) or k.dim() not in (1, 2):
         raise ValueError("k and v must be pools of one shape, [layers, elements] or [elements]")
-    dev = k.get_device()
-    _need_all(dev, ("k", k, torch.bfloat16, k.shape), ("v", v, torch.bfloat16, k.shape))
-    return (k.shape[0] if k.dim() == 2 else 1), k.shape[-1], dev
+    shape, dev, bf16 = k.shape, k.get_device(), torch.bfloat16
+    if not (isinstance(v, torch.Tensor) and k.dtype is bf16 and v.dtype is bf16 and v.shape == shape and v.get_device() == dev >= 0
+            and k.is_contiguous() and v.is_contiguous()):
+        _need_all(dev, ("k", k, bf16, shape), ("v", v, bf16, shape))
+    return (shape[0] if len(shape) == 2 else 1), shape[-1], dev
 
 
 _KV_SLAB, _KV_MOVE = struct.Struct("qii"), struct.Struct("qiiii")  # flyai_kv_slab, flyai_kv_move

@@ -98,8 +98,9 @@ class KVWorkspace:
         w = self if src_ws is None else src_ws
         if w.n_kv_heads != self.n_kv_heads or w.n_layers < self.n_layers:
             raise ValueError("fork needs workspaces of the same heads and layers")
+        src_k, src_v = (None, None) if w is self else (w.k_pools[:self.n_layers], w.v_pools[:self.n_layers])
         ops.kv_fork(self.k_pools, self.v_pools, self.n_kv_heads, w._slab_of(src), [self._slab_of(d) for d in dsts], lo, hi,
-                    src_k=w.k_pools[:self.n_layers], src_v=w.v_pools[:self.n_layers])
+                    src_k=src_k, src_v=src_v)
 
     def compact(self, slots, starts, keeps):
         """For each of the slots, move positions start + keep[i] to start + i, every layer, in one launch

@@ -324,7 +324,7 @@ def _need_all(device, *tensors):
     """``_need`` of each (name, tensor, dtype, shape), and all on one device; the checks that pass cost little."""
     for name, t, dtype, shape in tensors:
         if not (isinstance(t, torch.Tensor) and t.dtype is dtype and t.shape == shape and t.is_contiguous()
-                and t.get_device() == device and device >= 0):
+                and t.get_device() == device >= 0):
             _need(t, dtype, shape, name)
             raise ValueError(f"{name} is on {t.device}, the first tensor on another device")
 
@@ -332,10 +332,12 @@ def _need_all(device, *tensors):
 def _on(device, fn, *args):
     """fn(*args, the current stream of the device) with the device current: a launch goes to the current device."""
     if device == torch._C._cuda_getDevice():
-        check(fn(*args, torch._C._cuda_getCurrentRawStream(device)))
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(device))
     else:
         with torch.cuda.device(device):
-            check(fn(*args, torch._C._cuda_getCurrentRawStream(device)))
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(device))
+    if rc:
+        check(rc)
 
 
 def _address(t):
@@ -412,10 +414,12 @@ def rope(x, positions, inv_freq, layout="half", scaling=1.0, inverse=False, out=
     _need_all(dev, ("positions", positions, torch.int32, (T,)), ("inv_freq", inv_freq, torch.float64, (pairs,)))
     if out is None:
         out = torch.empty(T, H, D, dtype=x.dtype, device=x.device)
-    elif out.dtype != x.dtype or out.shape != x.shape or out.get_device() != dev:
-        raise ValueError(f"out must be {x.dtype} of shape {tuple(x.shape)} on {x.device}")
+        ot, oh, od = H * D, D, 1
+    else:
+        if out.dtype != x.dtype or out.shape != x.shape or out.get_device() != dev:
+            raise ValueError(f"out must be {x.dtype} of shape {tuple(x.shape)} on {x.device}")
+        ot, oh, od = out.stride()
     xt, xh, xd = x.stride()
-    ot, oh, od = out.stride()
     if D > 1 and (xd != 1 or od != 1):
         raise ValueError("the last dim of x and out must be contiguous")
     if T == 0 or H == 0:

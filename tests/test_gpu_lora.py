@@ -110,6 +110,7 @@ def test_matches_64_bits(M, K, segments, n, R):
     (960, 64, (5120,), 3, 16),
     (1000, 128, (4096, 960), 2, 64),
     (803, 1088, (5072,), 300, 32),         # an adapter or two a row
+    (33000, 64, (16,), 3, 16),             # few features
 ])
 @pytest.mark.parametrize("residual", [False, True])
 def test_large_batches(M, K, segments, n, R, residual):

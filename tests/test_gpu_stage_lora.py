@@ -79,7 +79,9 @@ def _restore(kv, saved):
 BATCHES = {"decode": ((1, 1, 4, 7, 16), (300, 5, 1000, 0, 130), (0, -1, 1, 3, 2)),
            "verify": ((5,) * 20, tuple(range(10, 1010, 50)), tuple(i % 5 - 1 for i in range(20))),
            "prompts": ((200, 1, 90, 3), (0, 700, 64, 20), (1, 0, -1, 3)),
-           "one_prompt": ((260,), (37,), (1,))}
+           "one_prompt": ((260,), (37,), (1,)),
+           "long_prompt": ((1, 992, 3, 4), (5, 60, 700, 0), (2, 1, -1, 3)),
+           "longer_prompt": ((3, 1, 1500, 2), (0, 900, 17, 64), (0, 1, 1, 3))}
 
 
 @pytest.mark.parametrize("name", list(BATCHES))

@@ -209,6 +209,23 @@ def test_broken_adapters_and_rows_stay_apart(M):
     assert bool(got[4].isnan().all()) and bool(got[1, :128].float().isnan().any())
 
 
+@pytest.mark.parametrize("M,segments", [(300, (64, 64)), (1000, (4096, 1024))])
+@pytest.mark.parametrize("one", [False, True])
+def test_columns_past_a_rank_reach_nobody(M, segments, one):
+    """NaN and infinities past every rank, in tiles of one adapter and of several; then one adapter broken, others whole."""
+    c = _inputs(M, 192, segments, 5, 64, 20, ranks=[64, 41, 16, 33, 32])
+    adapter = torch.full((M,), 1, dtype=torch.int32, device=DEV) if one else torch.arange(M, device=DEV, dtype=torch.int32) % 6 - 1
+    want = _run(c, adapter)
+    _check(want, c, adapter)
+    for a, r in enumerate(c["ranks"].tolist()):
+        c["lora_b"][a, :, r:] = float("nan") if a % 2 else float("inf")
+        c["lora_a"].view(5, 2, 64, 192)[a, :, r:] = float("nan")
+    assert torch.equal(_run(c, adapter), want)
+    c["lora_b"][3], c["lora_a"][3] = float("nan"), float("inf")
+    fine = adapter != 3
+    assert torch.equal(_run(c, adapter)[fine], want[fine])
+
+
 def test_large_h_keeps_its_infinity():
     c = _inputs(3, 64, (32,), 1, 16, 9)
     c["scale"][:] = 3e38
@@ -255,6 +272,15 @@ def test_empty_batch_other_stream_and_two_at_once():
             got.append([_run(c, adapter) for _ in range(4)])
     torch.cuda.synchronize()
     assert all(torch.equal(g, want) for gs in got for g in gs)
+
+
+@pytest.mark.parametrize("M,segments", [(50, (1024, 64)), (500, (1024, 64)), (1000, (4096, 1024))])
+def test_calls_repeat_their_bits(M, segments):
+    c = _inputs(M, 2880, segments, 7, 32, 21)
+    adapter = _adapters(M, 7, 21)
+    want = _run(c, adapter)
+    for _ in range(30):
+        assert torch.equal(_run(c, adapter), want)
 
 
 @pytest.mark.parametrize("M", [6, 300])

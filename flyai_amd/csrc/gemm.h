@@ -42,10 +42,11 @@ __global__ __launch_bounds__(64 * WAVES, LORA ? 2 : 1) void gemm_splitk_bf16_ker
   typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
   __shared__ u32x4 as[kGemmRows][kKQW * 16 + 1];  // 64 rows x 512 bf16, +16 B per row vs bank conflicts
   if constexpr (LORA) {
-    typedef LoraDownLds<WAVES, kTiledMinRows / kDownRows> down_lds;
+    constexpr int kTiles = kTiledMinRows / kDownRows;
+    typedef LoraDownLds<WAVES, kTiles, kTiles> down_lds;
     static_assert(sizeof(as) >= sizeof(down_lds), "the down product's LDS");
     if ((int)blockIdx.x < wgs) {
-      lora_down<WAVES, kTiledMinRows / kDownRows>(x, M, K, lo, blockIdx.x, wgs, *reinterpret_cast<down_lds*>(as));
+      lora_down<WAVES, kTiles, kTiles>(x, M, K, lo, blockIdx.x, wgs, *reinterpret_cast<down_lds*>(as));
       return;
     }
   }
@@ -136,6 +137,5 @@ __global__ __launch_bounds__(64 * WAVES, LORA ? 2 : 1) void gemm_splitk_bf16_ker
 }
 
 int gemm_slices(int K);
-bool splitk_eight_waves(int M, int N, int slices);
 
 }  // namespace flyai

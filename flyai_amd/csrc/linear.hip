@@ -709,7 +709,7 @@ int gemm_planes(int M, int K) { return gemm_is_tiled(M) ? 1 : gemm_slices(K); }
 
 size_t linear_partials_bytes(int M, int N, int K) { return (size_t)gemm_slices(K) * M * N * sizeof(float); }
 
-bool splitk_eight_waves(int M, int N, int slices) {
+static bool splitk_eight_waves(int M, int N, int slices) {
   // Past 64 rows eight waves and 128 features a workgroup, where those workgroups have a CU each and those of four waves
   // would not.  With fewer, half of the chip is idle; with more, the second round is as long as the first.  Kernel and
   // finalize at 137 rows, four waves / eight: 512 x 512 (4 workgroups of eight waves) 11.0 / 15.0 us, 1,024 x 2,880

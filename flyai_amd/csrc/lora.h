@@ -44,33 +44,67 @@ __device__ __forceinline__ int lora_segment(const LoraArgs& a, int f) {
 }
 
 // ---- down ----------------------------------------------------------------------------------------------------------
-// The batch's work is the pairs of a 64-row tile and an adapter among its rows, times the groups of 32 rank columns in
-// every segment.  Each workgroup lists the pairs for itself (adapters of up to 64 * TILES rows in LDS, and how many distinct
-// ones each tile has) and takes every wgs-th item: none is launched in vain, whatever the mix.
-// An item multiplies the tile's rows that have the adapter, gathered, 16 to an MFMA tile, or (split) a half or a quarter of
-// them where the batch has few tiles, with 32 rows of A.  K is cut into
+// The batch's work is the pairs of a window of rows and an adapter among them, up to 64 of its rows at a time, times the
+// groups of 32 rank columns in every segment.  Each workgroup lists the pairs for itself (adapters of up to 64 * TILES rows
+// in LDS, and how many pairs each window has) and takes every wgs-th item: none is launched in vain, whatever the mix.
+// A window is WINDOW x 64 rows: wide ones gather an adapter's scattered rows into fewer items, but their list, a wave's, takes
+// longer.  Beside the split-K kernel all of its rows (100 rows of 24 adapters 20.4 us, with windows of 64 rows 25.0; 200 rows
+// 29.9 / 31.1); alone 128 (64 / 128 / 256: 2,096 rows of 12 adapters 20.6 / 17.3 / 18.8, 800 of 20 16.8 / 15.6 / 17.7, 1,000 of 20 at
+// K = 4,096 16.8 / 17.0 / 19.7, 2,096 of one 15.4 / 15.5 / 16.4).
+// An item multiplies the window's rows that have the adapter, gathered, 16 to an MFMA tile, or (split) a half or a quarter of
+// them where the batch has few, with 32 rows of A.  K is cut into
 // eight parts, summed in pairs and then in order through LDS, a wave one part or (with four waves) a pair of them; lane
 // (r, g) of an MFMA holds row r in its second operand, so a row's products never meet another row's: a row's h depends
 // neither on its tile nor on the launch.
 // What bounds it is how fast rows of x and A come from L2.  A wave loads whole 128-byte runs (8 rows an instruction) and
 // turns them round in LDS of its own (the tiled GEMM's swizzle); loaded as MFMA operands, 16 rows of 64 bytes an
-// instruction, every quarter of an instruction touched 16 lines, and 2,096 rows of 192 rank columns took 51 us; now 20.3.
+// instruction, every quarter of an instruction touched 16 lines, and 2,096 rows of 192 rank columns took 51 us; now 17.3.
 // h is kept as two bf16 terms, the value and what its rounding left out: 16 significant bits (2^-17 of d at most) for the
 // bytes of one fp32 value, and the up product takes them as they are.
 constexpr int kDownParts = 8;   // parts of K
-constexpr int kDownRows = 64;   // rows of a tile
+constexpr int kDownRows = 64;   // rows of an item
 constexpr int kDownCols = kLoraCols;
 
-template <int WAVES, int TILES>
+template <int WAVES, int TILES, int WINDOW>
 struct LoraDownLds {
   union {
     char stage[WAVES][(kDownRows + kDownCols) * 128];       // a wave's 64-K group: rows of x, rows of A
     float red[WAVES][kDownRows][kDownCols + 4];
   };
   int adapter[kDownRows * TILES];       // -1 where the row has none, or one of rank 0
-  int first[TILES + 1];                 // pairs before the tile
+  int first[TILES / WINDOW + 1];        // pairs before the window
   int of_seq[64 * WAVES], rank_of[64 * WAVES];
-  int row[WAVES][kDownRows];            // the item's rows within its tile, for each wave
+  int row[WAVES][kDownRows];            // the item's rows within its window, for each wave
+};
+
+// A window's rows by adapter, in a wave's lanes: take() finds the first adapter that is left, the rows that have it (of) and
+// their count, and they leave.
+template <int WINDOW>
+struct DownRows {
+  int key[WINDOW];
+  uint64_t left[WINDOW], of[WINDOW];
+  int ad, count;
+  __device__ __forceinline__ void start(int s, int adapter) { key[s] = adapter, left[s] = __ballot(adapter >= 0); }
+  __device__ __forceinline__ bool any() const {
+    uint64_t some = 0;
+#pragma unroll
+    for (int s = 0; s < WINDOW; ++s) some |= left[s];
+    return some;
+  }
+  __device__ __forceinline__ void take() {
+    int k = key[WINDOW - 1];
+    uint64_t from = left[WINDOW - 1];
+#pragma unroll
+    for (int s = WINDOW - 2; s >= 0; --s) k = left[s] ? key[s] : k, from = left[s] ? left[s] : from;
+    ad = __builtin_amdgcn_readlane(k, __builtin_ctzll(from));
+    count = 0;
+#pragma unroll
+    for (int s = 0; s < WINDOW; ++s) {
+      of[s] = __ballot(key[s] == ad);
+      left[s] &= ~of[s];
+      count += __builtin_popcountll(of[s]);
+    }
+  }
 };
 
 inline int lora_down_groups(const LoraArgs& a) { return a.n_seg * (lora_cols(a.R) / kDownCols); }
@@ -149,12 +183,13 @@ __device__ __forceinline__ void lora_down_part(const uint16_t* __restrict__ x, c
   }
 }
 
-template <int WAVES, int TILES>
+template <int WAVES, int TILES, int WINDOW>
 __device__ __forceinline__ void lora_down(const uint16_t* __restrict__ x, int M, int K, const LoraArgs& a, int wg, int wgs,
-                                          LoraDownLds<WAVES, TILES>& l) {
+                                          LoraDownLds<WAVES, TILES, WINDOW>& l) {
   constexpr int kThreads = 64 * WAVES, kPairs = kDownParts / WAVES;  // parts a wave
   static_assert(kPairs == 1 || kPairs == 2, "a wave takes a part or a pair");
-  constexpr int kMine = (TILES + WAVES - 1) / WAVES;  // tiles a wave lists
+  constexpr int kSpan = kDownRows * WINDOW;
+  constexpr int kWindows = TILES / WINDOW, kMine = (kWindows + WAVES - 1) / WAVES;  // windows a wave lists
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), r = lane & 15, g = lane >> 4;
   const int cols = lora_cols(a.R), per_seg = cols / kDownCols, groups = a.n_seg * per_seg;
   const int KG = (K + 63) / 64;
@@ -181,12 +216,15 @@ __device__ __forceinline__ void lora_down(const uint16_t* __restrict__ x, int M,
       todo &= ~__ballot(key1 == __builtin_amdgcn_readlane(key1, __builtin_ctzll(todo)));
   }
   for (int t0 = 0; t0 < M; t0 += kDownRows * TILES) {
-    const int rows = min(M - t0, kDownRows * TILES), tiles = (rows + kDownRows - 1) / kDownRows;
+    const int rows = min(M - t0, kDownRows * TILES), windows = (rows + kSpan - 1) / kSpan;
     if (!one) {
       if (t0) __syncthreads();
-      int fetched[kMine];
+      int fetched[kMine][WINDOW];
 #pragma unroll
-      for (int j = 0; j < kMine; ++j) fetched[j] = row_of[t0 + min(kDownRows * (wave + WAVES * j) + lane, rows - 1)];
+      for (int j = 0; j < kMine; ++j)
+#pragma unroll
+        for (int s = 0; s < WINDOW; ++s)
+          fetched[j][s] = row_of[t0 + min(kSpan * (wave + WAVES * j) + kDownRows * s + lane, rows - 1)];
       if (t0 == 0 && small) {
         if (tid < a.n) l.rank_of[tid] = min(max(a.ranks[tid], 0), a.R);
         if (a.row_seq && tid < a.n_seqs) l.of_seq[tid] = a.adapter[tid];
@@ -195,71 +233,103 @@ __device__ __forceinline__ void lora_down(const uint16_t* __restrict__ x, int M,
       __syncthreads();
 #pragma unroll
       for (int j = 0; j < kMine; ++j) {
-        const int t = wave + WAVES * j, i = kDownRows * t + lane;
-        if (t >= tiles) break;
-        int ad = fetched[j], rank = 0;
-        if (a.row_seq) {
-          const bool in = (unsigned)ad < (unsigned)a.n_seqs;
-          const int sq = in ? ad : 0;
-          ad = small ? l.of_seq[sq] : a.adapter[sq];
-          if (!in) ad = -1;
+        const int w = wave + WAVES * j;
+        if (w >= windows) break;
+        DownRows<WINDOW> left;
+#pragma unroll
+        for (int s = 0; s < WINDOW; ++s) {
+          const int i = kSpan * w + kDownRows * s + lane;
+          int ad = fetched[j][s], rank = 0;
+          if (a.row_seq) {
+            const bool in = (unsigned)ad < (unsigned)a.n_seqs;
+            const int sq = in ? ad : 0;
+            ad = small ? l.of_seq[sq] : a.adapter[sq];
+            if (!in) ad = -1;
+          }
+          if ((unsigned)ad < (unsigned)a.n) rank = small ? l.rank_of[ad] : min(max(a.ranks[ad], 0), a.R);
+          if (i >= rows || rank == 0) ad = -1;
+          l.adapter[i] = ad;
+          if (wg == 0 && i < rows) a.meta[t0 + i] = make_int2(ad, ad < 0 ? 0 : rank);
+          left.start(s, ad);
         }
-        if ((unsigned)ad < (unsigned)a.n) rank = small ? l.rank_of[ad] : min(max(a.ranks[ad], 0), a.R);
-        if (i >= rows || rank == 0) ad = -1;
-        l.adapter[i] = ad;
-        if (wg == 0 && i < rows) a.meta[t0 + i] = make_int2(ad, ad < 0 ? 0 : rank);
         int n = 0;
-        for (uint64_t todo = __ballot(ad >= 0); todo; ++n)
-          todo &= ~__ballot(ad == __builtin_amdgcn_readlane(ad, __builtin_ctzll(todo)));
-        if (lane == 0) l.first[t + 1] = n;
+        while (left.any()) {
+          left.take();
+          n += (left.count + kDownRows - 1) / kDownRows;
+        }
+        if (lane == 0) l.first[w + 1] = n;
       }
       __syncthreads();
       if (wave == 0) {  // running sums
-        static_assert(TILES <= 64, "a lane a tile");
-        int sum = lane < tiles ? l.first[lane + 1] : 0;
+        static_assert(kWindows <= 64, "a lane a window");
+        int sum = lane < windows ? l.first[lane + 1] : 0;
 #pragma unroll
-        for (int off = 1; off < TILES; off <<= 1) {
+        for (int off = 1; off < kWindows; off <<= 1) {
           const int o = __shfl_up(sum, off, 64);
           if (lane >= off) sum += o;
         }
-        if (lane < tiles) l.first[lane + 1] = sum;
+        if (lane < windows) l.first[lane + 1] = sum;
       }
       __syncthreads();
     }
-    const int pairs = one ? pairs1 : __builtin_amdgcn_readfirstlane(l.first[tiles]);
+    const int pairs = one ? pairs1 : __builtin_amdgcn_readfirstlane(l.first[windows]);
     // few items of many rows are split as far as the workgroups last: 512 rows of one adapter of 192 rank columns are 48 items
     // of 64 rows, 14.1 us, or 192 of 16, 10.4
     const int split = rows < 32 * pairs ? 1 : 4 * pairs * groups <= wgs ? 4 : 2 * pairs * groups <= wgs ? 2 : 1;
     const int items = pairs * groups * split;
-    const int before = one ? 0 : l.first[min(lane, tiles)];
+    const int before = one ? 0 : l.first[min(lane, windows)];
     // Long items first, and the second round's back from the last workgroup on, so that a short item is followed by another:
     // tiles of many adapters are often at one end of a batch, and the items of the other end are the longer (2,096 rows of 12
     // adapters 22.5 us -> 20.3, 800 rows of 20 20.7 -> 16.8).  Where rows share adapters, an adapter's groups of columns, which
     // read the same rows, go to one XCD, whose L2 then reads them once: 2,096 rows of one adapter 19.3 us -> 15.5, 4,096 of two
     // 30.7 -> 22; where they do not, it is 1,000 rows of 20 adapters 17.8 so and 16.8 in turn.
-    const bool back = !one && l.first[1] > pairs - l.first[tiles - 1];
+    const bool back = !one && l.first[1] > pairs - l.first[windows - 1];
     const int me = rows >= 32 * pairs && wg < wgs / 8 * 8 ? wg % 8 * (wgs / 8) + wg / 8 : wg;
     for (int round = 0; round * wgs < items; ++round) {
       const int turn = round * wgs + (round & 1 ? wgs - 1 - me : me);
       if (turn >= items) continue;
       const int it = back ? items - 1 - turn : turn;
-      const int q0 = it % split * (kDownRows / split), ig = it / split;  // the first of the item's rows
+      int q0 = it % split * (kDownRows / split);  // the first of the item's rows among the adapter's
+      const int ig = it / split;
       const int pair = ig / groups, seg = ig % groups / per_seg, c0 = ig % groups % per_seg * kDownCols;
-      const int tile = __builtin_popcountll(__ballot(lane < tiles && before <= pair)) - 1;  // the last that starts at or before it
-      const int nth = pair - __builtin_amdgcn_readlane(before, tile);
-      const int m0 = t0 + kDownRows * tile;
-      const int mine = one ? key1 : l.adapter[kDownRows * tile + lane];
-      uint64_t todo = __ballot(mine >= 0);
-      for (int i = 0; i < nth; ++i) todo &= ~__ballot(mine == __builtin_amdgcn_readlane(mine, __builtin_ctzll(todo)));
-      const int lead = __builtin_ctzll(todo), ad = __builtin_amdgcn_readlane(mine, lead);
-      const uint64_t rows_of = __ballot(mine == ad);
-      const int n = min(__builtin_popcountll(rows_of) - q0, kDownRows / split);
-      const int rank = one ? __builtin_amdgcn_readlane(rank1, lead)
-                           : __builtin_amdgcn_readfirstlane(small ? l.rank_of[ad] : min(max(a.ranks[ad], 0), a.R));
+      const uint64_t below = (1ull << lane) - 1;
+      int m0 = t0, ad, n, rank;
+      if (one) {
+        uint64_t todo = __ballot(key1 >= 0);
+        for (int i = 0; i < pair; ++i) todo &= ~__ballot(key1 == __builtin_amdgcn_readlane(key1, __builtin_ctzll(todo)));
+        const int lead = __builtin_ctzll(todo);
+        ad = __builtin_amdgcn_readlane(key1, lead), rank = __builtin_amdgcn_readlane(rank1, lead);
+        const uint64_t rows_of = __ballot(key1 == ad);
+        n = min(__builtin_popcountll(rows_of) - q0, kDownRows / split);
+        const int at = __builtin_popcountll(rows_of & below) - q0;
+        if (key1 == ad && at >= 0) l.row[wave][at] = lane;
+      } else {
+        const int w = __builtin_popcountll(__ballot(lane < windows && before <= pair)) - 1;  // the last that starts at or before it
+        int nth = pair - __builtin_amdgcn_readlane(before, w);
+        m0 += kSpan * w;
+        DownRows<WINDOW> left;
+#pragma unroll
+        for (int s = 0; s < WINDOW; ++s) left.start(s, l.adapter[kSpan * w + kDownRows * s + lane]);
+        for (;;) {
+          left.take();
+          const int parts = (left.count + kDownRows - 1) / kDownRows;
+          if (nth < parts) break;
+          nth -= parts;
+        }
+        ad = left.ad;
+        q0 += kDownRows * nth;
+        n = min(left.count - q0, kDownRows / split);
+        rank = __builtin_amdgcn_readfirstlane(small ? l.rank_of[ad] : min(max(a.ranks[ad], 0), a.R));
+        int past = -q0;
+#pragma unroll
+        for (int s = 0; s < WINDOW; ++s) {
+          const int at = past + __builtin_popcountll(left.of[s] & below);
+          if ((left.of[s] >> lane & 1) && at >= 0 && at < n) l.row[wave][at] = kDownRows * s + lane;
+          past += __builtin_popcountll(left.of[s]);
+        }
+      }
       if (n <= 0 || c0 >= rank) continue;  // the same in every wave: columns past the rank's last 32 are never read
       const float scale = a.scale[ad];
-      const int at = __builtin_popcountll(rows_of & ((1ull << lane) - 1)) - q0;
-      if (mine == ad && at >= 0) l.row[wave][at] = lane;
       asm volatile("" ::: "memory");  // a wave's LDS operations complete in order
       f32x4_t acc[4][2];
 #pragma unroll

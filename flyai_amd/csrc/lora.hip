@@ -19,11 +19,11 @@ int gemm_planes(int M, int K);
 
 // The down product by itself, for batches whose projection takes the tiled kernel (smaller ones have it in the
 // projection's launch, gemm_splitk_bf16_kernel).
-constexpr int kDownTiles = 64;
+constexpr int kDownTiles = 64, kDownWindow = 2;
 
 __global__ __launch_bounds__(64 * kDownParts) void lora_down_kernel(const uint16_t* __restrict__ x, int M, int K, LoraArgs a) {
-  __shared__ LoraDownLds<kDownParts, kDownTiles> lds;
-  lora_down<kDownParts, kDownTiles>(x, M, K, a, blockIdx.x, gridDim.x, lds);
+  __shared__ LoraDownLds<kDownParts, kDownTiles, kDownWindow> lds;
+  lora_down<kDownParts, kDownTiles, kDownWindow>(x, M, K, a, blockIdx.x, gridDim.x, lds);
 }
 
 // ---- up, and the projection's finalize ---------------------------------------------------------------------------
@@ -141,13 +141,15 @@ static size_t align256(size_t v) { return (v + 255) & ~(size_t)255; }
 
 static size_t partial_bytes(int M, int N, int K) { return (size_t)gemm_planes(M, K) * M * N * sizeof(float); }
 
-// No more workgroups than items there can be: a tile has at most as many adapters as rows, or as the bank.
-static int down_wgs(const LoraArgs& a, int M, int split, int wgs) {
-  return (int)std::min<int64_t>(wgs, (int64_t)ceil_div(M, kDownRows) * std::min({kDownRows, M, a.n}) * lora_down_groups(a) * split);
+// No more workgroups than items there can be: a window has at most as many adapters as rows, or as the bank, and one more
+// item for every 64 rows.
+static int down_wgs(const LoraArgs& a, int M, int span, int split, int wgs) {
+  const int64_t pairs = (int64_t)ceil_div(M, span) * std::min({span, M, a.n}) + (M - 1) / kDownRows;
+  return (int)std::min<int64_t>(wgs, pairs * lora_down_groups(a) * split);
 }
 
 int launch_lora_down(const uint16_t* x, int M, int K, const LoraArgs& a, hipStream_t s) {
-  hipLaunchKernelGGL(lora_down_kernel, dim3(down_wgs(a, M, 4, device_cus())), dim3(64 * kDownParts), 0, s, x, M, K, a);
+  hipLaunchKernelGGL(lora_down_kernel, dim3(down_wgs(a, M, kDownRows * kDownWindow, 4, device_cus())), dim3(64 * kDownParts), 0, s, x, M, K, a);
   return check_launch("lora_down");
 }
 
@@ -164,7 +166,7 @@ static int launch_gemm_lora(const uint16_t* x, const uint16_t* W, int M, int N, 
   // 2,880: 21.9 us with 12 workgroups for h, 26.7 with 48); and for more than two tiles of rows, where the projection's own
   // workgroups take long, at most one for every other CU.  24 adapters of 192 rank columns, 5,120 x 2,880, up to one a CU / half
   // of that: 30 rows 14.0 / 18.8 us, 64 rows 15.0 / 21.0, 100 rows 24.5 / 29.0, 200 rows 32.8 / 30.6
-  const int wgs = down_wgs(a, M, 1, M <= 2 * kDownRows ? device_cus() : device_cus() / 2);
+  const int wgs = down_wgs(a, M, kTiledMinRows, 1, M <= 2 * kDownRows ? device_cus() : device_cus() / 2);
   const int bxs = ceil_div(N, 64);
   hipLaunchKernelGGL((gemm_splitk_bf16_kernel<4, true>), dim3(wgs + bxs * *slices), dim3(256), 0, s, x, W, M, N, K, part, a, wgs, bxs);
   return check_launch("gemm_splitk_lora");

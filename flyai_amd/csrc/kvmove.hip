@@ -77,17 +77,23 @@ __global__ __launch_bounds__(kForkThreads) void kv_fork_kernel(ForkArgs a) {
 // 12 launches), 106 with parts of 1,024 in registers (whose unrolled code, 20 KB, cost a launch of 6 rows 18 us), now 62,
 // 4.3 TB/s; parts of 128, 512 and 1,024 take 67, 68 and 71.  1,501 scattered rows of 6,000 (two slabs, 12 layers): 98 us, 82
 // and 67, most of it for lines that few kept positions share.
+// Each part costs a workgroup some 1.2 us whatever it keeps, so where few positions stay the parts are wider, as many blocks
+// (16 to 64) as keep 256 positions at most, and V's elements are read one by one: 600 of 8,000 positions of one layer 38 us in
+// parts of 256, 13.4 in wide ones, 100 of 4,000 (two slabs, three layers) 22 and 5.3.  Parts of eight blocks so were slower (a
+// quarter of the positions kept: 76 us, 66 in parts of four).
 constexpr int kMoveThreads = 256;
 constexpr int kMoveBlocks = 4;    // 64-position blocks of a part
-constexpr int kMoveRow = 64 * kMoveBlocks + 8;  // a dim's positions in LDS, + 16 B vs bank conflicts
-constexpr int kMoveWords = 416;   // words of a launch: 26,624 positions
+constexpr int kMoveWide = 64;     // ... of a part that keeps few
+constexpr int kMoveKept = 64 * kMoveBlocks;  // positions that a part keeps at most
+constexpr int kMoveRow = kMoveKept + 8;      // a dim's positions in LDS, + 16 B vs bank conflicts
+constexpr int kMoveWords = 336;   // words of a launch: 21,504 positions
 constexpr int kMoveSlabs = 16;
 
 struct MoveSlab {
   int64_t base;
   int cap, dst;             // the first kept position goes to dst
   int block, first, words;  // words[first ..] are blocks block .. block + words - 1
-  int pad;
+  int part, kept;           // blocks of a part, positions kept in all
 };
 
 struct MoveArgs {
@@ -95,28 +101,46 @@ struct MoveArgs {
   int64_t layer;
   MoveSlab slab[kMoveSlabs];
   uint64_t words[kMoveWords];
+  uint16_t before[kMoveWords];  // positions that the slab's words before it keep
 };
 static_assert(sizeof(MoveArgs) <= 4096 && sizeof(ForkArgs) <= 4096, "kernel arguments are at most 4 KiB");
 
-__global__ __launch_bounds__(kMoveThreads) void kv_compact_kernel(MoveArgs a) {
-  __shared__ uint16_t kept[64 * kMoveBlocks];  // of the part: offsets from its first position
-  __shared__ __align__(16) uint16_t data[16 * kMoveRow];
+struct MoveLds {
+  uint16_t kept[kMoveKept];  // of the part: offsets from its first position
+  __align__(16) uint16_t data[16 * kMoveRow];
+  uint64_t bits[kMoveWords];  // WIDE: the slab's words and `before`, read once
+  int before[kMoveWords + 1];
+};
+
+// WIDE: parts of m.part blocks, kMoveBlocks otherwise.
+template <bool WIDE>
+__device__ __forceinline__ void compact_slab(const MoveArgs& a, const MoveSlab& m, MoveLds& l) {
+  uint16_t *kept = l.kept, *data = l.data;
+  uint64_t* bits = l.bits;
+  int* before = l.before;
   const int kind = blockIdx.x & 1, dq = (blockIdx.x >> 1) & 3, head = blockIdx.x >> 3;
-  const MoveSlab& m = a.slab[blockIdx.y];
   uint16_t* region = a.pool[kind] + blockIdx.z * a.layer + m.base + (int64_t)head * m.cap * 64;
   const int tid = threadIdx.x;
+  const int part = WIDE ? m.part : kMoveBlocks;
+  if constexpr (WIDE) {
+    for (int i = tid; i <= m.words; i += kMoveThreads) {
+      if (i < m.words) bits[i] = a.words[m.first + i];
+      before[i] = i < m.words ? a.before[m.first + i] : m.kept;
+    }
+    __syncthreads();
+  }
   int dst = m.dst;
-  for (int b0 = 0; b0 < m.words; b0 += kMoveBlocks) {
+  for (int b0 = 0; b0 < m.words; b0 += part) {
     const int p0 = 64 * (m.block + b0);
     uint64_t words[kMoveBlocks];
     int n = 0;
+    if constexpr (!WIDE) {
 #pragma unroll
-    for (int i = 0; i < kMoveBlocks; ++i) {
-      words[i] = b0 + i < m.words ? a.words[min(m.first + b0 + i, kMoveWords - 1)] : 0;
-      n += __builtin_popcountll(words[i]);
-    }
-    if (n == 0) continue;
-    {
+      for (int i = 0; i < kMoveBlocks; ++i) {
+        words[i] = b0 + i < m.words ? a.words[min(m.first + b0 + i, kMoveWords - 1)] : 0;
+        n += __builtin_popcountll(words[i]);
+      }
+      if (n == 0) continue;
       constexpr int kPer = 64 * kMoveBlocks / kMoveThreads;  // positions a thread
       const int blk = kPer * tid / 64, bit = kPer * tid % 64;
       uint64_t word = 0;
@@ -130,6 +154,17 @@ __global__ __launch_bounds__(kMoveThreads) void kv_compact_kernel(MoveArgs a) {
 #pragma unroll
       for (int i = 0; i < kPer; ++i)
         if (word >> (bit + i) & 1) kept[at++] = (uint16_t)(64 * blk + bit + i);
+    } else {
+      n = __builtin_amdgcn_readfirstlane(before[min(b0 + part, m.words)] - before[b0]);
+      if (n == 0) continue;
+      const int per = 64 * part / kMoveThreads;  // positions a thread, of one word
+      const int w = per * tid / 64, bit = per * tid % 64;
+      if (b0 + w < m.words) {
+        const uint64_t word = bits[b0 + w];
+        int at = before[b0 + w] - before[b0] + __builtin_popcountll(word & ((1ull << bit) - 1));
+        for (uint32_t some = word >> bit & ((1u << per) - 1); some; some &= some - 1)
+          kept[at++] = (uint16_t)(64 * w + bit + __builtin_ctz(some));
+      }
     }
     if (kind == 0) {
       // K: 16 dims of a row are two 16-byte chunks
@@ -143,18 +178,25 @@ __global__ __launch_bounds__(kMoveThreads) void kv_compact_kernel(MoveArgs a) {
         *reinterpret_cast<u32x4_t*>(region + kv_k_off(dst + (u >> 1), 16 * dq + 8 * (u & 1))) = reinterpret_cast<u32x4_t*>(data)[u];
     } else {
       // V: a chunk is one dim of eight positions; those with none kept are not read.  A destination chunk's elements come
-      // from wherever each lies.
-      constexpr int kBlocks = kMoveThreads / 16 / 8;  // that an iteration reads
-      static_assert(kMoveBlocks % kBlocks == 0 && kMoveThreads % 128 == 0, "whole iterations of whole blocks");
+      // from wherever each lies.  A wide part's are read one by one, in their order.
+      if constexpr (WIDE) {
+        __syncthreads();
+#pragma unroll 4
+        for (int u = tid; u < 16 * n; u += kMoveThreads)
+          data[(u & 15) * kMoveRow + (u >> 4)] = region[kv_v_off(p0 + kept[u >> 4], 16 * dq + (u & 15))];
+      } else {
+        constexpr int kBlocks = kMoveThreads / 16 / 8;  // that an iteration reads
+        static_assert(kMoveBlocks % kBlocks == 0 && kMoveThreads % 128 == 0, "whole iterations of whole blocks");
 #pragma unroll
-      for (int j = 0; j < 16 * 8 * kMoveBlocks / kMoveThreads; ++j) {
-        const int u = tid + kMoveThreads * j, d = u & 15, g = u >> 4;  // chunk: dim, eighth positions
-        uint64_t word = 0;
+        for (int j = 0; j < 16 * 8 * kMoveBlocks / kMoveThreads; ++j) {
+          const int u = tid + kMoveThreads * j, d = u & 15, g = u >> 4;  // chunk: dim, eighth positions
+          uint64_t word = 0;
 #pragma unroll
-        for (int i = 0; i < kBlocks; ++i)
-          if (g >> 3 == kBlocks * j + i) word = words[kBlocks * j + i];
-        if (word >> (8 * (g & 7)) & 255)
-          *reinterpret_cast<u32x4_t*>(data + d * kMoveRow + 8 * g) = *reinterpret_cast<const u32x4_t*>(region + kv_v_off(p0 + 8 * g, 16 * dq + d));
+          for (int i = 0; i < kBlocks; ++i)
+            if (g >> 3 == kBlocks * j + i) word = words[kBlocks * j + i];
+          if (word >> (8 * (g & 7)) & 255)
+            *reinterpret_cast<u32x4_t*>(data + d * kMoveRow + 8 * g) = *reinterpret_cast<const u32x4_t*>(region + kv_v_off(p0 + 8 * g, 16 * dq + d));
+        }
       }
       __syncthreads();
       const int g0 = dst >> 3, units = 16 * (((dst + n - 1) >> 3) - g0 + 1);
@@ -162,7 +204,10 @@ __global__ __launch_bounds__(kMoveThreads) void kv_compact_kernel(MoveArgs a) {
         const int d = u & 15, at = 8 * (g0 + (u >> 4)), i0 = at - dst;
         uint16_t e[8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) e[i] = data[d * kMoveRow + kept[min(max(i0 + i, 0), n - 1)]];
+        for (int i = 0; i < 8; ++i) {
+          const int at_i = min(max(i0 + i, 0), n - 1);
+          e[i] = data[d * kMoveRow + (WIDE ? at_i : kept[at_i])];
+        }
         uint16_t* to = region + kv_v_off(at, 16 * dq + d);
         if (i0 >= 0 && i0 + 7 < n) {
           u32x4_t w;
@@ -179,6 +224,13 @@ __global__ __launch_bounds__(kMoveThreads) void kv_compact_kernel(MoveArgs a) {
     __syncthreads();  // the part's LDS is free again
     dst += n;
   }
+}
+
+__global__ __launch_bounds__(kMoveThreads) void kv_compact_kernel(MoveArgs a) {
+  __shared__ MoveLds lds;
+  const MoveSlab& m = a.slab[blockIdx.y];
+  if (m.part > kMoveBlocks) compact_slab<true>(a, m, lds);
+  else compact_slab<false>(a, m, lds);
 }
 
 static int check_slab(const char* what, int64_t base, int cap, int heads, int64_t pool_elems) {
@@ -314,13 +366,22 @@ extern "C" int flyai_kv_compact(uint16_t* k_pool, uint16_t* v_pool, int64_t laye
       // a slab's kept positions go into one launch as far as its words last; the next launch takes up from there
       if (slabs == kMoveSlabs || words == kMoveWords) RUN(flush());
       MoveSlab& out = a.slab[slabs++];
-      out = MoveSlab{m.base, m.cap, m.start + r, (m.start + keep[r]) >> 6, words, 0, 0};
+      out = MoveSlab{m.base, m.cap, m.start + r, (m.start + keep[r]) >> 6, words, 0, kMoveWide, -r};
       for (; r < m.n; ++r) {
         const int pos = m.start + keep[r], w = (pos >> 6) - out.block;
         if (out.first + w >= kMoveWords) break;
         for (; out.words <= w; ++out.words) a.words[words++] = 0;
         a.words[out.first + w] |= 1ull << (pos & 63);
       }
+      out.kept += r;
+      // the widest parts none of which keeps too many, from 1,024 positions on
+      for (int w = 0, n = 0; w < out.words; ++w) a.before[out.first + w] = (uint16_t)n, n += __builtin_popcountll(a.words[out.first + w]);
+      auto fits = [&](int part) {
+        for (int w = 0; w < out.words; w += part)
+          if ((w + part < out.words ? a.before[out.first + w + part] : out.kept) - a.before[out.first + w] > kMoveKept) return false;
+        return true;
+      };
+      while (out.part > kMoveBlocks && (out.part == 2 * kMoveBlocks || out.words <= out.part / 2 || !fits(out.part))) out.part /= 2;
       if (r < m.n) RUN(flush());  // the rest moves into positions that this piece reads
     }
   }

@@ -490,7 +490,7 @@ def _packed(layout, rows):
 
 def kv_compact(k, v, n_kv_heads, moves):
     """For each move (base, cap, start, keep): position start + i of the slab takes what position start + keep[i] held
-    before the call, every layer, in one launch (or one per 26,624 positions).  keep: host integers (list, numpy or CPU
+    before the call, every layer, in one launch (or one per 21,504 positions).  keep: host integers (list, numpy or CPU
     tensor), strictly ascending.  The moves' slabs must not overlap."""
     L, n, dev = _kv_pools(k, v)
     keeps = [_host_positions(m[3]) for m in moves]

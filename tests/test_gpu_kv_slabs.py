@@ -94,6 +94,23 @@ def test_compact(name):
     assert torch.equal(_bits(k), _bits(wk)) and torch.equal(_bits(v), _bits(wv))
 
 
+@pytest.mark.parametrize("rows,span", [(1, 9000), (40, 9000), (255, 4000), (600, 9000), (1100, 9000), (2100, 9000), (4600, 9000),
+                                       (257, 300), (9, 600)])
+@pytest.mark.parametrize("start", [0, 45])
+def test_compact_by_density(rows, span, start):
+    """From a few positions of a long context to half of them, and all of them in one stretch of it."""
+    heads, cap = 2, 9088
+    rng = np.random.RandomState(rows)
+    k, v = _pools(2, heads * cap * 64, 6)
+    for shift in (0, 9000 - span):
+        keep = shift + np.sort(rng.choice(span, rows, replace=False))
+        src, dst = start + keep, start + np.arange(rows)
+        wk, wv = _moved(k, "k", heads, src, dst, (0, cap), (0, cap)), _moved(v, "v", heads, src, dst, (0, cap), (0, cap))
+        gk, gv = k.clone(), v.clone()
+        ops.kv_compact(gk, gv, heads, [(0, cap, start, keep)])
+        assert torch.equal(_bits(gk), _bits(wk)) and torch.equal(_bits(gv), _bits(wv))
+
+
 def test_compact_past_one_launch():
     """More positions than one launch's words: pieces of a long slab, beside a short one."""
     heads, cap = 1, 60032

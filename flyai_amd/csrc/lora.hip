@@ -70,15 +70,18 @@ __global__ __launch_bounds__(256) void lora_finalize_kernel(const float* __restr
   if (todo) {
     int ad = -1, rank = 0;
     u32x4_t nb[2];
+    uint32_t off[2];  // of the lane's chunks in an adapter's rows from f0 on
+#pragma unroll
+    for (int i = 0; i < 2; ++i) off[i] = (8 * i + (lane >> 3)) * a.R + lora_chunk(8 * i, 0, a.R);
     auto next = [&]() __attribute__((always_inline)) {
       ad = -1;
       if (!todo) return;
       const int first = __builtin_ctzll(todo);
       ad = __builtin_amdgcn_readlane(key, first), rank = __builtin_amdgcn_readlane(who.y, first);
       todo &= ~__ballot(key == ad);
+      const uint16_t* B = a.B + ((size_t)ad * N + f0) * a.R;
 #pragma unroll
-      for (int i = 0; i < 2; ++i)
-        nb[i] = *reinterpret_cast<const u32x4_t*>(a.B + ((size_t)ad * N + f0 + 8 * i + (lane >> 3)) * a.R + lora_chunk(8 * i, 0, a.R));
+      for (int i = 0; i < 2; ++i) nb[i] = *reinterpret_cast<const u32x4_t*>(B + off[i]);
     };
     next();
 #pragma unroll

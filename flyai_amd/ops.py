@@ -345,8 +345,9 @@ def _address(t):
 
 
 @functools.lru_cache(maxsize=64)
-def _int32s(values):
-    return (C.c_int32 * len(values))(*values)
+def _segments(widths):
+    """(how many, their int32 array)."""
+    return len(widths), (C.c_int32 * len(widths))(*map(_position, widths))
 
 
 @functools.lru_cache(maxsize=256)
@@ -363,8 +364,7 @@ def linear_lora(x, w, b, lora_a, lora_b, scale, ranks, adapter, segments=None, r
     [0, n) mean no adapter, and such a row has ``linear``'s bits.  A row's result depends on that row alone."""
     M, K = x.shape
     N = w.shape[0]
-    segments = (N,) if segments is None else tuple(_position(v) for v in segments)
-    S = len(segments)
+    S, widths = _segments((N,) if segments is None else tuple(segments))
     if lora_b.dim() != 3:
         raise ValueError("lora_b must be [adapters, N, R]")
     n, _, R = lora_b.shape
@@ -384,7 +384,7 @@ def linear_lora(x, w, b, lora_a, lora_b, scale, ranks, adapter, segments=None, r
         y = torch.empty(M, N, dtype=bf16, device=x.device)
     ws = torch.empty(_lora_workspace_bytes(M, N, K, R, S), dtype=torch.uint8, device=x.device)
     _on(dev, lib().flyai_linear_lora_bf16, x.data_ptr(), w.data_ptr(), _address(b), M, N, K, lora_a.data_ptr(),
-        lora_b.data_ptr(), scale.data_ptr(), ranks.data_ptr(), n, R, _int32s(segments), S, adapter.data_ptr(),
+        lora_b.data_ptr(), scale.data_ptr(), ranks.data_ptr(), n, R, widths, S, adapter.data_ptr(),
         _address(row_seq), n_ids, _address(y), _address(residual), ws.data_ptr())
     return residual if residual is not None else y
 

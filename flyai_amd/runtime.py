@@ -27,6 +27,12 @@ def _round_up(v, m):
     return (v + m - 1) // m * m
 
 
+def _int32(v):
+    """v for a C int: what is out of its range goes to the nearest end, which the C checks refuse (ctypes would take it
+    modulo 2^32)."""
+    return min(max(int(v), -0x80000000), 0x7fffffff)
+
+
 class KVWorkspace:
     """Per-layer K/V pools holding ``n_slots`` sequence slabs in the tiled layout of
     ``flyai_amd.kvlayout`` (what the attention kernel streams).  Every slab holds ``maxlen`` positions,
@@ -279,7 +285,8 @@ class RaggedStage:
         de = np.ascontiguousarray(dep, dtype=np.int32)
         check(lib().flyai_stage_forward_tree_lora(
             self._h, int(start), M, pa.ctypes.data_as(C.c_void_p), de.ctypes.data_as(C.c_void_p),
-            self.kv.base(int(slot)), self.kv.slot_cap(int(slot)), -1 if adapter is None else int(adapter), C.c_void_p(hidden.data_ptr()),
+            self.kv.base(int(slot)), self.kv.slot_cap(int(slot)), -1 if adapter is None else _int32(adapter),
+            C.c_void_p(hidden.data_ptr()),
             C.c_void_p(torch.cuda.current_stream(self.device).cuda_stream)))
         return hidden
 

@@ -1,0 +1,53 @@
+"""Edges of the calls that serve many requests, on the host: what a C argument would take modulo 2^32, and what is refused
+before a launch.  The stage is bound to addresses that are never read; a call that passes every check stops at the unset
+workspace."""
+import ctypes as C
+from types import SimpleNamespace
+
+import pytest
+import torch
+
+from flyai_amd import _lib
+from flyai_amd._lib import FlyaiError
+from flyai_amd.runtime import KVWorkspace, RaggedStage
+
+FAKE = 0x100000
+HIDDEN, CAP = 64, 128
+
+
+@pytest.fixture
+def stage(monkeypatch):
+    """A RaggedStage of one layer with a bank of two adapters, and no workspace."""
+    lib = _lib.lib()
+    cfg = _lib.StageConfig(n_layers=1, hidden=HIDDEN, n_q_heads=8, n_kv_heads=1, head_dim=64, n_experts=4, top_k=2, intermediate=64,
+                           window=128, max_tokens=64, max_seqs=4, max_attn_items=64, rope_positions=4096, attn_split_keys=1024,
+                           rms_eps=1e-5, attn_prefill_min=32)
+    h = C.c_void_p()
+    assert lib.flyai_stage_create(C.byref(cfg), C.byref(h)) == 0
+    kv = KVWorkspace(1, 2, CAP, 1, 64, "cpu")
+    names = ("ln1", "ln2", "wqkv", "bqkv", "wo", "bo", "sinks", "router_w", "router_b", "w13_packed", "b13", "w2_packed", "b2",
+             "k_pool", "v_pool")
+    d = _lib.LayerDesc(**{f: FAKE for f in names}, sliding=0, pad=0, kv_pool_elems=kv.k[0].numel())
+    assert lib.flyai_stage_set_layer(h, 0, C.byref(d)) == 0
+    rows = (_lib.LoraLayer * 1)(_lib.LoraLayer(FAKE, FAKE, FAKE, FAKE))
+    bank = _lib.StageLora(2, 16, FAKE, FAKE, rows, FAKE, int(lib.flyai_stage_lora_workspace_bytes(h, 16)))
+    assert lib.flyai_stage_set_lora(h, C.byref(bank)) == 0
+    st = object.__new__(RaggedStage)
+    st.__dict__.update(_h=h, _destroy=lib.flyai_stage_destroy, _sync=lambda d: None, device=torch.device("cpu"), kv=kv,
+                       shape=SimpleNamespace(hidden=HIDDEN))
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda d=None: SimpleNamespace(cuda_stream=None))
+    return st
+
+
+def _tree(st, start=3, **kw):
+    return st.forward_tree(torch.zeros(2, HIDDEN, dtype=torch.bfloat16), start, [-1, 0], [0, 1], 0, **kw)
+
+
+def test_adapter_ids_past_32_bits(stage):
+    """An id is the bank's or refused: taken modulo 2^32, 2^32 would be adapter 0 and 2^32 - 1 none."""
+    for good in (None, -1, 0, 1):
+        with pytest.raises(FlyaiError, match="workspace not set"):
+            _tree(stage, adapter=good)
+    for bad in (2, -2, 2 ** 31, 2 ** 32 - 1, 2 ** 32, 2 ** 32 + 1, -2 ** 32, -2 ** 32 - 1, 2 ** 64):
+        with pytest.raises(FlyaiError, match="outside"):
+            _tree(stage, adapter=bad)

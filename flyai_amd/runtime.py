@@ -250,14 +250,15 @@ class RaggedStage:
         if len(set(int(s) for s in slots)) != S:
             raise ValueError("two sequences of one step share a KV slot (their K/V writes would race)")
         ql = np.ascontiguousarray(q_lens, dtype=np.int32)
-        st = np.ascontiguousarray(starts, dtype=np.int32)
+        at = np.asarray(starts, dtype=np.int64)
         base = np.ascontiguousarray([self.kv.base(int(s)) for s in slots], dtype=np.int64)
         cap = np.ascontiguousarray([self.kv.slot_cap(int(s)) for s in slots], dtype=np.int32)
         lim = np.asarray([self.kv.maxlens[int(s)] for s in slots], dtype=np.int64)
-        need = st.astype(np.int64) + ql
-        if np.any(need > lim):
-            b = int(np.argmax(need > lim))
-            raise ContextOverflow(_lib.FLYAI_ERANGE, f"sequence {b} needs {int(need[b])} positions > max_ctx {int(lim[b])}")
+        over = at > lim - ql
+        if np.any(over):
+            b = int(np.argmax(over))
+            raise ContextOverflow(_lib.FLYAI_ERANGE, f"sequence {b} needs {int(at[b]) + int(ql[b])} positions > max_ctx {int(lim[b])}")
+        st = np.ascontiguousarray(np.maximum(at, -1), dtype=np.int32)  # below it too it is refused, not taken modulo 2^32
         ad = None
         if adapters is not None:
             if len(adapters) != S:
@@ -284,7 +285,7 @@ class RaggedStage:
         pa = np.ascontiguousarray(par, dtype=np.int32)
         de = np.ascontiguousarray(dep, dtype=np.int32)
         check(lib().flyai_stage_forward_tree_lora(
-            self._h, int(start), M, pa.ctypes.data_as(C.c_void_p), de.ctypes.data_as(C.c_void_p),
+            self._h, _int32(start), M, pa.ctypes.data_as(C.c_void_p), de.ctypes.data_as(C.c_void_p),
             self.kv.base(int(slot)), self.kv.slot_cap(int(slot)), -1 if adapter is None else _int32(adapter),
             C.c_void_p(hidden.data_ptr()),
             C.c_void_p(torch.cuda.current_stream(self.device).cuda_stream)))

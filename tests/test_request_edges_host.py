@@ -4,11 +4,12 @@ workspace."""
 import ctypes as C
 from types import SimpleNamespace
 
+import numpy as np
 import pytest
 import torch
 
 from flyai_amd import _lib
-from flyai_amd._lib import FlyaiError
+from flyai_amd._lib import ContextOverflow, FlyaiError
 from flyai_amd.runtime import KVWorkspace, RaggedStage
 
 FAKE = 0x100000
@@ -51,3 +52,23 @@ def test_adapter_ids_past_32_bits(stage):
     for bad in (2, -2, 2 ** 31, 2 ** 32 - 1, 2 ** 32, 2 ** 32 + 1, -2 ** 32, -2 ** 32 - 1, 2 ** 64):
         with pytest.raises(FlyaiError, match="outside"):
             _tree(stage, adapter=bad)
+
+
+def test_starts_past_32_bits(stage):
+    """A position past the context overflows it: taken modulo 2^32, 2^32 would write K/V over the first positions."""
+    with pytest.raises(FlyaiError, match="workspace not set"):
+        _tree(stage, CAP - 2)
+    rows = torch.zeros(2, HIDDEN, dtype=torch.bfloat16)
+    step = lambda starts: stage.forward(rows, [1, 1], starts, [0, 1])
+    with pytest.raises(FlyaiError, match="workspace not set"):
+        step(np.array([CAP - 1, 0]))
+    for far in (CAP, 2 ** 31, 2 ** 32, 2 ** 32 + 5, 2 ** 62):
+        with pytest.raises(ContextOverflow):
+            _tree(stage, far)
+        with pytest.raises(ContextOverflow):
+            step(np.array([0, far]))
+    for below in (-1, -2 ** 32, -2 ** 32 + 3):
+        with pytest.raises(FlyaiError, match="start"):
+            _tree(stage, below)
+        with pytest.raises(FlyaiError, match="start"):
+            step(np.array([0, below]))

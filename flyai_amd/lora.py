@@ -77,7 +77,7 @@ class AdapterBank:
         self.ranks[self._slot(index)] = 0
 
     def bind(self, stage):
-        """Bind the bank to a stage (its C handle) -> the workspace, to be kept as long as the binding."""
+        """Bind the bank to a stage (its C handle) -> the workspace, to be kept as long as the binding and the steps that use it."""
         size = int(lib().flyai_stage_lora_workspace_bytes(stage, self.max_rank))
         ws = torch.empty(size + 256, dtype=torch.uint8, device=self.scale.device)
         ptr = ws.data_ptr() + (-ws.data_ptr()) % 256

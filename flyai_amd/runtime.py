@@ -175,8 +175,9 @@ class RaggedStage:
             self.set_lora(lora)
 
     def set_lora(self, bank):
-        """Bind an ``AdapterBank`` (None: unbind).  Drops every captured step graph."""
+        """Bind an ``AdapterBank`` (None: unbind).  Waits for the device; drops every captured step graph."""
         if bank is None:
+            self._sync(self.device)
             check(lib().flyai_stage_set_lora(self._h, None))
             self.lora = self._lora_ws = None
             return
@@ -184,6 +185,8 @@ class RaggedStage:
             raise ValueError("the adapter bank is of another shape or number of layers")
         if bank.scale.device != self.workspace.device:
             raise ValueError(f"the adapter bank is on {bank.scale.device}, the stage on {self.workspace.device}")
+        # a step on another stream may still use the workspace that is dropped, or the memory that the new one gets
+        self._sync(self.device)
         ws = bank.bind(self._h)
         self.lora, self._lora_ws = bank, ws
 
@@ -203,8 +206,9 @@ class RaggedStage:
         self.layers[i] = lw
 
     def set_workspace(self):
-        """Bind a freshly allocated device workspace (and the pinned staging).  Drops every captured
-        step graph."""
+        """Bind a freshly allocated device workspace (and the pinned staging).  Waits for the device (as ``set_lora``);
+        drops every captured step graph."""
+        self._sync(self.device)
         dev_bytes = int(lib().flyai_stage_workspace_bytes(self._h))
         ws = torch.empty(dev_bytes + 256, dtype=torch.uint8, device=self.device)
         ptr = ws.data_ptr() + (-ws.data_ptr()) % 256

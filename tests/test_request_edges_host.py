@@ -2,6 +2,7 @@
 before a launch.  The stage is bound to addresses that are never read; a call that passes every check stops at the unset
 workspace."""
 import ctypes as C
+import weakref
 from types import SimpleNamespace
 
 import numpy as np
@@ -72,3 +73,31 @@ def test_starts_past_32_bits(stage):
             _tree(stage, below)
         with pytest.raises(FlyaiError, match="start"):
             step(np.array([0, below]))
+
+
+def test_rebinding_waits_for_running_steps(stage, monkeypatch):
+    """A step on another stream may still use the adapters' workspace, the bank or the stage's workspace when they are bound anew:
+    the device is waited for while the old ones are held, and before the next step may use the new one's memory."""
+    from flyai_amd import runtime
+    from flyai_amd.lora import AdapterBank
+    from flyai_amd.weights import GptOssShape
+
+    stage.shape = GptOssShape(hidden=HIDDEN, n_q_heads=8, n_kv_heads=1, head_dim=64)
+    stage.layers, stage.workspace, stage.lora, stage._lora_ws = [None], torch.empty(1), None, None
+    bank = lambda: AdapterBank(stage.shape, 1, 2, 16, "cpu")
+    waits = []
+    for new in (bank(), bank(), None):
+        old = weakref.ref(stage._lora_ws) if stage._lora_ws is not None else lambda: True
+        old_bank = weakref.ref(stage.lora) if stage.lora is not None else lambda: True
+        stage._sync = lambda d: waits.append(old() is not None and old_bank() is not None)
+        stage.set_lora(new)
+        assert waits and all(waits) and (stage._lora_ws is None) == (new is None) and stage.lora is new
+        del new
+        waits.clear()
+    # the stage's own workspace (the C call needs a device: here it only says how large)
+    monkeypatch.setattr(runtime, "lib", lambda: SimpleNamespace(flyai_stage_workspace_bytes=lambda h: 512,
+                                                                flyai_stage_set_workspace=lambda *a: 0))
+    stage.staging, old = torch.empty(8), weakref.ref(stage.workspace)
+    stage._sync = lambda d: waits.append(old() is not None)
+    stage.set_workspace()
+    assert waits and all(waits) and old() is None

@@ -1027,18 +1027,16 @@ int launch_qkv_rope_kv(const uint16_t* x, const uint16_t* Wqkv, const uint16_t* 
     const int tiles = ceil_div(width, kTileN) * ceil_div(T, kTileM);
     const QkvEpilogue ep{bqkv, positions, seq_id, cos_tab, sin_tab, kv_base, kv_cap, q_out, k_pool, v_pool,
                          rope_positions, Hq, Hkv};
-    if (lo && gemm_tiled_lora_fits(T, H, *lo)) {
+    if (lo) {  // heads of 64: no wave's features straddle two segments
       const int rc = launch_lora_down(x, T, H, *lo, s);
       if (rc) return rc;
       hipLaunchKernelGGL((gemm_tiled_lds_kernel<kEpiQkv, true>), dim3(8 * ceil_div(tiles, 8)), dim3(64 * kTiledWaves), 0, s, x,
                          Wqkv, T, width, H, part, ep, LinearEpilogue{}, *lo);
       return check_launch("gemm_tiled_lds_qkv_lora");
     }
-    if (!lo) {
-      hipLaunchKernelGGL((gemm_tiled_lds_kernel<kEpiQkv, false>), dim3(8 * ceil_div(tiles, 8)), dim3(64 * kTiledWaves), 0, s, x,
-                         Wqkv, T, width, H, part, ep, LinearEpilogue{}, LoraArgs{});
-      return check_launch("gemm_tiled_lds_qkv");
-    }
+    hipLaunchKernelGGL((gemm_tiled_lds_kernel<kEpiQkv, false>), dim3(8 * ceil_div(tiles, 8)), dim3(64 * kTiledWaves), 0, s, x,
+                       Wqkv, T, width, H, part, ep, LinearEpilogue{}, LoraArgs{});
+    return check_launch("gemm_tiled_lds_qkv");
   }
   int slices = 0;
   int rc = gemm_with(lo, x, Wqkv, T, width, H, part, &slices, s);

@@ -177,7 +177,9 @@ static int launch_gemm_lora(const uint16_t* x, const uint16_t* W, int M, int N, 
 
 int launch_gemm_lora_planes(const uint16_t* x, const uint16_t* W, int M, int N, int K, float* part, int* slices, const LoraArgs& a,
                             hipStream_t s) {
-  if (gemm_tiled_lora_fits(M, K, a)) {
+  if (gemm_is_tiled(M)) {
+    // a stage's K and segments are multiples of 64 (flyai_stage_create), and it keeps room for one plane from here on
+    FLYAI_REQUIRE(gemm_tiled_lora_fits(M, K, a), "lora: planes of %d rows need K and segments in multiples of 64", M);
     *slices = 1;
     const int rc = launch_lora_down(x, M, K, a, s);
     if (rc) return rc;

@@ -101,3 +101,13 @@ def test_rebinding_waits_for_running_steps(stage, monkeypatch):
     stage._sync = lambda d: waits.append(old() is not None)
     stage.set_workspace()
     assert waits and all(waits) and old() is None
+
+
+@pytest.mark.parametrize("change", [{"hidden": 96}, {"hidden": 32}, {"head_dim": 32}, {"head_dim": 128}])
+def test_stages_are_of_whole_tiles(change):
+    """What a step with adapters rests on from 256 rows on: K and the q, k and v segments in multiples of 64, one plane of sums."""
+    sizes = dict(n_layers=1, hidden=HIDDEN, n_q_heads=8, n_kv_heads=1, head_dim=64, n_experts=4, top_k=2, intermediate=64, window=128,
+                 max_tokens=300, max_seqs=4, max_attn_items=64, rope_positions=4096, attn_split_keys=1024, rms_eps=1e-5,
+                 attn_prefill_min=32)
+    cfg, h = _lib.StageConfig(**{**sizes, **change}), C.c_void_p()
+    assert _lib.lib().flyai_stage_create(C.byref(cfg), C.byref(h)) == _lib.FLYAI_EINVAL and not h

@@ -200,9 +200,10 @@ void lora_bind(LoraArgs* a, char* ws, int M) {
 int launch_linear_lora(const uint16_t* x, const uint16_t* W, const uint16_t* b, int M, int N, int K, LoraArgs a, uint16_t* y,
                        uint16_t* residual, char* ws, hipStream_t s) {
   float* part = reinterpret_cast<float*>(ws);
-  lora_bind(&a, ws + align256(partial_bytes(M, N, K)), M);
+  const bool ends = gemm_tiled_lora_fits(M, K, a);  // the tiled kernel ends the projection: no planes
+  lora_bind(&a, ws + (ends ? 0 : align256(partial_bytes(M, N, K))), M);
   int slices = 0, rc;
-  if (gemm_tiled_lora_fits(M, K, a)) {
+  if (ends) {
     rc = launch_lora_down(x, M, K, a, s);
     if (rc) return rc;
     return (gemm_tall_pays(M, N) ? launch_gemm_tall_lora : launch_gemm_tiled_lora)(x, W, b, M, N, K, nullptr, y, residual, a, s);
@@ -237,7 +238,9 @@ using namespace flyai;
 
 extern "C" size_t flyai_linear_lora_workspace_bytes(int32_t M, int32_t N, int32_t K, int32_t R, int32_t n_segments) {
   if (M <= 0 || N <= 0 || K <= 0 || R <= 0 || n_segments <= 0) return 0;
-  return align256(partial_bytes(M, N, K)) + lora_h_bytes(M, R, n_segments);
+  // of several segments the widths are not known here: they may straddle a wave's features
+  const bool ends = gemm_is_tiled(M) && K % 64 == 0 && n_segments == 1;
+  return (ends ? 0 : align256(partial_bytes(M, N, K))) + lora_h_bytes(M, R, n_segments);
 }
 
 extern "C" int flyai_linear_lora_bf16(const uint16_t* x, const uint16_t* w, const uint16_t* b, int32_t M, int32_t N,

@@ -111,3 +111,14 @@ def test_stages_are_of_whole_tiles(change):
                  attn_prefill_min=32)
     cfg, h = _lib.StageConfig(**{**sizes, **change}), C.c_void_p()
     assert _lib.lib().flyai_stage_create(C.byref(cfg), C.byref(h)) == _lib.FLYAI_EINVAL and not h
+
+
+def test_lora_workspace_has_no_plane_that_no_kernel_writes():
+    """One segment and K % 64 == 0: from 256 rows on the tiled kernel ends the projection, and h is all that is kept."""
+    size = lambda *a: int(_lib.lib().flyai_linear_lora_workspace_bytes(*a))
+    for M, N, K, R in ((256, 2880, 4096, 64), (2096, 2880, 4096, 16), (1 << 19, 5120, 2880, 128)):
+        h = M * ((R + 31) // 32 * 32) * 4 + M * 8                # two bf16 terms a column; adapter and rank
+        assert h <= size(M, N, K, R, 1) <= h + 512
+        assert size(M, N, K - 32, R, 1) >= h + 4 * M * N         # another kernel's, with a finalize behind it
+        assert size(M, N, K, R, 2) >= 2 * h - 8 * M + 4 * M * N  # segments may straddle a wave's features
+    assert size(255, 2880, 4096, 64, 1) >= 255 * (8 * 2880 * 4 + 64 * 4 + 8)

@@ -344,9 +344,13 @@ def _address(t):
     return t.data_ptr() if t is not None else None
 
 
-@functools.lru_cache(maxsize=64)
 def _segments(widths):
-    """(how many, their int32 array)."""
+    """(how many, their int32 array), the array made once for the same widths."""
+    return _segment_array(tuple([operator.index(w) for w in widths]))
+
+
+@functools.lru_cache(maxsize=64)
+def _segment_array(widths):
     return len(widths), (C.c_int32 * len(widths))(*map(_position, widths))
 
 
@@ -364,7 +368,7 @@ def linear_lora(x, w, b, lora_a, lora_b, scale, ranks, adapter, segments=None, r
     [0, n) mean no adapter, and such a row has ``linear``'s bits.  A row's result depends on that row alone."""
     M, K = x.shape
     N = w.shape[0]
-    S, widths = _segments((N,) if segments is None else tuple(segments))
+    S, widths = _segments((N,) if segments is None else segments)
     if lora_b.dim() != 3:
         raise ValueError("lora_b must be [adapters, N, R]")
     n, _, R = lora_b.shape

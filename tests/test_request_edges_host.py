@@ -9,7 +9,7 @@ import numpy as np
 import pytest
 import torch
 
-from flyai_amd import _lib
+from flyai_amd import _lib, ops
 from flyai_amd._lib import ContextOverflow, FlyaiError
 from flyai_amd.runtime import KVWorkspace, RaggedStage
 
@@ -122,3 +122,16 @@ def test_lora_workspace_has_no_plane_that_no_kernel_writes():
         assert size(M, N, K - 32, R, 1) >= h + 4 * M * N         # another kernel's, with a finalize behind it
         assert size(M, N, K, R, 2) >= 2 * h - 8 * M + 4 * M * N  # segments may straddle a wave's features
     assert size(255, 2880, 4096, 64, 1) >= 255 * (8 * 2880 * 4 + 64 * 4 + 8)
+
+
+def test_segments_are_read_at_every_call():
+    """The cached C array is found by the widths themselves: a tensor that holds one may change between calls, and what is no
+    integer is refused each time."""
+    width = torch.tensor(64)
+    assert list(ops._segments((width, 32))[1]) == [64, 32]
+    width.fill_(16)
+    assert list(ops._segments((width, 32))[1]) == [16, 32]
+    for _ in range(2):
+        assert list(ops._segments((64, 32))[1]) == [64, 32] and ops._segments(())[0] == 0
+        with pytest.raises(TypeError):
+            ops._segments((64.0, 32))

@@ -451,6 +451,8 @@ def kv_fork(k, v, n_kv_heads, src, dsts, lo, hi, src_k=None, src_v=None):
     """Copy positions [lo, hi) of slab src to the same positions of the slabs dsts, every layer, in one launch.  k, v: pools
     bf16 [L, elements] in the tiled slab layout; a slab is (base, cap).  src_k, src_v: the pools that hold src, when
     they are others.  Nothing outside [lo, hi) changes.  Positions past a slab raise ContextOverflow."""
+    if (src_k is None) != (src_v is None):
+        raise ValueError("a source in other pools needs both src_k and src_v")
     L, n, dev = _kv_pools(k, v)
     sn = n
     if src_k is None:

@@ -135,3 +135,10 @@ def test_segments_are_read_at_every_call():
         assert list(ops._segments((64, 32))[1]) == [64, 32] and ops._segments(())[0] == 0
         with pytest.raises(TypeError):
             ops._segments((64.0, 32))
+
+
+def test_a_source_needs_both_pools():
+    k = torch.zeros(2, 1024, dtype=torch.bfloat16)
+    for pools in ({"src_k": k}, {"src_v": k}):
+        with pytest.raises(ValueError, match="both"):
+            ops.kv_fork(k, k, 1, (0, 64), [(64 * 64, 64)], 0, 1, **pools)

@@ -1,4 +1,5 @@
-// The cache's slabs forked and compacted: every layer, K and V, every kv head in one launch.
+// The cache's slabs forked and compacted: every layer, K and V, every kv head in a launch (kForkDsts slabs; kMoveSlabs slabs and
+// kMoveWords blocks of what they span).
 #include <algorithm>
 
 #include "common.h"

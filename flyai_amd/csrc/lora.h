@@ -59,8 +59,9 @@ __device__ __forceinline__ int lora_segment(const LoraArgs& a, int f) {
 // What bounds it is how fast rows of x and A come from L2.  A wave loads whole 128-byte runs (8 rows an instruction) and
 // turns them round in LDS of its own (the tiled GEMM's swizzle); loaded as MFMA operands, 16 rows of 64 bytes an
 // instruction, every quarter of an instruction touched 16 lines, and 2,096 rows of 192 rank columns took 51 us; now 17.3.
-// h is kept as two bf16 terms, the value and what its rounding left out: 16 significant bits (2^-17 of d at most) for the
-// bytes of one fp32 value, and the up product takes them as they are.
+// h is kept as two bf16 terms, the value and what its rounding left out: 16 significant bits for the
+// bytes of one fp32 value, and the up product takes them as they are.  Each h is off by 2^-17 of itself, d = sum h B by 2^-17 of
+// sum |h| |B| at most, which where the sum cancels is more than 2^-17 of d.
 constexpr int kDownParts = 8;   // parts of K
 constexpr int kDownRows = 64;   // rows of an item
 constexpr int kDownCols = kLoraCols;

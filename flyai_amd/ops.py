@@ -365,7 +365,8 @@ def linear_lora(x, w, b, lora_a, lora_b, scale, ranks, adapter, segments=None, r
     int32 [n] (adapter a uses the first ranks[a] of R rows of each segment's A and columns of B; nothing past them is
     used); R a multiple of 16 up to 128.  segments: the S (at most 4) widths of the output's runs that have an A of
     their own (None: one of N).  adapter int32: of each row [M], or with row_seq int32 [M] of each sequence; ids outside
-    [0, n) mean no adapter, and such a row has ``linear``'s bits.  A row's result depends on that row alone."""
+    [0, n) mean no adapter, and such a row has ``linear``'s bits.  A row's result depends on that row alone.  h = s_a x A_a^T is
+    kept to 16 significant bits, in two terms: where B is infinite the result may be NaN in place of an infinity."""
     M, K = x.shape
     N = w.shape[0]
     S, widths = _segments((N,) if segments is None else segments)
@@ -448,8 +449,8 @@ _KV_SLAB, _KV_MOVE = struct.Struct("qii"), struct.Struct("qiiii")  # flyai_kv_sl
 
 
 def kv_fork(k, v, n_kv_heads, src, dsts, lo, hi, src_k=None, src_v=None):
-    """Copy positions [lo, hi) of slab src to the same positions of the slabs dsts, every layer, in one launch.  k, v: pools
-    bf16 [L, elements] in the tiled slab layout; a slab is (base, cap).  src_k, src_v: the pools that hold src, when
+    """Copy positions [lo, hi) of slab src to the same positions of the slabs dsts, every layer, in one launch for every 64 of
+    them.  k, v: pools bf16 [L, elements] in the tiled slab layout; a slab is (base, cap).  src_k, src_v: the pools that hold src, when
     they are others.  Nothing outside [lo, hi) changes.  Positions past a slab raise ContextOverflow."""
     if (src_k is None) != (src_v is None):
         raise ValueError("a source in other pools needs both src_k and src_v")
@@ -496,8 +497,9 @@ def _packed(layout, rows):
 
 def kv_compact(k, v, n_kv_heads, moves):
     """For each move (base, cap, start, keep): position start + i of the slab takes what position start + keep[i] held
-    before the call, every layer, in one launch (or one per 21,504 positions).  keep: host integers (list, numpy or CPU
-    tensor), strictly ascending.  The moves' slabs must not overlap."""
+    before the call, every layer.  keep: host integers (list, numpy or CPU tensor), strictly ascending.  The moves' slabs
+    must not overlap.  A launch takes up to 16 slabs and 336 of their 64-position blocks, a slab's counted from its first
+    position that moves to its last that stays; more take more launches."""
     L, n, dev = _kv_pools(k, v)
     keeps = [_host_positions(m[3]) for m in moves]
     rows = _packed(_KV_MOVE, [(base, cap, start, len(a) // 4, 0) for (base, cap, start, _), a in zip(moves, keeps)])

@@ -99,8 +99,8 @@ class KVWorkspace:
 
     def fork(self, src, dsts, hi, lo=0, src_ws=None):
         """Copy positions [lo, hi) of slot src (of src_ws, if it is in another workspace) to the same positions of the
-        slots dsts, every layer, in one launch (``ops.kv_fork``): a prompt's K/V shared by several samples, or a stream
-        that branches.  Nothing else of dsts changes.  Raises ContextOverflow before any write."""
+        slots dsts, every layer, in one launch for every 64 slots (``ops.kv_fork``): a prompt's K/V shared by several samples,
+        or a stream that branches.  Nothing else of dsts changes.  Raises ContextOverflow before any write."""
         w = self if src_ws is None else src_ws
         if w.n_kv_heads != self.n_kv_heads or w.n_layers < self.n_layers:
             raise ValueError("fork needs workspaces of the same heads and layers")
@@ -109,8 +109,8 @@ class KVWorkspace:
                     src_k=src_k, src_v=src_v)
 
     def compact(self, slots, starts, keeps):
-        """For each of the slots, move positions start + keep[i] to start + i, every layer, in one launch
-        (``ops.kv_compact``): the accepted path of a drafted tree, or the part of a context that stays in the cache.
+        """For each of the slots, move positions start + keep[i] to start + i, every layer, in one launch for every 16 slots
+        or 21,504 positions that the moves span (``ops.kv_compact``): the accepted path of a drafted tree, or the part of a context that stays in the cache.
         Raises ContextOverflow before any write."""
         if not (len(slots) == len(starts) == len(keeps)):
             raise ValueError("slots, starts and keeps must have one entry per slot")

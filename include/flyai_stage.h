@@ -318,7 +318,8 @@ int flyai_attn_prefill(const uint16_t* q, const uint16_t* k_pool, const uint16_t
  * row t, or with row_seq int32 [M] of row t's sequence (adapter[row_seq[t]], n_seqs entries); an adapter
  * outside [0, n_adapters) or a sequence outside [0, n_seqs) means none.  With residual the result is bf16(residual +
  * y), written to residual; the result must not overlap x.  A row's result depends on that row alone: not on its batch, nor on what other
- * rows' adapters hold.  All bf16 matrices and the workspace are 16-byte aligned (b need not be).  workspace:
+ * rows' adapters hold.  h = scale (x A^T) is kept as two bf16 terms, 2^-17 of each h off (of d: of sum |h| |B|); where B is
+ * infinite the result may be NaN in place of an infinity.  All bf16 matrices and the workspace are 16-byte aligned (b need not be).  workspace:
  * flyai_linear_lora_workspace_bytes; two calls that may overlap need one each.  M <= 524288, N % 16 == 0,
  * K % 32 == 0, K <= 8192. */
 size_t flyai_linear_lora_workspace_bytes(int32_t M, int32_t N, int32_t K, int32_t R, int32_t n_segments);
@@ -344,15 +345,16 @@ int flyai_rope(const void* x, int64_t x_token, int64_t x_head, const int32_t* po
                int64_t o_head, flyai_stream_t stream);
 
 /* Slabs of the KV cache (the layout of flyai_rope_kv_append) forked and compacted, every layer, K and V and
- * kv head in one launch (replaces the per-layer index copies of FastVerify.tree_gather,
+ * kv head in a launch (replaces the per-layer index copies of FastVerify.tree_gather,
  * phase0/fastverify.py:301-309, and BatchedFastVerify.load_prefix, phase0/batchverify.py:125-130).  A pool is n_layers layers of
  * `elems` elements, `layer` elements apart.  All descriptions are host memory, read before the call returns
  * and passed to the kernel by value.
  * fork: positions [lo, hi) of the source slab to the same positions of n_dst other slabs; nothing else of
- * them changes.  Slabs of one pool must not overlap.
+ * them changes.  Slabs of one pool must not overlap.  A launch for every 64 slabs.
  * compact: for each move, slab position start + i takes what position start + keep[i] held before the call
  * (keep_host holds the moves' entries one after the other, each move's strictly ascending).  The moves' slabs must
- * not overlap.
+ * not overlap.  A launch takes up to 16 slabs and 336 of their 64-position blocks, counted from the first position that
+ * moves to the last that stays.
  * Positions past a slab -> FLYAI_ERANGE, before any launch. */
 typedef struct {
   int64_t base;  /* element offset of the slab in a layer's pool (base % 8 == 0) */

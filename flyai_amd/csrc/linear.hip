@@ -754,8 +754,9 @@ int launch_gemm(const uint16_t* x, const uint16_t* W, int M, int N, int K, float
 }
 
 // The tiled kernel ends a projection with adapters by itself where it runs (K % 64 == 0) and no wave's 64 features
-// straddle two segments: 2,096 rows of 12 adapters, 5,120 x 2,880, 92 us (72.5 in lora_gemm.hip's tiles); the plain kernel,
-// 76.5, with a finalize behind it, 56.5, is for the others.  (300 rows of 2,880 x 4,096: 30.7 us, or 28.4 + 7.6.)
+// straddle two segments: 2,096 rows of 12 adapters, 5,120 x 2,880, 83 us (73 in lora_gemm.hip's tiles); the plain kernel,
+// 79, with a finalize behind it, 57, is for the others.  (300 rows of 2,880 x 4,096: one adapter 30.5 us, or 27.6 + 7.4; eight in
+// sequences of three 37.3, or 27.7 + 10.4.)
 bool gemm_tiled_lora_fits(int M, int K, const LoraArgs& a) {
   bool whole = true;
   for (int i = 0; i + 1 < a.n_seg; ++i) whole &= a.seg_end[i] % 64 == 0;

@@ -48,9 +48,11 @@ __device__ __forceinline__ int lora_segment(const LoraArgs& a, int f) {
 // groups of 32 rank columns in every segment.  Each workgroup lists the pairs for itself (adapters of up to 64 * TILES rows
 // in LDS, and how many pairs each window has) and takes every wgs-th item: none is launched in vain, whatever the mix.
 // A window is WINDOW x 64 rows: wide ones gather an adapter's scattered rows into fewer items, but their list, a wave's, takes
-// longer.  Beside the split-K kernel all of its rows (100 rows of 24 adapters 20.4 us, with windows of 64 rows 25.0; 200 rows
-// 29.9 / 31.1); alone 128 (64 / 128 / 256: 2,096 rows of 12 adapters 20.6 / 17.3 / 18.8, 800 of 20 16.8 / 15.6 / 17.7, 1,000 of 20 at
-// K = 4,096 16.8 / 17.0 / 19.7, 2,096 of one 15.4 / 15.5 / 16.4).
+// longer.  Beside the split-K kernel all of its rows (100 rows of 24 adapters 20.9 us, with windows of 64 rows 25.7; 200 rows
+// 29.1 / 37.9); alone 128: a prompt with short sequences beside it (64 / 128 / 256: 2,096 rows of 12 adapters 21.1 / 17.6 / 18.9,
+// 800 of 20 17.5 / 18.0 / 18.6, 1,000 of 20 at K = 4,096 16.5 / 17.0 / 19.8, 2,096 of one 16.6 / 15.8 / 17.1) is what it is chosen for;
+// batches of nothing but short sequences would rather have 256 (2,096 of 12 in threes 62.9 / 41.9 / 35.5, 800 of 20
+// 43.3 / 32.4 / 23.6).
 // An item multiplies the window's rows that have the adapter, gathered, 16 to an MFMA tile, or (split) a half or a quarter of
 // them where the batch has few, with 32 rows of A.  K is cut into
 // eight parts, summed in pairs and then in order through LDS, a wave one part or (with four waves) a pair of them; lane
@@ -58,7 +60,7 @@ __device__ __forceinline__ int lora_segment(const LoraArgs& a, int f) {
 // neither on its tile nor on the launch.
 // What bounds it is how fast rows of x and A come from L2.  A wave loads whole 128-byte runs (8 rows an instruction) and
 // turns them round in LDS of its own (the tiled GEMM's swizzle); loaded as MFMA operands, 16 rows of 64 bytes an
-// instruction, every quarter of an instruction touched 16 lines, and 2,096 rows of 192 rank columns took 51 us; now 17.3.
+// instruction, every quarter of an instruction touched 16 lines, and 2,096 rows of 192 rank columns took 51 us; now 17 to 19.
 // h is kept as two bf16 terms, the value and what its rounding left out: 16 significant bits for the
 // bytes of one fp32 value, and the up product takes them as they are.  Each h is off by 2^-17 of itself, d = sum h B by 2^-17 of
 // sum |h| |B| at most, which where the sum cancels is more than 2^-17 of d.
@@ -281,9 +283,9 @@ __device__ __forceinline__ void lora_down(const uint16_t* __restrict__ x, int M,
     const int before = one ? 0 : l.first[min(lane, windows)];
     // Long items first, and the second round's back from the last workgroup on, so that a short item is followed by another:
     // tiles of many adapters are often at one end of a batch, and the items of the other end are the longer (2,096 rows of 12
-    // adapters 22.5 us -> 20.3, 800 rows of 20 20.7 -> 16.8).  Where rows share adapters, an adapter's groups of columns, which
-    // read the same rows, go to one XCD, whose L2 then reads them once: 2,096 rows of one adapter 19.3 us -> 15.5, 4,096 of two
-    // 30.7 -> 22; where they do not, it is 1,000 rows of 20 adapters 17.8 so and 16.8 in turn.
+    // adapters 20.9 us -> 17.6, 800 rows of 20 22.0 -> 18.0; in sequences of three, items of one length, 800 of 20 30.0 -> 32.4).  Where rows share adapters, an adapter's groups of columns, which
+    // read the same rows, go to one XCD, whose L2 then reads them once: 2,096 rows of one adapter 19.4 us -> 15.8, 4,096 of two
+    // 33.9 -> 26.7; where they do not, it is 1,000 rows of 20 adapters at K = 4,096 17.7 so and 17.0 in turn.
     const bool back = !one && l.first[1] > pairs - l.first[windows - 1];
     const int me = rows >= 32 * pairs && wg < wgs / 8 * 8 ? wg % 8 * (wgs / 8) + wg / 8 : wg;
     for (int round = 0; round * wgs < items; ++round) {
@@ -404,7 +406,7 @@ __device__ __forceinline__ int lora_chunk(int at, int c0, int end) {
 // The tile of workgroup b of a tiled GEMM, row-fastest (-1: none).  As in gemm_tiled_lds_kernel an XCD takes a band of whole
 // feature columns, but within it the first and the last rows' tiles come first: a batch's short sequences, and with them
 // tiles of many adapters, which take longer, are often at one of its ends, and a long tile must not start last.  2,096 rows of
-// which 120 have 12 adapters, 5,120 x 2,880: 79.7 us in the other's order, 72.5 in this.
+// which 120 have 12 adapters, 5,120 x 2,880: 78.4 us in the other's order, 72.9 in this (4,096 rows of two 146.5 and 150.1).
 __device__ __forceinline__ int lora_tile(int b, int gm, int gn) {
   const int per = (gm * gn + 7) / 8, start = b % 8 * per, end = min(start + per, gm * gn), i = b / 8;
   if (start + i >= end) return -1;

@@ -166,9 +166,9 @@ static int launch_gemm_lora(const uint16_t* x, const uint16_t* W, int M, int N, 
   }
   *slices = gemm_slices(K);
   // not split: the workgroups share the CUs with the projection's, which want all of them (200 rows of one adapter, 5,120 x
-  // 2,880: 21.9 us with 12 workgroups for h, 26.7 with 48); and for more than two tiles of rows, where the projection's own
+  // 2,880: 22.2 us with 12 workgroups for h, 26.3 with 48); and for more than two tiles of rows, where the projection's own
   // workgroups take long, at most one for every other CU.  24 adapters of 192 rank columns, 5,120 x 2,880, up to one a CU / half
-  // of that: 30 rows 14.0 / 18.8 us, 64 rows 15.0 / 21.0, 100 rows 24.5 / 29.0, 200 rows 32.8 / 30.6
+  // of that: 30 rows 14.3 / 20.1 us, 64 rows 14.8 / 20.0, 100 rows 20.6 / 27.4, 200 rows 30.7 / 28.8
   const int wgs = down_wgs(a, M, kTiledMinRows, 1, M <= 2 * kDownRows ? device_cus() : device_cus() / 2);
   const int bxs = ceil_div(N, 64);
   hipLaunchKernelGGL((gemm_splitk_bf16_kernel<4, true>), dim3(wgs + bxs * *slices), dim3(256), 0, s, x, W, M, N, K, part, a, wgs, bxs);

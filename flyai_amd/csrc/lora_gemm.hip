@@ -202,10 +202,11 @@ int launch_gemm_tall_lora(const uint16_t* x, const uint16_t* W, const uint16_t* 
   return check_launch("gemm_tall_lora");
 }
 
-// Rounds over the CUs, one workgroup each: a round takes 35 to 37 us (K = 2,880), one of 128 x 128 tiles 30 to 34.  5,120 x 2,880,
-// these tiles / those: 800 rows of 20 adapters (1 round / 2) 47.5 / 48.7 us, 1,000 of 5 (1 / 2) 40.4 / 53.1, 2,096 of 12 (2 / 3) 72.5
-// / 92; 2,880 x 4,096: 1,500 rows of 8 (1 / 2) 51 / 64, 2,000 of 24 (1 / 2) 63 / 75; 3,000 rows
-// of 9, 5,120 x 2,880 (3 / 4) 105 / 121, 4,096 of 2 (4 / 5) 154 / 168.
+// Rounds over the CUs, one workgroup each: a round takes 35 to 40 us (K = 2,880), one of 128 x 128 tiles 28 to 34.  5,120 x 2,880,
+// these tiles / those, a prompt with short sequences beside it: 800 rows of 20 adapters (1 round / 2) 50.0 / 49.3 us, 1,000 of 5
+// (1 / 2) 40.6 / 50.0, 2,096 of 12 (2 / 3) 71 to 76 / 82 to 85, 3,000 of 9 (3 / 4) 107 / 128, 4,096 of 2 (4 / 5) 150 / 167; in
+// sequences of three 800 of 20 50.8 / 64.8, 2,096 of 12 92.9 / 107.6; 2,880 x 4,096: 1,500 rows of 8 (1 / 2) 51.0 / 64.7, 2,000 of 24 in
+// threes (1 / 2) 65.9 / 88.8.
 bool gemm_tall_pays(int M, int N) {
   const int cus = device_cus(), n = ceil_div(N, kTallN);
   return ceil_div(ceil_div(M, kTallM) * n, cus) < ceil_div(ceil_div(M, 128) * n, cus);

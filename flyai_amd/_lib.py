@@ -105,6 +105,12 @@ _PROTOS = {
     "flyai_rope": (C.c_int, [P, I64, I64, P, P, F32, I32, I32, I32, I32, I32, I32, I32, P, I64, I64, P]),
     "flyai_kv_fork": (C.c_int, [P, P, I64, I64, P, P, I64, I64, I32, I32, I32, P, P, I32, I32, I32, P]),
     "flyai_kv_compact": (C.c_int, [P, P, I64, I64, I32, I32, I32, P, I32, P, P]),
+    "flyai_pack_shared": (C.c_int, [P, P, P, P, P, P, I32, I32, I32, I32, P, P, P, P, P, P, P, P]),
+    "flyai_rope_kv_append_at": (C.c_int, [P, P, P, P, P, P, I32, I32, I32, I32, I32, P, P, P, P, P, P]),
+    "flyai_attn_shared_plan_bytes": (SZ, [I32, I32, I32]),
+    "flyai_attn_shared_workspace_bytes": (SZ, [I32, I32]),
+    "flyai_attn_shared_plan": (C.c_int, [P, P, P, P, P, P, P, P, I32, I32, I32, I32, I32, I64, P, P]),
+    "flyai_attn_shared": (C.c_int, [P, P, P, P, I32, I32, I32, I32, I32, I32, P, P, P, P]),
     "flyai_bf16_tile_packed_bytes": (SZ, [I32, I32]),
     "flyai_bf16_tile_repack": (C.c_int, [P, I32, I32, P, P]),
     "flyai_embed_gather": (C.c_int, [P, P, I32, I32, I32, P, P]),

@@ -1006,11 +1006,11 @@ __global__ __launch_bounds__(256) void qkv_rope_kv_vec_kernel(
 int launch_rope_kv(const uint16_t* qkv, const int32_t* positions, const int32_t* seq_id,
                    const uint16_t* cos_tab, const uint16_t* sin_tab, int rope_positions, int T,
                    int Hq, int Hkv, int D, const int64_t* kv_base, const int32_t* kv_cap,
-                   uint16_t* q_out, uint16_t* k_pool, uint16_t* v_pool, hipStream_t s) {
+                   uint16_t* q_out, uint16_t* k_pool, uint16_t* v_pool, const int32_t* kv_pos, hipStream_t s) {
   if (T == 0) return FLYAI_OK;
   hipLaunchKernelGGL(rope_kv_append_kernel<false>, dim3(T), dim3(256), 0, s, qkv, nullptr, 0, T,
                      nullptr, positions, seq_id, cos_tab, sin_tab, rope_positions, Hq, Hkv, D, kv_base,
-                     kv_cap, q_out, k_pool, v_pool, nullptr);
+                     kv_cap, q_out, k_pool, v_pool, kv_pos);
   return check_launch("rope_kv_append");
 }
 
@@ -1144,17 +1144,35 @@ extern "C" int flyai_linear_bf16_noalloc(const uint16_t* x, const uint16_t* w, c
   return launch_linear(x, w, b, M, N, K, y, residual, part, as_stream(stream));
 }
 
-extern "C" int flyai_rope_kv_append(const uint16_t* qkv, const int32_t* positions,
-                                    const int32_t* seq_id, const uint16_t* cos_tab,
-                                    const uint16_t* sin_tab, int32_t rope_positions, int32_t T,
-                                    int32_t Hq, int32_t Hkv, int32_t D, const int64_t* kv_base,
-                                    const int32_t* kv_cap, uint16_t* q_out, uint16_t* k_pool,
-                                    uint16_t* v_pool, flyai_stream_t stream) {
+static int rope_kv_append(const uint16_t* qkv, const int32_t* positions, const int32_t* kv_pos, const int32_t* seq_id,
+                          const uint16_t* cos_tab, const uint16_t* sin_tab, int32_t rope_positions, int32_t T,
+                          int32_t Hq, int32_t Hkv, int32_t D, const int64_t* kv_base, const int32_t* kv_cap,
+                          uint16_t* q_out, uint16_t* k_pool, uint16_t* v_pool, flyai_stream_t stream) {
   FLYAI_REQUIRE(T >= 0 && Hq > 0 && Hkv > 0 && D == 64 && rope_positions > 0,
                 "rope_kv: bad shape (the tiled KV layout needs head_dim 64)");
   FLYAI_REQUIRE(qkv && positions && seq_id && cos_tab && sin_tab && kv_base && kv_cap && q_out &&
                     k_pool && v_pool,
                 "rope_kv: null pointer");
   return launch_rope_kv(qkv, positions, seq_id, cos_tab, sin_tab, rope_positions, T, Hq, Hkv, D,
-                        kv_base, kv_cap, q_out, k_pool, v_pool, as_stream(stream));
+                        kv_base, kv_cap, q_out, k_pool, v_pool, kv_pos, as_stream(stream));
+}
+
+extern "C" int flyai_rope_kv_append(const uint16_t* qkv, const int32_t* positions,
+                                    const int32_t* seq_id, const uint16_t* cos_tab,
+                                    const uint16_t* sin_tab, int32_t rope_positions, int32_t T,
+                                    int32_t Hq, int32_t Hkv, int32_t D, const int64_t* kv_base,
+                                    const int32_t* kv_cap, uint16_t* q_out, uint16_t* k_pool,
+                                    uint16_t* v_pool, flyai_stream_t stream) {
+  return rope_kv_append(qkv, positions, nullptr, seq_id, cos_tab, sin_tab, rope_positions, T, Hq, Hkv, D, kv_base, kv_cap,
+                        q_out, k_pool, v_pool, stream);
+}
+
+extern "C" int flyai_rope_kv_append_at(const uint16_t* qkv, const int32_t* positions, const int32_t* kv_pos,
+                                       const int32_t* seq_id, const uint16_t* cos_tab, const uint16_t* sin_tab,
+                                       int32_t rope_positions, int32_t T, int32_t Hq, int32_t Hkv, int32_t D,
+                                       const int64_t* kv_base, const int32_t* kv_cap, uint16_t* q_out, uint16_t* k_pool,
+                                       uint16_t* v_pool, flyai_stream_t stream) {
+  FLYAI_REQUIRE(kv_pos, "rope_kv: null pointer");
+  return rope_kv_append(qkv, positions, kv_pos, seq_id, cos_tab, sin_tab, rope_positions, T, Hq, Hkv, D, kv_base, kv_cap,
+                        q_out, k_pool, v_pool, stream);
 }

@@ -108,6 +108,83 @@ __global__ __launch_bounds__(kPackThreads) void pack_norm_kernel(
     rmsnorm_row(x, w, H, eps, y, blockIdx.x - 1);
 }
 
+// The packing of sequences behind shared prefixes: a sequence's slab holds what follows its prefix.  Each workgroup scans the
+// lengths (8 a thread at most: cheaper than a launch that leaves them behind) and takes its share of the tokens; the first one
+// writes what there is one of for each sequence.
+constexpr int kPackSharedTokens = 2048;  // of a workgroup
+
+__global__ __launch_bounds__(kPackThreads) void pack_shared_kernel(
+    const int32_t* __restrict__ q_lens, const int32_t* __restrict__ starts, const int64_t* __restrict__ kv_base,
+    const int32_t* __restrict__ kv_cap, const int32_t* __restrict__ prefix_of, const int32_t* __restrict__ prefix_len, int S,
+    int n_prefix, int head_dim, int max_tokens, int32_t* __restrict__ cu_out, int32_t* __restrict__ positions,
+    int32_t* __restrict__ seq_id, int32_t* __restrict__ kv_pos, int64_t* __restrict__ kv_slot, int32_t* __restrict__ kv_len,
+    int32_t* __restrict__ status_out) {
+  __shared__ int32_t cu[kPackMaxSeqs + 1];  // (a sum past int32 is held at its largest value: max_tokens ends before that)
+  __shared__ int64_t wave_tot[kPackThreads / 64];
+  __shared__ int32_t status_s;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const bool first = blockIdx.x == 0;
+  if (tid == 0) status_s = 0;
+  const int per = (S + kPackThreads - 1) / kPackThreads;
+  const int s0 = min(S, tid * per), s1 = min(S, s0 + per);
+  int64_t local = 0;
+  for (int s = s0; s < s1; ++s) local += max(q_lens[s], 0);
+  int64_t incl = local;
+#pragma unroll
+  for (int off = 1; off < 64; off <<= 1) {
+    const int64_t v = __shfl_up(incl, off, 64);
+    if (lane >= off) incl += v;
+  }
+  if (lane == 63) wave_tot[wave] = incl;
+  __syncthreads();
+  int64_t run = incl - local;
+  for (int w = 0; w < wave; ++w) run += wave_tot[w];
+  // positions of a sequence that lie in its prefix's slab; -1: there is no such prefix
+  auto behind = [&](int s) __attribute__((always_inline)) {
+    const int p = prefix_of[s];
+    return p < 0 ? 0 : p < n_prefix ? prefix_len[p] : -1;
+  };
+  int status = 0;
+  for (int s = s0; s < s1; ++s) {
+    const int c = (int)min(run, (int64_t)INT32_MAX);
+    cu[s] = c;
+    run += max(q_lens[s], 0);
+    if (!first) continue;
+    cu_out[s] = c;
+    const int q = q_lens[s], start = starts[s], P = behind(s);
+    const int64_t len = (int64_t)start + max(q, 0);
+    kv_len[s] = (int)min(len, (int64_t)INT32_MAX);
+    if (q < 0 || start < 0) status |= 16;
+    else if (P < 0) status |= 8;
+    else if (start < P) status |= 4;
+    else if (len - P > kv_cap[s]) status |= 1;
+    if (run > max_tokens) status |= 2;
+  }
+  if (s0 < s1 && s1 == S) {
+    cu[S] = (int)min(run, (int64_t)INT32_MAX);
+    if (first) cu_out[S] = cu[S];
+  }
+  if (first && status) atomicOr(&status_s, status);
+  __syncthreads();
+  if (first && tid == 0) *status_out = status_s;
+  const int Tw = min(cu[S], max_tokens);
+  const int t1 = min(Tw, (int)(blockIdx.x + 1) * kPackSharedTokens);
+  for (int t = blockIdx.x * kPackSharedTokens + tid; t < t1; t += kPackThreads) {
+    int lo = 0, hi = S - 1;  // last s with cu[s] <= t
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) >> 1;
+      if (cu[mid] <= t) lo = mid; else hi = mid - 1;
+    }
+    const int P = behind(lo);
+    const int64_t pos = (int64_t)starts[lo] + (t - cu[lo]), at = pos - P;
+    const bool fits = P >= 0 && starts[lo] >= 0 && at >= 0 && at < kv_cap[lo];
+    positions[t] = (int)min(pos, (int64_t)INT32_MAX);
+    seq_id[t] = lo;
+    kv_pos[t] = P < 0 ? -1 : (int)max(min(at, (int64_t)INT32_MAX), (int64_t)-1);
+    kv_slot[t] = fits ? kv_base[lo] + at * head_dim : (int64_t)-1;
+  }
+}
+
 }  // namespace flyai
 
 using namespace flyai;
@@ -127,6 +204,23 @@ extern "C" int flyai_pack_ragged(const int32_t* q_lens, const int32_t* starts,
                      q_lens, starts, kv_base, kv_cap, n_seqs, head_dim, max_tokens, cu_seqlens,
                      positions, seq_id, kv_len, kv_slot, status_dev, nullptr, nullptr);
   return check_launch("pack_ragged");
+}
+
+extern "C" int flyai_pack_shared(const int32_t* q_lens, const int32_t* starts, const int64_t* kv_base, const int32_t* kv_cap,
+                                 const int32_t* prefix_of, const int32_t* prefix_len, int32_t n_seqs, int32_t n_prefixes,
+                                 int32_t head_dim, int32_t max_tokens, int32_t* cu_seqlens, int32_t* positions, int32_t* seq_id,
+                                 int32_t* kv_pos, int64_t* kv_slot, int32_t* kv_len, int32_t* status_dev, flyai_stream_t stream) {
+  FLYAI_REQUIRE(n_seqs >= 1 && n_seqs <= kPackMaxSeqs, "pack_shared: n_seqs %d out of [1, %d]", n_seqs, kPackMaxSeqs);
+  FLYAI_REQUIRE(n_prefixes >= 0 && head_dim > 0 && max_tokens >= 0 && max_tokens <= (1 << 24),
+                "pack_shared: bad n_prefixes, head_dim or max_tokens");
+  FLYAI_REQUIRE(q_lens && starts && kv_base && kv_cap && prefix_of && (n_prefixes == 0 || prefix_len) && cu_seqlens && kv_len &&
+                    status_dev && (max_tokens == 0 || (positions && seq_id && kv_pos && kv_slot)),
+                "pack_shared: null pointer");
+  const int grid = max_tokens > 0 ? ceil_div(max_tokens, kPackSharedTokens) : 1;
+  hipLaunchKernelGGL(pack_shared_kernel, dim3(grid), dim3(kPackThreads), 0, as_stream(stream), q_lens, starts, kv_base, kv_cap,
+                     prefix_of, prefix_len, n_seqs, n_prefixes, head_dim, max_tokens, cu_seqlens, positions, seq_id, kv_pos, kv_slot,
+                     kv_len, status_dev);
+  return check_launch("pack_shared");
 }
 
 namespace flyai {

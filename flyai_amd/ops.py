@@ -232,7 +232,8 @@ def linear(x, w, b=None, residual=None):
 
 
 def rope_kv_append(qkv, positions, seq_id, cos_tab, sin_tab, n_q_heads, n_kv_heads, head_dim,
-                   kv_base, kv_cap, k_pool, v_pool):
+                   kv_base, kv_cap, k_pool, v_pool, kv_pos=None):
+    """kv_pos int32: where a token's K and V go in its slab, when that is not its position (``pack_shared``)."""
     T = qkv.shape[0]
     _need(qkv, torch.bfloat16, (T, (n_q_heads + 2 * n_kv_heads) * head_dim), "qkv")
     _need(positions, torch.int32, None, "positions")
@@ -246,6 +247,14 @@ def rope_kv_append(qkv, positions, seq_id, cos_tab, sin_tab, n_q_heads, n_kv_hea
     if positions.numel() < T or seq_id.numel() < T:
         raise ValueError("positions/seq_id shorter than the token count")
     q = torch.empty(T, n_q_heads, head_dim, dtype=torch.bfloat16, device=qkv.device)
+    if kv_pos is not None:
+        _need(kv_pos, torch.int32, None, "kv_pos")
+        if kv_pos.numel() < T:
+            raise ValueError("kv_pos shorter than the token count")
+        check(lib().flyai_rope_kv_append_at(_ptr(qkv), _ptr(positions), _ptr(kv_pos), _ptr(seq_id), _ptr(cos_tab), _ptr(sin_tab),
+                                            cos_tab.shape[0], T, n_q_heads, n_kv_heads, head_dim, _ptr(kv_base), _ptr(kv_cap),
+                                            _ptr(q), _ptr(k_pool), _ptr(v_pool), _stream()))
+        return q
     check(lib().flyai_rope_kv_append(_ptr(qkv), _ptr(positions), _ptr(seq_id), _ptr(cos_tab),
                                      _ptr(sin_tab), cos_tab.shape[0], T, n_q_heads, n_kv_heads, head_dim, _ptr(kv_base),
                                      _ptr(kv_cap), _ptr(q), _ptr(k_pool), _ptr(v_pool), _stream()))
@@ -504,6 +513,97 @@ def kv_compact(k, v, n_kv_heads, moves):
     keeps = [_host_positions(m[3]) for m in moves]
     rows = _packed(_KV_MOVE, [(base, cap, start, len(a) // 4, 0) for (base, cap, start, _), a in zip(moves, keeps)])
     _on(dev, lib().flyai_kv_compact, k.data_ptr(), v.data_ptr(), n, n, L, _position(n_kv_heads), 64, rows, len(moves), b"".join(keeps))
+
+
+# ---- batches that share prompts -----------------------------------------------------------------
+
+# The status word of pack_shared and of a plan
+PAST_SLAB, PAST_TOKENS, BEFORE_PREFIX, BAD_PREFIX, BAD_SEQUENCE = 1, 2, 4, 8, 16
+
+
+def pack_shared(q_lens, starts, kv_base, kv_cap, prefix_of, prefix_len, head_dim, max_tokens):
+    """``pack_ragged`` for sequences behind shared prefixes: sequence b's first prefix_len[prefix_of[b]] positions lie in a slab
+    that it shares (prefix_of negative: none), its own slab (kv_base, kv_cap) holds what follows.  Device int32 q_lens,
+    starts (the first new token's position), kv_cap, prefix_of [S], prefix_len [n], int64 kv_base [S] -> dict of cu_seqlens,
+    positions, seq_id, kv_len as in ``pack_ragged``, kv_pos int32 (a token's slab position), kv_slot int64 (its element, -1 outside
+    the slab) and status (PAST_SLAB, ... bits; 0: all is well).  Lengths may come from the GPU: nothing is read back."""
+    S, n = q_lens.numel(), prefix_len.numel()
+    i32 = torch.int32
+    dev = q_lens.get_device()
+    _need_all(dev, ("q_lens", q_lens, i32, (S,)), ("starts", starts, i32, (S,)), ("kv_base", kv_base, torch.int64, (S,)),
+              ("kv_cap", kv_cap, i32, (S,)), ("prefix_of", prefix_of, i32, (S,)), ("prefix_len", prefix_len, i32, (n,)))
+    max_tokens = _position(max_tokens)
+    at = q_lens.device
+    m = max(max_tokens, 0)
+    out = {k: torch.empty(c, dtype=i32, device=at) for k, c in (("cu_seqlens", S + 1), ("positions", m), ("seq_id", m), ("kv_pos", m),
+                                                               ("kv_len", S), ("status", 1))}
+    out["kv_slot"] = torch.empty(m, dtype=torch.int64, device=at)
+    _on(dev, lib().flyai_pack_shared, q_lens.data_ptr(), starts.data_ptr(), kv_base.data_ptr(), kv_cap.data_ptr(), prefix_of.data_ptr(),
+        prefix_len.data_ptr(), S, n, _position(head_dim), max_tokens, out["cu_seqlens"].data_ptr(), out["positions"].data_ptr(),
+        out["seq_id"].data_ptr(), out["kv_pos"].data_ptr(), out["kv_slot"].data_ptr(), out["kv_len"].data_ptr(), out["status"].data_ptr())
+    return out
+
+
+class AttnSharedPlan:
+    """The work lists of a batch and a window (``attn_shared_plan``), on the GPU.  status int32 [1]: PAST_SLAB, ... bits."""
+
+    __slots__ = ("buffer", "n_tokens", "n_seqs", "n_prefixes", "n_kv_heads", "window", "pool_elems")
+
+    def __init__(self, *values):
+        for name, v in zip(self.__slots__, values):
+            setattr(self, name, v)
+
+    @property
+    def status(self):
+        return self.buffer[12:16].view(torch.int32)
+
+
+@functools.lru_cache(maxsize=256)
+def _attn_shared_bytes(T, S, n, Hkv):
+    return int(lib().flyai_attn_shared_plan_bytes(T, S, n)), int(lib().flyai_attn_shared_workspace_bytes(T, Hkv))
+
+
+def attn_shared_plan(q_lens, starts, kv_base, kv_cap, prefix_of, prefix_len, prefix_base, prefix_cap, n_kv_heads, window, n_tokens,
+                     pool_elems):
+    """The work lists of ``attn_shared`` for a batch as in ``pack_shared`` and a window (0: full attention): made on the GPU, once for
+    all layers of a step.  prefix_len, prefix_cap int32 [n], prefix_base int64 [n]: the prefixes' lengths and slabs, in the same pools
+    as the sequences' (pool_elems elements each).  n_tokens: rows of q (the batch's tokens, or more)."""
+    S, n = q_lens.numel(), prefix_len.numel()
+    i32, i64 = torch.int32, torch.int64
+    dev = q_lens.get_device()
+    _need_all(dev, ("q_lens", q_lens, i32, (S,)), ("starts", starts, i32, (S,)), ("kv_base", kv_base, i64, (S,)),
+              ("kv_cap", kv_cap, i32, (S,)), ("prefix_of", prefix_of, i32, (S,)), ("prefix_len", prefix_len, i32, (n,)),
+              ("prefix_base", prefix_base, i64, (n,)), ("prefix_cap", prefix_cap, i32, (n,)))
+    T, Hkv, window = _position(n_tokens), _position(n_kv_heads), _position(window)
+    size, _ = _attn_shared_bytes(T, S, n, Hkv)
+    plan = AttnSharedPlan(torch.empty(max(size, 16), dtype=torch.uint8, device=q_lens.device), T, S, n, Hkv, window, operator.index(pool_elems))
+    _on(dev, lib().flyai_attn_shared_plan, q_lens.data_ptr(), starts.data_ptr(), kv_base.data_ptr(), kv_cap.data_ptr(),
+        prefix_of.data_ptr(), prefix_len.data_ptr(), prefix_base.data_ptr(), prefix_cap.data_ptr(), S, n, Hkv, window, T,
+        plan.pool_elems, plan.buffer.data_ptr())
+    return plan
+
+
+def attn_shared(q, k_pool, v_pool, sinks, plan, out=None):
+    """Attention of a batch that shares prefixes (``attn_ragged`` with each prefix's keys read once for all the rows behind it): q bf16
+    [T, Hq, 64] rotated, k_pool and v_pool bf16 (the slabs that the plan names), sinks fp32 [Hq], Hq = 8 kv heads.  Returns
+    out bf16 [T, Hq, 64] (None: a new one); rows behind the last sequence are left as they were, those of a sequence that the plan
+    refused (plan.status) are zeros.  A row's bits depend on its own sequence, its prefix and the window, not on the batch.
+    K and V outside the positions that a row sees may hold anything."""
+    T, Hkv = plan.n_tokens, plan.n_kv_heads
+    dev, bf16 = q.get_device(), torch.bfloat16
+    _need_all(dev, ("q", q, bf16, (T, 8 * Hkv, 64)), ("k_pool", k_pool, bf16, k_pool.shape), ("v_pool", v_pool, bf16, k_pool.shape),
+              ("sinks", sinks, torch.float32, (8 * Hkv,)), ("plan", plan.buffer, torch.uint8, plan.buffer.shape))
+    if k_pool.numel() < plan.pool_elems:
+        raise ValueError(f"the pools have {k_pool.numel()} elements, the plan was made for {plan.pool_elems}")
+    if out is None:
+        out = torch.empty_like(q)
+    else:
+        _need_all(dev, ("out", out, bf16, q.shape))
+    _, size = _attn_shared_bytes(T, plan.n_seqs, plan.n_prefixes, Hkv)
+    ws = torch.empty(max(size, 16), dtype=torch.uint8, device=q.device)
+    _on(dev, lib().flyai_attn_shared, q.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), sinks.data_ptr(), 8 * Hkv, Hkv, 64, T,
+        plan.n_seqs, plan.n_prefixes, plan.buffer.data_ptr(), ws.data_ptr(), out.data_ptr())
+    return out
 
 
 # ---- DeepSeek-V3-shaped FP8 MoE ------------------------------------------------------------------

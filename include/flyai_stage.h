@@ -378,6 +378,43 @@ int flyai_kv_compact(uint16_t* k_pool, uint16_t* v_pool, int64_t layer, int64_t 
                      int32_t Hkv, int32_t D, const flyai_kv_move* moves_host, int32_t n_moves,
                      const int32_t* keep_host, flyai_stream_t stream);
 
+/* ---- batches that share prompts -------------------------------------------------------------------
+ * A prefix is a run of positions 0 .. len - 1 whose K/V lies in one slab and is read by every sequence behind it; a
+ * sequence's own slab holds what follows: position p at its slab's position p - len.  prefix_of[b] names sequence b's prefix
+ * (negative: none, and the slab holds all).  All arrays are device memory, so that lengths which were made on the GPU never
+ * come to the host; what they hold is checked there, and reported as bits of a status word: 1 a sequence past its slab, 2
+ * more tokens than max_tokens (n_tokens), 4 a sequence that starts before its prefix ends, 8 a prefix that is none (id,
+ * length or slab), 16 a bad length, start or slab.  q_lens[b] = 0 is a sequence without tokens.
+ * flyai_pack_shared is flyai_pack_ragged for such sequences: positions[t] and kv_len[b] count from the prefix's start,
+ * kv_pos[t] (-1 before the slab) is the token's slab position and kv_slot[t] = kv_base + kv_pos * head_dim, -1 outside
+ * the slab.  Nothing is written behind the last token.  n_seqs <= 8192, max_tokens <= 2^24. */
+int flyai_pack_shared(const int32_t* q_lens, const int32_t* starts, const int64_t* kv_base, const int32_t* kv_cap,
+                      const int32_t* prefix_of, const int32_t* prefix_len, int32_t n_seqs, int32_t n_prefixes,
+                      int32_t head_dim, int32_t max_tokens, int32_t* cu_seqlens, int32_t* positions, int32_t* seq_id,
+                      int32_t* kv_pos, int64_t* kv_slot, int32_t* kv_len, int32_t* status_dev, flyai_stream_t stream);
+/* flyai_rope_kv_append with the token's slab position apart from its rotary position (kv_pos int32 [T]; outside
+ * [0, kv_cap) nothing is written). */
+int flyai_rope_kv_append_at(const uint16_t* qkv, const int32_t* positions, const int32_t* kv_pos, const int32_t* seq_id,
+                            const uint16_t* cos_tab, const uint16_t* sin_tab, int32_t rope_positions,
+                            int32_t T, int32_t Hq, int32_t Hkv, int32_t D, const int64_t* kv_base,
+                            const int32_t* kv_cap, uint16_t* q_out, uint16_t* k_pool, uint16_t* v_pool, flyai_stream_t stream);
+/* flyai_attn_ragged for such sequences: the rows of a prefix's sequences read its keys together.  flyai_attn_shared_plan makes the work lists
+ * of a batch and a window (0: full) on the GPU, into `plan` (16-byte aligned, flyai_attn_shared_plan_bytes); flyai_attn_shared runs
+ * them, as often as layers have that batch and window, with workspace of flyai_attn_shared_workspace_bytes (calls that may
+ * overlap need one each).  T: rows of q and out, at most 65,536; the rows behind the last sequence are left as they were, those of a
+ * sequence that was refused (the status word, the plan's fourth int32) are zeros.  Slabs and prefixes are checked against pool_elems, the elements of a pool.
+ * A row's bits depend on its own sequence, its prefix and the window alone.  D == 64, Hq == 8 Hkv, Hkv <= 64, n_seqs <= 8192, n_prefixes <= 1024;
+ * q, pools, out, workspace 16-byte aligned. */
+size_t flyai_attn_shared_plan_bytes(int32_t T, int32_t n_seqs, int32_t n_prefixes);
+size_t flyai_attn_shared_workspace_bytes(int32_t T, int32_t Hkv);
+int flyai_attn_shared_plan(const int32_t* q_lens, const int32_t* starts, const int64_t* kv_base, const int32_t* kv_cap,
+                           const int32_t* prefix_of, const int32_t* prefix_len, const int64_t* prefix_base,
+                           const int32_t* prefix_cap, int32_t n_seqs, int32_t n_prefixes, int32_t Hkv, int32_t window,
+                           int32_t T, int64_t pool_elems, void* plan, flyai_stream_t stream);
+int flyai_attn_shared(const uint16_t* q, const uint16_t* k_pool, const uint16_t* v_pool, const float* sinks, int32_t Hq,
+                      int32_t Hkv, int32_t D, int32_t T, int32_t n_seqs, int32_t n_prefixes, const void* plan,
+                      void* workspace, uint16_t* out, flyai_stream_t stream);
+
 /* ---- head and tail of a served model (the continuous-batch backend's token step) --------------
  * Embedding: replaces parts["embed"](token_ids) (phase0/specpipe.py:595-596, :779): out[t] =
  * table[ids[t]] (bf16 [V, H] table; an id outside [0, V) gives a zero row).  H % 8 == 0.

@@ -120,6 +120,8 @@ _PROTOS = {
     "flyai_sample_rows": (C.c_int, [P, I32, I32, F32, I32, F32, P, P, P, P, P, P]),
     "flyai_sample_workspace_bytes": (SZ, [I32, I32]),
     "flyai_sample_rows_ws": (C.c_int, [P, I32, I32, F32, I32, F32, P, P, P, P, P, P, P]),
+    "flyai_spec_verify_workspace_bytes": (SZ, [I32, I32, I32]),
+    "flyai_spec_verify": (C.c_int, [P, I32, I32, P, I32, P, P, P, P, P, P, F32, I32, F32, P, I32, P, P, P, P, P, P]),
     "flyai_sample_probs": (C.c_int, [P, I32, C.c_double, P, P]),
     "flyai_stage_create": (C.c_int, [P, P]),
     "flyai_stage_destroy": (None, [P]),

@@ -784,6 +784,56 @@ def sample_rows(logits, temp, top_k=0, top_p=1.0, draft=None, u=None, want_p_dra
     return out
 
 
+@functools.lru_cache(maxsize=256)
+def _spec_verify_bytes(R, V, S):
+    return max(8, int(lib().flyai_spec_verify_workspace_bytes(R, V, S)))
+
+
+def spec_verify(logits, cu_rows, draft, u, u_draw, temp, top_k=0, top_p=1.0, draft_probs=None, probs_row=None):
+    """Drafted tokens of many streams verified at once (``Sampler.accept``'s rule).  Stream s has the rows cu_rows[s] ..
+    cu_rows[s + 1] - 1 of logits bf16 [R, V] (cu_rows int32 [S + 1], ascending); row r judges the token draft[r] (int32 [R]; -1: none, as in the
+    last row of a stream, whose token is a bonus).  temp, top_k, top_p: numbers, or fp32, int32, fp32 [S] for each stream (temp <= 0:
+    greedy).  draft_probs fp32 [n, V]: the distributions that the drafts were drawn from, row probs_row[r] (int32 [R]; -1: none;
+    None: row r) for row r; a draft without one was not drawn.  u fp64 [R] and u_draw fp64 [S]: uniforms in [0, 1) for the
+    acceptances and for each stream's draw.
+
+    Returns (tokens int32 [R], counts int32 [S], p fp32 [R]), all on the GPU: in a stream's rows its accepted drafts, then the drawn
+    token, then -1; how many tokens it got; and each token's probability under the filtered target (0 behind the end)."""
+    R, V = logits.shape
+    S = cu_rows.numel() - 1
+    if S < 0:
+        raise ValueError("cu_rows needs at least one entry")
+    dev = logits.get_device()
+    f32, i32, f64 = torch.float32, torch.int32, torch.float64
+    _need_all(dev, ("logits", logits, torch.bfloat16, (R, V)), ("cu_rows", cu_rows, i32, (S + 1,)), ("draft", draft, i32, (R,)),
+              ("u", u, f64, (R,)), ("u_draw", u_draw, f64, (S,)))
+    params = [None, None, None]
+    for i, (name, v, dtype) in enumerate((("temp", temp, f32), ("top_k", top_k, i32), ("top_p", top_p, f32))):
+        if isinstance(v, torch.Tensor):
+            _need_all(dev, (name, v, dtype, (S,)))
+            params[i] = v
+    temp, top_k, top_p = (d if p is not None else v for p, v, d in zip(params, (temp, top_k, top_p), (0.0, 0, 1.0)))
+    n = 0
+    if draft_probs is not None:
+        n = draft_probs.shape[0]
+        _need_all(dev, ("draft_probs", draft_probs, f32, (n, V)))
+        if probs_row is None and n != R:
+            raise ValueError(f"draft_probs has {n} rows for {R} rows of logits: probs_row has to say whose they are")
+    elif probs_row is not None:
+        raise ValueError("probs_row without draft_probs")
+    if probs_row is not None:
+        _need_all(dev, ("probs_row", probs_row, i32, (R,)))
+    at = logits.device
+    tokens = torch.empty(R, dtype=i32, device=at)
+    counts = torch.empty(S, dtype=i32, device=at)
+    p = torch.empty(R, dtype=f32, device=at)
+    ws = torch.empty(_spec_verify_bytes(R, V, S), dtype=torch.uint8, device=at)
+    _on(dev, lib().flyai_spec_verify, logits.data_ptr(), R, V, cu_rows.data_ptr(), S, draft.data_ptr(), u.data_ptr(), u_draw.data_ptr(),
+        _address(params[0]), _address(params[1]), _address(params[2]), float(temp), _position(top_k), float(top_p), _address(draft_probs), n,
+        _address(probs_row), tokens.data_ptr(), counts.data_ptr(), p.data_ptr(), ws.data_ptr())
+    return tokens, counts, p
+
+
 def sample_probs(probs, u):
     """One draw from a fp32 probability vector [V] (device) at uniform u in [0, 1): int32 [1] on device."""
     V = probs.numel()

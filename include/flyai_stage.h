@@ -471,6 +471,25 @@ int flyai_sample_rows_ws(const uint16_t* logits, int32_t R, int32_t V, float tem
  * same inverse-CDF rule with uniform u in [0, 1); out (device int32) gets the id (0 when all are 0). */
 int flyai_sample_probs(const float* probs, int32_t V, double u, int32_t* out, flyai_stream_t stream);
 
+/* Drafted tokens of many streams verified (Sampler.accept, phase0/specsample.py:79-107, for a batch, and with the drafter's
+ * own distribution where there is one).  Stream s has the logits rows cu_rows[s] .. cu_rows[s + 1] - 1 (ascending; bf16 [R, V]),
+ * row r judges the token draft[r] (-1 or outside [0, V): none, as in a stream's last row).  temps fp32, top_ks int32, top_ps
+ * fp32 [S]: each stream's, or NULL: temp, top_k, top_p for all (a top_k below 1 and a top_p outside (0, 1) are off).  With w the row's
+ * integer weights as in flyai_sample_rows and W their sum, draft d is accepted if u[r] q(d) W < w[d] in fp64, q = 1 or the
+ * drafter's distribution: row probs_row[r] of draft_probs fp32 [n_probs, V] (probs_row NULL: row r, n_probs == R; outside [0,
+ * n_probs): none; negative and NaN entries count as 0).  The first row that is not accepted ends the stream with the draw flyai_sample_rows makes with u_draw[s] over w without
+ * the draft, with a distribution over max(0, w - floor(q W)), without a draft over w.  temp <= 0: a draft is accepted if it is
+ * the first id of maximal logit, which else ends the stream.  tokens int32 [R]: the accepted drafts, then the drawn token,
+ * then -1; counts int32 [S]: tokens of each stream; p fp32 [R]: the filtered target's probability of each token (greedy: 1; 0 behind
+ * the end).  Rows behind cu_rows[S] are left as they were.  u, u_draw fp64 in [0, 1).  Sums are of integers: results do not
+ * depend on the launch.  V <= 2^22, S <= 65535; workspace: flyai_spec_verify_workspace_bytes, 8-byte aligned, not initialised. */
+size_t flyai_spec_verify_workspace_bytes(int32_t R, int32_t V, int32_t S);
+int flyai_spec_verify(const uint16_t* logits, int32_t R, int32_t V, const int32_t* cu_rows, int32_t S, const int32_t* draft,
+                      const double* u, const double* u_draw, const float* temps, const int32_t* top_ks, const float* top_ps,
+                      float temp, int32_t top_k, float top_p, const float* draft_probs, int32_t n_probs,
+                      const int32_t* probs_row, int32_t* tokens, int32_t* counts, float* p, void* workspace,
+                      flyai_stream_t stream);
+
 /* ---- a10: stage step driver ----------------------------------------------------------------------
  * The per-layer loop of FastVerify._layers / BatchedFastVerify._layers (phase0/fastverify.py:116-122,
  * phase0/batchverify.py:132-138) over GptOssDecoderLayer.forward (modeling_gpt_oss.py:347-376), for

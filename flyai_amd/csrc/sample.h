@@ -23,10 +23,10 @@ __device__ __forceinline__ float key_f32(uint32_t k) {
 // into a 32-bit head, so k * head is exact, and a tail) and the degree-13 Taylor polynomial of e^r
 // (truncation error below 5e-18), each fp64 operation rounded on its own (no fused multiply-add):
 // within one unit of the exact floor.  d below -27.75 gives 0 (2^40 e^d < 1 there).
-__device__ __forceinline__ uint64_t samp_weight(float z, float zmax) {
+__device__ __forceinline__ double samp_weight_f64(float z, float zmax) {  // (a double holds it: it is at most 2^40)
 #pragma clang fp contract(off)
   const double d = (double)z - (double)zmax;
-  if (!(d >= -27.75)) return 0;
+  if (!(d >= -27.75)) return 0.0;
   const double k = rint(d * 0x1.71547652b82fep+0);
   const double r = (d - k * 0x1.62e42feep-1) - k * 0x1.a39ef35793c76p-33;
   double p = 0x1.6124613a86d09p-33;
@@ -43,8 +43,10 @@ __device__ __forceinline__ uint64_t samp_weight(float z, float zmax) {
   p = p * r + 0x1p-1;
   p = p * r + 1.0;
   p = p * r + 1.0;
-  return (uint64_t)floor(ldexp(p, (int)k + 40));
+  return floor(ldexp(p, (int)k + 40));
 }
+
+__device__ __forceinline__ uint64_t samp_weight(float z, float zmax) { return (uint64_t)samp_weight_f64(z, zmax); }
 
 // block sums over the 1024 threads through LDS (one slot per wave)
 template <class T>

@@ -14,8 +14,8 @@
 // maximal logit and ends with it.  All sums are of integers: no result depends on the launch.
 //
 // Three launches: verify_rows_kernel finds each row's filter, W, and whether its draft is accepted; a stream's first row that
-// is not is then the only one whose weights are needed one by one: verify_chunks_kernel sums w' over chunks of its ids, and
-// verify_draw_kernel finds the chunk and the id, and writes what comes out.
+// is not is then the only one whose weights are needed one by one: verify_pieces_kernel sums w' over pieces of its ids, and
+// verify_draw_kernel finds the piece and the id, and writes what comes out.
 #include <algorithm>
 
 #include "sample.h"
@@ -32,8 +32,11 @@ struct VerRow {
   float p;            // the draft's probability
 };
 
-struct VerChunk {
-  uint64_t above, tie;  // w' of the chunk's kept tokens above pkey, of all its ties at pkey
+// A piece is kPiece consecutive ids of a stream's last row: 8 for each lane of a wave.
+constexpr int kPiece = 512;
+
+struct VerPiece {
+  uint64_t above, tie;  // w' of the piece's kept tokens above pkey, of all its ties at pkey
   uint32_t ties, pad;
 };
 
@@ -47,7 +50,7 @@ struct VerArgs {
   int32_t top_k1;
   const float* probs;         // [n_probs, V], or null
   const int32_t* probs_row;   // row of probs for each row, or null: the row itself
-  int32_t n_probs, R, V, S, chunk, n_chunks;
+  int32_t n_probs, R, V, S, pieces;
 };
 
 struct VerParams {
@@ -91,10 +94,10 @@ __device__ __forceinline__ bool ver_accepts(const VerArgs& a, int r, int d, uint
   return ver_uniform(a.u[r]) * qd * (double)W < (double)wd;
 }
 
-// what a rejected draft's distribution takes from a weight
-__device__ __forceinline__ uint64_t ver_rest(uint64_t w, float q, uint64_t W) {
-  const double t = floor((double)fmaxf(q, 0.f) * (double)W);
-  return t >= (double)w ? 0 : w - (uint64_t)t;
+// what a rejected draft's distribution leaves of a weight (whole numbers up to 2^40, which doubles hold)
+__device__ __forceinline__ double ver_rest(double w, float q, double W) {
+  const double left = w - floor((double)fmaxf(q, 0.f) * W);
+  return left > 0.0 ? left : 0.0;
 }
 
 // One row by a workgroup, for any logits: every pass reads the row again.
@@ -102,27 +105,6 @@ __device__ __forceinline__ void ver_row_general(const VerArgs& a, int row, const
   const uint16_t* x = a.logits + (size_t)row * a.V;
   const int tid = threadIdx.x, V = a.V, d = ver_draft(a, row);
   VerRow o = {};
-  if (!(p.temp > 0.f)) {
-    uint64_t best = 0;
-    for (int v = tid; v < V; v += kSampThreads) {
-      const uint64_t k = ((uint64_t)f32_key(bf2f(x[v])) << 32) | (uint32_t)~v;
-      best = k > best ? k : best;
-    }
-#pragma unroll
-    for (int off = 32; off >= 1; off >>= 1) {
-      const uint64_t y = __shfl_xor(best, off, 64);
-      best = y > best ? y : best;
-    }
-    __syncthreads();
-    if ((tid & 63) == 0) sh.red64[tid >> 6] = best;
-    __syncthreads();
-    for (int w = 0; w < kSampWaves; ++w) best = sh.red64[w] > best ? sh.red64[w] : best;
-    o.arg = (int)~(uint32_t)best;
-    o.accept = d == o.arg;
-    o.p = d == o.arg ? 1.f : 0.f;
-    if (tid == 0) *out = o;
-    return;
-  }
   auto zof = [&](int v) __attribute__((always_inline)) { return __fdiv_rn(bf2f(x[v]), p.tdiv); };
   uint32_t kth = 0;
   if (p.top_k > 0 && p.top_k < V) {
@@ -178,6 +160,307 @@ __device__ __forceinline__ void ver_row_general(const VerArgs& a, int row, const
   *out = o;
 }
 
+// ---- a greedy row ----
+// Two values of a word at once, in an order that 16-bit integers have: negative ones' magnitude bits turned round.  A thread keeps the
+// largest value and the first of its vectors that holds it; -0 orders below +0, so a row whose largest is a zero is looked at
+// again for the first zero of either sign.
+typedef short s16x2_t __attribute__((ext_vector_type(2)));
+
+struct __attribute__((packed, aligned(2))) VerVec { u32x4_t v; };  // 16 bytes at any element's address
+
+__device__ __forceinline__ s16x2_t ver_ordered(uint32_t w) {
+  const s16x2_t x = __builtin_bit_cast(s16x2_t, w);
+  return x ^ ((x >> 15) & (s16x2_t){0x7fff, 0x7fff});
+}
+
+struct VerGreedy {
+  uint64_t best[kSampWaves];
+  int at;
+};
+
+__device__ __forceinline__ void ver_row_greedy(const VerArgs& a, int row, VerGreedy& sh, VerRow* out) {
+  const uint16_t* x = a.logits + (size_t)row * a.V;
+  const int tid = threadIdx.x, V = a.V, full = V & ~7;
+  int best = -0x8001, at = V;  // (a thread without a vector: below every value)
+  constexpr int kAhead = 4;
+  for (int v0 = tid * 8; v0 < full; v0 += kAhead * kSampThreads * 8) {
+    u32x4_t w[kAhead];
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j) {
+      const int v = v0 + j * kSampThreads * 8;
+      if (v < full) w[j] = reinterpret_cast<const VerVec*>(x + v)->v;
+    }
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j) {
+      const int v = v0 + j * kSampThreads * 8;
+      if (v >= full) break;
+      const s16x2_t m = __builtin_elementwise_max(__builtin_elementwise_max(ver_ordered(w[j].x), ver_ordered(w[j].y)),
+                                                  __builtin_elementwise_max(ver_ordered(w[j].z), ver_ordered(w[j].w)));
+      const int top = max((int)m.x, (int)m.y);
+      if (top > best) {
+        best = top;
+        at = v;
+      }
+    }
+  }
+  auto one = [&](int v) __attribute__((always_inline)) { return (int)ver_ordered(x[v]).x; };
+  if (at < V) {  // the first of the vector
+    int i = 0;
+    while (i < 7 && one(at + i) != best) ++i;
+    at += i;
+  }
+  if (tid < V - full && one(full + tid) > best) {
+    best = one(full + tid);
+    at = full + tid;
+  }
+  // the largest, then the smallest id
+  uint64_t key = ((uint64_t)(uint32_t)(best + 0x8001) << 32) | (uint32_t)~at;
+#pragma unroll
+  for (int o = 32; o >= 1; o >>= 1) {
+    const uint64_t y = __shfl_xor(key, o, 64);
+    key = y > key ? y : key;
+  }
+  if ((tid & 63) == 0) sh.best[tid >> 6] = key;
+  if (tid == 0) sh.at = V;
+  __syncthreads();
+  for (int w = 0; w < kSampWaves; ++w) key = sh.best[w] > key ? sh.best[w] : key;
+  int arg = (int)~(uint32_t)key;
+  if ((int)(key >> 32) == 0x8001) {  // +0 (uniform)
+    for (int v = tid; v < V; v += kSampThreads)
+      if ((x[v] & 0x7fff) == 0) {
+        atomicMin(&sh.at, v);
+        break;
+      }
+    __syncthreads();
+    arg = sh.at;
+  }
+  if (tid) return;
+  VerRow o = {};
+  o.arg = arg;
+  o.accept = ver_draft(a, row) == arg;
+  o.p = o.accept ? 1.f : 0.f;
+  *out = o;
+}
+
+// ---- a row by the counts of its values ----
+// A bf16 row has few distinct values: the row is read once, each logit counted in LDS at its value's place, and everything else --
+// the maximum, the weights (fp64 exponentials), their sum, top-k, top-p -- runs over the values.  Places: |x| in [2^-40, 2^24)
+// of either sign, 8,192 each, and zero.  -inf and lower values than those have no weight wherever the maximum is one of these
+// (checked), and are left out; a row with any other value, or whose quotients x / temp are not all normal, is left to
+// ver_row_general.
+constexpr int kVerHalf = 8192;        // places of a sign
+constexpr uint32_t kVerFirst = 0x2b80;  // the bits of 2^-40
+constexpr int kVerBlocks = 2 * kVerHalf / 64 + 1;  // of 64 places, in descending order; the middle one is zero alone
+constexpr int kVerZeroBlock = kVerHalf / 64;
+
+struct VerHist {
+  uint32_t cnt[2 * kVerHalf];  // by the bits: positive ones, then negative ones, each ascending in |x|
+  uint64_t bw[kVerBlocks];
+  uint32_t bc[kVerBlocks];
+  uint32_t zeros, bad, low;    // zero's count; a value that has no place; the largest (as f32 key) of the low ones
+  int first;
+  uint64_t above, W;
+  uint32_t kplace, pplace;     // places in descending order + 1; 0: none
+  uint64_t tie_keep;
+  uint32_t before;
+};
+
+// the value of a place in descending order (block, lane), and its count
+__device__ __forceinline__ float ver_place_value(int b, int lane) {
+  if (b == kVerZeroBlock) return 0.f;
+  const uint32_t i = b < kVerZeroBlock ? kVerHalf - 1 - (b * 64 + lane) : (b - kVerZeroBlock - 1) * 64 + lane;
+  return bf2f((uint16_t)(kVerFirst + i + (b < kVerZeroBlock ? 0u : 0x8000u)));
+}
+__device__ __forceinline__ uint32_t ver_place_count(const VerHist& h, int b, int lane) {
+  if (b == kVerZeroBlock) return lane == 0 ? h.zeros : 0;
+  return h.cnt[b < kVerZeroBlock ? kVerHalf - 1 - (b * 64 + lane) : kVerHalf + (b - kVerZeroBlock - 1) * 64 + lane];
+}
+
+template <class T>
+__device__ __forceinline__ T wave_total(T v) {
+#pragma unroll
+  for (int o = 32; o >= 1; o >>= 1) v += __shfl_xor(v, o, 64);
+  return v;
+}
+
+// By one wave: the place, from the largest value down, where the running total of mass first exceeds limit, as block * 64 + lane + 1
+// (0: the total does not), and the total above it.  totals[b]: the blocks' masses; mass(b): this lane's.
+template <class Totals, class Mass>
+__device__ __forceinline__ uint32_t ver_select(Totals&& totals, Mass&& mass, uint64_t limit, uint64_t* above) {
+  const int lane = threadIdx.x & 63;
+  uint64_t run = 0;
+  for (int b0 = 0; b0 < kVerBlocks; b0 += 64) {
+    const uint64_t v = b0 + lane < kVerBlocks ? totals(b0 + lane) : 0, incl = wave_incl_scan(v);
+    const uint64_t hit = __ballot(run + incl > limit);
+    if (hit) {
+      const int l = __ffsll((unsigned long long)hit) - 1, b = b0 + l;
+      run += __shfl(incl - v, l, 64);
+      const uint64_t m = mass(b), in = wave_incl_scan(m);
+      const int k = __ffsll((unsigned long long)__ballot(run + in > limit)) - 1;
+      *above = run + __shfl(in - m, k, 64);
+      return (uint32_t)(b * 64 + k + 1);
+    }
+    run += __shfl(incl, 63, 64);
+  }
+  *above = run;
+  return 0;
+}
+
+// what there is no place for: counted where it has no weight, else the row is left to the general path
+__device__ __forceinline__ void ver_odd_value(VerHist& h, uint32_t bits) {
+  const uint32_t mag = bits & 0x7fffu;
+  if (mag == 0) atomicAdd(&h.zeros, 1u);
+  else if (mag - kVerFirst < (uint32_t)kVerHalf) atomicAdd(&h.cnt[(mag - kVerFirst) + (bits & 0x8000u ? kVerHalf : 0)], 1u);
+  else if ((bits & 0x8000u) && mag > kVerFirst) atomicMax(&h.low, f32_key(bf2f((uint16_t)bits)));
+  else h.bad = 1;
+}
+
+// false: the row is not one for this path (every thread)
+__device__ __forceinline__ bool ver_row_counts(const VerArgs& a, int row, const VerParams& p, VerHist& h, VerRow* out) {
+  const uint16_t* x = a.logits + (size_t)row * a.V;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, V = a.V, d = ver_draft(a, row);
+  if (!(p.tdiv < 0x1p60f)) return false;
+  for (int i = tid; i < 2 * kVerHalf / 4; i += kSampThreads) reinterpret_cast<uint4*>(h.cnt)[i] = make_uint4(0, 0, 0, 0);
+  if (tid == 0) {
+    h.zeros = h.bad = h.low = 0;
+    h.first = kVerBlocks;
+    h.before = 0;
+  }
+  __syncthreads();
+  // (two 16-bit places of a word at once; 0x6000 tells a value without one)
+  auto count = [&](uint32_t w) __attribute__((always_inline)) {
+    typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+    u16x2 t2 = __builtin_bit_cast(u16x2, w);
+    t2 -= (u16x2){(unsigned short)kVerFirst, (unsigned short)kVerFirst};
+    const uint32_t t = __builtin_bit_cast(uint32_t, t2);
+    if (t & 0x60006000u) {
+      ver_odd_value(h, w & 0xffffu);
+      ver_odd_value(h, w >> 16);
+      return;
+    }
+    const uint32_t at = ((t << 2) & 0x7ffc7ffcu) | (t & 0x80008000u);  // byte addresses
+    char* c = reinterpret_cast<char*>(h.cnt);
+    atomicAdd(reinterpret_cast<uint32_t*>(c + (at & 0xffffu)), 1u);
+    atomicAdd(reinterpret_cast<uint32_t*>(c + (at >> 16)), 1u);
+  };
+  const int full = V & ~7;
+  constexpr int kAhead = 4;
+  for (int v0 = tid * 8; v0 < full; v0 += kAhead * kSampThreads * 8) {
+    u32x4_t w[kAhead];
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j) {
+      const int v = v0 + j * kSampThreads * 8;
+      if (v < full) w[j] = reinterpret_cast<const VerVec*>(x + v)->v;
+    }
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j)
+      if (v0 + j * kSampThreads * 8 < full) {
+        count(w[j].x);
+        count(w[j].y);
+        count(w[j].z);
+        count(w[j].w);
+      }
+  }
+  if (tid < V - full) ver_odd_value(h, x[full + tid]);
+  const uint16_t dbits = d >= 0 ? x[d] : 0;
+  __syncthreads();
+  // the blocks' counts, and the first one with any
+  int mine = kVerBlocks;
+  for (int b = wave; b < kVerBlocks; b += kSampWaves) {
+    uint32_t n = ver_place_count(h, b, lane);
+    if (__ballot(n != 0)) {
+      mine = min(mine, b);
+      n = wave_total(n);
+    }
+    if (lane == 0) h.bc[b] = n;
+  }
+  if (lane == 0) atomicMin(&h.first, mine);
+  __syncthreads();
+  const int first = h.first;
+  if (h.bad || first == kVerBlocks) return false;
+  const int top = __ffsll((unsigned long long)__ballot(ver_place_count(h, first, lane) > 0)) - 1;
+  const float zmax = __fdiv_rn(ver_place_value(first, top), p.tdiv);
+  // (a row whose maximum is so low that a low value has weight; key 0: there was none)
+  if (h.low && samp_weight(__fdiv_rn(key_f32(h.low), p.tdiv), zmax) != 0) return false;
+  auto mass = [&](int b) __attribute__((always_inline)) -> uint64_t {
+    const uint32_t n = ver_place_count(h, b, lane);
+    return n ? n * samp_weight(__fdiv_rn(ver_place_value(b, lane), p.tdiv), zmax) : 0;
+  };
+  for (int b = wave; b < kVerBlocks; b += kSampWaves) {
+    uint64_t m = 0;
+    if (h.bc[b]) m = wave_total(mass(b));  // uniform
+    if (lane == 0) h.bw[b] = m;
+  }
+  __syncthreads();
+  if (wave == 0) {
+    uint64_t W = 0, above = 0;
+    uint32_t kplace = 0, pplace = 0;
+    uint64_t tie_keep = ~0ull;
+    for (int b = lane; b < kVerBlocks; b += 64) W += h.bw[b];
+    W = wave_total(W);
+    if (p.top_k > 0 && p.top_k < V)
+      kplace = ver_select([&](int b) { return (uint64_t)h.bc[b]; }, [&](int b) { return (uint64_t)ver_place_count(h, b, lane); },
+                          (uint64_t)(p.top_k - 1), &above);
+    const int kb = kplace ? (int)(kplace - 1) / 64 : kVerBlocks, kl = kplace ? (int)(kplace - 1) % 64 : 0;
+    auto kept = [&](int b) __attribute__((always_inline)) { return b > kb || (b == kb && lane > kl) ? 0 : mass(b); };
+    uint64_t kmass = 0;  // of the border's block
+    if (kplace) {
+      kmass = wave_total(kept(kb));
+      W = 0;
+      for (int b = lane; b < kb; b += 64) W += h.bw[b];
+      W = wave_total(W) + kmass;
+    }
+    if (p.top_p > 0.f && p.top_p < 1.f) {
+      const uint64_t T = (uint64_t)floor((double)p.top_p * (double)W);
+      pplace = ver_select([&](int b) { return b < kb ? h.bw[b] : b == kb ? kmass : (uint64_t)0; }, kept, T, &above);
+      if (pplace) {
+        const int pb = (int)(pplace - 1) / 64, pl = (int)(pplace - 1) % 64;
+        const uint64_t n = __shfl(ver_place_count(h, pb, lane), pl, 64);
+        const uint64_t wb = samp_weight(__fdiv_rn(ver_place_value(pb, pl), p.tdiv), zmax);
+        tie_keep = min(n, (T - above) / wb + 1);
+        W = above + tie_keep * wb;
+      }
+    }
+    if (lane == 0) {
+      h.W = W;
+      h.kplace = kplace;
+      h.pplace = pplace;
+      h.tie_keep = tie_keep;
+    }
+  }
+  __syncthreads();
+  VerRow o = {};
+  o.W = h.W;
+  o.tie_keep = h.tie_keep;
+  o.zmax = zmax;
+  auto key_of = [&](uint32_t place) __attribute__((always_inline)) {
+    return place ? f32_key(__fdiv_rn(ver_place_value((int)(place - 1) / 64, (int)(place - 1) % 64), p.tdiv)) : 0u;
+  };
+  o.kkey = key_of(h.kplace);
+  o.pkey = key_of(h.pplace);
+  uint64_t wd = 0;
+  if (d >= 0) {
+    const float z = __fdiv_rn(bf2f(dbits), p.tdiv);
+    const uint32_t k = f32_key(z);
+    bool in = k >= o.kkey && k >= o.pkey;
+    if (in && o.pkey && k == o.pkey) {  // a tie at the border: its rank in id order (uniform)
+      uint32_t n = 0;
+      for (int v = tid; v < d; v += kSampThreads) n += bf_key(x[v]) == bf_key(dbits);
+      n = wave_total(n);
+      if (lane == 0 && n) atomicAdd(&h.before, n);
+      __syncthreads();
+      in = h.before < o.tie_keep;
+    }
+    if (in) wd = samp_weight(z, zmax);
+  }
+  if (tid == 0) {
+    o.p = (float)((double)wd / (double)o.W);
+    o.accept = ver_accepts(a, row, d, wd, o.W);
+    *out = o;
+  }
+  return true;
+}
+
 // the stream of a row (the last one, should malformed cu_rows name several), -1 behind the last
 __device__ __forceinline__ int ver_stream(const VerArgs& a, int row, int* found) {
   if (threadIdx.x == 0) *found = -1;
@@ -188,12 +471,19 @@ __device__ __forceinline__ int ver_stream(const VerArgs& a, int row, int* found)
   return *found;
 }
 
-__global__ __launch_bounds__(kSampThreads) void verify_rows_kernel(VerArgs a, VerRow* __restrict__ rows) {
-  __shared__ SampShared sh;
+__global__ __launch_bounds__(kSampThreads, 8) void verify_rows_kernel(VerArgs a, VerRow* __restrict__ rows) {
+  __shared__ union { VerHist hist; VerGreedy greedy; SampShared gen; } sh;
   __shared__ int found;
   const int row = blockIdx.x, s = ver_stream(a, row, &found);
   if (s < 0) return;
-  ver_row_general(a, row, ver_params(a, s), sh, rows + row);
+  const VerParams p = ver_params(a, s);
+  if (!(p.temp > 0.f)) {
+    ver_row_greedy(a, row, sh.greedy, rows + row);
+    return;
+  }
+  if (ver_row_counts(a, row, p, sh.hist, rows + row)) return;
+  __syncthreads();  // every thread has read the union's other side
+  ver_row_general(a, row, p, sh.gen, rows + row);
 }
 
 // the first of a stream's rows that ends it (its end: none does); every thread gets it
@@ -212,87 +502,138 @@ struct VerWeights {
   const float* q;
   float tdiv, zmax;
   uint32_t kkey, pkey;
-  uint64_t W;
+  double W;
   int d;  // the rejected draft, where no distribution goes with it (else -1)
 
-  __device__ __forceinline__ uint64_t kept(uint16_t bits, bool* tie) const {
+  __device__ __forceinline__ double kept(uint16_t bits, bool* tie) const {
     const float z = __fdiv_rn(bf2f(bits), tdiv);
     const uint32_t k = f32_key(z);
     *tie = false;
-    if (k < kkey || k < pkey) return 0;
+    if (k < kkey || k < pkey) return 0.0;
     *tie = pkey != 0 && k == pkey;
-    return samp_weight(z, zmax);
+    return samp_weight_f64(z, zmax);
   }
-  __device__ __forceinline__ uint64_t rest(int v, uint64_t w) const { return v == d ? 0 : q && w ? ver_rest(w, q[v], W) : w; }
+  __device__ __forceinline__ double rest(int v, double w) const { return v == d ? 0.0 : q ? ver_rest(w, q[v], W) : w; }
 };
 
 __device__ __forceinline__ VerWeights ver_weights(const VerArgs& a, int s, int row, const VerRow& r) {
   const int d = ver_draft(a, row);
   const float* q = d >= 0 ? ver_probs(a, row) : nullptr;
-  return {a.logits + (size_t)row * a.V, q, ver_params(a, s).tdiv, r.zmax, r.kkey, r.pkey, r.W, q ? -1 : d};
+  return {a.logits + (size_t)row * a.V, q, ver_params(a, s).tdiv, r.zmax, r.kkey, r.pkey, (double)r.W, q ? -1 : d};
 }
 
-__global__ __launch_bounds__(kChunkThreads) void verify_chunks_kernel(VerArgs a, const VerRow* __restrict__ rows,
-                                                                      VerChunk* __restrict__ chunks) {
-  __shared__ uint64_t red[kChunkThreads / 64];
+// w' of the stop row's pieces, a wave each at a time, the next one's loads in flight.  Without a filter nearly every token has weight: the
+// weights of the common values are made once for each workgroup then, and looked up (kVerTable values of either sign from 2^-8 on).  A
+// piece's sums stay below 2^49 and are exact in doubles.
+constexpr int kVerTable = 16 * 128;
+constexpr uint32_t kVerTableFirst = 0x3b80;  // the bits of 2^-8
+constexpr int kPieceThreads = 256;
+
+struct __attribute__((packed, aligned(4))) VerVec4 { f32x4_t v; };
+
+__global__ __launch_bounds__(kPieceThreads, 4) void verify_pieces_kernel(VerArgs a, const VerRow* __restrict__ rows,
+                                                                         VerPiece* __restrict__ pieces) {
+  __shared__ double table[2 * kVerTable];
   __shared__ int stop_s;
-  const int c = blockIdx.x, s = blockIdx.y;
+  const int s = blockIdx.y, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int2 range = ver_range(a, s);
   const int stop = ver_stop(a, rows, range, &stop_s);
   if (stop >= range.y) return;
   if (!(ver_params(a, s).temp > 0.f)) return;
   const VerRow r = rows[stop];
   const VerWeights w = ver_weights(a, s, stop, r);
-  uint64_t above = 0, tie = 0, total;
-  uint32_t ties = 0;
-  for_chunk(w.x, c * a.chunk, min(a.V, (c + 1) * a.chunk), a.V % 8 == 0 && ((uintptr_t)a.logits & 15) == 0, [&](int v, uint16_t bits) {
-    bool is_tie;
-    const uint64_t k = w.rest(v, w.kept(bits, &is_tie));
-    if (is_tie) {
-      tie += k;
-      ++ties;
+  struct Loaded {
+    u32x4_t x;
+    f32x4_t q[2];
+  };
+  const int last = a.V >= 8 ? a.V - 8 : 0;
+  // 8 ids a lane; where the row ends within them, the row's last 8 (those before the lane's ids are left out below)
+  auto load = [&](int c) __attribute__((always_inline)) {
+    Loaded l = {};
+    const int v = min(c * kPiece + lane * 8, last);
+    if (a.V >= 8) {
+      l.x = reinterpret_cast<const VerVec*>(w.x + v)->v;
+      if (w.q) {
+        l.q[0] = reinterpret_cast<const VerVec4*>(w.q + v)->v;
+        l.q[1] = reinterpret_cast<const VerVec4*>(w.q + v + 4)->v;
+      }
     } else {
-      above += k;
+      uint32_t b[4] = {0, 0, 0, 0};
+#pragma unroll
+      for (int j = 0; j < 7; ++j)
+        if (j < a.V) {
+          b[j >> 1] |= (uint32_t)w.x[j] << (16 * (j & 1));
+          if (w.q) l.q[j >> 2][j & 3] = w.q[j];
+        }
+      l.x = u32x4_t{b[0], b[1], b[2], b[3]};
     }
-  });
-  VerChunk o;
-  block_excl_scan<kChunkThreads>(above, red, &total);
-  o.above = total;
-  block_excl_scan<kChunkThreads>(tie, red, &total);
-  o.tie = total;
-  block_excl_scan<kChunkThreads>((uint64_t)ties, red, &total);
-  o.ties = (uint32_t)total;
-  o.pad = 0;
-  if (threadIdx.x == 0) chunks[(size_t)s * a.n_chunks + c] = o;
-}
-
-// The ids of chunk c of which thread t has a run of consecutive ones, their ties ranked from `rank` on: f(id, w') in order.
-template <class F>
-__device__ __forceinline__ void ver_walk(const VerArgs& a, const VerWeights& w, int v0, int v1, uint64_t rank, uint64_t tie_keep, F&& f) {
-  for (int v = v0; v < v1; ++v) {
-    bool tie;
-    uint64_t k = w.kept(w.x[v], &tie);
-    if (tie && rank++ >= tie_keep) k = 0;
-    f(v, w.rest(v, k), k);
+    return l;
+  };
+  const int step = gridDim.x * (kPieceThreads / 64);
+  int c = blockIdx.x * (kPieceThreads / 64) + wave;
+  Loaded next = {};
+  if (c < a.pieces) next = load(c);
+  const bool look_up = r.kkey == 0 && r.pkey == 0;
+  if (look_up) {
+    for (int i = threadIdx.x; i < 2 * kVerTable; i += kPieceThreads) {
+      const uint32_t bits = kVerTableFirst + (i < kVerTable ? i : i - kVerTable + 0x8000u);
+      table[i] = samp_weight_f64(__fdiv_rn(bf2f((uint16_t)bits), w.tdiv), w.zmax);
+    }
+    __syncthreads();
+  }
+  for (; c < a.pieces; c += step) {
+    const Loaded l = next;
+    if (c + step < a.pieces) next = load(c + step);
+    const int first = c * kPiece + lane * 8, v0 = min(first, last);
+    const uint32_t x4[4] = {l.x.x, l.x.y, l.x.z, l.x.w};
+    double above = 0, tie = 0;
+    uint32_t ties = 0;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const uint16_t bits = (uint16_t)(x4[j >> 1] >> (16 * (j & 1)));
+      const int v = v0 + j;
+      double k;
+      bool is_tie = false;
+      const uint32_t at = (bits & 0x7fffu) - kVerTableFirst;
+      if (look_up && at < (uint32_t)kVerTable) k = table[at + (bits & 0x8000u ? kVerTable : 0)];
+      else k = w.kept(bits, &is_tie);
+      if (w.q) k = ver_rest(k, l.q[j >> 2][j & 3], w.W);
+      const bool here = v >= first && v < a.V;
+      if (v == w.d || !here) k = 0.0;
+      if (is_tie && here) {
+        tie += k;
+        ++ties;
+      } else {
+        above += k;
+      }
+    }
+    above = wave_total(above);
+    if (r.pkey) {  // uniform
+      tie = wave_total(tie);
+      ties = wave_total(ties);
+    }
+    if (lane == 0) pieces[(size_t)s * a.pieces + c] = {(uint64_t)above, (uint64_t)tie, ties, 0};
   }
 }
 
-__global__ __launch_bounds__(kSampThreads) void verify_draw_kernel(VerArgs a, const VerRow* __restrict__ rows,
-                                                                   const VerChunk* __restrict__ chunks, int32_t* __restrict__ tokens,
-                                                                   int32_t* __restrict__ counts, float* __restrict__ p_out) {
-  __shared__ uint64_t red[kSampWaves];
-  __shared__ uint64_t sum_s[kMaxChunks], tie_s[kMaxChunks];
+__global__ __launch_bounds__(kPiece) void verify_draw_kernel(VerArgs a, const VerRow* __restrict__ rows,
+                                                             const VerPiece* __restrict__ pieces, int32_t* __restrict__ tokens,
+                                                             int32_t* __restrict__ counts, float* __restrict__ p_out) {
+  __shared__ uint64_t red[kPiece / 64];
   __shared__ int stop_s, hit_s, part_s;
-  __shared__ uint64_t left_s;
+  __shared__ uint64_t left_s, part_before_s, hit_before_s, part_sum_s;
   const int s = blockIdx.x, tid = threadIdx.x;
   const int2 range = ver_range(a, s);
   const int stop = ver_stop(a, rows, range, &stop_s);
-  for (int r = range.x + tid; r < range.y; r += kSampThreads) {
+  for (int r = range.x + tid; r < range.y; r += kPiece) {
     if (r == stop) continue;
     tokens[r] = r < stop ? a.draft[r] : -1;
     p_out[r] = r < stop ? rows[r].p : 0.f;
   }
-  if (tid == 0) counts[s] = min(stop + 1, range.y) - range.x;
+  if (tid == 0) {
+    counts[s] = min(stop + 1, range.y) - range.x;
+    part_s = hit_s = -1;
+  }
   if (stop >= range.y) return;
   const VerRow r = rows[stop];
   if (!(ver_params(a, s).temp > 0.f)) {
@@ -303,81 +644,87 @@ __global__ __launch_bounds__(kSampThreads) void verify_draw_kernel(VerArgs a, co
     return;
   }
   const VerWeights w = ver_weights(a, s, stop, r);
-  auto run_of = [&](int c, int* v0, int* v1) __attribute__((always_inline)) {
-    const int c0 = c * a.chunk, c1 = min(a.V, c0 + a.chunk), per = (c1 - c0 + kSampThreads - 1) / kSampThreads;
-    *v0 = min(c1, c0 + tid * per);
-    *v1 = min(c1, *v0 + per);
-  };
-  // the rank of a thread's first tie
-  auto rank_of = [&](int c, int v0, int v1) __attribute__((always_inline)) {
-    uint64_t n = 0, all;
-    for (int v = v0; v < v1; ++v) {
-      bool tie;
-      w.kept(w.x[v], &tie);
-      n += tie;
+  // one id of a piece a thread: its w' and kept weight, with `before` ties in the pieces before
+  auto one = [&](int c, uint64_t before, double* kept) __attribute__((always_inline)) -> uint64_t {
+    const int v = c * kPiece + tid;
+    bool tie = false;
+    double k = v < a.V ? w.kept(w.x[v], &tie) : 0.0;
+    if (r.pkey) {  // uniform
+      uint64_t n;
+      const uint64_t rank = before + block_excl_scan<kPiece>((uint64_t)tie, red, &n);
+      if (tie && rank >= r.tie_keep) k = 0.0;
     }
-    return tie_s[c] + block_excl_scan<kSampThreads>(n, red, &all);
+    *kept = k;
+    return v < a.V ? (uint64_t)w.rest(v, k) : 0;
   };
-  // every chunk's w', and the one whose ties are kept in part
-  if (tid == 0) part_s = -1;
+  // a run of consecutive pieces a thread; the one whose ties are kept in part is summed anew
+  const VerPiece* mine = pieces + (size_t)s * a.pieces;
+  const int per = (a.pieces + kPiece - 1) / kPiece, c0 = min(a.pieces, tid * per), c1 = min(a.pieces, c0 + per);
+  uint64_t ties = 0, all;
+  for (int c = c0; c < c1; ++c) ties += mine[c].ties;
+  const uint64_t ties0 = r.pkey ? block_excl_scan<kPiece>(ties, red, &all) : 0;
+  uint64_t t = ties0;
   __syncthreads();
-  if (tid < 64) {
-    VerChunk c = {0, 0, 0, 0};
-    if (tid < a.n_chunks) c = chunks[(size_t)s * a.n_chunks + tid];
-    const uint64_t before = wave_incl_scan((uint64_t)c.ties) - c.ties;
-    tie_s[tid] = before;
-    sum_s[tid] = c.above + (before + c.ties <= r.tie_keep ? c.tie : 0);
-    if (before < r.tie_keep && before + c.ties > r.tie_keep) part_s = tid;
+  for (int c = c0; c < c1; ++c) {
+    const uint64_t n = mine[c].ties;
+    if (t < r.tie_keep && t + n > r.tie_keep) {
+      part_s = c;
+      part_before_s = t;
+    }
+    t += n;
   }
   __syncthreads();
   if (part_s >= 0) {  // uniform
-    int v0, v1;
-    run_of(part_s, &v0, &v1);
-    uint64_t mine = 0, total;
-    const uint64_t rank = rank_of(part_s, v0, v1);
-    ver_walk(a, w, v0, v1, rank, r.tie_keep, [&](int, uint64_t k, uint64_t) { mine += k; });
-    block_excl_scan<kSampThreads>(mine, red, &total);
-    if (tid == 0) sum_s[part_s] = total;
+    double kept;
+    uint64_t total;
+    const uint64_t k = one(part_s, part_before_s, &kept);
+    block_excl_scan<kPiece>(k, red, &total);
+    if (tid == 0) part_sum_s = total;
     __syncthreads();
   }
-  if (tid < 64) {
-    const uint64_t n = sum_s[tid], incl = wave_incl_scan(n), total = __shfl(incl, 63, 64);
-    if (tid == 0) hit_s = -1;
-    uint64_t target = (uint64_t)(ver_uniform(a.u_draw[s]) * (double)total);
-    target = total && target >= total ? total - 1 : target;
-    if (target >= incl - n && target < incl) {
-      hit_s = tid;
-      left_s = target - (incl - n);
+  auto sum_of = [&](int c, uint64_t before) __attribute__((always_inline)) {
+    const VerPiece m = mine[c];
+    return c == part_s ? part_sum_s : m.above + (before + m.ties <= r.tie_keep ? m.tie : 0);
+  };
+  uint64_t sum = 0, total;
+  t = ties0;
+  for (int c = c0; c < c1; ++c) {
+    sum += sum_of(c, t);
+    t += mine[c].ties;
+  }
+  uint64_t run = block_excl_scan<kPiece>(sum, red, &total);
+  uint64_t target = (uint64_t)(ver_uniform(a.u_draw[s]) * (double)total);
+  target = total && target >= total ? total - 1 : target;
+  if (target >= run && target < run + sum) {  // one thread, unless nothing is left
+    t = ties0;
+    for (int c = c0; c < c1; ++c) {
+      const uint64_t n = sum_of(c, t);
+      if (target >= run && target < run + n) {
+        hit_s = c;
+        left_s = target - run;
+        hit_before_s = t;
+      }
+      run += n;
+      t += mine[c].ties;
     }
   }
   __syncthreads();
-  const int c = hit_s;
-  if (c >= 0) {
-    int v0, v1;
-    run_of(c, &v0, &v1);
-    const uint64_t rank = rank_of(c, v0, v1);
-    uint64_t mine = 0, total;
-    ver_walk(a, w, v0, v1, rank, r.tie_keep, [&](int, uint64_t k, uint64_t) { mine += k; });
-    uint64_t run = block_excl_scan<kSampThreads>(mine, red, &total);
-    if (left_s >= run && left_s < run + mine) {
-      bool done = false;
-      ver_walk(a, w, v0, v1, rank, r.tie_keep, [&](int v, uint64_t k, uint64_t full) {
-        run += k;
-        if (!done && run > left_s) {
-          done = true;
-          tokens[stop] = v;
-          p_out[stop] = (float)((double)full / (double)r.W);
-        }
-      });
+  if (hit_s >= 0) {
+    double kept;
+    const uint64_t k = one(hit_s, hit_before_s, &kept);
+    run = block_excl_scan<kPiece>(k, red, &all);
+    if (left_s >= run && left_s < run + k) {
+      tokens[stop] = hit_s * kPiece + tid;
+      p_out[stop] = (float)(kept / (double)r.W);
     }
     return;
   }
   // nothing is left: the first id of maximal weight (the ties at the filter's border keep its first, which is the only one that counts here)
   uint64_t best = 0;
   int at = 0x7fffffff;
-  for (int v = tid; v < a.V; v += kSampThreads) {
+  for (int v = tid; v < a.V; v += kPiece) {
     bool tie;
-    const uint64_t k = w.kept(w.x[v], &tie);
+    const uint64_t k = (uint64_t)w.kept(w.x[v], &tie);
     if (k > best) {
       best = k;
       at = v;
@@ -392,7 +739,7 @@ __global__ __launch_bounds__(kSampThreads) void verify_draw_kernel(VerArgs a, co
   if ((tid & 63) == 0) red[tid >> 6] = top;
   if (tid == 0) hit_s = 0x7fffffff;
   __syncthreads();
-  for (int i = 0; i < kSampWaves; ++i) top = red[i] > top ? red[i] : top;
+  for (int i = 0; i < kPiece / 64; ++i) top = red[i] > top ? red[i] : top;
   if (best == top) atomicMin(&hit_s, at);
   __syncthreads();
   if (tid == 0) {
@@ -401,21 +748,13 @@ __global__ __launch_bounds__(kSampThreads) void verify_draw_kernel(VerArgs a, co
   }
 }
 
-static void verify_chunks(int V, int* chunk, int* n_chunks) {
-  const int steps = (int)(((int64_t)V + (int64_t)kMaxChunks * kChunkStep - 1) / ((int64_t)kMaxChunks * kChunkStep));
-  *chunk = std::max(kMinChunk, steps * kChunkStep);
-  *n_chunks = ceil_div(V, *chunk);
-}
-
 }  // namespace flyai
 
 using namespace flyai;
 
 extern "C" size_t flyai_spec_verify_workspace_bytes(int32_t R, int32_t V, int32_t S) {
   if (R < 0 || V < 1 || V > (1 << 22) || S < 0) return 0;
-  int chunk, n;
-  verify_chunks(V, &chunk, &n);
-  return (size_t)R * sizeof(VerRow) + (size_t)S * n * sizeof(VerChunk);
+  return (size_t)R * sizeof(VerRow) + (size_t)S * ceil_div(V, kPiece) * sizeof(VerPiece);
 }
 
 extern "C" int flyai_spec_verify(const uint16_t* logits, int32_t R, int32_t V, const int32_t* cu_rows, int32_t S, const int32_t* draft,
@@ -431,15 +770,17 @@ extern "C" int flyai_spec_verify(const uint16_t* logits, int32_t R, int32_t V, c
   FLYAI_REQUIRE(!draft_probs || probs_row || n_probs == R, "spec_verify: draft_probs of other rows need probs_row");
   FLYAI_REQUIRE(top_k >= 0, "spec_verify: top_k must be >= 0");
   FLYAI_REQUIRE(((uintptr_t)workspace & 7) == 0, "spec_verify: the workspace must be 8-byte aligned");
-  VerArgs a = {logits, cu_rows, draft, u, u_draw, temps, top_ps, top_ks, temp, top_p, top_k, draft_probs, probs_row, n_probs, R, V, S, 0, 0};
-  verify_chunks(V, &a.chunk, &a.n_chunks);
+  const VerArgs a = {logits, cu_rows, draft, u, u_draw, temps, top_ps, top_ks, temp, top_p, top_k, draft_probs, probs_row, n_probs, R, V, S,
+                     ceil_div(V, kPiece)};
   VerRow* rows = static_cast<VerRow*>(workspace);
-  VerChunk* chunks = reinterpret_cast<VerChunk*>(rows + R);
+  VerPiece* pieces = reinterpret_cast<VerPiece*>(rows + R);
   hipStream_t s = as_stream(stream);
   if (R > 0) {
     hipLaunchKernelGGL(verify_rows_kernel, dim3(R), dim3(kSampThreads), 0, s, a, rows);
-    hipLaunchKernelGGL(verify_chunks_kernel, dim3(a.n_chunks, S), dim3(kChunkThreads), 0, s, a, rows, chunks);
+    // four workgroups a CU, a piece a wave at least
+    const int wgs = std::max(1, std::min(ceil_div(a.pieces, kPieceThreads / 64), 4 * device_cus() / S));
+    hipLaunchKernelGGL(verify_pieces_kernel, dim3(wgs, S), dim3(kPieceThreads), 0, s, a, rows, pieces);
   }
-  hipLaunchKernelGGL(verify_draw_kernel, dim3(S), dim3(kSampThreads), 0, s, a, rows, chunks, tokens, counts, p);
+  hipLaunchKernelGGL(verify_draw_kernel, dim3(S), dim3(kPiece), 0, s, a, rows, pieces, tokens, counts, p);
   return check_launch("spec_verify");
 }

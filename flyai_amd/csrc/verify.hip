@@ -24,19 +24,21 @@ namespace flyai {
 
 struct VerRow {
   uint64_t W;         // kept weight
-  uint64_t tie_keep;  // ties at pkey that are kept, in id order
+  uint64_t tie_keep;  // ties at `edge` that are kept, in id order
   float zmax;
-  uint32_t kkey, pkey;  // f32 keys: z >= kkey and above pkey (0: no such bound) are kept
+  float lo, edge;     // kept are values from lo (top-k) and edge (top-p) on, -inf: no such bound; values of x, or of z = x / temp (by_z)
+  int32_t by_z;
   int32_t accept;
   int32_t arg;        // greedy: the first id of maximal logit
   float p;            // the draft's probability
+  int32_t pad;
 };
 
 // A piece is kPiece consecutive ids of a stream's last row: 8 for each lane of a wave.
 constexpr int kPiece = 512;
 
 struct VerPiece {
-  uint64_t above, tie;  // w' of the piece's kept tokens above pkey, of all its ties at pkey
+  uint64_t above, tie;  // w' of the piece's kept tokens above the edge, of all its ties there
   uint32_t ties, pad;
 };
 
@@ -120,7 +122,6 @@ __device__ __forceinline__ void ver_row_general(const VerArgs& a, int row, const
   for (int v = tid; v < V; v += kSampThreads) mkey = max(mkey, f32_key(zof(v)));
   mkey = block_max_u32(mkey, sh.red32);
   o.zmax = key_f32(mkey);
-  o.kkey = kth;
   uint64_t sum = 0;
   for (int v = tid; v < V; v += kSampThreads) {
     uint32_t k;
@@ -128,17 +129,18 @@ __device__ __forceinline__ void ver_row_general(const VerArgs& a, int row, const
   }
   o.W = block_sum(sum, sh.red64);
   o.tie_keep = ~0ull;
+  uint32_t pkey = 0;
   if (p.top_p > 0.f && p.top_p < 1.f) {
     const uint64_t T = (uint64_t)floor((double)p.top_p * (double)o.W);
     uint64_t above = 0;
-    o.pkey = radix_select(V, kept_k, [&](int v) { return samp_weight(zof(v), o.zmax); }, T, &above, sh);
-    if (o.pkey) {
+    pkey = radix_select(V, kept_k, [&](int v) { return samp_weight(zof(v), o.zmax); }, T, &above, sh);
+    if (pkey) {
       // tie j (0-based, id order) of the boundary value is kept iff above + j * wb <= T (tie 0 always is)
-      const uint64_t wb = samp_weight(key_f32(o.pkey), o.zmax);
+      const uint64_t wb = samp_weight(key_f32(pkey), o.zmax);
       uint32_t ties = 0;
-      for (int v = tid; v < V; v += kSampThreads) ties += f32_key(zof(v)) == o.pkey;
+      for (int v = tid; v < V; v += kSampThreads) ties += f32_key(zof(v)) == pkey;
       const uint64_t n = block_sum((uint64_t)ties, sh.red64);
-      o.tie_keep = wb == 0 ? n : min(n, (T - above) / wb + 1);
+      o.tie_keep = min(n, (T - above) / wb + 1);
       o.W = above + o.tie_keep * wb;
     }
   }
@@ -146,18 +148,64 @@ __device__ __forceinline__ void ver_row_general(const VerArgs& a, int row, const
   uint64_t wd = 0;
   if (d >= 0) {
     const uint32_t k = f32_key(zof(d));
-    bool kept = k >= kth && k >= o.pkey;
-    if (kept && o.pkey && k == o.pkey) {
+    bool kept = k >= kth && k >= pkey;
+    if (kept && pkey && k == pkey) {
       uint32_t before = 0;
-      for (int v = tid; v < d; v += kSampThreads) before += f32_key(zof(v)) == o.pkey;
+      for (int v = tid; v < d; v += kSampThreads) before += f32_key(zof(v)) == pkey;
       kept = block_sum((uint64_t)before, sh.red64) < o.tie_keep;
     }
     if (kept) wd = samp_weight(zof(d), o.zmax);
   }
   if (tid) return;
+  // (bounds that are NaN go with a NaN maximum, where nothing has weight)
+  o.lo = kth ? key_f32(kth) : -INFINITY;
+  o.edge = pkey ? key_f32(pkey) : -INFINITY;
+  o.by_z = 1;
   o.p = o.W ? (float)((double)wd / (double)o.W) : 0.f;
   o.accept = ver_accepts(a, row, d, wd, o.W);
   *out = o;
+}
+
+// the stream of a row (the last one, should malformed cu_rows name several), -1 behind the last
+__device__ __forceinline__ int ver_stream(const VerArgs& a, int row, int* found) {
+  if (threadIdx.x == 0) *found = -1;
+  __syncthreads();
+  for (int s = threadIdx.x; s < a.S; s += blockDim.x)
+    if (a.cu_rows[s] <= row && row < a.cu_rows[s + 1]) atomicMax(found, s);
+  __syncthreads();
+  return *found;
+}
+
+// ---- a row, 16 bytes a thread at a time ----
+struct __attribute__((packed, aligned(2))) VerVec { u32x4_t v; };  // 16 bytes at any element's address
+
+constexpr int kVerAhead = 2;
+constexpr int kVerBatch = kVerAhead * kSampThreads * 8;
+struct VerLoaded { u32x4_t w[kVerAhead]; };
+
+__device__ __forceinline__ VerLoaded ver_load(const uint16_t* __restrict__ x, int v0, int full) {
+  VerLoaded l;
+#pragma unroll
+  for (int j = 0; j < kVerAhead; ++j) {
+    const int v = v0 + j * kSampThreads * 8;
+    l.w[j] = u32x4_t{0, 0, 0, 0};
+    if (v < full) l.w[j] = reinterpret_cast<const VerVec*>(x + v)->v;
+  }
+  return l;
+}
+
+// f(first id, its 8 values) over the thread's vectors of [0, full), the next batch's loads in flight; `l` holds the first batch
+template <class F>
+__device__ __forceinline__ void ver_each(const uint16_t* __restrict__ x, int full, VerLoaded l, F&& f) {
+  for (int v0 = (int)threadIdx.x * 8; v0 < full; v0 += kVerBatch) {
+    const VerLoaded next = ver_load(x, v0 + kVerBatch, full);
+#pragma unroll
+    for (int j = 0; j < kVerAhead; ++j) {
+      const int v = v0 + j * kSampThreads * 8;
+      if (v < full) f(v, l.w[j]);
+    }
+    l = next;
+  }
 }
 
 // ---- a greedy row ----
@@ -165,8 +213,6 @@ __device__ __forceinline__ void ver_row_general(const VerArgs& a, int row, const
 // largest value and the first of its vectors that holds it; -0 orders below +0, so a row whose largest is a zero is looked at
 // again for the first zero of either sign.
 typedef short s16x2_t __attribute__((ext_vector_type(2)));
-
-struct __attribute__((packed, aligned(2))) VerVec { u32x4_t v; };  // 16 bytes at any element's address
 
 __device__ __forceinline__ s16x2_t ver_ordered(uint32_t w) {
   const s16x2_t x = __builtin_bit_cast(s16x2_t, w);
@@ -178,31 +224,19 @@ struct VerGreedy {
   int at;
 };
 
-__device__ __forceinline__ void ver_row_greedy(const VerArgs& a, int row, VerGreedy& sh, VerRow* out) {
+__device__ __forceinline__ void ver_row_greedy(const VerArgs& a, int row, const VerLoaded& l, VerGreedy& sh, VerRow* out) {
   const uint16_t* x = a.logits + (size_t)row * a.V;
   const int tid = threadIdx.x, V = a.V, full = V & ~7;
   int best = -0x8001, at = V;  // (a thread without a vector: below every value)
-  constexpr int kAhead = 4;
-  for (int v0 = tid * 8; v0 < full; v0 += kAhead * kSampThreads * 8) {
-    u32x4_t w[kAhead];
-#pragma unroll
-    for (int j = 0; j < kAhead; ++j) {
-      const int v = v0 + j * kSampThreads * 8;
-      if (v < full) w[j] = reinterpret_cast<const VerVec*>(x + v)->v;
+  ver_each(x, full, l, [&](int v, u32x4_t w) {
+    const s16x2_t m = __builtin_elementwise_max(__builtin_elementwise_max(ver_ordered(w.x), ver_ordered(w.y)),
+                                                __builtin_elementwise_max(ver_ordered(w.z), ver_ordered(w.w)));
+    const int top = max((int)m.x, (int)m.y);
+    if (top > best) {
+      best = top;
+      at = v;
     }
-#pragma unroll
-    for (int j = 0; j < kAhead; ++j) {
-      const int v = v0 + j * kSampThreads * 8;
-      if (v >= full) break;
-      const s16x2_t m = __builtin_elementwise_max(__builtin_elementwise_max(ver_ordered(w[j].x), ver_ordered(w[j].y)),
-                                                  __builtin_elementwise_max(ver_ordered(w[j].z), ver_ordered(w[j].w)));
-      const int top = max((int)m.x, (int)m.y);
-      if (top > best) {
-        best = top;
-        at = v;
-      }
-    }
-  }
+  });
   auto one = [&](int v) __attribute__((always_inline)) { return (int)ver_ordered(x[v]).x; };
   if (at < V) {  // the first of the vector
     int i = 0;
@@ -250,30 +284,36 @@ __device__ __forceinline__ void ver_row_greedy(const VerArgs& a, int row, VerGre
 // ver_row_general.
 constexpr int kVerHalf = 8192;        // places of a sign
 constexpr uint32_t kVerFirst = 0x2b80;  // the bits of 2^-40
-constexpr int kVerBlocks = 2 * kVerHalf / 64 + 1;  // of 64 places, in descending order; the middle one is zero alone
-constexpr int kVerZeroBlock = kVerHalf / 64;
+constexpr int kVerGroups = 2 * kVerHalf / 16;  // of 16 places in descending order; zero is in front of the first negative group's
 
 struct VerHist {
-  uint32_t cnt[2 * kVerHalf];  // by the bits: positive ones, then negative ones, each ascending in |x|
-  uint64_t bw[kVerBlocks];
-  uint32_t bc[kVerBlocks];
-  uint32_t zeros, bad, low;    // zero's count; a value that has no place; the largest (as f32 key) of the low ones
-  int first;
-  uint64_t above, W;
-  uint32_t kplace, pplace;     // places in descending order + 1; 0: none
+  uint32_t cnt[2 * kVerHalf];   // by the bits: positive ones, then negative ones, each ascending in |x|
+  uint64_t gsum[kVerGroups];    // the groups' weights
+  uint32_t gcnt[kVerGroups];    // ... and counts, for top-k
+  uint64_t red[kSampWaves];
+  uint32_t zeros, bad, low;     // zero's count; a value that has no place; the largest (as f32 key) of the low ones
+  int top;                      // the largest value's rank: negative ones from 0 on, zero, positive ones
+  int group;                    // what a selection found: the group, the total above it
+  uint64_t above, weight;
+  float edge;
   uint64_t tie_keep;
   uint32_t before;
 };
 
-// the value of a place in descending order (block, lane), and its count
-__device__ __forceinline__ float ver_place_value(int b, int lane) {
-  if (b == kVerZeroBlock) return 0.f;
-  const uint32_t i = b < kVerZeroBlock ? kVerHalf - 1 - (b * 64 + lane) : (b - kVerZeroBlock - 1) * 64 + lane;
-  return bf2f((uint16_t)(kVerFirst + i + (b < kVerZeroBlock ? 0u : 0x8000u)));
+__device__ __forceinline__ float ver_rank_value(int rank) {
+  if (rank == kVerHalf) return 0.f;
+  return bf2f((uint16_t)(kVerFirst + (rank > kVerHalf ? rank - kVerHalf - 1 : kVerHalf - 1 - rank + 0x8000)));
 }
-__device__ __forceinline__ uint32_t ver_place_count(const VerHist& h, int b, int lane) {
-  if (b == kVerZeroBlock) return lane == 0 ? h.zeros : 0;
-  return h.cnt[b < kVerZeroBlock ? kVerHalf - 1 - (b * 64 + lane) : kVerHalf + (b - kVerZeroBlock - 1) * 64 + lane];
+// place l (0 .. 16, in descending order) of a group: its value, and how often it is there
+__device__ __forceinline__ uint32_t ver_group_place(const VerHist& h, int g, int l, float* value) {
+  const int zero = g == kVerGroups / 2;
+  *value = 0.f;
+  if (zero && l == 0) return h.zeros;
+  l -= zero;
+  if (l < 0 || l >= 16) return 0;
+  const int i = g < kVerGroups / 2 ? kVerHalf - 1 - (g * 16 + l) : g * 16 + l;  // index of cnt
+  *value = bf2f((uint16_t)(kVerFirst + (i < kVerHalf ? i : i - kVerHalf + 0x8000)));
+  return h.cnt[i];
 }
 
 template <class T>
@@ -281,29 +321,6 @@ __device__ __forceinline__ T wave_total(T v) {
 #pragma unroll
   for (int o = 32; o >= 1; o >>= 1) v += __shfl_xor(v, o, 64);
   return v;
-}
-
-// By one wave: the place, from the largest value down, where the running total of mass first exceeds limit, as block * 64 + lane + 1
-// (0: the total does not), and the total above it.  totals[b]: the blocks' masses; mass(b): this lane's.
-template <class Totals, class Mass>
-__device__ __forceinline__ uint32_t ver_select(Totals&& totals, Mass&& mass, uint64_t limit, uint64_t* above) {
-  const int lane = threadIdx.x & 63;
-  uint64_t run = 0;
-  for (int b0 = 0; b0 < kVerBlocks; b0 += 64) {
-    const uint64_t v = b0 + lane < kVerBlocks ? totals(b0 + lane) : 0, incl = wave_incl_scan(v);
-    const uint64_t hit = __ballot(run + incl > limit);
-    if (hit) {
-      const int l = __ffsll((unsigned long long)hit) - 1, b = b0 + l;
-      run += __shfl(incl - v, l, 64);
-      const uint64_t m = mass(b), in = wave_incl_scan(m);
-      const int k = __ffsll((unsigned long long)__ballot(run + in > limit)) - 1;
-      *above = run + __shfl(in - m, k, 64);
-      return (uint32_t)(b * 64 + k + 1);
-    }
-    run += __shfl(incl, 63, 64);
-  }
-  *above = run;
-  return 0;
 }
 
 // what there is no place for: counted where it has no weight, else the row is left to the general path
@@ -315,17 +332,31 @@ __device__ __forceinline__ void ver_odd_value(VerHist& h, uint32_t bits) {
   else h.bad = 1;
 }
 
+// The group where the running total of the groups' masses (thread g: group g's, `run` before it) first exceeds limit, to h.group
+// (-1: none does) with the total above it.
+__device__ __forceinline__ void ver_find_group(VerHist& h, uint64_t run, uint64_t mass, uint64_t limit) {
+  if (threadIdx.x == 0) h.group = -1;
+  __syncthreads();
+  if (run <= limit && limit < run + mass) {
+    h.group = threadIdx.x;
+    h.above = run;
+  }
+  __syncthreads();
+}
+
 // false: the row is not one for this path (every thread)
-__device__ __forceinline__ bool ver_row_counts(const VerArgs& a, int row, const VerParams& p, VerHist& h, VerRow* out) {
+__device__ __forceinline__ bool ver_row_counts(const VerArgs& a, int row, const VerParams& p, const VerLoaded& l, VerHist& h, VerRow* out) {
   const uint16_t* x = a.logits + (size_t)row * a.V;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, V = a.V, d = ver_draft(a, row);
   if (!(p.tdiv < 0x1p60f)) return false;
   for (int i = tid; i < 2 * kVerHalf / 4; i += kSampThreads) reinterpret_cast<uint4*>(h.cnt)[i] = make_uint4(0, 0, 0, 0);
+  h.gsum[tid] = 0;
+  h.gcnt[tid] = 0;
   if (tid == 0) {
-    h.zeros = h.bad = h.low = 0;
-    h.first = kVerBlocks;
-    h.before = 0;
+    h.zeros = h.bad = h.low = h.before = 0;
+    h.top = -1;
   }
+  const uint16_t dbits = d >= 0 ? x[d] : 0;
   __syncthreads();
   // (two 16-bit places of a word at once; 0x6000 tells a value without one)
   auto count = [&](uint32_t w) __attribute__((always_inline)) {
@@ -344,144 +375,144 @@ __device__ __forceinline__ bool ver_row_counts(const VerArgs& a, int row, const 
     atomicAdd(reinterpret_cast<uint32_t*>(c + (at >> 16)), 1u);
   };
   const int full = V & ~7;
-  constexpr int kAhead = 4;
-  for (int v0 = tid * 8; v0 < full; v0 += kAhead * kSampThreads * 8) {
-    u32x4_t w[kAhead];
-#pragma unroll
-    for (int j = 0; j < kAhead; ++j) {
-      const int v = v0 + j * kSampThreads * 8;
-      if (v < full) w[j] = reinterpret_cast<const VerVec*>(x + v)->v;
-    }
-#pragma unroll
-    for (int j = 0; j < kAhead; ++j)
-      if (v0 + j * kSampThreads * 8 < full) {
-        count(w[j].x);
-        count(w[j].y);
-        count(w[j].z);
-        count(w[j].w);
-      }
-  }
+  ver_each(x, full, l, [&](int, u32x4_t w) {
+    count(w.x);
+    count(w.y);
+    count(w.z);
+    count(w.w);
+  });
   if (tid < V - full) ver_odd_value(h, x[full + tid]);
-  const uint16_t dbits = d >= 0 ? x[d] : 0;
   __syncthreads();
-  // the blocks' counts, and the first one with any
-  int mine = kVerBlocks;
-  for (int b = wave; b < kVerBlocks; b += kSampWaves) {
-    uint32_t n = ver_place_count(h, b, lane);
-    if (__ballot(n != 0)) {
-      mine = min(mine, b);
-      n = wave_total(n);
-    }
-    if (lane == 0) h.bc[b] = n;
+  // the values that are there: the largest, then their weights and counts by group
+  constexpr int kPer = 2 * kVerHalf / kSampThreads;
+  uint32_t n[kPer];
+  int top = -1;
+#pragma unroll
+  for (int j = 0; j < kPer; ++j) {
+    const int i = j * kSampThreads + tid;
+    n[j] = h.cnt[i];
+    if (n[j]) top = max(top, i < kVerHalf ? kVerHalf + 1 + i : 2 * kVerHalf - 1 - i);
   }
-  if (lane == 0) atomicMin(&h.first, mine);
+  if (tid == 0 && h.zeros) top = max(top, kVerHalf);
+#pragma unroll
+  for (int o = 32; o >= 1; o >>= 1) top = max(top, __shfl_xor(top, o, 64));
+  if (lane == 0) atomicMax(&h.top, top);
   __syncthreads();
-  const int first = h.first;
-  if (h.bad || first == kVerBlocks) return false;
-  const int top = __ffsll((unsigned long long)__ballot(ver_place_count(h, first, lane) > 0)) - 1;
-  const float zmax = __fdiv_rn(ver_place_value(first, top), p.tdiv);
+  if (h.bad || h.top < 0) return false;
+  const float zmax = __fdiv_rn(ver_rank_value(h.top), p.tdiv);
   // (a row whose maximum is so low that a low value has weight; key 0: there was none)
   if (h.low && samp_weight(__fdiv_rn(key_f32(h.low), p.tdiv), zmax) != 0) return false;
-  auto mass = [&](int b) __attribute__((always_inline)) -> uint64_t {
-    const uint32_t n = ver_place_count(h, b, lane);
-    return n ? n * samp_weight(__fdiv_rn(ver_place_value(b, lane), p.tdiv), zmax) : 0;
-  };
-  for (int b = wave; b < kVerBlocks; b += kSampWaves) {
-    uint64_t m = 0;
-    if (h.bc[b]) m = wave_total(mass(b));  // uniform
-    if (lane == 0) h.bw[b] = m;
+  const bool use_k = p.top_k > 0 && p.top_k < V, use_p = p.top_p > 0.f && p.top_p < 1.f;
+#pragma unroll
+  for (int j = 0; j < kPer; ++j) {
+    if (!n[j]) continue;
+    const int i = j * kSampThreads + tid;
+    const float v = bf2f((uint16_t)(kVerFirst + (i < kVerHalf ? i : i - kVerHalf + 0x8000)));
+    const uint64_t m = n[j] * samp_weight(__fdiv_rn(v, p.tdiv), zmax);
+    const int g = i < kVerHalf ? (kVerHalf - 1 - i) >> 4 : i >> 4;
+    if (m) atomicAdd((unsigned long long*)&h.gsum[g], (unsigned long long)m);
+    if (use_k) atomicAdd(&h.gcnt[g], n[j]);
+  }
+  if (tid == 0 && h.zeros) {
+    const uint64_t m = h.zeros * samp_weight(0.f, zmax);
+    atomicAdd((unsigned long long*)&h.gsum[kVerGroups / 2], (unsigned long long)m);
+    atomicAdd(&h.gcnt[kVerGroups / 2], h.zeros);
   }
   __syncthreads();
-  if (wave == 0) {
-    uint64_t W = 0, above = 0;
-    uint32_t kplace = 0, pplace = 0;
-    uint64_t tie_keep = ~0ull;
-    for (int b = lane; b < kVerBlocks; b += 64) W += h.bw[b];
-    W = wave_total(W);
-    if (p.top_k > 0 && p.top_k < V)
-      kplace = ver_select([&](int b) { return (uint64_t)h.bc[b]; }, [&](int b) { return (uint64_t)ver_place_count(h, b, lane); },
-                          (uint64_t)(p.top_k - 1), &above);
-    const int kb = kplace ? (int)(kplace - 1) / 64 : kVerBlocks, kl = kplace ? (int)(kplace - 1) % 64 : 0;
-    auto kept = [&](int b) __attribute__((always_inline)) { return b > kb || (b == kb && lane > kl) ? 0 : mass(b); };
-    uint64_t kmass = 0;  // of the border's block
-    if (kplace) {
-      kmass = wave_total(kept(kb));
-      W = 0;
-      for (int b = lane; b < kb; b += 64) W += h.bw[b];
-      W = wave_total(W) + kmass;
-    }
-    if (p.top_p > 0.f && p.top_p < 1.f) {
-      const uint64_t T = (uint64_t)floor((double)p.top_p * (double)W);
-      pplace = ver_select([&](int b) { return b < kb ? h.bw[b] : b == kb ? kmass : (uint64_t)0; }, kept, T, &above);
-      if (pplace) {
-        const int pb = (int)(pplace - 1) / 64, pl = (int)(pplace - 1) % 64;
-        const uint64_t n = __shfl(ver_place_count(h, pb, lane), pl, 64);
-        const uint64_t wb = samp_weight(__fdiv_rn(ver_place_value(pb, pl), p.tdiv), zmax);
-        tie_keep = min(n, (T - above) / wb + 1);
-        W = above + tie_keep * wb;
-      }
-    }
-    if (lane == 0) {
-      h.W = W;
-      h.kplace = kplace;
-      h.pplace = pplace;
-      h.tie_keep = tie_keep;
-    }
-  }
-  __syncthreads();
+  uint64_t mass = h.gsum[tid], W;
+  const uint64_t run = block_excl_scan<kSampThreads>(mass, h.red, &W);
   VerRow o = {};
-  o.W = h.W;
-  o.tie_keep = h.tie_keep;
   o.zmax = zmax;
-  auto key_of = [&](uint32_t place) __attribute__((always_inline)) {
-    return place ? f32_key(__fdiv_rn(ver_place_value((int)(place - 1) / 64, (int)(place - 1) % 64), p.tdiv)) : 0u;
-  };
-  o.kkey = key_of(h.kplace);
-  o.pkey = key_of(h.pplace);
+  o.lo = o.edge = -INFINITY;
+  o.tie_keep = ~0ull;
+  if (use_k) {  // the border's group, then its place, by the first wave's lanes
+    uint64_t all;
+    const uint64_t c = h.gcnt[tid], before = block_excl_scan<kSampThreads>(c, h.red, &all);
+    ver_find_group(h, before, c, (uint64_t)(p.top_k - 1));
+    const int g = h.group;
+    if (g >= 0) {
+      if (wave == 0) {
+        float v;
+        const uint32_t m = ver_group_place(h, g, lane, &v);
+        const uint64_t incl = wave_incl_scan((uint64_t)m);
+        const int k = __ffsll((unsigned long long)__ballot(h.above + incl > (uint64_t)(p.top_k - 1))) - 1;
+        const uint64_t kept = wave_total(m && lane <= k ? m * samp_weight(__fdiv_rn(v, p.tdiv), zmax) : 0);
+        if (lane == k) {
+          h.edge = v;
+          h.weight = kept;
+        }
+      }
+      __syncthreads();
+      o.lo = h.edge;
+      if (tid > g) mass = 0;
+      if (tid == g) {
+        mass = h.weight;
+        h.above = run + mass;
+      }
+      __syncthreads();
+      W = h.above;
+    }
+  }
+  if (use_p) {
+    const uint64_t T = (uint64_t)floor((double)p.top_p * (double)W);
+    ver_find_group(h, run, mass, T);
+    const int g = h.group;
+    if (g >= 0) {
+      if (wave == 0) {
+        float v;
+        const uint32_t m = ver_group_place(h, g, lane, &v);
+        const uint64_t w = m && v >= o.lo ? samp_weight(__fdiv_rn(v, p.tdiv), zmax) : 0;
+        const uint64_t incl = h.above + wave_incl_scan(m * w);
+        const int k = __ffsll((unsigned long long)__ballot(incl > T)) - 1;
+        if (lane == k) {
+          const uint64_t above = incl - m * w;
+          h.edge = v;
+          h.tie_keep = min((uint64_t)m, (T - above) / w + 1);
+          h.weight = above + h.tie_keep * w;
+        }
+      }
+      __syncthreads();
+      o.edge = h.edge;
+      o.tie_keep = h.tie_keep;
+      W = h.weight;
+    }
+  }
+  o.W = W;
   uint64_t wd = 0;
   if (d >= 0) {
-    const float z = __fdiv_rn(bf2f(dbits), p.tdiv);
-    const uint32_t k = f32_key(z);
-    bool in = k >= o.kkey && k >= o.pkey;
-    if (in && o.pkey && k == o.pkey) {  // a tie at the border: its rank in id order (uniform)
-      uint32_t n = 0;
-      for (int v = tid; v < d; v += kSampThreads) n += bf_key(x[v]) == bf_key(dbits);
-      n = wave_total(n);
-      if (lane == 0 && n) atomicAdd(&h.before, n);
+    const float v = bf2f(dbits);
+    bool in = v >= o.lo && v >= o.edge;
+    if (in && use_p && v == o.edge) {  // a tie at the border: its rank in id order (uniform)
+      uint32_t c = 0;
+      for (int i = tid; i < d; i += kSampThreads) c += bf2f(x[i]) == v;
+      c = wave_total(c);
+      if (lane == 0 && c) atomicAdd(&h.before, c);
       __syncthreads();
       in = h.before < o.tie_keep;
     }
-    if (in) wd = samp_weight(z, zmax);
+    if (in) wd = samp_weight(__fdiv_rn(v, p.tdiv), zmax);
   }
   if (tid == 0) {
-    o.p = (float)((double)wd / (double)o.W);
-    o.accept = ver_accepts(a, row, d, wd, o.W);
+    o.p = (float)((double)wd / (double)W);
+    o.accept = ver_accepts(a, row, d, wd, W);
     *out = o;
   }
   return true;
 }
 
-// the stream of a row (the last one, should malformed cu_rows name several), -1 behind the last
-__device__ __forceinline__ int ver_stream(const VerArgs& a, int row, int* found) {
-  if (threadIdx.x == 0) *found = -1;
-  __syncthreads();
-  for (int s = threadIdx.x; s < a.S; s += blockDim.x)
-    if (a.cu_rows[s] <= row && row < a.cu_rows[s + 1]) atomicMax(found, s);
-  __syncthreads();
-  return *found;
-}
-
 __global__ __launch_bounds__(kSampThreads, 8) void verify_rows_kernel(VerArgs a, VerRow* __restrict__ rows) {
   __shared__ union { VerHist hist; VerGreedy greedy; SampShared gen; } sh;
   __shared__ int found;
-  const int row = blockIdx.x, s = ver_stream(a, row, &found);
+  const int row = blockIdx.x;
+  const VerLoaded l = ver_load(a.logits + (size_t)row * a.V, (int)threadIdx.x * 8, a.V & ~7);  // while the stream is looked up
+  const int s = ver_stream(a, row, &found);
   if (s < 0) return;
   const VerParams p = ver_params(a, s);
   if (!(p.temp > 0.f)) {
-    ver_row_greedy(a, row, sh.greedy, rows + row);
+    ver_row_greedy(a, row, l, sh.greedy, rows + row);
     return;
   }
-  if (ver_row_counts(a, row, p, sh.hist, rows + row)) return;
+  if (ver_row_counts(a, row, p, l, sh.hist, rows + row)) return;
   __syncthreads();  // every thread has read the union's other side
   ver_row_general(a, row, p, sh.gen, rows + row);
 }
@@ -500,18 +531,16 @@ __device__ __forceinline__ int ver_stop(const VerArgs& a, const VerRow* __restri
 struct VerWeights {
   const uint16_t* x;
   const float* q;
-  float tdiv, zmax;
-  uint32_t kkey, pkey;
+  float tdiv, zmax, lo, edge;
+  bool by_z;
   double W;
   int d;  // the rejected draft, where no distribution goes with it (else -1)
 
-  __device__ __forceinline__ double kept(uint16_t bits, bool* tie) const {
-    const float z = __fdiv_rn(bf2f(bits), tdiv);
-    const uint32_t k = f32_key(z);
-    *tie = false;
-    if (k < kkey || k < pkey) return 0.0;
-    *tie = pkey != 0 && k == pkey;
-    return samp_weight_f64(z, zmax);
+  __device__ __forceinline__ double kept(uint32_t bits, bool* tie) const {
+    const float v = bf2f((uint16_t)bits), y = by_z ? __fdiv_rn(v, tdiv) : v;
+    *tie = y == edge;
+    if (!(y >= lo && y >= edge)) return 0.0;
+    return samp_weight_f64(by_z ? y : __fdiv_rn(v, tdiv), zmax);
   }
   __device__ __forceinline__ double rest(int v, double w) const { return v == d ? 0.0 : q ? ver_rest(w, q[v], W) : w; }
 };
@@ -519,21 +548,22 @@ struct VerWeights {
 __device__ __forceinline__ VerWeights ver_weights(const VerArgs& a, int s, int row, const VerRow& r) {
   const int d = ver_draft(a, row);
   const float* q = d >= 0 ? ver_probs(a, row) : nullptr;
-  return {a.logits + (size_t)row * a.V, q, ver_params(a, s).tdiv, r.zmax, r.kkey, r.pkey, (double)r.W, q ? -1 : d};
+  return {a.logits + (size_t)row * a.V, q, ver_params(a, s).tdiv, r.zmax, r.lo, r.edge, r.by_z != 0, (double)r.W, q ? -1 : d};
 }
 
-// w' of the stop row's pieces, a wave each at a time, the next one's loads in flight.  Without a filter nearly every token has weight: the
-// weights of the common values are made once for each workgroup then, and looked up (kVerTable values of either sign from 2^-8 on).  A
-// piece's sums stay below 2^49 and are exact in doubles.
+// w' of the stop row's pieces, a wave each at a time, the next one's loads in flight.  A piece's sums stay below 2^49 and are exact in
+// doubles.  Without a filter nearly every token has weight: a workgroup with many pieces makes the weights of the common values once
+// (kVerTable values of either sign from 2^-8 on) and looks them up; the others are made one by one.
 constexpr int kVerTable = 16 * 128;
 constexpr uint32_t kVerTableFirst = 0x3b80;  // the bits of 2^-8
 constexpr int kPieceThreads = 256;
+constexpr int kTablePieces = 32;  // four times as many tokens as the table has values
 
 struct __attribute__((packed, aligned(4))) VerVec4 { f32x4_t v; };
 
 __global__ __launch_bounds__(kPieceThreads, 4) void verify_pieces_kernel(VerArgs a, const VerRow* __restrict__ rows,
                                                                          VerPiece* __restrict__ pieces) {
-  __shared__ double table[2 * kVerTable];
+  __shared__ double table[2 * kVerTable + 1];  // the last one: 0
   __shared__ int stop_s;
   const int s = blockIdx.y, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int2 range = ver_range(a, s);
@@ -543,29 +573,29 @@ __global__ __launch_bounds__(kPieceThreads, 4) void verify_pieces_kernel(VerArgs
   const VerRow r = rows[stop];
   const VerWeights w = ver_weights(a, s, stop, r);
   struct Loaded {
-    u32x4_t x;
+    uint32_t x[4];
     f32x4_t q[2];
   };
   const int last = a.V >= 8 ? a.V - 8 : 0;
-  // 8 ids a lane; where the row ends within them, the row's last 8 (those before the lane's ids are left out below)
+  // 8 ids a lane; where the row ends within them, the row's last 8 (those before the lane's ids are taken out below)
   auto load = [&](int c) __attribute__((always_inline)) {
     Loaded l = {};
     const int v = min(c * kPiece + lane * 8, last);
     if (a.V >= 8) {
-      l.x = reinterpret_cast<const VerVec*>(w.x + v)->v;
+      const u32x4_t x = reinterpret_cast<const VerVec*>(w.x + v)->v;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) l.x[j] = x[j];
       if (w.q) {
         l.q[0] = reinterpret_cast<const VerVec4*>(w.q + v)->v;
         l.q[1] = reinterpret_cast<const VerVec4*>(w.q + v + 4)->v;
       }
     } else {
-      uint32_t b[4] = {0, 0, 0, 0};
 #pragma unroll
       for (int j = 0; j < 7; ++j)
         if (j < a.V) {
-          b[j >> 1] |= (uint32_t)w.x[j] << (16 * (j & 1));
+          l.x[j >> 1] |= (uint32_t)w.x[j] << (16 * (j & 1));
           if (w.q) l.q[j >> 2][j & 3] = w.q[j];
         }
-      l.x = u32x4_t{b[0], b[1], b[2], b[3]};
     }
     return l;
   };
@@ -573,44 +603,76 @@ __global__ __launch_bounds__(kPieceThreads, 4) void verify_pieces_kernel(VerArgs
   int c = blockIdx.x * (kPieceThreads / 64) + wave;
   Loaded next = {};
   if (c < a.pieces) next = load(c);
-  const bool look_up = r.kkey == 0 && r.pkey == 0;
+  const bool look_up = r.lo == -INFINITY && r.edge == -INFINITY && a.pieces >= kTablePieces * (int)gridDim.x;
   if (look_up) {
     for (int i = threadIdx.x; i < 2 * kVerTable; i += kPieceThreads) {
       const uint32_t bits = kVerTableFirst + (i < kVerTable ? i : i - kVerTable + 0x8000u);
       table[i] = samp_weight_f64(__fdiv_rn(bf2f((uint16_t)bits), w.tdiv), w.zmax);
     }
+    if (threadIdx.x == 0) table[2 * kVerTable] = 0.0;
     __syncthreads();
   }
   for (; c < a.pieces; c += step) {
-    const Loaded l = next;
+    Loaded l = next;
     if (c + step < a.pieces) next = load(c + step);
     const int first = c * kPiece + lane * 8, v0 = min(first, last);
-    const uint32_t x4[4] = {l.x.x, l.x.y, l.x.z, l.x.w};
+    const int no = look_up ? w.d : -1;  // (a filter counts the draft among its ties)
+    if ((c + 1) * kPiece > a.V || (no >= 0 && no / kPiece == c)) {  // ids that are others' or none, and the draft: -inf has no weight
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const int v = v0 + j;
+        if (v < first || v >= a.V || v == no) l.x[j >> 1] = j & 1 ? (l.x[j >> 1] & 0xffffu) | 0xff800000u : (l.x[j >> 1] & 0xffff0000u) | 0xff80u;
+      }
+    }
     double above = 0, tie = 0;
     uint32_t ties = 0;
+    if (look_up) {
+      typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+      uint32_t at[4], odd = 0;  // byte addresses of a word's two values; the bits that tell values outside the table
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const uint16_t bits = (uint16_t)(x4[j >> 1] >> (16 * (j & 1)));
-      const int v = v0 + j;
-      double k;
-      bool is_tie = false;
-      const uint32_t at = (bits & 0x7fffu) - kVerTableFirst;
-      if (look_up && at < (uint32_t)kVerTable) k = table[at + (bits & 0x8000u ? kVerTable : 0)];
-      else k = w.kept(bits, &is_tie);
-      if (w.q) k = ver_rest(k, l.q[j >> 2][j & 3], w.W);
-      const bool here = v >= first && v < a.V;
-      if (v == w.d || !here) k = 0.0;
-      if (is_tie && here) {
-        tie += k;
-        ++ties;
-      } else {
+      for (int i = 0; i < 4; ++i) {
+        u16x2 t2 = __builtin_bit_cast(u16x2, l.x[i]);
+        t2 -= (u16x2){(unsigned short)kVerTableFirst, (unsigned short)kVerTableFirst};
+        const uint32_t t = __builtin_bit_cast(uint32_t, t2);
+        at[i] = ((t << 3) & 0x3ff83ff8u) | ((t >> 1) & 0x40004000u);
+        odd |= ((t & 0x78000000u) ? 2u : 0u) << (2 * i) | ((t & 0x7800u) ? 1u : 0u) << (2 * i);
+      }
+      const char* tab = reinterpret_cast<const char*>(table);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        uint32_t b = j & 1 ? at[j >> 1] >> 16 : at[j >> 1] & 0xffffu;
+        if (odd >> j & 1) b = 2 * kVerTable * 8;
+        double k = *reinterpret_cast<const double*>(tab + b);
+        if (w.q) k = ver_rest(k, l.q[j >> 2][j & 3], w.W);
         above += k;
+      }
+      while (odd) {  // a lane's next value that has no entry
+        const int v = v0 + __ffs(odd) - 1;
+        odd &= odd - 1;
+        bool none;
+        if (v >= first && v < a.V && v != w.d) above += w.rest(v, w.kept(w.x[v], &none));
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        bool is_tie;
+        double k = w.kept(j & 1 ? l.x[j >> 1] >> 16 : l.x[j >> 1] & 0xffffu, &is_tie);
+        if (w.q) k = ver_rest(k, l.q[j >> 2][j & 3], w.W);
+        if (v0 + j == w.d) k = 0.0;
+        if (is_tie) {
+          tie += k;
+          ++ties;
+        } else {
+          above += k;
+        }
       }
     }
     above = wave_total(above);
-    if (r.pkey) {  // uniform
+    if (r.edge > -INFINITY) {  // uniform
       tie = wave_total(tie);
       ties = wave_total(ties);
+    } else {  // (ties with -inf are none)
+      ties = 0;
     }
     if (lane == 0) pieces[(size_t)s * a.pieces + c] = {(uint64_t)above, (uint64_t)tie, ties, 0};
   }
@@ -649,7 +711,7 @@ __global__ __launch_bounds__(kPiece) void verify_draw_kernel(VerArgs a, const Ve
     const int v = c * kPiece + tid;
     bool tie = false;
     double k = v < a.V ? w.kept(w.x[v], &tie) : 0.0;
-    if (r.pkey) {  // uniform
+    if (r.edge > -INFINITY) {  // uniform
       uint64_t n;
       const uint64_t rank = before + block_excl_scan<kPiece>((uint64_t)tie, red, &n);
       if (tie && rank >= r.tie_keep) k = 0.0;
@@ -662,7 +724,7 @@ __global__ __launch_bounds__(kPiece) void verify_draw_kernel(VerArgs a, const Ve
   const int per = (a.pieces + kPiece - 1) / kPiece, c0 = min(a.pieces, tid * per), c1 = min(a.pieces, c0 + per);
   uint64_t ties = 0, all;
   for (int c = c0; c < c1; ++c) ties += mine[c].ties;
-  const uint64_t ties0 = r.pkey ? block_excl_scan<kPiece>(ties, red, &all) : 0;
+  const uint64_t ties0 = r.edge > -INFINITY ? block_excl_scan<kPiece>(ties, red, &all) : 0;
   uint64_t t = ties0;
   __syncthreads();
   for (int c = c0; c < c1; ++c) {

@@ -20,7 +20,7 @@ namespace flyai {
 
 constexpr int kShRowTokens = 16;      // tokens of a prefix item's tile (4 waves x 2 tiles of 16 rows x 2 tokens)
 constexpr int kShWaveTokens = 4;      // tokens of a wave item
-constexpr int kShMaxSeqs = 8192, kShMaxPrefixes = 1024;
+constexpr int kShMaxSeqs = 4096, kShMaxPrefixes = 1024;
 constexpr int kShChunks = 16;         // a prefix's chunks: at most this many
 constexpr int kShMinChunk = 128;
 constexpr int kShOwnChunk = 512;
@@ -84,27 +84,35 @@ __host__ __device__ inline ShLayout sh_layout(int T, int S, int n_prefix) {
 
 constexpr int kShPlanThreads = 1024;
 
-template <class T>
-__device__ __forceinline__ T sh_excl_scan(T v, T* red, T* total) {
+// inclusive sum over the wave's lanes, by DPP (no LDS round trips): within rows of 16, then across them
+__device__ __forceinline__ int sh_wave_scan(int v) {
+  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, true);  // row_shr:1
+  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, true);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, true);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, true);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, true);  // row_bcast:15 to rows 1 and 3
+  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, true);  // row_bcast:31 to rows 2 and 3
+  return v;
+}
+
+// N exclusive sums over the workgroup at once; total gets the sums
+template <int N>
+__device__ __forceinline__ void sh_excl_scan(int (&v)[N], int (&total)[N], int (&red)[N][kShPlanThreads / 64]) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  T incl = v;
+  int incl[N];
 #pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const T y = __shfl_up(incl, o, 64);
-    if (lane >= o) incl += y;
-  }
+  for (int i = 0; i < N; ++i) incl[i] = sh_wave_scan(v[i]);
   __syncthreads();  // the last use of red is over
-  if (lane == 63) red[wave] = incl;
-  __syncthreads();
-  T sums = lane < kShPlanThreads / 64 ? red[lane] : (T)0;
 #pragma unroll
-  for (int o = 1; o < kShPlanThreads / 64; o <<= 1) {
-    const T y = __shfl_up(sums, o, 64);
-    if (lane >= o) sums += y;
+  for (int i = 0; i < N; ++i)
+    if (lane == 63) red[i][wave] = incl[i];
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const int sums = sh_wave_scan(lane < kShPlanThreads / 64 ? red[i][lane] : 0);
+    total[i] = __builtin_amdgcn_readlane(sums, kShPlanThreads / 64 - 1);
+    v[i] = incl[i] - v[i] + (wave ? __builtin_amdgcn_readlane(sums, max(wave, 1) - 1) : 0);
   }
-  *total = __shfl(sums, kShPlanThreads / 64 - 1, 64);
-  const T base = wave ? __shfl(sums, wave - 1, 64) : (T)0;
-  return base + incl - v;
 }
 
 __device__ __forceinline__ int sh_prefix_chunk(int P) {
@@ -129,9 +137,27 @@ __device__ __forceinline__ bool sh_slab_ok(int64_t base, int cap, int Hkv, int64
   return cap > 0 && cap % 64 == 0 && base >= 0 && base % 8 == 0 && base <= pool - (int64_t)Hkv * cap * 64;
 }
 
-// One workgroup.  Sequences, then prefixes are counted and scanned in LDS, then the lists are written token by token and entry by
-// entry.  A prefix's tokens are listed in the order in which its sequences' counts arrive at an LDS counter: which rows share
-// a tile may change from launch to launch, a row's result does not (no row's steps depend on its tile mates).
+// What the plan keeps of a sequence and of a prefix, in LDS.
+struct ShSeqs {
+  int32_t cu[kShMaxSeqs + 1];  // its first token
+  int32_t own0[kShMaxSeqs];    // the slab position of its first token; -1: the sequence has no tokens, or is refused
+  int32_t prefix[kShMaxSeqs];  // -1: none
+  int32_t place[kShMaxSeqs];   // its first listed token's place among its prefix's
+  int32_t wave0[kShMaxSeqs], rec0[kShMaxSeqs];  // its first wave entry and record
+};
+struct ShPrefixes {
+  int32_t len[kShMaxPrefixes];  // -1: refused
+  int32_t cap[kShMaxPrefixes];
+  int64_t base[kShMaxPrefixes];
+  int32_t count[kShMaxPrefixes];  // listed tokens
+  int32_t lo[kShMaxPrefixes];     // the first position that any of them sees
+  int32_t list0[kShMaxPrefixes], entry0[kShMaxPrefixes], rec0[kShMaxPrefixes];
+};
+constexpr int kShMaxOwnChunks = 4096;  // of a sequence, for the counts to stay in 32 bits: past it no sequence is split
+
+// One workgroup, so that nothing but LDS lies between the counts and the lists: one round trip for the lengths, three sums over the
+// workgroup, the lists.  A prefix's tokens are listed in the order in which its sequences' counts arrive at an LDS counter: which rows
+// share a tile may change from launch to launch, a row's result does not (no row's steps depend on its tile mates).
 __global__ __launch_bounds__(kShPlanThreads) void attn_shared_plan_kernel(ShBatch b, char* __restrict__ plan) {
   const ShLayout L = sh_layout(b.T, b.S, b.n_prefix);
   ShHeader* hdr = reinterpret_cast<ShHeader*>(plan);
@@ -139,260 +165,228 @@ __global__ __launch_bounds__(kShPlanThreads) void attn_shared_plan_kernel(ShBatc
   ShEntry* waves = reinterpret_cast<ShEntry*>(plan + L.o_waves);
   int2* list = reinterpret_cast<int2*>(plan + L.o_list);
   ShToken* tokens = reinterpret_cast<ShToken*>(plan + L.o_tokens);
-  __shared__ int32_t cu_s[kShMaxSeqs + 1];    // first token of each sequence
-  __shared__ int32_t place_s[kShMaxSeqs];     // of its first listed token among its prefix's
-  __shared__ int32_t wbase_s[kShMaxSeqs];     // its first wave entry
-  __shared__ int32_t pcnt_s[kShMaxPrefixes];  // listed tokens of a prefix
-  __shared__ int32_t plo_s[kShMaxPrefixes];   // the first of its positions that any of them sees
-  __shared__ int32_t plist_s[kShMaxPrefixes], pent_s[kShMaxPrefixes], prec_s[kShMaxPrefixes];
-  __shared__ int64_t red[kShPlanThreads / 64];
-  __shared__ int32_t status_s;
+  __shared__ ShSeqs sq;
+  __shared__ ShPrefixes px;
+  __shared__ int red[6][kShPlanThreads / 64];
+  __shared__ int status_s;
   const int tid = threadIdx.x;
-  if (tid == 0) status_s = 0;
-  for (int p = tid; p < b.n_prefix; p += kShPlanThreads) {
-    pcnt_s[p] = 0;
-    plo_s[p] = INT32_MAX;
-  }
-  __syncthreads();
-  int32_t status = 0;
   const int per = (b.S + kShPlanThreads - 1) / kShPlanThreads;
-  const int s0 = min(b.S, tid * per), s1 = min(b.S, s0 + per);
-
-  int64_t local = 0, total;
-#pragma unroll 1
-  for (int s = s0; s < s1; ++s) local += max(b.q_lens[s], 0);
-  int64_t run = sh_excl_scan(local, red, &total);
-  if (total > b.T) status |= kShPastTokens;
-  // a sequence as it counts: no tokens where anything about it is out of bounds
-  struct Seq {
-    int q, P, own0;  // tokens, positions before its own slab's, the first token's slab position
-    int p;           // its prefix, if its tokens see any of it
-  };
-  auto seq_of = [&](int s, int64_t first, int32_t* st) __attribute__((always_inline)) {
-    Seq r = {0, 0, 0, -1};
-    const int q = b.q_lens[s], start = b.starts[s], p = b.prefix_of[s];
-    if (q < 0 || start < 0) *st |= kShBadSequence;
-    if (q <= 0 || start < 0 || first + q > b.T) return r;
-    int P = 0;
-    if (p >= 0) {
-      if (p >= b.n_prefix) { *st |= kShBadPrefix; return r; }
-      P = b.prefix_len[p];
-      if (P < 0 || P > b.prefix_cap[p] || !sh_slab_ok(b.prefix_base[p], b.prefix_cap[p], b.Hkv, b.pool_elems)) { *st |= kShBadPrefix; return r; }
+  constexpr int kPer = kShMaxSeqs / kShPlanThreads;
+  const int s0 = tid * per;
+  int32_t status = 0;
+  // everything that the batch is described by, in one round trip
+  int q[kPer], start[kPer], prefix[kPer], cap[kPer];
+  int64_t base[kPer];
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    const bool there = i < per && s0 + i < b.S;
+    const int s = there ? s0 + i : 0;
+    q[i] = start[i] = cap[i] = 0;
+    prefix[i] = -1;
+    base[i] = 0;
+    if (there) {
+      q[i] = b.q_lens[s];
+      start[i] = b.starts[s];
+      prefix[i] = b.prefix_of[s];
+      cap[i] = b.kv_cap[s];
+      base[i] = b.kv_base[s];
     }
-    if (start < P) { *st |= kShBeforePrefix; return r; }
-    if (!sh_slab_ok(b.kv_base[s], b.kv_cap[s], b.Hkv, b.pool_elems)) { *st |= kShBadSequence; return r; }
-    if ((int64_t)start - P + q > b.kv_cap[s]) { *st |= kShPastSlab; return r; }
-    r.q = q;
-    r.P = P;
-    r.own0 = start - P;
-    r.p = p;
-    return r;
-  };
+  }
+  if (tid < b.n_prefix) {  // (at most one a thread)
+    const int len = b.prefix_len[tid], c = b.prefix_cap[tid];
+    const int64_t pb = b.prefix_base[tid];
+    px.len[tid] = len >= 0 && len <= c && sh_slab_ok(pb, c, b.Hkv, b.pool_elems) ? len : -1;
+    px.cap[tid] = c;
+    px.base[tid] = pb;
+    px.count[tid] = 0;
+    px.lo[tid] = INT32_MAX;
+  }
+  if (tid == 0) status_s = 0;
+  int sum[1] = {0}, total[1];
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) sum[0] += min(max(q[i], 0), b.T + 1);  // (what is past T is refused: no sum passes 2^31)
+  sh_excl_scan<1>(sum, total, reinterpret_cast<int (&)[1][kShPlanThreads / 64]>(red));
+  const int n_tokens = min(total[0], b.T);
+  if (total[0] > b.T) status |= kShPastTokens;
+
   // the tokens of a sequence that see its prefix: the first of them, those below P + window - 1
-  auto listed = [&](const Seq& r) __attribute__((always_inline)) {
-    if (r.p < 0 || r.P == 0) return 0;
-    return b.window > 0 ? (int)min((int64_t)r.q, max((int64_t)0, (int64_t)b.window - 1 - r.own0)) : r.q;
+  auto listed = [&](int n, int own0, int p) __attribute__((always_inline)) {
+    if (p < 0 || px.len[p] == 0) return 0;
+    return b.window > 0 ? (int)min((int64_t)n, max((int64_t)0, (int64_t)b.window - 1 - own0)) : n;
   };
   // the first chunk and the number of chunks of its own keys
-  auto own_chunks = [&](const Seq& r, int* c0) __attribute__((always_inline)) {
-    *c0 = b.window > 0 ? max(0, r.own0 - b.window + 1) / kShOwnChunk : 0;
-    return (r.own0 + r.q - 1) / kShOwnChunk + 1 - *c0;
+  auto own_chunks = [&](int n, int own0, int* c0) __attribute__((always_inline)) {
+    *c0 = b.window > 0 ? max(0, own0 - b.window + 1) / kShOwnChunk : 0;
+    return (own0 + n - 1) / kShOwnChunk + 1 - *c0;
   };
-  auto groups_of = [](int q) { return (q + kShWaveTokens - 1) / kShWaveTokens; };
+  auto groups_of = [](int n) { return (n + kShWaveTokens - 1) / kShWaveTokens; };
 
-  // groups of tokens; wave entries and records if the sequences' keys are split by chunks
-  int64_t my_groups = 0, my_split = 0, my_recs = 0;
-#pragma unroll 1
-  for (int s = s0; s < s1; ++s) {
-    cu_s[s] = (int)min(run, (int64_t)INT32_MAX);
-    const Seq r = seq_of(s, run, &status);
-    if (r.q > 0) {
-      const int n = listed(r);
-      if (n > 0) {
-        place_s[s] = atomicAdd(&pcnt_s[r.p], n);
-        atomicMin(&plo_s[r.p], b.window > 0 ? max(0, r.P + r.own0 - b.window + 1) : 0);
-      }
-      int c0;
-      const int nch = own_chunks(r, &c0);
-      my_groups += groups_of(r.q);
-      my_split += (int64_t)groups_of(r.q) * nch;
-      my_recs += (int64_t)r.q * nch;
+  int own[kPer];
+  int seqs[4] = {0, 0, 0, 0};  // groups of tokens, wave entries and records of split sequences, whether any is too long to be split
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    own[i] = -1;
+    const int s = s0 + i;
+    if (i >= per || s >= b.S) continue;
+    const int first = sum[0];
+    sum[0] += min(max(q[i], 0), b.T + 1);
+    int st = 0, o = -1;
+    if (q[i] < 0 || start[i] < 0) {
+      st = kShBadSequence;
+    } else if (q[i] > 0 && (int64_t)first + q[i] <= b.T) {
+      const int p = prefix[i];
+      const int P = p < 0 ? 0 : p < b.n_prefix ? px.len[p] : -1;
+      if (P < 0) st = kShBadPrefix;
+      else if (start[i] < P) st = kShBeforePrefix;
+      else if (!sh_slab_ok(base[i], cap[i], b.Hkv, b.pool_elems)) st = kShBadSequence;
+      else if ((int64_t)start[i] - P + q[i] > cap[i]) st = kShPastSlab;
+      else o = start[i] - P;
     }
-    run += max(b.q_lens[s], 0);
-  }
-  if (s1 == b.S && s0 < s1) cu_s[b.S] = (int)min(run, (int64_t)INT32_MAX);
-  int64_t n_groups, split_entries, split_recs;
-  sh_excl_scan(my_groups, red, &n_groups);
-  sh_excl_scan(my_split, red, &split_entries);
-  sh_excl_scan(my_recs, red, &split_recs);  // (its barriers also end the counting)
-
-  // the prefixes: tiles, entries, records
-  const int pper = (b.n_prefix + kShPlanThreads - 1) / kShPlanThreads;
-  const int p0 = min(b.n_prefix, tid * pper), p1 = min(b.n_prefix, p0 + pper);
-  auto chunks_of = [&](int p, int* c0) __attribute__((always_inline)) {
-    const int P = b.prefix_len[p], C = sh_prefix_chunk(P);
-    *c0 = plo_s[p] / C;
-    return (P - 1) / C + 1 - *c0;
-  };
-  int64_t my_list = 0, my_tiles = 0, my_parts = 0, my_prec = 0, my_few = 0, my_few_parts = 0;
-#pragma unroll 1
-  for (int p = p0; p < p1; ++p) {
-    const int n = pcnt_s[p];
-    if (!n) continue;
-    int c0;
-    const int nch = chunks_of(p, &c0);
-    const bool few = n <= kShWaveTokens;
-    const int tiles = few ? 1 : (n + kShRowTokens - 1) / kShRowTokens;
-    my_list += n;
-    (few ? my_few : my_tiles) += tiles;
-    (few ? my_few_parts : my_parts) += (int64_t)tiles * nch;
-    my_prec += (int64_t)n * nch;
-  }
-  int64_t n_list, n_tiles, n_parts, n_prec, n_few, n_few_parts;
-  const int64_t list0 = sh_excl_scan(my_list, red, &n_list);
-  sh_excl_scan(my_tiles, red, &n_tiles);
-  sh_excl_scan(my_parts, red, &n_parts);
-  sh_excl_scan(my_prec, red, &n_prec);
-  sh_excl_scan(my_few, red, &n_few);
-  sh_excl_scan(my_few_parts, red, &n_few_parts);
-  // Few tiles leave the chip idle: a chunk an item then, as far as the lists and the records hold them.
-  const bool psplit = n_tiles * b.Hkv < kShGrid && n_parts <= L.max_entries && n_prec + b.T <= L.max_recs &&
-                      n_few_parts + n_groups <= L.max_waves;
-  const int64_t precs = psplit ? n_prec : n_list;
-  const int64_t few_waves = psplit ? n_few_parts : n_few;
-  const bool osplit = split_entries * b.Hkv < 8 * kShGrid && few_waves + split_entries <= L.max_waves &&
-                      precs + split_recs <= L.max_recs;
-  {
-    int64_t e = 0, r = 0, f = 0, tot;
-#pragma unroll 1
-    for (int p = p0; p < p1; ++p) {
-      const int n = pcnt_s[p];
-      if (!n) continue;
-      int c0;
-      const int nch = psplit ? chunks_of(p, &c0) : 1;
-      if (n <= kShWaveTokens) f += nch;
-      else e += (int64_t)((n + kShRowTokens - 1) / kShRowTokens) * nch;
-      r += (int64_t)n * nch;
+    status |= st;
+    own[i] = o;
+    sq.cu[s] = min(first, b.T);
+    if (s == b.S - 1) sq.cu[b.S] = n_tokens;
+    sq.own0[s] = o;
+    sq.prefix[s] = prefix[i] < 0 ? -1 : prefix[i];
+    if (o < 0) continue;
+    const int n = listed(q[i], o, prefix[i]);
+    if (n > 0) {
+      sq.place[s] = atomicAdd(&px.count[prefix[i]], n);
+      atomicMin(&px.lo[prefix[i]], b.window > 0 ? max(0, start[i] - b.window + 1) : 0);
     }
-    int64_t e0 = sh_excl_scan(e, red, &tot), r0 = sh_excl_scan(r, red, &tot), f0 = sh_excl_scan(f, red, &tot), l0 = list0;
-#pragma unroll 1
-    for (int p = p0; p < p1; ++p) {
-      const int n = pcnt_s[p];
-      if (!n) continue;
-      int c0;
-      const int nch = psplit ? chunks_of(p, &c0) : 1;
-      const bool few = n <= kShWaveTokens;
-      plist_s[p] = (int)l0;
-      prec_s[p] = (int)r0;
-      pent_s[p] = (int)(few ? f0 : e0);
-      l0 += n;
-      r0 += (int64_t)n * nch;
-      if (few) f0 += nch;
-      else e0 += (int64_t)((n + kShRowTokens - 1) / kShRowTokens) * nch;
-    }
-  }
-  // the sequences' wave entries and records
-  int64_t my_w = 0, my_r = 0, tot_w, tot_r;
-#pragma unroll 1
-  for (int s = s0; s < s1; ++s) {
-    int32_t ignore = 0;
-    const Seq r = seq_of(s, cu_s[s], &ignore);
-    if (!r.q) continue;
     int c0;
-    const int nch = osplit ? own_chunks(r, &c0) : 1;
-    my_w += (int64_t)groups_of(r.q) * nch;
-    my_r += (int64_t)r.q * nch;
-  }
-  int64_t w0 = few_waves + sh_excl_scan(my_w, red, &tot_w), r0 = precs + sh_excl_scan(my_r, red, &tot_r);
-  __shared__ int32_t rbase_s[kShMaxSeqs];
-#pragma unroll 1
-  for (int s = s0; s < s1; ++s) {
-    int32_t ignore = 0;
-    const Seq r = seq_of(s, cu_s[s], &ignore);
-    wbase_s[s] = (int)w0;
-    rbase_s[s] = r.q ? (int)r0 : -1;
-    if (!r.q) continue;
-    int c0;
-    const int nch = osplit ? own_chunks(r, &c0) : 1;
-    w0 += (int64_t)groups_of(r.q) * nch;
-    r0 += (int64_t)r.q * nch;
+    const int nch = own_chunks(q[i], o, &c0);
+    seqs[0] += groups_of(q[i]);
+    seqs[1] += groups_of(q[i]) * min(nch, kShMaxOwnChunks);
+    seqs[2] += q[i] * min(nch, kShMaxOwnChunks);
+    seqs[3] += nch > kShMaxOwnChunks;
   }
   if (status) atomicOr(&status_s, status);
-  __syncthreads();
-  const int Tw = min(cu_s[b.S], b.T);
+  int n_seqs[4];
+  sh_excl_scan<4>(seqs, n_seqs, reinterpret_cast<int (&)[4][kShPlanThreads / 64]>(red));  // (its barriers also end the counting)
+
+  // the prefixes: a thread has one
+  const int np = tid < b.n_prefix ? px.count[tid] : 0;
+  const bool few = np <= kShWaveTokens;
+  int P = 0, C = 64, chunk0 = 0, chunks = 0, tiles = 0;
+  if (np > 0) {
+    P = px.len[tid];
+    C = sh_prefix_chunk(P);
+    chunk0 = px.lo[tid] / C;
+    chunks = (P - 1) / C + 1 - chunk0;
+    tiles = few ? 1 : (np + kShRowTokens - 1) / kShRowTokens;
+  }
+  // listed tokens; tiles whole and by chunks, of workgroups, then of waves; records by chunks
+  int ps[6] = {np, few ? 0 : tiles, few ? 0 : tiles * chunks, few ? tiles : 0, few ? tiles * chunks : 0, np * chunks}, n_ps[6];
+  sh_excl_scan<6>(ps, n_ps, red);
+  // Few tiles leave the chip idle: a chunk an item then, as far as the lists and the records hold them.
+  const bool psplit = n_ps[1] * b.Hkv < kShGrid && n_ps[2] <= L.max_entries && n_ps[5] + b.T <= L.max_recs &&
+                      n_ps[4] + n_seqs[0] <= L.max_waves;
+  const int precs = psplit ? n_ps[5] : n_ps[0], few_waves = psplit ? n_ps[4] : n_ps[3];
+  const bool osplit = n_seqs[3] == 0 && (int64_t)n_seqs[1] * b.Hkv < 8 * kShGrid && few_waves + n_seqs[1] <= L.max_waves &&
+                      precs + n_seqs[2] <= L.max_recs;
+  if (np > 0) {
+    px.list0[tid] = ps[0];
+    px.entry0[tid] = few ? (psplit ? ps[4] : ps[3]) : (psplit ? ps[2] : ps[1]);
+    px.rec0[tid] = psplit ? ps[5] : ps[0];
+  }
+  // the sequences' entries and records: as scanned if they are split, else by groups and tokens
+  int at[2] = {seqs[1], seqs[2]};
+  if (!osplit) {
+    int all[2];
+    at[0] = at[1] = 0;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i)
+      if (own[i] >= 0) {
+        at[0] += groups_of(q[i]);
+        at[1] += q[i];
+      }
+    sh_excl_scan<2>(at, all, reinterpret_cast<int (&)[2][kShPlanThreads / 64]>(red));
+  }
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    if (own[i] < 0) continue;
+    int c0;
+    const int nch = osplit ? own_chunks(q[i], own[i], &c0) : 1;
+    sq.wave0[s0 + i] = few_waves + at[0];
+    sq.rec0[s0 + i] = precs + at[1];
+    at[0] += groups_of(q[i]) * nch;
+    at[1] += q[i] * nch;
+  }
   if (tid == 0) {
-    hdr->n_entries = (int)(psplit ? n_parts : n_tiles);
-    hdr->n_waves = (int)(few_waves + tot_w);
-    hdr->n_tokens = Tw;
-    hdr->status = status_s;
+    hdr->n_entries = psplit ? n_ps[2] : n_ps[1];
+    hdr->n_waves = few_waves + (osplit ? n_seqs[1] : n_seqs[0]);
+    hdr->n_tokens = n_tokens;
     hdr->window = b.window;
   }
+  __syncthreads();
+  if (tid == 0) hdr->status = status_s;
   // a prefix's entries, chunk by chunk: the tiles that read the same keys are neighbours
   for (int p = tid >> 6; p < b.n_prefix; p += kShPlanThreads / 64) {
-    const int n = pcnt_s[p];
+    const int n = px.count[p];
     if (!n) continue;
-    int c0;
-    const int P = b.prefix_len[p], C = sh_prefix_chunk(P), nch_all = chunks_of(p, &c0), nch = psplit ? nch_all : 1;
-    const bool few = n <= kShWaveTokens;
-    const int tiles = few ? 1 : (n + kShRowTokens - 1) / kShRowTokens;
-    ShEntry* out = (few ? waves : entries) + pent_s[p];
-    for (int i = tid & 63; i < tiles * nch; i += 64) {
-      const int c = i / tiles, t = i % tiles;
+    const int len = px.len[p], c = sh_prefix_chunk(len), lo = px.lo[p], c0 = lo / c;
+    const int nch = psplit ? (len - 1) / c + 1 - c0 : 1;
+    const bool w = n <= kShWaveTokens;
+    const int nt = w ? 1 : (n + kShRowTokens - 1) / kShRowTokens;
+    ShEntry* out = (w ? waves : entries) + px.entry0[p];
+    for (int i = tid & 63; i < nt * nch; i += 64) {
+      const int k = i / nt, t = i % nt;
       ShEntry e;
-      e.base = b.prefix_base[p];
-      e.cap = b.prefix_cap[p];
-      e.first = plist_s[p] + t * kShRowTokens;
+      e.base = px.base[p];
+      e.cap = px.cap[p];
+      e.first = px.list0[p] + t * kShRowTokens;
       e.ntok = min(kShRowTokens, n - t * kShRowTokens);
       e.pos0 = 0;
       e.list = 1;
-      e.key_lo = psplit ? max(plo_s[p], (c0 + c) * C) : plo_s[p];
-      e.key_hi = psplit ? min(P, (c0 + c + 1) * C) : P;
-      e.chunk = C;
-      e.rec = prec_s[p] + c * n + t * kShRowTokens;
+      e.key_lo = psplit ? max(lo, (c0 + k) * c) : lo;
+      e.key_hi = psplit ? min(len, (c0 + k + 1) * c) : len;
+      e.chunk = c;
+      e.rec = px.rec0[p] + k * n + t * kShRowTokens;
       e.pad = 0;
       out[i] = e;
     }
   }
-  for (int t = tid; t < Tw; t += kShPlanThreads) {
+  for (int t = tid; t < n_tokens; t += kShPlanThreads) {
     int lo = 0, hi = b.S - 1;  // last sequence with cu <= t
     while (lo < hi) {
       const int mid = (lo + hi + 1) >> 1;
-      if (cu_s[mid] <= t) lo = mid; else hi = mid - 1;
+      if (sq.cu[mid] <= t) lo = mid; else hi = mid - 1;
     }
     ShToken k = {0, 0, 0, 0, 0, 0};
-    int32_t ignore = 0;
-    const Seq r = seq_of(lo, cu_s[lo], &ignore);
-    const int i = t - cu_s[lo];
-    if (r.q) {
+    const int own0 = sq.own0[lo], i = t - sq.cu[lo];
+    if (own0 >= 0) {
+      const int n = sq.cu[lo + 1] - sq.cu[lo], p = sq.prefix[lo];
       int c0;
-      const int nch_all = own_chunks(r, &c0), nch = osplit ? nch_all : 1;
-      k.o_rec = rbase_s[lo] + i;
+      const int all = own_chunks(n, own0, &c0), nch = osplit ? all : 1;
+      k.o_rec = sq.rec0[lo] + i;
       k.o_n = nch;
-      k.o_stride = r.q;
-      if (i < listed(r)) {
-        int pc0;
-        const int n = pcnt_s[r.p], at = place_s[lo] + i;
-        k.p_rec = prec_s[r.p] + at;
-        k.p_n = psplit ? chunks_of(r.p, &pc0) : 1;
-        k.p_stride = n;
-        list[plist_s[r.p] + at] = make_int2(t, r.P + r.own0 + i);
+      k.o_stride = n;
+      if (i < listed(n, own0, p)) {
+        const int len = px.len[p], c = sh_prefix_chunk(len), where = sq.place[lo] + i;
+        k.p_rec = px.rec0[p] + where;
+        k.p_n = psplit ? (len - 1) / c + 1 - px.lo[p] / c : 1;
+        k.p_stride = px.count[p];
+        list[px.list0[p] + where] = make_int2(t, len + own0 + i);
       }
       if (i % kShWaveTokens == 0) {  // its group's entries
+        const int64_t kv = b.kv_base[lo];
+        const int kc = b.kv_cap[lo];
         for (int c = 0; c < nch; ++c) {
           ShEntry e;
-          e.base = b.kv_base[lo];
-          e.cap = b.kv_cap[lo];
+          e.base = kv;
+          e.cap = kc;
           e.first = t;
-          e.ntok = min(kShWaveTokens, r.q - i);
-          e.pos0 = r.own0 + i;
+          e.ntok = min(kShWaveTokens, n - i);
+          e.pos0 = own0 + i;
           e.list = 0;
           const int klo = b.window > 0 ? max(0, e.pos0 - b.window + 1) : 0, khi = e.pos0 + e.ntok;
           e.key_lo = osplit ? max(klo, (c0 + c) * kShOwnChunk) : klo;
           e.key_hi = osplit ? min(khi, (c0 + c + 1) * kShOwnChunk) : khi;
           e.chunk = kShOwnChunk;
-          e.rec = rbase_s[lo] + c * r.q + i;
+          e.rec = sq.rec0[lo] + c * n + i;
           e.pad = 0;
-          waves[wbase_s[lo] + (i / kShWaveTokens) * nch + c] = e;
+          waves[sq.wave0[lo] + (i / kShWaveTokens) * nch + c] = e;
         }
       }
     }

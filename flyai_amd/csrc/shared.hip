@@ -8,9 +8,9 @@
 // Every key range is cut into chunks whose borders go by the slab alone (from its position 0).  A chunk's
 // (m, l, O[64]) starts afresh, and a range's total folds its chunks in ascending order (fold below):
 //   M' = max(M, m);  O' = O_c 2^(m - M') + O 2^(M - M');  L likewise.
-// A work item takes either one chunk or all of them: the items' records are folded by attn_shared_merge_kernel, or the item folds in
-// its registers, by the same operations in the same order.  So the work is split where there are few rows
-// and not where there are many, and a row's bits depend on neither, nor on the rest of the batch.
+// A work item takes a run of a range's chunks and leaves a record of each, which attn_shared_merge_kernel folds; or it takes the whole
+// range and folds in its registers, by the same operations in the same order.  So the work is split where there are few
+// rows and not where there are many, and a row's bits depend on neither, nor on the rest of the batch.
 //
 // The work lists are made on the GPU (attn_shared_plan_kernel), once for a step's layers: the host needs
 // no lengths, only bounds, and the grids are sized by those.
@@ -19,18 +19,22 @@
 namespace flyai {
 
 constexpr int kShRowTokens = 16;      // tokens of a prefix item's tile (4 waves x 2 tiles of 16 rows x 2 tokens)
-constexpr int kShWaveTokens = 4;      // tokens of a wave item
+constexpr int kShWaveTokens = 2;      // tokens of a wave item
+constexpr int kShWaveSeq = 4;         // the most new tokens of a sequence whose own keys go to waves; more go to tiles
 constexpr int kShMaxSeqs = 4096, kShMaxPrefixes = 1024;
-constexpr int kShChunks = 16;         // a prefix's chunks: at most this many
-constexpr int kShMinChunk = 128;
-constexpr int kShOwnChunk = 512;
+constexpr int kShChunks = 24;         // a prefix's chunks: at most this many
+constexpr int kShMinChunk = 384, kShChunkStep = 192;
+constexpr int kShOwnChunk = 576;
 constexpr int kShSpareEntries = 1024;  // list entries beyond one for each tile, for prefixes split by chunks
 constexpr int kShSpareWaves = 2048;    // ... and beyond one for each group of a sequence's tokens
 constexpr int kShSpareRecs = 8192;     // records beyond two for each token
 constexpr int kShGrid = 512;           // workgroups on the chip at once: two a CU
+// workgroups of a kv head: head g's are those with blockIdx % Hkv == g, with 8 heads an XCD each, so that its L2 holds one head's keys
+__host__ __device__ constexpr int sh_per_head(int Hkv) { return kShGrid / Hkv > 0 ? kShGrid / Hkv : 1; }
 
-// What an item reads and where it writes.  Its rows are `ntok` tokens: from `first` on in the list of a prefix's tokens (list),
-// or token first + i at the slab's position pos0 + i.
+// A unit of work: `ntok` rows' tokens -- from `first` on in the list of a prefix's tokens (list), or token first + i at the slab's
+// position pos0 + i -- and their keys from key_lo on.  stride 0: all the keys up to `end`, folded; otherwise those of key_lo's chunk, and
+// the next `left` units are the same rows' next chunks.
 struct ShEntry {
   int64_t base;   // of the slab
   int32_t cap;
@@ -38,9 +42,11 @@ struct ShEntry {
   int32_t ntok;
   int32_t pos0;
   int32_t list;
-  int32_t key_lo, key_hi;  // slab positions
-  int32_t chunk;           // positions of a chunk
-  int32_t rec;             // record of the first token; token i's is rec + i
+  int32_t key_lo, end;  // slab positions
+  int32_t chunk;        // positions of a chunk
+  int32_t rec;          // record of the first token; token i's is rec + i, the next chunk's `stride` behind
+  int32_t stride;
+  int32_t left;
   int32_t pad;
 };
 
@@ -49,9 +55,10 @@ struct ShToken {  // where a token's records lie: n of them, stride apart
   int32_t o_rec, o_n, o_stride;
 };
 
+// The units of workgroups: whole prefix tiles, then chunks of prefix tiles, then the sequences' own tiles; and those of waves.
 struct ShHeader {
-  int32_t n_entries, n_waves, n_tokens, status;
-  int32_t window, pad[11];
+  int32_t n_whole, n_split, n_own, status;
+  int32_t n_waves, n_tokens, window, pad[9];
 };
 
 // Byte layout of a plan, and how much each list holds at most.
@@ -63,8 +70,9 @@ struct ShLayout {
 __host__ __device__ inline ShLayout sh_layout(int T, int S, int n_prefix) {
   ShLayout l;
   l.T = T;
-  l.max_entries = T / kShRowTokens + (n_prefix < T ? n_prefix : T) + kShSpareEntries;
-  // a sequence's groups, and the prefixes whose few tokens go to waves
+  // the prefixes' tiles, those of the sequences with more than kShWaveSeq tokens
+  l.max_entries = 2 * (T / kShRowTokens) + (n_prefix < T ? n_prefix : T) + T / (kShWaveSeq + 1) + kShSpareEntries;
+  // the other sequences' groups, and the prefixes whose few tokens go to waves
   l.max_waves = T / kShWaveTokens + (S < T ? S : T) + (n_prefix < T ? n_prefix : T) + kShSpareWaves;
   l.max_recs = 2 * T + kShSpareRecs;
   size_t o = sizeof(ShHeader);
@@ -116,7 +124,7 @@ __device__ __forceinline__ void sh_excl_scan(int (&v)[N], int (&total)[N], int (
 }
 
 __device__ __forceinline__ int sh_prefix_chunk(int P) {
-  const int c = ((P + kShChunks - 1) / kShChunks + 63) & ~63;
+  const int c = ((P + kShChunks - 1) / kShChunks + kShChunkStep - 1) / kShChunkStep * kShChunkStep;
   return c > kShMinChunk ? c : kShMinChunk;
 }
 
@@ -143,7 +151,7 @@ struct ShSeqs {
   int32_t own0[kShMaxSeqs];    // the slab position of its first token; -1: the sequence has no tokens, or is refused
   int32_t prefix[kShMaxSeqs];  // -1: none
   int32_t place[kShMaxSeqs];   // its first listed token's place among its prefix's
-  int32_t wave0[kShMaxSeqs], rec0[kShMaxSeqs];  // its first wave entry and record
+  int32_t entry0[kShMaxSeqs], rec0[kShMaxSeqs];  // its first entry (of its kind) and record
 };
 struct ShPrefixes {
   int32_t len[kShMaxPrefixes];  // -1: refused
@@ -151,7 +159,9 @@ struct ShPrefixes {
   int64_t base[kShMaxPrefixes];
   int32_t count[kShMaxPrefixes];  // listed tokens
   int32_t lo[kShMaxPrefixes];     // the first position that any of them sees
-  int32_t list0[kShMaxPrefixes], entry0[kShMaxPrefixes], rec0[kShMaxPrefixes];
+  int32_t list0[kShMaxPrefixes];
+  int32_t tile0[kShMaxPrefixes];  // its first tile, of all prefixes' (wave entry, for a prefix of few tokens)
+  int32_t unit0[kShMaxPrefixes], rec0[kShMaxPrefixes];  // of its tiles that are split: the first unit and record
 };
 constexpr int kShMaxOwnChunks = 4096;  // of a sequence, for the counts to stay in 32 bits: past it no sequence is split
 
@@ -219,10 +229,12 @@ __global__ __launch_bounds__(kShPlanThreads) void attn_shared_plan_kernel(ShBatc
     *c0 = b.window > 0 ? max(0, own0 - b.window + 1) / kShOwnChunk : 0;
     return (own0 + n - 1) / kShOwnChunk + 1 - *c0;
   };
-  auto groups_of = [](int n) { return (n + kShWaveTokens - 1) / kShWaveTokens; };
+  auto groups_of = [](int n) { return n <= kShWaveSeq ? (n + kShWaveTokens - 1) / kShWaveTokens : (n + kShRowTokens - 1) / kShRowTokens; };
 
   int own[kPer];
-  int seqs[4] = {0, 0, 0, 0};  // groups of tokens, wave entries and records of split sequences, whether any is too long to be split
+  // the groups of tokens that go to waves and to tiles, their entries and the records if they are split by chunks; whether a sequence
+  // is too long for that
+  int seqs[6] = {0, 0, 0, 0, 0, 0};
 #pragma unroll
   for (int i = 0; i < kPer; ++i) {
     own[i] = -1;
@@ -256,14 +268,15 @@ __global__ __launch_bounds__(kShPlanThreads) void attn_shared_plan_kernel(ShBatc
     }
     int c0;
     const int nch = own_chunks(q[i], o, &c0);
-    seqs[0] += groups_of(q[i]);
-    seqs[1] += groups_of(q[i]) * min(nch, kShMaxOwnChunks);
-    seqs[2] += q[i] * min(nch, kShMaxOwnChunks);
-    seqs[3] += nch > kShMaxOwnChunks;
+    const int kind = q[i] > kShWaveSeq;
+    seqs[kind] += groups_of(q[i]);
+    seqs[2 + kind] += groups_of(q[i]) * min(nch, kShMaxOwnChunks);
+    seqs[4] += q[i] * min(nch, kShMaxOwnChunks);
+    seqs[5] += nch > kShMaxOwnChunks;
   }
   if (status) atomicOr(&status_s, status);
-  int n_seqs[4];
-  sh_excl_scan<4>(seqs, n_seqs, reinterpret_cast<int (&)[4][kShPlanThreads / 64]>(red));  // (its barriers also end the counting)
+  int n_seqs[6];
+  sh_excl_scan<6>(seqs, n_seqs, red);  // (its barriers also end the counting)
 
   // the prefixes: a thread has one
   const int np = tid < b.n_prefix ? px.count[tid] : 0;
@@ -276,62 +289,78 @@ __global__ __launch_bounds__(kShPlanThreads) void attn_shared_plan_kernel(ShBatc
     chunks = (P - 1) / C + 1 - chunk0;
     tiles = few ? 1 : (np + kShRowTokens - 1) / kShRowTokens;
   }
-  // listed tokens; tiles whole and by chunks, of workgroups, then of waves; records by chunks
-  int ps[6] = {np, few ? 0 : tiles, few ? 0 : tiles * chunks, few ? tiles : 0, few ? tiles * chunks : 0, np * chunks}, n_ps[6];
-  sh_excl_scan<6>(ps, n_ps, red);
-  // Few tiles leave the chip idle: a chunk an item then, as far as the lists and the records hold them.
-  const bool psplit = n_ps[1] * b.Hkv < kShGrid && n_ps[2] <= L.max_entries && n_ps[5] + b.T <= L.max_recs &&
-                      n_ps[4] + n_seqs[0] <= L.max_waves;
-  const int precs = psplit ? n_ps[5] : n_ps[0], few_waves = psplit ? n_ps[4] : n_ps[3];
-  const bool osplit = n_seqs[3] == 0 && (int64_t)n_seqs[1] * b.Hkv < 8 * kShGrid && few_waves + n_seqs[1] <= L.max_waves &&
-                      precs + n_seqs[2] <= L.max_recs;
+  // listed tokens; tiles of workgroups; entries of waves whole and by chunks, their records by chunks
+  int ps[5] = {np, few ? 0 : tiles, few ? tiles : 0, few ? tiles * chunks : 0, few ? np * chunks : 0}, n_ps[5];
+  sh_excl_scan<5>(ps, n_ps, reinterpret_cast<int (&)[5][kShPlanThreads / 64]>(red));
+  // As many whole tiles as give every workgroup the same number; the rest by chunks, if the lists and the records hold them.
+  const int per_head = sh_per_head(b.Hkv);
+  int whole = n_ps[1] / per_head * per_head;
+  auto split_of = [&](int w) __attribute__((always_inline)) { return few ? 0 : max(0, ps[1] + tiles - max(ps[1], w)); };
+  int split = split_of(whole), split_tokens = np > 0 ? min(np, np - (tiles - split) * kShRowTokens) : 0;
+  if (!split) split_tokens = 0;
+  int us[2] = {split * chunks, split_tokens * chunks}, n_us[2];
+  sh_excl_scan<2>(us, n_us, reinterpret_cast<int (&)[2][kShPlanThreads / 64]>(red));
+  const bool fsplit = n_ps[3] + n_seqs[0] <= L.max_waves && n_ps[0] + n_ps[4] + b.T <= L.max_recs;
+  const int few_recs = fsplit ? n_ps[4] : 0, few_waves = fsplit ? n_ps[3] : n_ps[2];
+  if (whole + n_us[0] + n_seqs[1] > L.max_entries || n_ps[0] + few_recs + n_us[1] + b.T > L.max_recs) {  // (uniform)
+    whole = n_ps[1];
+    split = split_tokens = us[0] = us[1] = n_us[0] = n_us[1] = 0;
+  }
+  // records: one for each listed token, then those of the chunks, then the sequences' own
+  const int ptiles = whole + n_us[0], precs = n_ps[0] + few_recs + n_us[1];
+  const bool osplit = n_seqs[5] == 0 && ((int64_t)n_seqs[2] + 4 * n_seqs[3]) * b.Hkv < 8 * kShGrid &&
+                      few_waves + n_seqs[2] <= L.max_waves && ptiles + n_seqs[3] <= L.max_entries && precs + n_seqs[4] <= L.max_recs;
   if (np > 0) {
     px.list0[tid] = ps[0];
-    px.entry0[tid] = few ? (psplit ? ps[4] : ps[3]) : (psplit ? ps[2] : ps[1]);
-    px.rec0[tid] = psplit ? ps[5] : ps[0];
+    px.tile0[tid] = few ? (fsplit ? ps[3] : ps[2]) : ps[1];
+    px.unit0[tid] = us[0];
+    px.rec0[tid] = n_ps[0] + (few ? ps[4] : few_recs + us[1]);
   }
   // the sequences' entries and records: as scanned if they are split, else by groups and tokens
-  int at[2] = {seqs[1], seqs[2]};
+  int at[3] = {seqs[2], seqs[3], seqs[4]};
   if (!osplit) {
-    int all[2];
-    at[0] = at[1] = 0;
+    int all[3];
+    at[0] = seqs[0];
+    at[1] = seqs[1];
+    at[2] = 0;
 #pragma unroll
     for (int i = 0; i < kPer; ++i)
-      if (own[i] >= 0) {
-        at[0] += groups_of(q[i]);
-        at[1] += q[i];
-      }
-    sh_excl_scan<2>(at, all, reinterpret_cast<int (&)[2][kShPlanThreads / 64]>(red));
+      if (own[i] >= 0) at[2] += q[i];
+    int tokens_at[1] = {at[2]};
+    sh_excl_scan<1>(tokens_at, reinterpret_cast<int (&)[1]>(all), reinterpret_cast<int (&)[1][kShPlanThreads / 64]>(red));
+    at[2] = tokens_at[0];
   }
 #pragma unroll
   for (int i = 0; i < kPer; ++i) {
     if (own[i] < 0) continue;
     int c0;
-    const int nch = osplit ? own_chunks(q[i], own[i], &c0) : 1;
-    sq.wave0[s0 + i] = few_waves + at[0];
-    sq.rec0[s0 + i] = precs + at[1];
-    at[0] += groups_of(q[i]) * nch;
-    at[1] += q[i] * nch;
+    const int nch = osplit ? own_chunks(q[i], own[i], &c0) : 1, kind = q[i] > kShWaveSeq;
+    sq.entry0[s0 + i] = kind ? ptiles + at[1] : few_waves + at[0];
+    sq.rec0[s0 + i] = precs + at[2];
+    (kind ? at[1] : at[0]) += groups_of(q[i]) * nch;
+    at[2] += q[i] * nch;
   }
   if (tid == 0) {
-    hdr->n_entries = psplit ? n_ps[2] : n_ps[1];
-    hdr->n_waves = few_waves + (osplit ? n_seqs[1] : n_seqs[0]);
+    hdr->n_whole = whole;
+    hdr->n_split = n_us[0];
+    hdr->n_own = osplit ? n_seqs[3] : n_seqs[1];
+    hdr->n_waves = few_waves + (osplit ? n_seqs[2] : n_seqs[0]);
     hdr->n_tokens = n_tokens;
     hdr->window = b.window;
   }
   __syncthreads();
   if (tid == 0) hdr->status = status_s;
-  // a prefix's entries, chunk by chunk: the tiles that read the same keys are neighbours
+  // a prefix's units: tiles, or a tile's chunks behind one another
+  auto first_split = [&](int p) __attribute__((always_inline)) { return max(0, whole - px.tile0[p]); };  // its first tile that is split
   for (int p = tid >> 6; p < b.n_prefix; p += kShPlanThreads / 64) {
     const int n = px.count[p];
     if (!n) continue;
-    const int len = px.len[p], c = sh_prefix_chunk(len), lo = px.lo[p], c0 = lo / c;
-    const int nch = psplit ? (len - 1) / c + 1 - c0 : 1;
+    const int len = px.len[p], c = sh_prefix_chunk(len), lo = px.lo[p], c0 = lo / c, nch = (len - 1) / c + 1 - c0;
     const bool w = n <= kShWaveTokens;
-    const int nt = w ? 1 : (n + kShRowTokens - 1) / kShRowTokens;
-    ShEntry* out = (w ? waves : entries) + px.entry0[p];
-    for (int i = tid & 63; i < nt * nch; i += 64) {
-      const int k = i / nt, t = i % nt;
+    const int nt = w ? 1 : (n + kShRowTokens - 1) / kShRowTokens, ts = w ? (fsplit ? 0 : 1) : min(nt, first_split(p));
+    for (int i = tid & 63; i < ts + (nt - ts) * nch; i += 64) {
+      const bool one = i < ts;  // whole
+      const int t = one ? i : ts + (i - ts) / nch, k = one ? 0 : (i - ts) % nch;
       ShEntry e;
       e.base = px.base[p];
       e.cap = px.cap[p];
@@ -339,11 +368,14 @@ __global__ __launch_bounds__(kShPlanThreads) void attn_shared_plan_kernel(ShBatc
       e.ntok = min(kShRowTokens, n - t * kShRowTokens);
       e.pos0 = 0;
       e.list = 1;
-      e.key_lo = psplit ? max(lo, (c0 + k) * c) : lo;
-      e.key_hi = psplit ? min(len, (c0 + k + 1) * c) : len;
+      e.key_lo = max(lo, (c0 + k) * c);
+      e.end = len;
       e.chunk = c;
-      e.rec = px.rec0[p] + k * n + t * kShRowTokens;
+      e.stride = one ? 0 : n - ts * kShRowTokens;
+      e.rec = one ? e.first : px.rec0[p] + k * e.stride + (t - ts) * kShRowTokens;
+      e.left = one ? 0 : nch - 1 - k;
       e.pad = 0;
+      ShEntry* out = w ? waves + px.tile0[p] : one ? entries + px.tile0[p] : entries + whole + px.unit0[p] - ts;
       out[i] = e;
     }
   }
@@ -363,13 +395,20 @@ __global__ __launch_bounds__(kShPlanThreads) void attn_shared_plan_kernel(ShBatc
       k.o_n = nch;
       k.o_stride = n;
       if (i < listed(n, own0, p)) {
-        const int len = px.len[p], c = sh_prefix_chunk(len), where = sq.place[lo] + i;
-        k.p_rec = px.rec0[p] + where;
-        k.p_n = psplit ? (len - 1) / c + 1 - px.lo[p] / c : 1;
-        k.p_stride = px.count[p];
+        const int len = px.len[p], c = sh_prefix_chunk(len), where = sq.place[lo] + i, count = px.count[p];
+        const bool w = count <= kShWaveTokens;
+        const int ts = w ? (fsplit ? 0 : 1) : first_split(p);
         list[px.list0[p] + where] = make_int2(t, len + own0 + i);
+        k.p_n = 1;
+        k.p_rec = px.list0[p] + where;
+        if (where >= ts * kShRowTokens) {
+          k.p_n = (len - 1) / c + 1 - px.lo[p] / c;
+          k.p_stride = count - ts * kShRowTokens;
+          k.p_rec = px.rec0[p] + where - ts * kShRowTokens;
+        }
       }
-      if (i % kShWaveTokens == 0) {  // its group's entries
+      const int size = n <= kShWaveSeq ? kShWaveTokens : kShRowTokens;
+      if (i % size == 0) {  // its group's entries
         const int64_t kv = b.kv_base[lo];
         const int kc = b.kv_cap[lo];
         for (int c = 0; c < nch; ++c) {
@@ -377,16 +416,18 @@ __global__ __launch_bounds__(kShPlanThreads) void attn_shared_plan_kernel(ShBatc
           e.base = kv;
           e.cap = kc;
           e.first = t;
-          e.ntok = min(kShWaveTokens, n - i);
+          e.ntok = min(size, n - i);
           e.pos0 = own0 + i;
           e.list = 0;
-          const int klo = b.window > 0 ? max(0, e.pos0 - b.window + 1) : 0, khi = e.pos0 + e.ntok;
+          const int klo = b.window > 0 ? max(0, e.pos0 - b.window + 1) : 0;
           e.key_lo = osplit ? max(klo, (c0 + c) * kShOwnChunk) : klo;
-          e.key_hi = osplit ? min(khi, (c0 + c + 1) * kShOwnChunk) : khi;
+          e.end = osplit ? min(e.pos0 + e.ntok, (c0 + c + 1) * kShOwnChunk) : e.pos0 + e.ntok;  // (a chunk before the window is empty)
           e.chunk = kShOwnChunk;
           e.rec = sq.rec0[lo] + c * n + i;
+          e.stride = osplit ? n : 0;
+          e.left = 0;
           e.pad = 0;
-          waves[sq.wave0[lo] + (i / kShWaveTokens) * nch + c] = e;
+          (n <= kShWaveSeq ? waves : entries)[sq.entry0[lo] + (i / size) * nch + c] = e;
         }
       }
     }
@@ -403,10 +444,20 @@ struct ShRows {
   bf16x8_t qf[QT][2];
   int lo[QT], hi[QT];
   bool val[QT];
-  float m[QT], tm[QT];
-  f32x4_t O[QT][4], L[QT], tO[QT][4];
-  float tL[QT];  // (every element of L is the row's sum)
+  float m[QT], tm[QT], tL[QT];
+  f32x4_t O[QT][4], L[QT], tO[QT][4];  // (every element of L is the row's sum)
 };
+
+template <int QT>
+__device__ __forceinline__ void sh_nothing(ShRows<QT>& R) {
+#pragma unroll
+  for (int qt = 0; qt < QT; ++qt) {
+    R.tm[qt] = -1e30f;
+    R.tL[qt] = 0.f;
+#pragma unroll
+    for (int dt = 0; dt < 4; ++dt) R.tO[qt][dt] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+  }
+}
 
 template <int QT>
 __device__ __forceinline__ void sh_fresh(ShRows<QT>& R) {
@@ -465,11 +516,8 @@ __device__ __forceinline__ void sh_rows_init(ShRows<QT>& R, const ShEntry& e, in
     }
     R.qf[qt][0] = as_bf16x8(a);
     R.qf[qt][1] = as_bf16x8(b);
-    R.tm[qt] = -1e30f;
-    R.tL[qt] = 0.f;
-#pragma unroll
-    for (int dt = 0; dt < 4; ++dt) R.tO[qt][dt] = f32x4_t{0.f, 0.f, 0.f, 0.f};
   }
+  sh_nothing(R);
   sh_fresh(R);
 }
 
@@ -623,14 +671,20 @@ __device__ __forceinline__ float* sh_rec_ml(float* parts, int max_recs, int rec,
   return parts + (size_t)max_recs * Hkv * 512 + (((size_t)rec * Hkv + g) * 8 + h) * 2;
 }
 
+// the end of the keys of `run` units from e on
+__device__ __forceinline__ int sh_key_end(const ShEntry& e, int run) {
+  return e.stride ? (int)min((int64_t)e.end, ((int64_t)(e.key_lo / e.chunk) + run) * e.chunk) : e.end;
+}
+
+// The last chunk folded in, and the total to the item's records.
 template <int QT>
-__device__ __forceinline__ void sh_write(const ShRows<QT>& R, const ShEntry& e, int tok0, int kv_head, int Hkv, int max_recs,
-                                         float* __restrict__ parts) {
+__device__ __forceinline__ void sh_put(ShRows<QT>& R, int rec0, int tok0, int kv_head, int Hkv, int max_recs, float* __restrict__ parts) {
   const int lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
+  sh_fold_chunk(R);
 #pragma unroll
   for (int qt = 0; qt < QT; ++qt) {
     if (!R.val[qt]) continue;
-    const int rq = 16 * qt + n, rec = e.rec + tok0 + (rq >> 3);
+    const int rq = 16 * qt + n, rec = rec0 + tok0 + (rq >> 3);
     float* o = sh_rec_o(parts, rec, Hkv, kv_head, rq & 7) + 4 * g;
 #pragma unroll
     for (int dt = 0; dt < 4; ++dt) *reinterpret_cast<f32x4_t*>(o + 16 * dt) = R.tO[qt][dt];
@@ -638,12 +692,13 @@ __device__ __forceinline__ void sh_write(const ShRows<QT>& R, const ShEntry& e, 
   }
 }
 
-// An item of up to 4 tokens by one wave, K and V straight from the slab.
+// An item of up to 2 tokens by one wave, K and V straight from the slab.
 template <int QT>
 __device__ __forceinline__ void sh_wave_item(const ShEntry& e, int kv_head, const int2* __restrict__ list, const uint16_t* __restrict__ q,
                                              const uint16_t* __restrict__ k_pool, const uint16_t* __restrict__ v_pool, int Hq, int Hkv,
                                              int window, int max_recs, float* __restrict__ parts) {
   const int lane = threadIdx.x & 63;
+  const int key_hi = sh_key_end(e, 1);
   const int64_t base = e.base + (int64_t)kv_head * e.cap * 64;
   const uint16_t *K = k_pool + base, *V = v_pool + base;
   ShRows<QT> R;
@@ -651,12 +706,12 @@ __device__ __forceinline__ void sh_wave_item(const ShEntry& e, int kv_head, cons
   int int_lo, int_hi;
   sh_interior(R, &int_lo, &int_hi);
   int_lo = max(int_lo, e.key_lo);
-  int_hi = min(int_hi, e.key_hi - 1);
+  int_hi = min(int_hi, key_hi - 1);
   uint4 kc[4][2], vc[4][2];
   int kb = e.key_lo & ~63;
-  if (kb < e.key_hi) load_k_tile(kc, K, kb, lane);
+  if (kb < key_hi) load_k_tile(kc, K, kb, lane);
   int next_fold = (kb / e.chunk + 1) * e.chunk;
-  for (; kb < e.key_hi; kb += 64) {
+  for (; kb < key_hi; kb += 64) {
     if (kb == next_fold) {
       sh_fold_chunk(R);
       sh_fresh(R);
@@ -665,24 +720,25 @@ __device__ __forceinline__ void sh_wave_item(const ShEntry& e, int kv_head, cons
     load_v_tile(vc, V, kb, lane);
     // the next block's K goes into this one's registers once the scores are made
     auto next_k = [&]() __attribute__((always_inline)) {
-      if (kb + 64 < e.key_hi) load_k_tile(kc, K, kb + 64, lane);
+      if (kb + 64 < key_hi) load_k_tile(kc, K, kb + 64, lane);
     };
     auto kf = [&](int kt, int st) __attribute__((always_inline)) { return kc[kt][st]; };
     auto vf = [&](int dt, int h) __attribute__((always_inline)) { return vc[dt][h]; };
-    sh_block<QT, true, true>(R, kf, vf, next_k, kb, kb >= int_lo && kb + 63 <= int_hi, e.key_lo, e.key_hi);
+    sh_block<QT, true, true>(R, kf, vf, next_k, kb, kb >= int_lo && kb + 63 <= int_hi, e.key_lo, key_hi);
   }
-  sh_fold_chunk(R);
-  sh_write(R, e, 0, kv_head, Hkv, max_recs, parts);
+  sh_put(R, e.rec, 0, kv_head, Hkv, max_recs, parts);
 }
 
-// An item of up to 16 tokens by a workgroup of 4 waves, 4 tokens each: a block's K and V go to LDS once for all of them (two
-// buffers, the next block's loads in flight while this one computes).
-__device__ __forceinline__ void sh_tile_item(const ShEntry& e, int kv_head, const int2* __restrict__ list, const uint16_t* __restrict__ q,
+// `run` units from e on, of up to 16 tokens, by a workgroup of 4 waves, 4 tokens each: a block's K and V go to LDS once for all of them (two
+// buffers, the next block's loads in flight while this one computes).  The buffers are arrays of their own, picked at compile time, so
+// that the compiler does not wait for one's loads before it reads the other.
+__device__ __forceinline__ void sh_tile_item(const ShEntry& e, int run, int kv_head, const int2* __restrict__ list, const uint16_t* __restrict__ q,
                                              const uint16_t* __restrict__ k_pool, const uint16_t* __restrict__ v_pool, int Hq, int Hkv,
                                              int window, int max_recs, float* __restrict__ parts, uint4 (&buf0)[2][512],
                                              uint4 (&buf1)[2][512]) {
   typedef __attribute__((address_space(3))) void* lds_ptr;
   const int lane = threadIdx.x & 63, wave = scalar((int)threadIdx.x >> 6);
+  const int key_hi = sh_key_end(e, run);
   const int64_t base = e.base + (int64_t)kv_head * e.cap * 64;
   const char *Kb = reinterpret_cast<const char*>(k_pool + base), *Vb = reinterpret_cast<const char*>(v_pool + base);
   auto issue = [&](uint4 (&dst)[2][512], int kb) __attribute__((always_inline)) {
@@ -704,33 +760,36 @@ __device__ __forceinline__ void sh_tile_item(const ShEntry& e, int kv_head, cons
   int int_lo, int_hi;
   sh_interior(R, &int_lo, &int_hi);
   int_lo = max(int_lo, e.key_lo);
-  int_hi = min(int_hi, e.key_hi - 1);
+  int_hi = min(int_hi, key_hi - 1);
   const bool mine = 4 * wave < e.ntok;
   landed();
-  int next_fold = (kb_first / e.chunk + 1) * e.chunk;
+  int rec = e.rec, next_fold = (kb_first / e.chunk + 1) * e.chunk;
   auto step = [&](uint4 (&cur)[2][512], uint4 (&nxt)[2][512], int kb) __attribute__((always_inline)) {
-    if (kb + 64 < e.key_hi) issue(nxt, kb + 64);
+    if (kb + 64 < key_hi) issue(nxt, kb + 64);
     if (mine) {
       if (kb == next_fold) {
-        sh_fold_chunk(R);
+        if (e.stride) {
+          sh_put(R, rec, 4 * wave, kv_head, Hkv, max_recs, parts);
+          sh_nothing(R);
+          rec += e.stride;
+        } else {
+          sh_fold_chunk(R);
+        }
         sh_fresh(R);
         next_fold += e.chunk;
       }
       auto kf = [&](int kt, int st) __attribute__((always_inline)) { return cur[0][kt * 128 + st * 64 + lane]; };
       auto vf = [&](int dt, int h) __attribute__((always_inline)) { return cur[1][h * 256 + dt * 64 + lane]; };
-      if (kb >= int_lo && kb + 63 <= int_hi) sh_block<2, false, false>(R, kf, vf, [] {}, kb, true, e.key_lo, e.key_hi);
-      else sh_block<2, true, false>(R, kf, vf, [] {}, kb, false, e.key_lo, e.key_hi);
+      if (kb >= int_lo && kb + 63 <= int_hi) sh_block<2, false, false>(R, kf, vf, [] {}, kb, true, e.key_lo, key_hi);
+      else sh_block<2, true, false>(R, kf, vf, [] {}, kb, false, e.key_lo, key_hi);
     }
     landed();
   };
-  for (int kb = kb_first; kb < e.key_hi; kb += 128) {
+  for (int kb = kb_first; kb < key_hi; kb += 128) {
     step(buf0, buf1, kb);
-    if (kb + 64 < e.key_hi) step(buf1, buf0, kb + 64);
+    if (kb + 64 < key_hi) step(buf1, buf0, kb + 64);
   }
-  if (mine) {
-    sh_fold_chunk(R);
-    sh_write(R, e, 4 * wave, kv_head, Hkv, max_recs, parts);
-  }
+  if (mine) sh_put(R, rec, 4 * wave, kv_head, Hkv, max_recs, parts);
 }
 
 __global__ __launch_bounds__(256, 2) void attn_shared_kernel(const uint16_t* __restrict__ q, const uint16_t* __restrict__ k_pool,
@@ -741,26 +800,42 @@ __global__ __launch_bounds__(256, 2) void attn_shared_kernel(const uint16_t* __r
   const ShEntry* entries = reinterpret_cast<const ShEntry*>(plan + L.o_entries);
   const ShEntry* waves = reinterpret_cast<const ShEntry*>(plan + L.o_waves);
   const int2* list = reinterpret_cast<const int2*>(plan + L.o_list);
-  const int n_tile = hdr->n_entries * Hkv, n_wave = hdr->n_waves * Hkv, window = hdr->window;
-  const int n = n_tile + (n_wave + 3) / 4;
-  for (int i = blockIdx.x; i < n; i += gridDim.x) {
-    if (i < n_tile) {
-      const ShEntry e = entries[i / Hkv];
-      sh_tile_item(e, i % Hkv, list, q, k_pool, v_pool, Hq, Hkv, window, L.max_recs, parts, buf0, buf1);
+  const int per_head = gridDim.x / Hkv, w = blockIdx.x / Hkv, g = blockIdx.x % Hkv;
+  const int n_whole = hdr->n_whole, n_split = hdr->n_split, n_own = hdr->n_own, n_waves = hdr->n_waves, window = hdr->window;
+  auto tile = [&](int i, int run) __attribute__((always_inline)) {
+    const ShEntry e = entries[i];
+    sh_tile_item(e, run, g, list, q, k_pool, v_pool, Hq, Hkv, window, L.max_recs, parts, buf0, buf1);
+  };
+  // the whole tiles dealt out, the split ones in equal shares of consecutive units, the sequences' own from the other end
+  const int s0 = n_whole + (int)((int64_t)n_split * w / per_head), s1 = n_whole + (int)((int64_t)n_split * (w + 1) / per_head);
+  int i = w < n_whole ? w : s0, own = per_head - 1 - w;
+  for (;;) {
+    int at, run = 1;
+    if (i < n_whole) {
+      at = i;
+      i += per_head;
+      if (i >= n_whole) i = s0;
+    } else if (i < s1) {
+      at = i;
+      run = min(s1 - i, entries[i].left + 1);
+      i += run;
+    } else if (own < n_own) {
+      at = n_whole + n_split + own;
+      own += per_head;
     } else {
-      const int w = (i - n_tile) * 4 + scalar((int)threadIdx.x >> 6);
-      if (w < n_wave) {
-        const ShEntry e = waves[w / Hkv];
-        if (e.ntok <= 2) sh_wave_item<1>(e, w % Hkv, list, q, k_pool, v_pool, Hq, Hkv, window, L.max_recs, parts);
-        else sh_wave_item<2>(e, w % Hkv, list, q, k_pool, v_pool, Hq, Hkv, window, L.max_recs, parts);
-      }
+      break;
     }
+    tile(at, run);
+  }
+  for (int i = (per_head - 1 - w) * 4 + scalar((int)threadIdx.x >> 6); i < n_waves; i += per_head * 4) {
+    const ShEntry e = waves[i];
+    sh_wave_item<1>(e, g, list, q, k_pool, v_pool, Hq, Hkv, window, L.max_recs, parts);
   }
 }
 
 // The records of a token's 8 rows of a kv head, folded: the prefix's, the sequence's own, then both and the sink.  Thread (h = tid / 8,
 // part = tid % 8) takes 8 dims.  A token without any record (its sequence was refused) gets zeros.
-constexpr int kShMergeAhead = 4;
+constexpr int kShMergeAhead = 8;
 
 __global__ __launch_bounds__(64) void attn_shared_merge_kernel(const float* __restrict__ parts_in, const char* __restrict__ plan, ShLayout L,
                                                                const float* __restrict__ sinks, int Hq, int Hkv, uint16_t* __restrict__ out) {
@@ -866,8 +941,7 @@ extern "C" int flyai_attn_shared(const uint16_t* q, const uint16_t* k_pool, cons
                 "attn_shared: q, the pools, out, plan and workspace must be 16-byte aligned");
   const ShLayout L = sh_layout(T, S, n_prefix);
   hipStream_t s = as_stream(stream);
-  const int64_t most = (int64_t)L.max_entries * Hkv + ((int64_t)L.max_waves * Hkv + 3) / 4;
-  hipLaunchKernelGGL(attn_shared_kernel, dim3((unsigned)(most < kShGrid ? most : kShGrid)), dim3(256), 0, s, q, k_pool, v_pool, Hq, Hkv, L,
+  hipLaunchKernelGGL(attn_shared_kernel, dim3((unsigned)(sh_per_head(Hkv) * Hkv)), dim3(256), 0, s, q, k_pool, v_pool, Hq, Hkv, L,
                      static_cast<const char*>(plan), static_cast<float*>(workspace));
   const int rc2 = check_launch("attn_shared");
   if (rc2) return rc2;

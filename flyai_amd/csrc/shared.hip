@@ -539,46 +539,48 @@ __device__ __forceinline__ void sh_interior(const ShRows<QT>& R, int* lo, int* h
   *hi = scalar(b);
 }
 
-__device__ __forceinline__ bool bf16_pair_wild(uint32_t w) {
-  return (w & 0x7f800000u) == 0x7f800000u || (w & 0x7f80u) == 0x7f80u;
-}
-
 // Where a block has keys that some row does not see, their values may be infinite or NaN, and P is 0 there: 0 x inf would be NaN.
-// Such values are left out of v, and rows that see one get it by what the products of P with the classes' indicators say.
+// Such values are left out of v (all of a block's fragments), and rows that see one get it by what the products of P with the
+// classes' indicators say.  (A loop over the classes: the code is rarely run, and long.)
 template <int QT>
-__device__ __forceinline__ void sh_wild_values(ShRows<QT>& R, uint4& v0, uint4& v1, int dt, const bf16x8_t (&pt)[QT][2]) {
-  uint32_t w[8] = {v0.x, v0.y, v0.z, v0.w, v1.x, v1.y, v1.z, v1.w};
-#pragma unroll
-  for (int kind = 0; kind < 3; ++kind) {  // +inf, -inf, NaN
-    uint32_t f[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      uint32_t o = 0;
-#pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        const uint32_t x = (w[i] >> (16 * half)) & 0xffffu;
-        const bool is = kind == 0 ? x == 0x7f80u : kind == 1 ? x == 0xff80u : (x & 0x7fffu) > 0x7f80u;
-        if (is) o |= 0x3f80u << (16 * half);
-      }
-      f[i] = o;
-    }
+__device__ __forceinline__ void sh_wild_values(ShRows<QT>& R, uint4 (&v)[4][2], const bf16x8_t (&pt)[QT][2]) {
+#pragma unroll 1
+  for (uint32_t kind = 0; kind < 3; ++kind) {  // +inf, -inf, NaN
+    const uint32_t lo = kind == 0 ? 0x7f80u : kind == 1 ? 0xff80u : 0x7f81u, span = kind == 2 ? 0x7eu : 0u, mask = kind == 2 ? 0x7fffu : 0xffffu;
     const float add = kind == 0 ? INFINITY : kind == 1 ? -INFINITY : NAN;
-    const bf16x8_t f0 = as_bf16x8(make_uint4(f[0], f[1], f[2], f[3])), f1 = as_bf16x8(make_uint4(f[4], f[5], f[6], f[7]));
 #pragma unroll
-    for (int qt = 0; qt < QT; ++qt) {
-      f32x4_t c = mfma16x16x32(f0, pt[qt][0], f32x4_t{0.f, 0.f, 0.f, 0.f});
-      c = mfma16x16x32(f1, pt[qt][1], c);
+    for (int dt = 0; dt < 4; ++dt) {
+      bf16x8_t f[2];
 #pragma unroll
-      for (int v = 0; v < 4; ++v) R.O[qt][dt][v] += c[v] > 0.f ? add : 0.f;
+      for (int h = 0; h < 2; ++h) {
+        const uint32_t w[4] = {v[dt][h].x, v[dt][h].y, v[dt][h].z, v[dt][h].w};
+        uint32_t o[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          o[i] = ((w[i] & mask) - lo <= span ? 0x3f80u : 0u) | (((w[i] >> 16) & mask) - lo <= span ? 0x3f800000u : 0u);
+        f[h] = as_bf16x8(make_uint4(o[0], o[1], o[2], o[3]));
+      }
+#pragma unroll
+      for (int qt = 0; qt < QT; ++qt) {
+        f32x4_t c = mfma16x16x32(f[0], pt[qt][0], f32x4_t{0.f, 0.f, 0.f, 0.f});
+        c = mfma16x16x32(f[1], pt[qt][1], c);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) R.O[qt][dt][i] += c[i] > 0.f ? add : 0.f;
+      }
     }
   }
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    if ((w[i] & 0x7f80u) == 0x7f80u) w[i] &= 0xffff0000u;
-    if ((w[i] & 0x7f800000u) == 0x7f800000u) w[i] &= 0xffffu;
-  }
-  v0 = make_uint4(w[0], w[1], w[2], w[3]);
-  v1 = make_uint4(w[4], w[5], w[6], w[7]);
+  for (int dt = 0; dt < 4; ++dt)
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      uint32_t w[4] = {v[dt][h].x, v[dt][h].y, v[dt][h].z, v[dt][h].w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if ((w[i] & 0x7f80u) == 0x7f80u) w[i] &= 0xffff0000u;
+        if ((w[i] & 0x7f800000u) == 0x7f800000u) w[i] &= 0xffffu;
+      }
+      v[dt][h] = make_uint4(w[0], w[1], w[2], w[3]);
+    }
 }
 
 // One 64-key block against the wave's rows.  k(kt, step) and v(dt, half) give its fragments.  As in attn.hip: scores S^T = K . Q^T,
@@ -610,22 +612,22 @@ __device__ __forceinline__ void sh_block(ShRows<QT>& R, KF&& k, VF&& v, AF&& aft
       const int qt = q0 + j;
       float bmax = -INFINITY;
       if (MASKED && !interior) {
-        const int lo = max(key_lo, R.lo[qt]), hi = min(key_hi - 1, R.hi[qt]);
+        // (tile_key(kt, 4 g + i) is 8 g + tile_key(kt, i); a row that sees nothing has a count of 0)
+        const int lo = max(key_lo, R.lo[qt]), from = kb + 8 * g - lo;
+        const uint32_t count = (uint32_t)max(min(key_hi - 1, R.hi[qt]) - lo + 1, 0);
 #pragma unroll
         for (int kt = 0; kt < 4; ++kt)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int key = kb + tile_key(kt, 4 * g + i);
-            s[j][kt][i] = key >= lo && key <= hi ? s[j][kt][i] : -INFINITY;
-          }
+          for (int i = 0; i < 4; ++i) s[j][kt][i] = (uint32_t)(from + tile_key(kt, i)) < count ? s[j][kt][i] : -INFINITY;
       }
 #pragma unroll
       for (int kt = 0; kt < 4; ++kt)
 #pragma unroll
         for (int i = 0; i < 4; ++i) bmax = fmaxf(bmax, s[j][kt][i]);
-      const float m_blk = max_lane_groups(bmax) * scale;
-      const bool move = m_blk > R.m[qt] + kMaxSlack;
-      if (__ballot(move)) {
+      // (a row's largest score lies in one of its four lanes: they are compared only where one of the wave's lanes is past its row's slack)
+      if (__ballot(bmax * scale > R.m[qt] + kMaxSlack)) {
+        const float m_blk = max_lane_groups(bmax) * scale;
+        const bool move = m_blk > R.m[qt] + kMaxSlack;
         const float m_new = move ? m_blk : R.m[qt];
         const float alpha = __builtin_amdgcn_exp2f(R.m[qt] - m_new);
         R.m[qt] = m_new;
@@ -643,24 +645,97 @@ __device__ __forceinline__ void sh_block(ShRows<QT>& R, KF&& k, VF&& v, AF&& aft
       R.L[qt] = mfma16x16x32(ones, pt[qt][1], R.L[qt]);
     }
   }
+  if (MASKED && !interior) {
+    uint4 w[4][2];
+    uint32_t wild = 0;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      // keys outside the item's range may never have been written
+      const uint4 all = make_uint4(~0u, ~0u, ~0u, ~0u), there = mask_keys(all, kb + 32 * h + 8 * g, key_lo, key_hi);
+#pragma unroll
+      for (int dt = 0; dt < 4; ++dt) {
+        uint4 x = v(dt, h);
+        x = make_uint4(x.x & there.x, x.y & there.y, x.z & there.z, x.w & there.w);
+        w[dt][h] = x;
+        // (the sum's top bit of a half is set where its exponent is all ones)
+        wild |= ((x.x & 0x7fff7fffu) + 0x00800080u) | ((x.y & 0x7fff7fffu) + 0x00800080u) | ((x.z & 0x7fff7fffu) + 0x00800080u) |
+                ((x.w & 0x7fff7fffu) + 0x00800080u);
+      }
+    }
+    if (__ballot((wild & 0x80008000u) != 0)) sh_wild_values(R, w, pt);
+#pragma unroll
+    for (int dt = 0; dt < 4; ++dt)
+#pragma unroll
+      for (int qt = 0; qt < QT; ++qt) {
+        R.O[qt][dt] = mfma16x16x32(as_bf16x8(w[dt][0]), pt[qt][0], R.O[qt][dt]);
+        R.O[qt][dt] = mfma16x16x32(as_bf16x8(w[dt][1]), pt[qt][1], R.O[qt][dt]);
+      }
+    return;
+  }
 #pragma unroll
   for (int dt = 0; dt < 4; ++dt) {
-    uint4 v0 = v(dt, 0), v1 = v(dt, 1);
-    if (MASKED && !interior) {
-      if (kb < key_lo || kb + 64 > key_hi) {  // keys outside the item's range may never have been written
-        v0 = mask_keys(v0, kb + 8 * g, key_lo, key_hi);
-        v1 = mask_keys(v1, kb + 32 + 8 * g, key_lo, key_hi);
-      }
-      const bool wild = bf16_pair_wild(v0.x) || bf16_pair_wild(v0.y) || bf16_pair_wild(v0.z) || bf16_pair_wild(v0.w) ||
-                        bf16_pair_wild(v1.x) || bf16_pair_wild(v1.y) || bf16_pair_wild(v1.z) || bf16_pair_wild(v1.w);
-      if (__ballot(wild)) sh_wild_values(R, v0, v1, dt, pt);
-    }
+    const uint4 v0 = v(dt, 0), v1 = v(dt, 1);
 #pragma unroll
     for (int qt = 0; qt < QT; ++qt) {
       R.O[qt][dt] = mfma16x16x32(as_bf16x8(v0), pt[qt][0], R.O[qt][dt]);
       R.O[qt][dt] = mfma16x16x32(as_bf16x8(v1), pt[qt][1], R.O[qt][dt]);
     }
   }
+}
+
+// The same for a block that every row sees whole and that moves no row's maximum: straight-line code, so that the accumulators stay
+// where they are.  (A rescale's branch, or a branch around the block, costs 40 register copies a block: the two ways' accumulators
+// meet in other registers.)  false: some row's maximum has to move, and nothing was done.
+template <int QT, class KF, class VF>
+__device__ __forceinline__ bool sh_fast_block(ShRows<QT>& R, KF&& k, VF&& v) {
+  const float scale = 0.125f * kLog2e;
+  const bf16x8_t ones = as_bf16x8(make_uint4(0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u));
+  f32x4_t s[QT][4];
+#pragma unroll
+  for (int kt = 0; kt < 4; ++kt) {
+    const bf16x8_t k0 = as_bf16x8(k(kt, 0)), k1 = as_bf16x8(k(kt, 1));
+#pragma unroll
+    for (int qt = 0; qt < QT; ++qt) {
+      s[qt][kt] = mfma16x16x32(k0, R.qf[qt][0], f32x4_t{0.f, 0.f, 0.f, 0.f});
+      s[qt][kt] = mfma16x16x32(k1, R.qf[qt][1], s[qt][kt]);
+    }
+  }
+  bool past = false;  // (sh_block's rule)
+#pragma unroll
+  for (int qt = 0; qt < QT; ++qt) {
+    float bmax = -INFINITY;
+#pragma unroll
+    for (int kt = 0; kt < 4; ++kt)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) bmax = fmaxf(bmax, s[qt][kt][i]);
+    past |= bmax * scale > R.m[qt] + kMaxSlack;
+  }
+  if (__ballot(past)) return false;
+  // (the wave with the exponentials goes first: the SIMD's other wave has its matrix products to fill with)
+  __builtin_amdgcn_s_setprio(1);
+  bf16x8_t pt[QT][2];
+#pragma unroll
+  for (int qt = 0; qt < QT; ++qt) {
+    const float neg_m = -R.m[qt];
+#pragma unroll
+    for (int kt = 0; kt < 4; ++kt)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        pt[qt][kt >> 1][(kt & 1) * 4 + i] = (__bf16)__builtin_amdgcn_exp2f(fmaf(s[qt][kt][i], scale, neg_m));
+    R.L[qt] = mfma16x16x32(ones, pt[qt][0], R.L[qt]);
+    R.L[qt] = mfma16x16x32(ones, pt[qt][1], R.L[qt]);
+  }
+  __builtin_amdgcn_s_setprio(0);
+#pragma unroll
+  for (int dt = 0; dt < 4; ++dt) {
+    const uint4 v0 = v(dt, 0), v1 = v(dt, 1);
+#pragma unroll
+    for (int qt = 0; qt < QT; ++qt) {
+      R.O[qt][dt] = mfma16x16x32(as_bf16x8(v0), pt[qt][0], R.O[qt][dt]);
+      R.O[qt][dt] = mfma16x16x32(as_bf16x8(v1), pt[qt][1], R.O[qt][dt]);
+    }
+  }
+  return true;
 }
 
 // A record: O[64] of (record, kv head, head of the group), and apart from it (m, l).
@@ -738,7 +813,7 @@ __device__ __forceinline__ void sh_tile_item(const ShEntry& e, int run, int kv_h
                                              uint4 (&buf1)[2][512]) {
   typedef __attribute__((address_space(3))) void* lds_ptr;
   const int lane = threadIdx.x & 63, wave = scalar((int)threadIdx.x >> 6);
-  const int key_hi = sh_key_end(e, run);
+  const int key_lo = e.key_lo, key_hi = sh_key_end(e, run);
   const int64_t base = e.base + (int64_t)kv_head * e.cap * 64;
   const char *Kb = reinterpret_cast<const char*>(k_pool + base), *Vb = reinterpret_cast<const char*>(v_pool + base);
   auto issue = [&](uint4 (&dst)[2][512], int kb) __attribute__((always_inline)) {
@@ -761,35 +836,72 @@ __device__ __forceinline__ void sh_tile_item(const ShEntry& e, int run, int kv_h
   sh_interior(R, &int_lo, &int_hi);
   int_lo = max(int_lo, e.key_lo);
   int_hi = min(int_hi, key_hi - 1);
-  const bool mine = 4 * wave < e.ntok;
   landed();
-  int rec = e.rec, next_fold = (kb_first / e.chunk + 1) * e.chunk;
-  auto step = [&](uint4 (&cur)[2][512], uint4 (&nxt)[2][512], int kb) __attribute__((always_inline)) {
-    if (kb + 64 < key_hi) issue(nxt, kb + 64);
-    if (mine) {
-      if (kb == next_fold) {
-        if (e.stride) {
-          sh_put(R, rec, 4 * wave, kv_head, Hkv, max_recs, parts);
-          sh_nothing(R);
-          rec += e.stride;
-        } else {
-          sh_fold_chunk(R);
-        }
-        sh_fresh(R);
-        next_fold += e.chunk;
+  if (4 * wave >= e.ntok) {  // no rows: its part of the loads, and the barriers
+    int odd = 0;
+    for (int kb = kb_first; kb < key_hi; kb += 64, odd ^= 1) {
+      if (kb + 64 < key_hi) {
+        if (odd) issue(buf0, kb + 64);
+        else issue(buf1, kb + 64);
       }
-      auto kf = [&](int kt, int st) __attribute__((always_inline)) { return cur[0][kt * 128 + st * 64 + lane]; };
-      auto vf = [&](int dt, int h) __attribute__((always_inline)) { return cur[1][h * 256 + dt * 64 + lane]; };
-      if (kb >= int_lo && kb + 63 <= int_hi) sh_block<2, false, false>(R, kf, vf, [] {}, kb, true, e.key_lo, key_hi);
-      else sh_block<2, true, false>(R, kf, vf, [] {}, kb, false, e.key_lo, key_hi);
+      landed();
     }
-    landed();
-  };
-  for (int kb = kb_first; kb < key_hi; kb += 128) {
-    step(buf0, buf1, kb);
-    if (kb + 64 < key_hi) step(buf1, buf0, kb + 64);
+    return;
   }
-  if (mine) sh_put(R, rec, 4 * wave, kv_head, Hkv, max_recs, parts);
+  int rec = e.rec, next_fold = (kb_first / e.chunk + 1) * e.chunk;
+  // a block by the straight-line code: false if it has to be done by the long one (its successor's loads are out by then)
+  auto fast = [&](uint4 (&cur)[2][512], uint4 (&nxt)[2][512], int kb) __attribute__((always_inline)) {
+    if (kb + 64 < key_hi) issue(nxt, kb + 64);
+    if (!sh_fast_block(R, [&](int kt, int st) __attribute__((always_inline)) { return cur[0][kt * 128 + st * 64 + lane]; },
+                       [&](int dt, int h) __attribute__((always_inline)) { return cur[1][h * 256 + dt * 64 + lane]; }))
+      return false;
+    landed();
+    return true;
+  };
+  int odd = 0;
+  for (int kb = kb_first; kb < key_hi;) {
+    if (kb == next_fold) {
+      if (e.stride) {
+        sh_put(R, rec, 4 * wave, kv_head, Hkv, max_recs, parts);
+        sh_nothing(R);
+        rec += e.stride;
+      } else {
+        sh_fold_chunk(R);
+      }
+      sh_fresh(R);
+      next_fold += e.chunk;
+    }
+    // blocks up to the fold that every row sees whole
+    const int fast_end = min(min(next_fold, key_hi), int_hi - 62);
+    bool issued = false;
+    if (kb >= int_lo)
+      while (kb < fast_end) {
+        if (!odd) {
+          issued = !fast(buf0, buf1, kb);
+          if (issued) break;
+          kb += 64;
+          odd = 1;
+          if (kb >= fast_end) break;
+        }
+        issued = !fast(buf1, buf0, kb);
+        if (issued) break;
+        kb += 64;
+        odd = 0;
+      }
+    if (kb >= key_hi || kb == next_fold) continue;
+    if (!issued && kb + 64 < key_hi) {
+      if (odd) issue(buf0, kb + 64);
+      else issue(buf1, kb + 64);
+    }
+    const uint4* cur = odd ? &buf1[0][0] : &buf0[0][0];
+    sh_block<2, true, false>(R, [&](int kt, int st) __attribute__((always_inline)) { return cur[kt * 128 + st * 64 + lane]; },
+                             [&](int dt, int h) __attribute__((always_inline)) { return cur[512 + h * 256 + dt * 64 + lane]; }, [] {}, kb,
+                             kb >= int_lo && kb + 63 <= int_hi, key_lo, key_hi);
+    landed();
+    kb += 64;
+    odd ^= 1;
+  }
+  sh_put(R, rec, 4 * wave, kv_head, Hkv, max_recs, parts);
 }
 
 __global__ __launch_bounds__(256, 2) void attn_shared_kernel(const uint16_t* __restrict__ q, const uint16_t* __restrict__ k_pool,

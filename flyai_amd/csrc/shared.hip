@@ -14,6 +14,8 @@
 //
 // The work lists are made on the GPU (attn_shared_plan_kernel), once for a step's layers: the host needs
 // no lengths, only bounds, and the grids are sized by those.
+#include <type_traits>
+
 #include "attn.h"
 
 namespace flyai {
@@ -23,8 +25,8 @@ constexpr int kShWaveTokens = 2;      // tokens of a wave item
 constexpr int kShWaveSeq = 4;         // the most new tokens of a sequence whose own keys go to waves; more go to tiles
 constexpr int kShMaxSeqs = 4096, kShMaxPrefixes = 1024;
 constexpr int kShChunks = 24;         // a prefix's chunks: at most this many
-constexpr int kShMinChunk = 384, kShChunkStep = 192;
-constexpr int kShOwnChunk = 576;
+constexpr int kShMinChunk = 384, kShChunkStep = 192;  // (few positions are cut finer: their items are latency)
+constexpr int kShOwnChunk = 192;
 constexpr int kShSpareEntries = 1024;  // list entries beyond one for each tile, for prefixes split by chunks
 constexpr int kShSpareWaves = 2048;    // ... and beyond one for each group of a sequence's tokens
 constexpr int kShSpareRecs = 8192;     // records beyond two for each token
@@ -90,7 +92,6 @@ __host__ __device__ inline ShLayout sh_layout(int T, int S, int n_prefix) {
 
 // ---- the plan -------------------------------------------------------------------------------------
 
-constexpr int kShPlanThreads = 1024;
 
 // inclusive sum over the wave's lanes, by DPP (no LDS round trips): within rows of 16, then across them
 __device__ __forceinline__ int sh_wave_scan(int v) {
@@ -104,8 +105,8 @@ __device__ __forceinline__ int sh_wave_scan(int v) {
 }
 
 // N exclusive sums over the workgroup at once; total gets the sums
-template <int N>
-__device__ __forceinline__ void sh_excl_scan(int (&v)[N], int (&total)[N], int (&red)[N][kShPlanThreads / 64]) {
+template <int NT, int N>
+__device__ __forceinline__ void sh_excl_scan(int (&v)[N], int (&total)[N], int (&red)[6][NT / 64]) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   int incl[N];
 #pragma unroll
@@ -117,15 +118,16 @@ __device__ __forceinline__ void sh_excl_scan(int (&v)[N], int (&total)[N], int (
   __syncthreads();
 #pragma unroll
   for (int i = 0; i < N; ++i) {
-    const int sums = sh_wave_scan(lane < kShPlanThreads / 64 ? red[i][lane] : 0);
-    total[i] = __builtin_amdgcn_readlane(sums, kShPlanThreads / 64 - 1);
+    const int sums = sh_wave_scan(lane < NT / 64 ? red[i][lane] : 0);
+    total[i] = __builtin_amdgcn_readlane(sums, NT / 64 - 1);
     v[i] = incl[i] - v[i] + (wave ? __builtin_amdgcn_readlane(sums, max(wave, 1) - 1) : 0);
   }
 }
 
 __device__ __forceinline__ int sh_prefix_chunk(int P) {
   const int c = ((P + kShChunks - 1) / kShChunks + kShChunkStep - 1) / kShChunkStep * kShChunkStep;
-  return c > kShMinChunk ? c : kShMinChunk;
+  const int least = P <= 8 * kShChunkStep ? kShChunkStep : kShMinChunk;
+  return c > least ? c : least;
 }
 
 struct ShBatch {
@@ -146,49 +148,52 @@ __device__ __forceinline__ bool sh_slab_ok(int64_t base, int cap, int Hkv, int64
 }
 
 // What the plan keeps of a sequence and of a prefix, in LDS.
+template <int MAX>
 struct ShSeqs {
-  int32_t cu[kShMaxSeqs + 1];  // its first token
-  int32_t own0[kShMaxSeqs];    // the slab position of its first token; -1: the sequence has no tokens, or is refused
-  int32_t prefix[kShMaxSeqs];  // -1: none
-  int32_t place[kShMaxSeqs];   // its first listed token's place among its prefix's
-  int32_t entry0[kShMaxSeqs], rec0[kShMaxSeqs];  // its first entry (of its kind) and record
+  int32_t cu[MAX + 1];  // its first token
+  int32_t own0[MAX];    // the slab position of its first token; -1: the sequence has no tokens, or is refused
+  int32_t prefix[MAX];  // -1: none
+  int32_t place[MAX];   // its first listed token's place among its prefix's
+  int32_t entry0[MAX], rec0[MAX];  // its first entry (of its kind) and record
 };
+template <int MAX>
 struct ShPrefixes {
-  int32_t len[kShMaxPrefixes];  // -1: refused
-  int32_t cap[kShMaxPrefixes];
-  int64_t base[kShMaxPrefixes];
-  int32_t count[kShMaxPrefixes];  // listed tokens
-  int32_t lo[kShMaxPrefixes];     // the first position that any of them sees
-  int32_t list0[kShMaxPrefixes];
-  int32_t tile0[kShMaxPrefixes];  // its first tile, of all prefixes' (wave entry, for a prefix of few tokens)
-  int32_t unit0[kShMaxPrefixes], rec0[kShMaxPrefixes];  // of its tiles that are split: the first unit and record
+  int32_t len[MAX];  // -1: refused
+  int32_t cap[MAX];
+  int64_t base[MAX];
+  int32_t count[MAX];  // listed tokens
+  int32_t lo[MAX];     // the first position that any of them sees
+  int32_t list0[MAX];
+  int32_t tile0[MAX];  // its first tile, of all prefixes' (wave entry, for a prefix of few tokens)
+  int32_t unit0[MAX], rec0[MAX];  // of its tiles that are split: the first unit and record
 };
 constexpr int kShMaxOwnChunks = 4096;  // of a sequence, for the counts to stay in 32 bits: past it no sequence is split
 
 // One workgroup, so that nothing but LDS lies between the counts and the lists: one round trip for the lengths, three sums over the
 // workgroup, the lists.  A prefix's tokens are listed in the order in which its sequences' counts arrive at an LDS counter: which rows
 // share a tile may change from launch to launch, a row's result does not (no row's steps depend on its tile mates).
-__global__ __launch_bounds__(kShPlanThreads) void attn_shared_plan_kernel(ShBatch b, char* __restrict__ plan) {
+// Small batches have a workgroup of their own size: fewer waves at each barrier, and half the code to fetch.
+template <int NT, int PER>
+__global__ __launch_bounds__(NT) void attn_shared_plan_kernel(ShBatch b, char* __restrict__ plan) {
   const ShLayout L = sh_layout(b.T, b.S, b.n_prefix);
   ShHeader* hdr = reinterpret_cast<ShHeader*>(plan);
   ShEntry* entries = reinterpret_cast<ShEntry*>(plan + L.o_entries);
   ShEntry* waves = reinterpret_cast<ShEntry*>(plan + L.o_waves);
   int2* list = reinterpret_cast<int2*>(plan + L.o_list);
   ShToken* tokens = reinterpret_cast<ShToken*>(plan + L.o_tokens);
-  __shared__ ShSeqs sq;
-  __shared__ ShPrefixes px;
-  __shared__ int red[6][kShPlanThreads / 64];
+  __shared__ ShSeqs<NT * PER> sq;
+  __shared__ ShPrefixes<NT> px;
+  __shared__ int red[6][NT / 64];
   __shared__ int status_s;
   const int tid = threadIdx.x;
-  const int per = (b.S + kShPlanThreads - 1) / kShPlanThreads;
-  constexpr int kPer = kShMaxSeqs / kShPlanThreads;
+  const int per = (b.S + NT - 1) / NT;
   const int s0 = tid * per;
   int32_t status = 0;
   // everything that the batch is described by, in one round trip
-  int q[kPer], start[kPer], prefix[kPer], cap[kPer];
-  int64_t base[kPer];
+  int q[PER], start[PER], prefix[PER], cap[PER];
+  int64_t base[PER];
 #pragma unroll
-  for (int i = 0; i < kPer; ++i) {
+  for (int i = 0; i < PER; ++i) {
     const bool there = i < per && s0 + i < b.S;
     const int s = there ? s0 + i : 0;
     q[i] = start[i] = cap[i] = 0;
@@ -214,8 +219,8 @@ __global__ __launch_bounds__(kShPlanThreads) void attn_shared_plan_kernel(ShBatc
   if (tid == 0) status_s = 0;
   int sum[1] = {0}, total[1];
 #pragma unroll
-  for (int i = 0; i < kPer; ++i) sum[0] += min(max(q[i], 0), b.T + 1);  // (what is past T is refused: no sum passes 2^31)
-  sh_excl_scan<1>(sum, total, reinterpret_cast<int (&)[1][kShPlanThreads / 64]>(red));
+  for (int i = 0; i < PER; ++i) sum[0] += min(max(q[i], 0), b.T + 1);  // (what is past T is refused: no sum passes 2^31)
+  sh_excl_scan<NT, 1>(sum, total, red);
   const int n_tokens = min(total[0], b.T);
   if (total[0] > b.T) status |= kShPastTokens;
 
@@ -231,12 +236,12 @@ __global__ __launch_bounds__(kShPlanThreads) void attn_shared_plan_kernel(ShBatc
   };
   auto groups_of = [](int n) { return n <= kShWaveSeq ? (n + kShWaveTokens - 1) / kShWaveTokens : (n + kShRowTokens - 1) / kShRowTokens; };
 
-  int own[kPer];
+  int own[PER];
   // the groups of tokens that go to waves and to tiles, their entries and the records if they are split by chunks; whether a sequence
   // is too long for that
   int seqs[6] = {0, 0, 0, 0, 0, 0};
 #pragma unroll
-  for (int i = 0; i < kPer; ++i) {
+  for (int i = 0; i < PER; ++i) {
     own[i] = -1;
     const int s = s0 + i;
     if (i >= per || s >= b.S) continue;
@@ -276,7 +281,7 @@ __global__ __launch_bounds__(kShPlanThreads) void attn_shared_plan_kernel(ShBatc
   }
   if (status) atomicOr(&status_s, status);
   int n_seqs[6];
-  sh_excl_scan<6>(seqs, n_seqs, red);  // (its barriers also end the counting)
+  sh_excl_scan<NT, 6>(seqs, n_seqs, red);  // (its barriers also end the counting)
 
   // the prefixes: a thread has one
   const int np = tid < b.n_prefix ? px.count[tid] : 0;
@@ -291,7 +296,7 @@ __global__ __launch_bounds__(kShPlanThreads) void attn_shared_plan_kernel(ShBatc
   }
   // listed tokens; tiles of workgroups; entries of waves whole and by chunks, their records by chunks
   int ps[5] = {np, few ? 0 : tiles, few ? tiles : 0, few ? tiles * chunks : 0, few ? np * chunks : 0}, n_ps[5];
-  sh_excl_scan<5>(ps, n_ps, reinterpret_cast<int (&)[5][kShPlanThreads / 64]>(red));
+  sh_excl_scan<NT, 5>(ps, n_ps, red);
   // As many whole tiles as give every workgroup the same number; the rest by chunks, if the lists and the records hold them.
   const int per_head = sh_per_head(b.Hkv);
   int whole = n_ps[1] / per_head * per_head;
@@ -299,7 +304,7 @@ __global__ __launch_bounds__(kShPlanThreads) void attn_shared_plan_kernel(ShBatc
   int split = split_of(whole), split_tokens = np > 0 ? min(np, np - (tiles - split) * kShRowTokens) : 0;
   if (!split) split_tokens = 0;
   int us[2] = {split * chunks, split_tokens * chunks}, n_us[2];
-  sh_excl_scan<2>(us, n_us, reinterpret_cast<int (&)[2][kShPlanThreads / 64]>(red));
+  sh_excl_scan<NT, 2>(us, n_us, red);
   const bool fsplit = n_ps[3] + n_seqs[0] <= L.max_waves && n_ps[0] + n_ps[4] + b.T <= L.max_recs;
   const int few_recs = fsplit ? n_ps[4] : 0, few_waves = fsplit ? n_ps[3] : n_ps[2];
   if (whole + n_us[0] + n_seqs[1] > L.max_entries || n_ps[0] + few_recs + n_us[1] + b.T > L.max_recs) {  // (uniform)
@@ -324,14 +329,14 @@ __global__ __launch_bounds__(kShPlanThreads) void attn_shared_plan_kernel(ShBatc
     at[1] = seqs[1];
     at[2] = 0;
 #pragma unroll
-    for (int i = 0; i < kPer; ++i)
+    for (int i = 0; i < PER; ++i)
       if (own[i] >= 0) at[2] += q[i];
     int tokens_at[1] = {at[2]};
-    sh_excl_scan<1>(tokens_at, reinterpret_cast<int (&)[1]>(all), reinterpret_cast<int (&)[1][kShPlanThreads / 64]>(red));
+    sh_excl_scan<NT, 1>(tokens_at, reinterpret_cast<int (&)[1]>(all), red);
     at[2] = tokens_at[0];
   }
 #pragma unroll
-  for (int i = 0; i < kPer; ++i) {
+  for (int i = 0; i < PER; ++i) {
     if (own[i] < 0) continue;
     int c0;
     const int nch = osplit ? own_chunks(q[i], own[i], &c0) : 1, kind = q[i] > kShWaveSeq;
@@ -352,7 +357,7 @@ __global__ __launch_bounds__(kShPlanThreads) void attn_shared_plan_kernel(ShBatc
   if (tid == 0) hdr->status = status_s;
   // a prefix's units: tiles, or a tile's chunks behind one another
   auto first_split = [&](int p) __attribute__((always_inline)) { return max(0, whole - px.tile0[p]); };  // its first tile that is split
-  for (int p = tid >> 6; p < b.n_prefix; p += kShPlanThreads / 64) {
+  for (int p = tid >> 6; p < b.n_prefix; p += NT / 64) {
     const int n = px.count[p];
     if (!n) continue;
     const int len = px.len[p], c = sh_prefix_chunk(len), lo = px.lo[p], c0 = lo / c, nch = (len - 1) / c + 1 - c0;
@@ -379,7 +384,7 @@ __global__ __launch_bounds__(kShPlanThreads) void attn_shared_plan_kernel(ShBatc
       out[i] = e;
     }
   }
-  for (int t = tid; t < n_tokens; t += kShPlanThreads) {
+  for (int t = tid; t < n_tokens; t += NT) {
     int lo = 0, hi = b.S - 1;  // last sequence with cu <= t
     while (lo < hi) {
       const int mid = (lo + hi + 1) >> 1;
@@ -686,7 +691,8 @@ __device__ __forceinline__ void sh_block(ShRows<QT>& R, KF&& k, VF&& v, AF&& aft
 // The same for a block that every row sees whole and that moves no row's maximum: straight-line code, so that the accumulators stay
 // where they are.  (A rescale's branch, or a branch around the block, costs 40 register copies a block: the two ways' accumulators
 // meet in other registers.)  false: some row's maximum has to move, and nothing was done.
-template <int QT, class KF, class VF>
+// FIRST: the rows' state is a fresh one, and the maximum is set (nothing is there that would have to be rescaled).
+template <int QT, bool FIRST, class KF, class VF>
 __device__ __forceinline__ bool sh_fast_block(ShRows<QT>& R, KF&& k, VF&& v) {
   const float scale = 0.125f * kLog2e;
   const bf16x8_t ones = as_bf16x8(make_uint4(0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u));
@@ -708,9 +714,14 @@ __device__ __forceinline__ bool sh_fast_block(ShRows<QT>& R, KF&& k, VF&& v) {
     for (int kt = 0; kt < 4; ++kt)
 #pragma unroll
       for (int i = 0; i < 4; ++i) bmax = fmaxf(bmax, s[qt][kt][i]);
-    past |= bmax * scale > R.m[qt] + kMaxSlack;
+    if (FIRST) {
+      const float m_blk = max_lane_groups(bmax) * scale;
+      R.m[qt] = m_blk > R.m[qt] + kMaxSlack ? m_blk : R.m[qt];
+    } else {
+      past |= bmax * scale > R.m[qt] + kMaxSlack;
+    }
   }
-  if (__ballot(past)) return false;
+  if (!FIRST && __ballot(past)) return false;
   // (the wave with the exponentials goes first: the SIMD's other wave has its matrix products to fill with)
   __builtin_amdgcn_s_setprio(1);
   bf16x8_t pt[QT][2];
@@ -722,7 +733,7 @@ __device__ __forceinline__ bool sh_fast_block(ShRows<QT>& R, KF&& k, VF&& v) {
 #pragma unroll
       for (int i = 0; i < 4; ++i)
         pt[qt][kt >> 1][(kt & 1) * 4 + i] = (__bf16)__builtin_amdgcn_exp2f(fmaf(s[qt][kt][i], scale, neg_m));
-    R.L[qt] = mfma16x16x32(ones, pt[qt][0], R.L[qt]);
+    R.L[qt] = mfma16x16x32(ones, pt[qt][0], FIRST ? f32x4_t{0.f, 0.f, 0.f, 0.f} : R.L[qt]);
     R.L[qt] = mfma16x16x32(ones, pt[qt][1], R.L[qt]);
   }
   __builtin_amdgcn_s_setprio(0);
@@ -731,7 +742,7 @@ __device__ __forceinline__ bool sh_fast_block(ShRows<QT>& R, KF&& k, VF&& v) {
     const uint4 v0 = v(dt, 0), v1 = v(dt, 1);
 #pragma unroll
     for (int qt = 0; qt < QT; ++qt) {
-      R.O[qt][dt] = mfma16x16x32(as_bf16x8(v0), pt[qt][0], R.O[qt][dt]);
+      R.O[qt][dt] = mfma16x16x32(as_bf16x8(v0), pt[qt][0], FIRST ? f32x4_t{0.f, 0.f, 0.f, 0.f} : R.O[qt][dt]);
       R.O[qt][dt] = mfma16x16x32(as_bf16x8(v1), pt[qt][1], R.O[qt][dt]);
     }
   }
@@ -782,9 +793,13 @@ __device__ __forceinline__ void sh_wave_item(const ShEntry& e, int kv_head, cons
   sh_interior(R, &int_lo, &int_hi);
   int_lo = max(int_lo, e.key_lo);
   int_hi = min(int_hi, key_hi - 1);
-  uint4 kc[4][2], vc[4][2];
+  // K and V of the next block are loaded while this one computes, K into the same registers once the scores are made
+  uint4 kc[4][2], vc[4][2], vn[4][2];
   int kb = e.key_lo & ~63;
-  if (kb < key_hi) load_k_tile(kc, K, kb, lane);
+  if (kb < key_hi) {
+    load_k_tile(kc, K, kb, lane);
+    load_v_tile(vn, V, kb, lane);
+  }
   int next_fold = (kb / e.chunk + 1) * e.chunk;
   for (; kb < key_hi; kb += 64) {
     if (kb == next_fold) {
@@ -792,14 +807,20 @@ __device__ __forceinline__ void sh_wave_item(const ShEntry& e, int kv_head, cons
       sh_fresh(R);
       next_fold += e.chunk;
     }
-    load_v_tile(vc, V, kb, lane);
-    // the next block's K goes into this one's registers once the scores are made
-    auto next_k = [&]() __attribute__((always_inline)) {
-      if (kb + 64 < key_hi) load_k_tile(kc, K, kb + 64, lane);
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+      vc[t][0] = vn[t][0];
+      vc[t][1] = vn[t][1];
+    }
+    auto next = [&]() __attribute__((always_inline)) {
+      if (kb + 64 < key_hi) {
+        load_k_tile(kc, K, kb + 64, lane);
+        load_v_tile(vn, V, kb + 64, lane);
+      }
     };
-    auto kf = [&](int kt, int st) __attribute__((always_inline)) { return kc[kt][st]; };
-    auto vf = [&](int dt, int h) __attribute__((always_inline)) { return vc[dt][h]; };
-    sh_block<QT, true, true>(R, kf, vf, next_k, kb, kb >= int_lo && kb + 63 <= int_hi, e.key_lo, key_hi);
+    sh_block<QT, true, true>(R, [&](int kt, int st) __attribute__((always_inline)) { return kc[kt][st]; },
+                             [&](int dt, int h) __attribute__((always_inline)) { return vc[dt][h]; }, next, kb,
+                             kb >= int_lo && kb + 63 <= int_hi, e.key_lo, key_hi);
   }
   sh_put(R, e.rec, 0, kv_head, Hkv, max_recs, parts);
 }
@@ -850,15 +871,16 @@ __device__ __forceinline__ void sh_tile_item(const ShEntry& e, int run, int kv_h
   }
   int rec = e.rec, next_fold = (kb_first / e.chunk + 1) * e.chunk;
   // a block by the straight-line code: false if it has to be done by the long one (its successor's loads are out by then)
-  auto fast = [&](uint4 (&cur)[2][512], uint4 (&nxt)[2][512], int kb) __attribute__((always_inline)) {
+  auto fast = [&](uint4 (&cur)[2][512], uint4 (&nxt)[2][512], int kb, auto first) __attribute__((always_inline)) {
     if (kb + 64 < key_hi) issue(nxt, kb + 64);
-    if (!sh_fast_block(R, [&](int kt, int st) __attribute__((always_inline)) { return cur[0][kt * 128 + st * 64 + lane]; },
-                       [&](int dt, int h) __attribute__((always_inline)) { return cur[1][h * 256 + dt * 64 + lane]; }))
+    if (!sh_fast_block<2, decltype(first)::value>(R, [&](int kt, int st) __attribute__((always_inline)) { return cur[0][kt * 128 + st * 64 + lane]; },
+                                                  [&](int dt, int h) __attribute__((always_inline)) { return cur[1][h * 256 + dt * 64 + lane]; }))
       return false;
     landed();
     return true;
   };
   int odd = 0;
+  bool fresh = true;
   for (int kb = kb_first; kb < key_hi;) {
     if (kb == next_fold) {
       if (e.stride) {
@@ -870,36 +892,55 @@ __device__ __forceinline__ void sh_tile_item(const ShEntry& e, int run, int kv_h
       }
       sh_fresh(R);
       next_fold += e.chunk;
+      fresh = true;
     }
     // blocks up to the fold that every row sees whole
     const int fast_end = min(min(next_fold, key_hi), int_hi - 62);
     bool issued = false;
-    if (kb >= int_lo)
+    if (kb >= int_lo && kb < fast_end) {
+      if (fresh) {
+        if (odd) fast(buf1, buf0, kb, std::true_type{});
+        else fast(buf0, buf1, kb, std::true_type{});
+        kb += 64;
+        odd ^= 1;
+        fresh = false;
+      }
       while (kb < fast_end) {
         if (!odd) {
-          issued = !fast(buf0, buf1, kb);
+          issued = !fast(buf0, buf1, kb, std::false_type{});
           if (issued) break;
           kb += 64;
           odd = 1;
           if (kb >= fast_end) break;
         }
-        issued = !fast(buf1, buf0, kb);
+        issued = !fast(buf1, buf0, kb, std::false_type{});
         if (issued) break;
         kb += 64;
         odd = 0;
       }
-    if (kb >= key_hi || kb == next_fold) continue;
+      if (!issued) continue;
+    }
+    // any other block: its fragments are read before the next one's loads go out, with the buffer chosen at run time
+    const uint4* cur = odd ? &buf1[0][0] : &buf0[0][0];
+    uint4 kc[4][2], vc[4][2];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        kc[i][j] = cur[i * 128 + j * 64 + lane];
+        vc[i][j] = cur[512 + j * 256 + i * 64 + lane];
+      }
     if (!issued && kb + 64 < key_hi) {
       if (odd) issue(buf0, kb + 64);
       else issue(buf1, kb + 64);
     }
-    const uint4* cur = odd ? &buf1[0][0] : &buf0[0][0];
-    sh_block<2, true, false>(R, [&](int kt, int st) __attribute__((always_inline)) { return cur[kt * 128 + st * 64 + lane]; },
-                             [&](int dt, int h) __attribute__((always_inline)) { return cur[512 + h * 256 + dt * 64 + lane]; }, [] {}, kb,
-                             kb >= int_lo && kb + 63 <= int_hi, key_lo, key_hi);
+    sh_block<2, true, true>(R, [&](int kt, int st) __attribute__((always_inline)) { return kc[kt][st]; },
+                            [&](int dt, int h) __attribute__((always_inline)) { return vc[dt][h]; }, [] {}, kb,
+                            kb >= int_lo && kb + 63 <= int_hi, key_lo, key_hi);
     landed();
     kb += 64;
     odd ^= 1;
+    fresh = false;
   }
   sh_put(R, rec, 4 * wave, kv_head, Hkv, max_recs, parts);
 }
@@ -919,7 +960,8 @@ __global__ __launch_bounds__(256, 2) void attn_shared_kernel(const uint16_t* __r
     sh_tile_item(e, run, g, list, q, k_pool, v_pool, Hq, Hkv, window, L.max_recs, parts, buf0, buf1);
   };
   // the whole tiles dealt out, the split ones in equal shares of consecutive units, the sequences' own from the other end
-  const int s0 = n_whole + (int)((int64_t)n_split * w / per_head), s1 = n_whole + (int)((int64_t)n_split * (w + 1) / per_head);
+  const int share = n_split / per_head, more = n_split % per_head;
+  const int s0 = n_whole + w * share + min(w, more), s1 = s0 + share + (w < more);
   int i = w < n_whole ? w : s0, own = per_head - 1 - w;
   for (;;) {
     int at, run = 1;
@@ -945,36 +987,37 @@ __global__ __launch_bounds__(256, 2) void attn_shared_kernel(const uint16_t* __r
   }
 }
 
-// The records of a token's 8 rows of a kv head, folded: the prefix's, the sequence's own, then both and the sink.  Thread (h = tid / 8,
-// part = tid % 8) takes 8 dims.  A token without any record (its sequence was refused) gets zeros.
-constexpr int kShMergeAhead = 8;
+// The records of a token's 8 rows of a kv head, folded: the prefix's, the sequence's own, then both and the sink.  Thread (h = tid / 16,
+// part = tid % 16) takes 4 dims, with kShMergeAhead records' loads out at once (one round trip to memory for most tokens).  A token
+// without any record (its sequence was refused) gets zeros.
+constexpr int kShMergeAhead = 12;
 
-__global__ __launch_bounds__(64) void attn_shared_merge_kernel(const float* __restrict__ parts_in, const char* __restrict__ plan, ShLayout L,
-                                                               const float* __restrict__ sinks, int Hq, int Hkv, uint16_t* __restrict__ out) {
+__global__ __launch_bounds__(128) void attn_shared_merge_kernel(const float* __restrict__ parts_in, const char* __restrict__ plan, ShLayout L,
+                                                                const float* __restrict__ sinks, int Hq, int Hkv, uint16_t* __restrict__ out) {
   const ShHeader* hdr = reinterpret_cast<const ShHeader*>(plan);
   const int t = blockIdx.x, g = blockIdx.y;
-  if (t >= hdr->n_tokens) return;  // behind the last sequence: left as it was
-  const ShToken k = reinterpret_cast<const ShToken*>(plan + L.o_tokens)[t];
+  const ShToken k = reinterpret_cast<const ShToken*>(plan + L.o_tokens)[t];  // (of a row behind the last sequence: whatever is there, not used)
+  if (t >= hdr->n_tokens) return;  // left as it was
   float* parts = const_cast<float*>(parts_in);
-  const int h = threadIdx.x >> 3, part = threadIdx.x & 7;
-  float Mt[2], Lt[2], Ot[2][8];
+  const int h = threadIdx.x >> 4, part = threadIdx.x & 15;
+  const float sink = sinks[g * 8 + h] * kLog2e;
+  float Mt[2], Lt[2];
+  f32x4_t Ot[2];
 #pragma unroll
   for (int w = 0; w < 2; ++w) {
     const int rec0 = w ? k.o_rec : k.p_rec, n = w ? k.o_n : k.p_n, stride = w ? k.o_stride : k.p_stride;
     Mt[w] = -1e30f;
     Lt[w] = 0.f;
-#pragma unroll
-    for (int d = 0; d < 8; ++d) Ot[w][d] = 0.f;
+    Ot[w] = f32x4_t{0.f, 0.f, 0.f, 0.f};
     for (int c0 = 0; c0 < n; c0 += kShMergeAhead) {
       float2 ml[kShMergeAhead];
-      float4 o[kShMergeAhead][2];
+      f32x4_t o[kShMergeAhead];
 #pragma unroll
       for (int j = 0; j < kShMergeAhead; ++j) {
-        const int rec = rec0 + min(c0 + j, n - 1) * stride;
+        if (c0 + j >= n) break;  // uniform
+        const int rec = rec0 + (c0 + j) * stride;
         ml[j] = *reinterpret_cast<const float2*>(sh_rec_ml(parts, L.max_recs, rec, Hkv, g, h));
-        const float4* r = reinterpret_cast<const float4*>(sh_rec_o(parts, rec, Hkv, g, h) + part * 8);
-        o[j][0] = r[0];
-        o[j][1] = r[1];
+        o[j] = *reinterpret_cast<const f32x4_t*>(sh_rec_o(parts, rec, Hkv, g, h) + part * 4);
       }
 #pragma unroll
       for (int j = 0; j < kShMergeAhead; ++j)
@@ -982,25 +1025,22 @@ __global__ __launch_bounds__(64) void attn_shared_merge_kernel(const float* __re
           const ShFold f = sh_fold(Mt[w], ml[j].x);
           Mt[w] = f.M;
           Lt[w] = fmaf(ml[j].y, f.c, Lt[w] * f.a);
-          const float v[8] = {o[j][0].x, o[j][0].y, o[j][0].z, o[j][0].w, o[j][1].x, o[j][1].y, o[j][1].z, o[j][1].w};
 #pragma unroll
-          for (int d = 0; d < 8; ++d) Ot[w][d] = fmaf(v[d], f.c, Ot[w][d] * f.a);
+          for (int d = 0; d < 4; ++d) Ot[w][d] = fmaf(o[j][d], f.c, Ot[w][d] * f.a);
         }
     }
   }
-  const int head = g * 8 + h;
-  const float sink = sinks[head] * kLog2e;
   const float M = fmaxf(sink, fmaxf(Mt[0], Mt[1]));
   const float a = __builtin_amdgcn_exp2f(Mt[0] - M), c = __builtin_amdgcn_exp2f(Mt[1] - M);
   const float total = fmaf(Lt[1], c, Lt[0] * a) + __builtin_amdgcn_exp2f(sink - M);
   const float inv = k.o_n > 0 ? 1.0f / total : 0.f;
-  uint32_t w4[4];
+  uint32_t w2[2];
 #pragma unroll
-  for (int d = 0; d < 4; ++d) {
+  for (int d = 0; d < 2; ++d) {
     const float x = fmaf(Ot[1][2 * d], c, Ot[0][2 * d] * a) * inv, y = fmaf(Ot[1][2 * d + 1], c, Ot[0][2 * d + 1] * a) * inv;
-    w4[d] = (uint32_t)f2bf(x) | ((uint32_t)f2bf(y) << 16);
+    w2[d] = (uint32_t)f2bf(x) | ((uint32_t)f2bf(y) << 16);
   }
-  *reinterpret_cast<uint4*>(out + ((size_t)t * Hq + head) * 64 + part * 8) = make_uint4(w4[0], w4[1], w4[2], w4[3]);
+  *reinterpret_cast<uint2*>(out + ((size_t)t * Hq + g * 8 + h) * 64 + part * 4) = make_uint2(w2[0], w2[1]);
 }
 
 static int check_shared_shape(const char* what, int T, int S, int n_prefix, int Hkv) {
@@ -1036,7 +1076,10 @@ extern "C" int flyai_attn_shared_plan(const int32_t* q_lens, const int32_t* star
                     (n_prefix == 0 || (prefix_len && prefix_base && prefix_cap)) && plan && ((uintptr_t)plan & 15) == 0,
                 "attn_shared_plan: null pointer, or a plan that is not 16-byte aligned");
   const ShBatch b = {q_lens, starts, kv_base, kv_cap, prefix_of, prefix_len, prefix_base, prefix_cap, S, n_prefix, Hkv, window, T, pool_elems};
-  hipLaunchKernelGGL(attn_shared_plan_kernel, dim3(1), dim3(kShPlanThreads), 0, as_stream(stream), b, static_cast<char*>(plan));
+  if (S <= 256 && n_prefix <= 256 && T <= 512)
+    hipLaunchKernelGGL((attn_shared_plan_kernel<256, 1>), dim3(1), dim3(256), 0, as_stream(stream), b, static_cast<char*>(plan));
+  else
+    hipLaunchKernelGGL((attn_shared_plan_kernel<1024, kShMaxSeqs / 1024>), dim3(1), dim3(1024), 0, as_stream(stream), b, static_cast<char*>(plan));
   return check_launch("attn_shared_plan");
 }
 
@@ -1057,7 +1100,7 @@ extern "C" int flyai_attn_shared(const uint16_t* q, const uint16_t* k_pool, cons
                      static_cast<const char*>(plan), static_cast<float*>(workspace));
   const int rc2 = check_launch("attn_shared");
   if (rc2) return rc2;
-  hipLaunchKernelGGL(attn_shared_merge_kernel, dim3(T, Hkv), dim3(64), 0, s, static_cast<const float*>(workspace),
+  hipLaunchKernelGGL(attn_shared_merge_kernel, dim3(T, Hkv), dim3(128), 0, s, static_cast<const float*>(workspace),
                      static_cast<const char*>(plan), L, sinks, Hq, Hkv, out);
   return check_launch("attn_shared_merge");
 }

@@ -99,7 +99,7 @@ __device__ __forceinline__ bool ver_accepts(const VerArgs& a, int r, int d, uint
 // what a rejected draft's distribution leaves of a weight (whole numbers up to 2^40, which doubles hold)
 __device__ __forceinline__ double ver_rest(double w, float q, double W) {
   const double left = w - floor((double)fmaxf(q, 0.f) * W);
-  return left > 0.0 ? left : 0.0;
+  return fmax(left, 0.0);
 }
 
 // One row by a workgroup, for any logits: every pass reads the row again.
@@ -553,11 +553,11 @@ __device__ __forceinline__ VerWeights ver_weights(const VerArgs& a, int s, int r
 
 // w' of the stop row's pieces, a wave each at a time, the next one's loads in flight.  A piece's sums stay below 2^49 and are exact in
 // doubles.  Without a filter nearly every token has weight: a workgroup with many pieces makes the weights of the common values once
-// (kVerTable values of either sign from 2^-8 on) and looks them up; the others are made one by one.
-constexpr int kVerTable = 16 * 128;
-constexpr uint32_t kVerTableFirst = 0x3b80;  // the bits of 2^-8
-constexpr int kPieceThreads = 256;
-constexpr int kTablePieces = 32;  // four times as many tokens as the table has values
+// (|x| in [2^-24, 2^8)) and looks them up; the others are made one by one.
+constexpr int kVerTable = 32 * 128;      // values of a sign
+constexpr uint32_t kVerTableFirst = 0x3380;  // the bits of 2^-24
+constexpr int kPieceThreads = 1024;
+constexpr int kTablePieces = 32;  // twice as many tokens as the table has values
 
 struct __attribute__((packed, aligned(4))) VerVec4 { f32x4_t v; };
 
@@ -607,7 +607,8 @@ __global__ __launch_bounds__(kPieceThreads, 4) void verify_pieces_kernel(VerArgs
   if (look_up) {
     for (int i = threadIdx.x; i < 2 * kVerTable; i += kPieceThreads) {
       const uint32_t bits = kVerTableFirst + (i < kVerTable ? i : i - kVerTable + 0x8000u);
-      table[i] = samp_weight_f64(__fdiv_rn(bf2f((uint16_t)bits), w.tdiv), w.zmax);
+      const float z = __fdiv_rn(bf2f((uint16_t)bits), w.tdiv);
+      table[i] = z <= w.zmax ? samp_weight_f64(z, w.zmax) : 0.0;  // (no value of the row lies above)
     }
     if (threadIdx.x == 0) table[2 * kVerTable] = 0.0;
     __syncthreads();
@@ -634,8 +635,8 @@ __global__ __launch_bounds__(kPieceThreads, 4) void verify_pieces_kernel(VerArgs
         u16x2 t2 = __builtin_bit_cast(u16x2, l.x[i]);
         t2 -= (u16x2){(unsigned short)kVerTableFirst, (unsigned short)kVerTableFirst};
         const uint32_t t = __builtin_bit_cast(uint32_t, t2);
-        at[i] = ((t << 3) & 0x3ff83ff8u) | ((t >> 1) & 0x40004000u);
-        odd |= ((t & 0x78000000u) ? 2u : 0u) << (2 * i) | ((t & 0x7800u) ? 1u : 0u) << (2 * i);
+        at[i] = ((t << 3) & 0x7ff87ff8u) | (t & 0x80008000u);
+        odd |= ((t & 0x70000000u) ? 2u : 0u) << (2 * i) | ((t & 0x7000u) ? 1u : 0u) << (2 * i);
       }
       const char* tab = reinterpret_cast<const char*>(table);
 #pragma unroll
@@ -839,8 +840,8 @@ extern "C" int flyai_spec_verify(const uint16_t* logits, int32_t R, int32_t V, c
   hipStream_t s = as_stream(stream);
   if (R > 0) {
     hipLaunchKernelGGL(verify_rows_kernel, dim3(R), dim3(kSampThreads), 0, s, a, rows);
-    // four workgroups a CU, a piece a wave at least
-    const int wgs = std::max(1, std::min(ceil_div(a.pieces, kPieceThreads / 64), 4 * device_cus() / S));
+    // a workgroup a CU, a piece a wave at least
+    const int wgs = std::max(1, std::min(ceil_div(a.pieces, kPieceThreads / 64), device_cus() / S));
     hipLaunchKernelGGL(verify_pieces_kernel, dim3(wgs, S), dim3(kPieceThreads), 0, s, a, rows, pieces);
   }
   hipLaunchKernelGGL(verify_draw_kernel, dim3(S), dim3(kPiece), 0, s, a, rows, pieces, tokens, counts, p);

@@ -535,13 +535,15 @@ def pack_shared(q_lens, starts, kv_base, kv_cap, prefix_of, prefix_len, head_dim
     max_tokens = _position(max_tokens)
     at = q_lens.device
     m = max(max_tokens, 0)
-    out = {k: torch.empty(c, dtype=i32, device=at) for k, c in (("cu_seqlens", S + 1), ("positions", m), ("seq_id", m), ("kv_pos", m),
-                                                               ("kv_len", S), ("status", 1))}
-    out["kv_slot"] = torch.empty(m, dtype=torch.int64, device=at)
+    # (one allocation for the int32s: six would cost more than the kernel)
+    ints = torch.empty(2 * S + 2 + 3 * m, dtype=i32, device=at)
+    kv_slot = torch.empty(m, dtype=torch.int64, device=at)
+    p = ints.data_ptr()
+    cu, pos, seq, kv_pos, kv_len = p, p + 4 * (S + 1), p + 4 * (S + 1 + m), p + 4 * (S + 1 + 2 * m), p + 4 * (S + 1 + 3 * m)
     _on(dev, lib().flyai_pack_shared, q_lens.data_ptr(), starts.data_ptr(), kv_base.data_ptr(), kv_cap.data_ptr(), prefix_of.data_ptr(),
-        prefix_len.data_ptr(), S, n, _position(head_dim), max_tokens, out["cu_seqlens"].data_ptr(), out["positions"].data_ptr(),
-        out["seq_id"].data_ptr(), out["kv_pos"].data_ptr(), out["kv_slot"].data_ptr(), out["kv_len"].data_ptr(), out["status"].data_ptr())
-    return out
+        prefix_len.data_ptr(), S, n, _position(head_dim), max_tokens, cu, pos, seq, kv_pos, kv_slot.data_ptr(), kv_len, kv_len + 4 * S)
+    cu, pos, seq, kv_pos, kv_len, status = ints.split((S + 1, m, m, m, S, 1))
+    return dict(cu_seqlens=cu, positions=pos, seq_id=seq, kv_pos=kv_pos, kv_len=kv_len, kv_slot=kv_slot, status=status)
 
 
 class AttnSharedPlan:
@@ -549,9 +551,9 @@ class AttnSharedPlan:
 
     __slots__ = ("buffer", "n_tokens", "n_seqs", "n_prefixes", "n_kv_heads", "window", "pool_elems")
 
-    def __init__(self, *values):
-        for name, v in zip(self.__slots__, values):
-            setattr(self, name, v)
+    def __init__(self, buffer, n_tokens, n_seqs, n_prefixes, n_kv_heads, window, pool_elems):
+        self.buffer, self.n_tokens, self.n_seqs, self.n_prefixes = buffer, n_tokens, n_seqs, n_prefixes
+        self.n_kv_heads, self.window, self.pool_elems = n_kv_heads, window, pool_elems
 
     @property
     def status(self):

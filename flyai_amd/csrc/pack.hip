@@ -168,8 +168,13 @@ __global__ __launch_bounds__(kPackThreads) void pack_shared_kernel(
   __syncthreads();
   if (first && tid == 0) *status_out = status_s;
   const int Tw = min(cu[S], max_tokens);
-  const int t1 = min(Tw, (int)(blockIdx.x + 1) * kPackSharedTokens);
+  const int t1 = min(max_tokens, (int)(blockIdx.x + 1) * kPackSharedTokens);
   for (int t = blockIdx.x * kPackSharedTokens + tid; t < t1; t += kPackThreads) {
+    if (t >= Tw) {  // a row of no sequence: position -1, which the append skips
+      positions[t] = seq_id[t] = kv_pos[t] = -1;
+      kv_slot[t] = -1;
+      continue;
+    }
     int lo = 0, hi = S - 1;  // last s with cu[s] <= t
     while (lo < hi) {
       const int mid = (lo + hi + 1) >> 1;

@@ -12,7 +12,8 @@ integer weights w = floor(2^40 e^(z - max z)); only the uniforms come from the h
 generator seeded with ``seed``, so a run's receipts are reproducible (the reference seeds a torch
 generator instead; its stream cannot be matched, and the distribution of every output is what the
 accept rule preserves).  ``accept`` makes one launch for the K+1 drafted probabilities, one host copy,
-and one launch for the residual or bonus draw."""
+and one launch for the residual or bonus draw; ``accept_batch`` verifies the chunks of many sequences in one call
+(``flyai_spec_verify``), with the drafter's distributions if it has any."""
 import numpy as np
 import torch
 
@@ -97,6 +98,31 @@ class Sampler:
             return r
         r[K] = self._draw_row(x[K:K + 1], -1)
         return r
+
+    def accept_batch(self, logits, drafts, probs=None):
+        """``accept`` of many sequences at once: logits [sum of (K_s + 1), V] bf16, their rows one sequence after the other; drafts: a
+        list of K_s ids for each.  probs float32 [sum of K_s, V] on self.device: the distributions that the drafts were drawn from (None: deterministic
+        drafts), a draft accepted with probability min(1, p(d) / q(d)) then.  Returns for each sequence the accepted ids and the token
+        after them (the residual draw or the bonus draw; greedy: the argmax).  Consumes a uniform per row, then one per sequence."""
+        x = self._rows(logits)
+        R, V = x.shape
+        if sum(len(d) + 1 for d in drafts) != R:
+            raise ValueError(f"accept_batch: the drafts need {sum(len(d) + 1 for d in drafts)} logits rows, got {R}")
+        if any(not 0 <= int(i) < V for d in drafts for i in d):
+            raise ValueError("accept_batch: drafted token id outside the vocabulary")
+        if not drafts:
+            return []
+        flat, row, cu = [], [], [0]
+        for d in drafts:
+            row += [len(flat) - len(cu) + 1 + j for j in range(len(d))] + [-1]
+            flat += [int(i) for i in d] + [-1]
+            cu.append(len(flat))
+        put = lambda a, dtype: torch.tensor(a, dtype=dtype).to(self.device)  # noqa: E731
+        q = {} if probs is None else dict(draft_probs=probs, probs_row=put(row, torch.int32))
+        tokens, counts, _ = ops.spec_verify(x, put(cu, torch.int32), put(flat, torch.int32), put(self.gen.random(R), torch.float64),
+                                            put(self.gen.random(len(drafts)), torch.float64), self.temp, self.top_k, self.top_p, **q)
+        got = torch.cat((tokens, counts)).tolist()
+        return [got[a:a + n] for a, n in zip(cu, got[R:])]
 
 
 def tail_tokens(parts, h, sampler, prefill=False, draft=None):

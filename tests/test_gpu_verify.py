@@ -4,6 +4,7 @@ import pytest
 import torch
 
 from flyai_amd import ops
+from flyai_amd.sampling import Sampler
 from oracle import verify as oracle
 
 pytestmark = pytest.mark.gpu
@@ -274,3 +275,27 @@ def test_refusals():
                           (dict(draft_probs=torch.zeros(n, 99, device=DEV)), ValueError)):
         with pytest.raises(error):
             c.run(**change)
+
+
+@pytest.mark.parametrize("temp,top_k,top_p", [(0.0, 0, 1.0), (0.8, 0, 0.9), (1.0, 50, 1.0)])
+@pytest.mark.parametrize("probs", ["none", "all"])
+def test_sampler_accept_batch(temp, top_k, top_p, probs):
+    """Sampler.accept_batch: the oracle's tokens for the uniforms that the sampler's generator gives; greedy, accept's."""
+    drafts = [3, 0, 5, 1]
+    c = Case(1000, [n + 1 for n in drafts], [(temp, top_k, np.float32(top_p))] * 4, seed=11, probs=probs)
+    rows = [r for r in range(len(c.draft)) if c.draft[r] >= 0]
+    lists = [[int(c.draft[r]) for r in range(a, e - 1)] for a, e in zip(c.cu[:-1], c.cu[1:])]
+    c.probs_row[[e - 1 for e in c.cu[1:]]] = -1
+    gen = np.random.Generator(np.random.PCG64(5))
+    c.u, c.u_draw = gen.random(len(c.u)), gen.random(4)
+    sm = Sampler(temp=temp, top_p=top_p, top_k=top_k, seed=5, device=DEV)
+    got = sm.accept_batch(c.logits.to(DEV), lists, probs=torch.from_numpy(c.probs[rows]).to(DEV) if probs == "all" else None)
+    want, counts, _ = c.expected()
+    assert got == [want[a:a + n].tolist() for a, n in zip(c.cu, counts)]
+    if temp == 0:
+        assert got == [sm.accept(c.logits[a:e].to(DEV), d)[:len(g)] for a, e, d, g in zip(c.cu[:-1], c.cu[1:], lists, got)]
+    assert sm.accept_batch(c.logits[:0].to(DEV), []) == []
+    with pytest.raises(ValueError):
+        sm.accept_batch(c.logits.to(DEV), lists[:-1])
+    with pytest.raises(ValueError):
+        sm.accept_batch(c.logits.to(DEV), [[1000, 0, 0], *lists[1:]])

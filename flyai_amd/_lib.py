@@ -135,6 +135,9 @@ _PROTOS = {
     "flyai_stage_lora_workspace_bytes": (SZ, [P, I32]),
     "flyai_stage_set_lora": (C.c_int, [P, P]),
     "flyai_stage_forward_lora": (C.c_int, [P, P, P, P, P, P, I32, P, P]),
+    "flyai_stage_shared_workspace_bytes": (SZ, [P]),
+    "flyai_stage_set_shared": (C.c_int, [P, P, SZ]),
+    "flyai_stage_forward_shared": (C.c_int, [P, P, P, P, P, P, I32, P, P, P, P, I32, P, P]),
     "flyai_stage_forward_tree_lora": (C.c_int, [P, I32, I32, P, P, I64, I32, I32, P, P]),
     "flyai_stage_debug_buffer": (P, [P, I32]),
     "flyai_stage_set_graphs": (C.c_int, [P, I32]),

@@ -131,7 +131,7 @@ struct flyai_stage {
   bool graphs = false;
   hipStream_t capture_stream = nullptr;
   struct Graph {
-    int64_t key[13];
+    int64_t key[14];
     hipGraphExec_t exec;
     uint64_t last_use;
   };
@@ -144,6 +144,7 @@ struct flyai_stage {
   bool has_lora = false;
   flyai_stage_lora lora = {};
   std::vector<flyai_lora_layer> lora_layers;
+  char* shared = nullptr;       // workspace of steps whose sequences share prefixes (flyai_stage_set_shared): two plans, then the attention's
   std::vector<char> tree_img;   // host image of a tree step's flyai_attn_tree (header, depths, masks)
   std::vector<int> tree_order;  // host scratch: the nodes in order of depth
 };
@@ -171,7 +172,8 @@ static size_t blob_bytes(int S, int n_items0, int n_items1, int n_groups0, int n
   return align256(4 * sizeof(int32_t)) + align256((size_t)S * 4) * 3 + align256((size_t)S * 8) +
          align256((size_t)n_items0 * sizeof(flyai_attn_item)) + align256((size_t)n_items1 * sizeof(flyai_attn_item)) +
          align256((size_t)n_groups0 * sizeof(flyai_attn_group)) + align256((size_t)n_groups1 * sizeof(flyai_attn_group)) +
-         2 * align256((size_t)n_pitems * sizeof(flyai_attn_item)) + align256(tree_bytes(tree_nodes)) + align256((size_t)S * 4);
+         2 * align256((size_t)n_pitems * sizeof(flyai_attn_item)) + align256(tree_bytes(tree_nodes)) + align256((size_t)S * 4) +
+         3 * align256((size_t)S * 4) + align256((size_t)S * 8);  // (a prefix of its own for each sequence)
 }
 
 static void layout(flyai_stage* st) {
@@ -370,6 +372,30 @@ extern "C" int flyai_stage_set_lora(flyai_stage* st, const flyai_stage_lora* lor
   return FLYAI_OK;
 }
 
+// A plan of the largest step, and what the attention of one needs behind two of them; 0: not a shape that flyai_attn_shared has.
+static size_t shared_plan_bytes(const flyai_stage* st) {
+  const flyai_stage_config& c = st->cfg;
+  return align256(flyai_attn_shared_plan_bytes(c.max_tokens, c.max_seqs, std::min(c.max_seqs, 1024)));
+}
+
+extern "C" size_t flyai_stage_shared_workspace_bytes(const flyai_stage* st) {
+  if (!st) return 0;
+  const flyai_stage_config& c = st->cfg;
+  const size_t plan = shared_plan_bytes(st), attn = flyai_attn_shared_workspace_bytes(c.max_tokens, c.n_kv_heads);
+  return plan && attn && c.head_dim == 64 && c.n_q_heads == 8 * c.n_kv_heads ? 2 * plan + align256(attn) : 0;
+}
+
+extern "C" int flyai_stage_set_shared(flyai_stage* st, void* workspace, size_t bytes) {
+  FLYAI_REQUIRE(st, "set_shared: null stage");
+  const size_t need = flyai_stage_shared_workspace_bytes(st);
+  FLYAI_REQUIRE(!workspace || need, "set_shared: needs head_dim 64, 8 query heads a kv head, at most 64 kv heads, 65536 tokens and 4096 sequences");
+  FLYAI_REQUIRE(!workspace || (((uintptr_t)workspace & 255) == 0 && bytes >= need), "set_shared: needs a 256-byte aligned workspace of %zu bytes",
+                need);
+  drop_graphs(st);
+  st->shared = static_cast<char*>(workspace);
+  return FLYAI_OK;
+}
+
 extern "C" size_t flyai_stage_workspace_bytes(const flyai_stage* st) { return st ? st->dev_bytes : 0; }
 extern "C" size_t flyai_stage_host_staging_bytes(const flyai_stage* st) {
   return st ? 2 * st->host_half : 0;
@@ -438,8 +464,24 @@ struct StepPlan {
   bool lora = false;  // some sequence has an adapter: the blob carries theirs at off_adapter
   size_t off_adapter = 0;
   size_t off_tree = 0, off_tree_depth = 0;
+  int n_prefix = 0;  // > 0: the sequences lie behind prefixes, which the blob carries
+  size_t off_pof = 0, off_plen = 0, off_pbase = 0, off_pcap = 0;
+};
+
+// The prefixes of a step (host memory): which one each sequence is behind, and their lengths and slabs.
+struct StepPrefixes {
+  const int32_t *of, *len;
+  const int64_t* base;
+  const int32_t* cap;
+  int n;
 };
 }  // namespace
+
+static int64_t smallest_pool(const flyai_stage* st) {
+  int64_t pool = INT64_MAX;
+  for (int l = 0; l < st->cfg.n_layers; ++l) pool = std::min(pool, st->layers[l].kv_pool_elems);
+  return pool;
+}
 
 // The step's kernel sequence: ragged packing, then every layer.  Runs eagerly or under capture.
 // counts != nullptr: the attention grids are capacities and the kernels read the live counts there.
@@ -454,15 +496,31 @@ static int record_step(flyai_stage* st, const StepPlan& sp, const int32_t* count
   const int64_t* base_d = reinterpret_cast<const int64_t*>(blob + sp.off_base);
   const int32_t* cap_d = reinterpret_cast<const int32_t*>(blob + sp.off_cap);
   const flyai_attn_tree* tree_d = sp.tree ? reinterpret_cast<const flyai_attn_tree*>(blob + sp.off_tree) : nullptr;
-  const int32_t* kv_pos = sp.tree ? I32(st->o_kvpos) : nullptr;
+  const int32_t* kv_pos = sp.tree || sp.n_prefix ? I32(st->o_kvpos) : nullptr;
 
   const int Tn = sp.Tn;
   // the projections' partial planes: a step with adapters has one more of them below the tiled kernel's rows
   float* planes = sp.lora && !gemm_is_tiled(Tn) ? static_cast<float*>(st->lora.workspace) : F32(st->o_gemm);
   const int H = c.hidden, E = c.n_experts, k = c.top_k, I = c.intermediate;
   const bool fused_route = Tn <= 256 && Tn * k <= 4096;
+  char* plans[2] = {};  // of full and of sliding layers
+  if (sp.n_prefix) {
+    auto pre = [&](size_t o) { return reinterpret_cast<const int32_t*>(blob + o); };
+    const int64_t* pbase = reinterpret_cast<const int64_t*>(blob + sp.off_pbase);
+    RUN(flyai_pack_shared(pre(sp.off_q), pre(sp.off_st), base_d, cap_d, pre(sp.off_pof), pre(sp.off_plen), sp.S, sp.n_prefix, c.head_dim,
+                          Tn, I32(st->o_cu), I32(st->o_pos), I32(st->o_sid), I32(st->o_kvpos), reinterpret_cast<int64_t*>(d + st->o_slot),
+                          I32(st->o_kvlen), I32(st->o_status), s));
+    RUN(launch_rmsnorm(hidden, st->layers[0].ln1, Tn, H, c.rms_eps, B16(st->o_xn), s));
+    for (int l = 0; l < c.n_layers; ++l) {
+      const int p = st->layers[l].sliding ? 1 : 0;
+      if (plans[p]) continue;
+      plans[p] = st->shared + p * shared_plan_bytes(st);
+      RUN(flyai_attn_shared_plan(pre(sp.off_q), pre(sp.off_st), base_d, cap_d, pre(sp.off_pof), pre(sp.off_plen), pbase,
+                                 pre(sp.off_pcap), sp.S, sp.n_prefix, c.n_kv_heads, p ? c.window : 0, Tn, smallest_pool(st), plans[p], s));
+    }
+  }
   // the batch packing and the first layer's input RMSNorm in one launch (independent of each other)
-  RUN(launch_pack(reinterpret_cast<const int32_t*>(blob + sp.off_q),
+  else RUN(launch_pack(reinterpret_cast<const int32_t*>(blob + sp.off_q),
                   reinterpret_cast<const int32_t*>(blob + sp.off_st), base_d, cap_d, sp.S, c.head_dim,
                   c.max_tokens, I32(st->o_cu), I32(st->o_pos), I32(st->o_sid), I32(st->o_kvlen),
                   reinterpret_cast<int64_t*>(d + st->o_slot), I32(st->o_status),
@@ -484,7 +542,10 @@ static int record_step(flyai_stage* st, const StepPlan& sp, const int32_t* count
                            I32(st->o_sid), st->cos_tab, st->sin_tab, c.rope_positions, Tn, H,
                            c.n_q_heads, c.n_kv_heads, c.head_dim, base_d, cap_d, B16(st->o_qrot),
                            L.k_pool, L.v_pool, kv_pos, qkv_lora, s));
-    if (sp.n_pitems[p] > 0 && !tree_d) {
+    if (sp.n_prefix) {
+      RUN(flyai_attn_shared(B16(st->o_qrot), L.k_pool, L.v_pool, L.sinks, c.n_q_heads, c.n_kv_heads, c.head_dim, Tn, sp.S, sp.n_prefix,
+                            plans[p], st->shared + 2 * shared_plan_bytes(st), B16(st->o_attn), s));
+    } else if (sp.n_pitems[p] > 0 && !tree_d) {
       // prefill and split items share one launch (attn_step_kernel)
       RUN(launch_attn_step(B16(st->o_qrot), L.k_pool, L.v_pool, base_d, cap_d, L.sinks, L.sliding ? c.window : 0,
                            c.n_q_heads, reinterpret_cast<const flyai_attn_item*>(blob + sp.off_items[p]),
@@ -553,8 +614,8 @@ static int hip_fail(const char* what, hipError_t e) {
 
 // The executable graph for this step's key, captured on first use (least recently used evicted).
 static int step_graph(flyai_stage* st, const StepPlan& sp, hipGraphExec_t* out) {
-  const int64_t key[13] = {sp.Tn, sp.S, sp.grid_items[0], sp.grid_items[1], sp.grid_groups[0], sp.grid_groups[1],
-                           sp.n_pitems[0], sp.n_pitems[1], sp.merge[0], sp.merge[1], sp.lean[0], sp.lean[1], sp.lora};
+  const int64_t key[14] = {sp.Tn, sp.S, sp.grid_items[0], sp.grid_items[1], sp.grid_groups[0], sp.grid_groups[1],
+                           sp.n_pitems[0], sp.n_pitems[1], sp.merge[0], sp.merge[1], sp.lean[0], sp.lean[1], sp.lora, sp.n_prefix};
   ++st->use_clock;
   for (auto& g : st->graph_cache)
     if (memcmp(g.key, key, sizeof(key)) == 0) {
@@ -619,7 +680,8 @@ static int plan_needs_merge(const flyai_attn_group* groups, int n) {
 // launch (blob_fetch_kernel; an H2D copy if the staging is not mapped).
 static int stage_blob(flyai_stage* st, StepPlan& sp, const int32_t* q_lens, const int32_t* starts,
                       const int64_t* kv_base, const int32_t* kv_cap, const int* n_items,
-                      const int* n_groups, const std::vector<char>* tree, const int32_t* adapter, hipStream_t s) {
+                      const int* n_groups, const std::vector<char>* tree, const int32_t* adapter, const StepPrefixes* pre,
+                      hipStream_t s) {
   const int S = sp.S;
   Carve b;
   sp.off_counts = b.take(4 * sizeof(int32_t));
@@ -637,6 +699,13 @@ static int stage_blob(flyai_stage* st, StepPlan& sp, const int32_t* q_lens, cons
   }
   sp.lora = adapter != nullptr;
   if (adapter) sp.off_adapter = b.take((size_t)S * 4);
+  if (pre) {
+    sp.n_prefix = pre->n;
+    sp.off_pof = b.take((size_t)S * 4);
+    sp.off_plen = b.take((size_t)pre->n * 4);
+    sp.off_pcap = b.take((size_t)pre->n * 4);
+    sp.off_pbase = b.take((size_t)pre->n * 8);
+  }
   if (b.off > st->blob_max) return set_error(FLYAI_ERANGE, "batch blob exceeds its reservation");
   // wait until the GPU consumed this staging half's previous contents, then fill it
   const int h = st->half;
@@ -657,6 +726,12 @@ static int stage_blob(flyai_stage* st, StepPlan& sp, const int32_t* q_lens, cons
   }
   if (tree) memcpy(hb + sp.off_tree, tree->data(), tree->size());
   if (adapter) memcpy(hb + sp.off_adapter, adapter, (size_t)S * 4);
+  if (pre) {
+    memcpy(hb + sp.off_pof, pre->of, (size_t)S * 4);
+    memcpy(hb + sp.off_plen, pre->len, (size_t)pre->n * 4);
+    memcpy(hb + sp.off_pcap, pre->cap, (size_t)pre->n * 4);
+    memcpy(hb + sp.off_pbase, pre->base, (size_t)pre->n * 8);
+  }
   if (st->host_dev)
     RUN(launch_blob_fetch(st->host_dev + h * st->host_half, st->dev + st->o_blob, b.off, s));
   else
@@ -672,8 +747,7 @@ static int stage_blob(flyai_stage* st, StepPlan& sp, const int32_t* q_lens, cons
 // phase0/fastverify.py:23-26).
 static int check_slabs(flyai_stage* st, const int64_t* kv_base, const int32_t* kv_cap, int S) {
   const flyai_stage_config& c = st->cfg;
-  int64_t pool = INT64_MAX;
-  for (int l = 0; l < c.n_layers; ++l) pool = std::min(pool, st->layers[l].kv_pool_elems);
+  const int64_t pool = smallest_pool(st);
   const int64_t per_pos = (int64_t)c.n_kv_heads * c.head_dim;
   for (int b = 0; b < S; ++b) {
     const int64_t end = kv_base[b] + (int64_t)kv_cap[b] * per_pos;
@@ -694,6 +768,39 @@ static int check_slabs(flyai_stage* st, const int64_t* kv_base, const int32_t* k
   return FLYAI_OK;
 }
 
+// The prefixes' slabs must lie in the pools, and no sequence may append where one is read: a sequence's slab is apart from
+// every prefix's, or the same one, with the sequence behind no prefix and past the positions that are read.  order: the sequences by
+// kv_base, as check_slabs left it (a single one has no order).
+static int check_prefixes(flyai_stage* st, const int32_t* starts, const int64_t* kv_base, const int32_t* kv_cap, int S, const StepPrefixes& pre) {
+  const flyai_stage_config& c = st->cfg;
+  const int64_t pool = smallest_pool(st), per_pos = (int64_t)c.n_kv_heads * c.head_dim;
+  FLYAI_REQUIRE(pre.n <= std::min(c.max_seqs, 1024), "forward: %d prefixes above %d (max_seqs, 1024)", pre.n, std::min(c.max_seqs, 1024));
+  FLYAI_REQUIRE(st->shared, "forward: prefixes need flyai_stage_set_shared");
+  for (int b = 0; b < S; ++b) {
+    FLYAI_REQUIRE(pre.of[b] >= -1 && pre.of[b] < pre.n, "sequence %d: prefix %d outside [-1, %d)", b, pre.of[b], pre.n);
+    FLYAI_REQUIRE(pre.of[b] < 0 || starts[b] >= pre.len[pre.of[b]], "sequence %d starts at %d, before its prefix of %d positions ends", b,
+                  starts[b], pre.len[pre.of[b]]);
+  }
+  int* order = st->slab_order.data();
+  if (S == 1) order[0] = 0;
+  for (int i = 0; i < pre.n; ++i) {
+    const int64_t lo = pre.base[i], hi = lo + (int64_t)pre.cap[i] * per_pos;
+    FLYAI_REQUIRE(pre.len[i] >= 0 && pre.cap[i] >= pre.len[i] && pre.cap[i] % 64 == 0 && lo >= 0 && lo % 8 == 0,
+                  "prefix %d needs 0 <= length <= cap, cap %% 64 == 0 and base %% 8 == 0", i);
+    if (hi > pool)
+      return set_error(FLYAI_ERANGE, "prefix %d: KV slab [%lld, %lld) ends past the pools (%lld elements)", i, (long long)lo, (long long)hi,
+                       (long long)pool);
+    // the first sequence whose slab ends past lo, and those behind it (the slabs are apart, so their ends ascend too)
+    const int* at = std::partition_point(order, order + S, [&](int b) { return kv_base[b] + (int64_t)kv_cap[b] * per_pos <= lo; });
+    for (; at < order + S && kv_base[*at] < hi; ++at) {
+      const int b = *at;
+      const bool reads_its_own = kv_base[b] == lo && kv_cap[b] == pre.cap[i] && pre.of[b] < 0 && starts[b] >= pre.len[i];
+      FLYAI_REQUIRE(reads_its_own, "sequence %d appends to the slab of prefix %d", b, i);
+    }
+  }
+  return FLYAI_OK;
+}
+
 // The adapters of a step's sequences: *used is null if there are none.
 static int check_adapters(const flyai_stage* st, const int32_t* adapter, int S, const int32_t** used) {
   *used = nullptr;
@@ -708,6 +815,9 @@ static int check_adapters(const flyai_stage* st, const int32_t* adapter, int S, 
   return FLYAI_OK;
 }
 
+static int stage_forward(flyai_stage* st, const int32_t* q_lens, const int32_t* starts, const int64_t* kv_base, const int32_t* kv_cap,
+                         const int32_t* adapter, const StepPrefixes* pre, int32_t S, uint16_t* hidden, flyai_stream_t stream);
+
 extern "C" int flyai_stage_forward(flyai_stage* st, const int32_t* q_lens, const int32_t* starts,
                                    const int64_t* kv_base, const int32_t* kv_cap, int32_t S,
                                    uint16_t* hidden, flyai_stream_t stream) {
@@ -717,6 +827,22 @@ extern "C" int flyai_stage_forward(flyai_stage* st, const int32_t* q_lens, const
 extern "C" int flyai_stage_forward_lora(flyai_stage* st, const int32_t* q_lens, const int32_t* starts,
                                         const int64_t* kv_base, const int32_t* kv_cap, const int32_t* adapter, int32_t S,
                                         uint16_t* hidden, flyai_stream_t stream) {
+  return stage_forward(st, q_lens, starts, kv_base, kv_cap, adapter, nullptr, S, hidden, stream);
+}
+
+extern "C" int flyai_stage_forward_shared(flyai_stage* st, const int32_t* q_lens, const int32_t* starts, const int64_t* kv_base,
+                                          const int32_t* kv_cap, const int32_t* adapter, int32_t S, const int32_t* prefix_of,
+                                          const int32_t* prefix_len, const int64_t* prefix_base, const int32_t* prefix_cap,
+                                          int32_t n_prefixes, uint16_t* hidden, flyai_stream_t stream) {
+  FLYAI_REQUIRE(n_prefixes >= 0, "forward: n_prefixes must be >= 0");
+  if (n_prefixes == 0) return stage_forward(st, q_lens, starts, kv_base, kv_cap, adapter, nullptr, S, hidden, stream);
+  FLYAI_REQUIRE(prefix_of && prefix_len && prefix_base && prefix_cap, "forward: null pointer");
+  const StepPrefixes pre = {prefix_of, prefix_len, prefix_base, prefix_cap, n_prefixes};
+  return stage_forward(st, q_lens, starts, kv_base, kv_cap, adapter, &pre, S, hidden, stream);
+}
+
+static int stage_forward(flyai_stage* st, const int32_t* q_lens, const int32_t* starts, const int64_t* kv_base, const int32_t* kv_cap,
+                         const int32_t* adapter, const StepPrefixes* pre, int32_t S, uint16_t* hidden, flyai_stream_t stream) {
   FLYAI_REQUIRE(st && q_lens && starts && kv_base && kv_cap && hidden, "forward: null pointer");
   const flyai_stage_config& c = st->cfg;
   FLYAI_REQUIRE(S >= 1 && S <= c.max_seqs, "forward: n_seqs %d out of [1, %d]", S, c.max_seqs);
@@ -727,9 +853,10 @@ extern "C" int flyai_stage_forward_lora(flyai_stage* st, const int32_t* q_lens, 
     FLYAI_REQUIRE(kv_cap[b] > 0 && kv_cap[b] % 64 == 0 && kv_base[b] >= 0 && kv_base[b] % 8 == 0,
                   "forward: sequence %d needs kv_cap %% 64 == 0 and kv_base %% 8 == 0", b);
     const int64_t need = (int64_t)starts[b] + q_lens[b];
-    if (need > kv_cap[b])
+    const int64_t own = need - (pre && pre->of[b] >= 0 && pre->of[b] < pre->n ? pre->len[pre->of[b]] : 0);
+    if (own > kv_cap[b])
       return set_error(FLYAI_ERANGE, "sequence %d needs %lld positions > KV capacity %d", b,
-                       (long long)need, kv_cap[b]);
+                       (long long)own, kv_cap[b]);
     if (need > c.rope_positions)
       return set_error(FLYAI_ERANGE, "sequence %d needs %lld positions > rope table %d", b,
                        (long long)need, c.rope_positions);
@@ -740,6 +867,7 @@ extern "C" int flyai_stage_forward_lora(flyai_stage* st, const int32_t* q_lens, 
   for (int l = 0; l < c.n_layers; ++l)
     FLYAI_REQUIRE(st->layers[l].wqkv, "forward: layer %d not bound", l);
   RUN(check_slabs(st, kv_base, kv_cap, S));
+  if (pre) RUN(check_prefixes(st, starts, kv_base, kv_cap, S, *pre));
   RUN(check_adapters(st, adapter, S, &adapter));
   FLYAI_REQUIRE(st->dev && st->host, "forward: workspace not set");
   FLYAI_REQUIRE(st->cos_tab && st->sin_tab, "forward: rope tables not set");
@@ -748,8 +876,12 @@ extern "C" int flyai_stage_forward_lora(flyai_stage* st, const int32_t* q_lens, 
   StepPlan sp;
   sp.Tn = (int)T;
   sp.S = S;
-  int n_items[2], n_groups[2];
+  int n_items[2] = {}, n_groups[2] = {};
   for (int p = 0; p < 2; ++p) {
+    if (pre) {  // (planned on the GPU)
+      sp.grid_items[p] = sp.grid_groups[p] = sp.n_small[p] = sp.n_pitems[p] = sp.merge[p] = sp.lean[p] = 0;
+      continue;
+    }
     RUN(attn_plan(q_lens, starts, S, c.n_kv_heads, p == 0 ? 0 : c.window, c.attn_split_keys,
                   st->plan_items[p].data(), c.max_attn_items, st->plan_groups[p].data(), st->max_groups,
                   &n_items[p], &n_groups[p], &sp.n_small[p], c.attn_prefill_min, st->plan_pitems[p].data(),
@@ -762,7 +894,7 @@ extern "C" int flyai_stage_forward_lora(flyai_stage* st, const int32_t* q_lens, 
     sp.merge[p] = plan_needs_merge(st->plan_groups[p].data(), n_groups[p]);
     sp.lean[p] = sp.n_small[p] == n_items[p];
   }
-  RUN(stage_blob(st, sp, q_lens, starts, kv_base, kv_cap, n_items, n_groups, nullptr, adapter, s));
+  RUN(stage_blob(st, sp, q_lens, starts, kv_base, kv_cap, n_items, n_groups, nullptr, adapter, pre, s));
   if (!st->graphs) return record_step(st, sp, nullptr, hidden, s);
 
   hipGraphExec_t exec = nullptr;
@@ -876,6 +1008,6 @@ extern "C" int flyai_stage_forward_tree_lora(flyai_stage* st, int32_t start, int
     sp.lean[p] = 0;
   }
   const int32_t q_len = n, st0 = start;
-  RUN(stage_blob(st, sp, &q_len, &st0, &kv_base, &kv_cap, n_items, n_groups, &st->tree_img, adapter, s));
+  RUN(stage_blob(st, sp, &q_len, &st0, &kv_base, &kv_cap, n_items, n_groups, &st->tree_img, adapter, nullptr, s));
   return record_step(st, sp, nullptr, hidden, s);
 }

@@ -170,7 +170,7 @@ class RaggedStage:
         self.set_workspace()
         self.use_graphs = False
         self.set_graphs(use_graphs)
-        self.lora = self._lora_ws = None
+        self.lora = self._lora_ws = self._shared_ws = None
         if lora is not None:
             self.set_lora(lora)
 
@@ -189,6 +189,19 @@ class RaggedStage:
         self._sync(self.device)
         ws = bank.bind(self._h)
         self.lora, self._lora_ws = bank, ws
+
+    def set_prefixes(self, enable=True):
+        """Bind (or let go) the workspace of steps whose sequences share prefixes (``forward``'s prefixes).  Waits for the device; drops every
+        captured step graph."""
+        self._sync(self.device)
+        if not enable:
+            check(lib().flyai_stage_set_shared(self._h, None, 0))
+            self._shared_ws = None
+            return
+        size = int(lib().flyai_stage_shared_workspace_bytes(self._h))
+        ws = torch.empty(size + 256, dtype=torch.uint8, device=self.device)
+        check(lib().flyai_stage_set_shared(self._h, C.c_void_p(ws.data_ptr() + (-ws.data_ptr()) % 256), size))
+        self._shared_ws = ws
 
     def set_layer(self, i, lw):
         """Bind layer i to the weights of ``lw`` and the workspace's layer-i KV pools.  Drops every
@@ -237,11 +250,14 @@ class RaggedStage:
                 pass
             self._destroy(h)
 
-    def forward(self, hidden, q_lens, starts, slots, adapters=None):
+    def forward(self, hidden, q_lens, starts, slots, adapters=None, prefixes=None):
         """hidden bf16 [T, H] (packed token order, updated in place and returned); q_lens/starts/slots
         per sequence (host ints); adapters: the bank's slot of each sequence, -1 or None for none (None: of all).  K/V that a
-        sequence shares (``KVWorkspace.fork``) belongs to the adapter it was computed with.  Raises ContextOverflow
-        before any write."""
+        sequence shares (``KVWorkspace.fork``, or a prefix) belongs to the adapter it was computed with.  prefixes (after
+        ``set_prefixes``): for each sequence (slot, n), whose first n positions are read from that slot, once for all the sequences behind it,
+        while the sequence's own slot holds position p at p - n; or None.  starts count from the prefix's first position.  A
+        prefix's slot is no sequence's own in the step, but of one without a prefix that starts at n or later.  Raises ContextOverflow before
+        any write."""
         S = len(q_lens)
         if not (len(starts) == S == len(slots)):
             raise ValueError("q_lens, starts and slots must have one entry per sequence")
@@ -258,6 +274,9 @@ class RaggedStage:
         base = np.ascontiguousarray([self.kv.base(int(s)) for s in slots], dtype=np.int64)
         cap = np.ascontiguousarray([self.kv.slot_cap(int(s)) for s in slots], dtype=np.int32)
         lim = np.asarray([self.kv.maxlens[int(s)] for s in slots], dtype=np.int64)
+        if prefixes is not None:
+            ids, of = self._prefixes(prefixes, S)
+            lim += [0 if p is None else int(p[1]) for p in prefixes]
         over = at > lim - ql
         if np.any(over):
             b = int(np.argmax(over))
@@ -268,12 +287,38 @@ class RaggedStage:
             if len(adapters) != S:
                 raise ValueError("adapters must have one entry per sequence")
             ad = np.ascontiguousarray([-1 if a is None else int(a) for a in adapters], dtype=np.int32)
+        if prefixes is not None and ids:
+            plen, pcap = (np.ascontiguousarray(a, dtype=np.int32) for a in ([n for _, n in ids], [self.kv.slot_cap(s) for s, _ in ids]))
+            pbase = np.ascontiguousarray([self.kv.base(s) for s, _ in ids], dtype=np.int64)
+            check(lib().flyai_stage_forward_shared(
+                self._h, *(C.c_void_p(a.ctypes.data) for a in (ql, st, base, cap)), None if ad is None else C.c_void_p(ad.ctypes.data), S,
+                *(C.c_void_p(a.ctypes.data) for a in (of, plen, pbase, pcap)), len(ids), C.c_void_p(hidden.data_ptr()),
+                C.c_void_p(torch.cuda.current_stream(self.device).cuda_stream)))
+            return hidden
         check(lib().flyai_stage_forward_lora(
             self._h, ql.ctypes.data_as(C.c_void_p), st.ctypes.data_as(C.c_void_p),
             base.ctypes.data_as(C.c_void_p), cap.ctypes.data_as(C.c_void_p),
             None if ad is None else ad.ctypes.data_as(C.c_void_p), S,
             C.c_void_p(hidden.data_ptr()), C.c_void_p(torch.cuda.current_stream(self.device).cuda_stream)))
         return hidden
+
+    def _prefixes(self, prefixes, S):
+        """The distinct (slot, length) of a step's prefixes, and each sequence's among them (-1: none)."""
+        if len(prefixes) != S:
+            raise ValueError("prefixes must have one entry per sequence")
+        ids, of = {}, np.full(S, -1, dtype=np.int32)
+        for b, p in enumerate(prefixes):
+            if p is None:
+                continue
+            slot, n = (int(v) for v in p)
+            if not 0 <= slot < self.kv.n_slots:
+                raise ValueError(f"prefix slot {slot} out of range")
+            if not 0 <= n <= self.kv.maxlens[slot]:
+                raise ValueError(f"prefix of {n} positions of slot {slot}, which holds {self.kv.maxlens[slot]}")
+            of[b] = ids.setdefault((slot, n), len(ids))
+        if ids and self._shared_ws is None:
+            raise ValueError("prefixes need set_prefixes()")
+        return list(ids), of
 
     def forward_tree(self, hidden, start, par, dep, slot=0, adapter=None):
         """Tree verify of one sequence (``FastVerify.tree_decode``, phase0/fastverify.py:281-299):

@@ -613,6 +613,20 @@ int flyai_stage_forward_lora(flyai_stage* st, const int32_t* q_lens_host, const 
 int flyai_stage_forward_tree_lora(flyai_stage* st, int32_t start, int32_t n_nodes,
                                   const int32_t* parent_host, const int32_t* depth_host, int64_t kv_base,
                                   int32_t kv_cap, int32_t adapter, uint16_t* hidden, flyai_stream_t stream);
+/* Sequences behind shared prefixes in a step (flyai_pack_shared, flyai_attn_shared in place of flyai_pack_ragged, flyai_attn_ragged):
+ * flyai_stage_set_shared binds a device workspace of flyai_stage_shared_workspace_bytes, 256-byte aligned (NULL unbinds it), and drops every
+ * captured step graph.  flyai_stage_forward_shared is flyai_stage_forward_lora with prefix prefix_of[b] (-1: none) for sequence b: its
+ * positions [0, prefix_len) are read from the prefix's slab, and its own slab holds position p at p - prefix_len.  All arrays are host
+ * memory; n_prefixes <= max_seqs and 1024, 0 is flyai_stage_forward_lora.  starts[b] < the prefix's length, a prefix that is none or a
+ * slab that overlaps a prefix's -> FLYAI_EINVAL, but for the slab of a sequence without a prefix that is a prefix's own, if the
+ * sequence starts past what is read of it; positions past kv_cap (counted in the slab) or the rope table, a slab past the pools -> FLYAI_ERANGE;
+ * both before any launch.  With graphs, one is captured for each (tokens, sequences, prefixes). */
+size_t flyai_stage_shared_workspace_bytes(const flyai_stage* st);
+int flyai_stage_set_shared(flyai_stage* st, void* workspace, size_t bytes);
+int flyai_stage_forward_shared(flyai_stage* st, const int32_t* q_lens, const int32_t* starts, const int64_t* kv_base,
+                               const int32_t* kv_cap, const int32_t* adapter, int32_t n_seqs, const int32_t* prefix_of,
+                               const int32_t* prefix_len, const int64_t* prefix_base, const int32_t* prefix_cap,
+                               int32_t n_prefixes, uint16_t* hidden, flyai_stream_t stream);
 /* HIP-graph replay of flyai_stage_forward (the CUDA-graph capture of FastVerify.decode /
  * BatchedFastVerify.decode, phase0/fastverify.py:221-231, phase0/batchverify.py:180-190).  When
  * enabled, each step's kernels are one graph per (tokens, sequences, attention-plan capacity) key:

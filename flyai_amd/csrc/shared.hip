@@ -692,8 +692,9 @@ __device__ __forceinline__ void sh_block(ShRows<QT>& R, KF&& k, VF&& v, AF&& aft
 // where they are.  (A rescale's branch, or a branch around the block, costs 40 register copies a block: the two ways' accumulators
 // meet in other registers.)  false: some row's maximum has to move, and nothing was done.
 // FIRST: the rows' state is a fresh one, and the maximum is set (nothing is there that would have to be rescaled).
-template <int QT, bool FIRST, class KF, class VF>
-__device__ __forceinline__ bool sh_fast_block(ShRows<QT>& R, KF&& k, VF&& v) {
+template <bool FIRST, class KF, class VF>
+__device__ __forceinline__ bool sh_fast_block(ShRows<2>& R, KF&& k, VF&& v) {
+  constexpr int QT = 2;
   const float scale = 0.125f * kLog2e;
   const bf16x8_t ones = as_bf16x8(make_uint4(0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u));
   f32x4_t s[QT][4];
@@ -721,30 +722,44 @@ __device__ __forceinline__ bool sh_fast_block(ShRows<QT>& R, KF&& k, VF&& v) {
       past |= bmax * scale > R.m[qt] + kMaxSlack;
     }
   }
-  if (!FIRST && __ballot(past)) return false;
   // (the wave with the exponentials goes first: the SIMD's other wave has its matrix products to fill with)
   __builtin_amdgcn_s_setprio(1);
   bf16x8_t pt[QT][2];
+  auto weight = [&](int qt, int kt, int i) __attribute__((always_inline)) {
+    pt[qt][kt >> 1][(kt & 1) * 4 + i] = (__bf16)__builtin_amdgcn_exp2f(fmaf(s[qt][kt][i], scale, -R.m[qt]));
+  };
+  // the weights of the first 32 keys; those of the others between their products, which a wave's own matrix units run beside them.
+  // (The branch comes behind the first weights: they do not wait for the maxima.)
 #pragma unroll
-  for (int qt = 0; qt < QT; ++qt) {
-    const float neg_m = -R.m[qt];
+  for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
-    for (int kt = 0; kt < 4; ++kt)
+    for (int qt = 0; qt < QT; ++qt)
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        pt[qt][kt >> 1][(kt & 1) * 4 + i] = (__bf16)__builtin_amdgcn_exp2f(fmaf(s[qt][kt][i], scale, neg_m));
-    R.L[qt] = mfma16x16x32(ones, pt[qt][0], FIRST ? f32x4_t{0.f, 0.f, 0.f, 0.f} : R.L[qt]);
-    R.L[qt] = mfma16x16x32(ones, pt[qt][1], R.L[qt]);
+      for (int i = 0; i < 4; ++i) weight(qt, kt, i);
+  if (!FIRST && __ballot(past)) {
+    __builtin_amdgcn_s_setprio(0);
+    return false;
   }
-  __builtin_amdgcn_s_setprio(0);
+#pragma unroll
+  for (int qt = 0; qt < QT; ++qt) R.L[qt] = mfma16x16x32(ones, pt[qt][0], FIRST ? f32x4_t{0.f, 0.f, 0.f, 0.f} : R.L[qt]);
 #pragma unroll
   for (int dt = 0; dt < 4; ++dt) {
-    const uint4 v0 = v(dt, 0), v1 = v(dt, 1);
+    const uint4 v0 = v(dt, 0);
 #pragma unroll
     for (int qt = 0; qt < QT; ++qt) {
       R.O[qt][dt] = mfma16x16x32(as_bf16x8(v0), pt[qt][0], FIRST ? f32x4_t{0.f, 0.f, 0.f, 0.f} : R.O[qt][dt]);
-      R.O[qt][dt] = mfma16x16x32(as_bf16x8(v1), pt[qt][1], R.O[qt][dt]);
+#pragma unroll
+      for (int i = 0; i < 2; ++i) weight(dt & 1, 2 + (dt >> 1), 2 * qt + i);
     }
+  }
+  __builtin_amdgcn_s_setprio(0);
+#pragma unroll
+  for (int qt = 0; qt < QT; ++qt) R.L[qt] = mfma16x16x32(ones, pt[qt][1], R.L[qt]);
+#pragma unroll
+  for (int dt = 0; dt < 4; ++dt) {
+    const uint4 v1 = v(dt, 1);
+#pragma unroll
+    for (int qt = 0; qt < QT; ++qt) R.O[qt][dt] = mfma16x16x32(as_bf16x8(v1), pt[qt][1], R.O[qt][dt]);
   }
   return true;
 }
@@ -873,7 +888,7 @@ __device__ __forceinline__ void sh_tile_item(const ShEntry& e, int run, int kv_h
   // a block by the straight-line code: false if it has to be done by the long one (its successor's loads are out by then)
   auto fast = [&](uint4 (&cur)[2][512], uint4 (&nxt)[2][512], int kb, auto first) __attribute__((always_inline)) {
     if (kb + 64 < key_hi) issue(nxt, kb + 64);
-    if (!sh_fast_block<2, decltype(first)::value>(R, [&](int kt, int st) __attribute__((always_inline)) { return cur[0][kt * 128 + st * 64 + lane]; },
+    if (!sh_fast_block<decltype(first)::value>(R, [&](int kt, int st) __attribute__((always_inline)) { return cur[0][kt * 128 + st * 64 + lane]; },
                                                   [&](int dt, int h) __attribute__((always_inline)) { return cur[1][h * 256 + dt * 64 + lane]; }))
       return false;
     landed();

@@ -479,6 +479,8 @@ def kv_fork(k, v, n_kv_heads, src, dsts, lo, hi, src_k=None, src_v=None):
 
 def _position(p):
     """An int32 that is out of range where p is: what a C int would make of a larger one may be a position."""
+    if type(p) is int and -1 <= p <= 0x7fffffff:  # (most of them: a third of the time)
+        return p
     return min(max(operator.index(p), -1), 0x7fffffff)
 
 
@@ -535,16 +537,14 @@ def pack_shared(q_lens, starts, kv_base, kv_cap, prefix_of, prefix_len, head_dim
     _need_all(dev, ("q_lens", q_lens, i32, (S,)), ("starts", starts, i32, (S,)), ("kv_base", kv_base, torch.int64, (S,)),
               ("kv_cap", kv_cap, i32, (S,)), ("prefix_of", prefix_of, i32, (S,)), ("prefix_len", prefix_len, i32, (n,)))
     max_tokens = _position(max_tokens)
-    at = q_lens.device
     m = max(max_tokens, 0)
     # (one allocation for the int32s: six would cost more than the kernel)
-    ints = torch.empty(2 * S + 2 + 3 * m, dtype=i32, device=at)
-    kv_slot = torch.empty(m, dtype=torch.int64, device=at)
+    ints, kv_slot = q_lens.new_empty(2 * S + 2 + 3 * m), kv_base.new_empty(m)
     p = ints.data_ptr()
     cu, pos, seq, kv_pos, kv_len = p, p + 4 * (S + 1), p + 4 * (S + 1 + m), p + 4 * (S + 1 + 2 * m), p + 4 * (S + 1 + 3 * m)
     _on(dev, lib().flyai_pack_shared, q_lens.data_ptr(), starts.data_ptr(), kv_base.data_ptr(), kv_cap.data_ptr(), prefix_of.data_ptr(),
         prefix_len.data_ptr(), S, n, _position(head_dim), max_tokens, cu, pos, seq, kv_pos, kv_slot.data_ptr(), kv_len, kv_len + 4 * S)
-    cu, pos, seq, kv_pos, kv_len, status = ints.split((S + 1, m, m, m, S, 1))
+    cu, pos, seq, kv_pos, kv_len, status = ints.split_with_sizes((S + 1, m, m, m, S, 1))
     return dict(cu_seqlens=cu, positions=pos, seq_id=seq, kv_pos=kv_pos, kv_len=kv_len, kv_slot=kv_slot, status=status)
 
 
@@ -559,7 +559,7 @@ class AttnSharedPlan:
 
     @property
     def status(self):
-        return self.buffer[12:16].view(torch.int32)
+        return self.buffer[3:4]
 
 
 @functools.lru_cache(maxsize=256)
@@ -580,7 +580,7 @@ def attn_shared_plan(q_lens, starts, kv_base, kv_cap, prefix_of, prefix_len, pre
               ("prefix_base", prefix_base, i64, (n,)), ("prefix_cap", prefix_cap, i32, (n,)))
     T, Hkv, window = _position(n_tokens), _position(n_kv_heads), _position(window)
     size, _ = _attn_shared_bytes(T, S, n, Hkv)
-    plan = AttnSharedPlan(torch.empty(max(size, 16), dtype=torch.uint8, device=q_lens.device), T, S, n, Hkv, window, operator.index(pool_elems))
+    plan = AttnSharedPlan(q_lens.new_empty(max(size // 4, 4)), T, S, n, Hkv, window, operator.index(pool_elems))
     _on(dev, lib().flyai_attn_shared_plan, q_lens.data_ptr(), starts.data_ptr(), kv_base.data_ptr(), kv_cap.data_ptr(),
         prefix_of.data_ptr(), prefix_len.data_ptr(), prefix_base.data_ptr(), prefix_cap.data_ptr(), S, n, Hkv, window, T,
         plan.pool_elems, plan.buffer.data_ptr())
@@ -596,7 +596,7 @@ def attn_shared(q, k_pool, v_pool, sinks, plan, out=None):
     T, Hkv = plan.n_tokens, plan.n_kv_heads
     dev, bf16 = q.get_device(), torch.bfloat16
     _need_all(dev, ("q", q, bf16, (T, 8 * Hkv, 64)), ("k_pool", k_pool, bf16, k_pool.shape), ("v_pool", v_pool, bf16, k_pool.shape),
-              ("sinks", sinks, torch.float32, (8 * Hkv,)), ("plan", plan.buffer, torch.uint8, plan.buffer.shape))
+              ("sinks", sinks, torch.float32, (8 * Hkv,)), ("plan", plan.buffer, torch.int32, plan.buffer.shape))
     if k_pool.numel() < plan.pool_elems:
         raise ValueError(f"the pools have {k_pool.numel()} elements, the plan was made for {plan.pool_elems}")
     if out is None:
@@ -604,7 +604,7 @@ def attn_shared(q, k_pool, v_pool, sinks, plan, out=None):
     else:
         _need_all(dev, ("out", out, bf16, q.shape))
     _, size = _attn_shared_bytes(T, plan.n_seqs, plan.n_prefixes, Hkv)
-    ws = torch.empty(max(size, 16), dtype=torch.uint8, device=q.device)
+    ws = sinks.new_empty(max(size // 4, 4))
     _on(dev, lib().flyai_attn_shared, q.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), sinks.data_ptr(), 8 * Hkv, Hkv, 64, T,
         plan.n_seqs, plan.n_prefixes, plan.buffer.data_ptr(), ws.data_ptr(), out.data_ptr())
     return out
@@ -790,7 +790,7 @@ def sample_rows(logits, temp, top_k=0, top_p=1.0, draft=None, u=None, want_p_dra
 
 @functools.lru_cache(maxsize=256)
 def _spec_verify_bytes(R, V, S):
-    return max(8, int(lib().flyai_spec_verify_workspace_bytes(R, V, S)))
+    return int(lib().flyai_spec_verify_workspace_bytes(R, V, S)) + 15
 
 
 def spec_verify(logits, cu_rows, draft, u, u_draw, temp, top_k=0, top_p=1.0, draft_probs=None, probs_row=None):
@@ -827,11 +827,8 @@ def spec_verify(logits, cu_rows, draft, u, u_draw, temp, top_k=0, top_p=1.0, dra
         raise ValueError("probs_row without draft_probs")
     if probs_row is not None:
         _need_all(dev, ("probs_row", probs_row, i32, (R,)))
-    at = logits.device
-    tokens = torch.empty(R, dtype=i32, device=at)
-    counts = torch.empty(S, dtype=i32, device=at)
-    p = torch.empty(R, dtype=f32, device=at)
-    ws = torch.empty(_spec_verify_bytes(R, V, S), dtype=torch.uint8, device=at)
+    tokens, counts, p = draft.new_empty(R), draft.new_empty(S), draft.new_empty(R, dtype=f32)
+    ws = u.new_empty(_spec_verify_bytes(R, V, S) // 8)
     _on(dev, lib().flyai_spec_verify, logits.data_ptr(), R, V, cu_rows.data_ptr(), S, draft.data_ptr(), u.data_ptr(), u_draw.data_ptr(),
         _address(params[0]), _address(params[1]), _address(params[2]), float(temp), _position(top_k), float(top_p), _address(draft_probs), n,
         _address(probs_row), tokens.data_ptr(), counts.data_ptr(), p.data_ptr(), ws.data_ptr())

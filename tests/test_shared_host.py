@@ -89,7 +89,7 @@ def test_arguments_of_the_ops():
                    dict(draft_probs=f(torch.float32, 2, 100), probs_row=i32(3))):
         with pytest.raises((ValueError, TypeError)):
             ops.spec_verify(**{**good, **change})
-    plan = ops.AttnSharedPlan(torch.zeros(64, dtype=torch.uint8), 8, 3, 2, 1, 0, 4096)
+    plan = ops.AttnSharedPlan(torch.zeros(64, dtype=torch.int32), 8, 3, 2, 1, 0, 4096)
     q, pool = f(torch.bfloat16, 8, 8, 64), f(torch.bfloat16, 4096)
     for change in (dict(q=q[:7]), dict(q=q.float()), dict(k_pool=pool[:4000]), dict(v_pool=pool[:100]), dict(sinks=f(torch.float32, 7)), dict(out=q[:4])):
         args = dict(q=q, k_pool=pool, v_pool=pool, sinks=f(torch.float32, 8), plan=plan, out=None)

@@ -24,9 +24,13 @@ constexpr int kShRowTokens = 16;      // tokens of a prefix item's tile (4 waves
 constexpr int kShWaveTokens = 2;      // tokens of a wave item
 constexpr int kShWaveSeq = 4;         // the most new tokens of a sequence whose own keys go to waves; more go to tiles
 constexpr int kShMaxSeqs = 4096, kShMaxPrefixes = 1024;
-constexpr int kShChunks = 24;         // a prefix's chunks: at most this many
-constexpr int kShMinChunk = 384, kShChunkStep = 192;  // (few positions are cut finer: their items are latency)
-constexpr int kShOwnChunk = 192;
+// A prefix's chunks: up to 16, or up to 24 where they would have more than 1,152 positions, of 384 positions at least (192 behind up
+// to 1,536).  Finer ones give few rows more workgroups, coarser ones leave fewer records.  With 24 throughout, 32 streams' drafts behind
+// 16,000 positions take 97 us in place of 90; with 16 throughout, 3 streams behind 32,000 take 41 in place of 33; with 768 at least, 8
+// streams behind 4,000 take 24 in place of 20 (and 100 behind 6,000 51 in place of 54).
+constexpr int kShChunks = 16, kShMoreChunks = 24, kShMoreFrom = 1152;
+constexpr int kShMinChunk = 384, kShChunkStep = 192;
+constexpr int kShOwnChunk = 384;  // (192: two to three percent slower with some hundred own positions a stream)
 constexpr int kShSpareEntries = 1024;  // list entries beyond one for each tile, for prefixes split by chunks
 constexpr int kShSpareWaves = 2048;    // ... and beyond one for each group of a sequence's tokens
 constexpr int kShSpareRecs = 8192;     // records beyond two for each token
@@ -125,7 +129,8 @@ __device__ __forceinline__ void sh_excl_scan(int (&v)[N], int (&total)[N], int (
 }
 
 __device__ __forceinline__ int sh_prefix_chunk(int P) {
-  const int c = ((P + kShChunks - 1) / kShChunks + kShChunkStep - 1) / kShChunkStep * kShChunkStep;
+  auto part = [&](int n) { return ((P + n - 1) / n + kShChunkStep - 1) / kShChunkStep * kShChunkStep; };
+  const int few = part(kShChunks), more = part(kShMoreChunks), c = max(min(few, kShMoreFrom), more);
   const int least = P <= 8 * kShChunkStep ? kShChunkStep : kShMinChunk;
   return c > least ? c : least;
 }

@@ -34,6 +34,7 @@ constexpr int kShOwnChunk = 384;  // (192: two to three percent slower with some
 constexpr int kShSpareEntries = 1024;  // list entries beyond one for each tile, for prefixes split by chunks
 constexpr int kShSpareWaves = 2048;    // ... and beyond one for each group of a sequence's tokens
 constexpr int kShSpareRecs = 8192;     // records beyond two for each token
+constexpr int kShRecCost = 600;       // what a chunk's records cost, in positions
 constexpr int kShGrid = 512;           // workgroups on the chip at once: two a CU
 // workgroups of a kv head: head g's are those with blockIdx % Hkv == g, with 8 heads an XCD each, so that its L2 holds one head's keys
 __host__ __device__ constexpr int sh_per_head(int Hkv) { return kShGrid / Hkv > 0 ? kShGrid / Hkv : 1; }
@@ -300,11 +301,15 @@ __global__ __launch_bounds__(NT) void attn_shared_plan_kernel(ShBatch b, char* _
     tiles = few ? 1 : (np + kShRowTokens - 1) / kShRowTokens;
   }
   // listed tokens; tiles of workgroups; entries of waves whole and by chunks, their records by chunks
-  int ps[5] = {np, few ? 0 : tiles, few ? tiles : 0, few ? tiles * chunks : 0, few ? np * chunks : 0}, n_ps[5];
-  sh_excl_scan<NT, 5>(ps, n_ps, red);
-  // As many whole tiles as give every workgroup the same number; the rest by chunks, if the lists and the records hold them.
+  int ps[6] = {np, few ? 0 : tiles, few ? tiles : 0, few ? tiles * chunks : 0, few ? np * chunks : 0, few ? 0 : tiles * min(C, 4096)}, n_ps[6];
+  sh_excl_scan<NT, 6>(ps, n_ps, red);
+  // As many whole tiles as give every workgroup the same number; the rest by chunks, if the lists and the records hold them.  A chunk of C
+  // positions costs what C + kShRecCost would without its records, so the rest stays whole where its chunks would take longer than a
+  // round that not all workgroups have a tile in: with 43 and 92 tiles of 4,099 positions (64 workgroups) 110 and 164 us whole, 119 and
+  // 175 by chunks; with 23 and 84 77 and 165, 71 and 158.
   const int per_head = sh_per_head(b.Hkv);
   int whole = n_ps[1] / per_head * per_head;
+  if ((int64_t)(n_ps[1] - whole) * (n_ps[5] + (int64_t)kShRecCost * n_ps[1]) > (int64_t)per_head * n_ps[5]) whole = n_ps[1];
   auto split_of = [&](int w) __attribute__((always_inline)) { return few ? 0 : max(0, ps[1] + tiles - max(ps[1], w)); };
   int split = split_of(whole), split_tokens = np > 0 ? min(np, np - (tiles - split) * kShRowTokens) : 0;
   if (!split) split_tokens = 0;

@@ -33,7 +33,7 @@ constexpr int kShMinChunk = 384, kShChunkStep = 192;
 constexpr int kShOwnChunk = 384;  // (192: two to three percent slower with some hundred own positions a stream)
 constexpr int kShSpareEntries = 1024;  // list entries beyond one for each tile, for prefixes split by chunks
 constexpr int kShSpareWaves = 2048;    // ... and beyond one for each group of a sequence's tokens
-constexpr int kShSpareRecs = 8192;     // records beyond two for each token
+constexpr int kShSpareRecs = 16384, kShSpareRecsOfToken = 256;  // records beyond two for each token: so many for a token, and at most
 constexpr int kShRecCost = 600;       // what a chunk's records cost, in positions
 constexpr int kShGrid = 512;           // workgroups on the chip at once: two a CU
 // workgroups of a kv head: head g's are those with blockIdx % Hkv == g, with 8 heads an XCD each, so that its L2 holds one head's keys
@@ -81,7 +81,7 @@ __host__ __device__ inline ShLayout sh_layout(int T, int S, int n_prefix) {
   l.max_entries = 2 * (T / kShRowTokens) + (n_prefix < T ? n_prefix : T) + T / (kShWaveSeq + 1) + kShSpareEntries;
   // the other sequences' groups, and the prefixes whose few tokens go to waves
   l.max_waves = T / kShWaveTokens + (S < T ? S : T) + (n_prefix < T ? n_prefix : T) + kShSpareWaves;
-  l.max_recs = 2 * T + kShSpareRecs;
+  l.max_recs = 2 * T + (T < kShSpareRecs / kShSpareRecsOfToken ? T * kShSpareRecsOfToken : kShSpareRecs);
   size_t o = sizeof(ShHeader);
   l.o_entries = o;
   o += (size_t)l.max_entries * sizeof(ShEntry);

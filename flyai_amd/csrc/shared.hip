@@ -65,18 +65,22 @@ struct ShToken {  // where a token's records lie: n of them, stride apart
 // The units of workgroups: whole prefix tiles, then chunks of prefix tiles, then the sequences' own tiles; and those of waves.
 struct ShHeader {
   int32_t n_whole, n_split, n_own, status;
-  int32_t n_waves, n_tokens, window, pad[9];
+  int32_t n_waves, n_tokens, window;
+  int32_t T, S, n_prefix, Hkv;  // what the plan was made for
+  int32_t pad[5];
 };
 
 // Byte layout of a plan, and how much each list holds at most.
 struct ShLayout {
-  int32_t T, max_entries, max_waves, max_recs;
+  int32_t T, S, n_prefix, max_entries, max_waves, max_recs;
   size_t o_entries, o_waves, o_list, o_tokens, bytes;
 };
 
 __host__ __device__ inline ShLayout sh_layout(int T, int S, int n_prefix) {
   ShLayout l;
   l.T = T;
+  l.S = S;
+  l.n_prefix = n_prefix;
   // the prefixes' tiles, those of the sequences with more than kShWaveSeq tokens
   l.max_entries = 2 * (T / kShRowTokens) + (n_prefix < T ? n_prefix : T) + T / (kShWaveSeq + 1) + kShSpareEntries;
   // the other sequences' groups, and the prefixes whose few tokens go to waves
@@ -93,6 +97,11 @@ __host__ __device__ inline ShLayout sh_layout(int T, int S, int n_prefix) {
   o += (size_t)T * sizeof(ShToken);
   l.bytes = (o + 255) & ~(size_t)255;
   return l;
+}
+
+// a plan of another shape has its lists elsewhere: nothing is done with it
+__device__ __forceinline__ bool sh_plan_fits(const ShHeader* h, const ShLayout& L, int Hkv) {
+  return h->T == L.T && h->S == L.S && h->n_prefix == L.n_prefix && h->Hkv == Hkv;
 }
 
 // ---- the plan -------------------------------------------------------------------------------------
@@ -150,7 +159,7 @@ struct ShBatch {
 enum { kShPastSlab = 1, kShPastTokens = 2, kShBeforePrefix = 4, kShBadPrefix = 8, kShBadSequence = 16 };
 
 __device__ __forceinline__ bool sh_slab_ok(int64_t base, int cap, int Hkv, int64_t pool) {
-  return cap > 0 && cap % 64 == 0 && base >= 0 && base % 8 == 0 && base <= pool - (int64_t)Hkv * cap * 64;
+  return cap > 0 && cap <= (1 << 30) && cap % 64 == 0 && base >= 0 && base % 8 == 0 && base <= pool - (int64_t)Hkv * cap * 64;
 }
 
 // What the plan keeps of a sequence and of a prefix, in LDS.
@@ -362,6 +371,10 @@ __global__ __launch_bounds__(NT) void attn_shared_plan_kernel(ShBatch b, char* _
     hdr->n_waves = few_waves + (osplit ? n_seqs[2] : n_seqs[0]);
     hdr->n_tokens = n_tokens;
     hdr->window = b.window;
+    hdr->T = b.T;
+    hdr->S = b.S;
+    hdr->n_prefix = b.n_prefix;
+    hdr->Hkv = b.Hkv;
   }
   __syncthreads();
   if (tid == 0) hdr->status = status_s;
@@ -979,6 +992,7 @@ __global__ __launch_bounds__(256, 2) void attn_shared_kernel(const uint16_t* __r
   const ShEntry* waves = reinterpret_cast<const ShEntry*>(plan + L.o_waves);
   const int2* list = reinterpret_cast<const int2*>(plan + L.o_list);
   const int per_head = gridDim.x / Hkv, w = blockIdx.x / Hkv, g = blockIdx.x % Hkv;
+  if (!sh_plan_fits(hdr, L, Hkv)) return;
   const int n_whole = hdr->n_whole, n_split = hdr->n_split, n_own = hdr->n_own, n_waves = hdr->n_waves, window = hdr->window;
   auto tile = [&](int i, int run) __attribute__((always_inline)) {
     const ShEntry e = entries[i];
@@ -1021,8 +1035,8 @@ __global__ __launch_bounds__(128) void attn_shared_merge_kernel(const float* __r
                                                                 const float* __restrict__ sinks, int Hq, int Hkv, uint16_t* __restrict__ out) {
   const ShHeader* hdr = reinterpret_cast<const ShHeader*>(plan);
   const int t = blockIdx.x, g = blockIdx.y;
-  const ShToken k = reinterpret_cast<const ShToken*>(plan + L.o_tokens)[t];  // (of a row behind the last sequence: whatever is there, not used)
-  if (t >= hdr->n_tokens) return;  // left as it was
+  if (t >= hdr->n_tokens || !sh_plan_fits(hdr, L, Hkv)) return;  // left as it was
+  const ShToken k = reinterpret_cast<const ShToken*>(plan + L.o_tokens)[t];
   float* parts = const_cast<float*>(parts_in);
   const int h = threadIdx.x >> 4, part = threadIdx.x & 15;
   const float sink = sinks[g * 8 + h] * kLog2e;

@@ -254,3 +254,41 @@ def test_positions_past_32_bits_of_elements():
                   pool_elems=k.numel())
     got = ops.attn_shared(b.q.to(DEV), k, v, b.sinks.to(DEV), plan)
     assert got.equal(want)
+
+
+def test_a_plan_of_another_shape():
+    """Nothing is done with it."""
+    b = Batch([130], [(2, 70, 0), (1, 3, 0), (9, 100, 0)], Hkv=2, seed=4)
+    plan = b.plan(0)
+    q, sinks = b.q.to(DEV), b.sinks.to(DEV)
+    for change in (dict(n_tokens=b.T - 1), dict(n_seqs=2), dict(n_prefixes=0), dict(n_kv_heads=1)):
+        other = ops.AttnSharedPlan(**{**{n: getattr(plan, n) for n in plan.__slots__}, **change})
+        T, Hkv = other.n_tokens, other.n_kv_heads
+        out = torch.full((T, 8 * Hkv, 64), 7.0, dtype=torch.bfloat16, device=DEV)
+        ops.attn_shared(q[:T, :8 * Hkv].contiguous(), b.k, b.v, sinks[:8 * Hkv].contiguous(), other, out=out)
+        assert bool((out == 7).all()), change
+
+
+@pytest.mark.parametrize("window", [0, 5000])
+@pytest.mark.parametrize("P", [6145, 18433, 18432, 27700, 33000])
+def test_long_prefixes(P, window):
+    """Chunks of other lengths, and own keys of several chunks."""
+    b = Batch([P], [(1, 900, 0), (3, 0, 0), (9, 385, 0)], Hkv=1, seed=P)
+    got, plan = b.run(window)
+    assert int(plan.status) == 0
+    check(got, *b.expected(window))
+
+
+@pytest.mark.parametrize("n", [1, 40, 65, 90])
+def test_tiles_and_rounds(n):
+    """Tiles that fill no round of the workgroups, more than one, and whole or split rests: every row's bits are those that its sequence
+    has in a batch of its own."""
+    b = Batch([1600], [(16, 3 * i % 70, 0) for i in range(n)], Hkv=8, seed=n)
+    got, _ = b.run(0)
+    alone = Batch.__new__(Batch)
+    alone.__dict__.update(b.__dict__)
+    for i in {0, n // 2, n - 1}:
+        alone.seqs, alone.q_lens, alone.starts, alone.prefix_of = ([x[i]] for x in (b.seqs, b.q_lens, b.starts, b.prefix_of))
+        alone.q, alone.T = b.q[16 * i:16 * i + 16], 16
+        alone.bases, alone.caps = [*b.bases[:1], b.bases[1 + i], None], [b.caps[0], b.caps[1 + i]]
+        assert alone.run(0)[0].equal(got[16 * i:16 * i + 16]), i

@@ -24,7 +24,7 @@ namespace flyai {
 
 struct VerRow {
   uint64_t W;         // kept weight
-  uint64_t tie_keep;  // ties at `edge` that are kept, in id order
+  uint64_t tie_keep;  // ties at `edge` that are kept, in id order; ~0: all
   float zmax;
   float lo, edge;     // kept are values from lo (top-k) and edge (top-p) on, -inf: no such bound; values of x, or of z = x / temp (by_z)
   int32_t by_z;
@@ -467,8 +467,9 @@ __device__ __forceinline__ bool ver_row_counts(const VerArgs& a, int row, const 
         if (lane == k) {
           const uint64_t above = incl - m * w;
           h.edge = v;
-          h.tie_keep = min((uint64_t)m, (T - above) / w + 1);
-          h.weight = above + h.tie_keep * w;
+          const uint64_t keep = min((uint64_t)m, (T - above) / w + 1);
+          h.tie_keep = keep == m ? ~0ull : keep;
+          h.weight = above + keep * w;
         }
       }
       __syncthreads();
@@ -482,9 +483,22 @@ __device__ __forceinline__ bool ver_row_counts(const VerArgs& a, int row, const 
   if (d >= 0) {
     const float v = bf2f(dbits);
     bool in = v >= o.lo && v >= o.edge;
-    if (in && use_p && v == o.edge) {  // a tie at the border: its rank in id order (uniform)
+    if (in && use_p && v == o.edge && o.tie_keep != ~0ull) {  // a tie at the border: its rank in id order (uniform)
+      // (the ids before it as the row is read; two values of a word at once, -0 the same as +0)
       uint32_t c = 0;
-      for (int i = tid; i < d; i += kSampThreads) c += bf2f(x[i]) == v;
+      const int whole = d & ~7;
+      const uint32_t one = (dbits & 0x7fff) ? 0xffff : 0x7fff, mask = one | one << 16, want = (dbits | (uint32_t)dbits << 16) & mask;
+      auto count = [&](uint32_t w) __attribute__((always_inline)) {
+        const uint32_t t = (w & mask) ^ want;
+        c += ((t & 0xffffu) == 0) + (t >> 16 == 0);
+      };
+      ver_each(x, whole, ver_load(x, tid * 8, whole), [&](int, u32x4_t w) {
+        count(w.x);
+        count(w.y);
+        count(w.z);
+        count(w.w);
+      });
+      if (whole + tid < d) c += bf2f(x[whole + tid]) == v;
       c = wave_total(c);
       if (lane == 0 && c) atomicAdd(&h.before, c);
       __syncthreads();
@@ -668,11 +682,13 @@ __global__ __launch_bounds__(kPieceThreads, 4) void verify_pieces_kernel(VerArgs
         }
       }
     }
-    above = wave_total(above);
-    if (r.edge > -INFINITY) {  // uniform
+    const bool apart = r.tie_keep != ~0ull;  // some ties are kept and some are not (uniform)
+    above = wave_total(apart ? above : above + tie);
+    if (apart) {
       tie = wave_total(tie);
       ties = wave_total(ties);
-    } else {  // (ties with -inf are none)
+    } else {
+      tie = 0;
       ties = 0;
     }
     if (lane == 0) pieces[(size_t)s * a.pieces + c] = {(uint64_t)above, (uint64_t)tie, ties, 0};
@@ -712,7 +728,7 @@ __global__ __launch_bounds__(kPiece) void verify_draw_kernel(VerArgs a, const Ve
     const int v = c * kPiece + tid;
     bool tie = false;
     double k = v < a.V ? w.kept(w.x[v], &tie) : 0.0;
-    if (r.edge > -INFINITY) {  // uniform
+    if (r.tie_keep != ~0ull) {  // uniform
       uint64_t n;
       const uint64_t rank = before + block_excl_scan<kPiece>((uint64_t)tie, red, &n);
       if (tie && rank >= r.tie_keep) k = 0.0;
@@ -725,7 +741,7 @@ __global__ __launch_bounds__(kPiece) void verify_draw_kernel(VerArgs a, const Ve
   const int per = (a.pieces + kPiece - 1) / kPiece, c0 = min(a.pieces, tid * per), c1 = min(a.pieces, c0 + per);
   uint64_t ties = 0, all;
   for (int c = c0; c < c1; ++c) ties += mine[c].ties;
-  const uint64_t ties0 = r.edge > -INFINITY ? block_excl_scan<kPiece>(ties, red, &all) : 0;
+  const uint64_t ties0 = r.tie_keep != ~0ull ? block_excl_scan<kPiece>(ties, red, &all) : 0;
   uint64_t t = ties0;
   __syncthreads();
   for (int c = c0; c < c1; ++c) {

@@ -299,3 +299,21 @@ def test_sampler_accept_batch(temp, top_k, top_p, probs):
         sm.accept_batch(c.logits.to(DEV), lists[:-1])
     with pytest.raises(ValueError):
         sm.accept_batch(c.logits.to(DEV), [[1000, 0, 0], *lists[1:]])
+
+
+@pytest.mark.parametrize("value", [0.0, 1.5])
+@pytest.mark.parametrize("V", [5000, 20003])
+def test_drafts_that_are_ties_at_the_border(V, value):
+    """Half of the ids share the border's value (as +0 and -0 too): a draft among them is kept by its rank in id order."""
+    c = Case(V, [2] * 12, [(1.0, 0, np.float32(0.5))] * 12, seed=3, probs="none")
+    rng = np.random.default_rng(V)
+    x = np.full(c.logits.shape, -1.0, dtype=np.float32)
+    ties = np.sort(rng.permutation(V)[:V // 2])
+    x[:, ties] = np.where(rng.random(len(ties)) < 0.5, value, -value if value == 0 else value)
+    c.logits = torch.from_numpy(x).to(torch.bfloat16)
+    w = np.float64(V // 2) + (V - V // 2) * np.exp(-1.0 - value)
+    keep = int(0.5 * w)  # about: the ids around the last that is kept
+    c.draft[::2] = ties[[0, 1, 7, keep // 2, *range(keep - 4, keep + 4)]]
+    c.u[:] = 0.0
+    c.check()
+    assert 0 < len(set(c.expected()[1].tolist())) <= 2

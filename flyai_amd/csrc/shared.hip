@@ -14,6 +14,14 @@
 //
 // The work lists are made on the GPU (attn_shared_plan_kernel), once for a step's layers: the host needs
 // no lengths, only bounds, and the grids are sized by those.
+//
+// What bounds it: with many rows instruction issue.  A wave's block (32 rows, 64 keys) is 36 matrix instructions (576 clocks at their
+// peak rate) and 32 exponentials, 32 fused multiply-adds, 16 maxima of three and 16 conversions (some 770): with two waves a SIMD the
+// larger of the two if nothing were in the way.  256 streams of up to 4 tokens behind 32,749 positions (554 GFLOP) take 603 to 618 us,
+// 0.9 PFLOP/s (a library's large product: 1.43); six questions of up to 300 tokens behind 4,099 (102 GFLOP) 164.  With few rows the
+// chain of a unit -- entry, token list, queries, then 0.65 us a block where the SIMD has one wave -- and the launches: 48 streams behind
+// 8,000 positions 32 us, of which the plan's 6, the items' 19 and the merge's 5; 2 streams behind 513 21 (6, 6 and 3; the host's two calls
+// are as long).  Three waves a SIMD (168 registers) and three buffers in turn were slower than two.
 #include <type_traits>
 
 #include "attn.h"
@@ -22,7 +30,9 @@ namespace flyai {
 
 constexpr int kShRowTokens = 16;      // tokens of a prefix item's tile (4 waves x 2 tiles of 16 rows x 2 tokens)
 constexpr int kShWaveTokens = 2;      // tokens of a wave item
-constexpr int kShWaveSeq = 4;         // the most new tokens of a sequence whose own keys go to waves; more go to tiles
+// The most new tokens of a sequence whose own keys go to waves; more go to tiles (32 streams of up to 8 tokens: 80.3 us with 4, 81.9
+// with 8, 79.7 with 1, which costs batches of two-token chunks a tile of 16 rows each).
+constexpr int kShWaveSeq = 4;
 constexpr int kShMaxSeqs = 4096, kShMaxPrefixes = 1024;
 // A prefix's chunks: up to 16, or up to 24 where they would have more than 1,152 positions, of 384 positions at least (192 behind up
 // to 1,536).  Finer ones give few rows more workgroups, coarser ones leave fewer records.  With 24 throughout, 32 streams' drafts behind
@@ -184,10 +194,11 @@ struct ShPrefixes {
 };
 constexpr int kShMaxOwnChunks = 4096;  // of a sequence, for the counts to stay in 32 bits: past it no sequence is split
 
-// One workgroup, so that nothing but LDS lies between the counts and the lists: one round trip for the lengths, three sums over the
+// Made by one workgroup, so that nothing but LDS lies between the counts and the lists: one round trip for the lengths, three sums over the
 // workgroup, the lists.  A prefix's tokens are listed in the order in which its sequences' counts arrive at an LDS counter: which rows
 // share a tile may change from launch to launch, a row's result does not (no row's steps depend on its tile mates).
-// Small batches have a workgroup of their own size: fewer waves at each barrier, and half the code to fetch.
+// Small batches have a workgroup of their own size, with fewer waves at each barrier and half the code to fetch: 5.8 us in place of 7.5
+// with 2 sequences; 256 sequences of 1,000 tokens take the large one, 9.3.
 template <int NT, int PER>
 __global__ __launch_bounds__(NT) void attn_shared_plan_kernel(ShBatch b, char* __restrict__ plan) {
   const ShLayout L = sh_layout(b.T, b.S, b.n_prefix);
@@ -1027,7 +1038,8 @@ __global__ __launch_bounds__(256, 2) void attn_shared_kernel(const uint16_t* __r
 }
 
 // The records of a token's 8 rows of a kv head, folded: the prefix's, the sequence's own, then both and the sink.  Thread (h = tid / 16,
-// part = tid % 16) takes 4 dims, with kShMergeAhead records' loads out at once (one round trip to memory for most tokens).  A token
+// part = tid % 16) takes 4 dims, with kShMergeAhead records' loads out at once (one round trip to memory for most tokens): 4.9 us for 48
+// tokens of 14 + 1 records a head, 13 us for 1,478 of two.  A token
 // without any record (its sequence was refused) gets zeros.
 constexpr int kShMergeAhead = 12;
 

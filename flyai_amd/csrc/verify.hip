@@ -16,6 +16,12 @@
 // Three launches: verify_rows_kernel finds each row's filter, W, and whether its draft is accepted; a stream's first row that
 // is not is then the only one whose weights are needed one by one: verify_pieces_kernel sums w' over pieces of its ids, and
 // verify_draw_kernel finds the piece and the id, and writes what comes out.
+//
+// With a vocabulary of 201,088 (us): 128 streams' 1,152 rows 159, of which the rows 116 (463 MB, 4.0 TB/s; a copy's read side reaches 6.3),
+// the pieces 36, the draw 7; 24 streams' 120 rows 48 (30, 11, 7); one stream's 5 rows 35 (24, 6, 5), where a row is one CU's: 14 us
+// of counting in LDS, some 10 of sums over the values.  The rows that many passes over the logits took (ver_row_general's way for all)
+// were 1,215 us of 128 streams, 482 of one.  Rows counted in up to eight parts, then added up, made one stream's 32 us and 24 streams' 53;
+// a workgroup a CU with the next row's loads ahead 205 of 128 streams' 159.
 #include <algorithm>
 
 #include "sample.h"
@@ -514,6 +520,7 @@ __device__ __forceinline__ bool ver_row_counts(const VerArgs& a, int row, const 
   return true;
 }
 
+// A row a workgroup, two workgroups a CU: one's counting hides part of the other's sums.
 __global__ __launch_bounds__(kSampThreads, 8) void verify_rows_kernel(VerArgs a, VerRow* __restrict__ rows) {
   __shared__ union { VerHist hist; VerGreedy greedy; SampShared gen; } sh;
   __shared__ int found;
@@ -567,11 +574,12 @@ __device__ __forceinline__ VerWeights ver_weights(const VerArgs& a, int s, int r
 
 // w' of the stop row's pieces, a wave each at a time, the next one's loads in flight.  A piece's sums stay below 2^49 and are exact in
 // doubles.  Without a filter nearly every token has weight: a workgroup with many pieces makes the weights of the common values once
-// (|x| in [2^-24, 2^8)) and looks them up; the others are made one by one.
+// (|x| in [2^-24, 2^8)) and looks them up; the others are made one by one.  128 streams 35 us with the tables (one of 1,024 threads a
+// CU; 47 with four of 256 threads, which make it four times), 73 without; the unfiltered ones among 24 streams 11 and 17.
 constexpr int kVerTable = 32 * 128;      // values of a sign
 constexpr uint32_t kVerTableFirst = 0x3380;  // the bits of 2^-24
 constexpr int kPieceThreads = 1024;
-constexpr int kTablePieces = 32;  // twice as many tokens as the table has values
+constexpr int kTablePieces = 32;  // of a workgroup, for a table: twice as many tokens as it has values
 
 struct __attribute__((packed, aligned(4))) VerVec4 { f32x4_t v; };
 
@@ -695,6 +703,8 @@ __global__ __launch_bounds__(kPieceThreads, 4) void verify_pieces_kernel(VerArgs
   }
 }
 
+// A stream a workgroup: two sums over its pieces, one over the ids of the piece that is hit, and of the one whose ties are kept in part;
+// a chain of round trips (5 to 8 us).
 __global__ __launch_bounds__(kPiece) void verify_draw_kernel(VerArgs a, const VerRow* __restrict__ rows,
                                                              const VerPiece* __restrict__ pieces, int32_t* __restrict__ tokens,
                                                              int32_t* __restrict__ counts, float* __restrict__ p_out) {

@@ -802,7 +802,8 @@ def spec_verify(logits, cu_rows, draft, u, u_draw, temp, top_k=0, top_p=1.0, dra
     acceptances and for each stream's draw.
 
     Returns (tokens int32 [R], counts int32 [S], p fp32 [R]), all on the GPU: in a stream's rows its accepted drafts, then the drawn
-    token, then -1; how many tokens it got; and each token's probability under the filtered target (0 behind the end)."""
+    token, then -1; how many tokens it got; and each token's probability under the filtered target (0 behind the end).  Rows of no stream
+    are not written."""
     R, V = logits.shape
     S = cu_rows.numel() - 1
     if S < 0:

@@ -185,14 +185,14 @@ __device__ __forceinline__ int ver_stream(const VerArgs& a, int row, int* found)
 // ---- a row, 16 bytes a thread at a time ----
 struct __attribute__((packed, aligned(2))) VerVec { u32x4_t v; };  // 16 bytes at any element's address
 
-constexpr int kVerAhead = 2;
-constexpr int kVerBatch = kVerAhead * kSampThreads * 8;
-struct VerLoaded { u32x4_t w[kVerAhead]; };
+template <int AHEAD>
+struct VerLoaded { u32x4_t w[AHEAD]; };
 
-__device__ __forceinline__ VerLoaded ver_load(const uint16_t* __restrict__ x, int v0, int full) {
-  VerLoaded l;
+template <int AHEAD>
+__device__ __forceinline__ VerLoaded<AHEAD> ver_load(const uint16_t* __restrict__ x, int v0, int full) {
+  VerLoaded<AHEAD> l;
 #pragma unroll
-  for (int j = 0; j < kVerAhead; ++j) {
+  for (int j = 0; j < AHEAD; ++j) {
     const int v = v0 + j * kSampThreads * 8;
     l.w[j] = u32x4_t{0, 0, 0, 0};
     if (v < full) l.w[j] = reinterpret_cast<const VerVec*>(x + v)->v;
@@ -201,12 +201,13 @@ __device__ __forceinline__ VerLoaded ver_load(const uint16_t* __restrict__ x, in
 }
 
 // f(first id, its 8 values) over the thread's vectors of [0, full), the next batch's loads in flight; `l` holds the first batch
-template <class F>
-__device__ __forceinline__ void ver_each(const uint16_t* __restrict__ x, int full, VerLoaded l, F&& f) {
-  for (int v0 = (int)threadIdx.x * 8; v0 < full; v0 += kVerBatch) {
-    const VerLoaded next = ver_load(x, v0 + kVerBatch, full);
+template <int AHEAD, class F>
+__device__ __forceinline__ void ver_each(const uint16_t* __restrict__ x, int full, VerLoaded<AHEAD> l, F&& f) {
+  constexpr int kBatch = AHEAD * kSampThreads * 8;
+  for (int v0 = (int)threadIdx.x * 8; v0 < full; v0 += kBatch) {
+    const VerLoaded<AHEAD> next = ver_load<AHEAD>(x, v0 + kBatch, full);
 #pragma unroll
-    for (int j = 0; j < kVerAhead; ++j) {
+    for (int j = 0; j < AHEAD; ++j) {
       const int v = v0 + j * kSampThreads * 8;
       if (v < full) f(v, l.w[j]);
     }
@@ -230,7 +231,8 @@ struct VerGreedy {
   int at;
 };
 
-__device__ __forceinline__ void ver_row_greedy(const VerArgs& a, int row, const VerLoaded& l, VerGreedy& sh, VerRow* out) {
+template <int AHEAD>
+__device__ __forceinline__ void ver_row_greedy(const VerArgs& a, int row, const VerLoaded<AHEAD>& l, VerGreedy& sh, VerRow* out) {
   const uint16_t* x = a.logits + (size_t)row * a.V;
   const int tid = threadIdx.x, V = a.V, full = V & ~7;
   int best = -0x8001, at = V;  // (a thread without a vector: below every value)
@@ -329,13 +331,25 @@ __device__ __forceinline__ T wave_total(T v) {
   return v;
 }
 
-// what there is no place for: counted where it has no weight, else the row is left to the general path
-__device__ __forceinline__ void ver_odd_value(VerHist& h, uint32_t bits) {
-  const uint32_t mag = bits & 0x7fffu;
-  if (mag == 0) atomicAdd(&h.zeros, 1u);
-  else if (mag - kVerFirst < (uint32_t)kVerHalf) atomicAdd(&h.cnt[(mag - kVerFirst) + (bits & 0x8000u ? kVerHalf : 0)], 1u);
-  else if ((bits & 0x8000u) && mag > kVerFirst) atomicMax(&h.low, f32_key(bf2f((uint16_t)bits)));
-  else h.bad = 1;
+// the sum of 16 lanes, in the last of them
+__device__ __forceinline__ uint32_t row_total(uint32_t v) {
+  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, true);  // row_shr:1
+  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, true);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, true);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, true);
+  return v;
+}
+__device__ __forceinline__ uint64_t row_total(uint64_t v) {
+  auto add = [&](uint32_t lo, uint32_t hi) __attribute__((always_inline)) { v += (uint64_t)hi << 32 | lo; };
+#define FLYAI_ROW_STEP(ctrl)                                                            \
+  add(__builtin_amdgcn_update_dpp(0, (uint32_t)v, ctrl, 0xf, 0xf, true), \
+      __builtin_amdgcn_update_dpp(0, (uint32_t)(v >> 32), ctrl, 0xf, 0xf, true))
+  FLYAI_ROW_STEP(0x111);
+  FLYAI_ROW_STEP(0x112);
+  FLYAI_ROW_STEP(0x114);
+  FLYAI_ROW_STEP(0x118);
+#undef FLYAI_ROW_STEP
+  return v;
 }
 
 // The group where the running total of the groups' masses (thread g: group g's, `run` before it) first exceeds limit, to h.group
@@ -351,7 +365,8 @@ __device__ __forceinline__ void ver_find_group(VerHist& h, uint64_t run, uint64_
 }
 
 // false: the row is not one for this path (every thread)
-__device__ __forceinline__ bool ver_row_counts(const VerArgs& a, int row, const VerParams& p, const VerLoaded& l, VerHist& h, VerRow* out) {
+template <int AHEAD>
+__device__ __forceinline__ bool ver_row_counts(const VerArgs& a, int row, const VerParams& p, const VerLoaded<AHEAD>& l, VerHist& h, VerRow* out) {
   const uint16_t* x = a.logits + (size_t)row * a.V;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, V = a.V, d = ver_draft(a, row);
   if (!(p.tdiv < 0x1p60f)) return false;
@@ -365,29 +380,45 @@ __device__ __forceinline__ bool ver_row_counts(const VerArgs& a, int row, const 
   const uint16_t dbits = d >= 0 ? x[d] : 0;
   __syncthreads();
   // (two 16-bit places of a word at once; 0x6000 tells a value without one)
-  auto count = [&](uint32_t w) __attribute__((always_inline)) {
-    typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
-    u16x2 t2 = __builtin_bit_cast(u16x2, w);
-    t2 -= (u16x2){(unsigned short)kVerFirst, (unsigned short)kVerFirst};
-    const uint32_t t = __builtin_bit_cast(uint32_t, t2);
-    if (t & 0x60006000u) {
-      ver_odd_value(h, w & 0xffffu);
-      ver_odd_value(h, w >> 16);
-      return;
-    }
+  auto count = [&](uint32_t t) __attribute__((always_inline)) {
     const uint32_t at = ((t << 2) & 0x7ffc7ffcu) | (t & 0x80008000u);  // byte addresses
     char* c = reinterpret_cast<char*>(h.cnt);
     atomicAdd(reinterpret_cast<uint32_t*>(c + (at & 0xffffu)), 1u);
     atomicAdd(reinterpret_cast<uint32_t*>(c + (at >> 16)), 1u);
   };
+  // a value that may have no place: one that has no weight is left out (`low` is the largest one's magnitude), another one leaves the
+  // row to the general path
+  uint32_t zeros = 0, bad = 0, low = 0xffffu;
+  auto one = [&](uint32_t bits) __attribute__((always_inline)) {
+    const uint32_t mag = bits & 0x7fffu, t = mag - kVerFirst;
+    const bool none = t >= (uint32_t)kVerHalf, neg = bits & 0x8000u;
+    if (!none) atomicAdd(&h.cnt[t + (neg ? kVerHalf : 0)], 1u);
+    zeros += mag == 0;
+    const bool below = none && neg && mag > kVerFirst;
+    low = below ? min(low, mag) : low;
+    bad |= none && !below && mag != 0;
+  };
   const int full = V & ~7;
   ver_each(x, full, l, [&](int, u32x4_t w) {
-    count(w.x);
-    count(w.y);
-    count(w.z);
-    count(w.w);
+    typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+    uint32_t t[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      t[i] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(u16x2, (uint32_t)w[i]) - (u16x2){(unsigned short)kVerFirst, (unsigned short)kVerFirst});
+    if ((t[0] | t[1] | t[2] | t[3]) & 0x60006000u) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) one((i & 1 ? w[i >> 1] >> 16 : w[i >> 1]) & 0xffffu);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) count(t[i]);
+    }
   });
-  if (tid < V - full) ver_odd_value(h, x[full + tid]);
+  if (tid < V - full) one(x[full + tid]);
+  if (__ballot(zeros || bad || low != 0xffffu)) {
+    if (zeros) atomicAdd(&h.zeros, zeros);
+    if (bad) h.bad = 1;
+    if (low != 0xffffu) atomicMax(&h.low, f32_key(bf2f((uint16_t)(low | 0x8000u))));
+  }
   __syncthreads();
   // the values that are there: the largest, then their weights and counts by group
   constexpr int kPer = 2 * kVerHalf / kSampThreads;
@@ -411,21 +442,22 @@ __device__ __forceinline__ bool ver_row_counts(const VerArgs& a, int row, const 
   const bool use_k = p.top_k > 0 && p.top_k < V, use_p = p.top_p > 0.f && p.top_p < 1.f;
 #pragma unroll
   for (int j = 0; j < kPer; ++j) {
-    if (!n[j]) continue;
+    if (!__ballot(n[j])) continue;
     const int i = j * kSampThreads + tid;
     const float v = bf2f((uint16_t)(kVerFirst + (i < kVerHalf ? i : i - kVerHalf + 0x8000)));
-    const uint64_t m = n[j] * samp_weight(__fdiv_rn(v, p.tdiv), zmax);
+    uint64_t m = n[j] ? n[j] * samp_weight(__fdiv_rn(v, p.tdiv), zmax) : 0;
+    // 16 lanes are a group: their sum to the last one
     const int g = i < kVerHalf ? (kVerHalf - 1 - i) >> 4 : i >> 4;
-    if (m) atomicAdd((unsigned long long*)&h.gsum[g], (unsigned long long)m);
-    if (use_k) atomicAdd(&h.gcnt[g], n[j]);
+    m = row_total(m);
+    if ((lane & 15) == 15) h.gsum[g] = m;
+    if (use_k) {
+      const uint32_t c = row_total(n[j]);
+      if ((lane & 15) == 15) h.gcnt[g] = c;
+    }
   }
-  if (tid == 0 && h.zeros) {
-    const uint64_t m = h.zeros * samp_weight(0.f, zmax);
-    atomicAdd((unsigned long long*)&h.gsum[kVerGroups / 2], (unsigned long long)m);
-    atomicAdd(&h.gcnt[kVerGroups / 2], h.zeros);
-  }
+  const bool zero_too = tid == kVerGroups / 2 && h.zeros;  // that group's: zero's besides
   __syncthreads();
-  uint64_t mass = h.gsum[tid], W;
+  uint64_t mass = h.gsum[tid] + (zero_too ? h.zeros * samp_weight(0.f, zmax) : 0), W;
   const uint64_t run = block_excl_scan<kSampThreads>(mass, h.red, &W);
   VerRow o = {};
   o.zmax = zmax;
@@ -433,7 +465,7 @@ __device__ __forceinline__ bool ver_row_counts(const VerArgs& a, int row, const 
   o.tie_keep = ~0ull;
   if (use_k) {  // the border's group, then its place, by the first wave's lanes
     uint64_t all;
-    const uint64_t c = h.gcnt[tid], before = block_excl_scan<kSampThreads>(c, h.red, &all);
+    const uint64_t c = h.gcnt[tid] + (zero_too ? h.zeros : 0), before = block_excl_scan<kSampThreads>(c, h.red, &all);
     ver_find_group(h, before, c, (uint64_t)(p.top_k - 1));
     const int g = h.group;
     if (g >= 0) {
@@ -498,7 +530,7 @@ __device__ __forceinline__ bool ver_row_counts(const VerArgs& a, int row, const 
         const uint32_t t = (w & mask) ^ want;
         c += ((t & 0xffffu) == 0) + (t >> 16 == 0);
       };
-      ver_each(x, whole, ver_load(x, tid * 8, whole), [&](int, u32x4_t w) {
+      ver_each(x, whole, ver_load<AHEAD>(x, tid * 8, whole), [&](int, u32x4_t w) {
         count(w.x);
         count(w.y);
         count(w.z);
@@ -520,12 +552,14 @@ __device__ __forceinline__ bool ver_row_counts(const VerArgs& a, int row, const 
   return true;
 }
 
-// A row a workgroup, two workgroups a CU: one's counting hides part of the other's sums.
-__global__ __launch_bounds__(kSampThreads, 8) void verify_rows_kernel(VerArgs a, VerRow* __restrict__ rows) {
+// A row a workgroup.  With more rows than CUs two workgroups a CU, so that one's counting hides part of the other's sums (1,152 rows 115
+// us; one a CU with twice the loads ahead 122); otherwise one, which has the registers for that (120 rows 27 us for 30).
+template <int PER_CU, int AHEAD>
+__global__ __launch_bounds__(kSampThreads, 4 * PER_CU) void verify_rows_kernel(VerArgs a, VerRow* __restrict__ rows) {
   __shared__ union { VerHist hist; VerGreedy greedy; SampShared gen; } sh;
   __shared__ int found;
   const int row = blockIdx.x;
-  const VerLoaded l = ver_load(a.logits + (size_t)row * a.V, (int)threadIdx.x * 8, a.V & ~7);  // while the stream is looked up
+  const VerLoaded<AHEAD> l = ver_load<AHEAD>(a.logits + (size_t)row * a.V, (int)threadIdx.x * 8, a.V & ~7);  // while the stream is looked up
   const int s = ver_stream(a, row, &found);
   if (s < 0) return;
   const VerParams p = ver_params(a, s);
@@ -635,6 +669,7 @@ __global__ __launch_bounds__(kPieceThreads, 4) void verify_pieces_kernel(VerArgs
     if (threadIdx.x == 0) table[2 * kVerTable] = 0.0;
     __syncthreads();
   }
+  const float down = (w.zmax - 28.f) * w.tdiv, least = down - fabsf(down) * 0x1p-20f;  // below it there is no weight (that starts 27.75 down)
   for (; c < a.pieces; c += step) {
     Loaded l = next;
     if (c + step < a.pieces) next = load(c + step);
@@ -668,6 +703,11 @@ __global__ __launch_bounds__(kPieceThreads, 4) void verify_pieces_kernel(VerArgs
         double k = *reinterpret_cast<const double*>(tab + b);
         if (w.q) k = ver_rest(k, l.q[j >> 2][j & 3], w.W);
         above += k;
+      }
+      if (odd) {  // (masked ids and the like have no weight)
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          if (bf2f((uint16_t)(j & 1 ? l.x[j >> 1] >> 16 : l.x[j >> 1])) < least) odd &= ~(1u << j);
       }
       while (odd) {  // a lane's next value that has no entry
         const int v = v0 + __ffs(odd) - 1;
@@ -865,7 +905,10 @@ extern "C" int flyai_spec_verify(const uint16_t* logits, int32_t R, int32_t V, c
   VerPiece* pieces = reinterpret_cast<VerPiece*>(rows + R);
   hipStream_t s = as_stream(stream);
   if (R > 0) {
-    hipLaunchKernelGGL(verify_rows_kernel, dim3(R), dim3(kSampThreads), 0, s, a, rows);
+    if (R > device_cus())
+      hipLaunchKernelGGL((verify_rows_kernel<2, 2>), dim3(R), dim3(kSampThreads), 0, s, a, rows);
+    else
+      hipLaunchKernelGGL((verify_rows_kernel<1, 4>), dim3(R), dim3(kSampThreads), 0, s, a, rows);
     // a workgroup a CU, a piece a wave at least
     const int wgs = std::max(1, std::min(ceil_div(a.pieces, kPieceThreads / 64), device_cus() / S));
     hipLaunchKernelGGL(verify_pieces_kernel, dim3(wgs, S), dim3(kPieceThreads), 0, s, a, rows, pieces);

@@ -317,3 +317,16 @@ def test_drafts_that_are_ties_at_the_border(V, value):
     c.u[:] = 0.0
     c.check()
     assert 0 < len(set(c.expected()[1].tolist())) <= 2
+
+
+@pytest.mark.parametrize("streams", [6, 90])
+@pytest.mark.parametrize("value", [-float("inf"), float(torch.finfo(torch.bfloat16).min), -100.0, 0.0, -1e-30])
+@pytest.mark.parametrize("share", [0.7, 0.9995])
+def test_masked_ids(value, share, streams):
+    """Most ids masked, by several values: batches of fewer rows than CUs and of more."""
+    params = [(1.0, 0, 1.0), (0.7, 0, np.float32(0.95)), (1.0, 30, 1.0)] * (streams // 3)
+    c = Case(5003, [3] * streams, params, seed=streams)
+    m = torch.rand(c.logits.shape, generator=torch.Generator().manual_seed(1)) < share
+    m[:, 7] = False
+    c.logits[m] = value
+    c.check()

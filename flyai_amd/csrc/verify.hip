@@ -387,16 +387,15 @@ __device__ __forceinline__ bool ver_row_counts(const VerArgs& a, int row, const 
     atomicAdd(reinterpret_cast<uint32_t*>(c + (at >> 16)), 1u);
   };
   // a value that may have no place: one that has no weight is left out (`low` is the largest one's magnitude), another one leaves the
-  // row to the general path
-  uint32_t zeros = 0, bad = 0, low = 0xffffu;
+  // row to the general path (low 0)
+  uint32_t zeros = 0, low = 0xffffu;
   auto one = [&](uint32_t bits) __attribute__((always_inline)) {
     const uint32_t mag = bits & 0x7fffu, t = mag - kVerFirst;
     const bool none = t >= (uint32_t)kVerHalf, neg = bits & 0x8000u;
     if (!none) atomicAdd(&h.cnt[t + (neg ? kVerHalf : 0)], 1u);
     zeros += mag == 0;
     const bool below = none && neg && mag > kVerFirst;
-    low = below ? min(low, mag) : low;
-    bad |= none && !below && mag != 0;
+    low = min(low, below ? mag : none && mag != 0 ? 0u : 0xffffu);
   };
   const int full = V & ~7;
   ver_each(x, full, l, [&](int, u32x4_t w) {
@@ -414,11 +413,9 @@ __device__ __forceinline__ bool ver_row_counts(const VerArgs& a, int row, const 
     }
   });
   if (tid < V - full) one(x[full + tid]);
-  if (__ballot(zeros || bad || low != 0xffffu)) {
-    if (zeros) atomicAdd(&h.zeros, zeros);
-    if (bad) h.bad = 1;
-    if (low != 0xffffu) atomicMax(&h.low, f32_key(bf2f((uint16_t)(low | 0x8000u))));
-  }
+  if (zeros) atomicAdd(&h.zeros, zeros);
+  if (low == 0) h.bad = 1;
+  else if (low != 0xffffu) atomicMax(&h.low, f32_key(bf2f((uint16_t)(low | 0x8000u))));
   __syncthreads();
   // the values that are there: the largest, then their weights and counts by group
   constexpr int kPer = 2 * kVerHalf / kSampThreads;

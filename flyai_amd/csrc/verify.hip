@@ -17,9 +17,9 @@
 // is not is then the only one whose weights are needed one by one: verify_pieces_kernel sums w' over pieces of its ids, and
 // verify_draw_kernel finds the piece and the id, and writes what comes out.
 //
-// With a vocabulary of 201,088 (us): 128 streams' 1,152 rows 159, of which the rows 116 (463 MB, 4.0 TB/s; a copy's read side reaches 6.3),
-// the pieces 36, the draw 7; 24 streams' 120 rows 48 (30, 11, 7); one stream's 5 rows 35 (24, 6, 5), where a row is one CU's: 14 us
-// of counting in LDS, some 10 of sums over the values.  The rows that many passes over the logits took (ver_row_general's way for all)
+// With a vocabulary of 201,088 (us): 128 streams' 1,152 rows 159 to 163, of which the rows 118 (463 MB, 3.9 TB/s; a product of two arrays
+// reaches 6.3), the pieces 36, the draw 7; 24 streams' 120 rows 44 (27, 11, 7); one stream's 5 rows 35 (23, 6, 5), where a row is one CU's:
+// 12 us of counting in LDS, some 8 of sums over the values.  The rows that many passes over the logits took (ver_row_general's way for all)
 // were 1,215 us of 128 streams, 482 of one.  Rows counted in up to eight parts, then added up, made one stream's 32 us and 24 streams' 53;
 // a workgroup a CU with the next row's loads ahead 205 of 128 streams' 159.
 #include <algorithm>
@@ -549,8 +549,8 @@ __device__ __forceinline__ bool ver_row_counts(const VerArgs& a, int row, const 
   return true;
 }
 
-// A row a workgroup.  With more rows than CUs two workgroups a CU, so that one's counting hides part of the other's sums (1,152 rows 115
-// us; one a CU with twice the loads ahead 122); otherwise one, which has the registers for that (120 rows 27 us for 30).
+// A row a workgroup.  With more rows than CUs two workgroups a CU, so that one's counting hides part of the other's sums (1,152 rows 118
+// us; one a CU with twice the loads ahead 122); otherwise one, which has the registers for that (120 rows 26 us for 30).
 template <int PER_CU, int AHEAD>
 __global__ __launch_bounds__(kSampThreads, 4 * PER_CU) void verify_rows_kernel(VerArgs a, VerRow* __restrict__ rows) {
   __shared__ union { VerHist hist; VerGreedy greedy; SampShared gen; } sh;

@@ -79,17 +79,17 @@ class GptOssModel:
     def per_job_state_bytes(self):
         return self.n_layers * 2 * self.kv.slab * 2
 
-    def step(self, chunks, starts, slots, pick, adapters=None):
+    def step(self, chunks, starts, slots, pick, adapters=None, prefixes=None):
         """One ragged step.  chunks[i]: token ids fed for sequence i at positions starts[i]...; slots[i]
         its KV slot; pick[i]: whether to return the greedy token after its last row; adapters[i]: its adapter's slot in the
-        bank, or None.  Returns a list with a token id (or None) per sequence."""
+        bank, or None; prefixes[i] (after ``stage.set_prefixes()``): the (slot, positions) that it lies behind, or None.  Returns a list with a token id (or None) per sequence."""
         q_lens = [len(c) for c in chunks]
         T = sum(q_lens)
         if T > self.max_step_rows:
             raise ValueError(f"step of {T} rows exceeds {self.max_step_rows}")
         flat = torch.tensor([t for c in chunks for t in c], dtype=torch.int32).to(self.device, non_blocking=True)
         h = ops.embed_gather(self.embed, flat)
-        self.stage.forward(h, q_lens, starts, slots, adapters)
+        self.stage.forward(h, q_lens, starts, slots, adapters, prefixes)
         xn = ops.rmsnorm(h, self.norm_w, self.shape.rms_eps)
         ends = np.cumsum(q_lens) - 1
         rows = [int(ends[i]) for i in range(len(chunks)) if pick[i]]

@@ -174,3 +174,28 @@ def test_refusals():
     st.set_prefixes(False)
     with pytest.raises(ValueError, match="set_prefixes"):
         step()
+
+
+def test_a_served_model_behind_one_prompt():
+    """GptOssModel.step(prefixes=): requests behind one prompt's slot, continued greedily together, commit what each commits alone."""
+    from test_gpu_request_edges import _served
+    m = _served(False)
+    m.stage.set_prefixes()
+    prompt = [(7 * i + 3) % 1024 for i in range(60)]
+    m.step([prompt], [0], [0], [False])
+    own = [[3, 1, 4, 1, 5], [9, 2, 6], [5]]
+
+    def serve(which, steps=5):
+        chunks, starts, out = [own[i] for i in which], [60] * len(which), [[] for _ in which]
+        for _ in range(steps):
+            toks = m.step(chunks, starts, [1 + i for i in which], [True] * len(which), prefixes=[(0, 60)] * len(which))
+            starts = [s + len(c) for s, c in zip(starts, chunks)]
+            chunks = [[t] for t in toks]
+            for o, t in zip(out, toks):
+                o.append(t)
+        return out
+
+    together = serve([0, 1, 2])
+    for i in range(3):
+        assert serve([i]) == [together[i]], i
+    assert len(set(map(tuple, together))) == 3

@@ -332,10 +332,13 @@ def attn_ragged(q, k_pool, v_pool, kv_base, kv_cap, sinks, window, items, groups
 def _need_all(device, *tensors):
     """``_need`` of each (name, tensor, dtype, shape), and all on one device; the checks that pass cost little."""
     for name, t, dtype, shape in tensors:
-        if not (isinstance(t, torch.Tensor) and t.dtype is dtype and t.shape == shape and t.is_contiguous()
-                and t.get_device() == device >= 0):
-            _need(t, dtype, shape, name)
-            raise ValueError(f"{name} is on {t.device}, the first tensor on another device")
+        try:
+            if t.dtype is dtype and t.shape == shape and t.is_contiguous() and t.get_device() == device >= 0:
+                continue
+        except AttributeError:  # (no tensor)
+            pass
+        _need(t, dtype, shape, name)
+        raise ValueError(f"{name} is on {t.device}, the first tensor on another device")
 
 
 def _on(device, fn, *args):
@@ -563,8 +566,9 @@ class AttnSharedPlan:
 
 
 @functools.lru_cache(maxsize=256)
-def _attn_shared_bytes(T, S, n, Hkv):
-    return int(lib().flyai_attn_shared_plan_bytes(T, S, n)), int(lib().flyai_attn_shared_workspace_bytes(T, Hkv))
+def _attn_shared_sizes(T, S, n, Hkv):
+    """int32s of a plan, fp32s of a workspace."""
+    return max(4, int(lib().flyai_attn_shared_plan_bytes(T, S, n)) // 4), max(4, int(lib().flyai_attn_shared_workspace_bytes(T, Hkv)) // 4)
 
 
 def attn_shared_plan(q_lens, starts, kv_base, kv_cap, prefix_of, prefix_len, prefix_base, prefix_cap, n_kv_heads, window, n_tokens,
@@ -579,8 +583,8 @@ def attn_shared_plan(q_lens, starts, kv_base, kv_cap, prefix_of, prefix_len, pre
               ("kv_cap", kv_cap, i32, (S,)), ("prefix_of", prefix_of, i32, (S,)), ("prefix_len", prefix_len, i32, (n,)),
               ("prefix_base", prefix_base, i64, (n,)), ("prefix_cap", prefix_cap, i32, (n,)))
     T, Hkv, window = _position(n_tokens), _position(n_kv_heads), _position(window)
-    size, _ = _attn_shared_bytes(T, S, n, Hkv)
-    plan = AttnSharedPlan(q_lens.new_empty(max(size // 4, 4)), T, S, n, Hkv, window, operator.index(pool_elems))
+    size, _ = _attn_shared_sizes(T, S, n, Hkv)
+    plan = AttnSharedPlan(q_lens.new_empty(size), T, S, n, Hkv, window, operator.index(pool_elems))
     _on(dev, lib().flyai_attn_shared_plan, q_lens.data_ptr(), starts.data_ptr(), kv_base.data_ptr(), kv_cap.data_ptr(),
         prefix_of.data_ptr(), prefix_len.data_ptr(), prefix_base.data_ptr(), prefix_cap.data_ptr(), S, n, Hkv, window, T,
         plan.pool_elems, plan.buffer.data_ptr())
@@ -600,11 +604,11 @@ def attn_shared(q, k_pool, v_pool, sinks, plan, out=None):
     if k_pool.numel() < plan.pool_elems:
         raise ValueError(f"the pools have {k_pool.numel()} elements, the plan was made for {plan.pool_elems}")
     if out is None:
-        out = torch.empty_like(q)
+        out = q.new_empty(q.shape)
     else:
         _need_all(dev, ("out", out, bf16, q.shape))
-    _, size = _attn_shared_bytes(T, plan.n_seqs, plan.n_prefixes, Hkv)
-    ws = sinks.new_empty(max(size // 4, 4))
+    _, size = _attn_shared_sizes(T, plan.n_seqs, plan.n_prefixes, Hkv)
+    ws = sinks.new_empty(size)
     _on(dev, lib().flyai_attn_shared, q.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), sinks.data_ptr(), 8 * Hkv, Hkv, 64, T,
         plan.n_seqs, plan.n_prefixes, plan.buffer.data_ptr(), ws.data_ptr(), out.data_ptr())
     return out

@@ -41,9 +41,11 @@ constexpr int kShMaxSeqs = 4096, kShMaxPrefixes = 1024;
 constexpr int kShChunks = 16, kShMoreChunks = 24, kShMoreFrom = 1152;
 constexpr int kShMinChunk = 384, kShChunkStep = 192;
 constexpr int kShOwnChunk = 384;  // (192: two to three percent slower with some hundred own positions a stream)
-constexpr int kShSpareEntries = 1024;  // list entries beyond one for each tile, for prefixes split by chunks
-constexpr int kShSpareWaves = 2048;    // ... and beyond one for each group of a sequence's tokens
-constexpr int kShSpareRecs = 16384, kShSpareRecsOfToken = 256;  // records beyond two for each token: so many for a token, and at most
+// What is split by chunks has room of its own: entries of workgroups and waves beyond one for each tile and group, and records beyond two
+// for each token.  A prefix's tiles are split where they fill less than a round (kShRecCost), so up to some 2 / 3 of kShGrid / Hkv tiles of
+// 16 tokens in up to 24 chunks; a sequence's own keys where they make fewer than 8 kShGrid items of up to 4 tokens a wave.  (What does not fit stays whole.)
+constexpr int kShSpareEntries = 8192, kShSpareWaves = 4096;
+constexpr int kShSplitRecs = 131072, kShOwnRecs = 16384;  // of all kv heads: 277 and 35 MB
 constexpr int kShRecCost = 600;       // what a chunk's records cost, in positions
 constexpr int kShGrid = 512;           // workgroups on the chip at once: two a CU
 // workgroups of a kv head: head g's are those with blockIdx % Hkv == g, with 8 heads an XCD each, so that its L2 holds one head's keys
@@ -86,16 +88,17 @@ struct ShLayout {
   size_t o_entries, o_waves, o_list, o_tokens, bytes;
 };
 
-__host__ __device__ inline ShLayout sh_layout(int T, int S, int n_prefix) {
+__host__ __device__ inline ShLayout sh_layout(int T, int S, int n_prefix, int Hkv) {
+  auto least = [](int a, int b) { return a < b ? a : b; };
   ShLayout l;
   l.T = T;
   l.S = S;
   l.n_prefix = n_prefix;
   // the prefixes' tiles, those of the sequences with more than kShWaveSeq tokens
-  l.max_entries = 2 * (T / kShRowTokens) + (n_prefix < T ? n_prefix : T) + T / (kShWaveSeq + 1) + kShSpareEntries;
+  l.max_entries = 2 * (T / kShRowTokens) + (n_prefix < T ? n_prefix : T) + T / (kShWaveSeq + 1) + least(1024 + 2 * T, kShSpareEntries);
   // the other sequences' groups, and the prefixes whose few tokens go to waves
   l.max_waves = T / kShWaveTokens + (S < T ? S : T) + (n_prefix < T ? n_prefix : T) + kShSpareWaves;
-  l.max_recs = 2 * T + (T < kShSpareRecs / kShSpareRecsOfToken ? T * kShSpareRecsOfToken : kShSpareRecs);
+  l.max_recs = 2 * T + least(kShMoreChunks * T, kShSplitRecs / Hkv) + least(256 * T, kShOwnRecs / Hkv);
   size_t o = sizeof(ShHeader);
   l.o_entries = o;
   o += (size_t)l.max_entries * sizeof(ShEntry);
@@ -201,7 +204,7 @@ constexpr int kShMaxOwnChunks = 4096;  // of a sequence, for the counts to stay 
 // with 2 sequences; 256 sequences of 1,000 tokens take the large one, 9.3.
 template <int NT, int PER>
 __global__ __launch_bounds__(NT) void attn_shared_plan_kernel(ShBatch b, char* __restrict__ plan) {
-  const ShLayout L = sh_layout(b.T, b.S, b.n_prefix);
+  const ShLayout L = sh_layout(b.T, b.S, b.n_prefix, b.Hkv);
   ShHeader* hdr = reinterpret_cast<ShHeader*>(plan);
   ShEntry* entries = reinterpret_cast<ShEntry*>(plan + L.o_entries);
   ShEntry* waves = reinterpret_cast<ShEntry*>(plan + L.o_waves);
@@ -1108,12 +1111,12 @@ using namespace flyai;
 
 extern "C" size_t flyai_attn_shared_plan_bytes(int32_t T, int32_t S, int32_t n_prefix) {
   if (T < 0 || T > 65536 || S < 0 || S > kShMaxSeqs || n_prefix < 0 || n_prefix > kShMaxPrefixes) return 0;
-  return sh_layout(T, S, n_prefix).bytes;
+  return sh_layout(T, S, n_prefix, 1).bytes;
 }
 
 extern "C" size_t flyai_attn_shared_workspace_bytes(int32_t T, int32_t Hkv) {
   if (T < 0 || T > 65536 || Hkv < 1 || Hkv > 64) return 0;
-  return (size_t)sh_layout(T, 0, 0).max_recs * Hkv * 8 * (64 + 2) * sizeof(float);
+  return (size_t)sh_layout(T, 0, 0, Hkv).max_recs * Hkv * 8 * (64 + 2) * sizeof(float);
 }
 
 extern "C" int flyai_attn_shared_plan(const int32_t* q_lens, const int32_t* starts, const int64_t* kv_base, const int32_t* kv_cap,
@@ -1145,7 +1148,7 @@ extern "C" int flyai_attn_shared(const uint16_t* q, const uint16_t* k_pool, cons
   FLYAI_REQUIRE(((uintptr_t)q & 15) == 0 && ((uintptr_t)k_pool & 15) == 0 && ((uintptr_t)v_pool & 15) == 0 &&
                     ((uintptr_t)out & 15) == 0 && ((uintptr_t)workspace & 15) == 0 && ((uintptr_t)plan & 15) == 0,
                 "attn_shared: q, the pools, out, plan and workspace must be 16-byte aligned");
-  const ShLayout L = sh_layout(T, S, n_prefix);
+  const ShLayout L = sh_layout(T, S, n_prefix, Hkv);
   hipStream_t s = as_stream(stream);
   hipLaunchKernelGGL(attn_shared_kernel, dim3((unsigned)(sh_per_head(Hkv) * Hkv)), dim3(256), 0, s, q, k_pool, v_pool, Hq, Hkv, L,
                      static_cast<const char*>(plan), static_cast<float*>(workspace));

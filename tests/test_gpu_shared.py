@@ -279,11 +279,11 @@ def test_long_prefixes(P, window):
     check(got, *b.expected(window))
 
 
-@pytest.mark.parametrize("n", [1, 40, 65, 90])
-def test_tiles_and_rounds(n):
+@pytest.mark.parametrize("n,Hkv,P", [(1, 8, 1600), (40, 8, 1600), (65, 8, 1600), (90, 8, 1600), (60, 1, 30000), (200, 1, 2000), (20, 16, 9000)])
+def test_tiles_and_rounds(n, Hkv, P):
     """Tiles that fill no round of the workgroups, more than one, and whole or split rests: every row's bits are those that its sequence
     has in a batch of its own."""
-    b = Batch([1600], [(16, 3 * i % 70, 0) for i in range(n)], Hkv=8, seed=n)
+    b = Batch([P], [(16, 3 * i % 70, 0) for i in range(n)], Hkv=Hkv, seed=n)
     got, _ = b.run(0)
     alone = Batch.__new__(Batch)
     alone.__dict__.update(b.__dict__)

@@ -8,8 +8,8 @@
 // Every key range is cut into chunks whose borders go by the slab alone (from its position 0).  A chunk's
 // (m, l, O[64]) starts afresh, and a range's total folds its chunks in ascending order (fold below):
 //   M' = max(M, m);  O' = O_c 2^(m - M') + O 2^(M - M');  L likewise.
-// A work item takes a run of a range's chunks and leaves a record of each, which attn_shared_merge_kernel folds; or it takes the whole
-// range and folds in its registers, by the same operations in the same order.  So the work is split where there are few
+// A work item takes a run of a range's chunks and leaves a record of each (one, of a run from the range's first chunk on: folded), which
+// attn_shared_merge_kernel folds; or it takes the whole range and folds in its registers, by the same operations in the same order.  So the work is split where there are few
 // rows and not where there are many, and a row's bits depend on neither, nor on the rest of the batch.
 //
 // The work lists are made on the GPU (attn_shared_plan_kernel), once for a step's layers: the host needs
@@ -46,7 +46,7 @@ constexpr int kShOwnChunk = 384;  // (192: two to three percent slower with some
 // 16 tokens in up to 24 chunks; a sequence's own keys where they make fewer than 8 kShGrid items of up to 4 tokens a wave.  (What does not fit stays whole.)
 constexpr int kShSpareEntries = 8192, kShSpareWaves = 4096;
 constexpr int kShSplitRecs = 131072, kShOwnRecs = 16384;  // of all kv heads: 277 and 35 MB
-constexpr int kShRecCost = 600;       // what a chunk's records cost, in positions
+constexpr int kShRecCost = 700;       // what a chunk's records cost, in positions
 constexpr int kShGrid = 512;           // workgroups on the chip at once: two a CU
 // workgroups of a kv head: head g's are those with blockIdx % Hkv == g, with 8 heads an XCD each, so that its L2 holds one head's keys
 __host__ __device__ constexpr int sh_per_head(int Hkv) { return kShGrid / Hkv > 0 ? kShGrid / Hkv : 1; }
@@ -66,13 +66,23 @@ struct ShEntry {
   int32_t rec;          // record of the first token; token i's is rec + i, the next chunk's `stride` behind
   int32_t stride;
   int32_t left;
-  int32_t pad;
+  int32_t is_first;     // of a split tile's units: its first chunk's.  The chunks that a workgroup takes from there on are folded into one record.
 };
 
 struct ShToken {  // where a token's records lie: n of them, stride apart
   int32_t p_rec, p_n, p_stride;
+  int32_t p_folded;  // chunks that the prefix's first record holds: the next one is that of chunk p_folded
   int32_t o_rec, o_n, o_stride;
+  int32_t pad;
 };
+
+// The split units are dealt out in shares of consecutive ones, the first n % per_head of them one larger: the end of the share that holds
+// unit u.
+__device__ __forceinline__ int sh_share_end(int n, int per_head, int u) {
+  const int share = n / per_head, more = n % per_head;
+  const int w = u < more * (share + 1) ? u / (share + 1) : more + (u - more * (share + 1)) / max(share, 1);
+  return (w + 1) * share + min(w + 1, more);
+}
 
 // The units of workgroups: whole prefix tiles, then chunks of prefix tiles, then the sequences' own tiles; and those of waves.
 struct ShHeader {
@@ -327,12 +337,14 @@ __global__ __launch_bounds__(NT) void attn_shared_plan_kernel(ShBatch b, char* _
   int ps[6] = {np, few ? 0 : tiles, few ? tiles : 0, few ? tiles * chunks : 0, few ? np * chunks : 0, few ? 0 : tiles * min(C, 4096)}, n_ps[6];
   sh_excl_scan<NT, 6>(ps, n_ps, red);
   // As many whole tiles as give every workgroup the same number; the rest by chunks, if the lists and the records hold them.  A chunk of C
-  // positions costs what C + kShRecCost would without its records, so the rest stays whole where its chunks would take longer than a
-  // round that not all workgroups have a tile in: with 43 and 92 tiles of 4,099 positions (64 workgroups) 110 and 164 us whole, 119 and
-  // 175 by chunks; with 23 and 84 77 and 165, 71 and 158.
+  // positions costs what C + kShRecCost would without its records; of a rest that is the part r of a round some 0.7 r of the chunks are
+  // in their tile's first record.  So the rest stays whole where its chunks would take longer than a round that not all workgroups
+  // have a tile in.  With 43 and 93 tiles of 4,099 positions (64 workgroups) whole and by chunks 106 and 116, 164 and 172 us; with 23 and 84
+  // 77 and 70, 165 and 156; with 35 of 9,000 175 and 143.
   const int per_head = sh_per_head(b.Hkv);
   int whole = n_ps[1] / per_head * per_head;
-  if ((int64_t)(n_ps[1] - whole) * (n_ps[5] + (int64_t)kShRecCost * n_ps[1]) > (int64_t)per_head * n_ps[5]) whole = n_ps[1];
+  const int64_t rest = n_ps[1] - whole, part = 10 * per_head - 7 * rest;  // 10 per_head (1 - 0.7 r)
+  if (rest * (10 * per_head * (int64_t)n_ps[5] + kShRecCost * part * n_ps[1]) > 10 * (int64_t)per_head * per_head * n_ps[5]) whole = n_ps[1];
   auto split_of = [&](int w) __attribute__((always_inline)) { return few ? 0 : max(0, ps[1] + tiles - max(ps[1], w)); };
   int split = split_of(whole), split_tokens = np > 0 ? min(np, np - (tiles - split) * kShRowTokens) : 0;
   if (!split) split_tokens = 0;
@@ -416,7 +428,7 @@ __global__ __launch_bounds__(NT) void attn_shared_plan_kernel(ShBatch b, char* _
       e.stride = one ? 0 : n - ts * kShRowTokens;
       e.rec = one ? e.first : px.rec0[p] + k * e.stride + (t - ts) * kShRowTokens;
       e.left = one ? 0 : nch - 1 - k;
-      e.pad = 0;
+      e.is_first = !one && k == 0;
       ShEntry* out = w ? waves + px.tile0[p] : one ? entries + px.tile0[p] : entries + whole + px.unit0[p] - ts;
       out[i] = e;
     }
@@ -427,7 +439,7 @@ __global__ __launch_bounds__(NT) void attn_shared_plan_kernel(ShBatch b, char* _
       const int mid = (lo + hi + 1) >> 1;
       if (sq.cu[mid] <= t) lo = mid; else hi = mid - 1;
     }
-    ShToken k = {0, 0, 0, 0, 0, 0};
+    ShToken k = {};
     const int own0 = sq.own0[lo], i = t - sq.cu[lo];
     if (own0 >= 0) {
       const int n = sq.cu[lo + 1] - sq.cu[lo], p = sq.prefix[lo];
@@ -441,12 +453,16 @@ __global__ __launch_bounds__(NT) void attn_shared_plan_kernel(ShBatch b, char* _
         const bool w = count <= kShWaveTokens;
         const int ts = w ? (fsplit ? 0 : 1) : first_split(p);
         list[px.list0[p] + where] = make_int2(t, len + own0 + i);
-        k.p_n = 1;
+        k.p_n = k.p_folded = 1;
         k.p_rec = px.list0[p] + where;
         if (where >= ts * kShRowTokens) {
           k.p_n = (len - 1) / c + 1 - px.lo[p] / c;
           k.p_stride = count - ts * kShRowTokens;
           k.p_rec = px.rec0[p] + where - ts * kShRowTokens;
+          if (!w) {
+            const int u = px.unit0[p] + (where / kShRowTokens - ts) * k.p_n;
+            k.p_folded = min(k.p_n, sh_share_end(n_us[0], per_head, u) - u);
+          }
         }
       }
       const int size = n <= kShWaveSeq ? kShWaveTokens : kShRowTokens;
@@ -468,7 +484,7 @@ __global__ __launch_bounds__(NT) void attn_shared_plan_kernel(ShBatch b, char* _
           e.rec = sq.rec0[lo] + c * n + i;
           e.stride = osplit ? n : 0;
           e.left = 0;
-          e.pad = 0;
+          e.is_first = 0;
           (n <= kShWaveSeq ? waves : entries)[sq.entry0[lo] + (i / size) * nch + c] = e;
         }
       }
@@ -935,7 +951,7 @@ __device__ __forceinline__ void sh_tile_item(const ShEntry& e, int run, int kv_h
   bool fresh = true;
   for (int kb = kb_first; kb < key_hi;) {
     if (kb == next_fold) {
-      if (e.stride) {
+      if (e.stride && !e.is_first) {
         sh_put(R, rec, 4 * wave, kv_head, Hkv, max_recs, parts);
         sh_nothing(R);
         rec += e.stride;
@@ -1013,7 +1029,7 @@ __global__ __launch_bounds__(256, 2) void attn_shared_kernel(const uint16_t* __r
     sh_tile_item(e, run, g, list, q, k_pool, v_pool, Hq, Hkv, window, L.max_recs, parts, buf0, buf1);
   };
   // the whole tiles dealt out, the split ones in equal shares of consecutive units, the sequences' own from the other end
-  const int share = n_split / per_head, more = n_split % per_head;
+  const int share = n_split / per_head, more = n_split % per_head;  // (sh_share_end's)
   const int s0 = n_whole + w * share + min(w, more), s1 = s0 + share + (w < more);
   int i = w < n_whole ? w : s0, own = per_head - 1 - w;
   for (;;) {
@@ -1059,7 +1075,8 @@ __global__ __launch_bounds__(128) void attn_shared_merge_kernel(const float* __r
   f32x4_t Ot[2];
 #pragma unroll
   for (int w = 0; w < 2; ++w) {
-    const int rec0 = w ? k.o_rec : k.p_rec, n = w ? k.o_n : k.p_n, stride = w ? k.o_stride : k.p_stride;
+    const int rec0 = w ? k.o_rec : k.p_rec, stride = w ? k.o_stride : k.p_stride;
+    const int skip = w ? 0 : max(k.p_folded - 1, 0), n = w ? k.o_n : k.p_n - skip;  // (what the first record holds besides)
     Mt[w] = -1e30f;
     Lt[w] = 0.f;
     Ot[w] = f32x4_t{0.f, 0.f, 0.f, 0.f};
@@ -1069,7 +1086,7 @@ __global__ __launch_bounds__(128) void attn_shared_merge_kernel(const float* __r
 #pragma unroll
       for (int j = 0; j < kShMergeAhead; ++j) {
         if (c0 + j >= n) break;  // uniform
-        const int rec = rec0 + (c0 + j) * stride;
+        const int rec = rec0 + (c0 + j + (c0 + j ? skip : 0)) * stride;
         ml[j] = *reinterpret_cast<const float2*>(sh_rec_ml(parts, L.max_recs, rec, Hkv, g, h));
         o[j] = *reinterpret_cast<const f32x4_t*>(sh_rec_o(parts, rec, Hkv, g, h) + part * 4);
       }

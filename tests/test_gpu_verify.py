@@ -330,3 +330,9 @@ def test_masked_ids(value, share, streams):
     m[:, 7] = False
     c.logits[m] = value
     c.check()
+
+
+def test_a_table_without_rows():
+    """draft_probs of no rows, and probs_row that names none: drafts without a distribution."""
+    c = Case(3000, [4, 2], [(0.8, 0, np.float32(0.9))] * 2, seed=8, probs="none")
+    c.check(draft_probs=torch.empty(0, 3000, device=DEV), probs_row=torch.full((6,), -1, dtype=torch.int32, device=DEV))

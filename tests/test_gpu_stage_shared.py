@@ -199,3 +199,27 @@ def test_a_served_model_behind_one_prompt():
     for i in range(3):
         assert serve([i]) == [together[i]], i
     assert len(set(map(tuple, together))) == 3
+
+
+@pytest.mark.parametrize("name", ["drafts", "questions"])
+def test_adapters_behind_prefixes(name):
+    """Adapters of sequences behind prefixes: K and V as on copies of the prompts, bit for bit, and not those without adapters."""
+    from test_gpu_stage_lora import _bank
+    case = _case(name, seed=9)
+    kv, n, ads = case["kv"], len(case["q_lens"]), [0, None, 1, 3, -1, 1]
+    bank = _bank(case["shape"], 1)
+    flat = KVWorkspace(1, n, 1024, kv.n_kv_heads, 64, DEV)
+    st = RaggedStage(case["shape"], case["layers"], case["rot"], flat, max_tokens=max(64, case["T"]), max_seqs=8, lora=bank)
+    st.forward(case["hidden"].clone(), case["q_lens"], case["starts"], list(range(n)), adapters=ads)
+    saved = _pools(kv)
+    _forward(_stage(case), case)
+    without = _pools(kv)
+    _restore(kv, saved)
+    for graphs in (False, True):
+        _restore(kv, saved)
+        _forward(_stage(case, lora=bank, use_graphs=graphs), case, adapters=ads)
+        for b, (slot, p, start, q) in enumerate(zip(case["slots"], case["prefixes"], case["starts"], case["q_lens"])):
+            new = torch.arange(start, start + q, device=DEV)
+            for f in ("k_dense", "v_dense"):
+                assert getattr(kv, f)(0, slot, new - (p[1] if p else 0)).equal(getattr(flat, f)(0, b, new)), (b, f)
+        assert not kv.k_pools.equal(without[0])

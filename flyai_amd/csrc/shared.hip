@@ -750,16 +750,24 @@ __device__ __forceinline__ bool sh_fast_block(ShRows<2>& R, KF&& k, VF&& v) {
   constexpr int QT = 2;
   const float scale = 0.125f * kLog2e;
   const bf16x8_t ones = as_bf16x8(make_uint4(0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u));
+  // (K's fragments are read at once, V's first half before the maxima, its second before its products: read where they are used,
+  // each is a wait for LDS)
+  bf16x8_t kf[4][2], vf[4];
+#pragma unroll
+  for (int kt = 0; kt < 4; ++kt)
+#pragma unroll
+    for (int st = 0; st < 2; ++st) kf[kt][st] = as_bf16x8(k(kt, st));
+  __builtin_amdgcn_sched_barrier(0);
   f32x4_t s[QT][4];
 #pragma unroll
-  for (int kt = 0; kt < 4; ++kt) {
-    const bf16x8_t k0 = as_bf16x8(k(kt, 0)), k1 = as_bf16x8(k(kt, 1));
+  for (int st = 0; st < 2; ++st)
 #pragma unroll
-    for (int qt = 0; qt < QT; ++qt) {
-      s[qt][kt] = mfma16x16x32(k0, R.qf[qt][0], f32x4_t{0.f, 0.f, 0.f, 0.f});
-      s[qt][kt] = mfma16x16x32(k1, R.qf[qt][1], s[qt][kt]);
-    }
-  }
+    for (int kt = 0; kt < 4; ++kt)
+#pragma unroll
+      for (int qt = 0; qt < QT; ++qt) s[qt][kt] = mfma16x16x32(kf[kt][st], R.qf[qt][st], st ? s[qt][kt] : f32x4_t{0.f, 0.f, 0.f, 0.f});
+#pragma unroll
+  for (int dt = 0; dt < 4; ++dt) vf[dt] = as_bf16x8(v(dt, 0));
+  __builtin_amdgcn_sched_barrier(0);
   bool past = false;  // (sh_block's rule)
 #pragma unroll
   for (int qt = 0; qt < QT; ++qt) {
@@ -797,23 +805,23 @@ __device__ __forceinline__ bool sh_fast_block(ShRows<2>& R, KF&& k, VF&& v) {
   for (int qt = 0; qt < QT; ++qt) R.L[qt] = mfma16x16x32(ones, pt[qt][0], FIRST ? f32x4_t{0.f, 0.f, 0.f, 0.f} : R.L[qt]);
 #pragma unroll
   for (int dt = 0; dt < 4; ++dt) {
-    const uint4 v0 = v(dt, 0);
 #pragma unroll
     for (int qt = 0; qt < QT; ++qt) {
-      R.O[qt][dt] = mfma16x16x32(as_bf16x8(v0), pt[qt][0], FIRST ? f32x4_t{0.f, 0.f, 0.f, 0.f} : R.O[qt][dt]);
+      R.O[qt][dt] = mfma16x16x32(vf[dt], pt[qt][0], FIRST ? f32x4_t{0.f, 0.f, 0.f, 0.f} : R.O[qt][dt]);
 #pragma unroll
       for (int i = 0; i < 2; ++i) weight(dt & 1, 2 + (dt >> 1), 2 * qt + i);
     }
   }
+#pragma unroll
+  for (int dt = 0; dt < 4; ++dt) vf[dt] = as_bf16x8(v(dt, 1));
+  __builtin_amdgcn_sched_barrier(0);
   __builtin_amdgcn_s_setprio(0);
 #pragma unroll
   for (int qt = 0; qt < QT; ++qt) R.L[qt] = mfma16x16x32(ones, pt[qt][1], R.L[qt]);
 #pragma unroll
-  for (int dt = 0; dt < 4; ++dt) {
-    const uint4 v1 = v(dt, 1);
+  for (int dt = 0; dt < 4; ++dt)
 #pragma unroll
-    for (int qt = 0; qt < QT; ++qt) R.O[qt][dt] = mfma16x16x32(as_bf16x8(v1), pt[qt][1], R.O[qt][dt]);
-  }
+    for (int qt = 0; qt < QT; ++qt) R.O[qt][dt] = mfma16x16x32(vf[dt], pt[qt][1], R.O[qt][dt]);
   return true;
 }
 

@@ -17,8 +17,8 @@
 //
 // What bounds it: with many rows instruction issue.  A wave's block (32 rows, 64 keys) is 36 matrix instructions (576 clocks at their
 // peak rate) and 32 exponentials, 32 fused multiply-adds, 16 maxima of three and 16 conversions (some 770): with two waves a SIMD the
-// larger of the two if nothing were in the way.  256 streams of up to 4 tokens behind 32,749 positions (554 GFLOP) take 599 to 618 us,
-// 0.9 PFLOP/s (a library's large product: 1.43); six questions of up to 300 tokens behind 4,099 (102 GFLOP) 165.  With few rows the
+// larger of the two if nothing were in the way.  256 streams of up to 4 tokens behind 32,749 positions (554 GFLOP) take 578 us,
+// 0.96 PFLOP/s (a library's large product: 1.43); six questions of up to 300 tokens behind 4,099 (102 GFLOP) 158.  With few rows the
 // chain of a unit -- entry, token list, queries (3.5 us), then 1.1 us a block, of which two waves a SIMD take as long as one -- and the launches: 48 streams behind
 // 8,000 positions 32 us, of which the plan's 6, the items' 19 and the merge's 5; 2 streams behind 513 21 (6, 6 and 3; the host's two calls
 // are as long).  Three waves a SIMD (168 registers) and three buffers in turn were slower than two.

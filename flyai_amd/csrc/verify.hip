@@ -746,7 +746,7 @@ __global__ __launch_bounds__(kPiece) void verify_draw_kernel(VerArgs a, const Ve
                                                              const VerPiece* __restrict__ pieces, int32_t* __restrict__ tokens,
                                                              int32_t* __restrict__ counts, float* __restrict__ p_out) {
   __shared__ uint64_t red[kPiece / 64];
-  __shared__ int stop_s, hit_s, part_s;
+  __shared__ int stop_s, hit_s, part_s, first_s;
   __shared__ uint64_t left_s, part_before_s, hit_before_s, part_sum_s;
   const int s = blockIdx.x, tid = threadIdx.x;
   const int2 range = ver_range(a, s);
@@ -759,6 +759,7 @@ __global__ __launch_bounds__(kPiece) void verify_draw_kernel(VerArgs a, const Ve
   if (tid == 0) {
     counts[s] = min(stop + 1, range.y) - range.x;
     part_s = hit_s = -1;
+    first_s = INT32_MAX;
   }
   if (stop >= range.y) return;
   const VerRow r = rows[stop];
@@ -845,9 +846,10 @@ __global__ __launch_bounds__(kPiece) void verify_draw_kernel(VerArgs a, const Ve
     }
     return;
   }
-  // nothing is left: the first id of maximal weight (the ties at the filter's border keep its first, which is the only one that counts here)
+  // nothing is left: the first id of maximal weight (the ties at the filter's border keep its first, which is the only one that counts here).
+  // It has a place of its own: waves that come late still read hit_s above, and no barrier lies between.
   uint64_t best = 0;
-  int at = 0x7fffffff;
+  int at = INT32_MAX;
   for (int v = tid; v < a.V; v += kPiece) {
     bool tie;
     const uint64_t k = (uint64_t)w.kept(w.x[v], &tie);
@@ -863,13 +865,12 @@ __global__ __launch_bounds__(kPiece) void verify_draw_kernel(VerArgs a, const Ve
     top = y > top ? y : top;
   }
   if ((tid & 63) == 0) red[tid >> 6] = top;
-  if (tid == 0) hit_s = 0x7fffffff;
   __syncthreads();
   for (int i = 0; i < kPiece / 64; ++i) top = red[i] > top ? red[i] : top;
-  if (best == top) atomicMin(&hit_s, at);
+  if (best == top) atomicMin(&first_s, at);
   __syncthreads();
   if (tid == 0) {
-    tokens[stop] = top ? hit_s : 0;
+    tokens[stop] = top ? first_s : 0;
     p_out[stop] = top ? (float)((double)top / (double)r.W) : 0.f;
   }
 }

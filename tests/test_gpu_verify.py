@@ -336,3 +336,18 @@ def test_a_table_without_rows():
     """draft_probs of no rows, and probs_row that names none: drafts without a distribution."""
     c = Case(3000, [4, 2], [(0.8, 0, np.float32(0.9))] * 2, seed=8, probs="none")
     c.check(draft_probs=torch.empty(0, 3000, device=DEV), probs_row=torch.full((6,), -1, dtype=torch.int32, device=DEV))
+
+
+@pytest.mark.parametrize("V", [1, 3, 65, 513, 5003])
+def test_nothing_is_left(V):
+    """A distribution that leaves no weight, for more streams than CUs: every stream draws the first id of maximal weight, with the
+    maximum alone and shared, with filters and without."""
+    S = 600
+    c = Case(V, [2] * S, [PARAMS[1 + i % (len(PARAMS) - 1)] for i in range(S)], seed=V, probs="none")
+    c.logits[::4] = torch.where(torch.arange(V) % 5 == 2, 9.0, c.logits[::4].float()).to(torch.bfloat16)
+    c.probs = np.full((1, V), 3.0, dtype=np.float32)
+    c.probs_row[:] = 0
+    c.u[:] = 0.9
+    tokens, counts, _ = c.expected()
+    assert counts.tolist() == [1] * S and (V < 4 or len(set(tokens[::2].tolist())) > 2)
+    c.check()

@@ -110,6 +110,8 @@ class Sampler:
             raise ValueError(f"accept_batch: the drafts need {sum(len(d) + 1 for d in drafts)} logits rows, got {R}")
         if any(not 0 <= int(i) < V for d in drafts for i in d):
             raise ValueError("accept_batch: drafted token id outside the vocabulary")
+        if probs is not None and tuple(probs.shape) != (R - len(drafts), V):  # (a draft without its row would pass for a deterministic one)
+            raise ValueError(f"accept_batch: probs must have shape {(R - len(drafts), V)}, a row for each drafted id, got {tuple(probs.shape)}")
         if not drafts:
             return []
         flat, row, cu = [], [], [0]

@@ -10,6 +10,7 @@ import torch
 from flyai_amd import _lib, ops
 from flyai_amd._lib import ContextOverflow, FlyaiError
 from flyai_amd.runtime import KVWorkspace, RaggedStage
+from flyai_amd.sampling import Sampler
 
 FAKE = 0x100000
 
@@ -174,3 +175,16 @@ def test_stage_prefixes_at_the_c_entry(stage):
     assert "workspace not set" in call()[1]  # what was bound is still there
     stage.set_prefixes(False)
     assert "flyai_stage_set_shared" in call()[1]
+
+
+def test_accept_batch_wants_a_distribution_for_each_draft():
+    """A row fewer, a row for each row of logits, another vocabulary: refused before the generator is asked."""
+    sm = Sampler(temp=1.0, seed=3, device="cpu")
+    before = sm.gen.bit_generator.state
+    logits, drafts = torch.zeros(6, 50, dtype=torch.bfloat16), [[1, 2], [], [3]]
+    for shape in ((2, 50), (6, 50), (4, 50), (0, 50), (3, 49), (3,), (1, 3, 50)):
+        with pytest.raises(ValueError, match="probs must have shape"):
+            sm.accept_batch(logits, drafts, probs=torch.zeros(shape))
+    with pytest.raises(ValueError, match="probs must have shape"):
+        sm.accept_batch(logits[:0], [], probs=torch.zeros(1, 50))
+    assert sm.gen.bit_generator.state == before

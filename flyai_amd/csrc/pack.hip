@@ -182,11 +182,12 @@ __global__ __launch_bounds__(kPackThreads) void pack_shared_kernel(
     }
     const int P = behind(lo);
     const int64_t pos = (int64_t)starts[lo] + (t - cu[lo]), at = pos - P;
-    const bool fits = P >= 0 && starts[lo] >= 0 && at >= 0 && at < kv_cap[lo];
+    // a sequence without a place in its slab (status 4, 8, 16) gets none for any token: its later ones would land on keys that are there
+    const bool placed = P >= 0 && starts[lo] >= P;
     positions[t] = (int)min(pos, (int64_t)INT32_MAX);
     seq_id[t] = lo;
-    kv_pos[t] = P < 0 ? -1 : (int)max(min(at, (int64_t)INT32_MAX), (int64_t)-1);
-    kv_slot[t] = fits ? kv_base[lo] + at * head_dim : (int64_t)-1;
+    kv_pos[t] = placed ? (int)min(at, (int64_t)INT32_MAX) : -1;
+    kv_slot[t] = placed && at < kv_cap[lo] ? kv_base[lo] + at * head_dim : (int64_t)-1;
   }
 }
 

@@ -530,8 +530,10 @@ def pack_shared(q_lens, starts, kv_base, kv_cap, prefix_of, prefix_len, head_dim
     """``pack_ragged`` for sequences behind shared prefixes: sequence b's first prefix_len[prefix_of[b]] positions lie in a slab
     that it shares (prefix_of negative: none), its own slab (kv_base, kv_cap) holds what follows.  Device int32 q_lens,
     starts (the first new token's position), kv_cap, prefix_of [S], prefix_len [n], int64 kv_base [S] -> dict of cu_seqlens,
-    positions, seq_id, kv_len as in ``pack_ragged``, kv_pos int32 (a token's slab position), kv_slot int64 (its element, -1 outside
-    the slab) and status (PAST_SLAB, ... bits; 0: all is well).  max_tokens may be more than the batch has: positions, seq_id, kv_pos
+    positions, seq_id, kv_len as in ``pack_ragged``, kv_pos int32 (a token's slab position), kv_slot int64 (its element, -1 past
+    the slab) and status (PAST_SLAB, ... bits; 0: all is well).  A sequence of BEFORE_PREFIX, BAD_PREFIX or BAD_SEQUENCE gets no kv_pos and
+    kv_slot (-1); of one past its slab or max_tokens the tokens that fit keep theirs.  That slabs lie in the pools is not checked here, but by
+    ``attn_shared_plan``.  max_tokens may be more than the batch has: positions, seq_id, kv_pos
     and kv_slot are -1 behind its last token, and ``rope_kv_append`` skips such rows.  Lengths may come from the GPU: nothing is read
     back."""
     S, n = q_lens.numel(), prefix_len.numel()

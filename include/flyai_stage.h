@@ -386,8 +386,11 @@ int flyai_kv_compact(uint16_t* k_pool, uint16_t* v_pool, int64_t layer, int64_t 
  * more tokens than max_tokens (n_tokens), 4 a sequence that starts before its prefix ends, 8 a prefix that is none (id,
  * length or slab), 16 a bad length, start or slab.  q_lens[b] = 0 is a sequence without tokens.
  * flyai_pack_shared is flyai_pack_ragged for such sequences: positions[t] and kv_len[b] count from the prefix's start,
- * kv_pos[t] (-1 before the slab) is the token's slab position and kv_slot[t] = kv_base + kv_pos * head_dim, -1 outside
- * the slab.  All four are -1 behind the last token, up to max_tokens: flyai_rope_kv_append_at skips such rows.  n_seqs <= 8192, max_tokens <= 2^24. */
+ * kv_pos[t] is the token's slab position and kv_slot[t] = kv_base + kv_pos * head_dim, -1 past the slab.  Both are -1 for every token of a
+ * sequence that starts before its prefix ends, or whose prefix, length or start is bad; of a sequence that runs past its slab or max_tokens
+ * the tokens that fit keep theirs (flyai_attn_shared refuses the sequence whole).  All four are -1 behind the last token, up to max_tokens.
+ * flyai_rope_kv_append_at skips rows of such positions.  The slabs themselves are not looked at here, nor by the append: a kv_base and kv_cap
+ * that leave the pools are the caller's fault, which flyai_attn_shared_plan alone reports.  n_seqs <= 8192, max_tokens <= 2^24. */
 int flyai_pack_shared(const int32_t* q_lens, const int32_t* starts, const int64_t* kv_base, const int32_t* kv_cap,
                       const int32_t* prefix_of, const int32_t* prefix_len, int32_t n_seqs, int32_t n_prefixes,
                       int32_t head_dim, int32_t max_tokens, int32_t* cu_seqlens, int32_t* positions, int32_t* seq_id,

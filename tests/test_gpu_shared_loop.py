@@ -231,3 +231,33 @@ def test_two_batches_on_two_streams():
     for i in range(2):
         for x, y in zip(got[i], want[i]):
             assert all(x[k][:R].equal(y[k][:R]) for k in y)
+
+
+def test_refused_sequences_are_appended_nowhere():
+    """A sequence that starts before its prefix ends, or whose prefix or start is bad, has no slab position at any of its tokens, and the
+    keys that lie in its slab stay.  One that runs past its slab, or past the rows, keeps the positions of the tokens that fit."""
+    i32 = lambda a: torch.tensor(a, dtype=torch.int32, device=DEV)  # noqa: E731
+    m, cap, q_lens = Model(6), 64, [3, 4, 2]
+    base = torch.arange(3, dtype=torch.int64, device=DEV) * HKV * cap * D
+    want = [5, 6, 7, 0, 1, 2, 3, 9, 10]  # of starts (105, 30, 9) behind 100 and 30 positions and none
+    for change, bit, lost in (({}, 0, ()), (dict(starts=[98, 30, 9]), ops.BEFORE_PREFIX, (0, 1, 2)), (dict(starts=[105, 29, 9]), ops.BEFORE_PREFIX, (3, 4, 5, 6)),
+                              (dict(starts=[105, 30, -1]), ops.BAD_SEQUENCE, (7, 8)), (dict(prefix_of=[0, 2, -1]), ops.BAD_PREFIX, (3, 4, 5, 6)),
+                              (dict(prefix_len=[-7, 30]), ops.BAD_PREFIX, (0, 1, 2)), (dict(prefix_len=[107, 30]), ops.BEFORE_PREFIX, (0, 1, 2)),
+                              (dict(starts=[162, 30, 9]), ops.PAST_SLAB, ()), (dict(max_tokens=8), ops.PAST_TOKENS, ())):
+        args = dict(starts=[105, 30, 9], prefix_of=[0, 1, -1], prefix_len=[100, 30], max_tokens=9)
+        args.update(change)
+        T = args["max_tokens"]
+        pk = ops.pack_shared(i32(q_lens), i32(args["starts"]), base, i32([cap] * 3), i32(args["prefix_of"]), i32(args["prefix_len"]), D, T)
+        at = [-1 if t in lost else w for t, w in enumerate(want)][:T]
+        if bit == ops.PAST_SLAB:
+            at[:3] = [62, 63, 64]
+        seq = [0, 0, 0, 1, 1, 1, 1, 2, 2]
+        slots = [int(base[seq[t]]) + p * D if 0 <= p < cap else -1 for t, p in enumerate(at)]
+        assert int(pk["status"]) == bit and pk["kv_pos"].tolist() == at and pk["kv_slot"].tolist() == slots, change
+        pools = [torch.zeros(3 * HKV * cap * D, dtype=torch.bfloat16, device=DEV) for _ in "kv"]
+        ops.rope_kv_append(m.table[:T], pk["positions"], pk["seq_id"], m.cos, m.sin, HQ, HKV, D, base, i32([cap] * 3), *pools, kv_pos=pk["kv_pos"])
+        for pool, which in zip(pools, "kv"):
+            for s in range(3):
+                rows = kvlayout.gather(pool.cpu()[s * HKV * cap * D:(s + 1) * HKV * cap * D], HKV, cap, which, torch.arange(cap))
+                there = {p for t, p in enumerate(at) if seq[t] == s and 0 <= p < cap}
+                assert {int(p) for p in torch.nonzero(rows.abs().sum((0, 2)))[:, 0]} == there, (change, s)

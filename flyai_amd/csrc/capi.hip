@@ -750,10 +750,10 @@ static int check_slabs(flyai_stage* st, const int64_t* kv_base, const int32_t* k
   const int64_t pool = smallest_pool(st);
   const int64_t per_pos = (int64_t)c.n_kv_heads * c.head_dim;
   for (int b = 0; b < S; ++b) {
-    const int64_t end = kv_base[b] + (int64_t)kv_cap[b] * per_pos;
-    if (end > pool)
-      return set_error(FLYAI_ERANGE, "sequence %d: KV slab [%lld, %lld) ends past the pools (%lld elements)", b,
-                       (long long)kv_base[b], (long long)end, (long long)pool);
+    const int64_t elems = (int64_t)kv_cap[b] * per_pos;
+    if (kv_base[b] > pool - elems)  // (the slab's end may pass 64 bits)
+      return set_error(FLYAI_ERANGE, "sequence %d: KV slab of %lld elements at %lld ends past the pools (%lld elements)", b,
+                       (long long)elems, (long long)kv_base[b], (long long)pool);
   }
   if (S < 2) return FLYAI_OK;
   int* order = st->slab_order.data();
@@ -784,12 +784,13 @@ static int check_prefixes(flyai_stage* st, const int32_t* starts, const int64_t*
   int* order = st->slab_order.data();
   if (S == 1) order[0] = 0;
   for (int i = 0; i < pre.n; ++i) {
-    const int64_t lo = pre.base[i], hi = lo + (int64_t)pre.cap[i] * per_pos;
+    const int64_t lo = pre.base[i], elems = (int64_t)pre.cap[i] * per_pos;
     FLYAI_REQUIRE(pre.len[i] >= 0 && pre.cap[i] >= pre.len[i] && pre.cap[i] % 64 == 0 && lo >= 0 && lo % 8 == 0,
                   "prefix %d needs 0 <= length <= cap, cap %% 64 == 0 and base %% 8 == 0", i);
-    if (hi > pool)
-      return set_error(FLYAI_ERANGE, "prefix %d: KV slab [%lld, %lld) ends past the pools (%lld elements)", i, (long long)lo, (long long)hi,
-                       (long long)pool);
+    if (lo > pool - elems)
+      return set_error(FLYAI_ERANGE, "prefix %d: KV slab of %lld elements at %lld ends past the pools (%lld elements)", i, (long long)elems,
+                       (long long)lo, (long long)pool);
+    const int64_t hi = lo + elems;
     // the first sequence whose slab ends past lo, and those behind it (the slabs are apart, so their ends ascend too)
     const int* at = std::partition_point(order, order + S, [&](int b) { return kv_base[b] + (int64_t)kv_cap[b] * per_pos <= lo; });
     for (; at < order + S && kv_base[*at] < hi; ++at) {

@@ -188,3 +188,24 @@ def test_accept_batch_wants_a_distribution_for_each_draft():
     with pytest.raises(ValueError, match="probs must have shape"):
         sm.accept_batch(logits[:0], [], probs=torch.zeros(1, 50))
     assert sm.gen.bit_generator.state == before
+
+
+@pytest.mark.parametrize("base", [2 ** 63 - 8, 2 ** 63 - 128 * 64, 2 ** 62, 2 ** 40])
+def test_slabs_whose_end_passes_64_bits(stage, base):
+    """The slab of a prefix and of a sequence, with prefixes in the step and without: past the pools, though the sum wraps round."""
+    lib, kv = _lib.lib(), stage.kv
+    stage.set_prefixes()
+    i32, i64 = (lambda *v: np.array(v, dtype=np.int32)), (lambda *v: np.array(v, dtype=np.int64))
+
+    def call(own, prefix):
+        arrays = [i32(1, 1), i32(100, 100), i64(kv.base(1), own), i32(128, 128), i32(0, 0), i32(100), i64(prefix), i32(128)]
+        p = [C.c_void_p(a.ctypes.data) for a in arrays]
+        return (lib.flyai_stage_forward_shared(stage._h, *p[:4], None, 2, *p[4:], 1, FAKE, None), lib.flyai_last_error().decode(),
+                lib.flyai_stage_forward(stage._h, *p[:4], 2, FAKE, None), lib.flyai_last_error().decode())
+
+    rc, text, _, _ = call(kv.base(2), base)
+    assert rc == _lib.FLYAI_ERANGE and "prefix 0" in text and "past the pools" in text
+    rc, text, plain, plain_text = call(base, kv.base(0))
+    assert rc == plain == _lib.FLYAI_ERANGE and all("sequence 1" in t and "past the pools" in t for t in (text, plain_text))
+    root = i32(-1), i32(0)
+    assert lib.flyai_stage_forward_tree(stage._h, 5, 1, *(C.c_void_p(a.ctypes.data) for a in root), base, 128, FAKE, None) == _lib.FLYAI_ERANGE

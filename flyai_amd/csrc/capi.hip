@@ -777,6 +777,7 @@ static int check_prefixes(flyai_stage* st, const int32_t* starts, const int64_t*
   FLYAI_REQUIRE(pre.n <= std::min(c.max_seqs, 1024), "forward: %d prefixes above %d (max_seqs, 1024)", pre.n, std::min(c.max_seqs, 1024));
   FLYAI_REQUIRE(st->shared, "forward: prefixes need flyai_stage_set_shared");
   for (int b = 0; b < S; ++b) {
+    FLYAI_REQUIRE(kv_cap[b] <= kShMaxCap, "sequence %d: a slab of %d positions above 2^30", b, kv_cap[b]);
     FLYAI_REQUIRE(pre.of[b] >= -1 && pre.of[b] < pre.n, "sequence %d: prefix %d outside [-1, %d)", b, pre.of[b], pre.n);
     FLYAI_REQUIRE(pre.of[b] < 0 || starts[b] >= pre.len[pre.of[b]], "sequence %d starts at %d, before its prefix of %d positions ends", b,
                   starts[b], pre.len[pre.of[b]]);
@@ -785,8 +786,9 @@ static int check_prefixes(flyai_stage* st, const int32_t* starts, const int64_t*
   if (S == 1) order[0] = 0;
   for (int i = 0; i < pre.n; ++i) {
     const int64_t lo = pre.base[i], elems = (int64_t)pre.cap[i] * per_pos;
-    FLYAI_REQUIRE(pre.len[i] >= 0 && pre.cap[i] >= pre.len[i] && pre.cap[i] % 64 == 0 && lo >= 0 && lo % 8 == 0,
-                  "prefix %d needs 0 <= length <= cap, cap %% 64 == 0 and base %% 8 == 0", i);
+    // (what the plan on the GPU would refuse besides: its status is not read in a step, whose rows would be zeros)
+    FLYAI_REQUIRE(pre.len[i] >= 0 && pre.cap[i] >= pre.len[i] && pre.cap[i] > 0 && pre.cap[i] <= kShMaxCap && pre.cap[i] % 64 == 0 && lo >= 0 && lo % 8 == 0,
+                  "prefix %d needs 0 <= length <= cap, 0 < cap <= 2^30, cap %% 64 == 0 and base %% 8 == 0", i);
     if (lo > pool - elems)
       return set_error(FLYAI_ERANGE, "prefix %d: KV slab of %lld elements at %lld ends past the pools (%lld elements)", i, (long long)elems,
                        (long long)lo, (long long)pool);

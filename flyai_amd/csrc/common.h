@@ -14,6 +14,8 @@ typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
 typedef float f32x4_t __attribute__((ext_vector_type(4)));
 
+constexpr int kShMaxCap = 1 << 30;  // positions of a slab at most, in batches that share prefixes (shared.hip)
+
 // ---- error reporting (thread-local last error, C-ABI returns negative codes) ------------------
 int set_error(int code, const char* fmt, ...);
 int check_launch(const char* what);

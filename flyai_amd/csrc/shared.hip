@@ -182,7 +182,7 @@ struct ShBatch {
 enum { kShPastSlab = 1, kShPastTokens = 2, kShBeforePrefix = 4, kShBadPrefix = 8, kShBadSequence = 16 };
 
 __device__ __forceinline__ bool sh_slab_ok(int64_t base, int cap, int Hkv, int64_t pool) {
-  return cap > 0 && cap <= (1 << 30) && cap % 64 == 0 && base >= 0 && base % 8 == 0 && base <= pool - (int64_t)Hkv * cap * 64;
+  return cap > 0 && cap <= kShMaxCap && cap % 64 == 0 && base >= 0 && base % 8 == 0 && base <= pool - (int64_t)Hkv * cap * 64;
 }
 
 // What the plan keeps of a sequence and of a prefix, in LDS.

@@ -209,3 +209,15 @@ def test_slabs_whose_end_passes_64_bits(stage, base):
     assert rc == plain == _lib.FLYAI_ERANGE and all("sequence 1" in t and "past the pools" in t for t in (text, plain_text))
     root = i32(-1), i32(0)
     assert lib.flyai_stage_forward_tree(stage._h, 5, 1, *(C.c_void_p(a.ctypes.data) for a in root), base, 128, FAKE, None) == _lib.FLYAI_ERANGE
+
+
+def test_slabs_without_positions(stage):
+    """What the plan on the GPU refuses, a step refuses before any launch: its rows would be zeros, and no error."""
+    lib, kv = _lib.lib(), stage.kv
+    stage.set_prefixes()
+    i32, i64 = (lambda *v: np.array(v, dtype=np.int32)), (lambda *v: np.array(v, dtype=np.int64))
+    for length, cap in ((0, 0), (0, -64), (0, 2 ** 30 + 64)):
+        arrays = [i32(1), i32(0), i64(kv.base(1)), i32(128), i32(0), i32(length), i64(kv.base(0)), i32(cap)]
+        p = [C.c_void_p(a.ctypes.data) for a in arrays]
+        rc = lib.flyai_stage_forward_shared(stage._h, *p[:4], None, 1, *p[4:], 1, FAKE, None)
+        assert rc == _lib.FLYAI_EINVAL and "prefix 0 needs" in lib.flyai_last_error().decode(), (length, cap)

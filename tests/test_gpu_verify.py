@@ -351,3 +351,32 @@ def test_nothing_is_left(V):
     tokens, counts, _ = c.expected()
     assert counts.tolist() == [1] * S and (V < 4 or len(set(tokens[::2].tolist())) > 2)
     c.check()
+
+
+@pytest.mark.parametrize("probs", ["none", "some"])
+@pytest.mark.parametrize("V,streams", [(16400, 300), (40003, 260), (V_GPTOSS, 24)])
+def test_weights_by_table(V, streams, probs):
+    """Streams without a filter that have enough ids a workgroup for a table of the common values' weights (on any number of CUs up to
+    256 here), and rows longer than their first loads: masked ids of several values, values below and above the table's, zeros of both signs,
+    the rejected draft among them, ties of the maximum; greedy and filtered streams between them."""
+    params = [(1.0, 0, 1.0), (30.0, 0, 1.0), (0.7, 0, 1.0), (1.0, 0, 1.0), (0.0, 0, 1.0), (0.8, 40, np.float32(0.95))]
+    c = Case(V, [1 + i % 2 for i in range(streams)], [params[i % len(params)] for i in range(streams)], seed=V, probs=probs)
+    R, g = len(c.draft), torch.Generator().manual_seed(V)
+    x = c.logits.float()
+    low = float(torch.finfo(torch.bfloat16).min)
+    some = lambda share: torch.rand(V, generator=g) < share  # noqa: E731
+    for r in range(R):
+        x[r, some(0.5)] = (float("-inf"), low, -100.0, -300.0, 0.0, 1.0)[r % 6]
+        for value in (2.0 ** -30, -2.0 ** -30, 0.0, -0.0, 2.0 ** -24, -2.0 ** -25, -255.0, -256.0, -float("inf")):
+            x[r, some(0.002)] = value
+        if r % 3 == 0:  # a maximum above the table, more than once
+            x[r, some(3.0 / V)] = 300.0
+        x[r, 7 + r % 3] = 290.0 if r % 5 == 0 else 12.0
+    c.logits = x.to(torch.bfloat16)
+    top = torch.argmax(c.logits.float(), 1).numpy()
+    c.draft = np.where((c.draft >= 0) & (np.arange(R) % 4 == 1), top, c.draft).astype(np.int32)  # a draft that has most of the weight
+    c.u[1::2] = 1 - 2.0 ** -53
+    with np.errstate(invalid="ignore", over="ignore"):
+        tokens, counts, _ = c.expected()
+        assert {1, 2} == set(counts.tolist()) and len(set(tokens.tolist())) > streams // 2
+        c.check()

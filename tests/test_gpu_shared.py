@@ -2,7 +2,7 @@
 import pytest
 import torch
 
-from flyai_amd import ops
+from flyai_amd import kvlayout, ops
 from oracle import shared as oracle
 from shared_batches import DEV, Batch, check
 
@@ -292,3 +292,163 @@ def test_tiles_and_rounds(n, Hkv, P):
         alone.q, alone.T = b.q[16 * i:16 * i + 16], 16
         alone.bases, alone.caps = [*b.bases[:1], b.bases[1 + i], None], [b.caps[0], b.caps[1 + i]]
         assert alone.run(0)[0].equal(got[16 * i:16 * i + 16]), i
+
+
+@pytest.mark.parametrize("window", [0, 90])
+@pytest.mark.parametrize("S,n", [(1025, 65), (2500, 300), (4096, 1024)])
+def test_thousands_of_sequences(S, n, window):
+    """Several sequences a thread of the plan, more prefixes than a wave has lanes, of 0 to 5 tokens, behind a prefix or none."""
+    prefixes = [(37 * i) % 150 for i in range(n)]
+    b = Batch(prefixes, [((i * 5 + i // 7) % 6, i * 11 % 60, (i * 7) % (n + 1) - 1) for i in range(S)], Hkv=1, seed=S)
+    got, plan = b.run(window)
+    assert plan.status.item() == 0
+    check(got, *b.expected(window))
+
+
+def test_the_most_rows():
+    """65,536 of them."""
+    b = Batch([500], [(256, 0, 0 if i % 8 else -1) for i in range(256)], Hkv=1, seed=12)
+    assert b.T == 65536
+    got, plan = b.run(0)
+    assert plan.status.item() == 0
+    check(got, *b.expected(0))
+
+
+class Counted(Batch):
+    """All keys zero, so that every key that a row sees has the weight 1, and the sinks too; value (kv head, dim) of position p is 1 where
+    (p + shift) % period is 64 * head + dim and 0 else.  A row's result is the number of such positions that it sees over all that it sees and
+    one: with up to 120 of them, a key that is lost or taken twice changes it by more than 2^-7 of itself, two half steps of bf16."""
+
+    def __init__(self, prefixes, seqs, Hkv=8, period=512, shift=0):
+        one = Batch([1] * len(prefixes), [(s[0], 0, -1) for s in seqs], Hkv=Hkv, seed=1)  # (for the queries)
+        self.__dict__.update(one.__dict__)
+        self.prefixes, self.seqs, self.period, self.shift = prefixes, seqs, period, shift
+        self.prefix_of = [s[2] for s in seqs]
+        self.behind = [prefixes[p] if p >= 0 else 0 for p in self.prefix_of]
+        self.starts = [b + s[1] for b, s in zip(self.behind, seqs)]
+        lens = [*prefixes, *(s[0] + s[1] for s in seqs)]
+        self.caps = [max(64, (n + 63) // 64 * 64) for n in lens]
+        self.bases = [0]
+        for c in self.caps:
+            self.bases.append(self.bases[-1] + Hkv * c * 64)
+        self.elems = self.bases[-1]
+        self.k = torch.full((self.elems,), float("nan"), dtype=torch.bfloat16, device=DEV)
+        self.v = self.k.clone()
+        for base, cap, n, first in zip(self.bases, self.caps, lens, [0] * len(prefixes) + self.behind):
+            if n:
+                c = (first + torch.arange(n, device=DEV) + shift) % period
+                rows = (c[:, None] == torch.arange(64 * Hkv, device=DEV)).reshape(n, Hkv, 64).transpose(0, 1)
+                slab = slice(base, base + Hkv * cap * 64)
+                kvlayout.scatter(self.k[slab], Hkv, cap, "k", torch.zeros_like(rows), torch.arange(n))
+                kvlayout.scatter(self.v[slab], Hkv, cap, "v", rows, torch.arange(n))
+        self.sinks.zero_()
+
+    def counts(self, window):
+        """(numbers [T, 64 Hkv], all that a row sees [T])."""
+        at = torch.tensor([a + i for a, s in zip(self.starts, self.seqs) for i in range(s[0])])
+        lo = (at - window + 1).clamp_min(0) if window else torch.zeros_like(at)
+        first = (torch.arange(64 * self.Hkv) - self.shift) % self.period
+        below = lambda n: (n[:, None] - first + self.period - 1) // self.period  # noqa: E731
+        return below(at + 1) - below(lo), at + 1 - lo
+
+    def check(self, window, **change):
+        """P, sums and folds are whole numbers below 2^24, exact; the reciprocal and its product round by 2^-24 each, the result by half a
+        step, 2^-8."""
+        got, plan = self.run(window, **change)
+        assert plan.status.item() == 0
+        n, seen = self.counts(window)
+        assert int(n.max()) <= 120
+        want = (n.double() / (seen + 1).double()[:, None]).reshape(-1, self.Hkv, 1, 64)
+        bad = (got.double().cpu().reshape(-1, self.Hkv, 8, 64) - want).abs() > want * (2.0 ** -8 + 2.0 ** -22)
+        assert not bool(bad.any()), (int(bad.sum()), torch.nonzero(bad)[:4].tolist())
+
+
+# one tile less and one more than a head's 64 workgroups, and rests that are split and whole; the sequence of a wave, of a tile and of several
+COUNTED = {"few": [(1, 900, 0), (3, 0, 0), (9, 385, 0)], "one": [(1, 0, 0)], "long": [(40, 770, 0), (300, 100, 0)],
+           "20": [(16, 3 * i % 70, 0) for i in range(20)], "63": [(16, 3 * i % 70, 0) for i in range(63)], "70": [(16, 5, 0)] * 70,
+           "130": [(16, 5, 0)] * 130, "crowd": [(1 + i % 5, 7 * i % 500, i % 2) for i in range(200)]}
+
+
+@pytest.mark.parametrize("window", [0, 1, 5000])
+@pytest.mark.parametrize("P", [1, 1537, 6145, 18433, 33000])
+@pytest.mark.parametrize("name", COUNTED)
+def test_every_key_counts_once(name, P, window):
+    Counted([P, max(P - 700, 0)], COUNTED[name]).check(window)
+
+
+@pytest.mark.parametrize("window", [0, 5000])
+@pytest.mark.parametrize("P", [6145, 18432, 18433, 27700, 33000])
+def test_border_keys_decide(P, window):
+    """64 positions of each kv head have a key along an axis of its own that outweighs all others for the rows along it: first and last
+    positions of blocks and of chunks, the prefix's last, the own slab's first, and both sides of the window's edge."""
+    seqs = [(1, 900, 0), (3, 0, 0), (9, 385, 0), (4, 5, 0)]
+    b = Batch([P], seqs, Hkv=2, seed=P)
+    c = 12.0  # scores 18: e^18 to the 34,000 others' some 1
+    rng = torch.Generator().manual_seed(P)
+    borders = [torch.arange(step, P, step) for step in (192, 64)]  # chunks are multiples of 192 positions, blocks 64
+    for h in range(2):
+        edge = [P - 1, 0, P - 2, 63, 64] + [P - 5000 + i for i in (-1, 0, 1, 2, 3) if P > 5001]
+        near = [int(s) - i % 2 for steps in borders for i, s in enumerate(steps[torch.randperm(len(steps), generator=rng)])]
+        at = list(dict.fromkeys(edge + near))[:64]
+        k = b.keys[0][h].float() * 0.05
+        k[at] = torch.eye(64) * c
+        b.keys[0][h] = k.to(torch.bfloat16)
+    for i in range(len(seqs)):
+        b.keys[1 + i] *= 0.05
+    b.k, b.v = b.k.cpu(), b.v.cpu()
+    for i, k in enumerate(b.keys):
+        b._write(b.bases[i], b.caps[i], k.shape[1], k, b.values[i])
+    b.k, b.v = b.k.to(DEV), b.v.to(DEV)
+    axis = torch.arange(b.T * 16).reshape(b.T, 2, 8) % 8 + 8 * (torch.arange(b.T)[:, None, None] % 8)  # a row's, of each kv head
+    b.q = (torch.eye(64)[axis.reshape(-1)] * c).reshape(b.T, 16, 64).to(torch.bfloat16)
+    got, plan = b.run(window)
+    assert plan.status.item() == 0
+    want, mag = b.expected(window)
+    assert float((want.abs().amax(2) > 0.5).float().mean()) > (0.95 if window == 0 else 0.1)  # the planted values come through
+    check(got, want, mag)
+
+
+def _behind_one_slab(b, n):
+    """The batch's prefix under n names."""
+    i32 = lambda v: torch.tensor(v, dtype=torch.int32, device=DEV)  # noqa: E731
+    return dict(prefix_len=i32(b.prefixes * n), prefix_cap=i32(b.caps[:1] * n), prefix_base=torch.tensor(b.bases[:1] * n, dtype=torch.int64, device=DEV))
+
+
+@pytest.mark.parametrize("n,each,P", [(1024, 1, 6145), (1024, 2, 6145), (300, 3, 27700), (300, 5, 27700)])
+def test_chunks_that_the_lists_do_not_hold(n, each, P):
+    """Prefixes of few rows (waves) and of more (tiles) with more chunks in all than there are entries stay whole: every key counts once, and
+    the rows' bits are those behind the one prefix that all the names mean."""
+    of = torch.arange(n * each, dtype=torch.int32, device=DEV) % n
+    for shift in (0, 200):
+        b = Counted([P], [(1, i % 40, 0) for i in range(n * each)], Hkv=1, shift=shift)
+        b.check(0, prefix_of=of, **_behind_one_slab(b, n))
+    for t in (b.k, b.v):
+        t.copy_(torch.randn(t.shape, device=DEV, generator=torch.Generator(device=DEV).manual_seed(n)))
+    want, _ = b.run(0)
+    got, _ = b.run(0, prefix_of=of, **_behind_one_slab(b, n))
+    assert got.equal(want) and bool(want.isfinite().all())
+
+
+def test_chunks_that_the_records_do_not_hold():
+    """400 tiles behind 200,000 positions, in 24 chunks each if there were room."""
+    b = Counted([200_000], [(16, 3 * i % 70, 0) for i in range(400)], Hkv=1, period=2048, shift=77)
+    b.check(0)
+
+
+def test_an_own_slab_of_more_chunks_than_are_split():
+    """A sequence alone of 1.6 million positions of its own: one wave takes them all.  Weights 1, and a value 1 in one of 64 positions of each dim."""
+    L, cap = 1_600_001, 1_600_064
+    k = torch.zeros(cap * 64, dtype=torch.bfloat16, device=DEV)
+    block = torch.empty(64 * 64, dtype=torch.bfloat16)
+    kvlayout.scatter(block, 1, 64, "v", torch.eye(64, dtype=torch.bfloat16)[None], torch.arange(64))
+    v = block.to(DEV).repeat(cap // 64)
+    i32 = lambda *a: torch.tensor(a, dtype=torch.int32, device=DEV)  # noqa: E731
+    base = torch.zeros(1, dtype=torch.int64, device=DEV)
+    plan = ops.attn_shared_plan(i32(1), i32(L - 1), base, i32(cap), i32(-1), i32(), base[:0], i32(), 1, 0, 1, k.numel())
+    q = torch.randn(1, 8, 64, generator=torch.Generator().manual_seed(0)).to(torch.bfloat16).to(DEV)
+    got = ops.attn_shared(q, k, v, torch.zeros(8, device=DEV), plan)
+    assert plan.status.item() == 0
+    n = torch.full((64,), L // 64, dtype=torch.float64)
+    n[:L % 64] += 1
+    want = n / (L + 1)
+    assert bool(((got[0].double().cpu() - want).abs() <= want * 2.0 ** -8).all())

@@ -641,69 +641,58 @@ __device__ __forceinline__ void sh_wild_values(ShRows<QT>& R, uint4 (&v)[4][2], 
     }
 }
 
-// One 64-key block against the wave's rows.  k(kt, step) and v(dt, half) give its fragments.  As in attn.hip: scores S^T = K . Q^T,
-// P = 2^(s scale - m) rounded to bf16 (2^-9 of each; the row sum takes the rounded values), O^T += V^T . P^T, L += 1 . P^T.
-template <int QT, bool MASKED, bool INREG, class KF, class VF, class AF>
+// One 64-key block against the wave's rows.  k(kt, step) and v(dt, half) give its fragments, from registers.  As in attn.hip: scores
+// S^T = K . Q^T, P = 2^(s scale - m) rounded to bf16 (2^-8 of each at most: the matrix units take 16 bits; the row sum takes the rounded
+// values), O^T += V^T . P^T, L += 1 . P^T.  One row tile's scores are live at a time.
+template <int QT, class KF, class VF, class AF>
 __device__ __forceinline__ void sh_block(ShRows<QT>& R, KF&& k, VF&& v, AF&& after_scores, int kb, bool interior, int key_lo, int key_hi) {
   const int g = (threadIdx.x & 63) >> 4;
   const float scale = 0.125f * kLog2e;
   const bf16x8_t ones = as_bf16x8(make_uint4(0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u));
   bf16x8_t pt[QT][2];
-  // the row tiles at once where the fragments come from LDS (each is read once), one after the other where they are in
-  // registers (half as many scores live)
-  constexpr int QN = INREG ? 1 : QT;
 #pragma unroll
-  for (int q0 = 0; q0 < QT; q0 += QN) {
-    f32x4_t s[QN][4];
+  for (int qt = 0; qt < QT; ++qt) {
+    f32x4_t s[4];
 #pragma unroll
     for (int kt = 0; kt < 4; ++kt) {
-      const bf16x8_t k0 = as_bf16x8(k(kt, 0)), k1 = as_bf16x8(k(kt, 1));
-#pragma unroll
-      for (int j = 0; j < QN; ++j) {
-        s[j][kt] = mfma16x16x32(k0, R.qf[q0 + j][0], f32x4_t{0.f, 0.f, 0.f, 0.f});
-        s[j][kt] = mfma16x16x32(k1, R.qf[q0 + j][1], s[j][kt]);
-      }
+      s[kt] = mfma16x16x32(as_bf16x8(k(kt, 0)), R.qf[qt][0], f32x4_t{0.f, 0.f, 0.f, 0.f});
+      s[kt] = mfma16x16x32(as_bf16x8(k(kt, 1)), R.qf[qt][1], s[kt]);
     }
-    if (q0 + QN == QT) after_scores();
-#pragma unroll
-    for (int j = 0; j < QN; ++j) {
-      const int qt = q0 + j;
-      float bmax = -INFINITY;
-      if (MASKED && !interior) {
-        // (tile_key(kt, 4 g + i) is 8 g + tile_key(kt, i); a row that sees nothing has a count of 0)
-        const int lo = max(key_lo, R.lo[qt]), from = kb + 8 * g - lo;
-        const uint32_t count = (uint32_t)max(min(key_hi - 1, R.hi[qt]) - lo + 1, 0);
-#pragma unroll
-        for (int kt = 0; kt < 4; ++kt)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) s[j][kt][i] = (uint32_t)(from + tile_key(kt, i)) < count ? s[j][kt][i] : -INFINITY;
-      }
+    if (qt == QT - 1) after_scores();
+    float bmax = -INFINITY;
+    if (!interior) {
+      // (tile_key(kt, 4 g + i) is 8 g + tile_key(kt, i); a row that sees nothing has a count of 0)
+      const int lo = max(key_lo, R.lo[qt]), from = kb + 8 * g - lo;
+      const uint32_t count = (uint32_t)max(min(key_hi - 1, R.hi[qt]) - lo + 1, 0);
 #pragma unroll
       for (int kt = 0; kt < 4; ++kt)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) bmax = fmaxf(bmax, s[j][kt][i]);
-      // (a row's largest score lies in one of its four lanes: they are compared only where one of the wave's lanes is past its row's slack)
-      if (__ballot(bmax * scale > R.m[qt] + kMaxSlack)) {
-        const float m_blk = max_lane_groups(bmax) * scale;
-        const bool move = m_blk > R.m[qt] + kMaxSlack;
-        const float m_new = move ? m_blk : R.m[qt];
-        const float alpha = __builtin_amdgcn_exp2f(R.m[qt] - m_new);
-        R.m[qt] = m_new;
-        R.L[qt] *= alpha;
-#pragma unroll
-        for (int dt = 0; dt < 4; ++dt) R.O[qt][dt] *= alpha;
-      }
-      const float neg_m = -R.m[qt];
-#pragma unroll
-      for (int kt = 0; kt < 4; ++kt)
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          pt[qt][kt >> 1][(kt & 1) * 4 + i] = (__bf16)__builtin_amdgcn_exp2f(fmaf(s[j][kt][i], scale, neg_m));
-      R.L[qt] = mfma16x16x32(ones, pt[qt][0], R.L[qt]);
-      R.L[qt] = mfma16x16x32(ones, pt[qt][1], R.L[qt]);
+        for (int i = 0; i < 4; ++i) s[kt][i] = (uint32_t)(from + tile_key(kt, i)) < count ? s[kt][i] : -INFINITY;
     }
+#pragma unroll
+    for (int kt = 0; kt < 4; ++kt)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) bmax = fmaxf(bmax, s[kt][i]);
+    // (a row's largest score lies in one of its four lanes: they are compared only where one of the wave's lanes is past its row's slack)
+    if (__ballot(bmax * scale > R.m[qt] + kMaxSlack)) {
+      const float m_blk = max_lane_groups(bmax) * scale;
+      const bool move = m_blk > R.m[qt] + kMaxSlack;
+      const float m_new = move ? m_blk : R.m[qt];
+      const float alpha = __builtin_amdgcn_exp2f(R.m[qt] - m_new);
+      R.m[qt] = m_new;
+      R.L[qt] *= alpha;
+#pragma unroll
+      for (int dt = 0; dt < 4; ++dt) R.O[qt][dt] *= alpha;
+    }
+    const float neg_m = -R.m[qt];
+#pragma unroll
+    for (int kt = 0; kt < 4; ++kt)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) pt[qt][kt >> 1][(kt & 1) * 4 + i] = (__bf16)__builtin_amdgcn_exp2f(fmaf(s[kt][i], scale, neg_m));
+    R.L[qt] = mfma16x16x32(ones, pt[qt][0], R.L[qt]);
+    R.L[qt] = mfma16x16x32(ones, pt[qt][1], R.L[qt]);
   }
-  if (MASKED && !interior) {
+  if (!interior) {
     uint4 w[4][2];
     uint32_t wild = 0;
 #pragma unroll
@@ -855,7 +844,6 @@ __device__ __forceinline__ void sh_put(ShRows<QT>& R, int rec0, int tok0, int kv
 }
 
 // An item of up to 2 tokens by one wave, K and V straight from the slab.
-template <int QT>
 __device__ __forceinline__ void sh_wave_item(const ShEntry& e, int kv_head, const int2* __restrict__ list, const uint16_t* __restrict__ q,
                                              const uint16_t* __restrict__ k_pool, const uint16_t* __restrict__ v_pool, int Hq, int Hkv,
                                              int window, int max_recs, float* __restrict__ parts) {
@@ -863,7 +851,7 @@ __device__ __forceinline__ void sh_wave_item(const ShEntry& e, int kv_head, cons
   const int key_hi = sh_key_end(e, 1);
   const int64_t base = e.base + (int64_t)kv_head * e.cap * 64;
   const uint16_t *K = k_pool + base, *V = v_pool + base;
-  ShRows<QT> R;
+  ShRows<1> R;
   sh_rows_init(R, e, 0, list, q, kv_head, Hq, window);
   int int_lo, int_hi;
   sh_interior(R, &int_lo, &int_hi);
@@ -894,9 +882,9 @@ __device__ __forceinline__ void sh_wave_item(const ShEntry& e, int kv_head, cons
         load_v_tile(vn, V, kb + 64, lane);
       }
     };
-    sh_block<QT, true, true>(R, [&](int kt, int st) __attribute__((always_inline)) { return kc[kt][st]; },
-                             [&](int dt, int h) __attribute__((always_inline)) { return vc[dt][h]; }, next, kb,
-                             kb >= int_lo && kb + 63 <= int_hi, e.key_lo, key_hi);
+    sh_block(R, [&](int kt, int st) __attribute__((always_inline)) { return kc[kt][st]; },
+             [&](int dt, int h) __attribute__((always_inline)) { return vc[dt][h]; }, next, kb,
+             kb >= int_lo && kb + 63 <= int_hi, e.key_lo, key_hi);
   }
   sh_put(R, e.rec, 0, kv_head, Hkv, max_recs, parts);
 }
@@ -1010,9 +998,9 @@ __device__ __forceinline__ void sh_tile_item(const ShEntry& e, int run, int kv_h
       if (odd) issue(buf0, kb + 64);
       else issue(buf1, kb + 64);
     }
-    sh_block<2, true, true>(R, [&](int kt, int st) __attribute__((always_inline)) { return kc[kt][st]; },
-                            [&](int dt, int h) __attribute__((always_inline)) { return vc[dt][h]; }, [] {}, kb,
-                            kb >= int_lo && kb + 63 <= int_hi, key_lo, key_hi);
+    sh_block(R, [&](int kt, int st) __attribute__((always_inline)) { return kc[kt][st]; },
+             [&](int dt, int h) __attribute__((always_inline)) { return vc[dt][h]; }, [] {}, kb,
+             kb >= int_lo && kb + 63 <= int_hi, key_lo, key_hi);
     landed();
     kb += 64;
     odd ^= 1;
@@ -1060,7 +1048,7 @@ __global__ __launch_bounds__(256, 2) void attn_shared_kernel(const uint16_t* __r
   }
   for (int i = (per_head - 1 - w) * 4 + scalar((int)threadIdx.x >> 6); i < n_waves; i += per_head * 4) {
     const ShEntry e = waves[i];
-    sh_wave_item<1>(e, g, list, q, k_pool, v_pool, Hq, Hkv, window, L.max_recs, parts);
+    sh_wave_item(e, g, list, q, k_pool, v_pool, Hq, Hkv, window, L.max_recs, parts);
   }
 }
 

@@ -155,9 +155,8 @@ __global__ __launch_bounds__(kPackThreads) void pack_shared_kernel(
     const int64_t len = (int64_t)start + max(q, 0);
     kv_len[s] = (int)min(len, (int64_t)INT32_MAX);
     if (q < 0 || start < 0) status |= 16;
-    else if (P < 0) status |= 8;
-    else if (start < P) status |= 4;
-    else if (len - P > kv_cap[s]) status |= 1;
+    else if (q > 0)  // (without tokens its prefix and slab may be those of another time; the attention's plan has the same rule)
+      status |= P < 0 ? 8 : start < P ? 4 : len - P > kv_cap[s] ? 1 : 0;
     if (run > max_tokens) status |= 2;
   }
   if (s0 < s1 && s1 == S) {

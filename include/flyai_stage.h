@@ -384,7 +384,8 @@ int flyai_kv_compact(uint16_t* k_pool, uint16_t* v_pool, int64_t layer, int64_t 
  * (negative: none, and the slab holds all).  All arrays are device memory, so that lengths which were made on the GPU never
  * come to the host; what they hold is checked there, and reported as bits of a status word: 1 a sequence past its slab, 2
  * more tokens than max_tokens (n_tokens), 4 a sequence that starts before its prefix ends, 8 a prefix that is none (id,
- * length or slab), 16 a bad length, start or slab.  q_lens[b] = 0 is a sequence without tokens.
+ * length or slab), 16 a bad length, start or slab.  q_lens[b] = 0 is a sequence without tokens,
+ * whose prefix and slab are not looked at.
  * flyai_pack_shared is flyai_pack_ragged for such sequences: positions[t] and kv_len[b] count from the prefix's start,
  * kv_pos[t] is the token's slab position and kv_slot[t] = kv_base + kv_pos * head_dim, -1 past the slab.  Both are -1 for every token of a
  * sequence that starts before its prefix ends, or whose prefix, length or start is bad; of a sequence that runs past its slab or max_tokens

@@ -261,3 +261,21 @@ def test_refused_sequences_are_appended_nowhere():
                 rows = kvlayout.gather(pool.cpu()[s * HKV * cap * D:(s + 1) * HKV * cap * D], HKV, cap, which, torch.arange(cap))
                 there = {p for t, p in enumerate(at) if seq[t] == s and 0 <= p < cap}
                 assert {int(p) for p in torch.nonzero(rows.abs().sum((0, 2)))[:, 0]} == there, (change, s)
+
+
+def test_idle_sequences_of_another_time():
+    """Sequences without tokens whose prefix, start or slab are no longer any: pack_shared and the plan pass over them alike, and the others' rows
+    are those of the batch without them."""
+    b = Batch([100, 30], [(2, 5, 0), (0, 3, 0), (3, 0, 1), (0, 4, -1), (0, 9, 1), (1, 7, -1)], Hkv=HKV, seed=8)
+    want, _ = b.run(0)
+    packed = ops.pack_shared(**b.lengths(), head_dim=D, max_tokens=b.T)
+    stale = b.lengths()
+    for name, i, v in (("prefix_of", 1, 7), ("starts", 3, 2 ** 31 - 1), ("kv_cap", 3, 0), ("kv_base", 3, -8), ("starts", 4, 3)):
+        stale[name][i] = v
+    got = ops.pack_shared(**stale, head_dim=D, max_tokens=b.T)
+    assert int(got["status"]) == 0
+    assert all(got[k].equal(packed[k]) for k in ("cu_seqlens", "positions", "seq_id", "kv_pos", "kv_slot"))
+    out, plan = b.run(0, **stale)
+    assert int(plan.status) == 0 and out.equal(want)
+    stale["starts"][1] = -1  # a start that is none is reported, with tokens or without
+    assert int(ops.pack_shared(**stale, head_dim=D, max_tokens=b.T)["status"]) == int(b.plan(0, **stale).status) == ops.BAD_SEQUENCE

@@ -890,6 +890,7 @@ extern "C" int flyai_spec_verify(const uint16_t* logits, int32_t R, int32_t V, c
                                  const int32_t* probs_row, int32_t* tokens, int32_t* counts, float* p, void* workspace,
                                  flyai_stream_t stream) {
   FLYAI_REQUIRE(R >= 0 && S >= 0 && V >= 1 && V <= (1 << 22), "spec_verify: needs R, S >= 0 and V in [1, 2^22]");
+  FLYAI_REQUIRE(R < (1 << 22), "spec_verify: %d rows, a launch takes 2^22 - 1 workgroups of 1,024 threads", R);
   FLYAI_REQUIRE(S <= 65535, "spec_verify: n_streams %d above 65535", S);
   if (S == 0) return FLYAI_OK;
   FLYAI_REQUIRE(cu_rows && counts && u_draw && (R == 0 || (logits && draft && u && tokens && p && workspace)), "spec_verify: null pointer");

@@ -487,7 +487,7 @@ int flyai_sample_probs(const float* probs, int32_t V, double u, int32_t* out, fl
  * the first id of maximal logit, which else ends the stream.  tokens int32 [R]: the accepted drafts, then the drawn token,
  * then -1; counts int32 [S]: tokens of each stream; p fp32 [R]: the filtered target's probability of each token (greedy: 1; 0 behind
  * the end).  Rows behind cu_rows[S] are left as they were.  u, u_draw fp64 in [0, 1).  Sums are of integers: results do not
- * depend on the launch.  V <= 2^22, S <= 65535; workspace: flyai_spec_verify_workspace_bytes, 8-byte aligned, not initialised. */
+ * depend on the launch.  V <= 2^22, S <= 65535, R < 2^22; workspace: flyai_spec_verify_workspace_bytes, 8-byte aligned, not initialised. */
 size_t flyai_spec_verify_workspace_bytes(int32_t R, int32_t V, int32_t S);
 int flyai_spec_verify(const uint16_t* logits, int32_t R, int32_t V, const int32_t* cu_rows, int32_t S, const int32_t* draft,
                       const double* u, const double* u_draw, const float* temps, const int32_t* top_ks, const float* top_ps,

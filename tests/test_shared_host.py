@@ -221,3 +221,9 @@ def test_slabs_without_positions(stage):
         p = [C.c_void_p(a.ctypes.data) for a in arrays]
         rc = lib.flyai_stage_forward_shared(stage._h, *p[:4], None, 1, *p[4:], 1, FAKE, None)
         assert rc == _lib.FLYAI_EINVAL and "prefix 0 needs" in lib.flyai_last_error().decode(), (length, cap)
+
+
+def test_spec_verify_rows_of_a_launch():
+    #       logits R    V  cu   S  draft u   u_draw temps ks   ps    t    k  p    probs n row   out ...       ws    stream
+    good = [FAKE, 0, 16, FAKE, 2, FAKE, FAKE, FAKE, None, None, None, 1.0, 0, 1.0, None, 0, None, FAKE, FAKE, FAKE, FAKE, None]
+    _each("flyai_spec_verify", good, [(1, 2 ** 22, "rows"), (1, 2 ** 31 - 1, "rows")])

@@ -15,13 +15,15 @@
 // The work lists are made on the GPU (attn_shared_plan_kernel), once for a step's layers: the host needs
 // no lengths, only bounds, and the grids are sized by those.
 //
-// What bounds it: with many rows instruction issue.  A wave's block (32 rows, 64 keys) is 36 matrix instructions (576 clocks at their
-// peak rate) and 32 exponentials, 32 fused multiply-adds, 16 maxima of three and 16 conversions (some 770): with two waves a SIMD the
-// larger of the two if nothing were in the way.  256 streams of up to 4 tokens behind 32,749 positions (554 GFLOP) take 578 us,
-// 0.96 PFLOP/s (a library's large product: 1.43); six questions of up to 300 tokens behind 4,099 (102 GFLOP) 158.  With few rows the
-// chain of a unit -- entry, token list, queries (3.5 us), then 1.1 us a block, of which two waves a SIMD take as long as one -- and the launches: 48 streams behind
-// 8,000 positions 32 us, of which the plan's 6, the items' 19 and the merge's 5; 2 streams behind 513 21 (6, 6 and 3; the host's two calls
-// are as long).  Three waves a SIMD (168 registers) and three buffers in turn were slower than two.
+// What bounds it: with many rows instruction issue.  A wave's block (32 rows, 64 keys) is 36 matrix instructions (576 clocks of the matrix
+// unit) and 32 exponentials, 32 fused multiply-adds, 16 maxima of three and 16 conversions (some 500: 8.6, 2.6 to 4, 4 and 4 each).  A
+// product keeps vector instructions from issue for about half of its 16 clocks: a loop of that mixture takes some 860 clocks a
+// block, 1,720 for a SIMD's two waves, whose blocks take some 2,150.  256 streams of up to 4 tokens behind 32,749 positions (554 GFLOP) take 578
+// to 616 us on different boxes, 0.96 to 0.90 PFLOP/s (a library's large product: 1.43); six questions of up to 300 tokens behind 4,099 (102
+// GFLOP) 158 to 164.  With few rows the chain of a unit -- entry, token list, queries (3.5 us), then 1.1 us a block, of which two waves a
+// SIMD take as long as one -- and the launches: 48 streams behind 8,000 positions 32 us, of which the plan's 7, the items' 21 and the merge's
+// 5; 2 streams behind 513 21 to 23 (6, 7 and 3; the host's two calls are as long).  Three waves a SIMD (168 registers) and three buffers in
+// turn were slower than two.
 #include <type_traits>
 
 #include "attn.h"

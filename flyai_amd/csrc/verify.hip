@@ -17,8 +17,8 @@
 // is not is then the only one whose weights are needed one by one: verify_pieces_kernel sums w' over pieces of its ids, and
 // verify_draw_kernel finds the piece and the id, and writes what comes out.
 //
-// With a vocabulary of 201,088 (us): 128 streams' 1,152 rows 159 to 163, of which the rows 118 (463 MB, 3.9 TB/s; a product of two arrays
-// reaches 6.3), the pieces 36, the draw 7; 24 streams' 120 rows 44 (27, 11, 7); one stream's 5 rows 35 (23, 6, 5), where a row is one CU's:
+// With a vocabulary of 201,088 (us): 128 streams' 1,152 rows 159 to 163, of which the rows 118 to 125 (463 MB, 3.9 to 3.7 TB/s; a product of
+// two arrays reaches 6.3), the pieces 36, the draw 7; 24 streams' 120 rows 44 (27, 11, 7); one stream's 5 rows 34 (23, 6, 5), where a row is one CU's:
 // 12 us of counting in LDS, some 8 of sums over the values.  The rows that many passes over the logits took (ver_row_general's way for all)
 // were 1,215 us of 128 streams, 482 of one.  Rows counted in up to eight parts, then added up, made one stream's 32 us and 24 streams' 53;
 // a workgroup a CU with the next row's loads ahead 205 of 128 streams' 159.

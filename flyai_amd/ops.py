@@ -598,7 +598,9 @@ def attn_shared(q, k_pool, v_pool, sinks, plan, out=None):
     [T, Hq, 64] rotated, k_pool and v_pool bf16 (the slabs that the plan names), sinks fp32 [Hq], Hq = 8 kv heads.  Returns
     out bf16 [T, Hq, 64] (None: a new one); rows behind the last sequence are left as they were, those of a sequence that the plan
     refused (plan.status) are zeros.  A row's bits depend on its own sequence, its prefix and the window, not on the batch.
-    K and V outside the positions that a row sees may hold anything."""
+    K and V outside the positions that a row sees may hold anything; an infinity in V that it sees with a weight below fp32's range counts for
+    nothing or as NaN, which may differ between batches.  Each call allocates its workspace: 63 MB for 64 tokens of 8 kv heads, 361 for
+    1,478, 2.5 GB for 65,536 (room for what may be split)."""
     T, Hkv = plan.n_tokens, plan.n_kv_heads
     dev, bf16 = q.get_device(), torch.bfloat16
     _need_all(dev, ("q", q, bf16, (T, 8 * Hkv, 64)), ("k_pool", k_pool, bf16, k_pool.shape), ("v_pool", v_pool, bf16, k_pool.shape),

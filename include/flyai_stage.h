@@ -408,7 +408,9 @@ int flyai_rope_kv_append_at(const uint16_t* qkv, const int32_t* positions, const
  * overlap need one each).  T: rows of q and out, at most 65,536; the rows behind the last sequence are left as they were, those of a
  * sequence that was refused (the status word, the plan's fourth int32) are zeros.  T, Hkv, n_seqs and n_prefixes of both calls must be the
  * same: nothing is done with a plan of others.  Slabs and prefixes are checked against pool_elems, the elements of a pool.
- * A row's bits depend on its own sequence, its prefix and the window alone.  D == 64, Hq == 8 Hkv, Hkv <= 64, n_seqs <= 4096, n_prefixes <= 1024;
+ * A row's bits depend on its own sequence, its prefix and the window alone (but for an infinity in V that it sees with a weight below fp32's
+ * range, which counts for nothing or as NaN).  The workspace is room for what may be split: 63 MB for 64 tokens of 8 kv heads, 361 for 1,478,
+ * 2.5 GB for 65,536.  D == 64, Hq == 8 Hkv, Hkv <= 64, n_seqs <= 4096, n_prefixes <= 1024;
  * q, pools, out, workspace 16-byte aligned. */
 size_t flyai_attn_shared_plan_bytes(int32_t T, int32_t n_seqs, int32_t n_prefixes);
 size_t flyai_attn_shared_workspace_bytes(int32_t T, int32_t Hkv);

@@ -21,8 +21,8 @@
 // block, 1,720 for a SIMD's two waves, whose blocks take some 2,150.  256 streams of up to 4 tokens behind 32,749 positions (554 GFLOP) take 578
 // to 616 us on different boxes, 0.96 to 0.90 PFLOP/s (a library's large product: 1.43); six questions of up to 300 tokens behind 4,099 (102
 // GFLOP) 158 to 164.  With few rows the chain of a unit -- entry, token list, queries (3.5 us), then 1.1 us a block, of which two waves a
-// SIMD take as long as one -- and the launches: 48 streams behind 8,000 positions 32 us, of which the plan's 7, the items' 21 and the merge's
-// 5; 2 streams behind 513 21 to 23 (6, 7 and 3; the host's two calls are as long).  Three waves a SIMD (168 registers) and three buffers in
+// SIMD take as long as one -- and the launches: 48 streams behind 8,000 positions 32 us, of which the plan's 7, the items' 22 and the merge's
+// 5; 2 streams behind 513 21 to 23 (6, 7.5 and 3 to 4; the host's two calls are as long).  Three waves a SIMD (168 registers) and three buffers in
 // turn were slower than two.
 #include <type_traits>
 
